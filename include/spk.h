@@ -441,6 +441,79 @@ int spk_bf16_gemm(const void *w, int rows, int cols, int ntok, const float *x, i
 int spk_bf16_gemm_pair(const void *gate, const void *up, int rows, int cols, int ntok, const float *x, int ldx,
                        float *y, int ldy, int act, void *stream);
 
+/* ------------------------------------------- batched serving: paged cache ---
+ * No counterpart in the reference, which runs one sequence. Many sequences keep their keys and
+ * values in pages of one pool, in 8 bits: e4m3 bytes under one f32 scale per (block of 16 tokens,
+ * KV head), keys and values apart. Per (page, KV head):
+ *   k        [page_tokens / 8][head_dim / 16][8 tokens][16 dims]
+ *   v        [page_tokens / 16][head_dim][16 tokens], byte b of a dim's 16 holding token
+ *            2 (b / 4) + b % 2 + 8 (b / 2 % 2) of the block
+ *   k_scale, v_scale   [page_tokens / 16]
+ * The pool needs no initial contents. head_dim 64, 128 or 256; page_tokens a multiple of 16;
+ * buffers 16-byte aligned. A page that two sequences share must be full: a call writes the whole
+ * of every 16-token block that it appends to. */
+typedef struct {
+    void *k, *v;                /* device [pages][kv_heads][page_tokens * head_dim] bytes */
+    float *k_scale, *v_scale;   /* device [pages][kv_heads][page_tokens / 16] */
+    int pages, page_tokens, kv_heads, head_dim;
+} spk_kv_pool;
+
+/* The rows of a call. Sequence s owns rows row0[s] .. row0[s + 1] - 1 (none is allowed), at
+ * positions kv_len[s] - n_s .. kv_len[s] - 1; position p lies in page table[s][p / page_tokens].
+ * The arrays are read on the device, so a captured graph follows what they hold. A batch that does
+ * not fit (rows out of range, a page id outside the pool or past max_pages) records a device error
+ * (spk_check_device_error) and touches nothing outside the pool. */
+typedef struct {
+    int nseq, rows;             /* sequences (1 to 1024); rows of all of them */
+    const int *row0;            /* device [nseq + 1], row0[0] = 0 */
+    const int *kv_len;          /* device [nseq]: cached tokens, this call's rows among them */
+    const int *table;           /* device [nseq][max_pages] page ids */
+    int max_pages;
+} spk_kv_batch;
+
+/* Appends the rows' keys and values: k, v [rows][kv_heads * head_dim] of `type` (0 f32, 1 f16,
+ * 2 bf16), rows ldk / ldv elements apart. Keys are rotated on the way as spk_attn_decode does
+ * (NeoX on the first pdim dims, angle f32(position * freq[i]); pdim a multiple of 8; freq NULL: as
+ * they are). A block that the call starts gets the scale max(amax / 448, 2^-100) of its rows; one
+ * that it continues keeps its scale if that is larger, and its earlier rows are rounded again if
+ * it is not. The rows of a block after the last appended one become 0. A NaN or infinity makes its
+ * block's scale NaN or infinite, never a byte. One launch, no sync. */
+int spk_paged_append(const spk_kv_pool *pool, const spk_kv_batch *batch, const void *k, long long ldk, const void *v,
+                     long long ldv, int type, const float *freq, int pdim, void *stream);
+
+/* Causal grouped-query attention of the rows over their sequences' pages (append them first):
+ *   out[t][h] = sigmoid(gate[t][h]) * softmax_j(scale * rope(q[t][h]) . K_j) V_j
+ * over j in [0, pos_t] (window 0) or (pos_t - window, pos_t]; q head h reads KV head
+ * h / (heads / kv_heads), any group. Sums and softmax in f32. A row that sees nothing gets 0.
+ * workspace: spk_paged_attn_workspace_bytes(head_dim) device bytes for the device current at the
+ * call, zeroed once and left ready; calls that share one must not overlap on the GPU. No sync. */
+typedef struct {
+    const void *q;              /* [rows][heads * head_dim] of type, rows ldq elements apart */
+    long long ldq;
+    int type, heads;            /* 0 f32, 1 f16, 2 bf16 (q, gate and out) */
+    const float *freq;          /* device [pdim / 2], or NULL: q is rotated already */
+    int pdim, window;
+    float scale;                /* 0: 1 / sqrt(head_dim) */
+    const void *gate;           /* [rows][heads] pre-sigmoid, rows ldgate apart, or NULL */
+    long long ldgate;
+    void *out;                  /* [rows][heads * head_dim], rows ldout apart */
+    long long ldout;
+    void *workspace;
+} spk_paged_attn_args;
+size_t spk_paged_attn_workspace_bytes(int head_dim);
+int spk_paged_attn(const spk_kv_pool *pool, const spk_kv_batch *batch, const spk_paged_attn_args *args, void *stream);
+
+/* What rows of logits say (scoring, n-best; the reference keeps the argmax alone, model.rs:594-604):
+ * for each of `rows` rows of `vocab` values of `type` (0 f32, 1 f16, 2 bf16), ld apart: logp (may
+ * be NULL) the log probability of target[row] (0 where the target is negative), entropy (may be
+ * NULL) of the distribution in nats, and the `top` (0 to 32) most likely tokens with their log
+ * probabilities, ties to the lower index, [rows][top]. -inf is a token that cannot come. A row
+ * with a NaN or +inf, or nothing but -inf, gives NaN. workspace: spk_logprobs_workspace_bytes
+ * device bytes, zeroed once and left ready; calls that share one must not overlap. One launch. */
+size_t spk_logprobs_workspace_bytes(int rows, int vocab);
+int spk_logprobs(const void *logits, int type, int rows, int vocab, long long ld, const int *target, float *logp,
+                 float *entropy, int top, int *top_ids, float *top_logp, void *workspace, void *stream);
+
 /* ------------------------------------------------------- tuning profiles */
 /* VQPROF 1 per-artifact tuning profiles (tools/vq/gpu/vq-profile.h:1-40, the format;
  * tools/vq-tune/src/profile.rs, the writer; vq-model-gpu.cu:1094-1122 and :301-324, how the

@@ -26,7 +26,7 @@ class SpkError(RuntimeError):
     pass
 
 
-_vp, _i, _f, _d, _cp = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_char_p
+_vp, _i, _f, _d, _cp, _ll = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_char_p, C.c_longlong
 _dp = C.POINTER(C.c_double)
 
 _PROTOS = {
@@ -122,6 +122,11 @@ _PROTOS = {
     "spk_vqprof_write": ([_cp, _vp], _i),
     "spk_model_use_profile": ([_vp, _vp], _i),
     "spk_model_kernel_of": ([_vp, _i, _i], _i),
+    "spk_paged_append": ([_vp, _vp, _vp, _ll, _vp, _ll, _i, _vp, _i, _vp], _i),
+    "spk_paged_attn_workspace_bytes": ([_i], C.c_size_t),
+    "spk_paged_attn": ([_vp, _vp, _vp, _vp], _i),
+    "spk_logprobs_workspace_bytes": ([_i, _i], C.c_size_t),
+    "spk_logprobs": ([_vp, _i, _i, _i, _ll, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp], _i),
 }
 
 
