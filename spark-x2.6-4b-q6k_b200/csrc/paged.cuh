@@ -83,25 +83,29 @@ __device__ __forceinline__ void unit_dims(int u, int pdim, int &d0, int &d1) {
     }
 }
 
-// Unit u of a row, rotated at position pos when it lies in the first pdim dims (model.rs:431-439:
-// the angle is the f32 product, each product of the rotation rounded).
+// Cosine and sine of the f32 product position * frequency (model.rs:431-439's angle). The whole turns
+// are taken out in f64, where a turn count up to 2^24 still leaves 29 bits of the fraction, and the
+// rest goes to sincospi: one path for every position, where sincosf branches at large angles.
+__device__ __forceinline__ void angle(int pos, float freq, float &c, float &s) {
+    const double turns = (double)__fmul_rn((float)pos, freq) * 0.15915494309189533577;
+    sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+}
+
 template <typename T>
-__device__ __forceinline__ void load_unit(const T *row, int u, const float *freq, int pdim, int pos, bool vec,
-                                          float (&a)[4], float (&b)[4]) {
+__device__ __forceinline__ void load_unit(const T *row, int u, int pdim, bool vec, float (&a)[4], float (&b)[4]) {
     int d0, d1;
     unit_dims(u, pdim, d0, d1);
     const float4 x = load4<T>(row + d0, vec), y = load4<T>(row + d1, vec);
     a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
     b[0] = y.x, b[1] = y.y, b[2] = y.z, b[3] = y.w;
-    if (u < pdim / 8) {
+}
+// The rotation of a unit's 4 pairs, each product rounded (model.rs:431-439).
+__device__ __forceinline__ void rotate_unit(float (&a)[4], float (&b)[4], const float (&c)[4], const float (&s)[4]) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float s, c;
-            sincosf(__fmul_rn((float)pos, __ldg(freq + d0 + i)), &s, &c);
-            const float p = a[i], q = b[i];
-            a[i] = __fsub_rn(__fmul_rn(p, c), __fmul_rn(q, s));
-            b[i] = __fadd_rn(__fmul_rn(q, c), __fmul_rn(p, s));
-        }
+    for (int i = 0; i < 4; i++) {
+        const float p = a[i], q = b[i];
+        a[i] = __fsub_rn(__fmul_rn(p, c[i]), __fmul_rn(q, s[i]));
+        b[i] = __fadd_rn(__fmul_rn(q, c[i]), __fmul_rn(p, s[i]));
     }
 }
 

@@ -1,7 +1,7 @@
 // paged_append.cu — new keys and values of a batch into the pages of the 8-bit cache.
 //
 // Row i of sequence s (rows row0[s] .. row0[s + 1] - 1) sits at position kv_len[s] - n_s + i. Its
-// key is rotated (paged.cuh load_unit), then, per KV head and per block of 16 tokens that the call
+// key is rotated (paged.cuh), then, per KV head and per block of 16 tokens that the call
 // touches, for keys and for values:
 //   d   = max(amax / 448, 2^-100), amax over the call's rows in the block; where the block holds
 //         earlier rows (the call starts inside it) also d >= its old scale
@@ -141,7 +141,13 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
         if (r >= lo && r < hi && lane < U) {
             const int row = r0 + blk * BLOCK + r - first;
             const T *src = keys ? (const T *)a.k + (size_t)row * a.ldk : (const T *)a.v + (size_t)row * a.ldv;
-            load_unit<T>(src + (size_t)head * HD, lane, a.freq, pdim, blk * BLOCK + r, keys ? a.kvec : a.vvec, p, q);
+            load_unit<T>(src + (size_t)head * HD, lane, pdim, keys ? a.kvec : a.vvec, p, q);
+            if (lane < pdim / 8) {
+                float c[4], sn[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) angle(blk * BLOCK + r, __ldg(a.freq + 4 * lane + e), c[e], sn[e]);
+                rotate_unit(p, q, c, sn);
+            }
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {

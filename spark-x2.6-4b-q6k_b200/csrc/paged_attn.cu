@@ -1,39 +1,51 @@
 // paged_attn.cu — causal grouped-query attention of each sequence's new rows over its pages of the
-// 8-bit cache, for few rows per sequence (decode steps, verify batches).
+// 8-bit cache, on the tcgen05 tensor cores: decode steps, verify batches and prompt chunks.
 //
 //   out[t][h] = sigmoid(gate[t][h]) * sum_j p_j V_j,  p = softmax_j(scale * rope(q[t][h]) . K_j),
 //   j in [0, pos_t], with a window in (pos_t - window, pos_t]; K_j = dk[block of j] * k_j and
 //   V_j = dv[block] * v_j with the cached e4m3 bytes k, v. A row that sees nothing gets 0.
 //
 // With w_j = exp(s_j) dv_j the value scale rides in the exponent: s'_j = s_j + log dv_j, one
-// running reference m per row, O = sum exp(s'_j - m) v_j and l = sum exp(s'_j - m) / dv_j, so that
-// the largest term of the sum is what the f16 weights are relative to, whatever the scales.
+// running reference m per row, O = sum exp(s'_j - m) v_j and l = sum exp(s'_j - m) / dv_j, so the
+// largest term of O's sum is what the weights are relative to, whatever the scales are.
 //
-// What bounds it: the cached bytes, read once per KV head. A (sequence, KV head) has n * group
-// query rows; a tile of R of them is one pass over the blocks, and the R rows are the 8 or 16
-// columns of the tensor-core products
-//   S^T[16 keys][cols] = K q^T     mma.sync m16n8k16, A = a block's key bytes as f16 (exact)
-//   O^T[hd][cols]     += V^T P^T   A = a block's value bytes, P^T by movmatrix
-// so no lane idles for want of rows and a block's scales are two scalars. f32 calls keep q and P as
-// f16 pairs (hi + lo columns, ~22 bits), f16 and bf16 calls as one f16; q's exponent is taken out
-// per row first.
+// The cache is read as it lies. Keys (and values) are the A operand, 128 tokens (128 dims) tall,
+// e4m3 straight from the bulk copies; the query rows are the N columns of the B operand, and what
+// 8 bits lack is made up in columns: a number x is the sum of T e4m3 terms, x = t0 + t1 / 32 +
+// t2 / 1024 .., each term the rounding of what the ones before left (4 bits and a sign a term), and
+// each term has a column of its own, so that it keeps its own scale and nothing underflows:
+//   S^T[128 keys][term, row]  = K . q^T     scores: sum of a row's T columns
+//   O^T[hd][term, row]       += V^T . P^T   weights split the same way, one byte a column
+// Products of e4m3 pairs are exact and are added in f32, so T terms carry about 4.6 T bits: two
+// hold bf16 (8 bits), three f16 (11), five f32.
 //
-// Work split: all (sequence, KV head, row tile, block) units in one line, cut into equal ranges,
-// one per CTA, one CTA per SM; a warp owns every 8th block of a range and streams it by two bulk
-// copies through its own ring of mbarrier slots, meeting the other warps only at the end of a
-// (sequence, KV head, row tile). Ranges that end inside one leave (O, m, l) in the workspace and
-// the last CTA to arrive (a ticket that it resets) adds them up in CTA order.
+// What bounds it: for few rows the cached bytes, read once per KV head (an MMA of 16 columns costs
+// what its A bytes cost to read from shared memory, and the softmax runs on keys x rows alone); for
+// prompt chunks the softmax's instructions, 64 bf16 rows against each 128 keys.
+//
+// Work split: all (sequence, KV head, row tile) groups stand in one line, each as long as the
+// tokens it reads plus SEG_COST for its fixed cost; the line is cut into equal ranges, one per CTA,
+// one CTA per SM. A 128-token tile belongs to the CTA in whose range its first token falls. A group
+// that several CTAs share leaves (O, m, l) in the workspace; the last CTA to arrive (a ticket that it
+// resets) adds the parts in CTA order.
+//
+// Warps: 0 bulk copies (pages, scales), 1 MMA issue, 2-5 queries of the next group, 6.. softmax:
+// a thread per key, and per output dim at the end of a group.
 #include "paged.cuh"
 
 namespace spk {
 namespace paged {
 namespace {
 
-constexpr int AT_WARPS = 8, AT_THREADS = AT_WARPS * 32;
-constexpr float M_NONE = -1e30f;      // reference of a row that has seen nothing
-constexpr float P_SHIFT = 7.0f;       // weights are kept as 2^7 exp(s' - m): f16 holds them from 2^-31 to 2^8
-constexpr float M_SLACK = 8.0f;       // the reference moves only when a score passes it by 2^8
+constexpr float M_NONE = -1e30f;      // reference of a part that has seen nothing
+// Weights are 2^(s' - m): a new reference sits W_TOP below the largest score, so weights start at 8, and
+// it moves only when a score passes m + 8, so they end at 256 (e4m3 holds 448).
+constexpr float W_TOP = 3.0f, W_MAX = 8.0f;
+constexpr float STEP = 32.0f;         // a term's scale over the one before: half an ulp of 256 is 8
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int TILE = 128, TB = TILE / BLOCK;   // keys of a tile, its blocks
+constexpr int SEG_COST = 16;          // a group's fixed cost in blocks
+constexpr int Q_WARPS = 4;
 
 struct AttnParams {
     Pool pool;
@@ -46,38 +58,127 @@ struct AttnParams {
     int pdim, heads, group, window;
     float scale;                      // softmax scale * log2(e)
     unsigned int *tickets;            // [gridDim.x], zero at rest
-    float *part;                      // [gridDim.x][2][R * (HD + 2)]
+    float *part;                      // [gridDim.x][2][PART]
     int *err;
 };
 
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
+// N columns, T terms, R rows a tile (T R <= N), SG softmax warpgroups
+template <int HD_, int N_, int T_, int R_>
+struct Cfg {
+    static constexpr int HD = HD_, N = N_, T = T_, R = R_;
+    static constexpr int SG = N >= 128 ? 2 : 1;
+    static constexpr int RG = R / SG;                         // rows of a warpgroup, side by side
+    static constexpr int CH = SG == 1 ? R : RG % 8 ? 4 : 8;   // rows handled together
+    static constexpr int NC = RG / CH;
+    static constexpr int LD = SG == 1 ? 8 : CH;               // columns of a tensor-memory access
+    static constexpr int LC = SG == 1 ? (T * R + 7) / 8 * 8 : CH * T;   // columns of a chunk: all, or CH a term
+    static constexpr int KB = BLOCK * HD;                     // bytes of a block's keys (or values)
+    static constexpr int STAGE = 2 * TB * KB;
+    static constexpr int NST = N >= 128 ? (HD == 256 ? 2 : HD == 128 ? 4 : 6) : (HD == 256 ? 3 : HD == 128 ? 6 : 8);
+    static constexpr int QB = N >= 128 && HD == 256 ? 1 : 2;  // query buffers
+    static constexpr int HH = HD == 256 ? 2 : 1;              // 128-dim halves of the output
+    static constexpr int TCOLS = (2 + HH) * N <= 64 ? 64 : (2 + HH) * N <= 128 ? 128 : (2 + HH) * N <= 256 ? 256 : 512;
+    static constexpr size_t Q_OFF = (size_t)NST * STAGE, P_OFF = Q_OFF + (size_t)QB * N * HD;
+    static constexpr size_t SMEM = P_OFF + (size_t)2 * N * TILE;
+    static constexpr int WARPS = 2 + Q_WARPS + 4 * SG, THREADS = WARPS * 32;
+    static constexpr int PART = (R * (HD + 2) + 3) / 4 * 4;   // floats of a partial: O, then m, then l; read 16 bytes at a time
+    static_assert(T * R <= N && R % SG == 0 && RG % CH == 0, "");
+    // access x of chunk ch of warpgroup sg: its column
+    static __device__ __forceinline__ int col(int sg, int ch, int x) { return SG == 1 ? 8 * x : x * R + sg * RG + ch * CH; }
+    static constexpr int TS = SG == 1 ? R : CH;               // a chunk's terms lie this far apart
+};
+
+// ------------------------------------------------------------------ tensor cores
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {   // K-major, no swizzle
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
+           ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// K columns of this thread's lane; tm_wait before their use
+template <int K>
+__device__ __forceinline__ void tm_ld(uint32_t addr, float *v) {
+    static_assert(K == 4 || K == 8, "");
+    if constexpr (K == 4)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                     : "r"(addr));
+    else
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                     : "r"(addr));
+}
+template <int K>
+__device__ __forceinline__ void tm_st(uint32_t addr, const float *v) {
+    if constexpr (K == 4)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0,%1,%2,%3};" ::"f"(v[0]), "f"(v[1]), "f"(v[2]),
+                     "f"(v[3]), "r"(addr)
+                     : "memory");
+    else
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"f"(v[0]), "f"(v[1]),
+                     "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "r"(addr)
+                     : "memory");
+}
+// The loads have landed; their registers pass through, so no use of them moves up.
+template <int K>
+__device__ __forceinline__ void tm_wait(float (&v)[K]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < K; i++) asm volatile("" : "+f"(v[i]));
 }
 
-// 4 e4m3 bytes as two exact f16 pairs (bytes 0,1 | bytes 2,3)
-__device__ __forceinline__ void e4m3x4_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-        : "=r"(lo), "=r"(hi)
-        : "r"(w));
-}
-
-__device__ __forceinline__ uint32_t movm(uint32_t x) {   // 8 x 8 f16 transpose across the warp
-    uint32_t r;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-    return r;
-}
-
-__device__ __forceinline__ uint32_t f16x2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// e4m3 pair (low byte a) and its values
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 e4m3x2_f32(uint32_t w) {
+    return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
+}
+
+// Two weights as T e4m3 terms, a pair of bytes each. Two terms go by f16 (11 bits, they hold 9).
+template <int T>
+__device__ __forceinline__ void split(float a, float b, uint32_t (&w)[T]) {
+    if constexpr (T == 2) {
+        const __half2 h = __floats2half2_rn(a, b);
+        uint16_t x, y;
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(x) : "r"(*reinterpret_cast<const uint32_t *>(&h)));
+        uint32_t f;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f) : "h"(x));
+        const __half2 r = __hmul2(__hsub2(h, *reinterpret_cast<const __half2 *>(&f)), __float2half2_rn(STEP));
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(y) : "r"(*reinterpret_cast<const uint32_t *>(&r)));
+        w[0] = x;
+        w[1] = y;
+    } else {
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            w[t] = e4m3x2(a, b);
+            if (t + 1 < T) {
+                const float2 v = e4m3x2_f32(w[t]);
+                a = (a - v.x) * STEP;
+                b = (b - v.y) * STEP;
+            }
+        }
+    }
+}
+__device__ __forceinline__ float warp_max(float x) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -98,501 +199,807 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <int HD, int NT, int TERMS>
-struct Cfg {
-    static constexpr int COLS = 8 * NT;
-    static constexpr int R = COLS / TERMS;                    // query rows of a tile
-    static constexpr int KB = BLOCK * HD, STAGE = 2 * KB;     // bytes of a block's keys; keys and values
-    static constexpr int NS = 512 / HD;                       // ring slots of a warp (16 KB)
-    static constexpr int QS = HD * 2 + 32;                    // bytes of a q column in shared memory (padded)
-    static constexpr int OR = R / NT;                         // rows merged at a time (one n-tile)
-    static constexpr size_t RING = (size_t)AT_WARPS * NS * STAGE;
-    static constexpr size_t MERGE = (size_t)AT_WARPS * OR * HD * 4;
-    static constexpr size_t SMEM = RING + MERGE + (size_t)COLS * QS;
-    static constexpr int PART = R * (HD + 2);                 // floats of a partial: O, then m, then l
-};
+// Bounded wait. The first one that runs out records the error and marks the CTA dead; from then on
+// waits return at once, copies and MMAs are no longer issued, and every warp still walks its range, so
+// that none is left at a barrier.
+__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, int *dead, int *err) {
+    for (uint32_t i = 0; i < SPK_WAIT_LIMIT; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255u) == 255u && *(volatile int *)dead) return false;
+    }
+    *(volatile int *)dead = 1;
+    if (err) atomicExch(err, DEV_WAIT_TIMEOUT);
+    return false;
+}
+__device__ __forceinline__ void mbar_expect(uint64_t *bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ bool bar_or(int id, int n, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %3, 0;\n\tbarrier.cta.red.or.pred q, %1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"(n), "r"((uint32_t)x)
+        : "memory");
+    return r != 0;
+}
 
-// units (16-token blocks x KV heads x row tiles) of sequence s; the first block any row sees
+// ------------------------------------------------------------------ the line of work
+// Lengths are in blocks and fit 32 bits (the entry point refuses a batch that could not).
 struct Seq {
-    int r0, n, len, first_blk, nblk, tiles;
+    int r0, n, len, tiles;            // rows of the call, cached tokens, row tiles
+    int c, slope;                     // group j is at most (c + slope (j + 1)) / 16 blocks long
 };
 __device__ __forceinline__ Seq seq_of(const AttnParams &a, int s, int R) {
     Seq q;
     q.r0 = __ldg(a.b.row0 + s);
     q.n = __ldg(a.b.row0 + s + 1) - q.r0;
     q.len = __ldg(a.b.kv_len + s);
-    q.first_blk = q.nblk = q.tiles = 0;
     const long long room = (long long)a.b.max_pages * a.pool.page_tokens;
-    if (q.n == 0) return q;
-    if (q.n < 0 || q.r0 < 0 || q.r0 > a.b.rows - q.n || q.len > room) {   // not a batch: nothing is read
+    if (q.n != 0 && (q.n < 0 || q.r0 < 0 || q.r0 > a.b.rows - q.n || q.len > room)) {   // not a batch: nothing is read
         if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
         q.n = 0;
-        return q;
     }
-    const int pos0 = q.len - q.n;
-    if (a.window > 0) q.first_blk = max(0, pos0 + 1 - a.window) / BLOCK;
-    // a sequence with nothing cached still has rows to write (zeros): one empty block
-    q.nblk = max(1, (q.len + BLOCK - 1) / BLOCK - q.first_blk);
     q.tiles = (int)(((long long)q.n * a.group + R - 1) / R);
+    const int step = (R + a.group - 1) / a.group, pos0 = max(0, q.len - q.n);
+    if (a.window > 0 && a.window < q.len) {
+        q.c = min(q.len, a.window + step + BLOCK);
+        q.slope = 0;
+    } else {
+        q.c = pos0;
+        q.slope = step;
+    }
     return q;
 }
+// Length of group j and of groups 0 .. j - 1: the tokens' sum, a partial block each, the fixed costs.
+__device__ __forceinline__ uint32_t before(const Seq &q, uint32_t j) {
+    const unsigned long long t = (unsigned long long)j * q.c + (unsigned long long)q.slope * j * (j + 1) / 2;
+    return (uint32_t)(t / BLOCK) + j * (SEG_COST + 2);
+}
 
-template <typename T, int HD, int NT, int TERMS>
-__global__ void __launch_bounds__(AT_THREADS, 1) attn_kernel(const AttnParams a) {
-    using C = Cfg<HD, NT, TERMS>;
-    constexpr int R = C::R, KT = HD / 16;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t bars[AT_WARPS][C::NS];
-    __shared__ float4 meta[AT_WARPS][C::NS];            // a slot's dk, log2 dv, 1 / dv, and whether it was issued
-    __shared__ long long pre[MAX_SEQ + 1];              // units before each sequence
-    __shared__ long long wsum[AT_WARPS];
-    __shared__ float wm[AT_WARPS][R], wl[AT_WARPS][R];
-    __shared__ float qf[R];                             // per row: score factor
-    __shared__ int qpos[R];                             // per row: position, -1 past the end
-    __shared__ float cw[256];
+struct Seg {
+    int s, r0, kvh;                   // sequence, its first row, KV head
+    int c0, c1, pos0;                 // columns (token * group + head) of the tile, c1 the last; position of row 0
+    int p_lo, p_hi, see0;             // first and last row's positions, first token that a row sees
+    int start, k0, k1;                // first token of tile 0; this CTA's tiles
+    int f0, f1;                       // the CTAs that share the group
+    int nblk;                         // blocks from start that some row sees (0: nothing is seen)
+};
+
+// Walks a CTA's range of the line.
+struct Walk {
+    uint32_t x0, x1, chunk, base;     // range; the group's place
+    int s, kvh, j;
+    Seq q;
+};
+__device__ __noinline__ void walk_begin(const AttnParams &a, const uint32_t *pre, int R, Walk &w) {
+    const uint32_t total = pre[a.b.nseq];
+    w.chunk = max((total + gridDim.x - 1) / gridDim.x, (uint32_t)TB);
+    w.x0 = w.chunk * blockIdx.x;
+    w.x1 = min(total, w.x0 + w.chunk);
+    w.s = w.kvh = w.j = 0;
+    w.base = w.x1;
+    if (w.x0 >= w.x1) return;
+    int lo = 0, hi = a.b.nseq;        // the last sequence with pre <= x0: it is not empty
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= w.x0) lo = mid;
+        else hi = mid;
+    }
+    w.s = lo;
+    w.q = seq_of(a, lo, R);
+    const uint32_t per = before(w.q, w.q.tiles), in = w.x0 - pre[lo];
+    w.kvh = in / per;
+    const uint32_t rem = in - w.kvh * per;
+    int a0 = 0, a1 = w.q.tiles;       // the last group with before <= rem
+    while (a1 - a0 > 1) {
+        const int mid = (a0 + a1) >> 1;
+        if (before(w.q, mid) <= rem) a0 = mid;
+        else a1 = mid;
+    }
+    w.j = a0;
+    w.base = pre[lo] + w.kvh * per + before(w.q, a0);
+}
+// The next group of which this CTA has tiles.
+__device__ __noinline__ bool walk_next(const AttnParams &a, const uint32_t *pre, int R, Walk &w, Seg &g) {
+    while (w.base < w.x1) {
+        const int G = a.group, c0 = w.j * R, c1 = min(c0 + R, w.q.n * G) - 1, pos0 = w.q.len - w.q.n;
+        const int p_lo = pos0 + c0 / G, p_hi = pos0 + c1 / G;
+        const int see0 = a.window > 0 ? max(0, p_lo + 1 - a.window) : 0, b0 = see0 / BLOCK;
+        const int nblk = p_hi < 0 ? 0 : p_hi / BLOCK + 1 - b0;
+        const int nt = max(1, (nblk + TB - 1) / TB);   // one empty tile where nothing is seen
+        const uint32_t t0 = w.base + SEG_COST;         // tile k stands at t0 + TB k, inside the group's length
+        const int d0 = (int)(w.x0 - t0), d1 = (int)(w.x1 - t0);
+        const int k0 = d0 <= 0 ? 0 : (d0 + TB - 1) / TB, k1 = d1 <= 0 ? 0 : min(nt, (d1 + TB - 1) / TB);
+        const bool mine = k0 < k1;
+        if (mine)
+            g = Seg{w.s, w.q.r0, w.kvh, c0, c1, pos0, p_lo, p_hi, see0, b0 * BLOCK, k0, k1,
+                    (int)(t0 / w.chunk), (int)((t0 + (uint32_t)(TB * (nt - 1))) / w.chunk), nblk};
+        const uint32_t at = before(w.q, w.j);
+        w.base += before(w.q, ++w.j) - at;
+        if (w.j == w.q.tiles) {
+            w.j = 0;
+            if (++w.kvh == a.pool.kv_heads) {
+                w.kvh = 0;
+                while (++w.s < a.b.nseq && pre[w.s + 1] == pre[w.s]) {}
+                if (w.s < a.b.nseq) w.q = seq_of(a, w.s, R);
+            }
+        }
+        if (mine) return true;
+    }
+    return false;
+}
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a) {
+    constexpr int HD = C::HD, N = C::N, TT = C::T, R = C::R, NST = C::NST, QB = C::QB;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ uint64_t full_k[NST], full_v[NST], empty[NST], s_full[2], p_full[2], pv_done[2], q_full[QB], q_empty[QB];
+    __shared__ float2 scales[NST][TB];                  // dk, dv of a tile's blocks
+    __shared__ uint32_t pre[MAX_SEQ + 1], wsum[C::WARPS];
+    __shared__ float q_up[4];                           // score factor of a query tile: the softmax may be two behind
+    __shared__ int dead;                                // a wait ran out: what follows no longer waits
+    __shared__ float red[C::SG][4][C::RG];              // per row: the warps' maxima, then their sums
+    __shared__ __align__(16) float mref[C::SG][(C::RG + 3) / 4 * 4];   // per row: the reference m
+    __shared__ uint32_t moved[C::SG][4];                // the warps' chunks whose reference has to move
+    __shared__ __align__(16) float fs[C::SG][(C::RG + 3) / 4 * 4];     // per row: a factor for all of its outputs
+    __shared__ int pos_s[R];                            // per row: position, -1 past the tile's last row
+    __shared__ size_t out_s[R];                         // per row: where its output lies
+    __shared__ float amax_s[Q_WARPS];
     __shared__ int last_in;
-    uint8_t *ring = smem;
-    float *merge = reinterpret_cast<float *>(smem + C::RING);
-    uint8_t *qs = smem + C::RING + C::MERGE;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    pdl_trigger();
-    if (tid < AT_WARPS * C::NS) mbar_init(&bars[0][0] + tid, 1);
-    fence_mbar_init();
-    pdl_wait();
+    __shared__ uint32_t tmem_s;
+    uint8_t *qs = smem + C::Q_OFF, *ps = smem + C::P_OFF;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-    // the line of units: an exclusive scan over the sequences
-    long long base = 0;
-    for (int s0 = 0; s0 < a.b.nseq; s0 += AT_THREADS) {
+    if (tid == 0) {
+        for (int i = 0; i < NST; i++) {
+            mbar_init(full_k + i, 1);
+            mbar_init(full_v + i, 1);
+            mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(s_full + i, 1);
+            mbar_init(p_full + i, 4 * C::SG);
+            mbar_init(pv_done + i, 1);
+        }
+        for (int i = 0; i < QB; i++) {
+            mbar_init(q_full + i, Q_WARPS);
+            mbar_init(q_empty + i, 1);
+        }
+        dead = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {   // this warp owns the tensor memory
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)),
+                     "r"((uint32_t)C::TCOLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    pdl_trigger();   // after the allocation: a dependent that took tensor memory first would wait on this kernel
+    pdl_wait();
+    const uint32_t tmem = tmem_s;
+
+    // the line: an exclusive scan over the sequences
+    uint32_t base = 0;
+    for (int s0 = 0; s0 < a.b.nseq; s0 += C::THREADS) {
         const int s = s0 + tid;
-        long long u = 0;
+        uint32_t u = 0;
         if (s < a.b.nseq) {
             const Seq q = seq_of(a, s, R);
-            u = (long long)q.nblk * q.tiles * a.pool.kv_heads;
+            u = before(q, q.tiles) * a.pool.kv_heads;
         }
-        long long x = u;
+        uint32_t x = u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
         if (lane == 31) wsum[warp] = x;
         __syncthreads();
-        long long add = base;
-        for (int w = 0; w < warp; w++) add += wsum[w];
+        uint32_t add = base, all = base;
+        for (int w = 0; w < C::WARPS; w++) {
+            if (w < warp) add += wsum[w];
+            all += wsum[w];
+        }
         if (s < a.b.nseq) pre[s] = add + x - u;
-        long long all = base;
-        for (int w = 0; w < AT_WARPS; w++) all += wsum[w];
         base = all;
         __syncthreads();
     }
     if (tid == 0) pre[a.b.nseq] = base;
     __syncthreads();
-    const long long total = base;
-    // equal ranges, at least a block per warp
-    long long chunk = (total + gridDim.x - 1) / gridDim.x;
-    if (chunk < AT_WARPS) chunk = AT_WARPS;
-    const long long u0 = chunk * blockIdx.x, u1 = min(total, u0 + chunk);
-    uint32_t used = 0;   // this warp's ring uses so far (slot used % NS, parity used / NS)
 
-    int s = 0;
-    if (u0 < u1) {   // the sequence of u0: the last with pre <= u0 that has units
-        int lo = 0, hi = a.b.nseq;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (pre[mid] <= u0) lo = mid;
-            else hi = mid;
-        }
-        s = lo;
-    }
-    for (long long u = u0; u < u1;) {
-        while (pre[s + 1] <= u) s++;
-        const Seq q = seq_of(a, s, R);
-        const long long in = u - pre[s];
-        const int gr = (int)(in / q.nblk), b0 = (int)(in - (long long)gr * q.nblk);   // group (KV head, row tile)
-        const int b1 = (int)min((long long)q.nblk, b0 + (u1 - u));
-        const int kvh = gr / q.tiles, tile = gr - kvh * q.tiles;
-        const int pos0 = q.len - q.n;
-        // blocks that some row of the tile sees
-        const int c0 = tile * R, c1 = min(c0 + R, q.n * a.group) - 1;
-        const int p_lo = pos0 + c0 / a.group, p_hi = pos0 + c1 / a.group;
-        const int see0 = a.window > 0 ? max(0, p_lo + 1 - a.window) : 0;
-        const int x0 = max(b0, see0 / BLOCK - q.first_blk), x1 = min(b1, p_hi < 0 ? 0 : p_hi / BLOCK + 1 - q.first_blk);
-        const int cnt = x1 > x0 + warp ? (x1 - x0 - warp + AT_WARPS - 1) / AT_WARPS : 0;   // this warp's blocks
-        const int bfirst = q.first_blk + x0 + warp;
-
-        // 32 of the warp's blocks at a time: lane l holds block i's place in the pool and its scales
-        size_t at = 0;
-        float dk = 0.f, dv = 1.f;
-        auto look = [&](int i0) {
-            const int i = i0 + lane;
-            at = 0;
-            if (i < cnt) {
-                const int blk = bfirst + i * AT_WARPS, per = a.pool.page_tokens / BLOCK;
-                int page = __ldg(a.b.table + (size_t)s * a.b.max_pages + blk / per);
-                if (page < 0 || page >= a.pool.pages) {
-                    if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
-                    page = 0;
+    Walk w;
+    Seg g;
+    walk_begin(a, pre, R, w);
+    if (w.x0 >= w.x1) {
+    } else if (warp == 0) {   // ------------------------------------------------------ copies
+        // lane l < 8: the keys and values of a tile's block l; its page comes one tile ahead
+        const int per = a.pool.page_tokens / BLOCK;
+        uint32_t i = 0;
+        while (walk_next(a, pre, R, w, g)) {
+            const int blk0 = g.start / BLOCK, nblk = g.nblk, k1 = g.k1, kvh = g.kvh;
+            const int *table = a.b.table + (size_t)g.s * a.b.max_pages;
+            auto page_of = [&](int k) {
+                int page = 0;
+                if (k < k1 && lane < min(TB, nblk - k * TB)) {
+                    page = __ldg(table + (blk0 + k * TB + lane) / per);
+                    if (page < 0 || page >= a.pool.pages) {
+                        if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
+                        page = 0;
+                    }
                 }
-                at = block_index(a.pool, page, kvh, blk % per);
-                dk = a.pool.ks[at];
-                dv = a.pool.vs[at];
+                return page;
+            };
+            int page = page_of(g.k0);
+            for (int k = g.k0; k < k1 && nblk > 0; k++) {
+                const int nb = min(TB, nblk - k * TB), st = i % NST;
+                const size_t bi = block_index(a.pool, page, kvh, (blk0 + k * TB + lane) % per);
+                float2 sc = make_float2(0.f, 1.f);
+                if (lane < nb) sc = make_float2(__ldg(a.pool.ks + bi), __ldg(a.pool.vs + bi));
+                page = page_of(k + 1);
+                const bool free_ = i < NST || wait_for(empty + st, ((i / NST) - 1) & 1, &dead, a.err);
+                i++;
+                if (!__all_sync(0xffffffffu, free_)) continue;
+                uint8_t *kd = smem + (size_t)st * C::STAGE, *vd = kd + TB * C::KB;
+                if (nb & 1) {   // the MMAs take values by two blocks: the missing one is 0
+                    for (int o = 16 * lane; o < C::KB; o += 512)
+                        *reinterpret_cast<uint4 *>(vd + nb * C::KB + o) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();
+                }
+                if (lane == 0) {
+                    mbar_expect(full_k + st, nb * C::KB);
+                    mbar_expect(full_v + st, nb * C::KB);
+                }
+                __syncwarp();
+                if (lane < nb) {
+                    bulk_g2s(kd + lane * C::KB, a.pool.k + bi * C::KB, C::KB, full_k + st);
+                    bulk_g2s(vd + lane * C::KB, a.pool.v + bi * C::KB, C::KB, full_v + st);
+                    scales[st][lane] = sc;
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(full_v + st);
+                    mbar_arrive(full_k + st);
+                }
             }
-        };
-        auto issue = [&](int i) {   // all lanes
-            if ((i & 31) == 0) look(i);
-            const size_t bi = __shfl_sync(0xffffffffu, at, i & 31);
-            const float k_ = __shfl_sync(0xffffffffu, dk, i & 31), v_ = __shfl_sync(0xffffffffu, dv, i & 31);
-            const int slot = (used + i) % C::NS;
-            __syncwarp();
-            if (lane == 0) {
-                meta[warp][slot] = make_float4(k_, log2f(v_), 1.0f / v_, 0.f);
-                uint8_t *d = ring + ((size_t)warp * C::NS + slot) * C::STAGE;
-                mbar_arrive_expect_tx(&bars[warp][slot], C::STAGE);
-                bulk_g2s(d, a.pool.k + bi * C::KB, C::KB, &bars[warp][slot]);
-                bulk_g2s(d + C::KB, a.pool.v + bi * C::KB, C::KB, &bars[warp][slot]);
+        }
+        if (*(volatile int *)&dead)   // copies in flight land before the CTA's memory goes
+            for (uint32_t x = i > NST ? i - NST : 0; x < i; x++)
+                for (uint32_t y = 0; y < (1u << 20) && !(mbar_try_wait(full_k + x % NST, (x / NST) & 1) &&
+                                                        mbar_try_wait(full_v + x % NST, (x / NST) & 1)); y++) {}
+    } else if (warp == 1) {   // ------------------------------------------------------ MMAs
+        if (lane == 0) {
+            const uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+            const uint32_t so = tmem, oo = tmem + 2 * N;
+            // descriptors move by their address field alone
+            const uint64_t kdesc = smem_desc(smem_u32(smem), 128, 8 * HD);
+            const uint64_t qdesc = smem_desc(smem_u32(qs), 128, 8 * HD);
+            const uint64_t vdesc = smem_desc(smem_u32(smem) + TB * C::KB, C::KB, 128);
+            const uint64_t pdesc = smem_desc(smem_u32(ps), 128, 1024);
+            uint32_t i = 0, qi = 0;   // tiles whose scores were issued; groups
+            // the tile whose values come next: its place, blocks, and whether it is its group's first
+            bool have = false, pfirst = false;
+            int pnb = 0;
+            uint32_t pi = 0;
+            auto values = [&]() {   // PV of tile pi
+                const int st = pi % NST;
+                if (!wait_for(p_full + (pi & 1), (pi >> 1) & 1, &dead, a.err) ||
+                    !wait_for(full_v + st, (pi / NST) & 1, &dead, a.err))
+                    return;
+                tc_after();
+                const uint64_t vd = vdesc + (uint32_t)(st * (C::STAGE / 16)), pd = pdesc + (uint32_t)((pi & 1) * (N * TILE / 16));
+#pragma unroll
+                for (int kk = 0; kk < TB / 2; kk++)
+                    if (2 * kk < pnb)
+#pragma unroll
+                        for (int h = 0; h < C::HH; h++)
+                            mma_e4m3(oo + h * N, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * 16, idesc,
+                                     !pfirst || kk > 0);
+                mma_commit(pv_done + (pi & 1));
+                mma_commit(empty + st);
+            };
+            while (walk_next(a, pre, R, w, g)) {
+                if (g.nblk == 0) continue;
+                const int qb = qi % QB, k0 = g.k0, k1 = g.k1, nblk = g.nblk;
+                const bool q_here = wait_for(q_full + qb, (qi / QB) & 1, &dead, a.err);
+                const uint64_t qd = qdesc + (uint32_t)(qb * (N * HD / 16));
+                for (int k = k0; k < k1; k++) {
+                    const int st = i % NST;
+                    if (wait_for(full_k + st, (i / NST) & 1, &dead, a.err) && q_here) {
+                        tc_after();
+                        const uint64_t kd = kdesc + (uint32_t)(st * (C::STAGE / 16));
+#pragma unroll
+                        for (int kk = 0; kk < HD / 32; kk++)
+                            mma_e4m3(so + (i & 1) * N, kd + kk * 16, qd + kk * 16, idesc, kk > 0);
+                        mma_commit(s_full + (i & 1));
+                        if (k + 1 == k1) mma_commit(q_empty + qb);
+                    }
+                    if (have) values();
+                    have = true;
+                    pi = i;
+                    pnb = min(TB, nblk - k * TB);
+                    pfirst = k == k0;
+                    i++;
+                }
+                qi++;
             }
-            __syncwarp();
-        };
-        for (int i = 0; i < C::NS && i < cnt; i++) issue(i);
-
-        // the tile's queries: a warp per row, rotated, scaled to [1, 2), as f16 (pairs)
-        for (int r = warp; r < R; r += AT_WARPS) {
-            const int c = c0 + r;
-            const bool real = c <= c1;
-            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-            const int tok = c / a.group, pos = pos0 + tok;
-            if (real && lane < HD / 8) {
-                const T *src = (const T *)a.q + (size_t)(q.r0 + tok) * a.ldq + (size_t)(kvh * a.group + c % a.group) * HD;
-                load_unit<T>(src, lane, a.freq, a.pdim, pos, a.qvec, x, y);
-            }
+            if (have) values();
+        }
+    } else if (warp < 2 + Q_WARPS) {   // ------------------------------------------------- queries
+        const int qw = warp - 2;
+        uint32_t qi = 0;
+        while (walk_next(a, pre, R, w, g)) {
+            if (g.nblk == 0) continue;
+            const int qb = qi % QB, c0 = g.c0, c1 = g.c1, pos0 = g.pos0;
+            const T *q0 = (const T *)a.q + (size_t)g.r0 * a.ldq + (size_t)g.kvh * a.group * HD;
+            // a warp takes RW rows side by side, QROWS at a time (they stay in registers where that is all)
+            constexpr int RW = (R + Q_WARPS - 1) / Q_WARPS, QROWS = RW < 4 ? RW : 4;
+            float x[QROWS][4], y[QROWS][4];
+            auto load = [&](int r0) {
+#pragma unroll
+                for (int r = 0; r < QROWS; r++) {
+                    const int row = qw * RW + r0 + r, c = c0 + row;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[r][e] = y[r][e] = 0.f;
+                    if (r0 + r < RW && row < R && c <= c1 && lane < HD / 8)
+                        load_unit<T>(q0 + (size_t)(c / a.group) * a.ldq + (size_t)(c % a.group) * HD, lane, a.pdim,
+                                     a.qvec, x[r], y[r]);
+                }
+            };
+            int d0, d1, turned = -1;
+            unit_dims(lane, a.pdim, d0, d1);
+            float cs[4], sn[4], fr[4];
+            if (lane < a.pdim / 8)
+#pragma unroll
+                for (int e = 0; e < 4; e++) fr[e] = __ldg(a.freq + d0 + e);
+            auto turn = [&](int tok) {   // the heads of a token share its angles
+                if (lane < a.pdim / 8 && tok != turned) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) angle(pos0 + tok, fr[e], cs[e], sn[e]);
+                    turned = tok;
+                }
+            };
+            // the tile's largest finite value: the rotation grows a pair by at most sqrt(2)
             float mx = 0.f;
+            for (int r0 = 0; r0 < RW; r0 += QROWS) {
+                load(r0);
+                if (r0 == 0) turn((c0 + qw * RW) / a.group);   // while the rows are on their way
 #pragma unroll
-            for (int e = 0; e < 4; e++) mx = fmaxf(mx, fmaxf(fabsf(x[e]), fabsf(y[e])));
+                for (int r = 0; r < QROWS; r++)
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            // 2^-e and 2^e by exponent bits; a row of zeros, denormals or infinities keeps 1
+                    for (int e = 0; e < 4; e++) {
+                        const float u = fabsf(x[r][e]), v = fabsf(y[r][e]);
+                        mx = fmaxf(mx, fmaxf(u < INFINITY ? u : 0.f, v < INFINITY ? v : 0.f));
+                    }
+            }
+            mx = warp_max(mx);
+            if (lane == 0) amax_s[qw] = mx;
+            bar_sync(3, Q_WARPS * 32);
+#pragma unroll
+            for (int e = 0; e < Q_WARPS; e++) mx = fmaxf(mx, amax_s[e]);
+            // times 2^(6 - e), so that it lies in [64, 128); a tile of zeros stays
             const int ex = (int)(__float_as_uint(mx) >> 23);
-            const bool ok = ex >= 2 && ex <= 252;
-            const float dn = ok ? __uint_as_float((uint32_t)(254 - ex) << 23) : 1.0f;
-            const float up = ok ? __uint_as_float((uint32_t)ex << 23) : 1.0f;
-            if (lane < HD / 8) {
-                int d0, d1;
-                unit_dims(lane, a.pdim, d0, d1);
-                const int col = TERMS == 2 ? (r >> 2) * 8 + (r & 3) : r;
+            const bool sane = ex >= 8 && ex <= 246;
+            const float dn = sane ? __uint_as_float((uint32_t)(260 - ex) << 23) : 1.0f;
+            const float up = sane ? __uint_as_float((uint32_t)(ex - 6) << 23) : 1.0f;
+            uint8_t *dst = qs + (size_t)qb * N * HD;
+            if (qi >= QB) wait_for(q_empty + qb, ((qi / QB) - 1) & 1, &dead, a.err);
+            for (int r0 = 0; r0 < RW; r0 += QROWS) {
+                if (RW > QROWS) load(r0);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[e] *= dn;
-                    y[e] *= dn;
-                }
-                uint8_t *at0 = qs + (size_t)col * C::QS;
-                *reinterpret_cast<uint2 *>(at0 + 2 * d0) = make_uint2(f16x2(x[0], x[1]), f16x2(x[2], x[3]));
-                *reinterpret_cast<uint2 *>(at0 + 2 * d1) = make_uint2(f16x2(y[0], y[1]), f16x2(y[2], y[3]));
-                if (TERMS == 2) {
+                for (int r = 0; r < QROWS; r++) {
+                    const int row = qw * RW + r0 + r;
+                    if (r0 + r >= RW || row >= R) continue;
+                    turn((c0 + row) / a.group);
+                    if (lane < a.pdim / 8) rotate_unit(x[r], y[r], cs, sn);
+                    if (lane >= HD / 8) continue;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        x[e] -= __half2float(__float2half_rn(x[e]));
-                        y[e] -= __half2float(__float2half_rn(y[e]));
+                        x[r][e] = fmaf(x[r][e], dn, x[r][e] - x[r][e]);   // an infinity becomes a NaN, which e4m3 has
+                        y[r][e] = fmaf(y[r][e], dn, y[r][e] - y[r][e]);
                     }
-                    at0 += 4 * C::QS;
-                    *reinterpret_cast<uint2 *>(at0 + 2 * d0) = make_uint2(f16x2(x[0], x[1]), f16x2(x[2], x[3]));
-                    *reinterpret_cast<uint2 *>(at0 + 2 * d1) = make_uint2(f16x2(y[0], y[1]), f16x2(y[2], y[3]));
+#pragma unroll
+                    for (int t = 0; t < TT; t++) {
+                        const int n = t * R + row;
+                        uint8_t *col = dst + (n >> 3) * (8 * HD) + (n & 7) * 16;
+                        const uint32_t x0 = e4m3x2(x[r][0], x[r][1]), x1 = e4m3x2(x[r][2], x[r][3]);
+                        const uint32_t y0 = e4m3x2(y[r][0], y[r][1]), y1 = e4m3x2(y[r][2], y[r][3]);
+                        *reinterpret_cast<uint32_t *>(col + (d0 >> 4) * 128 + (d0 & 15)) = x0 | (x1 << 16);
+                        *reinterpret_cast<uint32_t *>(col + (d1 >> 4) * 128 + (d1 & 15)) = y0 | (y1 << 16);
+                        if (t + 1 < TT) {   // what is left, on the next term's scale
+                            const float2 p0 = e4m3x2_f32(x0), p1 = e4m3x2_f32(x1), p2 = e4m3x2_f32(y0), p3 = e4m3x2_f32(y1);
+                            x[r][0] = (x[r][0] - p0.x) * STEP, x[r][1] = (x[r][1] - p0.y) * STEP;
+                            x[r][2] = (x[r][2] - p1.x) * STEP, x[r][3] = (x[r][3] - p1.y) * STEP;
+                            y[r][0] = (y[r][0] - p2.x) * STEP, y[r][1] = (y[r][1] - p2.y) * STEP;
+                            y[r][2] = (y[r][2] - p3.x) * STEP, y[r][3] = (y[r][3] - p3.y) * STEP;
+                        }
+                    }
                 }
             }
-            if (lane == 0) {
-                qf[r] = up * a.scale;
-                qpos[r] = real ? pos : -1;
-            }
+            if (tid == 64) q_up[qi & 3] = up * a.scale;
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full + qb);
+            bar_sync(3, Q_WARPS * 32);   // amax_s is free again
+            qi++;
         }
-        __syncthreads();
-
-        // a lane's columns 2t, 2t + 1 of each n-tile are these rows (pairs: hi and lo lanes share them)
-        float fac[NT][2];
-        int cpos[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int r = nt * (R / NT) + (TERMS == 2 ? 2 * (t & 1) + e : 2 * t + e);
-                fac[nt][e] = qf[r];
-                cpos[nt][e] = qpos[r];
+    } else {   // ------------------------------------------------------ softmax, outputs
+        const int sg = (warp - 2 - Q_WARPS) >> 2, q4 = warp & 3;   // warpgroup; the warp's lane quarter
+        const int key = 32 * q4 + lane, bid = 1 + sg;
+        const uint32_t lane_at = (uint32_t)(32 * q4) << 16;
+        // byte of this key in a column of P: values lie in the order of paged.cuh
+        const int kbyte = (key >> 4) * 128 + place(key & 15);
+        constexpr int RG = C::RG, CH = C::CH, LC = C::LC, LD = C::LD, TS = C::TS;
+        float *mr = mref[sg];
+        uint32_t i = 0, qi = 0;
+        while (walk_next(a, pre, R, w, g)) {
+            const int k0 = g.k0, k1 = g.nblk > 0 ? g.k1 : k0, nblk = g.nblk, start = g.start;
+            const int p_lo = g.p_lo, p_hi = g.p_hi, see0 = g.see0, window = a.window;
+            const int row = sg * RG + key, c = g.c0 + row;   // the row that this thread keeps the books of
+            const bool mine = key < RG && c <= g.c1;
+            float sig = 1.0f;
+            if (key < RG) {
+                const int tok = c / a.group, hq = g.kvh * a.group + c % a.group;
+                mr[key] = 0.f;
+                pos_s[row] = mine ? g.pos0 + tok : -1;
+                out_s[row] = (size_t)(g.r0 + tok) * a.ldout + (size_t)hq * HD;
+                if (a.gate && mine) sig = to_f32(((const T *)a.gate)[(size_t)(g.r0 + tok) * a.ldgate + hq]);
             }
-        uint32_t qb[NT == 1 ? KT : 1][2];
-        if constexpr (NT == 1)
+            float l[RG];
 #pragma unroll
-            for (int c = 0; c < KT; c++) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(qs + (size_t)g * C::QS + 32 * c + 8 * t);
-                qb[c][0] = w.x;
-                qb[c][1] = w.y;
-            }
-        float o[NT][KT][4], m[NT][2], l[NT][2];
+            for (int r = 0; r < RG; r++) l[r] = 0.f;
+            bar_sync(bid, 128);
+            for (int k = k0; k < k1; k++, i++) {
+                const int st = i % NST, nb = min(TB, nblk - k * TB);
+                wait_for(full_k + st, (i / NST) & 1, &dead, a.err);   // the scales
+                const float2 sc = scales[st][key >> 4];
+                const float fb = log2f(sc.y), isv = 1.0f / sc.y;
+                wait_for(s_full + (i & 1), (i >> 1) & 1, &dead, a.err);
+                __syncwarp();
+                tc_after();
+                const int j0 = start + k * TILE, j = j0 + key;
+                const float fa = sc.x * q_up[qi & 3];
+                const bool edge = j0 + TILE - 1 > p_lo || (window > 0 && j0 <= p_hi - window);
+                float t[RG];         // s' - m
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
+                for (int ch = 0; ch < C::NC; ch++) {
+                    float v[LC];
 #pragma unroll
-            for (int c = 0; c < KT; c++) o[nt][c][0] = o[nt][c][1] = o[nt][c][2] = o[nt][c][3] = 0.f;
-            m[nt][0] = m[nt][1] = M_NONE;
-            l[nt][0] = l[nt][1] = 0.f;
-        }
-
-        for (int i = 0; i < cnt; i++) {
-            const uint32_t use = used + i;
-            const int slot = use % C::NS;
-            const bool here = mbar_wait(&bars[warp][slot], (use / C::NS) & 1, a.err);
-            if (here) {
-                const uint8_t *kb = ring + ((size_t)warp * C::NS + slot) * C::STAGE, *vb = kb + C::KB;
-                const float4 mt = meta[warp][slot];
-                float sc[NT][2][4];
+                    for (int x = 0; x < LC / LD; x++)
+                        tm_ld<LD>(tmem + lane_at + (i & 1) * N + C::col(sg, ch, x), v + LD * x);
+                    tm_wait(v);
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                    for (int r = 0; r < CH; r++) {
+                        float u = v[(TT - 1) * TS + r];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) sc[nt][h][0] = sc[nt][h][1] = sc[nt][h][2] = sc[nt][h][3] = 0.f;
-                const uint8_t *ka = kb + g * 16 + 4 * t;
-#pragma unroll
-                for (int c = 0; c < KT; c++) {
-                    uint32_t a0, a1, a2, a3;
-                    e4m3x4_f16(*reinterpret_cast<const uint32_t *>(ka + c * 128), a0, a2);
-                    e4m3x4_f16(*reinterpret_cast<const uint32_t *>(ka + 8 * HD + c * 128), a1, a3);
-                    if constexpr (NT == 1) {
-                        mma16816(sc[0][c & 1], a0, a1, a2, a3, qb[c][0], qb[c][1]);
-                    } else {
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            const uint2 w =
-                                *reinterpret_cast<const uint2 *>(qs + (size_t)(nt * 8 + g) * C::QS + 32 * c + 8 * t);
-                            mma16816(sc[nt][c & 1], a0, a1, a2, a3, w.x, w.y);
-                        }
+                        for (int x = TT - 2; x >= 0; x--) u = fmaf(u, 1.0f / STEP, v[x * TS + r]);
+                        t[ch * CH + r] = fmaf(u, fa, fb);
                     }
                 }
-                const int j0 = (bfirst + i * AT_WARPS) * BLOCK;
-                // bytes of this lane's 4 value tokens that some row sees: a masked place never meets the product
-                uint32_t vmask = 0xffffffffu;
-                if (j0 + BLOCK - 1 > p_hi || j0 < see0) {
-                    vmask = 0;
+                if (edge) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int j = j0 + order(4 * t + e);
-                        if (j <= p_hi && j >= see0) vmask |= 0xffu << (8 * e);
+                    for (int r = 0; r < RG; r++) {
+                        const int p = pos_s[sg * RG + r];
+                        if (j > p || (window > 0 && j <= p - window)) t[r] = -INFINITY;
                     }
                 }
-                const bool edge = j0 + BLOCK - 1 > p_lo || (a.window > 0 && j0 <= p_hi - a.window);
-                uint32_t pb[NT][2];
+                uint32_t over = 0;   // chunks with a weight past 2^W_MAX
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    float sv[4];
+                for (int ch = 0; ch < C::NC; ch++) {
+                    float mx = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float x = sc[nt][0][e] + sc[nt][1][e];
-                        if (TERMS == 2) x += __shfl_xor_sync(0xffffffffu, x, 2);
-                        x = fmaf(x, mt.x * fac[nt][e & 1], mt.y);
-                        if (edge) {
-                            const int j = j0 + g + 8 * (e >> 1), p = cpos[nt][e & 1];
-                            if (j > p || (a.window > 0 && j <= p - a.window)) x = -INFINITY;
-                        }
-                        sv[e] = x;
+                    for (int r = 0; r < CH; r++) {
+                        t[ch * CH + r] -= mr[ch * CH + r];
+                        mx = fmaxf(mx, t[ch * CH + r]);
                     }
-                    const bool over = fmaxf(sv[0], sv[2]) > m[nt][0] + M_SLACK || fmaxf(sv[1], sv[3]) > m[nt][1] + M_SLACK;
-                    if (__any_sync(0xffffffffu, over)) {
-                        float mx[2] = {fmaxf(sv[0], sv[2]), fmaxf(sv[1], sv[3])};
+                    over |= mx > W_MAX ? 1u << ch : 0u;
+                }
+                // the first tile sets the references (a row sees its earliest token there or in none of the
+                // CTA's tiles); the answer is the same for the whole warpgroup
+                const bool first = k == k0;
+                if (bar_or(bid, 128, first || over != 0)) {
+                    over = first ? (1u << C::NC) - 1u : __reduce_or_sync(0xffffffffu, over);
+                    if (lane == 0) moved[sg][q4] = over;
 #pragma unroll
-                        for (int of = 4; of < 32; of <<= 1) {
-                            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], of));
-                            mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], of));
+                    for (int ch = 0; ch < C::NC; ch++)
+                        if (over >> ch & 1u)   // the warp's largest; a chunk that only another warp flags moves with its own
+#pragma unroll
+                            for (int r = 0; r < CH; r++) {
+                                const float x = warp_max(t[ch * CH + r]);
+                                if (lane == 0) red[sg][q4][ch * CH + r] = x;
+                            }
+                        else if (lane == 0)
+#pragma unroll
+                            for (int r = 0; r < CH; r++) red[sg][q4][ch * CH + r] = -INFINITY;
+                    bar_sync(bid, 128);
+                    over = moved[sg][0] | moved[sg][1] | moved[sg][2] | moved[sg][3];
+                    if (key < RG) {   // to W_TOP below the largest
+                        const float x = fmaxf(fmaxf(red[sg][0][key], red[sg][1][key]), fmaxf(red[sg][2][key], red[sg][3][key]));
+                        const float up = !first ? (x > W_MAX ? x - W_TOP : 0.f) : x == -INFINITY ? 0.f : x - W_TOP;
+                        fs[sg][key] = up;
+                        mr[key] += up;
+                    }
+                    bar_sync(bid, 128);
+#pragma unroll
+                    for (int r = 0; r < RG; r++) {
+                        const float up = fs[sg][r];
+                        t[r] -= up;
+                        if (!first) l[r] *= ex2(-up);
+                    }
+                    if (!first) {   // what is summed so far moves too, once its MMAs are done
+                        wait_for(pv_done + ((i - 1) & 1), ((i - 1) >> 1) & 1, &dead, a.err);
+                        __syncwarp();
+                        tc_after();
+#pragma unroll 1
+                        for (int ch = 0; ch < C::NC; ch++) {
+                            if (!(over >> ch & 1u)) continue;
+#pragma unroll 1
+                            for (int h = 0; h < C::HH; h++) {
+                                float v[LC];
+#pragma unroll
+                                for (int x = 0; x < LC / LD; x++)
+                                    tm_ld<LD>(tmem + lane_at + (2 + h) * N + C::col(sg, ch, x), v + LD * x);
+                                tm_wait(v);
+#pragma unroll
+                                for (int r = 0; r < TS; r++) {
+                                    const float f = ex2(-fs[sg][ch * CH + r]);
+#pragma unroll
+                                    for (int x = r; x < LC; x += TS) v[x] *= f;
+                                }
+#pragma unroll
+                                for (int x = 0; x < LC / LD; x++)
+                                    tm_st<LD>(tmem + lane_at + (2 + h) * N + C::col(sg, ch, x), v + LD * x);
+                            }
                         }
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
+                }
+                if (i >= 2) wait_for(pv_done + (i & 1), ((i - 2) >> 1) & 1, &dead, a.err);   // P's buffer is free
+                uint8_t *pb = ps + (size_t)(i & 1) * N * TILE + kbyte;
 #pragma unroll
+                for (int r = 0; r < RG; r += 2) {
+                    float x[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        if (r + e < RG) {
+                            x[e] = ex2(t[r + e]);
+                            if (!edge || t[r + e] != -INFINITY) l[r + e] = fmaf(x[e], isv, l[r + e]);
+                        }
+                    uint32_t b[TT];
+                    split<TT>(x[0], x[1], b);
+#pragma unroll
+                    for (int tt = 0; tt < TT; tt++) {
+                        const int n = tt * R + sg * RG + r;
+                        pb[(n >> 3) * 1024 + (n & 7) * 16] = (uint8_t)b[tt];
+                        if (r + 1 < RG) pb[((n + 1) >> 3) * 1024 + ((n + 1) & 7) * 16] = (uint8_t)(b[tt] >> 8);
+                    }
+                }
+                // values of tokens that no row sees, in a block that some are seen of: a masked place
+                // never meets the product
+                const int past = j0 + nb * BLOCK - 1 - p_hi, under = see0 - j0;
+                if (past > 0 || under > 0) {
+                    wait_for(full_v + st, (i / NST) & 1, &dead, a.err);
+                    if (sg == 0) {
+                        uint8_t *vb = smem + (size_t)st * C::STAGE + TB * C::KB;
+#pragma unroll 1
                         for (int e = 0; e < 2; e++) {
-                            const float nm = fmaxf(m[nt][e], mx[e]), f = ex2(m[nt][e] - nm);
-                            m[nt][e] = nm;
-                            l[nt][e] *= f;
+                            const int bad = e == 0 ? under : past, blk = e == 0 ? 0 : nb - 1;
+                            if (bad <= 0) continue;
+                            uint32_t keep[4];
 #pragma unroll
-                            for (int c = 0; c < KT; c++) {
-                                o[nt][c][e] *= f;
-                                o[nt][c][2 + e] *= f;
+                            for (int x = 0; x < 4; x++) {
+                                keep[x] = 0;
+#pragma unroll
+                                for (int y = 0; y < 4; y++)
+                                    if (e == 0 ? order(4 * x + y) >= bad : order(4 * x + y) < BLOCK - bad)
+                                        keep[x] |= 0xffu << (8 * y);
+                            }
+#pragma unroll 1
+                            for (int d = key; d < HD; d += 128) {
+                                uint4 *at = reinterpret_cast<uint4 *>(vb + blk * C::KB + 16 * d);
+                                uint4 u = *at;
+                                u.x &= keep[0], u.y &= keep[1], u.z &= keep[2], u.w &= keep[3];
+                                *at = u;
                             }
                         }
                     }
-                    float p[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        p[e] = ex2(sv[e] - m[nt][e & 1] + P_SHIFT);
-                        l[nt][e & 1] = fmaf(p[e], mt.z, l[nt][e & 1]);
-                    }
-                    if (TERMS == 2 && t >= 2) {   // the lo columns
-#pragma unroll
-                        for (int e = 0; e < 4; e++) p[e] -= __half2float(__float2half_rn(p[e]));
-                    }
-                    pb[nt][0] = movm(f16x2(p[0], p[1]));
-                    pb[nt][1] = movm(f16x2(p[2], p[3]));
                 }
-                const uint8_t *va = vb + g * 16 + 4 * t;
-#pragma unroll
-                for (int c = 0; c < KT; c++) {
-                    uint32_t a0, a1, a2, a3;
-                    e4m3x4_f16(*reinterpret_cast<const uint32_t *>(va + c * 256) & vmask, a0, a2);
-                    e4m3x4_f16(*reinterpret_cast<const uint32_t *>(va + c * 256 + 128) & vmask, a1, a3);
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma16816(o[nt][c], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-                }
+                fence_proxy_async();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + (i & 1));
             }
-            if (i + C::NS < cnt) issue(i + C::NS);
-        }
-        used += cnt;
+            if (k1 > k0) qi++;
 
-        // the warps' (O, m, l) into the tile's
+            // the rows' sums over the keys, and the factor of a row's outputs
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                float v = l[nt][e];
-#pragma unroll
-                for (int of = 4; of < 32; of <<= 1) v += __shfl_xor_sync(0xffffffffu, v, of);
-                l[nt][e] = v;
-                const int r = nt * C::OR + (TERMS == 2 ? 2 * (t & 1) + e : 2 * t + e);
-                if (g == 0 && (TERMS == 1 || t < 2)) {
-                    wm[warp][r] = m[nt][e];
-                    wl[warp][r] = v;
+            for (int r = 0; r < RG; r++) {
+                const float x = warp_sum(l[r]);
+                if (lane == 0) red[sg][q4][r] = x;
+            }
+            bar_sync(bid, 128);
+            const bool whole = g.f0 == g.f1;
+            float *slot = a.part + ((size_t)blockIdx.x * 2 + (g.k0 == 0 ? 1 : 0)) * C::PART;
+            sig = a.gate ? 1.0f + __expf(-sig) : 1.0f;   // 1 / sigmoid
+            if (key < RG) {
+                const float L = (red[sg][0][key] + red[sg][1][key]) + (red[sg][2][key] + red[sg][3][key]);
+                // a row (or part) that saw nothing: its products are 0 or were not made
+                fs[sg][key] = L == 0.f ? 0.f : whole ? 1.0f / (L * sig) : 1.0f;
+                if (!whole && mine) {
+                    slot[R * HD + row] = L == 0.f ? M_NONE : mr[key];
+                    slot[R * HD + R + row] = L;
                 }
             }
-        __syncthreads();
-        const bool whole = b0 == 0 && b1 == q.nblk;
-        float *slot = a.part + ((size_t)blockIdx.x * 2 + (b0 == 0 ? 1 : 0)) * C::PART;
-        if (!whole && tid < R) {
-            float M = M_NONE, L = 0.f;
-            for (int w = 0; w < AT_WARPS; w++) M = fmaxf(M, wm[w][tid]);
-            for (int w = 0; w < AT_WARPS; w++) L = fmaf(wl[w][tid], ex2(wm[w][tid] - M), L);
-            slot[R * HD + tid] = M;
-            slot[R * HD + R + tid] = L;
-        }
+            bar_sync(bid, 128);
+            if (k1 > k0) wait_for(pv_done + ((i - 1) & 1), ((i - 1) >> 1) & 1, &dead, a.err);
+            __syncwarp();
+            tc_after();
+            const int rows = g.c1 - g.c0 + 1;
+#pragma unroll 1
+            for (int x0 = 0; x0 < C::HH * C::NC; x0++) {
+                const int h = x0 / C::NC, ch = x0 - h * C::NC, d = 128 * h + key;
+                float v[LC];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
+                for (int x = 0; x < LC / LD; x++)
+                    tm_ld<LD>(tmem + lane_at + (2 + h) * N + C::col(sg, ch, x), v + LD * x);
+                tm_wait(v);
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int rr = TERMS == 2 ? 2 * (t & 1) + e : 2 * t + e, r = nt * C::OR + rr;
-                float M = M_NONE;
+                for (int r = 0; r < CH; r++) {
+                    float o = v[(TT - 1) * TS + r];
 #pragma unroll
-                for (int w = 0; w < AT_WARPS; w++) M = fmaxf(M, wm[w][r]);
-                const float f = ex2(m[nt][e] - M);
-                float *dst = merge + ((size_t)warp * C::OR + rr) * HD;
-#pragma unroll
-                for (int c = 0; c < KT; c++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        float v = o[nt][c][2 * h + e] * f;
-                        if (TERMS == 2) v += __shfl_xor_sync(0xffffffffu, v, 2);   // hi + lo columns
-                        if (TERMS == 1 || t < 2) dst[16 * c + 8 * h + g] = v;
-                    }
-            }
-            __syncthreads();
-            for (int i = tid; i < C::OR * HD; i += AT_THREADS) {
-                float v = 0.f;
-#pragma unroll
-                for (int w = 0; w < AT_WARPS; w++) v += merge[(size_t)w * C::OR * HD + i];
-                const int rr = i / HD, d = i - rr * HD, r = nt * C::OR + rr;
-                if (whole) {
-                    const int c = c0 + r;
-                    if (c <= c1) {
-                        float M = M_NONE, L = 0.f;
-#pragma unroll
-                        for (int w = 0; w < AT_WARPS; w++) M = fmaxf(M, wm[w][r]);
-#pragma unroll
-                        for (int w = 0; w < AT_WARPS; w++) L = fmaf(wl[w][r], ex2(wm[w][r] - M), L);
-                        v = L == 0.f ? 0.f : v / L;
-                        const int row = q.r0 + c / a.group, h = kvh * a.group + c % a.group;
-                        if (a.gate) v /= 1.0f + __expf(-to_f32(((const T *)a.gate)[(size_t)row * a.ldgate + h]));
-                        ((T *)a.out)[(size_t)row * a.ldout + (size_t)h * HD + d] = from_f32<T>(v);
-                    }
-                } else {
-                    slot[(size_t)r * HD + d] = v;
+                    for (int x = TT - 2; x >= 0; x--) o = fmaf(o, 1.0f / STEP, v[x * TS + r]);
+                    const int rr = ch * CH + r, ro = sg * RG + rr;
+                    const float f = fs[sg][rr];
+                    if (d >= HD || ro >= rows) continue;
+                    o = f == 0.f ? 0.f : o * f;
+                    if (whole) ((T *)a.out)[out_s[ro] + d] = from_f32<T>(o);
+                    else slot[(size_t)ro * HD + d] = o;
                 }
             }
-            __syncthreads();
-        }
-        if (!whole) {   // the last CTA of the group adds all parts in CTA order
-            const long long gs = u - b0, ge = gs + q.nblk;
-            const int f0 = (int)(gs / chunk), f1 = (int)((ge - 1) / chunk), parts = f1 - f0 + 1;
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) last_in = atomicAdd(a.tickets + f0, 1u) == (unsigned)(parts - 1);
-            __syncthreads();
-            if (last_in) {
+            if (!whole) {   // the last CTA of the group adds all parts in CTA order
+                const int parts = g.f1 - g.f0 + 1;
+                constexpr int ST = 128 * C::SG;
                 __threadfence();
-                const size_t step = (size_t)2 * C::PART;
-                const float *p0 = a.part + (size_t)f0 * step;   // CTA f0: slot 1, the others: slot 0
-                for (int i = tid; i < R * (HD / 4); i += AT_THREADS) {
-                    const int r = i / (HD / 4), d = 4 * (i - r * (HD / 4)), c = c0 + r;
-                    if (c > c1) continue;
-                    float M = M_NONE;
-                    for (int p = 0; p < parts; p++)
-                        M = fmaxf(M, __ldcg(p0 + p * step + (p == 0 ? C::PART : 0) + R * HD + r));
-                    float L = 0.f;
-                    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int p = 0; p < parts; p++) {
-                        const float *pp = p0 + p * step + (p == 0 ? C::PART : 0);
-                        const float f = ex2(__ldcg(pp + R * HD + r) - M);
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(pp + (size_t)r * HD + d));
-                        L = fmaf(__ldcg(pp + R * HD + R + r), f, L);
-                        O.x = fmaf(v.x, f, O.x);
-                        O.y = fmaf(v.y, f, O.y);
-                        O.z = fmaf(v.z, f, O.z);
-                        O.w = fmaf(v.w, f, O.w);
-                    }
-                    const int row = q.r0 + c / a.group, h = kvh * a.group + c % a.group;
-                    float f = L == 0.f ? 0.f : 1.0f / L;
-                    if (L == 0.f) O = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (a.gate) f /= 1.0f + __expf(-to_f32(((const T *)a.gate)[(size_t)row * a.ldgate + h]));
-                    T *dst = (T *)a.out + (size_t)row * a.ldout + (size_t)h * HD + d;
-                    dst[0] = from_f32<T>(O.x * f);
-                    dst[1] = from_f32<T>(O.y * f);
-                    dst[2] = from_f32<T>(O.z * f);
-                    dst[3] = from_f32<T>(O.w * f);
+                bar_sync(4, ST);
+                if (sg == 0 && key == 0) {
+                    const bool last = atomicAdd(a.tickets + g.f0, 1u) == (unsigned)(parts - 1);
+                    if (last) a.tickets[g.f0] = 0u;
+                    last_in = last;
                 }
-                if (tid == 0) a.tickets[f0] = 0u;
+                bar_sync(4, ST);
+                if (last_in) {
+                    __threadfence();
+                    const size_t step = (size_t)2 * C::PART;
+                    const float *p0 = a.part + (size_t)g.f0 * step;   // CTA f0: slot 1, the others: slot 0
+                    auto part = [&](int p) { return p0 + p * step + (p == 0 ? C::PART : 0); };
+                    // P is at rest: the parts' weights of a row, and their sums before
+                    float *wt = reinterpret_cast<float *>(ps), *wl = wt + N * TILE / 4;
+                    const int RB = min(R, N * TILE / 4 / parts);   // rows that fit (at least 2)
+                    for (int r0 = 0; r0 < rows; r0 += RB) {
+                        const int nr = min(RB, rows - r0);
+                        if (key < RG && row >= r0 && row < r0 + nr) red[sg][0][key] = sig;
+                        for (int x = sg * 128 + key; x < nr * parts; x += ST) {
+                            const int p = x / nr, r = x - p * nr;
+                            const float *pp = part(p) + R * HD + r0 + r;
+                            wt[r * parts + p] = __ldcg(pp);
+                            wl[r * parts + p] = __ldcg(pp + R);
+                        }
+                        bar_sync(4, ST);
+                        for (int r = sg * 4 + q4; r < nr; r += 4 * C::SG) {   // a warp per row
+                            float M = M_NONE, L = 0.f;
+                            for (int p = lane; p < parts; p += 32) M = fmaxf(M, wt[r * parts + p]);
+                            M = warp_max(M);
+                            for (int p = lane; p < parts; p += 32) {
+                                const float f = ex2(wt[r * parts + p] - M);
+                                wt[r * parts + p] = f;
+                                L = fmaf(wl[r * parts + p], f, L);
+                            }
+                            L = warp_sum(L);
+                            const float f = L == 0.f ? 0.f : 1.0f / (L * red[(r0 + r) / RG][0][(r0 + r) % RG]);
+                            for (int p = lane; p < parts; p += 32) wt[r * parts + p] *= f;
+                        }
+                        bar_sync(4, ST);
+                        const int items = nr * (HD / 4);
+                        for (int x = sg * 128 + key; x < items; x += ST) {
+                            const int r = x / (HD / 4), d = 4 * (x - r * (HD / 4));
+                            const size_t at = (size_t)(r0 + r) * HD + d;
+                            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+                            for (int pb = 0; pb < parts; pb += 8) {
+                                float4 v[8];
+#pragma unroll
+                                for (int p = 0; p < 8; p++)   // past the last part: the last one again, weight 0
+                                    v[p] = __ldcg(reinterpret_cast<const float4 *>(part(min(pb + p, parts - 1)) + at));
+#pragma unroll
+                                for (int p = 0; p < 8; p++) {
+                                    const float f = pb + p < parts ? wt[r * parts + pb + p] : 0.f;
+                                    O.x = fmaf(v[p].x, f, O.x);
+                                    O.y = fmaf(v[p].y, f, O.y);
+                                    O.z = fmaf(v[p].z, f, O.z);
+                                    O.w = fmaf(v[p].w, f, O.w);
+                                }
+                            }
+                            T *dst = (T *)a.out + out_s[r0 + r] + d;
+                            dst[0] = from_f32<T>(O.x);
+                            dst[1] = from_f32<T>(O.y);
+                            dst[2] = from_f32<T>(O.z);
+                            dst[3] = from_f32<T>(O.w);
+                        }
+                        bar_sync(4, ST);   // the weights and last_in are free again
+                    }
+                }
             }
-            __syncthreads();
+            tc_before();
+            bar_sync(bid, 128);   // the rows' books are free again
         }
-        u += b1 - b0;
+    }
+    tc_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::TCOLS));
     }
 }
 
 constexpr size_t TICKETS = 1024;   // bytes before the partials: one word per CTA (at most 256)
+constexpr int MAX_R = 64;
 
-template <typename T, int HD, int NT, int TERMS>
-cudaError_t launch_one(const AttnParams &a, cudaStream_t s) {
-    using C = Cfg<HD, NT, TERMS>;
+template <typename T, typename C>
+int launch_one(const AttnParams &a, cudaStream_t s, const char *who) {
+    // the line of work, at its longest: every row tile as long as the page table
+    const long long tiles = (long long)a.b.rows * a.group / C::R + a.b.nseq;
+    const long long blocks = (long long)a.b.max_pages * a.pool.page_tokens / BLOCK + SEG_COST + 3;
+    if ((double)tiles * blocks * a.pool.kv_heads > 2147483000.0)
+        return set_error("%s: %d rows over up to %d pages of %d tokens are too much for one call", who, a.b.rows,
+                         a.b.max_pages, a.pool.page_tokens);
     static bool set[64];
     int dev = 0;
     cudaGetDevice(&dev);
+    cudaError_t e = cudaSuccess;
     if (dev < 0 || dev >= 64 || !set[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_kernel<T, HD, NT, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)C::SMEM);
-        if (e != cudaSuccess) return e;
-        if (dev >= 0 && dev < 64) set[dev] = true;
+        e = cudaFuncSetAttribute(attn_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+        if (e == cudaSuccess && dev >= 0 && dev < 64) set[dev] = true;
     }
-    return launch_pdl(attn_kernel<T, HD, NT, TERMS>, dim3(sm_count()), dim3(AT_THREADS), C::SMEM, s, a);
+    if (e == cudaSuccess) e = launch_pdl(attn_kernel<T, C>, dim3(sm_count()), dim3(C::THREADS), C::SMEM, s, a);
+    return e == cudaSuccess ? 0 : cuda_fail(who, e);
 }
 
+// The columns follow the rows that a sequence has per KV head on average: the narrowest tile that
+// holds them, since a tile's cost grows with its columns and a second tile reads the cache again.
 template <typename T, int HD>
-cudaError_t launch(const AttnParams &a, cudaStream_t s) {
-    constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-    // two n-tiles when a sequence's rows of a KV head overfill one on average
-    const bool wide = (long long)a.b.rows * a.group > (long long)a.b.nseq * (8 / TERMS);
-    return wide ? launch_one<T, HD, 2, TERMS>(a, s) : launch_one<T, HD, 1, TERMS>(a, s);
+int launch(const AttnParams &a, cudaStream_t s, const char *who) {
+    const long long per = ((long long)a.b.rows * a.group + a.b.nseq - 1) / a.b.nseq;
+    if constexpr (sizeof(T) == 4) {
+        if (per <= 6) return launch_one<T, Cfg<HD, 32, 5, 6>>(a, s, who);
+        return launch_one<T, Cfg<HD, 128, 5, 24>>(a, s, who);
+    } else {
+        if (per <= 5) return launch_one<T, Cfg<HD, 16, 3, 5>>(a, s, who);
+        if (per <= 10) return launch_one<T, Cfg<HD, 32, 3, 10>>(a, s, who);
+        if constexpr (__is_same(T, __half)) return launch_one<T, Cfg<HD, 128, 3, 40>>(a, s, who);
+        else return launch_one<T, Cfg<HD, 128, 2, 64>>(a, s, who);
+    }
 }
 
 template <typename T>
-cudaError_t launch_hd(const AttnParams &a, cudaStream_t s) {
-    return a.pool.hd == 256 ? launch<T, 256>(a, s) : a.pool.hd == 128 ? launch<T, 128>(a, s) : launch<T, 64>(a, s);
+int launch_hd(const AttnParams &a, cudaStream_t s, const char *who) {
+    return a.pool.hd == 256   ? launch<T, 256>(a, s, who)
+           : a.pool.hd == 128 ? launch<T, 128>(a, s, who)
+                              : launch<T, 64>(a, s, who);
 }
 
 }  // namespace
 }  // namespace paged
 }  // namespace spk
-
 extern "C" {
 
 size_t spk_paged_attn_workspace_bytes(int head_dim) {
     using namespace spk::paged;
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
-    return TICKETS + (size_t)spk::sm_count() * 2 * 16 * (head_dim + 2) * sizeof(float);
+    return TICKETS + (size_t)spk::sm_count() * 2 * MAX_R * (head_dim + 2) * sizeof(float);
 }
 
 int spk_paged_attn(const spk_kv_pool *pool, const spk_kv_batch *batch, const spk_paged_attn_args *p, void *stream) {
@@ -637,10 +1044,9 @@ int spk_paged_attn(const spk_kv_pool *pool, const spk_kv_batch *batch, const spk
     a.part = (float *)((uint8_t *)p->workspace + TICKETS);
     a.err = device_error_ptr();
     const cudaStream_t s = (cudaStream_t)stream;
-    const cudaError_t e = p->type == T_F32   ? launch_hd<float>(a, s)
-                          : p->type == T_F16 ? launch_hd<__half>(a, s)
-                                             : launch_hd<__nv_bfloat16>(a, s);
-    return e == cudaSuccess ? 0 : cuda_fail(who, e);
+    return p->type == T_F32   ? launch_hd<float>(a, s, who)
+           : p->type == T_F16 ? launch_hd<__half>(a, s, who)
+                              : launch_hd<__nv_bfloat16>(a, s, who);
 }
 
 }  // extern "C"

@@ -57,13 +57,21 @@ def type_of(t) -> int:
     return n
 
 
-def stream_of(t, stream) -> int:
-    """The CUDA stream of a call on tensor t: the one given, else torch's current one."""
-    if stream is not None:
-        return stream.cuda_stream
-    import torch
+_cuda = None
 
-    return torch.cuda.current_stream(t.device).cuda_stream
+
+def stream_of(t, stream) -> int:
+    """The CUDA stream of a call on tensor t: the one given, else torch's current one. The library
+    launches on the current device, which has to be the tensor's."""
+    global _cuda
+    if _cuda is None:
+        import torch
+
+        _cuda = (torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)   # what torch.cuda's own calls wrap
+    i = t.get_device()
+    if _cuda[0]() != i:
+        raise SpkError(f"the rows lie on cuda:{i}, the current device is cuda:{_cuda[0]()}")
+    return stream.cuda_stream if stream is not None else _cuda[1](i)
 
 
 def rope_freq(theta: float, pdim: int, device="cuda"):
@@ -77,15 +85,16 @@ def rope_freq(theta: float, pdim: int, device="cuda"):
 
 def _rows(t, rows: int, width: int, what: str, like=None):
     """A row matrix [rows][width] whose last axis is dense: its row stride in elements."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+    if t.shape != (rows, width):
         raise SpkError(f"{what} is [{rows}, {width}]; got {list(t.shape)}")
-    if width > 1 and t.stride(1) != 1:
-        raise SpkError(f"{what}: the values of a row lie {t.stride(1)} apart")
+    ld, one = t.stride()
+    if one != 1 and width > 1:
+        raise SpkError(f"{what}: the values of a row lie {one} apart")
     if not t.is_cuda:
         raise SpkError("libspk takes device buffers; got a host tensor")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if like is not None and (t.dtype != like.dtype or t.get_device() != like.get_device()):
         raise SpkError(f"{what} is {t.dtype} on {t.device}, the other rows {like.dtype} on {like.device}")
-    return t.stride(0)
+    return ld
 
 
 class PagedCache:
