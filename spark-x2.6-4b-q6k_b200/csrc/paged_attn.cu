@@ -75,11 +75,13 @@ struct Cfg {
     static constexpr int KB = BLOCK * HD;                     // bytes of a block's keys (or values)
     static constexpr int STAGE = 2 * TB * KB;
     static constexpr int NST = N >= 128 ? (HD == 256 ? 2 : HD == 128 ? 4 : 6) : (HD == 256 ? 3 : HD == 128 ? 6 : 8);
-    static constexpr int QB = N >= 128 && HD == 256 ? 1 : 2;  // query buffers
+    // P: 16 keys of every column, then the next 16, 64 bytes further than they need so that the byte
+    // stores of a warp's two runs of 16 keys meet different banks. One buffer where two do not fit.
+    static constexpr int PK = N * 16 + 64, PB = TILE / 16 * PK, NP = N >= 128 && HD == 256 ? 1 : 2;
     static constexpr int HH = HD == 256 ? 2 : 1;              // 128-dim halves of the output
     static constexpr int TCOLS = (2 + HH) * N <= 64 ? 64 : (2 + HH) * N <= 128 ? 128 : (2 + HH) * N <= 256 ? 256 : 512;
-    static constexpr size_t Q_OFF = (size_t)NST * STAGE, P_OFF = Q_OFF + (size_t)QB * N * HD;
-    static constexpr size_t SMEM = P_OFF + (size_t)2 * N * TILE;
+    static constexpr size_t Q_OFF = (size_t)NST * STAGE, P_OFF = Q_OFF + (size_t)2 * N * HD;
+    static constexpr size_t SMEM = P_OFF + (size_t)NP * PB;
     static constexpr int WARPS = 2 + Q_WARPS + 4 * SG, THREADS = WARPS * 32;
     static constexpr int PART = (R * (HD + 2) + 3) / 4 * 4;   // floats of a partial: O, then m, then l; read 16 bytes at a time
     static_assert(T * R <= N && R % SG == 0 && RG % CH == 0, "");
@@ -274,23 +276,11 @@ struct Walk {
     int s, kvh, j;
     Seq q;
 };
-__device__ __noinline__ void walk_begin(const AttnParams &a, const uint32_t *pre, int R, Walk &w) {
-    const uint32_t total = pre[a.b.nseq];
-    w.chunk = max((total + gridDim.x - 1) / gridDim.x, (uint32_t)TB);
-    w.x0 = w.chunk * blockIdx.x;
-    w.x1 = min(total, w.x0 + w.chunk);
-    w.s = w.kvh = w.j = 0;
-    w.base = w.x1;
-    if (w.x0 >= w.x1) return;
-    int lo = 0, hi = a.b.nseq;        // the last sequence with pre <= x0: it is not empty
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (pre[mid] <= w.x0) lo = mid;
-        else hi = mid;
-    }
-    w.s = lo;
-    w.q = seq_of(a, lo, R);
-    const uint32_t per = before(w.q, w.q.tiles), in = w.x0 - pre[lo];
+// The group of sequence s that holds the start of the CTA's range.
+__device__ __forceinline__ void walk_at(const AttnParams &a, const uint32_t *pre, int s, int R, Walk &w) {
+    w.s = s;
+    w.q = seq_of(a, s, R);
+    const uint32_t per = before(w.q, w.q.tiles), in = w.x0 - pre[s];
     w.kvh = in / per;
     const uint32_t rem = in - w.kvh * per;
     int a0 = 0, a1 = w.q.tiles;       // the last group with before <= rem
@@ -300,7 +290,7 @@ __device__ __noinline__ void walk_begin(const AttnParams &a, const uint32_t *pre
         else a1 = mid;
     }
     w.j = a0;
-    w.base = pre[lo] + w.kvh * per + before(w.q, a0);
+    w.base = pre[s] + w.kvh * per + before(w.q, a0);
 }
 // The next group of which this CTA has tiles.
 __device__ __noinline__ bool walk_next(const AttnParams &a, const uint32_t *pre, int R, Walk &w, Seg &g) {
@@ -334,7 +324,7 @@ __device__ __noinline__ bool walk_next(const AttnParams &a, const uint32_t *pre,
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a) {
-    constexpr int HD = C::HD, N = C::N, TT = C::T, R = C::R, NST = C::NST, QB = C::QB;
+    constexpr int HD = C::HD, N = C::N, TT = C::T, R = C::R, NST = C::NST, QB = 2, NP = C::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ uint64_t full_k[NST], full_v[NST], empty[NST], s_full[2], p_full[2], pv_done[2], q_full[QB], q_empty[QB];
     __shared__ float2 scales[NST][TB];                  // dk, dv of a tile's blocks
@@ -350,6 +340,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     __shared__ float amax_s[Q_WARPS];
     __shared__ int last_in;
     __shared__ uint32_t tmem_s;
+    __shared__ Walk walk_s;                             // the walk behind the CTA's first group
+    __shared__ Seg first_s;
+    __shared__ bool some;
     uint8_t *qs = smem + C::Q_OFF, *ps = smem + C::P_OFF;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -369,6 +362,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             mbar_init(q_empty + i, 1);
         }
         dead = 0;
+        some = false;
         fence_mbar_init();
     }
     if (warp == 1) {   // this warp owns the tensor memory
@@ -413,15 +407,30 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     if (tid == 0) pre[a.b.nseq] = base;
     __syncthreads();
 
-    Walk w;
-    Seg g;
-    walk_begin(a, pre, R, w);
-    if (w.x0 >= w.x1) {
+    // the CTA's range; the thread of the sequence where it starts finds its first group for all
+    const uint32_t chunk = max((base + gridDim.x - 1) / gridDim.x, (uint32_t)TB), x0 = chunk * blockIdx.x;
+    for (int s = tid; s < a.b.nseq; s += C::THREADS)
+        if (pre[s] <= x0 && x0 < pre[s + 1]) {
+            Walk w;
+            w.chunk = chunk;
+            w.x0 = x0;
+            w.x1 = min(base, x0 + chunk);
+            walk_at(a, pre, s, R, w);
+            Seg g;
+            some = walk_next(a, pre, R, w, g);
+            walk_s = w;
+            first_s = g;
+        }
+    __syncthreads();
+    Walk w = walk_s;
+    Seg g = first_s;
+    bool more = some;
+    if (!more) {
     } else if (warp == 0) {   // ------------------------------------------------------ copies
         // lane l < 8: the keys and values of a tile's block l; its page comes one tile ahead
         const int per = a.pool.page_tokens / BLOCK;
         uint32_t i = 0;
-        while (walk_next(a, pre, R, w, g)) {
+        for (; more; more = walk_next(a, pre, R, w, g)) {
             const int blk0 = g.start / BLOCK, nblk = g.nblk, k1 = g.k1, kvh = g.kvh;
             const int *table = a.b.table + (size_t)g.s * a.b.max_pages;
             auto page_of = [&](int k) {
@@ -480,7 +489,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             const uint64_t kdesc = smem_desc(smem_u32(smem), 128, 8 * HD);
             const uint64_t qdesc = smem_desc(smem_u32(qs), 128, 8 * HD);
             const uint64_t vdesc = smem_desc(smem_u32(smem) + TB * C::KB, C::KB, 128);
-            const uint64_t pdesc = smem_desc(smem_u32(ps), 128, 1024);
+            const uint64_t pdesc = smem_desc(smem_u32(ps), C::PK, 128);
             uint32_t i = 0, qi = 0;   // tiles whose scores were issued; groups
             // the tile whose values come next: its place, blocks, and whether it is its group's first
             bool have = false, pfirst = false;
@@ -492,18 +501,18 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     !wait_for(full_v + st, (pi / NST) & 1, &dead, a.err))
                     return;
                 tc_after();
-                const uint64_t vd = vdesc + (uint32_t)(st * (C::STAGE / 16)), pd = pdesc + (uint32_t)((pi & 1) * (N * TILE / 16));
+                const uint64_t vd = vdesc + (uint32_t)(st * (C::STAGE / 16)), pd = pdesc + (uint32_t)((pi % NP) * (C::PB / 16));
 #pragma unroll
                 for (int kk = 0; kk < TB / 2; kk++)
                     if (2 * kk < pnb)
 #pragma unroll
                         for (int h = 0; h < C::HH; h++)
-                            mma_e4m3(oo + h * N, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * 16, idesc,
+                            mma_e4m3(oo + h * N, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * (2 * C::PK / 16), idesc,
                                      !pfirst || kk > 0);
                 mma_commit(pv_done + (pi & 1));
                 mma_commit(empty + st);
             };
-            while (walk_next(a, pre, R, w, g)) {
+            for (; more; more = walk_next(a, pre, R, w, g)) {
                 if (g.nblk == 0) continue;
                 const int qb = qi % QB, k0 = g.k0, k1 = g.k1, nblk = g.nblk;
                 const bool q_here = wait_for(q_full + qb, (qi / QB) & 1, &dead, a.err);
@@ -533,7 +542,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     } else if (warp < 2 + Q_WARPS) {   // ------------------------------------------------- queries
         const int qw = warp - 2;
         uint32_t qi = 0;
-        while (walk_next(a, pre, R, w, g)) {
+        for (; more; more = walk_next(a, pre, R, w, g)) {
             if (g.nblk == 0) continue;
             const int qb = qi % QB, c0 = g.c0, c1 = g.c1, pos0 = g.pos0;
             const T *q0 = (const T *)a.q + (size_t)g.r0 * a.ldq + (size_t)g.kvh * a.group * HD;
@@ -633,11 +642,11 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
         const int key = 32 * q4 + lane, bid = 1 + sg;
         const uint32_t lane_at = (uint32_t)(32 * q4) << 16;
         // byte of this key in a column of P: values lie in the order of paged.cuh
-        const int kbyte = (key >> 4) * 128 + place(key & 15);
+        const int kbyte = (key >> 4) * C::PK + place(key & 15);
         constexpr int RG = C::RG, CH = C::CH, LC = C::LC, LD = C::LD, TS = C::TS;
         float *mr = mref[sg];
         uint32_t i = 0, qi = 0;
-        while (walk_next(a, pre, R, w, g)) {
+        for (; more; more = walk_next(a, pre, R, w, g)) {
             const int k0 = g.k0, k1 = g.nblk > 0 ? g.k1 : k0, nblk = g.nblk, start = g.start;
             const int p_lo = g.p_lo, p_hi = g.p_hi, see0 = g.see0, window = a.window;
             const int row = sg * RG + key, c = g.c0 + row;   // the row that this thread keeps the books of
@@ -759,8 +768,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
                 }
-                if (i >= 2) wait_for(pv_done + (i & 1), ((i - 2) >> 1) & 1, &dead, a.err);   // P's buffer is free
-                uint8_t *pb = ps + (size_t)(i & 1) * N * TILE + kbyte;
+                if (i >= NP) wait_for(pv_done + ((i - NP) & 1), ((i - NP) >> 1) & 1, &dead, a.err);   // P's buffer is free
+                uint8_t *pb = ps + (size_t)(i % NP) * C::PB + kbyte;
 #pragma unroll
                 for (int r = 0; r < RG; r += 2) {
                     float x[2] = {0.f, 0.f};
@@ -775,8 +784,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
 #pragma unroll
                     for (int tt = 0; tt < TT; tt++) {
                         const int n = tt * R + sg * RG + r;
-                        pb[(n >> 3) * 1024 + (n & 7) * 16] = (uint8_t)b[tt];
-                        if (r + 1 < RG) pb[((n + 1) >> 3) * 1024 + ((n + 1) & 7) * 16] = (uint8_t)(b[tt] >> 8);
+                        pb[n * 16] = (uint8_t)b[tt];
+                        if (r + 1 < RG) pb[(n + 1) * 16] = (uint8_t)(b[tt] >> 8);
                     }
                 }
                 // values of tokens that no row sees, in a block that some are seen of: a masked place
@@ -864,22 +873,23 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             if (!whole) {   // the last CTA of the group adds all parts in CTA order
                 const int parts = g.f1 - g.f0 + 1;
                 constexpr int ST = 128 * C::SG;
-                __threadfence();
                 bar_sync(4, ST);
                 if (sg == 0 && key == 0) {
+                    __threadfence();   // for all of them: their stores came before the barrier
                     const bool last = atomicAdd(a.tickets + g.f0, 1u) == (unsigned)(parts - 1);
                     if (last) a.tickets[g.f0] = 0u;
+                    __threadfence();
                     last_in = last;
                 }
                 bar_sync(4, ST);
                 if (last_in) {
-                    __threadfence();
                     const size_t step = (size_t)2 * C::PART;
                     const float *p0 = a.part + (size_t)g.f0 * step;   // CTA f0: slot 1, the others: slot 0
                     auto part = [&](int p) { return p0 + p * step + (p == 0 ? C::PART : 0); };
                     // P is at rest: the parts' weights of a row, and their sums before
-                    float *wt = reinterpret_cast<float *>(ps), *wl = wt + N * TILE / 4;
-                    const int RB = min(R, N * TILE / 4 / parts);   // rows that fit (at least 2)
+                    constexpr int room = NP * C::PB / 8;
+                    float *wt = reinterpret_cast<float *>(ps), *wl = wt + room;
+                    const int RB = min(R, room / parts);   // rows that fit (at least 2)
                     for (int r0 = 0; r0 < rows; r0 += RB) {
                         const int nr = min(RB, rows - r0);
                         if (key < RG && row >= r0 && row < r0 + nr) red[sg][0][key] = sig;
