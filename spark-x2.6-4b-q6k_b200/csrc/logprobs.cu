@@ -8,12 +8,15 @@
 // row that holds a NaN or +inf, or only -inf, has no distribution: NaN for logp, H and the
 // alternatives' values (their indices stay those of the order, a NaN ranking as -inf).
 //
-// What bounds it: the row's bytes. A CTA streams a range of a row, 16 bytes a load, four loads a
-// thread in flight; each thread keeps its own (m, S, A) in f32 in base 2 and moves m when a vector
-// of values passes it. The best k (k <= 32) are a list sorted over a warp's lanes; a vector is
-// looked at again only if its largest value reaches the list's last, which few do. A row alone is cut
-// over many CTAs (rows x splits fill the SMs); the last one to arrive, by a ticket that it resets,
-// joins the parts in order.
+// What bounds it: the row's bytes, then the exponentials (16 a clock and SM: 30 us of the 42 us that
+// 1024 x 131072 bf16 values take to read). A CTA streams a range of a row, 16 bytes a load, four loads
+// a thread in flight; each thread keeps its own (m, S, A) in base 2, pairs of values by one f32x2
+// instruction, and moves m when a vector of values passes it. The best k (k <= 32) are a list over a
+// warp's lanes, as 64-bit keys (order of the value, then of the index). A vector is looked at again only
+// if its largest value reaches the best k-th value that any warp of the CTA has seen, which starts
+// at the k-th largest of a warp's lane maxima; lists join by half cleaners (5 exchanges). A row alone is
+// cut over many CTAs (rows x splits fill the SMs); the last one to arrive, by a ticket that it resets,
+// joins the parts.
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -22,11 +25,10 @@
 namespace spk {
 namespace {
 
-constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_TOP = 32;                 // the most alternatives
 constexpr int LP_SPLITS = 64;              // the most CTAs of a row
+constexpr int LP_PART = 4 + 2 * LP_TOP;    // floats of a part: m, S, A, then the keys
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr float FAR = -1e4f;               // 2^FAR is 0 and FAR * 0 too: where -inf ends in the sums
 constexpr float HUGE_M = 1e37f;            // references past it take the sums' slow form
 
 struct LpArgs {
@@ -39,7 +41,7 @@ struct LpArgs {
     int *ids;
     float *best;
     unsigned int *tickets;                 // [rows], zero at rest
-    float *part;                           // [rows][splits][4 + 2 * LP_TOP]
+    float *part;                           // [rows][splits][LP_PART]
     int *err;
 };
 
@@ -48,13 +50,28 @@ __device__ __forceinline__ float ex2f_(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ float max_nan_(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long pack2(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
     return r;
 }
 
-// (m, S, A) with values in base 2: t = (x - m) log2 e, S = sum 2^t, A = sum t 2^t
+// (m, S, A) in base 2: t = (x - m) log2 e, S = sum 2^t, A = sum t 2^t
 struct Stat {
     float m, s, a;
 };
@@ -72,69 +89,110 @@ __device__ __forceinline__ Stat join(Stat p, Stat q) {
     move(q, m);
     return Stat{m, p.s + q.s, p.a + q.a};
 }
-
-// lane i of the warp holds the i-th best (value, index); a candidate goes to its place
-__device__ __forceinline__ bool before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
-__device__ __forceinline__ void insert(float &lv, int &li, float v, int i, int lane) {
-    const bool mine = before(v, i, lv, li);
-    const float uv = __shfl_up_sync(0xffffffffu, lv, 1);
-    const int ui = __shfl_up_sync(0xffffffffu, li, 1);
-    const bool up = __shfl_up_sync(0xffffffffu, (int)mine, 1) && lane > 0;
-    if (mine) {
-        lv = up ? uv : v;
-        li = up ? ui : i;
-    }
+__device__ __forceinline__ Stat warp_join(Stat st) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        st = join(st, Stat{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
+                           __shfl_xor_sync(0xffffffffu, st.a, o)});
+    return st;
 }
-// offers each lane's candidate (ok) to the list; kth: the list's last place that counts
-__device__ __forceinline__ void offer(float &lv, int &li, float v, int i, bool ok, int kth, int lane) {
-    float tv = __shfl_sync(0xffffffffu, lv, kth);
-    int ti = __shfl_sync(0xffffffffu, li, kth);
-    unsigned left = __ballot_sync(0xffffffffu, ok && before(v, i, tv, ti));
+
+// Keys: larger is better; 0 is no token. The value's bits in order, then the index from the end.
+typedef unsigned long long Key;
+__device__ __forceinline__ uint32_t order_of(float x) {   // -0 as 0, NaN as -inf
+    const uint32_t b = __float_as_uint(fmaxf(x, -INFINITY) + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(Key k) {
+    const uint32_t o = (uint32_t)(k >> 32);
+    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ Key key_of(float x, int i) { return ((Key)order_of(x) << 32) | (0xffffffffu - (uint32_t)i); }
+__device__ __forceinline__ int index_of(Key k) { return (int)(0xffffffffu - (uint32_t)k); }
+
+__device__ __forceinline__ Key exchange(Key k, int o, bool large) {
+    const Key p = __shfl_xor_sync(0xffffffffu, k, o);
+    return (k > p) == large ? k : p;
+}
+__device__ __forceinline__ Key clean(Key k, int lane) {   // a bitonic sequence, descending
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) k = exchange(k, o, !(lane & o));
+    return k;
+}
+__device__ __forceinline__ Key sort32(Key k, int lane) {   // descending
+#pragma unroll
+    for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+        for (int o = n >> 1; o > 0; o >>= 1) k = exchange(k, o, !(lane & o) == !(lane & n));
+    return k;
+}
+// the best 32 of two descending lists; `rev`: the other one's key of lane 31 - lane
+__device__ __forceinline__ Key merge(Key k, Key rev, int lane) { return clean(k > rev ? k : rev, lane); }
+
+// Offers each lane's candidate (0: none) to the warp's list; kth: its last place that counts.
+__device__ __forceinline__ void offer(Key &list, Key cand, int kth, int lane) {
+    Key last = __shfl_sync(0xffffffffu, list, kth);
+    unsigned left = __ballot_sync(0xffffffffu, cand > last);
+    if (__popc(left) > 3) {
+        cand = sort32(cand, lane);
+        list = merge(list, __shfl_sync(0xffffffffu, cand, 31 - lane), lane);
+        return;
+    }
     while (left) {
-        const int src = __ffs(left) - 1;
-        insert(lv, li, __shfl_sync(0xffffffffu, v, src), __shfl_sync(0xffffffffu, i, src), lane);
-        tv = __shfl_sync(0xffffffffu, lv, kth);
-        ti = __shfl_sync(0xffffffffu, li, kth);
+        const Key c = __shfl_sync(0xffffffffu, cand, __ffs(left) - 1);
+        const bool mine = c > list;
+        const Key up = __shfl_up_sync(0xffffffffu, list, 1);
+        const bool shift = lane > 0 && c > up;
+        if (mine) list = shift ? up : c;
         left &= left - 1;
-        left &= __ballot_sync(0xffffffffu, ok && before(v, i, tv, ti));
     }
 }
 
 template <typename T>
-struct Vec {   // 16 bytes of T as f32
+struct Vec {   // 16 bytes of T
     static constexpr int N = 16 / sizeof(T);
-    static __device__ __forceinline__ void f32(uint4 w, float (&v)[N]) {
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (sizeof(T) == 4) {
-                v[i] = __uint_as_float(u[i]);
-            } else if constexpr (sizeof(T) == 2) {
-                if constexpr (__is_same(T, __half)) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
-                    v[2 * i] = f.x;
-                    v[2 * i + 1] = f.y;
-                } else {
-                    v[2 * i] = __uint_as_float(u[i] << 16);
-                    v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-                }
-            }
-        }
-    }
+    // sums take the fast form for references above this: -inf ends as FLOOR, far below all of them
+    static constexpr float LOW_M = __is_same(T, __half) ? -3e4f : -HUGE_M;
     static __device__ __forceinline__ float one(const T *p) {
         if constexpr (sizeof(T) == 4) return (float)*p;
         else if constexpr (__is_same(T, __half)) return __half2float(*p);
         else return __bfloat162float(*p);
     }
+    static __device__ __forceinline__ float2 two(uint32_t u) {   // of 16-bit types
+        if constexpr (__is_same(T, __half)) return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+        else return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    }
+    static __device__ __forceinline__ uint32_t max_(uint32_t a, uint32_t b) {   // of a pair (or of one f32), NaN is less
+        uint32_t r;
+        if constexpr (sizeof(T) == 4) r = __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+        else if constexpr (__is_same(T, __half)) asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        else asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t floor_(uint32_t a) {   // -inf becomes a finite value, a NaN stays
+        uint32_t r;
+        if constexpr (sizeof(T) == 4) asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xff167699u));   // -2e38
+        else if constexpr (__is_same(T, __half)) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xfbfffbffu));
+        else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xff16ff16u));
+        return r;
+    }
+    static constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
+    static __device__ __forceinline__ float at(const uint32_t (&w)[4], int e) {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+        else {
+            const float2 f = two(w[e >> 1]);
+            return e & 1 ? f.y : f.x;
+        }
+    }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const LpArgs a) {
+template <typename T, int LP_THREADS>
+__global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel(const LpArgs a) {
     using V = Vec<T>;
-    constexpr int N = V::N, UN = 4;
-    __shared__ float ws[LP_WARPS][3];
-    __shared__ float wv[LP_WARPS][LP_TOP];
-    __shared__ int wi[LP_WARPS][LP_TOP];
+    constexpr int N = V::N, UN = 4, LP_WARPS = LP_THREADS / 32;
+    __shared__ Stat ws[LP_WARPS];
+    __shared__ Key wk[LP_WARPS][32];
+    __shared__ uint32_t bar_s;                 // order of the best k-th value seen
     __shared__ int last_in;
     pdl_trigger();
     pdl_wait();
@@ -145,160 +203,237 @@ __global__ void __launch_bounds__(LP_THREADS, 2) logprobs_kernel(const LpArgs a)
     const int c0 = split * a.chunk, c1 = min(a.vocab, c0 + a.chunk);
     const int v0 = (c0 + mis) / N, v1 = (c1 + mis + N - 1) / N;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x - mis);
+    if (threadIdx.x == 0) bar_s = 0;
+    __syncthreads();
+    // the target's logit, on its way from the start
+    int target = -1;
+    float tx = 0.f;
+    if (threadIdx.x == 0 && a.logp) {
+        target = a.target[row];
+        if (target >= 0 && target < a.vocab) tx = V::one(x + target);
+    }
     Stat st{-INFINITY, 0.f, 0.f};
-    float lv = -INFINITY;
-    int li = 0x7fffffff;
+    unsigned long long s2 = 0, a2 = 0;         // S and A as pairs; st's own are 0 meanwhile
+    Key list = 0;
     const int kth = max(a.top, 1) - 1;
-    float tv = a.top ? -INFINITY : INFINITY;
+    float tv = a.top ? -INFINITY : NAN;        // what a value has to reach; nothing reaches a NaN
     for (int b = v0; b < v1; b += LP_THREADS * UN) {
-        float f[UN][N];
+        uint32_t w[UN][4];
 #pragma unroll
         for (int u = 0; u < UN; u++) {
             const int v = b + u * LP_THREADS + threadIdx.x, i0 = v * N - mis;
             if (v < v1 && i0 >= c0 && i0 + N <= c1) {
-                V::f32(__ldcs(xv + v), f[u]);
+                const uint4 q = __ldcs(xv + v);
+                w[u][0] = q.x, w[u][1] = q.y, w[u][2] = q.z, w[u][3] = q.w;
             } else {
 #pragma unroll
-                for (int e = 0; e < N; e++)
-                    f[u][e] = v < v1 && i0 + e >= c0 && i0 + e < c1 ? V::one(x + i0 + e) : -INFINITY;
+                for (int e = 0; e < 4; e++) w[u][e] = V::NONE;
+                if (v < v1)
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        if (i0 + e >= c0 && i0 + e < c1) {
+                            if constexpr (sizeof(T) == 4) w[u][e] = reinterpret_cast<const uint32_t *>(x)[i0 + e];
+                            else {
+                                const uint32_t h = reinterpret_cast<const uint16_t *>(x)[i0 + e];
+                                w[u][e >> 1] = e & 1 ? (w[u][e >> 1] & 0xffffu) | (h << 16) : (w[u][e >> 1] & 0xffff0000u) | h;
+                            }
+                        }
             }
         }
-        bool some[UN];
-        float mx = -INFINITY;
+        float vm[UN], mx = -INFINITY;
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            float w = f[u][0];
-#pragma unroll
-            for (int e = 1; e < N; e++) w = fmaxf(w, f[u][e]);
-            some[u] = w >= tv;
-            mx = fmaxf(mx, w);
+            const uint32_t q = V::max_(V::max_(w[u][0], w[u][1]), V::max_(w[u][2], w[u][3]));
+            if constexpr (sizeof(T) == 4) vm[u] = __uint_as_float(q);
+            else {
+                const float2 f = V::two(q);
+                vm[u] = fmaxf(f.x, f.y);
+            }
+            mx = fmaxf(mx, vm[u]);
         }
-        if (mx > st.m) move(st, mx);
-        if (fabsf(st.m) < HUGE_M) {
+        if (mx > st.m) {
+            const float2 s = unpack2(s2), t = unpack2(a2);
+            st.s = s.x + s.y;
+            st.a = t.x + t.y;
+            move(st, mx);
+            s2 = pack2(st.s, 0.f);
+            a2 = pack2(st.a, 0.f);
+        }
+        if (st.m > V::LOW_M && st.m < HUGE_M) {
             const float nm = -st.m * LOG2E;
-#pragma unroll
-            for (int u = 0; u < UN; u++)
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const float t = max_nan_(fmaf(f[u][e], LOG2E, nm), FAR), p = ex2f_(t);
-                    st.s += p;
-                    st.a = fmaf(p, t, st.a);
-                }
-        } else {   // nothing but -inf so far, or a row at the edge of f32 (masked whole by the lowest value)
-#pragma unroll
-            for (int u = 0; u < UN; u++)
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    if (f[u][e] == -INFINITY) continue;
-                    const float t = max_nan_((f[u][e] - st.m) * LOG2E, FAR), p = ex2f_(t);
-                    st.s += p;
-                    st.a = fmaf(p, t, st.a);
-                }
-        }
-        bool any = false;
-#pragma unroll
-        for (int u = 0; u < UN; u++) any |= some[u];
-        if (a.top && __any_sync(0xffffffffu, any)) {
+            const unsigned long long nm2 = pack2(nm, nm), l2 = pack2(LOG2E, LOG2E);
 #pragma unroll
             for (int u = 0; u < UN; u++) {
-                if (!__any_sync(0xffffffffu, some[u])) continue;
-                const int i0 = (b + u * LP_THREADS + threadIdx.x) * N - mis;
+                if (b + u * LP_THREADS >= v1) break;   // the same for the CTA
 #pragma unroll
-                for (int e = 0; e < N; e++)
-                    offer(lv, li, fmaxf(f[u][e], -INFINITY), i0 + e, i0 + e >= c0 && i0 + e < c1, kth, lane);
+                for (int e = 0; e < N; e += 2) {
+                    float2 f;
+                    if constexpr (sizeof(T) == 4)
+                        f = make_float2(__uint_as_float(V::floor_(w[u][e])), __uint_as_float(V::floor_(w[u][e + 1])));
+                    else f = V::two(V::floor_(w[u][e >> 1]));
+                    const unsigned long long t = fma2(pack2(f.x, f.y), l2, nm2);
+                    const float2 tt = unpack2(t);
+                    const unsigned long long p = pack2(ex2f_(tt.x), ex2f_(tt.y));
+                    s2 = add2(s2, p);
+                    a2 = fma2(p, t, a2);
+                }
             }
-            tv = __shfl_sync(0xffffffffu, lv, kth);
-        }
-    }
-    // the CTA's (m, S, A) and list
+        } else {   // nothing but -inf so far, or a row at its type's edge (masked whole by the lowest value)
+            float2 s = unpack2(s2), t2 = unpack2(a2);
+            for (int u = 0; u < UN; u++)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Stat q{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                     __shfl_xor_sync(0xffffffffu, st.a, o)};
-        st = join(st, q);
+                for (int e = 0; e < N; e++) {
+                    const float f = V::at(w[u], e);
+                    if (f == -INFINITY) continue;
+                    const float t = f - st.m, p = t < -1e4f ? 0.f : ex2f_(t * LOG2E);
+                    s.x += p;
+                    if (!(p == 0.f)) t2.x = fmaf(p, t * LOG2E, t2.x);
+                }
+            s2 = pack2(s.x, s.y);
+            a2 = pack2(t2.x, t2.y);
+        }
+        if (a.top) {
+            if (b == v0) {   // a first bar: the k-th largest of the warp's lane maxima, the best warp's
+                float k = mx;
+#pragma unroll
+                for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+                    for (int o = n >> 1; o > 0; o >>= 1) {
+                        const float p = __shfl_xor_sync(0xffffffffu, k, o);
+                        k = !(lane & o) == !(lane & n) ? fmaxf(k, p) : fminf(k, p);
+                    }
+                if (lane == kth) atomicMax(&bar_s, order_of(k));
+                __syncthreads();
+            }
+            const float seen = value_of((Key) * (volatile uint32_t *)&bar_s << 32);
+            tv = fmaxf(tv, seen);
+            bool any = false;
+#pragma unroll
+            for (int u = 0; u < UN; u++) any |= vm[u] >= tv;
+            if (__any_sync(0xffffffffu, any)) {
+#pragma unroll 1
+                for (int u = 0; u < UN; u++) {
+                    const float top = u == 0 ? vm[0] : u == 1 ? vm[1] : u == 2 ? vm[2] : vm[3];
+                    if (!__any_sync(0xffffffffu, top >= tv)) continue;
+                    uint32_t q[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) q[e] = u == 0 ? w[0][e] : u == 1 ? w[1][e] : u == 2 ? w[2][e] : w[3][e];
+                    const int i0 = (b + u * LP_THREADS + threadIdx.x) * N - mis;
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const float f = fmaxf(V::at(q, e), -INFINITY);
+                        const bool ok = f >= tv && i0 + e >= c0 && i0 + e < c1;
+                        if (__any_sync(0xffffffffu, ok)) offer(list, ok ? key_of(f, i0 + e) : 0, kth, lane);
+                    }
+                }
+                const Key last = __shfl_sync(0xffffffffu, list, kth);
+                if (last) {
+                    tv = fmaxf(tv, value_of(last));
+                    if (lane == 0 && value_of(last) > seen) atomicMax(&bar_s, (uint32_t)(last >> 32));
+                }
+            }
+        }
     }
-    if (lane == 0) {
-        ws[warp][0] = st.m;
-        ws[warp][1] = st.s;
-        ws[warp][2] = st.a;
-    }
-    wv[warp][lane] = lv;
-    wi[warp][lane] = li;
-    __syncthreads();
-    if (warp != 0) return;
-    st = Stat{ws[0][0], ws[0][1], ws[0][2]};
-    for (int w = 1; w < LP_WARPS; w++) {
-        st = join(st, Stat{ws[w][0], ws[w][1], ws[w][2]});
-        if (a.top) offer(lv, li, wv[w][lane], wi[w][lane], lane < a.top, kth, lane);
-    }
+    const float2 s = unpack2(s2), t = unpack2(a2);
+    st.s = s.x + s.y;
+    st.a = t.x + t.y;
+    st = warp_join(st);
+    // the CTA's (m, S, A) and list: a tree over the warps
+    auto cta = [&]() {
+        if (lane == 0) ws[warp] = st;
+        wk[warp][lane] = list;
+        __syncthreads();
+        if (a.top)
+#pragma unroll 1
+            for (int h = LP_WARPS / 2; h > 0; h >>= 1) {
+                if (warp < h) wk[warp][lane] = list = merge(list, wk[warp + h][31 - lane], lane);
+                __syncthreads();
+            }
+        if (warp == 0) st = warp_join(lane < LP_WARPS ? ws[lane] : Stat{-INFINITY, 0.f, 0.f});
+    };
+    cta();
     if (a.splits > 1) {
-        float *p = a.part + ((size_t)row * a.splits + split) * (4 + 2 * LP_TOP);
-        if (lane == 0) {
-            p[0] = st.m;
-            p[1] = st.s;
-            p[2] = st.a;
+        float *p = a.part + ((size_t)row * a.splits + split) * LP_PART;
+        if (warp == 0) {
+            if (lane == 0) {
+                p[0] = st.m;
+                p[1] = st.s;
+                p[2] = st.a;
+            }
+            reinterpret_cast<Key *>(p + 4)[lane] = list;
+            __syncwarp();
+            if (lane == 0) {
+                __threadfence();
+                last_in = atomicAdd(a.tickets + row, 1u) == (unsigned)(a.splits - 1);
+                __threadfence();
+            }
         }
-        p[4 + lane] = lv;
-        reinterpret_cast<int *>(p)[4 + LP_TOP + lane] = li;
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) last_in = atomicAdd(a.tickets + row, 1u) == (unsigned)(a.splits - 1);
-        __syncwarp();
+        __syncthreads();
         if (!last_in) return;
-        __threadfence();
-        if (lane == 0) a.tickets[row] = 0u;
-        p = a.part + (size_t)row * a.splits * (4 + 2 * LP_TOP);
-        lv = -INFINITY;
-        li = 0x7fffffff;
+        if (threadIdx.x == 0) a.tickets[row] = 0u;
+        p = a.part + (size_t)row * a.splits * LP_PART;
         st = Stat{-INFINITY, 0.f, 0.f};
-        for (int c = 0; c < a.splits; c++, p += 4 + 2 * LP_TOP) {
-            st = join(st, Stat{__ldcg(p), __ldcg(p + 1), __ldcg(p + 2)});
-            if (a.top)
-                offer(lv, li, __ldcg(p + 4 + lane), __ldcg(reinterpret_cast<const int *>(p) + 4 + LP_TOP + lane),
-                      lane < a.top, kth, lane);
+        list = 0;
+        for (int c0 = warp; c0 < a.splits; c0 += 4 * LP_WARPS) {   // 4 parts a warp in flight
+            Key k[4];
+            Stat q[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float *pc = p + (size_t)min(c0 + i * LP_WARPS, a.splits - 1) * LP_PART;
+                q[i] = Stat{__ldcg(pc), __ldcg(pc + 1), __ldcg(pc + 2)};
+                k[i] = __ldcg(reinterpret_cast<const Key *>(pc + 4) + 31 - lane);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (c0 + i * LP_WARPS >= a.splits) break;
+                if (lane == 0) st = join(st, q[i]);
+                if (a.top) list = merge(list, k[i], lane);
+            }
         }
+        cta();
     }
+    if (warp != 0) return;
     // no distribution: a NaN in the sums, +inf (whose reference makes them NaN) or nothing but -inf
-    const float ls2 = log2f(st.s);                     // log2 S
+    const float ls = log2f(st.s) * LN2;
     const bool sound = st.s > 0.f;
     if (lane == 0) {
-        if (a.logp && a.target) {
-            const int i = a.target[row];
-            float r = NAN;
-            if (i >= 0 && i < a.vocab) {
-                const float v = V::one(x + i);
-                r = sound ? (v - st.m) - ls2 * LN2 : NAN;
-            } else if (i < 0) {
-                r = 0.f;
-            } else if (a.err) {
-                atomicExch(a.err, DEV_BAD_INDEX);
-            }
-            a.logp[row] = r;
+        if (a.logp) {
+            a.logp[row] = target < 0 ? 0.f : target < a.vocab && sound ? (tx - st.m) - ls : NAN;
+            if (target >= a.vocab && a.err) atomicExch(a.err, DEV_BAD_INDEX);
         }
-        if (a.entropy) a.entropy[row] = sound ? fmaxf((ls2 - st.a / st.s) * LN2, 0.f) : NAN;
+        if (a.entropy) a.entropy[row] = sound ? fmaxf(ls - st.a / st.s * LN2, 0.f) : NAN;
     }
     if (lane < a.top) {
-        a.ids[(size_t)row * a.top + lane] = li;
-        a.best[(size_t)row * a.top + lane] = sound ? (lv - st.m) - ls2 * LN2 : NAN;
+        a.ids[(size_t)row * a.top + lane] = index_of(list);
+        a.best[(size_t)row * a.top + lane] = sound ? (value_of(list) - st.m) - ls : NAN;
     }
 }
 
-// CTAs of a row: enough to give every SM two CTAs, each at least two tiles of values
-int splits_of(int rows, int vocab, int size, int *chunk) {
-    const int tile = LP_THREADS * (16 / size);
-    long long s = (2ll * sm_count() + rows - 1) / rows;
-    const long long most = (vocab + 2ll * tile - 1) / (2ll * tile);
+// The CTAs of a row and their threads. An SM holds 1024 threads: 8 CTAs of 128, so that about as many
+// rows (or parts of rows) as the SMs hold run side by side and share the memory until the end; few
+// rows go over up to 64 CTAs of 512 threads each, whose 16 warps join the parts' lists faster
+// (131072 f32 values, 20 alternatives: see the file's head). A CTA has at least one tile of values.
+int plan(const LpArgs &a, int size, int *chunk, int *threads) {
+    const int slots = 8 * sm_count();
+    *threads = (long long)a.rows * LP_SPLITS <= slots ? 512 : 128;
+    const int tile = *threads * (16 / size);
+    long long s = *threads == 512 ? LP_SPLITS : slots / a.rows;
+    const long long most = ((long long)a.vocab + tile - 1) / tile;
     if (s > most) s = most;
     if (s > LP_SPLITS) s = LP_SPLITS;
     if (s < 1) s = 1;
-    const long long per = ((vocab + s - 1) / s + tile - 1) / tile * tile;
-    *chunk = (int)(per < vocab ? per : vocab);
-    return (int)((vocab + (long long)*chunk - 1) / *chunk);
+    const long long per = ((a.vocab + s - 1) / s + tile - 1) / tile * tile;
+    *chunk = (int)(per < a.vocab ? per : a.vocab);
+    return (int)((a.vocab + (long long)*chunk - 1) / *chunk);
 }
 
 template <typename T>
-cudaError_t launch(const LpArgs &a, cudaStream_t s) {
-    return launch_pdl(logprobs_kernel<T>, dim3(a.splits, a.rows), dim3(LP_THREADS), 0, s, a);
+cudaError_t launch(LpArgs &a, cudaStream_t s) {
+    int threads;
+    a.splits = plan(a, sizeof(T), &a.chunk, &threads);
+    const dim3 grid(a.splits, a.rows);
+    return threads == 512 ? launch_pdl(logprobs_kernel<T, 512>, grid, dim3(512), 0, s, a)
+                          : launch_pdl(logprobs_kernel<T, 128>, grid, dim3(128), 0, s, a);
 }
 
 size_t ticket_bytes(int rows) { return ((size_t)rows * 4 + 255) / 256 * 256; }
@@ -311,9 +446,8 @@ extern "C" {
 size_t spk_logprobs_workspace_bytes(int rows, int vocab) {
     using namespace spk;
     if (rows < 1 || vocab < 1) return 0;
-    return ticket_bytes(rows) + (size_t)rows * LP_SPLITS * (4 + 2 * LP_TOP) * sizeof(float);
+    return ticket_bytes(rows) + (size_t)rows * LP_SPLITS * LP_PART * sizeof(float);
 }
-
 int spk_logprobs(const void *logits, int type, int rows, int vocab, long long ld, const int *target, float *logp,
                  float *entropy, int top, int *top_ids, float *top_logp, void *workspace, void *stream) {
     using namespace spk;
@@ -323,6 +457,7 @@ int spk_logprobs(const void *logits, int type, int rows, int vocab, long long ld
     if (top < 0 || top > LP_TOP || top > vocab) return set_error("%s: %d alternatives (0 to %d, at most vocab)", who, top, LP_TOP);
     if (rows == 0) return 0;
     const int size = type == 0 ? 4 : 2;
+    if ((uintptr_t)workspace % 16) return set_error("%s: the workspace is not 16-byte aligned", who);
     if (!logits || !workspace || (logp && !target) || (top && (!top_ids || !top_logp)))
         return set_error("%s: null buffer", who);
     if ((uintptr_t)logits % size) return set_error("%s: unaligned logits", who);
@@ -333,7 +468,6 @@ int spk_logprobs(const void *logits, int type, int rows, int vocab, long long ld
     a.rows = rows;
     a.vocab = vocab;
     a.top = top;
-    a.splits = splits_of(rows, vocab, size, &a.chunk);
     a.target = target;
     a.logp = logp;
     a.entropy = entropy;
