@@ -177,23 +177,17 @@ struct Vec {   // 16 bytes of T
         return r;
     }
     static constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
-    static __device__ __forceinline__ float at(const uint32_t (&w)[4], int e) {
-        if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
-        else {
-            const float2 f = two(w[e >> 1]);
-            return e & 1 ? f.y : f.x;
-        }
-    }
 };
 
 template <typename T, int LP_THREADS>
-__global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel(const LpArgs a) {
+__global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(const LpArgs a) {
     using V = Vec<T>;
     constexpr int N = V::N, UN = 4, LP_WARPS = LP_THREADS / 32;
     __shared__ Stat ws[LP_WARPS];
     __shared__ Key wk[LP_WARPS][32];
     __shared__ uint32_t bar_s;                 // order of the best k-th value seen
     __shared__ int last_in;
+    __shared__ __align__(16) uint32_t look_s[LP_WARPS][UN * 4];   // one lane's values, for the whole warp to look at
     pdl_trigger();
     pdl_wait();
     const int row = blockIdx.y, split = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -202,6 +196,10 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
     const int mis = (int)(((uintptr_t)x % 16) / sizeof(T));
     const int c0 = split * a.chunk, c1 = min(a.vocab, c0 + a.chunk);
     const int v0 = (c0 + mis) / N, v1 = (c1 + mis + N - 1) / N;
+    // the vectors that lie whole in the range, and those of them that fill whole tiles
+    const int w0 = (c0 + mis + N - 1) / N, w1 = max(w0, (c1 + mis) / N);
+    constexpr int STRIDE = LP_THREADS * UN;
+    const int full = w0 + (w1 - w0) / STRIDE * STRIDE;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x - mis);
     if (threadIdx.x == 0) bar_s = 0;
     __syncthreads();
@@ -217,39 +215,19 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
     Key list = 0;
     const int kth = max(a.top, 1) - 1;
     float tv = a.top ? -INFINITY : NAN;        // what a value has to reach; nothing reaches a NaN
-    for (int b = v0; b < v1; b += LP_THREADS * UN) {
-        uint32_t w[UN][4];
+    bool barred = false;
+    // UN vectors of this thread, the first at value i0, the others STEP values apart; edge: some of
+    // their values lie outside of the range (they are -inf) and are not tokens
+    auto eat = [&](const uint32_t (&w)[UN][4], int i0, int used, bool edge) {
+        constexpr int STEP = LP_THREADS * N;
+        uint32_t q = V::max_(V::max_(w[0][0], w[0][1]), V::max_(w[0][2], w[0][3]));
 #pragma unroll
-        for (int u = 0; u < UN; u++) {
-            const int v = b + u * LP_THREADS + threadIdx.x, i0 = v * N - mis;
-            if (v < v1 && i0 >= c0 && i0 + N <= c1) {
-                const uint4 q = __ldcs(xv + v);
-                w[u][0] = q.x, w[u][1] = q.y, w[u][2] = q.z, w[u][3] = q.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) w[u][e] = V::NONE;
-                if (v < v1)
-#pragma unroll
-                    for (int e = 0; e < N; e++)
-                        if (i0 + e >= c0 && i0 + e < c1) {
-                            if constexpr (sizeof(T) == 4) w[u][e] = reinterpret_cast<const uint32_t *>(x)[i0 + e];
-                            else {
-                                const uint32_t h = reinterpret_cast<const uint16_t *>(x)[i0 + e];
-                                w[u][e >> 1] = e & 1 ? (w[u][e >> 1] & 0xffffu) | (h << 16) : (w[u][e >> 1] & 0xffff0000u) | h;
-                            }
-                        }
-            }
-        }
-        float vm[UN], mx = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < UN; u++) {
-            const uint32_t q = V::max_(V::max_(w[u][0], w[u][1]), V::max_(w[u][2], w[u][3]));
-            if constexpr (sizeof(T) == 4) vm[u] = __uint_as_float(q);
-            else {
-                const float2 f = V::two(q);
-                vm[u] = fmaxf(f.x, f.y);
-            }
-            mx = fmaxf(mx, vm[u]);
+        for (int u = 1; u < UN; u++) q = V::max_(q, V::max_(V::max_(w[u][0], w[u][1]), V::max_(w[u][2], w[u][3])));
+        float mx;
+        if constexpr (sizeof(T) == 4) mx = __uint_as_float(q);
+        else {
+            const float2 f = V::two(q);
+            mx = fmaxf(f.x, f.y);
         }
         if (mx > st.m) {
             const float2 s = unpack2(s2), t = unpack2(a2);
@@ -264,7 +242,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
             const unsigned long long nm2 = pack2(nm, nm), l2 = pack2(LOG2E, LOG2E);
 #pragma unroll
             for (int u = 0; u < UN; u++) {
-                if (b + u * LP_THREADS >= v1) break;   // the same for the CTA
+                if (u >= used) break;   // the same for the CTA
 #pragma unroll
                 for (int e = 0; e < N; e += 2) {
                     float2 f;
@@ -280,58 +258,118 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
             }
         } else {   // nothing but -inf so far, or a row at its type's edge (masked whole by the lowest value)
             float2 s = unpack2(s2), t2 = unpack2(a2);
-            for (int u = 0; u < UN; u++)
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const float f = V::at(w[u], e);
-                    if (f == -INFINITY) continue;
-                    const float t = f - st.m, p = t < -1e4f ? 0.f : ex2f_(t * LOG2E);
-                    s.x += p;
-                    if (!(p == 0.f)) t2.x = fmaf(p, t * LOG2E, t2.x);
+            for (int u = 0; u < UN; u++)
+#pragma unroll 1
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t word = e == 0 ? w[u][0] : e == 1 ? w[u][1] : e == 2 ? w[u][2] : w[u][3];
+                    float f[2] = {__uint_as_float(word), -INFINITY};
+                    if constexpr (sizeof(T) == 2) {
+                        const float2 g = V::two(word);
+                        f[0] = g.x, f[1] = g.y;
+                    }
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        if (f[y] == -INFINITY) continue;
+                        const float t = f[y] - st.m, p = t < -1e4f ? 0.f : ex2f_(t * LOG2E);
+                        s.x += p;
+                        if (!(p == 0.f)) t2.x = fmaf(p, t * LOG2E, t2.x);
+                    }
                 }
             s2 = pack2(s.x, s.y);
             a2 = pack2(t2.x, t2.y);
         }
-        if (a.top) {
-            if (b == v0) {   // a first bar: the k-th largest of the warp's lane maxima, the best warp's
-                float k = mx;
+        if (!a.top) return;
+        if (!barred) {   // a first bar: the k-th largest of the warp's lane maxima, the best warp's
+            barred = true;
+            float k = mx;
 #pragma unroll
-                for (int n = 2; n <= 32; n <<= 1)
+            for (int n = 2; n <= 32; n <<= 1)
 #pragma unroll
-                    for (int o = n >> 1; o > 0; o >>= 1) {
-                        const float p = __shfl_xor_sync(0xffffffffu, k, o);
-                        k = !(lane & o) == !(lane & n) ? fmaxf(k, p) : fminf(k, p);
-                    }
-                if (lane == kth) atomicMax(&bar_s, order_of(k));
-                __syncthreads();
+                for (int o = n >> 1; o > 0; o >>= 1) {
+                    const float p = __shfl_xor_sync(0xffffffffu, k, o);
+                    k = !(lane & o) == !(lane & n) ? fmaxf(k, p) : fminf(k, p);
+                }
+            if (lane == kth) atomicMax(&bar_s, order_of(k));
+            __syncthreads();
+        }
+        const float seen = value_of((Key) * (volatile uint32_t *)&bar_s << 32);
+        tv = fmaxf(tv, seen);
+        unsigned left = __ballot_sync(0xffffffffu, mx >= tv);
+        if (!left) return;
+        while (left) {   // the lanes with a value that may count: the warp looks at one lane's values together
+            const int src = __ffs(left) - 1;
+            left &= left - 1;
+            if (lane == src)
+#pragma unroll
+                for (int u = 0; u < UN; u++)
+                    *reinterpret_cast<uint4 *>(&look_s[warp][4 * u]) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+            const int base = __shfl_sync(0xffffffffu, i0, src);
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < UN * N; h += 32) {   // 16 or 32 values
+                const int v = h + lane, i = base + (v / N) * STEP + v % N;
+                Key k = 0;
+                if (v < UN * N && (!edge || (i >= c0 && i < c1))) {
+                    const float f = fmaxf(V::one(reinterpret_cast<const T *>(look_s[warp]) + v), -INFINITY);
+                    if (f >= tv) k = key_of(f, i);
+                }
+                offer(list, k, kth, lane);
             }
-            const float seen = value_of((Key) * (volatile uint32_t *)&bar_s << 32);
-            tv = fmaxf(tv, seen);
-            bool any = false;
+            __syncwarp();
+        }
+        const Key last = __shfl_sync(0xffffffffu, list, kth);
+        if (last) {
+            tv = fmaxf(tv, value_of(last));
+            if (lane == 0 && value_of(last) > seen) atomicMax(&bar_s, (uint32_t)(last >> 32));
+        }
+    };
+    auto fetch = [&](uint32_t (&w)[UN][4], int b) {
 #pragma unroll
-            for (int u = 0; u < UN; u++) any |= vm[u] >= tv;
-            if (__any_sync(0xffffffffu, any)) {
+        for (int u = 0; u < UN; u++) {
+            const uint4 q = __ldcs(xv + b + u * LP_THREADS + threadIdx.x);
+            w[u][0] = q.x, w[u][1] = q.y, w[u][2] = q.z, w[u][3] = q.w;
+        }
+    };
+    {
+        uint32_t w[UN][4];
+        if (w0 < full) fetch(w, w0);
+        for (int b = w0; b < full; b += STRIDE) {   // the next tile comes while this one is worked on
+            uint32_t n[UN][4];
+            const bool more = b + STRIDE < full;
+            if (more) fetch(n, b + STRIDE);
+            eat(w, (b + (int)threadIdx.x) * N - mis, UN, false);
+            if (more)
+#pragma unroll
+                for (int u = 0; u < UN; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[u][e] = n[u][e];
+        }
+        // what is left behind the whole tiles, then a cut vector before them
 #pragma unroll 1
-                for (int u = 0; u < UN; u++) {
-                    const float top = u == 0 ? vm[0] : u == 1 ? vm[1] : u == 2 ? vm[2] : vm[3];
-                    if (!__any_sync(0xffffffffu, top >= tv)) continue;
-                    uint32_t q[4];
+        for (int r = full < v1 ? 0 : 1; r < (v0 < w0 ? 2 : 1); r++) {
+            const int b = r == 0 ? full : v0, end = r == 0 ? v1 : w0;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) q[e] = u == 0 ? w[0][e] : u == 1 ? w[1][e] : u == 2 ? w[2][e] : w[3][e];
-                    const int i0 = (b + u * LP_THREADS + threadIdx.x) * N - mis;
+            for (int u = 0; u < UN; u++) {
+                const int v = b + u * LP_THREADS + threadIdx.x, i0 = v * N - mis;
 #pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        const float f = fmaxf(V::at(q, e), -INFINITY);
-                        const bool ok = f >= tv && i0 + e >= c0 && i0 + e < c1;
-                        if (__any_sync(0xffffffffu, ok)) offer(list, ok ? key_of(f, i0 + e) : 0, kth, lane);
-                    }
-                }
-                const Key last = __shfl_sync(0xffffffffu, list, kth);
-                if (last) {
-                    tv = fmaxf(tv, value_of(last));
-                    if (lane == 0 && value_of(last) > seen) atomicMax(&bar_s, (uint32_t)(last >> 32));
+                for (int e = 0; e < 4; e++) w[u][e] = V::NONE;
+                if (v >= w0 && v < w1 && v < end) {
+                    const uint4 q = __ldcs(xv + v);
+                    w[u][0] = q.x, w[u][1] = q.y, w[u][2] = q.z, w[u][3] = q.w;
+                } else if (v < end) {
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        if (i0 + e >= c0 && i0 + e < c1) {
+                            if constexpr (sizeof(T) == 4) w[u][e] = reinterpret_cast<const uint32_t *>(x)[i0 + e];
+                            else {
+                                const uint32_t h = reinterpret_cast<const uint16_t *>(x)[i0 + e];
+                                w[u][e >> 1] = e & 1 ? (w[u][e >> 1] & 0xffffu) | (h << 16) : (w[u][e >> 1] & 0xffff0000u) | h;
+                            }
+                        }
                 }
             }
+            eat(w, (b + (int)threadIdx.x) * N - mis, (end - b + LP_THREADS - 1) / LP_THREADS, true);
         }
     }
     const float2 s = unpack2(s2), t = unpack2(a2);
@@ -409,12 +447,12 @@ __global__ void __launch_bounds__(LP_THREADS, 1024 / LP_THREADS) logprobs_kernel
     }
 }
 
-// The CTAs of a row and their threads. An SM holds 1024 threads: 8 CTAs of 128, so that about as many
+// The CTAs of a row and their threads. An SM holds 768 threads: 6 CTAs of 128, so that about as many
 // rows (or parts of rows) as the SMs hold run side by side and share the memory until the end; few
 // rows go over up to 64 CTAs of 512 threads each, whose 16 warps join the parts' lists faster
 // (131072 f32 values, 20 alternatives: see the file's head). A CTA has at least one tile of values.
 int plan(const LpArgs &a, int size, int *chunk, int *threads) {
-    const int slots = 8 * sm_count();
+    const int slots = 6 * sm_count();
     *threads = (long long)a.rows * LP_SPLITS <= slots ? 512 : 128;
     const int tile = *threads * (16 / size);
     long long s = *threads == 512 ? LP_SPLITS : slots / a.rows;

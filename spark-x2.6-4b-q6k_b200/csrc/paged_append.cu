@@ -11,10 +11,12 @@
 // block's scale NaN or infinite (its rows read as NaN) and never a stored byte.
 //
 // What bounds it: bytes (each value read once, one byte written) for prompts, the chain of
-// dependent loads (sequence -> page -> row) for steps. A unit of work is one (block, KV head, keys
-// or values): one CTA of 4 warps, a warp per row, a row's unit of 8 values in one thread's
-// registers, so the block's amax is a max in registers, one shuffle tree and one exchange between
-// the warps; the bytes meet in shared memory and leave as 16-byte stores.
+// dependent loads (sequence -> page -> row) for steps. A CTA of 4 warps takes one block, keys or
+// values, and 256 values of a row at a time (256 / head_dim heads side by side): a warp 4 of the 16
+// rows, a lane 8 values of each, so that a head's amax is a max in registers, a shuffle tree and one
+// exchange between the warps. The bytes meet in shared memory (4 KB, 16-byte pieces spread over the
+// banks) and leave as 16-byte stores. Where there are many blocks a CTA walks several head groups,
+// which share the rows' angles: a cosine and sine cost as much as ten values' rounding and storing.
 #include "paged.cuh"
 
 namespace spk {
@@ -42,56 +44,244 @@ int check_batch(const spk_kv_batch *b, const char *who) {
 namespace {
 
 constexpr int AP_WARPS = 4, AP_THREADS = AP_WARPS * 32, AP_ROWS = BLOCK / AP_WARPS;
+constexpr int AP_WIDTH = 256;              // values of a row that a warp takes at once
 
 struct AppendArgs {
     Pool pool;
     Batch b;
     const void *k, *v;
     long long ldk, ldv;
-    int kvec, vvec;
+    int kvec, vvec;                        // alignment of the rows' pieces: 0 none, 1 four values, 2 eight too
     const float *freq;
     int pdim;
+    int passes;                            // head groups of a CTA
     int *err;
 };
 
-// max that keeps a NaN
+// max of |a|, |b|, |c| that keeps a NaN
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-
-// e4m3 of a and b (low byte a); a NaN is stored as 0: the block's scale tells of it
-__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
-    if (!(a == a)) a = 0.f;
-    if (!(b == b)) b = 0.f;
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {   // low byte a
     return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
-
-__device__ __forceinline__ float e4m3_f32(uint32_t byte) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+__device__ __forceinline__ float2 e4m3x2_f32(uint32_t w) {
+    return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
 }
 
-// 16-byte piece of the staging tile of values, spread so that a warp's 4-byte writes (dims 4 or 8
-// apart) meet fewer banks
-__device__ __forceinline__ int vpiece(int d) { return d ^ ((d >> 3) & 7); }
+// 8 consecutive values
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, int vec, float (&x)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        if (vec == 2) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (__is_same(T, __half)) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+                    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+                } else {
+                    x[2 * i] = __uint_as_float(u[i] << 16), x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+                }
+            }
+            return;
+        }
+    }
+    const float4 a = load4<T>(p, vec > 0), b = load4<T>(p + 4, vec > 0);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+
+// 16-byte piece of the staging tile, spread so that a warp's 4-byte writes (pieces 8 apart) meet few banks
+__device__ __forceinline__ int spread(int piece) { return piece ^ ((piece >> 3) & 7); }
+
+// Block `blk` of a sequence (its page's block bp), rows lo .. hi - 1 of it being the call's; row 0
+// of the block would be row `row` of the call.
+template <typename T, int HD, bool KEYS>
+__device__ __forceinline__ void append_block(const AppendArgs &a, int page, int bp, int blk, int lo, int hi, int row,
+                                             uint8_t *tile, float2 *turn, float (*wmax)[AP_WARPS]) {
+    constexpr int LPR = HD / 8, GH = AP_WIDTH / HD, PER = AP_WIDTH / AP_THREADS;   // lanes of a head; heads; pieces of a thread
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPR, u = lane % LPR;
+    const int pdim = KEYS ? a.pdim : 0, half = pdim / 2;
+    int d0, d1;
+    unit_dims(u, pdim, d0, d1);
+    if (KEYS && pdim) {   // the rows' angles, for all heads
+        for (int i = threadIdx.x; i < BLOCK * half; i += AP_THREADS) {
+            const int r = i / half, f = i - r * half;
+            if (r >= lo && r < hi) angle(blk * BLOCK + r, __ldg(a.freq + f), turn[i].x, turn[i].y);
+        }
+        __syncthreads();
+    }
+    uint8_t *pool = KEYS ? a.pool.k : a.pool.v;
+    float *scales = KEYS ? a.pool.ks : a.pool.vs;
+    const T *rows = KEYS ? (const T *)a.k : (const T *)a.v;
+    const long long ld = KEYS ? a.ldk : a.ldv;
+    const int vec = KEYS ? a.kvec : a.vvec;
+    for (int g = blockIdx.y * a.passes; g < (int)(blockIdx.y + 1) * a.passes && g * GH < a.pool.kv_heads; g++) {
+        const int head = g * GH + sub;
+        const bool real = head < a.pool.kv_heads;
+        const size_t bi = block_index(a.pool, page, min(head, a.pool.kv_heads - 1), bp);
+        // earlier rows and their scale, on their way while the new rows come in
+        uint4 old[PER];
+        float d_old = 0.f;
+        if (lo > 0) {
+            d_old = scales[bi];
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int pc = i * AP_THREADS + threadIdx.x, hd = g * GH + pc / HD;
+                if (hd < a.pool.kv_heads)
+                    old[i] = reinterpret_cast<const uint4 *>(pool + block_index(a.pool, page, hd, bp) * (BLOCK * HD))[pc % HD];
+            }
+        }
+        // warp w: rows 2w, 2w + 1, 2w + 8, 2w + 9, which are bytes 4w .. 4w + 3 of a value dim
+        float x[AP_ROWS][8];
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < AP_ROWS; i++) {
+            const int r = 2 * warp + (i & 1) + 8 * (i >> 1);
+            if (real && r >= lo && r < hi) {
+                const T *src = rows + (size_t)(row + r) * ld + (size_t)head * HD;
+                if (KEYS) {
+                    float p[4], q[4];
+                    load_unit<T>(src, u, pdim, vec > 0, p, q);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[i][e] = p[e], x[i][4 + e] = q[e];
+                } else {
+                    load8<T>(src + 8 * u, vec, x[i]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[i][e] = 0.f;
+            }
+        }
+        if (KEYS && u < pdim / 8) {
+#pragma unroll
+            for (int i = 0; i < AP_ROWS; i++) {
+                const int r = 2 * warp + (i & 1) + 8 * (i >> 1);
+                if (r < lo || r >= hi) continue;
+                const float4 *t = reinterpret_cast<const float4 *>(turn + r * half + d0);
+                const float4 t0 = t[0], t1 = t[1];
+                const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y, t0.w, t1.y, t1.w};
+                float p[4], q[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) p[e] = x[i][e], q[e] = x[i][4 + e];
+                rotate_unit(p, q, c, s);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[i][e] = p[e], x[i][4 + e] = q[e];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < AP_ROWS; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) mx = max_abs(mx, x[i][e], x[i][e + 1]);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        if (u == 0) wmax[sub][warp] = mx;
+        __syncthreads();   // the maxima are there, and the tile is free
+        mx = max_nan(max_nan(wmax[sub][0], wmax[sub][1]), max_nan(wmax[sub][2], wmax[sub][3]));
+        float d = max_nan(__fdiv_rn(mx, E4M3_MAX), SCALE_MIN);
+        if (lo > 0) d = max_nan(d, d_old);
+        if (lo > 0) {   // earlier rows, rounded again where the scale grew; 0 elsewhere
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int pc = i * AP_THREADS + threadIdx.x, hs = pc / HD, in = pc % HD;
+                float m2 = max_nan(max_nan(wmax[hs][0], wmax[hs][1]), max_nan(wmax[hs][2], wmax[hs][3]));
+                const int hd = g * GH + hs;
+                if (hd >= a.pool.kv_heads) continue;
+                const float o2 = scales[block_index(a.pool, page, hd, bp)];
+                m2 = max_nan(max_nan(__fdiv_rn(m2, E4M3_MAX), SCALE_MIN), o2);
+                const float ratio = m2 > o2 ? __fdiv_rn(o2, m2) : 1.0f;
+                // keys: piece = (8-token group, 16-dim chunk, token): one token; values: one dim's 16 tokens
+                const int ktok = 8 * (in / (HD / 2)) + (in & 7);
+                uint32_t w[4] = {old[i].x, old[i].y, old[i].z, old[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t v = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int t0 = KEYS ? ktok : order(4 * j + 2 * h), t1 = KEYS ? ktok : order(4 * j + 2 * h + 1);
+                        uint32_t pr = (w[j] >> (16 * h)) & 0xffffu;
+                        if (ratio != 1.0f) {
+                            const float2 f = e4m3x2_f32(pr);
+                            pr = e4m3x2(__fmul_rn(f.x, ratio), __fmul_rn(f.y, ratio));
+                        }
+                        if (t0 >= lo) pr &= 0xff00u;
+                        if (t1 >= lo) pr &= 0x00ffu;
+                        v |= pr << (16 * h);
+                    }
+                    w[j] = v;
+                }
+                reinterpret_cast<uint4 *>(tile)[spread(pc)] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __syncthreads();
+        }
+        // the new rows (all of the tile when nothing earlier is in the block); none where the scale is no number
+        const float inv = __fdiv_rn(1.0f, d);
+        const bool fine = d < INFINITY;
+        uint32_t q[AP_ROWS][4];   // e4m3 pairs
+#pragma unroll
+        for (int i = 0; i < AP_ROWS; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                q[i][e] = fine ? e4m3x2(__fmul_rn(x[i][2 * e], inv), __fmul_rn(x[i][2 * e + 1], inv)) : 0u;
+        if (KEYS) {
+#pragma unroll
+            for (int i = 0; i < AP_ROWS; i++) {
+                const int r = 2 * warp + (i & 1) + 8 * (i >> 1);
+                if (r < lo) continue;
+                const int pc = sub * HD + (r >> 3) * (HD / 2) + (r & 7);
+                *reinterpret_cast<uint32_t *>(tile + 16 * spread(pc + 8 * (d0 >> 4)) + (d0 & 15)) = __byte_perm(q[i][0], q[i][1], 0x5410);
+                *reinterpret_cast<uint32_t *>(tile + 16 * spread(pc + 8 * (d1 >> 4)) + (d1 & 15)) = __byte_perm(q[i][2], q[i][3], 0x5410);
+            }
+        } else {
+            uint32_t keep = 0;   // bytes that hold earlier rows
+#pragma unroll
+            for (int i = 0; i < AP_ROWS; i++)
+                if (2 * warp + (i & 1) + 8 * (i >> 1) < lo) keep |= 0xffu << (8 * i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {   // two dims: the rows' low bytes, the rows' high bytes
+                const uint32_t m = __byte_perm(q[0][e], q[1][e], 0x5410), n = __byte_perm(q[2][e], q[3][e], 0x5410);
+                const uint32_t w[2] = {__byte_perm(m, n, 0x6420), __byte_perm(m, n, 0x7531)};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t *at = reinterpret_cast<uint32_t *>(tile + 16 * spread(sub * HD + 8 * u + 2 * e + h)) + warp;
+                    *at = keep ? (*at & keep) | (w[h] & ~keep) : w[h];
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int pc = i * AP_THREADS + threadIdx.x, hd = g * GH + pc / HD;
+            if (hd < a.pool.kv_heads)
+                reinterpret_cast<uint4 *>(pool + block_index(a.pool, page, hd, bp) * (BLOCK * HD))[pc % HD] =
+                    reinterpret_cast<const uint4 *>(tile)[spread(pc)];
+        }
+        if (u == 0 && warp == 0 && real) scales[bi] = d;
+    }
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) {
-    constexpr int U = HD / 8;            // units of a row, one per lane (hd 256) or fewer
-    constexpr int PIECES = HD;           // 16-byte pieces of a block
-    __shared__ __align__(16) uint8_t tile[BLOCK * HD];
+    __shared__ __align__(16) uint8_t tile[BLOCK * AP_WIDTH];
+    __shared__ __align__(16) float2 turn[BLOCK * HD / 2];
+    __shared__ float wmax[AP_WIDTH / HD][AP_WARPS];
     __shared__ int who[3];               // sequence, its first row, its rows
-    __shared__ float wmax[AP_WARPS];
     pdl_trigger();
-    pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int unit = blockIdx.x, head = blockIdx.y;
-    const bool keys = blockIdx.z == 0;
-    // Units of sequence s: row0[s] / 16 + 2 s up to the next one's; n rows touch at most
-    // n / 16 + 2 blocks, so each sequence's blocks fit.
     if (threadIdx.x == 0) who[0] = -1;
     __syncthreads();
+    pdl_wait();
+    const int unit = blockIdx.x;
+    // Units of sequence s: row0[s] / 16 + 2 s up to the next one's; n rows touch at most
+    // n / 16 + 2 blocks, so each sequence's blocks fit.
     for (int s = threadIdx.x; s < a.b.nseq; s += AP_THREADS) {
         const int r0 = __ldg(a.b.row0 + s), r1 = __ldg(a.b.row0 + s + 1);
         if (r0 / BLOCK + 2 * s <= unit && unit < r1 / BLOCK + 2 * s + 2 && r1 > r0) {
@@ -107,141 +297,32 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
     const int len = __ldg(a.b.kv_len + s), first = len - n;
     const int blk = first / BLOCK + (unit - r0 / BLOCK - 2 * s);   // block of the sequence
     if (first >= 0 && blk * BLOCK >= len) return;
-    const int page_at = blk / (a.pool.page_tokens / BLOCK);
+    const int per = a.pool.page_tokens / BLOCK;
     int page = -1;
-    if (first >= 0 && blk >= 0 && r0 >= 0 && r0 + n <= a.b.rows && page_at < a.b.max_pages)
-        page = __ldg(a.b.table + (size_t)s * a.b.max_pages + page_at);
+    if (first >= 0 && blk >= 0 && r0 >= 0 && r0 + n <= a.b.rows && blk / per < a.b.max_pages)
+        page = __ldg(a.b.table + (size_t)s * a.b.max_pages + blk / per);
     if (page < 0 || page >= a.pool.pages) {   // the same for every thread
         if (threadIdx.x == 0 && a.err) atomicExch(a.err, DEV_BAD_INDEX);
         return;
     }
-    const size_t bi = block_index(a.pool, page, head, blk % (a.pool.page_tokens / BLOCK));
-    uint8_t *dst = (keys ? a.pool.k : a.pool.v) + bi * (BLOCK * HD);
-    float *scale = (keys ? a.pool.ks : a.pool.vs) + bi;
-    const int lo = max(first - blk * BLOCK, 0), hi = min(len - blk * BLOCK, BLOCK);   // the call's rows of the block
-    // earlier rows and their scale, on their way while the new rows come in
-    uint4 old[PIECES / AP_THREADS + (PIECES % AP_THREADS != 0)];
-    float d_old = 0.f;
-    if (lo > 0) {
-        d_old = *scale;
-#pragma unroll
-        for (int i = 0; i < (PIECES + AP_THREADS - 1) / AP_THREADS; i++) {
-            const int pc = i * AP_THREADS + threadIdx.x;
-            if (pc < PIECES) old[i] = reinterpret_cast<const uint4 *>(dst)[pc];
-        }
-    }
-    // warp w: rows 2w, 2w + 1, 2w + 8, 2w + 9, which are bytes 4w .. 4w + 3 of a value dim
-    float x[AP_ROWS][8];
-    float mx = 0.f;
-    const int pdim = keys && a.freq ? a.pdim : 0;
-#pragma unroll
-    for (int i = 0; i < AP_ROWS; i++) {
-        const int r = 2 * warp + (i & 1) + 8 * (i >> 1);
-        float p[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
-        if (r >= lo && r < hi && lane < U) {
-            const int row = r0 + blk * BLOCK + r - first;
-            const T *src = keys ? (const T *)a.k + (size_t)row * a.ldk : (const T *)a.v + (size_t)row * a.ldv;
-            load_unit<T>(src + (size_t)head * HD, lane, pdim, keys ? a.kvec : a.vvec, p, q);
-            if (lane < pdim / 8) {
-                float c[4], sn[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) angle(blk * BLOCK + r, __ldg(a.freq + 4 * lane + e), c[e], sn[e]);
-                rotate_unit(p, q, c, sn);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            x[i][e] = p[e];
-            x[i][4 + e] = q[e];
-            mx = max_nan(mx, max_nan(fabsf(p[e]), fabsf(q[e])));
-        }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (lane == 0) wmax[warp] = mx;
-    __syncthreads();
-    mx = max_nan(max_nan(wmax[0], wmax[1]), max_nan(wmax[2], wmax[3]));
-    float d = max_nan(__fdiv_rn(mx, E4M3_MAX), SCALE_MIN);
-    if (lo > 0) d = max_nan(d, d_old);
-    if (lo > 0) {   // earlier rows, rounded again where the scale grew; 0 elsewhere
-        const float ratio = d > d_old ? __fdiv_rn(d_old, d) : 1.0f;
-#pragma unroll
-        for (int i = 0; i < (PIECES + AP_THREADS - 1) / AP_THREADS; i++) {
-            const int pc = i * AP_THREADS + threadIdx.x;
-            if (pc >= PIECES) continue;
-            // keys: piece = (8-token group, 16-dim chunk, token): one token; values: one dim's 16 tokens
-            const int ktok = 8 * (pc / (HD / 2)) + (pc & 7);
-            uint32_t w[4] = {old[i].x, old[i].y, old[i].z, old[i].w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t v = 0;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t pr = (w[j] >> (16 * h)) & 0xffffu;
-                    const int t0 = keys ? ktok : order(4 * j + 2 * h), t1 = keys ? ktok : order(4 * j + 2 * h + 1);
-                    uint32_t np = ratio == 1.0f ? pr : e4m3x2(__fmul_rn(e4m3_f32(pr & 0xffu), ratio),
-                                                             __fmul_rn(e4m3_f32(pr >> 8), ratio));
-                    if (t0 >= lo) np &= 0xff00u;
-                    if (t1 >= lo) np &= 0x00ffu;
-                    v |= np << (16 * h);
-                }
-                w[j] = v;
-            }
-            reinterpret_cast<uint4 *>(tile)[keys ? pc : vpiece(pc)] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        __syncthreads();
-    }
-    // the new rows (all of the tile when nothing earlier is in the block)
-    const float inv = __fdiv_rn(1.0f, d);
-    int d0 = 0, d1 = 0;
-    unit_dims(lane, pdim, d0, d1);
-    if (lane < U) {
-        uint32_t q[AP_ROWS][4];   // e4m3 pairs: dims d0, d0 + 1 | d0 + 2, d0 + 3 | d1 .. | ..
-#pragma unroll
-        for (int i = 0; i < AP_ROWS; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) q[i][e] = e4m3x2(__fmul_rn(x[i][2 * e], inv), __fmul_rn(x[i][2 * e + 1], inv));
-        if (keys) {
-#pragma unroll
-            for (int i = 0; i < AP_ROWS; i++) {
-                const int r = 2 * warp + (i & 1) + 8 * (i >> 1);
-                if (r < lo) continue;
-                uint8_t *row = tile + (r >> 3) * (8 * HD) + (r & 7) * 16;
-                *reinterpret_cast<uint32_t *>(row + (d0 >> 4) * 128 + (d0 & 15)) = q[i][0] | (q[i][1] << 16);
-                *reinterpret_cast<uint32_t *>(row + (d1 >> 4) * 128 + (d1 & 15)) = q[i][2] | (q[i][3] << 16);
-            }
-        } else {
-            uint32_t keep = 0;   // bytes that hold earlier rows
-#pragma unroll
-            for (int i = 0; i < AP_ROWS; i++)
-                if (2 * warp + (i & 1) + 8 * (i >> 1) < lo) keep |= 0xffu << (8 * i);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int sh = 8 * (e & 1);
-                uint32_t w = 0;
-#pragma unroll
-                for (int i = 0; i < AP_ROWS; i++) w |= ((q[i][e >> 1] >> sh) & 0xffu) << (8 * i);
-                uint32_t *at = reinterpret_cast<uint32_t *>(tile + 16 * vpiece(e < 4 ? d0 + e : d1 + e - 4)) + warp;
-                *at = keep ? (*at & keep) | (w & ~keep) : w;
-            }
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < (PIECES + AP_THREADS - 1) / AP_THREADS; i++) {
-        const int pc = i * AP_THREADS + threadIdx.x;
-        if (pc < PIECES)
-            reinterpret_cast<uint4 *>(dst)[pc] = reinterpret_cast<const uint4 *>(tile)[keys ? pc : vpiece(pc)];
-    }
-    if (threadIdx.x == 0) *scale = d;
+    const int lo = max(first - blk * BLOCK, 0), hi = min(len - blk * BLOCK, BLOCK), row = r0 + blk * BLOCK - first;
+    if (blockIdx.z == 0) append_block<T, HD, true>(a, page, blk % per, blk, lo, hi, row, tile, turn, wmax);
+    else append_block<T, HD, false>(a, page, blk % per, blk, lo, hi, row, tile, turn, wmax);
 }
 
+template <typename T, int HD>
+cudaError_t launch(AppendArgs a, cudaStream_t s) {
+    const int groups = (a.pool.kv_heads + AP_WIDTH / HD - 1) / (AP_WIDTH / HD);
+    // head groups of a CTA: all of them share a block's angles, as long as the SMs have 16 CTAs each
+    const long long ctas = 2ll * groups * (a.b.rows / BLOCK);
+    const long long most = ctas / (16ll * sm_count());
+    a.passes = most < 1 ? 1 : most < groups ? (int)most : groups;
+    const dim3 grid(a.b.rows / BLOCK + 2 * a.b.nseq, (groups + a.passes - 1) / a.passes, 2);
+    return launch_pdl(append_kernel<T, HD>, grid, dim3(AP_THREADS), 0, s, a);
+}
 template <typename T>
 cudaError_t launch(const AppendArgs &a, cudaStream_t s) {
-    const dim3 grid(a.b.rows / BLOCK + 2 * a.b.nseq, a.pool.kv_heads, 2);
-    if (a.pool.hd == 256) return launch_pdl(append_kernel<T, 256>, grid, dim3(AP_THREADS), 0, s, a);
-    if (a.pool.hd == 128) return launch_pdl(append_kernel<T, 128>, grid, dim3(AP_THREADS), 0, s, a);
-    return launch_pdl(append_kernel<T, 64>, grid, dim3(AP_THREADS), 0, s, a);
+    return a.pool.hd == 256 ? launch<T, 256>(a, s) : a.pool.hd == 128 ? launch<T, 128>(a, s) : launch<T, 64>(a, s);
 }
 
 }  // namespace
@@ -265,8 +346,11 @@ extern "C" int spk_paged_append(const spk_kv_pool *pool, const spk_kv_batch *bat
     const int size = type == T_F32 ? 4 : 2;
     if ((uintptr_t)k % size || (uintptr_t)v % size) return set_error("%s: unaligned rows", who);
     if (pool->kv_heads > 65535) return set_error("%s: %d KV heads", who, pool->kv_heads);
-    AppendArgs a{pool_of(pool), batch_of(batch), k, v, ldk, ldv, rows_aligned(k, ldk, size), rows_aligned(v, ldv, size),
-                 freq, freq ? pdim : 0, device_error_ptr()};
+    auto aligned = [&](const void *p, long long ld) {
+        return !rows_aligned(p, ld, size) ? 0 : (uintptr_t)p % (8 * size) == 0 && ld % 8 == 0 ? 2 : 1;
+    };
+    const AppendArgs a{pool_of(pool), batch_of(batch), k, v, ldk, ldv, aligned(k, ldk), aligned(v, ldv),
+                       freq, freq ? pdim : 0, 1, device_error_ptr()};
     const cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = type == T_F32   ? launch<float>(a, s)
                           : type == T_F16 ? launch<__half>(a, s)
