@@ -45,6 +45,8 @@ namespace {
 
 constexpr int AP_WARPS = 4, AP_THREADS = AP_WARPS * 32, AP_ROWS = BLOCK / AP_WARPS;
 constexpr int AP_WIDTH = 256;              // values of a row that a warp takes at once
+constexpr int AP_CTAS = 6;                 // CTAs of an SM
+constexpr int AP_BLOCKS = 8;               // the most blocks of a CTA
 
 struct AppendArgs {
     Pool pool;
@@ -54,7 +56,7 @@ struct AppendArgs {
     int kvec, vvec;                        // alignment of the rows' pieces: 0 none, 1 four values, 2 eight too
     const float *freq;
     int pdim;
-    int passes;                            // head groups of a CTA
+    int passes, blocks;                    // head groups and blocks of a CTA
     int *err;
 };
 
@@ -76,56 +78,111 @@ __device__ __forceinline__ float2 e4m3x2_f32(uint32_t w) {
     return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
 }
 
-// 8 consecutive values
+// 8 values of a row as they lie in memory: two pieces of 4 (dims d0 .. and d1 ..)
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, int vec, float (&x)[8]) {
-    if constexpr (sizeof(T) == 2) {
-        if (vec == 2) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p));
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+struct Raw {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void load(const T *row, int d0, int d1, int vec) {
+        if (sizeof(T) == 2 && vec == 2 && d1 == d0 + 4) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + d0));
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        } else if (vec) {
+            if constexpr (sizeof(T) == 2) {
+                const uint2 a = __ldg(reinterpret_cast<const uint2 *>(row + d0)), b = __ldg(reinterpret_cast<const uint2 *>(row + d1));
+                w[0] = a.x, w[1] = a.y, w[2] = b.x, w[3] = b.y;
+            } else {
+                const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + d0)), b = __ldg(reinterpret_cast<const uint4 *>(row + d1));
+                w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+                w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const T *p = row + (e < 4 ? d0 + e : d1 + e - 4);
+                if constexpr (sizeof(T) == 4) w[e] = *reinterpret_cast<const uint32_t *>(p);
+                else {
+                    const uint32_t h = *reinterpret_cast<const uint16_t *>(p);
+                    w[e >> 1] = e & 1 ? w[e >> 1] | (h << 16) : h;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int i = 0; i < (int)(2 * sizeof(T)); i++) w[i] = 0;
+    }
+    __device__ __forceinline__ void f32(float (&x)[8]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = __uint_as_float(w[i]);
+        } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 if constexpr (__is_same(T, __half)) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
                     x[2 * i] = f.x, x[2 * i + 1] = f.y;
                 } else {
-                    x[2 * i] = __uint_as_float(u[i] << 16), x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+                    x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
                 }
             }
-            return;
         }
     }
-    const float4 a = load4<T>(p, vec > 0), b = load4<T>(p + 4, vec > 0);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
+};
 
 // 16-byte piece of the staging tile, spread so that a warp's 4-byte writes (pieces 8 apart) meet few banks
 __device__ __forceinline__ int spread(int piece) { return piece ^ ((piece >> 3) & 7); }
 
-// Block `blk` of a sequence (its page's block bp), rows lo .. hi - 1 of it being the call's; row 0
-// of the block would be row `row` of the call.
+// A block that the call appends to: its page and place in it, its first position, the call's rows
+// lo .. hi - 1 of it; row r of the block is row `row` + r of the call. hi 0: no block.
+struct Block {
+    int page, bp, pos, lo, hi, row;
+};
+
 template <typename T, int HD, bool KEYS>
-__device__ __forceinline__ void append_block(const AppendArgs &a, int page, int bp, int blk, int lo, int hi, int row,
-                                             uint8_t *tile, float2 *turn, float (*wmax)[AP_WARPS]) {
+__device__ __forceinline__ void append_blocks(const AppendArgs &a, const Block *blocks, int nb, uint8_t *tile, float2 *turn,
+                                              float (*wmax)[AP_WARPS]) {
     constexpr int LPR = HD / 8, GH = AP_WIDTH / HD, PER = AP_WIDTH / AP_THREADS;   // lanes of a head; heads; pieces of a thread
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPR, u = lane % LPR;
     const int pdim = KEYS ? a.pdim : 0, half = pdim / 2;
     int d0, d1;
     unit_dims(u, pdim, d0, d1);
-    if (KEYS && pdim) {   // the rows' angles, for all heads
-        for (int i = threadIdx.x; i < BLOCK * half; i += AP_THREADS) {
-            const int r = i / half, f = i - r * half;
-            if (r >= lo && r < hi) angle(blk * BLOCK + r, __ldg(a.freq + f), turn[i].x, turn[i].y);
-        }
-        __syncthreads();
-    }
     uint8_t *pool = KEYS ? a.pool.k : a.pool.v;
     float *scales = KEYS ? a.pool.ks : a.pool.vs;
     const T *rows = KEYS ? (const T *)a.k : (const T *)a.v;
     const long long ld = KEYS ? a.ldk : a.ldv;
     const int vec = KEYS ? a.kvec : a.vvec;
-    for (int g = blockIdx.y * a.passes; g < (int)(blockIdx.y + 1) * a.passes && g * GH < a.pool.kv_heads; g++) {
+    const int g0 = blockIdx.y * a.passes, groups = min(a.passes, (a.pool.kv_heads + GH - 1) / GH - g0);
+    // item: a head group of a block; its rows come while the one before is worked on
+    Raw<T> next[AP_ROWS];
+    auto fetch = [&](int it) {
+        const Block &b = blocks[it / groups];
+        const int head = (g0 + it % groups) * GH + sub;
+#pragma unroll
+        for (int i = 0; i < AP_ROWS; i++) {
+            // warp w: rows 2w, 2w + 1, 2w + 8, 2w + 9, which are bytes 4w .. 4w + 3 of a value dim
+            const int r = 2 * warp + (i & 1) + 8 * (i >> 1);
+            if (head < a.pool.kv_heads && r >= b.lo && r < b.hi)
+                next[i].load(rows + (size_t)(b.row + r) * ld + (size_t)head * HD, d0, d1, vec);
+            else next[i].none();
+        }
+    };
+    fetch(0);
+    for (int it = 0; it < nb * groups; it++) {
+        const Block b = blocks[it / groups];
+        const int g = g0 + it % groups, lo = b.lo, hi = b.hi, page = b.page, bp = b.bp;
+        if constexpr (KEYS)
+            if (half && it % groups == 0) {   // the rows' angles, for all heads
+                for (int i = threadIdx.x; i < BLOCK * half; i += AP_THREADS) {
+                    const int r = i / half;
+                    if (r >= lo && r < hi) angle(b.pos + r, __ldg(a.freq + i - r * half), turn[i].x, turn[i].y);
+                }
+                __syncthreads();
+            }
+        float x[AP_ROWS][8];
+#pragma unroll
+        for (int i = 0; i < AP_ROWS; i++) next[i].f32(x[i]);
+        if (it + 1 < nb * groups) fetch(it + 1);
+        if (hi == 0) continue;   // the same for the CTA
         const int head = g * GH + sub;
         const bool real = head < a.pool.kv_heads;
         const size_t bi = block_index(a.pool, page, min(head, a.pool.kv_heads - 1), bp);
@@ -141,27 +198,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, int page, int 
                     old[i] = reinterpret_cast<const uint4 *>(pool + block_index(a.pool, page, hd, bp) * (BLOCK * HD))[pc % HD];
             }
         }
-        // warp w: rows 2w, 2w + 1, 2w + 8, 2w + 9, which are bytes 4w .. 4w + 3 of a value dim
-        float x[AP_ROWS][8];
         float mx = 0.f;
-#pragma unroll
-        for (int i = 0; i < AP_ROWS; i++) {
-            const int r = 2 * warp + (i & 1) + 8 * (i >> 1);
-            if (real && r >= lo && r < hi) {
-                const T *src = rows + (size_t)(row + r) * ld + (size_t)head * HD;
-                if (KEYS) {
-                    float p[4], q[4];
-                    load_unit<T>(src, u, pdim, vec > 0, p, q);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[i][e] = p[e], x[i][4 + e] = q[e];
-                } else {
-                    load8<T>(src + 8 * u, vec, x[i]);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[i][e] = 0.f;
-            }
-        }
         if (KEYS && u < pdim / 8) {
 #pragma unroll
             for (int i = 0; i < AP_ROWS; i++) {
@@ -270,54 +307,59 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, int page, int 
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(AP_THREADS, AP_CTAS) append_kernel(const AppendArgs a) {
     __shared__ __align__(16) uint8_t tile[BLOCK * AP_WIDTH];
     __shared__ __align__(16) float2 turn[BLOCK * HD / 2];
     __shared__ float wmax[AP_WIDTH / HD][AP_WARPS];
-    __shared__ int who[3];               // sequence, its first row, its rows
+    __shared__ int4 who[AP_BLOCKS];      // sequence, its first row, its rows, its cached tokens
+    __shared__ Block blocks[AP_BLOCKS];
     pdl_trigger();
-    if (threadIdx.x == 0) who[0] = -1;
+    if (threadIdx.x < AP_BLOCKS) who[threadIdx.x].x = -1;
     __syncthreads();
     pdl_wait();
-    const int unit = blockIdx.x;
+    const int u0 = blockIdx.x * a.blocks;
     // Units of sequence s: row0[s] / 16 + 2 s up to the next one's; n rows touch at most
     // n / 16 + 2 blocks, so each sequence's blocks fit.
     for (int s = threadIdx.x; s < a.b.nseq; s += AP_THREADS) {
-        const int r0 = __ldg(a.b.row0 + s), r1 = __ldg(a.b.row0 + s + 1);
-        if (r0 / BLOCK + 2 * s <= unit && unit < r1 / BLOCK + 2 * s + 2 && r1 > r0) {
-            who[0] = s;
-            who[1] = r0;
-            who[2] = r1 - r0;
-        }
+        const int r0 = __ldg(a.b.row0 + s), r1 = __ldg(a.b.row0 + s + 1), len = __ldg(a.b.kv_len + s);
+        const int b0 = r0 / BLOCK + 2 * s, b1 = r1 / BLOCK + 2 * s + 2;
+        if (r1 > r0)
+            for (int u = max(b0, u0); u < min(b1, u0 + a.blocks); u++) who[u - u0] = make_int4(s, r0, r1 - r0, len);
     }
     __syncthreads();
-    const int s = who[0];
-    if (s < 0) return;
-    const int r0 = who[1], n = who[2];
-    const int len = __ldg(a.b.kv_len + s), first = len - n;
-    const int blk = first / BLOCK + (unit - r0 / BLOCK - 2 * s);   // block of the sequence
-    if (first >= 0 && blk * BLOCK >= len) return;
-    const int per = a.pool.page_tokens / BLOCK;
-    int page = -1;
-    if (first >= 0 && blk >= 0 && r0 >= 0 && r0 + n <= a.b.rows && blk / per < a.b.max_pages)
-        page = __ldg(a.b.table + (size_t)s * a.b.max_pages + blk / per);
-    if (page < 0 || page >= a.pool.pages) {   // the same for every thread
-        if (threadIdx.x == 0 && a.err) atomicExch(a.err, DEV_BAD_INDEX);
-        return;
+    if (threadIdx.x < a.blocks) {
+        const int4 w = who[threadIdx.x];
+        const int first = w.w - w.z, blk = first / BLOCK + (u0 + (int)threadIdx.x - w.y / BLOCK - 2 * w.x);
+        const int per = a.pool.page_tokens / BLOCK;
+        Block b{0, 0, 0, 0, 0, 0};
+        if (w.x >= 0 && (first < 0 || blk * BLOCK < w.w)) {
+            int page = -1;
+            if (first >= 0 && blk >= 0 && w.y >= 0 && w.y + w.z <= a.b.rows && blk / per < a.b.max_pages)
+                page = __ldg(a.b.table + (size_t)w.x * a.b.max_pages + blk / per);
+            if (page >= 0 && page < a.pool.pages)
+                b = Block{page, blk % per, blk * BLOCK, max(first - blk * BLOCK, 0), min(w.w - blk * BLOCK, BLOCK),
+                          w.y + blk * BLOCK - first};
+            else if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
+        }
+        blocks[threadIdx.x] = b;
     }
-    const int lo = max(first - blk * BLOCK, 0), hi = min(len - blk * BLOCK, BLOCK), row = r0 + blk * BLOCK - first;
-    if (blockIdx.z == 0) append_block<T, HD, true>(a, page, blk % per, blk, lo, hi, row, tile, turn, wmax);
-    else append_block<T, HD, false>(a, page, blk % per, blk, lo, hi, row, tile, turn, wmax);
+    __syncthreads();
+    if (blockIdx.z == 0) append_blocks<T, HD, true>(a, blocks, a.blocks, tile, turn, wmax);
+    else append_blocks<T, HD, false>(a, blocks, a.blocks, tile, turn, wmax);
 }
 
 template <typename T, int HD>
 cudaError_t launch(AppendArgs a, cudaStream_t s) {
     const int groups = (a.pool.kv_heads + AP_WIDTH / HD - 1) / (AP_WIDTH / HD);
-    // head groups of a CTA: all of them share a block's angles, as long as the SMs have 16 CTAs each
-    const long long ctas = 2ll * groups * (a.b.rows / BLOCK);
-    const long long most = ctas / (16ll * sm_count());
+    // A CTA takes all head groups of a block, and then up to AP_BLOCKS blocks, as long as every SM
+    // still gets its CTAs: the groups share a block's angles, the blocks hide each other's loads.
+    const int slots = AP_CTAS * sm_count(), units = a.b.rows / BLOCK;   // whole blocks: about what there is to do
+    long long most = 2ll * groups * units / slots;
     a.passes = most < 1 ? 1 : most < groups ? (int)most : groups;
-    const dim3 grid(a.b.rows / BLOCK + 2 * a.b.nseq, (groups + a.passes - 1) / a.passes, 2);
+    a.passes = (groups + (groups + a.passes - 1) / a.passes - 1) / ((groups + a.passes - 1) / a.passes);
+    most /= groups;
+    a.blocks = most < 1 ? 1 : most < AP_BLOCKS ? (int)most : AP_BLOCKS;
+    const dim3 grid((a.b.rows / BLOCK + 2 * a.b.nseq + a.blocks - 1) / a.blocks, (groups + a.passes - 1) / a.passes, 2);
     return launch_pdl(append_kernel<T, HD>, grid, dim3(AP_THREADS), 0, s, a);
 }
 template <typename T>
@@ -350,7 +392,7 @@ extern "C" int spk_paged_append(const spk_kv_pool *pool, const spk_kv_batch *bat
         return !rows_aligned(p, ld, size) ? 0 : (uintptr_t)p % (8 * size) == 0 && ld % 8 == 0 ? 2 : 1;
     };
     const AppendArgs a{pool_of(pool), batch_of(batch), k, v, ldk, ldv, aligned(k, ldk), aligned(v, ldv),
-                       freq, freq ? pdim : 0, 1, device_error_ptr()};
+                       freq, freq ? pdim : 0, 1, 1, device_error_ptr()};
     const cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = type == T_F32   ? launch<float>(a, s)
                           : type == T_F16 ? launch<__half>(a, s)
