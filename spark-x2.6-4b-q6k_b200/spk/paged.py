@@ -187,6 +187,14 @@ class PagedBatch:
         self._pool_p, self._batch_p, self._attn_p = C.addressof(cache._c), C.addressof(self._b), C.addressof(self._a)
         self._append, self._attn = L.spk_paged_append, L.spk_paged_attn
 
+    def use(self, cache: PagedCache) -> None:
+        """Turns the batch to another layer's pool of the same geometry (the page table is the layers' own)."""
+        c = self.cache
+        if (cache.pages, cache.page_tokens, cache.kv_heads, cache.head_dim, cache.device) != (
+                c.pages, c.page_tokens, c.kv_heads, c.head_dim, c.device):
+            raise SpkError("a pool of another geometry")
+        self.cache, self._pool_p = cache, C.addressof(cache._c)
+
     def append(self, k, v, freq=None, stream=None) -> None:
         """Rows k, v [rows][kv_heads * head_dim] (views of a wider matrix are fine) into the pages;
         keys are rotated over their first 2 * len(freq) dims when freq is given."""
