@@ -46,6 +46,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int TILE = 128, TB = TILE / BLOCK;   // keys of a tile, its blocks
 constexpr int SEG_COST = 16;          // a group's fixed cost in blocks
 constexpr int Q_WARPS = 4;
+constexpr int SQ = 4;                 // groups known ahead
 
 struct AttnParams {
     Pool pool;
@@ -62,29 +63,31 @@ struct AttnParams {
     int *err;
 };
 
-// N columns, T terms, R rows a tile (T R <= N), SG softmax warpgroups
-template <int HD_, int N_, int T_, int R_>
+// N columns, T terms, R rows a tile (T R <= N). SG warpgroups share a tile's rows (wide tiles: more
+// warps hide the softmax's latencies); PG sets of them take the groups in turn (narrow tiles: one
+// set's last products and outputs run beside the next one's first scores).
+template <int HD_, int N_, int T_, int R_, int SG_, int PG_>
 struct Cfg {
-    static constexpr int HD = HD_, N = N_, T = T_, R = R_;
-    static constexpr int SG = N >= 128 ? 2 : 1;
+    static constexpr int HD = HD_, N = N_, T = T_, R = R_, SG = SG_, PG = PG_;
     static constexpr int RG = R / SG;                         // rows of a warpgroup, side by side
-    static constexpr int CH = SG == 1 ? R : RG % 8 ? 4 : 8;   // rows handled together
+    static constexpr int CH = SG == 1 ? R : 8;                // rows handled together
     static constexpr int NC = RG / CH;
-    static constexpr int LD = SG == 1 ? 8 : CH;               // columns of a tensor-memory access
+    static constexpr int LD = 8;                              // columns of a tensor-memory access
     static constexpr int LC = SG == 1 ? (T * R + 7) / 8 * 8 : CH * T;   // columns of a chunk: all, or CH a term
     static constexpr int KB = BLOCK * HD;                     // bytes of a block's keys (or values)
     static constexpr int STAGE = 2 * TB * KB;
-    static constexpr int NST = N >= 128 ? (HD == 256 ? 2 : HD == 128 ? 4 : 6) : (HD == 256 ? 3 : HD == 128 ? 6 : 8);
+    static constexpr int NST = N >= 96 ? (HD == 256 ? 2 : HD == 128 ? 4 : 6) : (HD == 256 ? 3 : HD == 128 ? 6 : 8);
     // P: 16 keys of every column, then the next 16, 64 bytes further than they need so that the byte
     // stores of a warp's two runs of 16 keys meet different banks. One buffer where two do not fit.
-    static constexpr int PK = N * 16 + 64, PB = TILE / 16 * PK, NP = N >= 128 && HD == 256 ? 1 : 2;
+    static constexpr int PK = N * 16 + 64, PB = TILE / 16 * PK, NP = N >= 96 && HD == 256 ? 1 : 2;
     static constexpr int HH = HD == 256 ? 2 : 1;              // 128-dim halves of the output
-    static constexpr int TCOLS = (2 + HH) * N <= 64 ? 64 : (2 + HH) * N <= 128 ? 128 : (2 + HH) * N <= 256 ? 256 : 512;
+    static constexpr int TC = (2 + HH * PG) * N, TCOLS = TC <= 64 ? 64 : TC <= 128 ? 128 : TC <= 256 ? 256 : 512;
+    static constexpr int MW = 160 * (SG == 1 ? 1 : 4);        // weights that a merge of parts holds at once
     static constexpr size_t Q_OFF = (size_t)NST * STAGE, P_OFF = Q_OFF + (size_t)2 * N * HD;
     static constexpr size_t SMEM = P_OFF + (size_t)NP * PB;
-    static constexpr int WARPS = 2 + Q_WARPS + 4 * SG, THREADS = WARPS * 32;
+    static constexpr int WARPS = 2 + Q_WARPS + 4 * SG * PG, THREADS = WARPS * 32;
     static constexpr int PART = (R * (HD + 2) + 3) / 4 * 4;   // floats of a partial: O, then m, then l; read 16 bytes at a time
-    static_assert(T * R <= N && R % SG == 0 && RG % CH == 0, "");
+    static_assert(T * R <= N && TC <= 512 && R % SG == 0 && RG % CH == 0, "");
     // access x of chunk ch of warpgroup sg: its column
     static __device__ __forceinline__ int col(int sg, int ch, int x) { return SG == 1 ? 8 * x : x * R + sg * RG + ch * CH; }
     static constexpr int TS = SG == 1 ? R : CH;               // a chunk's terms lie this far apart
@@ -111,26 +114,16 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
 // K columns of this thread's lane; tm_wait before their use
 template <int K>
 __device__ __forceinline__ void tm_ld(uint32_t addr, float *v) {
-    static_assert(K == 4 || K == 8, "");
-    if constexpr (K == 4)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
-                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                     : "r"(addr));
-    else
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-                     : "r"(addr));
+    static_assert(K == 8, "");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "r"(addr));
 }
 template <int K>
 __device__ __forceinline__ void tm_st(uint32_t addr, const float *v) {
-    if constexpr (K == 4)
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0,%1,%2,%3};" ::"f"(v[0]), "f"(v[1]), "f"(v[2]),
-                     "f"(v[3]), "r"(addr)
-                     : "memory");
-    else
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"f"(v[0]), "f"(v[1]),
-                     "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "r"(addr)
-                     : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"f"(v[0]), "f"(v[1]),
+                 "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "r"(addr)
+                 : "memory");
 }
 // The loads have landed; their registers pass through, so no use of them moves up.
 template <int K>
@@ -326,23 +319,28 @@ template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a) {
     constexpr int HD = C::HD, N = C::N, TT = C::T, R = C::R, NST = C::NST, QB = 2, NP = C::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint64_t full_k[NST], full_v[NST], empty[NST], s_full[2], p_full[2], pv_done[2], q_full[QB], q_empty[QB];
+    __shared__ uint64_t full_k[NST], full_v[NST], empty[NST], p_full[2], pv_done[2], q_full[QB], q_empty[QB];
+    // a set waits on barriers that only its own tiles move, or on ones that its tile's scores imply: a wait by
+    // parity must not start more than a phase early or end more than one late
+    __shared__ uint64_t s_full[C::PG][2];
+    __shared__ uint64_t seg_full[SQ], seg_empty[SQ], o_full[C::PG];   // o_full: a group's sums are complete
+    __shared__ Seg segs[SQ];                            // the CTA's groups, as warp 0 finds them; k0 < 0: no more
     __shared__ float2 scales[NST][TB];                  // dk, dv of a tile's blocks
     __shared__ uint32_t pre[MAX_SEQ + 1], wsum[C::WARPS];
     __shared__ float q_up[4];                           // score factor of a query tile: the softmax may be two behind
     __shared__ int dead;                                // a wait ran out: what follows no longer waits
-    __shared__ float red[C::SG][4][C::RG];              // per row: the warps' maxima, then their sums
-    __shared__ __align__(16) float mref[C::SG][(C::RG + 3) / 4 * 4];   // per row: the reference m
-    __shared__ uint32_t moved[C::SG][4];                // the warps' chunks whose reference has to move
-    __shared__ __align__(16) float fs[C::SG][(C::RG + 3) / 4 * 4];     // per row: a factor for all of its outputs
-    __shared__ int pos_s[R];                            // per row: position, -1 past the tile's last row
-    __shared__ size_t out_s[R];                         // per row: where its output lies
+    constexpr int G = C::SG * C::PG;
+    __shared__ float red[G][4][C::RG];                  // per row: the warps' maxima, then their sums
+    __shared__ __align__(16) float mref[G][(C::RG + 3) / 4 * 4];   // per row: the reference m
+    __shared__ uint32_t moved[G][4];                    // the warps' chunks whose reference has to move
+    __shared__ __align__(16) float fs[G][(C::RG + 3) / 4 * 4];     // per row: a factor for all of its outputs
+    __shared__ int pos_s[C::PG][R];                     // per row: position, -1 past the tile's last row
+    __shared__ size_t out_s[C::PG][R];                  // per row: where its output lies
+    __shared__ float merge_s[C::PG][2 * C::MW];         // a row's weights of the parts, and their sums before
     __shared__ float amax_s[Q_WARPS];
-    __shared__ int last_in;
+    __shared__ int last_in[C::PG];
     __shared__ uint32_t tmem_s;
     __shared__ Walk walk_s;                             // the walk behind the CTA's first group
-    __shared__ Seg first_s;
-    __shared__ bool some;
     uint8_t *qs = smem + C::Q_OFF, *ps = smem + C::P_OFF;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -353,7 +351,6 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(s_full + i, 1);
             mbar_init(p_full + i, 4 * C::SG);
             mbar_init(pv_done + i, 1);
         }
@@ -361,8 +358,17 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             mbar_init(q_full + i, Q_WARPS);
             mbar_init(q_empty + i, 1);
         }
+        for (int i = 0; i < C::PG; i++) {
+            mbar_init(&s_full[i][0], 1);
+            mbar_init(&s_full[i][1], 1);
+            mbar_init(o_full + i, 1);
+        }
+        for (int i = 0; i < SQ; i++) {
+            mbar_init(seg_full + i, 1);
+            mbar_init(seg_empty + i, 1 + Q_WARPS + 4 * C::SG * C::PG);
+        }
         dead = 0;
-        some = false;
+        segs[0].k0 = -1;
         fence_mbar_init();
     }
     if (warp == 1) {   // this warp owns the tensor memory
@@ -417,20 +423,36 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             w.x1 = min(base, x0 + chunk);
             walk_at(a, pre, s, R, w);
             Seg g;
-            some = walk_next(a, pre, R, w, g);
+            if (walk_next(a, pre, R, w, g)) segs[0] = g;
             walk_s = w;
-            first_s = g;
         }
     __syncthreads();
-    Walk w = walk_s;
-    Seg g = first_s;
-    bool more = some;
-    if (!more) {
+    // group n of the CTA, for the warps that follow warp 0; false: there is none. A dead CTA walks on.
+    auto group = [&](uint32_t n, Seg &g) {
+        if (n > 0 && !mbar_wait(seg_full + n % SQ, (n / SQ) & 1, a.err)) return false;
+        g = segs[n % SQ];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(seg_empty + n % SQ);
+        return g.k0 >= 0;
+    };
+    Seg g;
+    if (segs[0].k0 < 0) {
     } else if (warp == 0) {   // ------------------------------------------------------ copies
         // lane l < 8: the keys and values of a tile's block l; its page comes one tile ahead
         const int per = a.pool.page_tokens / BLOCK;
         uint32_t i = 0;
-        for (; more; more = walk_next(a, pre, R, w, g)) {
+        Walk w = walk_s;
+        g = segs[0];
+        if (lane == 0) mbar_arrive(seg_full);   // group 0 is there
+        for (uint32_t n = 1; g.k0 >= 0; n++) {
+            Seg nx;
+            if (!walk_next(a, pre, R, w, nx)) nx.k0 = -1;
+            if (n >= SQ) mbar_wait(seg_empty + n % SQ, ((n / SQ) - 1) & 1, a.err);
+            __syncwarp();
+            if (lane == 0) {
+                segs[n % SQ] = nx;
+                mbar_arrive(seg_full + n % SQ);
+            }
             const int blk0 = g.start / BLOCK, nblk = g.nblk, k1 = g.k1, kvh = g.kvh;
             const int *table = a.b.table + (size_t)g.s * a.b.max_pages;
             auto page_of = [&](int k) {
@@ -476,6 +498,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     mbar_arrive(full_k + st);
                 }
             }
+            g = nx;
         }
         if (*(volatile int *)&dead)   // copies in flight land before the CTA's memory goes
             for (uint32_t x = i > NST ? i - NST : 0; x < i; x++)
@@ -491,9 +514,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             const uint64_t vdesc = smem_desc(smem_u32(smem) + TB * C::KB, C::KB, 128);
             const uint64_t pdesc = smem_desc(smem_u32(ps), C::PK, 128);
             uint32_t i = 0, qi = 0;   // tiles whose scores were issued; groups
+            uint32_t sets[C::PG] = {};   // tiles of each set
             // the tile whose values come next: its place, blocks, and whether it is its group's first
-            bool have = false, pfirst = false;
-            int pnb = 0;
+            bool have = false, pfirst = false, plast = false;
+            int pnb = 0, po = 0;
             uint32_t pi = 0;
             auto values = [&]() {   // PV of tile pi
                 const int st = pi % NST;
@@ -507,13 +531,28 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     if (2 * kk < pnb)
 #pragma unroll
                         for (int h = 0; h < C::HH; h++)
-                            mma_e4m3(oo + h * N, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * (2 * C::PK / 16), idesc,
+                            mma_e4m3(oo + (po + h) * N, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * (2 * C::PK / 16), idesc,
                                      !pfirst || kk > 0);
                 mma_commit(pv_done + (pi & 1));
+                if (plast) mma_commit(o_full + po / C::HH);
                 mma_commit(empty + st);
             };
-            for (; more; more = walk_next(a, pre, R, w, g)) {
-                if (g.nblk == 0) continue;
+            for (uint32_t n = 0;; n++) {
+                // a tile's values wait for the next tile's scores, but not for a group that is not there yet or
+                // has no tile: whoever is to make room for one may be waiting for them
+                if (n > 0 && !mbar_try_wait(seg_full + n % SQ, (n / SQ) & 1)) {
+                    if (have) values();
+                    have = false;
+                    if (!mbar_wait(seg_full + n % SQ, (n / SQ) & 1, a.err)) break;
+                }
+                g = segs[n % SQ];
+                mbar_arrive(seg_empty + n % SQ);
+                if (g.k0 < 0) break;
+                if (g.nblk == 0) {
+                    if (have) values();
+                    have = false;
+                    continue;
+                }
                 const int qb = qi % QB, k0 = g.k0, k1 = g.k1, nblk = g.nblk;
                 const bool q_here = wait_for(q_full + qb, (qi / QB) & 1, &dead, a.err);
                 const uint64_t qd = qdesc + (uint32_t)(qb * (N * HD / 16));
@@ -525,7 +564,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
 #pragma unroll
                         for (int kk = 0; kk < HD / 32; kk++)
                             mma_e4m3(so + (i & 1) * N, kd + kk * 16, qd + kk * 16, idesc, kk > 0);
-                        mma_commit(s_full + (i & 1));
+#pragma unroll
+                        for (int x = 0; x < C::PG; x++)
+                            if (x == (int)(n % C::PG)) mma_commit(&s_full[x][sets[x]++ & 1]);
                         if (k + 1 == k1) mma_commit(q_empty + qb);
                     }
                     if (have) values();
@@ -533,6 +574,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     pi = i;
                     pnb = min(TB, nblk - k * TB);
                     pfirst = k == k0;
+                    plast = k + 1 == k1;
+                    po = (n % C::PG) * C::HH;
                     i++;
                 }
                 qi++;
@@ -542,7 +585,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     } else if (warp < 2 + Q_WARPS) {   // ------------------------------------------------- queries
         const int qw = warp - 2;
         uint32_t qi = 0;
-        for (; more; more = walk_next(a, pre, R, w, g)) {
+        for (uint32_t n = 0; group(n, g); n++) {
             if (g.nblk == 0) continue;
             const int qb = qi % QB, c0 = g.c0, c1 = g.c1, pos0 = g.pos0;
             const T *q0 = (const T *)a.q + (size_t)g.r0 * a.ldq + (size_t)g.kvh * a.group * HD;
@@ -588,7 +631,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             }
             mx = warp_max(mx);
             if (lane == 0) amax_s[qw] = mx;
-            bar_sync(3, Q_WARPS * 32);
+            bar_sync(5, Q_WARPS * 32);
 #pragma unroll
             for (int e = 0; e < Q_WARPS; e++) mx = fmaxf(mx, amax_s[e]);
             // times 2^(6 - e), so that it lies in [64, 128); a tile of zeros stays
@@ -634,20 +677,26 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full + qb);
-            bar_sync(3, Q_WARPS * 32);   // amax_s is free again
+            bar_sync(5, Q_WARPS * 32);   // amax_s is free again
             qi++;
         }
     } else {   // ------------------------------------------------------ softmax, outputs
-        const int sg = (warp - 2 - Q_WARPS) >> 2, q4 = warp & 3;   // warpgroup; the warp's lane quarter
-        const int key = 32 * q4 + lane, bid = 1 + sg;
+        const int wg = (warp - 2 - Q_WARPS) >> 2, sg = wg % C::SG, pg = wg / C::SG;   // warpgroup: its rows, its turn
+        const int q4 = warp & 3, key = 32 * q4 + lane, bid = 1 + wg;                 // the warp's lane quarter
         const uint32_t lane_at = (uint32_t)(32 * q4) << 16;
         // byte of this key in a column of P: values lie in the order of paged.cuh
         const int kbyte = (key >> 4) * C::PK + place(key & 15);
         constexpr int RG = C::RG, CH = C::CH, LC = C::LC, LD = C::LD, TS = C::TS;
-        float *mr = mref[sg];
-        uint32_t i = 0, qi = 0;
-        for (; more; more = walk_next(a, pre, R, w, g)) {
+        float *mr = mref[wg];
+        uint32_t i = 0, qi = 0, mine_i = 0, own = 0;   // tiles and groups with tiles so far; those of this set
+        for (uint32_t n = 0; group(n, g); n++) {
             const int k0 = g.k0, k1 = g.nblk > 0 ? g.k1 : k0, nblk = g.nblk, start = g.start;
+            if ((int)(n % C::PG) != pg) {   // the other set's
+                i += k1 - k0;
+                qi += k1 > k0;
+                continue;
+            }
+            const uint32_t otm = tmem + lane_at + (2 + pg * C::HH) * N;   // the group's sums
             const int p_lo = g.p_lo, p_hi = g.p_hi, see0 = g.see0, window = a.window;
             const int row = sg * RG + key, c = g.c0 + row;   // the row that this thread keeps the books of
             const bool mine = key < RG && c <= g.c1;
@@ -655,8 +704,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             if (key < RG) {
                 const int tok = c / a.group, hq = g.kvh * a.group + c % a.group;
                 mr[key] = 0.f;
-                pos_s[row] = mine ? g.pos0 + tok : -1;
-                out_s[row] = (size_t)(g.r0 + tok) * a.ldout + (size_t)hq * HD;
+                pos_s[pg][row] = mine ? g.pos0 + tok : -1;
+                out_s[pg][row] = (size_t)(g.r0 + tok) * a.ldout + (size_t)hq * HD;
                 if (a.gate && mine) sig = to_f32(((const T *)a.gate)[(size_t)(g.r0 + tok) * a.ldgate + hq]);
             }
             float l[RG];
@@ -665,12 +714,13 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             bar_sync(bid, 128);
             for (int k = k0; k < k1; k++, i++) {
                 const int st = i % NST, nb = min(TB, nblk - k * TB);
-                wait_for(full_k + st, (i / NST) & 1, &dead, a.err);   // the scales
-                const float2 sc = scales[st][key >> 4];
-                const float fb = log2f(sc.y), isv = 1.0f / sc.y;
-                wait_for(s_full + (i & 1), (i >> 1) & 1, &dead, a.err);
+                wait_for(&s_full[pg][mine_i & 1], (mine_i >> 1) & 1, &dead, a.err);
+                wait_for(full_k + st, (i / NST) & 1, &dead, a.err);   // the scales: there, since the scores are
+                mine_i++;
                 __syncwarp();
                 tc_after();
+                const float2 sc = scales[st][key >> 4];
+                const float fb = log2f(sc.y), isv = 1.0f / sc.y;
                 const int j0 = start + k * TILE, j = j0 + key;
                 const float fa = sc.x * q_up[qi & 3];
                 const bool edge = j0 + TILE - 1 > p_lo || (window > 0 && j0 <= p_hi - window);
@@ -693,7 +743,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 if (edge) {
 #pragma unroll
                     for (int r = 0; r < RG; r++) {
-                        const int p = pos_s[sg * RG + r];
+                        const int p = pos_s[pg][sg * RG + r];
                         if (j > p || (window > 0 && j <= p - window)) t[r] = -INFINITY;
                     }
                 }
@@ -713,30 +763,30 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 const bool first = k == k0;
                 if (bar_or(bid, 128, first || over != 0)) {
                     over = first ? (1u << C::NC) - 1u : __reduce_or_sync(0xffffffffu, over);
-                    if (lane == 0) moved[sg][q4] = over;
+                    if (lane == 0) moved[wg][q4] = over;
 #pragma unroll
                     for (int ch = 0; ch < C::NC; ch++)
                         if (over >> ch & 1u)   // the warp's largest; a chunk that only another warp flags moves with its own
 #pragma unroll
                             for (int r = 0; r < CH; r++) {
                                 const float x = warp_max(t[ch * CH + r]);
-                                if (lane == 0) red[sg][q4][ch * CH + r] = x;
+                                if (lane == 0) red[wg][q4][ch * CH + r] = x;
                             }
                         else if (lane == 0)
 #pragma unroll
-                            for (int r = 0; r < CH; r++) red[sg][q4][ch * CH + r] = -INFINITY;
+                            for (int r = 0; r < CH; r++) red[wg][q4][ch * CH + r] = -INFINITY;
                     bar_sync(bid, 128);
-                    over = moved[sg][0] | moved[sg][1] | moved[sg][2] | moved[sg][3];
+                    over = moved[wg][0] | moved[wg][1] | moved[wg][2] | moved[wg][3];
                     if (key < RG) {   // to W_TOP below the largest
-                        const float x = fmaxf(fmaxf(red[sg][0][key], red[sg][1][key]), fmaxf(red[sg][2][key], red[sg][3][key]));
+                        const float x = fmaxf(fmaxf(red[wg][0][key], red[wg][1][key]), fmaxf(red[wg][2][key], red[wg][3][key]));
                         const float up = !first ? (x > W_MAX ? x - W_TOP : 0.f) : x == -INFINITY ? 0.f : x - W_TOP;
-                        fs[sg][key] = up;
+                        fs[wg][key] = up;
                         mr[key] += up;
                     }
                     bar_sync(bid, 128);
 #pragma unroll
                     for (int r = 0; r < RG; r++) {
-                        const float up = fs[sg][r];
+                        const float up = fs[wg][r];
                         t[r] -= up;
                         if (!first) l[r] *= ex2(-up);
                     }
@@ -752,17 +802,17 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                                 float v[LC];
 #pragma unroll
                                 for (int x = 0; x < LC / LD; x++)
-                                    tm_ld<LD>(tmem + lane_at + (2 + h) * N + C::col(sg, ch, x), v + LD * x);
+                                    tm_ld<LD>(otm + h * N + C::col(sg, ch, x), v + LD * x);
                                 tm_wait(v);
 #pragma unroll
                                 for (int r = 0; r < TS; r++) {
-                                    const float f = ex2(-fs[sg][ch * CH + r]);
+                                    const float f = ex2(-fs[wg][ch * CH + r]);
 #pragma unroll
                                     for (int x = r; x < LC; x += TS) v[x] *= f;
                                 }
 #pragma unroll
                                 for (int x = 0; x < LC / LD; x++)
-                                    tm_st<LD>(tmem + lane_at + (2 + h) * N + C::col(sg, ch, x), v + LD * x);
+                                    tm_st<LD>(otm + h * N + C::col(sg, ch, x), v + LD * x);
                             }
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -829,23 +879,24 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
 #pragma unroll
             for (int r = 0; r < RG; r++) {
                 const float x = warp_sum(l[r]);
-                if (lane == 0) red[sg][q4][r] = x;
+                if (lane == 0) red[wg][q4][r] = x;
             }
             bar_sync(bid, 128);
             const bool whole = g.f0 == g.f1;
             float *slot = a.part + ((size_t)blockIdx.x * 2 + (g.k0 == 0 ? 1 : 0)) * C::PART;
             sig = a.gate ? 1.0f + __expf(-sig) : 1.0f;   // 1 / sigmoid
             if (key < RG) {
-                const float L = (red[sg][0][key] + red[sg][1][key]) + (red[sg][2][key] + red[sg][3][key]);
+                const float L = (red[wg][0][key] + red[wg][1][key]) + (red[wg][2][key] + red[wg][3][key]);
                 // a row (or part) that saw nothing: its products are 0 or were not made
-                fs[sg][key] = L == 0.f ? 0.f : whole ? 1.0f / (L * sig) : 1.0f;
+                fs[wg][key] = L == 0.f ? 0.f : whole ? 1.0f / (L * sig) : 1.0f;
                 if (!whole && mine) {
                     slot[R * HD + row] = L == 0.f ? M_NONE : mr[key];
                     slot[R * HD + R + row] = L;
                 }
             }
             bar_sync(bid, 128);
-            if (k1 > k0) wait_for(pv_done + ((i - 1) & 1), ((i - 1) >> 1) & 1, &dead, a.err);
+            // not pv_done: the other set's tiles may have moved that on twice
+            if (k1 > k0) wait_for(o_full + pg, own++ & 1, &dead, a.err);
             __syncwarp();
             tc_after();
             const int rows = g.c1 - g.c0 + 1;
@@ -855,7 +906,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 float v[LC];
 #pragma unroll
                 for (int x = 0; x < LC / LD; x++)
-                    tm_ld<LD>(tmem + lane_at + (2 + h) * N + C::col(sg, ch, x), v + LD * x);
+                    tm_ld<LD>(otm + h * N + C::col(sg, ch, x), v + LD * x);
                 tm_wait(v);
 #pragma unroll
                 for (int r = 0; r < CH; r++) {
@@ -863,43 +914,41 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
 #pragma unroll
                     for (int x = TT - 2; x >= 0; x--) o = fmaf(o, 1.0f / STEP, v[x * TS + r]);
                     const int rr = ch * CH + r, ro = sg * RG + rr;
-                    const float f = fs[sg][rr];
+                    const float f = fs[wg][rr];
                     if (d >= HD || ro >= rows) continue;
                     o = f == 0.f ? 0.f : o * f;
-                    if (whole) ((T *)a.out)[out_s[ro] + d] = from_f32<T>(o);
+                    if (whole) ((T *)a.out)[out_s[pg][ro] + d] = from_f32<T>(o);
                     else slot[(size_t)ro * HD + d] = o;
                 }
             }
             if (!whole) {   // the last CTA of the group adds all parts in CTA order
                 const int parts = g.f1 - g.f0 + 1;
                 constexpr int ST = 128 * C::SG;
-                bar_sync(4, ST);
+                bar_sync(6 + pg, ST);
                 if (sg == 0 && key == 0) {
                     __threadfence();   // for all of them: their stores came before the barrier
                     const bool last = atomicAdd(a.tickets + g.f0, 1u) == (unsigned)(parts - 1);
                     if (last) a.tickets[g.f0] = 0u;
                     __threadfence();
-                    last_in = last;
+                    last_in[pg] = last;
                 }
-                bar_sync(4, ST);
-                if (last_in) {
+                bar_sync(6 + pg, ST);
+                if (last_in[pg]) {
                     const size_t step = (size_t)2 * C::PART;
                     const float *p0 = a.part + (size_t)g.f0 * step;   // CTA f0: slot 1, the others: slot 0
                     auto part = [&](int p) { return p0 + p * step + (p == 0 ? C::PART : 0); };
-                    // P is at rest: the parts' weights of a row, and their sums before
-                    constexpr int room = NP * C::PB / 8;
-                    float *wt = reinterpret_cast<float *>(ps), *wl = wt + room;
-                    const int RB = min(R, room / parts);   // rows that fit (at least 2)
+                    float *wt = merge_s[pg], *wl = wt + C::MW;
+                    const int RB = min(R, C::MW / parts);   // rows whose weights fit (at least one: 160 parts)
                     for (int r0 = 0; r0 < rows; r0 += RB) {
                         const int nr = min(RB, rows - r0);
-                        if (key < RG && row >= r0 && row < r0 + nr) red[sg][0][key] = sig;
+                        if (key < RG && row >= r0 && row < r0 + nr) red[wg][0][key] = sig;
                         for (int x = sg * 128 + key; x < nr * parts; x += ST) {
                             const int p = x / nr, r = x - p * nr;
                             const float *pp = part(p) + R * HD + r0 + r;
                             wt[r * parts + p] = __ldcg(pp);
                             wl[r * parts + p] = __ldcg(pp + R);
                         }
-                        bar_sync(4, ST);
+                        bar_sync(6 + pg, ST);
                         for (int r = sg * 4 + q4; r < nr; r += 4 * C::SG) {   // a warp per row
                             float M = M_NONE, L = 0.f;
                             for (int p = lane; p < parts; p += 32) M = fmaxf(M, wt[r * parts + p]);
@@ -910,10 +959,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                                 L = fmaf(wl[r * parts + p], f, L);
                             }
                             L = warp_sum(L);
-                            const float f = L == 0.f ? 0.f : 1.0f / (L * red[(r0 + r) / RG][0][(r0 + r) % RG]);
+                            const float f = L == 0.f ? 0.f : 1.0f / (L * red[pg * C::SG + (r0 + r) / RG][0][(r0 + r) % RG]);
                             for (int p = lane; p < parts; p += 32) wt[r * parts + p] *= f;
                         }
-                        bar_sync(4, ST);
+                        bar_sync(6 + pg, ST);
                         const int items = nr * (HD / 4);
                         for (int x = sg * 128 + key; x < items; x += ST) {
                             const int r = x / (HD / 4), d = 4 * (x - r * (HD / 4));
@@ -933,13 +982,13 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                                     O.w = fmaf(v[p].w, f, O.w);
                                 }
                             }
-                            T *dst = (T *)a.out + out_s[r0 + r] + d;
+                            T *dst = (T *)a.out + out_s[pg][r0 + r] + d;
                             dst[0] = from_f32<T>(O.x);
                             dst[1] = from_f32<T>(O.y);
                             dst[2] = from_f32<T>(O.z);
                             dst[3] = from_f32<T>(O.w);
                         }
-                        bar_sync(4, ST);   // the weights and last_in are free again
+                        bar_sync(6 + pg, ST);   // the weights and last_in are free again
                     }
                 }
             }
@@ -955,7 +1004,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     }
 }
 
-constexpr size_t TICKETS = 1024;   // bytes before the partials: one word per CTA (at most 256)
+constexpr size_t TICKETS = 1024;   // bytes before the partials: one word per CTA
 constexpr int MAX_R = 64;
 
 template <typename T, typename C>
@@ -984,13 +1033,13 @@ template <typename T, int HD>
 int launch(const AttnParams &a, cudaStream_t s, const char *who) {
     const long long per = ((long long)a.b.rows * a.group + a.b.nseq - 1) / a.b.nseq;
     if constexpr (sizeof(T) == 4) {
-        if (per <= 6) return launch_one<T, Cfg<HD, 32, 5, 6>>(a, s, who);
-        return launch_one<T, Cfg<HD, 128, 5, 24>>(a, s, who);
+        if (per <= 6) return launch_one<T, Cfg<HD, 32, 5, 6, 1, 2>>(a, s, who);
+        return launch_one<T, Cfg<HD, 128, 5, 24, 3, 1>>(a, s, who);
     } else {
-        if (per <= 5) return launch_one<T, Cfg<HD, 16, 3, 5>>(a, s, who);
-        if (per <= 10) return launch_one<T, Cfg<HD, 32, 3, 10>>(a, s, who);
-        if constexpr (__is_same(T, __half)) return launch_one<T, Cfg<HD, 128, 3, 40>>(a, s, who);
-        else return launch_one<T, Cfg<HD, 128, 2, 64>>(a, s, who);
+        if (per <= 5) return launch_one<T, Cfg<HD, 16, 3, 5, 1, 2>>(a, s, who);
+        if (per <= 10) return launch_one<T, Cfg<HD, 32, 3, 10, 1, 2>>(a, s, who);
+        if constexpr (__is_same(T, __half)) return launch_one<T, Cfg<HD, 96, 3, 32, 4, 1>>(a, s, who);
+        else return launch_one<T, Cfg<HD, 128, 2, 64, 4, 1>>(a, s, who);
     }
 }
 
@@ -1033,7 +1082,7 @@ int spk_paged_attn(const spk_kv_pool *pool, const spk_kv_batch *batch, const spk
     if ((uintptr_t)p->q % size || (uintptr_t)p->out % size || (uintptr_t)p->gate % size)
         return set_error("%s: unaligned rows", who);
     if ((uintptr_t)p->workspace % 16) return set_error("%s: the workspace is not 16-byte aligned", who);
-    if (sm_count() > (int)(TICKETS / 4)) return set_error("%s: a device of %d SMs", who, sm_count());
+    if (sm_count() > 160) return set_error("%s: a device of %d SMs", who, sm_count());
     AttnParams a;
     a.pool = pool_of(pool);
     a.b = batch_of(batch);
