@@ -47,6 +47,7 @@ constexpr int TILE = 128, TB = TILE / BLOCK;   // keys of a tile, its blocks
 constexpr int SEG_COST = 16;          // a group's fixed cost in blocks
 constexpr int Q_WARPS = 4;
 constexpr int SQ = 4;                 // groups known ahead
+constexpr int SCR = 16;               // tiles whose scales are kept: more than the copies are ahead of the softmax
 
 struct AttnParams {
     Pool pool;
@@ -75,15 +76,17 @@ struct Cfg {
     static constexpr int LD = 8;                              // columns of a tensor-memory access
     static constexpr int LC = SG == 1 ? (T * R + 7) / 8 * 8 : CH * T;   // columns of a chunk: all, or CH a term
     static constexpr int KB = BLOCK * HD;                     // bytes of a block's keys (or values)
-    static constexpr int STAGE = 2 * TB * KB;
-    static constexpr int NST = N >= 96 ? (HD == 256 ? 2 : HD == 128 ? 4 : 6) : (HD == 256 ? 3 : HD == 128 ? 6 : 8);
+    static constexpr int SLOT = TB * KB;                      // a tile's keys (or values)
+    // slots of keys and of values: a tile's keys are done with its scores, its values much later
+    static constexpr int NK = N >= 96 ? (HD == 256 ? 2 : 4) : HD == 256 ? 3 : HD == 128 ? 6 : 8;
+    static constexpr int NV = N >= 96 ? (HD == 256 ? 1 : 2) : NK;
     // P: 16 keys of every column, then the next 16, 64 bytes further than they need so that the byte
-    // stores of a warp's two runs of 16 keys meet different banks. One buffer where two do not fit.
-    static constexpr int PK = N * 16 + 64, PB = TILE / 16 * PK, NP = N >= 96 && HD == 256 ? 1 : 2;
+    // stores of a warp's two runs of 16 keys meet different banks.
+    static constexpr int PK = N * 16 + 64, PB = TILE / 16 * PK, NP = 2;
     static constexpr int HH = HD == 256 ? 2 : 1;              // 128-dim halves of the output
     static constexpr int TC = (2 + HH * PG) * N, TCOLS = TC <= 64 ? 64 : TC <= 128 ? 128 : TC <= 256 ? 256 : 512;
     static constexpr int MW = 160 * (SG == 1 ? 1 : 4);        // weights that a merge of parts holds at once
-    static constexpr size_t Q_OFF = (size_t)NST * STAGE, P_OFF = Q_OFF + (size_t)2 * N * HD;
+    static constexpr size_t V_OFF = (size_t)NK * SLOT, Q_OFF = V_OFF + (size_t)NV * SLOT, P_OFF = Q_OFF + (size_t)2 * N * HD;
     static constexpr size_t SMEM = P_OFF + (size_t)NP * PB;
     static constexpr int WARPS = 2 + Q_WARPS + 4 * SG * PG, THREADS = WARPS * 32;
     static constexpr int PART = (R * (HD + 2) + 3) / 4 * 4;   // floats of a partial: O, then m, then l; read 16 bytes at a time
@@ -206,9 +209,6 @@ __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, int *de
     if (err) atomicExch(err, DEV_WAIT_TIMEOUT);
     return false;
 }
-__device__ __forceinline__ void mbar_expect(uint64_t *bar, uint32_t bytes) {
-    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ bool bar_or(int id, int n, bool x) {
     uint32_t r;
@@ -317,15 +317,15 @@ __device__ __noinline__ bool walk_next(const AttnParams &a, const uint32_t *pre,
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a) {
-    constexpr int HD = C::HD, N = C::N, TT = C::T, R = C::R, NST = C::NST, QB = 2, NP = C::NP;
+    constexpr int HD = C::HD, N = C::N, TT = C::T, R = C::R, NK = C::NK, NV = C::NV, QB = 2, NP = C::NP;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint64_t full_k[NST], full_v[NST], empty[NST], p_full[2], pv_done[2], q_full[QB], q_empty[QB];
+    __shared__ uint64_t full_k[NK], empty_k[NK], full_v[NV], empty_v[NV], sc_full[SCR], p_full[2], pv_done[2], q_full[QB], q_empty[QB];
     // a set waits on barriers that only its own tiles move, or on ones that its tile's scores imply: a wait by
     // parity must not start more than a phase early or end more than one late
     __shared__ uint64_t s_full[C::PG][2];
     __shared__ uint64_t seg_full[SQ], seg_empty[SQ], o_full[C::PG];   // o_full: a group's sums are complete
     __shared__ Seg segs[SQ];                            // the CTA's groups, as warp 0 finds them; k0 < 0: no more
-    __shared__ float2 scales[NST][TB];                  // dk, dv of a tile's blocks
+    __shared__ float2 scales[SCR][TB];                  // dk, dv of a tile's blocks
     __shared__ uint32_t pre[MAX_SEQ + 1], wsum[C::WARPS];
     __shared__ float q_up[4];                           // score factor of a query tile: the softmax may be two behind
     __shared__ int dead;                                // a wait ran out: what follows no longer waits
@@ -345,11 +345,15 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     if (tid == 0) {
-        for (int i = 0; i < NST; i++) {
+        for (int i = 0; i < NK; i++) {
             mbar_init(full_k + i, 1);
-            mbar_init(full_v + i, 1);
-            mbar_init(empty + i, 1);
+            mbar_init(empty_k + i, 1);
         }
+        for (int i = 0; i < NV; i++) {
+            mbar_init(full_v + i, 1);
+            mbar_init(empty_v + i, 1);
+        }
+        for (int i = 0; i < SCR; i++) mbar_init(sc_full + i, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(p_full + i, 4 * C::SG);
             mbar_init(pv_done + i, 1);
@@ -441,6 +445,22 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
         // lane l < 8: the keys and values of a tile's block l; its page comes one tile ahead
         const int per = a.pool.page_tokens / BLOCK;
         uint32_t i = 0;
+        size_t vbi = 0;   // the last tile's blocks, whose values are still to come
+        int vnb = 0;
+        auto copy_values = [&](uint32_t t) {
+            uint64_t *full = full_v + t % NV;
+            uint8_t *vd = smem + C::V_OFF + (size_t)(t % NV) * C::SLOT;
+            if (t >= NV && !wait_for(empty_v + t % NV, ((t / NV) - 1) & 1, &dead, a.err)) return;
+            if (vnb & 1) {   // the MMAs take values by two blocks: the missing one is 0
+                for (int o = 16 * lane; o < C::KB; o += 512)
+                    *reinterpret_cast<uint4 *>(vd + vnb * C::KB + o) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(full, vnb * C::KB);
+            __syncwarp();
+            if (lane < vnb) bulk_g2s(vd + lane * C::KB, a.pool.v + vbi * C::KB, C::KB, full);
+        };
         Walk w = walk_s;
         g = segs[0];
         if (lane == 0) mbar_arrive(seg_full);   // group 0 is there
@@ -468,42 +488,35 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             };
             int page = page_of(g.k0);
             for (int k = g.k0; k < k1 && nblk > 0; k++) {
-                const int nb = min(TB, nblk - k * TB), st = i % NST;
+                const int nb = min(TB, nblk - k * TB);
                 const size_t bi = block_index(a.pool, page, kvh, (blk0 + k * TB + lane) % per);
                 float2 sc = make_float2(0.f, 1.f);
                 if (lane < nb) sc = make_float2(__ldg(a.pool.ks + bi), __ldg(a.pool.vs + bi));
                 page = page_of(k + 1);
-                const bool free_ = i < NST || wait_for(empty + st, ((i / NST) - 1) & 1, &dead, a.err);
+                if (i < NK || wait_for(empty_k + i % NK, ((i / NK) - 1) & 1, &dead, a.err)) {
+                    if (lane == 0) mbar_arrive_expect_tx(full_k + i % NK, nb * C::KB);
+                    __syncwarp();
+                    if (lane < nb)
+                        bulk_g2s(smem + (size_t)(i % NK) * C::SLOT + lane * C::KB, a.pool.k + bi * C::KB, C::KB, full_k + i % NK);
+                }
+                if (lane < TB) scales[i % SCR][lane] = sc;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sc_full + i % SCR);
+                if (vnb) copy_values(i - 1);   // behind the next tile's keys, which are wanted first
+                vbi = bi;
+                vnb = nb;
                 i++;
-                if (!__all_sync(0xffffffffu, free_)) continue;
-                uint8_t *kd = smem + (size_t)st * C::STAGE, *vd = kd + TB * C::KB;
-                if (nb & 1) {   // the MMAs take values by two blocks: the missing one is 0
-                    for (int o = 16 * lane; o < C::KB; o += 512)
-                        *reinterpret_cast<uint4 *>(vd + nb * C::KB + o) = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async();
-                }
-                if (lane == 0) {
-                    mbar_expect(full_k + st, nb * C::KB);
-                    mbar_expect(full_v + st, nb * C::KB);
-                }
-                __syncwarp();
-                if (lane < nb) {
-                    bulk_g2s(kd + lane * C::KB, a.pool.k + bi * C::KB, C::KB, full_k + st);
-                    bulk_g2s(vd + lane * C::KB, a.pool.v + bi * C::KB, C::KB, full_v + st);
-                    scales[st][lane] = sc;
-                }
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(full_v + st);
-                    mbar_arrive(full_k + st);
-                }
             }
             g = nx;
+            if (vnb && (g.k0 < 0 || g.nblk == 0)) {   // no tile follows at once
+                copy_values(i - 1);
+                vnb = 0;
+            }
         }
         if (*(volatile int *)&dead)   // copies in flight land before the CTA's memory goes
-            for (uint32_t x = i > NST ? i - NST : 0; x < i; x++)
-                for (uint32_t y = 0; y < (1u << 20) && !(mbar_try_wait(full_k + x % NST, (x / NST) & 1) &&
-                                                        mbar_try_wait(full_v + x % NST, (x / NST) & 1)); y++) {}
+            for (uint32_t x = i > 2 ? i - 2 : 0; x < i; x++)
+                for (uint32_t y = 0; y < (1u << 20) && !(mbar_try_wait(full_k + x % NK, (x / NK) & 1) &&
+                                                        mbar_try_wait(full_v + x % NV, (x / NV) & 1)); y++) {}
     } else if (warp == 1) {   // ------------------------------------------------------ MMAs
         if (lane == 0) {
             const uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
@@ -511,7 +524,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             // descriptors move by their address field alone
             const uint64_t kdesc = smem_desc(smem_u32(smem), 128, 8 * HD);
             const uint64_t qdesc = smem_desc(smem_u32(qs), 128, 8 * HD);
-            const uint64_t vdesc = smem_desc(smem_u32(smem) + TB * C::KB, C::KB, 128);
+            const uint64_t vdesc = smem_desc(smem_u32(smem) + (uint32_t)C::V_OFF, C::KB, 128);
             const uint64_t pdesc = smem_desc(smem_u32(ps), C::PK, 128);
             uint32_t i = 0, qi = 0;   // tiles whose scores were issued; groups
             uint32_t sets[C::PG] = {};   // tiles of each set
@@ -520,12 +533,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             int pnb = 0, po = 0;
             uint32_t pi = 0;
             auto values = [&]() {   // PV of tile pi
-                const int st = pi % NST;
+                const int st = pi % NV;
                 if (!wait_for(p_full + (pi & 1), (pi >> 1) & 1, &dead, a.err) ||
-                    !wait_for(full_v + st, (pi / NST) & 1, &dead, a.err))
+                    !wait_for(full_v + st, (pi / NV) & 1, &dead, a.err))
                     return;
                 tc_after();
-                const uint64_t vd = vdesc + (uint32_t)(st * (C::STAGE / 16)), pd = pdesc + (uint32_t)((pi % NP) * (C::PB / 16));
+                const uint64_t vd = vdesc + (uint32_t)(st * (C::SLOT / 16)), pd = pdesc + (uint32_t)((pi % NP) * (C::PB / 16));
 #pragma unroll
                 for (int kk = 0; kk < TB / 2; kk++)
                     if (2 * kk < pnb)
@@ -535,7 +548,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                                      !pfirst || kk > 0);
                 mma_commit(pv_done + (pi & 1));
                 if (plast) mma_commit(o_full + po / C::HH);
-                mma_commit(empty + st);
+                mma_commit(empty_v + st);
             };
             for (uint32_t n = 0;; n++) {
                 // a tile's values wait for the next tile's scores, but not for a group that is not there yet or
@@ -557,16 +570,17 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 const bool q_here = wait_for(q_full + qb, (qi / QB) & 1, &dead, a.err);
                 const uint64_t qd = qdesc + (uint32_t)(qb * (N * HD / 16));
                 for (int k = k0; k < k1; k++) {
-                    const int st = i % NST;
-                    if (wait_for(full_k + st, (i / NST) & 1, &dead, a.err) && q_here) {
+                    const int st = i % NK;
+                    if (wait_for(full_k + st, (i / NK) & 1, &dead, a.err) && q_here) {
                         tc_after();
-                        const uint64_t kd = kdesc + (uint32_t)(st * (C::STAGE / 16));
+                        const uint64_t kd = kdesc + (uint32_t)(st * (C::SLOT / 16));
 #pragma unroll
                         for (int kk = 0; kk < HD / 32; kk++)
                             mma_e4m3(so + (i & 1) * N, kd + kk * 16, qd + kk * 16, idesc, kk > 0);
 #pragma unroll
                         for (int x = 0; x < C::PG; x++)
                             if (x == (int)(n % C::PG)) mma_commit(&s_full[x][sets[x]++ & 1]);
+                        mma_commit(empty_k + st);
                         if (k + 1 == k1) mma_commit(q_empty + qb);
                     }
                     if (have) values();
@@ -713,13 +727,13 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             for (int r = 0; r < RG; r++) l[r] = 0.f;
             bar_sync(bid, 128);
             for (int k = k0; k < k1; k++, i++) {
-                const int st = i % NST, nb = min(TB, nblk - k * TB);
+                const int nb = min(TB, nblk - k * TB);
                 wait_for(&s_full[pg][mine_i & 1], (mine_i >> 1) & 1, &dead, a.err);
-                wait_for(full_k + st, (i / NST) & 1, &dead, a.err);   // the scales: there, since the scores are
+                wait_for(sc_full + i % SCR, (i / SCR) & 1, &dead, a.err);
                 mine_i++;
                 __syncwarp();
                 tc_after();
-                const float2 sc = scales[st][key >> 4];
+                const float2 sc = scales[i % SCR][key >> 4];
                 const float fb = log2f(sc.y), isv = 1.0f / sc.y;
                 const int j0 = start + k * TILE, j = j0 + key;
                 const float fa = sc.x * q_up[qi & 3];
@@ -842,9 +856,11 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 // never meets the product
                 const int past = j0 + nb * BLOCK - 1 - p_hi, under = see0 - j0;
                 if (past > 0 || under > 0) {
-                    wait_for(full_v + st, (i / NST) & 1, &dead, a.err);
+                    // one slot: its tile before has to be done with, or the wait reads a phase too early
+                    if (NV == 1 && i > 0) wait_for(pv_done + ((i - 1) & 1), ((i - 1) >> 1) & 1, &dead, a.err);
+                    wait_for(full_v + i % NV, (i / NV) & 1, &dead, a.err);
                     if (sg == 0) {
-                        uint8_t *vb = smem + (size_t)st * C::STAGE + TB * C::KB;
+                        uint8_t *vb = smem + C::V_OFF + (size_t)(i % NV) * C::SLOT;
 #pragma unroll 1
                         for (int e = 0; e < 2; e++) {
                             const int bad = e == 0 ? under : past, blk = e == 0 ? 0 : nb - 1;
