@@ -29,7 +29,8 @@
 // that several CTAs share leaves (O, m, l) in the workspace; the last CTA to arrive (a ticket that it
 // resets) adds the parts in CTA order.
 //
-// Warps: 0 bulk copies (pages, scales), 1 MMA issue, 2-5 queries of the next group, 6.. softmax:
+// Warps: 0 the groups and the copies of keys and scales, 1 MMA issue, 2 the copies of values, 3-6 the
+// queries of the next group, 7.. softmax:
 // a thread per key, and per output dim at the end of a group.
 #include "paged.cuh"
 
@@ -45,7 +46,7 @@ constexpr float STEP = 32.0f;         // a term's scale over the one before: hal
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int TILE = 128, TB = TILE / BLOCK;   // keys of a tile, its blocks
 constexpr int SEG_COST = 16;          // a group's fixed cost in blocks
-constexpr int Q_WARPS = 4;
+constexpr int FIRST_Q = 3, Q_WARPS = 4;   // the warps of the queries
 constexpr int SQ = 4;                 // groups known ahead
 constexpr int SCR = 16;               // tiles whose scales are kept: more than the copies are ahead of the softmax
 
@@ -88,7 +89,8 @@ struct Cfg {
     static constexpr int MW = 160 * (SG == 1 ? 1 : 4);        // weights that a merge of parts holds at once
     static constexpr size_t V_OFF = (size_t)NK * SLOT, Q_OFF = V_OFF + (size_t)NV * SLOT, P_OFF = Q_OFF + (size_t)2 * N * HD;
     static constexpr size_t SMEM = P_OFF + (size_t)NP * PB;
-    static constexpr int WARPS = 2 + Q_WARPS + 4 * SG * PG, THREADS = WARPS * 32;
+    static constexpr int LAG = PG == 1 ? 2 : 1;               // tiles that the values are behind the scores
+    static constexpr int WARPS = FIRST_Q + Q_WARPS + 4 * SG * PG, THREADS = WARPS * 32;
     static constexpr int PART = (R * (HD + 2) + 3) / 4 * 4;   // floats of a partial: O, then m, then l; read 16 bytes at a time
     static_assert(T * R <= N && TC <= 512 && R % SG == 0 && RG % CH == 0, "");
     // access x of chunk ch of warpgroup sg: its column
@@ -197,16 +199,37 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// The phase of that parity is over; sleeps up to a while before it says no, so that 20 waiting warps leave
+// the issue slots to those that work.
+__device__ __forceinline__ bool mbar_sleep(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+constexpr unsigned long long WAIT_NS = 4000000000ull;   // the longest wait
 // Bounded wait. The first one that runs out records the error and marks the CTA dead; from then on
 // waits return at once, copies and MMAs are no longer issued, and every warp still walks its range, so
 // that none is left at a barrier.
 __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, int *dead, int *err) {
-    for (uint32_t i = 0; i < SPK_WAIT_LIMIT; i++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 255u) == 255u && *(volatile int *)dead) return false;
+    if (mbar_sleep(bar, parity)) return true;
+    const unsigned long long t0 = now_ns();
+    while (!(dead && *(volatile int *)dead)) {
+        if (mbar_sleep(bar, parity)) return true;
+        if (now_ns() - t0 > WAIT_NS) {
+            if (dead) *(volatile int *)dead = 1;
+            if (err) atomicExch(err, DEV_WAIT_TIMEOUT);
+            break;
+        }
     }
-    *(volatile int *)dead = 1;
-    if (err) atomicExch(err, DEV_WAIT_TIMEOUT);
     return false;
 }
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
@@ -369,7 +392,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
         }
         for (int i = 0; i < SQ; i++) {
             mbar_init(seg_full + i, 1);
-            mbar_init(seg_empty + i, 1 + Q_WARPS + 4 * C::SG * C::PG);
+            mbar_init(seg_empty + i, 2 + Q_WARPS + 4 * C::SG * C::PG);
         }
         dead = 0;
         segs[0].k0 = -1;
@@ -433,66 +456,54 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     __syncthreads();
     // group n of the CTA, for the warps that follow warp 0; false: there is none. A dead CTA walks on.
     auto group = [&](uint32_t n, Seg &g) {
-        if (n > 0 && !mbar_wait(seg_full + n % SQ, (n / SQ) & 1, a.err)) return false;
+        if (n > 0 && !wait_for(seg_full + n % SQ, (n / SQ) & 1, nullptr, a.err)) return false;
         g = segs[n % SQ];
         __syncwarp();
         if (lane == 0) mbar_arrive(seg_empty + n % SQ);
         return g.k0 >= 0;
     };
+    // the tiles of a group for a warp that copies: lane l < 8 has block l, whose page comes one tile ahead
+    const int per = a.pool.page_tokens / BLOCK;
+    auto copy_group = [&](const Seg &g, auto &&tile) {
+        const int blk0 = g.start / BLOCK, nblk = g.nblk, k1 = g.k1, kvh = g.kvh;
+        const int *table = a.b.table + (size_t)g.s * a.b.max_pages;
+        auto page_of = [&](int k) {
+            int page = 0;
+            if (k < k1 && lane < min(TB, nblk - k * TB)) {
+                page = __ldg(table + (blk0 + k * TB + lane) / per);
+                if (page < 0 || page >= a.pool.pages) {
+                    if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
+                    page = 0;
+                }
+            }
+            return page;
+        };
+        int page = page_of(g.k0);
+        for (int k = g.k0; k < k1 && nblk > 0; k++) {
+            const size_t bi = block_index(a.pool, page, kvh, (blk0 + k * TB + lane) % per);
+            page = page_of(k + 1);
+            tile(min(TB, nblk - k * TB), bi);
+        }
+    };
     Seg g;
     if (segs[0].k0 < 0) {
-    } else if (warp == 0) {   // ------------------------------------------------------ copies
-        // lane l < 8: the keys and values of a tile's block l; its page comes one tile ahead
-        const int per = a.pool.page_tokens / BLOCK;
+    } else if (warp == 0) {   // ------------------------------------------------------ groups, keys, scales
         uint32_t i = 0;
-        size_t vbi = 0;   // the last tile's blocks, whose values are still to come
-        int vnb = 0;
-        auto copy_values = [&](uint32_t t) {
-            uint64_t *full = full_v + t % NV;
-            uint8_t *vd = smem + C::V_OFF + (size_t)(t % NV) * C::SLOT;
-            if (t >= NV && !wait_for(empty_v + t % NV, ((t / NV) - 1) & 1, &dead, a.err)) return;
-            if (vnb & 1) {   // the MMAs take values by two blocks: the missing one is 0
-                for (int o = 16 * lane; o < C::KB; o += 512)
-                    *reinterpret_cast<uint4 *>(vd + vnb * C::KB + o) = make_uint4(0, 0, 0, 0);
-                fence_proxy_async();
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive_expect_tx(full, vnb * C::KB);
-            __syncwarp();
-            if (lane < vnb) bulk_g2s(vd + lane * C::KB, a.pool.v + vbi * C::KB, C::KB, full);
-        };
         Walk w = walk_s;
         g = segs[0];
         if (lane == 0) mbar_arrive(seg_full);   // group 0 is there
         for (uint32_t n = 1; g.k0 >= 0; n++) {
             Seg nx;
             if (!walk_next(a, pre, R, w, nx)) nx.k0 = -1;
-            if (n >= SQ) mbar_wait(seg_empty + n % SQ, ((n / SQ) - 1) & 1, a.err);
+            if (n >= SQ) wait_for(seg_empty + n % SQ, ((n / SQ) - 1) & 1, nullptr, a.err);
             __syncwarp();
             if (lane == 0) {
                 segs[n % SQ] = nx;
                 mbar_arrive(seg_full + n % SQ);
             }
-            const int blk0 = g.start / BLOCK, nblk = g.nblk, k1 = g.k1, kvh = g.kvh;
-            const int *table = a.b.table + (size_t)g.s * a.b.max_pages;
-            auto page_of = [&](int k) {
-                int page = 0;
-                if (k < k1 && lane < min(TB, nblk - k * TB)) {
-                    page = __ldg(table + (blk0 + k * TB + lane) / per);
-                    if (page < 0 || page >= a.pool.pages) {
-                        if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
-                        page = 0;
-                    }
-                }
-                return page;
-            };
-            int page = page_of(g.k0);
-            for (int k = g.k0; k < k1 && nblk > 0; k++) {
-                const int nb = min(TB, nblk - k * TB);
-                const size_t bi = block_index(a.pool, page, kvh, (blk0 + k * TB + lane) % per);
+            copy_group(g, [&](int nb, size_t bi) {
                 float2 sc = make_float2(0.f, 1.f);
                 if (lane < nb) sc = make_float2(__ldg(a.pool.ks + bi), __ldg(a.pool.vs + bi));
-                page = page_of(k + 1);
                 if (i < NK || wait_for(empty_k + i % NK, ((i / NK) - 1) & 1, &dead, a.err)) {
                     if (lane == 0) mbar_arrive_expect_tx(full_k + i % NK, nb * C::KB);
                     __syncwarp();
@@ -502,21 +513,35 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 if (lane < TB) scales[i % SCR][lane] = sc;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sc_full + i % SCR);
-                if (vnb) copy_values(i - 1);   // behind the next tile's keys, which are wanted first
-                vbi = bi;
-                vnb = nb;
                 i++;
-            }
+            });
             g = nx;
-            if (vnb && (g.k0 < 0 || g.nblk == 0)) {   // no tile follows at once
-                copy_values(i - 1);
-                vnb = 0;
-            }
         }
         if (*(volatile int *)&dead)   // copies in flight land before the CTA's memory goes
-            for (uint32_t x = i > 2 ? i - 2 : 0; x < i; x++)
-                for (uint32_t y = 0; y < (1u << 20) && !(mbar_try_wait(full_k + x % NK, (x / NK) & 1) &&
-                                                        mbar_try_wait(full_v + x % NV, (x / NV) & 1)); y++) {}
+            for (uint32_t x = i > NK ? i - NK : 0; x < i; x++)
+                for (uint32_t y = 0; y < (1u << 20) && !mbar_try_wait(full_k + x % NK, (x / NK) & 1); y++) {}
+    } else if (warp == 2) {   // ------------------------------------------------------ values
+        uint32_t i = 0;
+        for (uint32_t n = 0; group(n, g); n++)
+            copy_group(g, [&](int nb, size_t bi) {
+                uint64_t *full = full_v + i % NV;
+                uint8_t *vd = smem + C::V_OFF + (size_t)(i % NV) * C::SLOT;
+                if (i < NV || wait_for(empty_v + i % NV, ((i / NV) - 1) & 1, &dead, a.err)) {
+                    if (nb & 1) {   // the MMAs take values by two blocks: the missing one is 0
+                        for (int o = 16 * lane; o < C::KB; o += 512)
+                            *reinterpret_cast<uint4 *>(vd + nb * C::KB + o) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async();
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_expect_tx(full, nb * C::KB);
+                    __syncwarp();
+                    if (lane < nb) bulk_g2s(vd + lane * C::KB, a.pool.v + bi * C::KB, C::KB, full);
+                }
+                i++;
+            });
+        if (*(volatile int *)&dead)
+            for (uint32_t x = i > NV ? i - NV : 0; x < i; x++)
+                for (uint32_t y = 0; y < (1u << 20) && !mbar_try_wait(full_v + x % NV, (x / NV) & 1); y++) {}
     } else if (warp == 1) {   // ------------------------------------------------------ MMAs
         if (lane == 0) {
             const uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
@@ -526,51 +551,65 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             const uint64_t qdesc = smem_desc(smem_u32(qs), 128, 8 * HD);
             const uint64_t vdesc = smem_desc(smem_u32(smem) + (uint32_t)C::V_OFF, C::KB, 128);
             const uint64_t pdesc = smem_desc(smem_u32(ps), C::PK, 128);
-            uint32_t i = 0, qi = 0;   // tiles whose scores were issued; groups
+            uint32_t i = 0, qi = 0;   // tiles whose scores were issued; groups with tiles
             uint32_t sets[C::PG] = {};   // tiles of each set
-            // the tile whose values come next: its place, blocks, and whether it is its group's first
-            bool have = false, pfirst = false, plast = false;
-            int pnb = 0, po = 0;
-            uint32_t pi = 0;
-            auto values = [&]() {   // PV of tile pi
-                const int st = pi % NV;
-                if (!wait_for(p_full + (pi & 1), (pi >> 1) & 1, &dead, a.err) ||
-                    !wait_for(full_v + st, (pi / NV) & 1, &dead, a.err))
-                    return;
+            // Up to LAG tiles' values are still to come. A wide tile's scores go before the values of the tile two
+            // before it, into the buffer that its softmax has just left, so that the softmax finds them ready; a
+            // narrow tile waits for memory, and its values leave their slot sooner.
+            struct Late {
+                uint32_t i;           // tile
+                int nb, po;           // its blocks, where its sums lie
+                bool first, last;     // of its group
+            } late[2] = {};
+            int nlate = 0;
+            auto weights = [&]() {    // of the oldest late tile: there
+                const bool ok = wait_for(p_full + (late[0].i & 1), (late[0].i >> 1) & 1, &dead, a.err);
                 tc_after();
-                const uint64_t vd = vdesc + (uint32_t)(st * (C::SLOT / 16)), pd = pdesc + (uint32_t)((pi % NP) * (C::PB / 16));
+                return ok;
+            };
+            auto values = [&](bool ok) {   // of the oldest late tile, whose weights are there
+                const Late t = late[0];
+                late[0] = late[1];
+                nlate--;
+                const int st = t.i % NV;
+                if (!wait_for(full_v + st, (t.i / NV) & 1, &dead, a.err) || !ok) return;
+                tc_after();
+                const uint64_t vd = vdesc + (uint32_t)(st * (C::SLOT / 16)), pd = pdesc + (uint32_t)((t.i % NP) * (C::PB / 16));
 #pragma unroll
                 for (int kk = 0; kk < TB / 2; kk++)
-                    if (2 * kk < pnb)
+                    if (2 * kk < t.nb)
 #pragma unroll
                         for (int h = 0; h < C::HH; h++)
-                            mma_e4m3(oo + (po + h) * N, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * (2 * C::PK / 16), idesc,
-                                     !pfirst || kk > 0);
-                mma_commit(pv_done + (pi & 1));
-                if (plast) mma_commit(o_full + po / C::HH);
+                            mma_e4m3(oo + (t.po + h) * N, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * (2 * C::PK / 16),
+                                     idesc, !t.first || kk > 0);
+                mma_commit(pv_done + (t.i & 1));
+                if (t.last) mma_commit(o_full + t.po / C::HH);
                 mma_commit(empty_v + st);
             };
+            auto flush = [&]() {
+                while (nlate) values(weights());
+            };
             for (uint32_t n = 0;; n++) {
-                // a tile's values wait for the next tile's scores, but not for a group that is not there yet or
-                // has no tile: whoever is to make room for one may be waiting for them
+                // but not behind a group that is not there yet or has no tile: whoever is to make room for one
+                // may be waiting for them
                 if (n > 0 && !mbar_try_wait(seg_full + n % SQ, (n / SQ) & 1)) {
-                    if (have) values();
-                    have = false;
-                    if (!mbar_wait(seg_full + n % SQ, (n / SQ) & 1, a.err)) break;
+                    flush();
+                    if (!wait_for(seg_full + n % SQ, (n / SQ) & 1, nullptr, a.err)) break;
                 }
                 g = segs[n % SQ];
                 mbar_arrive(seg_empty + n % SQ);
                 if (g.k0 < 0) break;
                 if (g.nblk == 0) {
-                    if (have) values();
-                    have = false;
+                    flush();
                     continue;
                 }
                 const int qb = qi % QB, k0 = g.k0, k1 = g.k1, nblk = g.nblk;
+                if (!mbar_try_wait(q_full + qb, (qi / QB) & 1)) flush();
                 const bool q_here = wait_for(q_full + qb, (qi / QB) & 1, &dead, a.err);
                 const uint64_t qd = qdesc + (uint32_t)(qb * (N * HD / 16));
                 for (int k = k0; k < k1; k++) {
                     const int st = i % NK;
+                    const bool there = nlate < 2 || weights();   // with LAG 2: then its scores' buffer is free, too
                     if (wait_for(full_k + st, (i / NK) & 1, &dead, a.err) && q_here) {
                         tc_after();
                         const uint64_t kd = kdesc + (uint32_t)(st * (C::SLOT / 16));
@@ -583,21 +622,16 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                         mma_commit(empty_k + st);
                         if (k + 1 == k1) mma_commit(q_empty + qb);
                     }
-                    if (have) values();
-                    have = true;
-                    pi = i;
-                    pnb = min(TB, nblk - k * TB);
-                    pfirst = k == k0;
-                    plast = k + 1 == k1;
-                    po = (n % C::PG) * C::HH;
+                    if (nlate == C::LAG) values(C::LAG == 2 ? there : weights());
+                    late[nlate++] = Late{i, min(TB, nblk - k * TB), (int)(n % C::PG) * C::HH, k == k0, k + 1 == k1};
                     i++;
                 }
                 qi++;
             }
-            if (have) values();
+            flush();
         }
-    } else if (warp < 2 + Q_WARPS) {   // ------------------------------------------------- queries
-        const int qw = warp - 2;
+    } else if (warp < FIRST_Q + Q_WARPS) {   // ------------------------------------------------- queries
+        const int qw = warp - FIRST_Q;
         uint32_t qi = 0;
         for (uint32_t n = 0; group(n, g); n++) {
             if (g.nblk == 0) continue;
@@ -687,7 +721,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     }
                 }
             }
-            if (tid == 64) q_up[qi & 3] = up * a.scale;
+            if (qw == 0 && lane == 0) q_up[qi & 3] = up * a.scale;
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full + qb);
@@ -695,7 +729,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             qi++;
         }
     } else {   // ------------------------------------------------------ softmax, outputs
-        const int wg = (warp - 2 - Q_WARPS) >> 2, sg = wg % C::SG, pg = wg / C::SG;   // warpgroup: its rows, its turn
+        const int wg = (warp - FIRST_Q - Q_WARPS) >> 2, sg = wg % C::SG, pg = wg / C::SG;   // warpgroup: its rows, its turn
         const int q4 = warp & 3, key = 32 * q4 + lane, bid = 1 + wg;                 // the warp's lane quarter
         const uint32_t lane_at = (uint32_t)(32 * q4) << 16;
         // byte of this key in a column of P: values lie in the order of paged.cuh
