@@ -48,7 +48,6 @@ constexpr int TILE = 128, TB = TILE / BLOCK;   // keys of a tile, its blocks
 constexpr int SEG_COST = 16;          // a group's fixed cost in blocks
 constexpr int FIRST_Q = 3, Q_WARPS = 4;   // the warps of the queries
 constexpr int SQ = 4;                 // groups known ahead
-constexpr int SCR = 16;               // tiles whose scales are kept: more than the copies are ahead of the softmax
 
 struct AttnParams {
     Pool pool;
@@ -81,6 +80,7 @@ struct Cfg {
     // slots of keys and of values: a tile's keys are done with its scores, its values much later
     static constexpr int NK = N >= 96 ? (HD == 256 ? 2 : 4) : HD == 256 ? 3 : HD == 128 ? 6 : 8;
     static constexpr int NV = N >= 96 ? (HD == 256 ? 1 : 2) : NK;
+    static constexpr int SCR = NK <= 4 ? 8 : 16;              // tiles whose scales are kept: the copies are up to NK + 3 ahead
     // P: 16 keys of every column, then the next 16, 64 bytes further than they need so that the byte
     // stores of a warp's two runs of 16 keys meet different banks.
     static constexpr int PK = N * 16 + 64, PB = TILE / 16 * PK, NP = 2;
@@ -138,6 +138,27 @@ __device__ __forceinline__ void tm_wait(float (&v)[K]) {
     for (int i = 0; i < K; i++) asm volatile("" : "+f"(v[i]));
 }
 
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -340,7 +361,7 @@ __device__ __noinline__ bool walk_next(const AttnParams &a, const uint32_t *pre,
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a) {
-    constexpr int HD = C::HD, N = C::N, TT = C::T, R = C::R, NK = C::NK, NV = C::NV, QB = 2, NP = C::NP;
+    constexpr int HD = C::HD, N = C::N, TT = C::T, R = C::R, NK = C::NK, NV = C::NV, QB = 2, NP = C::NP, SCR = C::SCR;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ uint64_t full_k[NK], empty_k[NK], full_v[NV], empty_v[NV], sc_full[SCR], p_full[2], pv_done[2], q_full[QB], q_empty[QB];
     // a set waits on barriers that only its own tiles move, or on ones that its tile's scores imply: a wait by
@@ -348,13 +369,13 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     __shared__ uint64_t s_full[C::PG][2];
     __shared__ uint64_t seg_full[SQ], seg_empty[SQ], o_full[C::PG];   // o_full: a group's sums are complete
     __shared__ Seg segs[SQ];                            // the CTA's groups, as warp 0 finds them; k0 < 0: no more
-    __shared__ float2 scales[SCR][TB];                  // dk, dv of a tile's blocks
+    __shared__ float4 scales[SCR][TB];                  // dk, log2 dv, 1 / dv of a tile's blocks
     __shared__ uint32_t pre[MAX_SEQ + 1], wsum[C::WARPS];
     __shared__ float q_up[4];                           // score factor of a query tile: the softmax may be two behind
     __shared__ int dead;                                // a wait ran out: what follows no longer waits
     constexpr int G = C::SG * C::PG;
     __shared__ float red[G][4][C::RG];                  // per row: the warps' maxima, then their sums
-    __shared__ __align__(16) float mref[G][(C::RG + 3) / 4 * 4];   // per row: the reference m
+    __shared__ __align__(16) float mref[G][(C::RG + 3) / 4 * 4];   // per row: -m, the reference
     __shared__ uint32_t moved[G][4];                    // the warps' chunks whose reference has to move
     __shared__ __align__(16) float fs[G][(C::RG + 3) / 4 * 4];     // per row: a factor for all of its outputs
     __shared__ int pos_s[C::PG][R];                     // per row: position, -1 past the tile's last row
@@ -510,7 +531,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     if (lane < nb)
                         bulk_g2s(smem + (size_t)(i % NK) * C::SLOT + lane * C::KB, a.pool.k + bi * C::KB, C::KB, full_k + i % NK);
                 }
-                if (lane < TB) scales[i % SCR][lane] = sc;
+                if (lane < TB) scales[i % SCR][lane] = make_float4(sc.x, log2f(sc.y), 1.0f / sc.y, 0.f);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sc_full + i % SCR);
                 i++;
@@ -767,8 +788,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 mine_i++;
                 __syncwarp();
                 tc_after();
-                const float2 sc = scales[i % SCR][key >> 4];
-                const float fb = log2f(sc.y), isv = 1.0f / sc.y;
+                const float4 sc = scales[i % SCR][key >> 4];
+                const float fb = sc.y, isv = sc.z;
                 const int j0 = start + k * TILE, j = j0 + key;
                 const float fa = sc.x * q_up[qi & 3];
                 const bool edge = j0 + TILE - 1 > p_lo || (window > 0 && j0 <= p_hi - window);
@@ -780,12 +801,25 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     for (int x = 0; x < LC / LD; x++)
                         tm_ld<LD>(tmem + lane_at + (i & 1) * N + C::col(sg, ch, x), v + LD * x);
                     tm_wait(v);
+                    if constexpr (RG % 2 == 0) {
+                        const f32x2 fa2 = pack2(fa, fa), fb2 = pack2(fb, fb), step2 = pack2(1.0f / STEP, 1.0f / STEP);
 #pragma unroll
-                    for (int r = 0; r < CH; r++) {
-                        float u = v[(TT - 1) * TS + r];
+                        for (int r = 0; r < CH; r += 2) {
+                            f32x2 u = pack2(v[(TT - 1) * TS + r], v[(TT - 1) * TS + r + 1]);
 #pragma unroll
-                        for (int x = TT - 2; x >= 0; x--) u = fmaf(u, 1.0f / STEP, v[x * TS + r]);
-                        t[ch * CH + r] = fmaf(u, fa, fb);
+                            for (int x = TT - 2; x >= 0; x--) u = fma2(u, step2, pack2(v[x * TS + r], v[x * TS + r + 1]));
+                            const float2 s = unpack2(fma2(u, fa2, fb2));
+                            t[ch * CH + r] = s.x;
+                            t[ch * CH + r + 1] = s.y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < CH; r++) {
+                            float u = v[(TT - 1) * TS + r];
+#pragma unroll
+                            for (int x = TT - 2; x >= 0; x--) u = fmaf(u, 1.0f / STEP, v[x * TS + r]);
+                            t[ch * CH + r] = fmaf(u, fa, fb);
+                        }
                     }
                 }
                 if (edge) {
@@ -799,10 +833,21 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
 #pragma unroll
                 for (int ch = 0; ch < C::NC; ch++) {
                     float mx = -INFINITY;
+                    if constexpr (RG % 2 == 0) {   // the references are kept negated
 #pragma unroll
-                    for (int r = 0; r < CH; r++) {
-                        t[ch * CH + r] -= mr[ch * CH + r];
-                        mx = fmaxf(mx, t[ch * CH + r]);
+                        for (int r = 0; r < CH; r += 2) {
+                            const float2 n = *reinterpret_cast<const float2 *>(mr + ch * CH + r);
+                            const float2 u = unpack2(add2(pack2(t[ch * CH + r], t[ch * CH + r + 1]), pack2(n.x, n.y)));
+                            t[ch * CH + r] = u.x;
+                            t[ch * CH + r + 1] = u.y;
+                            mx = fmaxf(mx, fmaxf(u.x, u.y));
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < CH; r++) {
+                            t[ch * CH + r] += mr[ch * CH + r];
+                            mx = fmaxf(mx, t[ch * CH + r]);
+                        }
                     }
                     over |= mx > W_MAX ? 1u << ch : 0u;
                 }
@@ -829,7 +874,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                         const float x = fmaxf(fmaxf(red[wg][0][key], red[wg][1][key]), fmaxf(red[wg][2][key], red[wg][3][key]));
                         const float up = !first ? (x > W_MAX ? x - W_TOP : 0.f) : x == -INFINITY ? 0.f : x - W_TOP;
                         fs[wg][key] = up;
-                        mr[key] += up;
+                        mr[key] -= up;
                     }
                     bar_sync(bid, 128);
 #pragma unroll
@@ -871,12 +916,20 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
 #pragma unroll
                 for (int r = 0; r < RG; r += 2) {
                     float x[2] = {0.f, 0.f};
+                    if (RG % 2 == 0 && !edge) {
+                        x[0] = ex2(t[r]);
+                        x[1] = ex2(t[r + 1]);
+                        const float2 n = unpack2(fma2(pack2(x[0], x[1]), pack2(isv, isv), pack2(l[r], l[r + 1])));
+                        l[r] = n.x;
+                        l[r + 1] = n.y;
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 2; e++)
-                        if (r + e < RG) {
-                            x[e] = ex2(t[r + e]);
-                            if (!edge || t[r + e] != -INFINITY) l[r + e] = fmaf(x[e], isv, l[r + e]);
-                        }
+                        for (int e = 0; e < 2; e++)
+                            if (r + e < RG) {
+                                x[e] = ex2(t[r + e]);
+                                if (!edge || t[r + e] != -INFINITY) l[r + e] = fmaf(x[e], isv, l[r + e]);
+                            }
+                    }
                     uint32_t b[TT];
                     split<TT>(x[0], x[1], b);
 #pragma unroll
@@ -940,7 +993,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 // a row (or part) that saw nothing: its products are 0 or were not made
                 fs[wg][key] = L == 0.f ? 0.f : whole ? 1.0f / (L * sig) : 1.0f;
                 if (!whole && mine) {
-                    slot[R * HD + row] = L == 0.f ? M_NONE : mr[key];
+                    slot[R * HD + row] = L == 0.f ? M_NONE : -mr[key];
                     slot[R * HD + R + row] = L;
                 }
             }
