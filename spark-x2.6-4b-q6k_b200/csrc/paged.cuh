@@ -44,32 +44,6 @@ __device__ __forceinline__ size_t block_index(const Pool &p, int page, int head,
     return ((size_t)page * p.kv_heads + head) * (p.page_tokens / BLOCK) + blk;
 }
 
-// 4 consecutive values as f32; vec: the 4 values' address is a multiple of their size.
-template <typename T>
-__device__ __forceinline__ float4 load4(const T *p, bool vec);
-template <>
-__device__ __forceinline__ float4 load4<float>(const float *p, bool vec) {
-    if (vec) return __ldg(reinterpret_cast<const float4 *>(p));
-    return make_float4(p[0], p[1], p[2], p[3]);
-}
-template <>
-__device__ __forceinline__ float4 load4<__half>(const __half *p, bool vec) {
-    if (!vec) return make_float4(__half2float(p[0]), __half2float(p[1]), __half2float(p[2]), __half2float(p[3]));
-    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
-    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-template <>
-__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16 *p, bool vec) {
-    if (!vec)
-        return make_float4(__bfloat162float(p[0]), __bfloat162float(p[1]), __bfloat162float(p[2]),
-                           __bfloat162float(p[3]));
-    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                       __uint_as_float(w.y & 0xffff0000u));
-}
-
 // A row of hd values is handled as hd / 8 units of two 4-value pieces, so that a rotated pair
 // (i, i + pdim / 2) is in one thread: unit u < pdim / 8 holds dims 4u .. and pdim / 2 + 4u ..,
 // the others 8 consecutive dims. The first dims of unit u's pieces:
@@ -91,14 +65,57 @@ __device__ __forceinline__ void angle(int pos, float freq, float &c, float &s) {
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
 }
 
+// 8 values of a row as they lie in memory: two pieces of 4 (dims d0 .. and d1 ..)
 template <typename T>
-__device__ __forceinline__ void load_unit(const T *row, int u, int pdim, bool vec, float (&a)[4], float (&b)[4]) {
-    int d0, d1;
-    unit_dims(u, pdim, d0, d1);
-    const float4 x = load4<T>(row + d0, vec), y = load4<T>(row + d1, vec);
-    a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
-    b[0] = y.x, b[1] = y.y, b[2] = y.z, b[3] = y.w;
-}
+struct Raw {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void load(const T *row, int d0, int d1, int vec) {
+        if (sizeof(T) == 2 && vec == 2 && d1 == d0 + 4) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + d0));
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        } else if (vec) {
+            if constexpr (sizeof(T) == 2) {
+                const uint2 a = __ldg(reinterpret_cast<const uint2 *>(row + d0)), b = __ldg(reinterpret_cast<const uint2 *>(row + d1));
+                w[0] = a.x, w[1] = a.y, w[2] = b.x, w[3] = b.y;
+            } else {
+                const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + d0)), b = __ldg(reinterpret_cast<const uint4 *>(row + d1));
+                w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+                w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const T *p = row + (e < 4 ? d0 + e : d1 + e - 4);
+                if constexpr (sizeof(T) == 4) w[e] = *reinterpret_cast<const uint32_t *>(p);
+                else {
+                    const uint32_t h = *reinterpret_cast<const uint16_t *>(p);
+                    w[e >> 1] = e & 1 ? w[e >> 1] | (h << 16) : h;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int i = 0; i < (int)(2 * sizeof(T)); i++) w[i] = 0;
+    }
+    __device__ __forceinline__ void f32(float (&x)[8]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = __uint_as_float(w[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (__is_same(T, __half)) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+                } else {
+                    x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+                }
+            }
+        }
+    }
+};
+
 // The rotation of a unit's 4 pairs, each product rounded (model.rs:431-439).
 __device__ __forceinline__ void rotate_unit(float (&a)[4], float (&b)[4], const float (&c)[4], const float (&s)[4]) {
 #pragma unroll
@@ -109,9 +126,11 @@ __device__ __forceinline__ void rotate_unit(float (&a)[4], float (&b)[4], const 
     }
 }
 
-// Whether 4-value pieces of rows at p with stride ld (elements of `size` bytes) are aligned.
-inline bool rows_aligned(const void *p, long long ld, int size) {
-    return ((uintptr_t)p % (4 * size)) == 0 && (ld % 4) == 0;
+// Alignment of the pieces of rows at p with stride ld (elements of `size` bytes): 0 none, 1 four values,
+// 2 eight, too.
+inline int rows_aligned(const void *p, long long ld, int size) {
+    if ((uintptr_t)p % (4 * size) || ld % 4) return 0;
+    return (uintptr_t)p % (8 * size) == 0 && ld % 8 == 0 ? 2 : 1;
 }
 
 int check_pool(const spk_kv_pool *p, const char *who);

@@ -78,57 +78,6 @@ __device__ __forceinline__ float2 e4m3x2_f32(uint32_t w) {
     return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
 }
 
-// 8 values of a row as they lie in memory: two pieces of 4 (dims d0 .. and d1 ..)
-template <typename T>
-struct Raw {
-    uint32_t w[2 * sizeof(T)];
-    __device__ __forceinline__ void load(const T *row, int d0, int d1, int vec) {
-        if (sizeof(T) == 2 && vec == 2 && d1 == d0 + 4) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + d0));
-            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-        } else if (vec) {
-            if constexpr (sizeof(T) == 2) {
-                const uint2 a = __ldg(reinterpret_cast<const uint2 *>(row + d0)), b = __ldg(reinterpret_cast<const uint2 *>(row + d1));
-                w[0] = a.x, w[1] = a.y, w[2] = b.x, w[3] = b.y;
-            } else {
-                const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + d0)), b = __ldg(reinterpret_cast<const uint4 *>(row + d1));
-                w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-                w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const T *p = row + (e < 4 ? d0 + e : d1 + e - 4);
-                if constexpr (sizeof(T) == 4) w[e] = *reinterpret_cast<const uint32_t *>(p);
-                else {
-                    const uint32_t h = *reinterpret_cast<const uint16_t *>(p);
-                    w[e >> 1] = e & 1 ? w[e >> 1] | (h << 16) : h;
-                }
-            }
-        }
-    }
-    __device__ __forceinline__ void none() {
-#pragma unroll
-        for (int i = 0; i < (int)(2 * sizeof(T)); i++) w[i] = 0;
-    }
-    __device__ __forceinline__ void f32(float (&x)[8]) const {
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = __uint_as_float(w[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if constexpr (__is_same(T, __half)) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                    x[2 * i] = f.x, x[2 * i + 1] = f.y;
-                } else {
-                    x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-                }
-            }
-        }
-    }
-};
-
 // 16-byte piece of the staging tile, spread so that a warp's 4-byte writes (pieces 8 apart) meet few banks
 __device__ __forceinline__ int spread(int piece) { return piece ^ ((piece >> 3) & 7); }
 
@@ -388,10 +337,7 @@ extern "C" int spk_paged_append(const spk_kv_pool *pool, const spk_kv_batch *bat
     const int size = type == T_F32 ? 4 : 2;
     if ((uintptr_t)k % size || (uintptr_t)v % size) return set_error("%s: unaligned rows", who);
     if (pool->kv_heads > 65535) return set_error("%s: %d KV heads", who, pool->kv_heads);
-    auto aligned = [&](const void *p, long long ld) {
-        return !rows_aligned(p, ld, size) ? 0 : (uintptr_t)p % (8 * size) == 0 && ld % 8 == 0 ? 2 : 1;
-    };
-    const AppendArgs a{pool_of(pool), batch_of(batch), k, v, ldk, ldv, aligned(k, ldk), aligned(v, ldv),
+    const AppendArgs a{pool_of(pool), batch_of(batch), k, v, ldk, ldv, rows_aligned(k, ldk, size), rows_aligned(v, ldv, size),
                        freq, freq ? pdim : 0, 1, 1, device_error_ptr()};
     const cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = type == T_F32   ? launch<float>(a, s)

@@ -658,20 +658,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             if (g.nblk == 0) continue;
             const int qb = qi % QB, c0 = g.c0, c1 = g.c1, pos0 = g.pos0;
             const T *q0 = (const T *)a.q + (size_t)g.r0 * a.ldq + (size_t)g.kvh * a.group * HD;
-            // a warp takes RW rows side by side, QROWS at a time (they stay in registers where that is all)
-            constexpr int RW = (R + Q_WARPS - 1) / Q_WARPS, QROWS = RW < 4 ? RW : 4;
-            float x[QROWS][4], y[QROWS][4];
-            auto load = [&](int r0) {
-#pragma unroll
-                for (int r = 0; r < QROWS; r++) {
-                    const int row = qw * RW + r0 + r, c = c0 + row;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[r][e] = y[r][e] = 0.f;
-                    if (r0 + r < RW && row < R && c <= c1 && lane < HD / 8)
-                        load_unit<T>(q0 + (size_t)(c / a.group) * a.ldq + (size_t)(c % a.group) * HD, lane, a.pdim,
-                                     a.qvec, x[r], y[r]);
-                }
-            };
+            // a warp takes RW rows side by side, RB at a time (they stay in registers where that is all)
+            constexpr int RW = (R + Q_WARPS - 1) / Q_WARPS, RB = RW < 8 ? RW : 8;
+            const int w0 = qw * RW;
             int d0, d1, turned = -1;
             unit_dims(lane, a.pdim, d0, d1);
             float cs[4], sn[4], fr[4];
@@ -685,18 +674,29 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     turned = tok;
                 }
             };
+            Raw<T> raw[RB];
+            auto load = [&](int r0) {
+#pragma unroll
+                for (int r = 0; r < RB; r++) {
+                    const int c = c0 + w0 + r0 + r;
+                    if (r0 + r < RW && w0 + r0 + r < R && c <= c1 && lane < HD / 8)
+                        raw[r].load(q0 + (size_t)(c / a.group) * a.ldq + (size_t)(c % a.group) * HD, d0, d1, a.qvec);
+                    else raw[r].none();
+                }
+            };
             // the tile's largest finite value: the rotation grows a pair by at most sqrt(2)
             float mx = 0.f;
-            for (int r0 = 0; r0 < RW; r0 += QROWS) {
+#pragma unroll 1
+            for (int r0 = 0; r0 < RW; r0 += RB) {
                 load(r0);
-                if (r0 == 0) turn((c0 + qw * RW) / a.group);   // while the rows are on their way
+                if (r0 == 0) turn((c0 + w0) / a.group);   // while the rows are on their way
 #pragma unroll
-                for (int r = 0; r < QROWS; r++)
+                for (int r = 0; r < RB; r++) {
+                    float x[8];
+                    raw[r].f32(x);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float u = fabsf(x[r][e]), v = fabsf(y[r][e]);
-                        mx = fmaxf(mx, fmaxf(u < INFINITY ? u : 0.f, v < INFINITY ? v : 0.f));
-                    }
+                    for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+                }
             }
             mx = warp_max(mx);
             if (lane == 0) amax_s[qw] = mx;
@@ -710,34 +710,39 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             const float up = sane ? __uint_as_float((uint32_t)(ex - 6) << 23) : 1.0f;
             uint8_t *dst = qs + (size_t)qb * N * HD;
             if (qi >= QB) wait_for(q_empty + qb, ((qi / QB) - 1) & 1, &dead, a.err);
-            for (int r0 = 0; r0 < RW; r0 += QROWS) {
-                if (RW > QROWS) load(r0);
+#pragma unroll 1
+            for (int r0 = 0; r0 < RW; r0 += RB) {
+                if (RW > RB) load(r0);
 #pragma unroll
-                for (int r = 0; r < QROWS; r++) {
-                    const int row = qw * RW + r0 + r;
+                for (int r = 0; r < RB; r++) {
+                    const int row = w0 + r0 + r;
                     if (r0 + r >= RW || row >= R) continue;
+                    float v[8], x[4], y[4];
+                    raw[r].f32(v);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = v[e], y[e] = v[4 + e];
                     turn((c0 + row) / a.group);
-                    if (lane < a.pdim / 8) rotate_unit(x[r], y[r], cs, sn);
+                    if (lane < a.pdim / 8) rotate_unit(x, y, cs, sn);
                     if (lane >= HD / 8) continue;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        x[r][e] = fmaf(x[r][e], dn, x[r][e] - x[r][e]);   // an infinity becomes a NaN, which e4m3 has
-                        y[r][e] = fmaf(y[r][e], dn, y[r][e] - y[r][e]);
+                        x[e] = fmaf(x[e], dn, x[e] - x[e]);   // an infinity becomes a NaN, which e4m3 has
+                        y[e] = fmaf(y[e], dn, y[e] - y[e]);
                     }
 #pragma unroll
                     for (int t = 0; t < TT; t++) {
                         const int n = t * R + row;
                         uint8_t *col = dst + (n >> 3) * (8 * HD) + (n & 7) * 16;
-                        const uint32_t x0 = e4m3x2(x[r][0], x[r][1]), x1 = e4m3x2(x[r][2], x[r][3]);
-                        const uint32_t y0 = e4m3x2(y[r][0], y[r][1]), y1 = e4m3x2(y[r][2], y[r][3]);
+                        const uint32_t x0 = e4m3x2(x[0], x[1]), x1 = e4m3x2(x[2], x[3]);
+                        const uint32_t y0 = e4m3x2(y[0], y[1]), y1 = e4m3x2(y[2], y[3]);
                         *reinterpret_cast<uint32_t *>(col + (d0 >> 4) * 128 + (d0 & 15)) = x0 | (x1 << 16);
                         *reinterpret_cast<uint32_t *>(col + (d1 >> 4) * 128 + (d1 & 15)) = y0 | (y1 << 16);
                         if (t + 1 < TT) {   // what is left, on the next term's scale
                             const float2 p0 = e4m3x2_f32(x0), p1 = e4m3x2_f32(x1), p2 = e4m3x2_f32(y0), p3 = e4m3x2_f32(y1);
-                            x[r][0] = (x[r][0] - p0.x) * STEP, x[r][1] = (x[r][1] - p0.y) * STEP;
-                            x[r][2] = (x[r][2] - p1.x) * STEP, x[r][3] = (x[r][3] - p1.y) * STEP;
-                            y[r][0] = (y[r][0] - p2.x) * STEP, y[r][1] = (y[r][1] - p2.y) * STEP;
-                            y[r][2] = (y[r][2] - p3.x) * STEP, y[r][3] = (y[r][3] - p3.y) * STEP;
+                            x[0] = (x[0] - p0.x) * STEP, x[1] = (x[1] - p0.y) * STEP;
+                            x[2] = (x[2] - p1.x) * STEP, x[3] = (x[3] - p1.y) * STEP;
+                            y[0] = (y[0] - p2.x) * STEP, y[1] = (y[1] - p2.y) * STEP;
+                            y[2] = (y[2] - p3.x) * STEP, y[3] = (y[3] - p3.y) * STEP;
                         }
                     }
                 }
