@@ -24,13 +24,13 @@
 // prompt chunks the softmax's instructions, 64 bf16 rows against each 128 keys.
 //
 // Work split: all (sequence, KV head, row tile) groups stand in one line, each as long as the
-// tokens it reads plus SEG_COST for its fixed cost; the line is cut into equal ranges, one per CTA,
+// tokens it reads plus COST for its fixed cost; the line is cut into equal ranges, one per CTA,
 // one CTA per SM. A 128-token tile belongs to the CTA in whose range its first token falls. A group
 // that several CTAs share leaves (O, m, l) in the workspace; the last CTA to arrive (a ticket that it
 // resets) adds the parts in CTA order.
 //
 // Warps: 0 the groups and the copies of keys and scales, 1 MMA issue, 2 the copies of values, 3-6 the
-// queries of the next group, 7.. softmax:
+// queries of the next group (of the first one with the others' help), 7.. softmax:
 // a thread per key, and per output dim at the end of a group.
 #include "paged.cuh"
 
@@ -45,7 +45,6 @@ constexpr float W_TOP = 3.0f, W_MAX = 8.0f;
 constexpr float STEP = 32.0f;         // a term's scale over the one before: half an ulp of 256 is 8
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int TILE = 128, TB = TILE / BLOCK;   // keys of a tile, its blocks
-constexpr int SEG_COST = 16;          // a group's fixed cost in blocks
 constexpr int FIRST_Q = 3, Q_WARPS = 4;   // the warps of the queries
 constexpr int SQ = 4;                 // groups known ahead
 
@@ -89,6 +88,9 @@ struct Cfg {
     static constexpr int MW = 160 * (SG == 1 ? 1 : 4);        // weights that a merge of parts holds at once
     static constexpr size_t V_OFF = (size_t)NK * SLOT, Q_OFF = V_OFF + (size_t)NV * SLOT, P_OFF = Q_OFF + (size_t)2 * N * HD;
     static constexpr size_t SMEM = P_OFF + (size_t)NP * PB;
+    // a group's fixed cost in blocks: what evened out the CTAs' times over 64 sequences of 1 to 9000 tokens
+    // (narrow: 8 40.4 us, 16 40.6, 32 42.0, 64 46.7) and 24 of 8 rows each (wide: 8 46 us, 16 37, 32 31, 64 33)
+    static constexpr int COST = PG == 1 ? 32 : 16;
     static constexpr int LAG = PG == 1 ? 2 : 1;               // tiles that the values are behind the scores
     static constexpr int WARPS = FIRST_Q + Q_WARPS + 4 * SG * PG, THREADS = WARPS * 32;
     static constexpr int PART = (R * (HD + 2) + 3) / 4 * 4;   // floats of a partial: O, then m, then l; read 16 bytes at a time
@@ -293,9 +295,9 @@ __device__ __forceinline__ Seq seq_of(const AttnParams &a, int s, int R) {
     return q;
 }
 // Length of group j and of groups 0 .. j - 1: the tokens' sum, a partial block each, the fixed costs.
-__device__ __forceinline__ uint32_t before(const Seq &q, uint32_t j) {
+__device__ __forceinline__ uint32_t before(const Seq &q, uint32_t j, int cost) {
     const unsigned long long t = (unsigned long long)j * q.c + (unsigned long long)q.slope * j * (j + 1) / 2;
-    return (uint32_t)(t / BLOCK) + j * (SEG_COST + 2);
+    return (uint32_t)(t / BLOCK) + j * (cost + 2);
 }
 
 struct Seg {
@@ -314,38 +316,38 @@ struct Walk {
     Seq q;
 };
 // The group of sequence s that holds the start of the CTA's range.
-__device__ __forceinline__ void walk_at(const AttnParams &a, const uint32_t *pre, int s, int R, Walk &w) {
+__device__ __forceinline__ void walk_at(const AttnParams &a, const uint32_t *pre, int s, int R, int cost, Walk &w) {
     w.s = s;
     w.q = seq_of(a, s, R);
-    const uint32_t per = before(w.q, w.q.tiles), in = w.x0 - pre[s];
+    const uint32_t per = before(w.q, w.q.tiles, cost), in = w.x0 - pre[s];
     w.kvh = in / per;
     const uint32_t rem = in - w.kvh * per;
     int a0 = 0, a1 = w.q.tiles;       // the last group with before <= rem
     while (a1 - a0 > 1) {
         const int mid = (a0 + a1) >> 1;
-        if (before(w.q, mid) <= rem) a0 = mid;
+        if (before(w.q, mid, cost) <= rem) a0 = mid;
         else a1 = mid;
     }
     w.j = a0;
-    w.base = pre[s] + w.kvh * per + before(w.q, a0);
+    w.base = pre[s] + w.kvh * per + before(w.q, a0, cost);
 }
 // The next group of which this CTA has tiles.
-__device__ __noinline__ bool walk_next(const AttnParams &a, const uint32_t *pre, int R, Walk &w, Seg &g) {
+__device__ __noinline__ bool walk_next(const AttnParams &a, const uint32_t *pre, int R, int cost, Walk &w, Seg &g) {
     while (w.base < w.x1) {
         const int G = a.group, c0 = w.j * R, c1 = min(c0 + R, w.q.n * G) - 1, pos0 = w.q.len - w.q.n;
         const int p_lo = pos0 + c0 / G, p_hi = pos0 + c1 / G;
         const int see0 = a.window > 0 ? max(0, p_lo + 1 - a.window) : 0, b0 = see0 / BLOCK;
         const int nblk = p_hi < 0 ? 0 : p_hi / BLOCK + 1 - b0;
         const int nt = max(1, (nblk + TB - 1) / TB);   // one empty tile where nothing is seen
-        const uint32_t t0 = w.base + SEG_COST;         // tile k stands at t0 + TB k, inside the group's length
+        const uint32_t t0 = w.base + cost;         // tile k stands at t0 + TB k, inside the group's length
         const int d0 = (int)(w.x0 - t0), d1 = (int)(w.x1 - t0);
         const int k0 = d0 <= 0 ? 0 : (d0 + TB - 1) / TB, k1 = d1 <= 0 ? 0 : min(nt, (d1 + TB - 1) / TB);
         const bool mine = k0 < k1;
         if (mine)
             g = Seg{w.s, w.q.r0, w.kvh, c0, c1, pos0, p_lo, p_hi, see0, b0 * BLOCK, k0, k1,
                     (int)(t0 / w.chunk), (int)((t0 + (uint32_t)(TB * (nt - 1))) / w.chunk), nblk};
-        const uint32_t at = before(w.q, w.j);
-        w.base += before(w.q, ++w.j) - at;
+        const uint32_t at = before(w.q, w.j, cost);
+        w.base += before(w.q, ++w.j, cost) - at;
         if (w.j == w.q.tiles) {
             w.j = 0;
             if (++w.kvh == a.pool.kv_heads) {
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     __shared__ int pos_s[C::PG][R];                     // per row: position, -1 past the tile's last row
     __shared__ size_t out_s[C::PG][R];                  // per row: where its output lies
     __shared__ float merge_s[C::PG][2 * C::MW];         // a row's weights of the parts, and their sums before
-    __shared__ float amax_s[Q_WARPS];
+    __shared__ float amax_s[C::WARPS - FIRST_Q];
     __shared__ int last_in[C::PG];
     __shared__ uint32_t tmem_s;
     __shared__ Walk walk_s;                             // the walk behind the CTA's first group
@@ -439,7 +441,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
         uint32_t u = 0;
         if (s < a.b.nseq) {
             const Seq q = seq_of(a, s, R);
-            u = before(q, q.tiles) * a.pool.kv_heads;
+            u = before(q, q.tiles, C::COST) * a.pool.kv_heads;
         }
         uint32_t x = u;
 #pragma unroll
@@ -469,9 +471,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             w.chunk = chunk;
             w.x0 = x0;
             w.x1 = min(base, x0 + chunk);
-            walk_at(a, pre, s, R, w);
+            walk_at(a, pre, s, R, C::COST, w);
             Seg g;
-            if (walk_next(a, pre, R, w, g)) segs[0] = g;
+            if (walk_next(a, pre, R, C::COST, w, g)) segs[0] = g;
             walk_s = w;
         }
     __syncthreads();
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
         if (lane == 0) mbar_arrive(seg_full);   // group 0 is there
         for (uint32_t n = 1; g.k0 >= 0; n++) {
             Seg nx;
-            if (!walk_next(a, pre, R, w, nx)) nx.k0 = -1;
+            if (!walk_next(a, pre, R, C::COST, w, nx)) nx.k0 = -1;
             if (n >= SQ) wait_for(seg_empty + n % SQ, ((n / SQ) - 1) & 1, nullptr, a.err);
             __syncwarp();
             if (lane == 0) {
@@ -651,15 +653,23 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             }
             flush();
         }
-    } else if (warp < FIRST_Q + Q_WARPS) {   // ------------------------------------------------- queries
+    } else if (warp >= FIRST_Q && (C::PG == 1 || warp < FIRST_Q + Q_WARPS)) {   // ---------- queries
+        // a wide tile's first ones by all the warps that have nothing to do yet
         const int qw = warp - FIRST_Q;
+        const bool keeps = qw < Q_WARPS;
         uint32_t qi = 0;
-        for (uint32_t n = 0; group(n, g); n++) {
+        for (uint32_t n = 0; n == 0 || keeps; n++) {
+            if (keeps) {
+                if (!group(n, g)) break;
+            } else {
+                g = segs[0];
+            }
             if (g.nblk == 0) continue;
+            const int helpers = C::PG == 1 && n == 0 ? C::WARPS - FIRST_Q : Q_WARPS, RW = (R + helpers - 1) / helpers;
             const int qb = qi % QB, c0 = g.c0, c1 = g.c1, pos0 = g.pos0;
             const T *q0 = (const T *)a.q + (size_t)g.r0 * a.ldq + (size_t)g.kvh * a.group * HD;
             // a warp takes RW rows side by side, RB at a time (they stay in registers where that is all)
-            constexpr int RW = (R + Q_WARPS - 1) / Q_WARPS, RB = RW < 8 ? RW : 8;
+            constexpr int RB = (R + Q_WARPS - 1) / Q_WARPS < 4 ? (R + Q_WARPS - 1) / Q_WARPS : 4;
             const int w0 = qw * RW;
             int d0, d1, turned = -1;
             unit_dims(lane, a.pdim, d0, d1);
@@ -700,9 +710,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             }
             mx = warp_max(mx);
             if (lane == 0) amax_s[qw] = mx;
-            bar_sync(5, Q_WARPS * 32);
-#pragma unroll
-            for (int e = 0; e < Q_WARPS; e++) mx = fmaxf(mx, amax_s[e]);
+            bar_sync(5, helpers * 32);
+            for (int e = 0; e < helpers; e++) mx = fmaxf(mx, amax_s[e]);
             // times 2^(6 - e), so that it lies in [64, 128); a tile of zeros stays
             const int ex = (int)(__float_as_uint(mx) >> 23);
             const bool sane = ex >= 8 && ex <= 246;
@@ -749,12 +758,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             }
             if (qw == 0 && lane == 0) q_up[qi & 3] = up * a.scale;
             fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full + qb);
-            bar_sync(5, Q_WARPS * 32);   // amax_s is free again
+            bar_sync(5, helpers * 32);   // all rows are there, and amax_s is free again
+            if (keeps && lane == 0) mbar_arrive(q_full + qb);
             qi++;
         }
-    } else {   // ------------------------------------------------------ softmax, outputs
+    }
+    if (warp >= FIRST_Q + Q_WARPS && segs[0].k0 >= 0) {   // ------------------------------ softmax, outputs
         const int wg = (warp - FIRST_Q - Q_WARPS) >> 2, sg = wg % C::SG, pg = wg / C::SG;   // warpgroup: its rows, its turn
         const int q4 = warp & 3, key = 32 * q4 + lane, bid = 1 + wg;                 // the warp's lane quarter
         const uint32_t lane_at = (uint32_t)(32 * q4) << 16;
@@ -1119,7 +1128,7 @@ template <typename T, typename C>
 int launch_one(const AttnParams &a, cudaStream_t s, const char *who) {
     // the line of work, at its longest: every row tile as long as the page table
     const long long tiles = (long long)a.b.rows * a.group / C::R + a.b.nseq;
-    const long long blocks = (long long)a.b.max_pages * a.pool.page_tokens / BLOCK + SEG_COST + 3;
+    const long long blocks = (long long)a.b.max_pages * a.pool.page_tokens / BLOCK + C::COST + 3;
     if ((double)tiles * blocks * a.pool.kv_heads > 2147483000.0)
         return set_error("%s: %d rows over up to %d pages of %d tokens are too much for one call", who, a.b.rows,
                          a.b.max_pages, a.pool.page_tokens);
