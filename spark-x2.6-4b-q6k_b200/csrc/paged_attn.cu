@@ -485,7 +485,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
         if (lane == 0) mbar_arrive(seg_empty + n % SQ);
         return g.k0 >= 0;
     };
-    // the tiles of a group for a warp that copies: lane l < 8 has block l, whose page comes one tile ahead
+    // the tiles of a group for a warp that copies: lane l < 8 has block l, whose page comes two tiles ahead, so
+    // that its place is known a tile ahead
     const int per = a.pool.page_tokens / BLOCK;
     auto copy_group = [&](const Seg &g, auto &&tile) {
         const int blk0 = g.start / BLOCK, nblk = g.nblk, k1 = g.k1, kvh = g.kvh;
@@ -501,11 +502,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             }
             return page;
         };
-        int page = page_of(g.k0);
+        auto place_of = [&](int page, int k) { return block_index(a.pool, page, kvh, (blk0 + k * TB + lane) % per); };
+        int page = page_of(g.k0), ahead = page_of(g.k0 + 1);
+        size_t bi = place_of(page, g.k0);
         for (int k = g.k0; k < k1 && nblk > 0; k++) {
-            const size_t bi = block_index(a.pool, page, kvh, (blk0 + k * TB + lane) % per);
-            page = page_of(k + 1);
-            tile(min(TB, nblk - k * TB), bi);
+            const size_t next = place_of(ahead, k + 1);
+            ahead = page_of(k + 2);
+            tile(min(TB, nblk - k * TB), bi, k == g.k0, k + 1 < k1 ? min(TB, nblk - (k + 1) * TB) : 0, next);
+            bi = next;
         }
     };
     Seg g;
@@ -524,9 +528,11 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 segs[n % SQ] = nx;
                 mbar_arrive(seg_full + n % SQ);
             }
-            copy_group(g, [&](int nb, size_t bi) {
-                float2 sc = make_float2(0.f, 1.f);
-                if (lane < nb) sc = make_float2(__ldg(a.pool.ks + bi), __ldg(a.pool.vs + bi));
+            float2 ahead = make_float2(0.f, 1.f);   // the next tile's scales, on their way
+            copy_group(g, [&](int nb, size_t bi, bool first, int nb1, size_t bi1) {
+                float2 sc = ahead;
+                if (first && lane < nb) sc = make_float2(__ldg(a.pool.ks + bi), __ldg(a.pool.vs + bi));
+                if (lane < nb1) ahead = make_float2(__ldg(a.pool.ks + bi1), __ldg(a.pool.vs + bi1));
                 if (i < NK || wait_for(empty_k + i % NK, ((i / NK) - 1) & 1, &dead, a.err)) {
                     if (lane == 0) mbar_arrive_expect_tx(full_k + i % NK, nb * C::KB);
                     __syncwarp();
@@ -546,7 +552,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     } else if (warp == 2) {   // ------------------------------------------------------ values
         uint32_t i = 0;
         for (uint32_t n = 0; group(n, g); n++)
-            copy_group(g, [&](int nb, size_t bi) {
+            copy_group(g, [&](int nb, size_t bi, bool, int, size_t) {
                 uint64_t *full = full_v + i % NV;
                 uint8_t *vd = smem + C::V_OFF + (size_t)(i % NV) * C::SLOT;
                 if (i < NV || wait_for(empty_v + i % NV, ((i / NV) - 1) & 1, &dead, a.err)) {
