@@ -116,6 +116,12 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
+// One thread of a warp that is together, always the same one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // K columns of this thread's lane; tm_wait before their use
@@ -572,93 +578,114 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             for (uint32_t x = i > NV ? i - NV : 0; x < i; x++)
                 for (uint32_t y = 0; y < (1u << 20) && !mbar_try_wait(full_v + x % NV, (x / NV) & 1); y++) {}
     } else if (warp == 1) {   // ------------------------------------------------------ MMAs
-        if (lane == 0) {
-            const uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
-            const uint32_t so = tmem, oo = tmem + 2 * N;
-            // descriptors move by their address field alone
-            const uint64_t kdesc = smem_desc(smem_u32(smem), 128, 8 * HD);
-            const uint64_t qdesc = smem_desc(smem_u32(qs), 128, 8 * HD);
-            const uint64_t vdesc = smem_desc(smem_u32(smem) + (uint32_t)C::V_OFF, C::KB, 128);
-            const uint64_t pdesc = smem_desc(smem_u32(ps), C::PK, 128);
-            uint32_t i = 0, qi = 0;   // tiles whose scores were issued; groups with tiles
-            uint32_t sets[C::PG] = {};   // tiles of each set
-            // Up to LAG tiles' values are still to come. A wide tile's scores go before the values of the tile two
-            // before it, into the buffer that its softmax has just left, so that the softmax finds them ready; a
-            // narrow tile waits for memory, and its values leave their slot sooner.
-            struct Late {
-                uint32_t i;           // tile
-                int nb, po;           // its blocks, where its sums lie
-                bool first, last;     // of its group
-            } late[2] = {};
-            int nlate = 0;
-            auto weights = [&]() {    // of the oldest late tile: there
-                const bool ok = wait_for(p_full + (late[0].i & 1), (late[0].i >> 1) & 1, &dead, a.err);
-                tc_after();
-                return ok;
-            };
-            auto values = [&](bool ok) {   // of the oldest late tile, whose weights are there
-                const Late t = late[0];
-                late[0] = late[1];
-                nlate--;
-                const int st = t.i % NV;
-                if (!wait_for(full_v + st, (t.i / NV) & 1, &dead, a.err) || !ok) return;
-                tc_after();
-                const uint64_t vd = vdesc + (uint32_t)(st * (C::SLOT / 16)), pd = pdesc + (uint32_t)((t.i % NP) * (C::PB / 16));
+        // The whole warp walks and waits and one elected thread issues, so the walk's state and the descriptors
+        // are the same in all its lanes (2048-row chunk 448 us; all of it in a branch of lane 0: 465).
+        const bool one = elect_one();
+        const uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+        const uint32_t so = __shfl_sync(0xffffffffu, tmem, 0), oo = so + 2 * N;
+        // descriptors move by their address field alone
+        const uint64_t kdesc = smem_desc(smem_u32(smem), 128, 8 * HD);
+        const uint64_t qdesc = smem_desc(smem_u32(qs), 128, 8 * HD);
+        const uint64_t vdesc = smem_desc(smem_u32(smem) + (uint32_t)C::V_OFF, C::KB, 128);
+        const uint64_t pdesc = smem_desc(smem_u32(ps), C::PK, 128);
+        uint32_t i = 0, qi = 0;   // tiles whose scores were issued; groups with tiles
+        uint32_t sets[C::PG] = {};   // tiles of each set
+        // Up to LAG tiles' values are still to come. A wide tile's scores go before the values of the tile two
+        // before it, into the buffer that its softmax has just left, so that the softmax finds them ready; a
+        // narrow tile waits for memory, and its values leave their slot sooner. The oldest late tile is i - nlate.
+        struct Late {
+            int nb, po;           // its blocks, where its sums lie
+            bool first, last;     // of its group
+        };
+        Late l0 = {0, 0, false, false}, l1 = l0;   // the oldest, the one behind it
+        int nlate = 0;
+        auto weights = [&]() {    // of the oldest late tile: there
+            const uint32_t t = i - nlate;
+            const bool ok = wait_for(p_full + (t & 1), (t >> 1) & 1, &dead, a.err);
+            tc_after();
+            return ok;
+        };
+        auto values = [&](uint32_t t, bool ok) {   // of the oldest late tile, whose weights are there
+            const Late l = l0;
+            l0 = l1;
+            nlate--;
+            const uint32_t st = t % NV;
+            if (!wait_for(full_v + st, (t / NV) & 1, &dead, a.err)) ok = false;
+            __syncwarp();
+            tc_after();
+            if (one && ok) {
+                const uint64_t vd = vdesc + st * (C::SLOT / 16), pd = pdesc + (t % NP) * (C::PB / 16);
 #pragma unroll
                 for (int kk = 0; kk < TB / 2; kk++)
-                    if (2 * kk < t.nb)
+                    if (2 * kk < l.nb)
 #pragma unroll
                         for (int h = 0; h < C::HH; h++)
-                            mma_e4m3(oo + (t.po + h) * N, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * (2 * C::PK / 16),
-                                     idesc, !t.first || kk > 0);
-                mma_commit(pv_done + (t.i & 1));
-                if (t.last) mma_commit(o_full + t.po / C::HH);
+                            mma_e4m3(oo + (l.po + h) * N, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * (2 * C::PK / 16),
+                                     idesc, !l.first || kk > 0);
+                mma_commit(pv_done + (t & 1));
+                if (l.last) mma_commit(o_full + l.po / C::HH);
                 mma_commit(empty_v + st);
-            };
-            auto flush = [&]() {
-                while (nlate) values(weights());
-            };
-            for (uint32_t n = 0;; n++) {
-                // but not behind a group that is not there yet or has no tile: whoever is to make room for one
-                // may be waiting for them
-                if (n > 0 && !mbar_try_wait(seg_full + n % SQ, (n / SQ) & 1)) {
-                    flush();
-                    if (!wait_for(seg_full + n % SQ, (n / SQ) & 1, nullptr, a.err)) break;
-                }
-                g = segs[n % SQ];
-                mbar_arrive(seg_empty + n % SQ);
-                if (g.k0 < 0) break;
-                if (g.nblk == 0) {
-                    flush();
-                    continue;
-                }
-                const int qb = qi % QB, k0 = g.k0, k1 = g.k1, nblk = g.nblk;
-                if (!mbar_try_wait(q_full + qb, (qi / QB) & 1)) flush();
-                const bool q_here = wait_for(q_full + qb, (qi / QB) & 1, &dead, a.err);
-                const uint64_t qd = qdesc + (uint32_t)(qb * (N * HD / 16));
-                for (int k = k0; k < k1; k++) {
-                    const int st = i % NK;
-                    const bool there = nlate < 2 || weights();   // with LAG 2: then its scores' buffer is free, too
-                    if (wait_for(full_k + st, (i / NK) & 1, &dead, a.err) && q_here) {
-                        tc_after();
-                        const uint64_t kd = kdesc + (uint32_t)(st * (C::SLOT / 16));
-#pragma unroll
-                        for (int kk = 0; kk < HD / 32; kk++)
-                            mma_e4m3(so + (i & 1) * N, kd + kk * 16, qd + kk * 16, idesc, kk > 0);
-#pragma unroll
-                        for (int x = 0; x < C::PG; x++)
-                            if (x == (int)(n % C::PG)) mma_commit(&s_full[x][sets[x]++ & 1]);
-                        mma_commit(empty_k + st);
-                        if (k + 1 == k1) mma_commit(q_empty + qb);
-                    }
-                    if (nlate == C::LAG) values(C::LAG == 2 ? there : weights());
-                    late[nlate++] = Late{i, min(TB, nblk - k * TB), (int)(n % C::PG) * C::HH, k == k0, k + 1 == k1};
-                    i++;
-                }
-                qi++;
             }
-            flush();
+            __syncwarp();
+        };
+        auto flush = [&]() {
+            while (nlate) {
+                const uint32_t t = i - nlate;
+                values(t, weights());
+            }
+        };
+        for (uint32_t n = 0;; n++) {
+            // but not behind a group that is not there yet or has no tile: whoever is to make room for one
+            // may be waiting for them
+            if (n > 0 && !__all_sync(0xffffffffu, mbar_try_wait(seg_full + n % SQ, (n / SQ) & 1))) {
+                flush();
+                if (!wait_for(seg_full + n % SQ, (n / SQ) & 1, nullptr, a.err)) break;
+            }
+            __syncwarp();
+            const int k0 = __shfl_sync(0xffffffffu, segs[n % SQ].k0, 0), k1 = __shfl_sync(0xffffffffu, segs[n % SQ].k1, 0);
+            const int nblk = __shfl_sync(0xffffffffu, segs[n % SQ].nblk, 0);
+            if (lane == 0) mbar_arrive(seg_empty + n % SQ);
+            if (k0 < 0) break;
+            if (nblk == 0) {
+                flush();
+                continue;
+            }
+            const uint32_t qb = qi % QB;
+            if (!__all_sync(0xffffffffu, mbar_try_wait(q_full + qb, (qi / QB) & 1))) flush();
+            const bool q_here = wait_for(q_full + qb, (qi / QB) & 1, &dead, a.err);
+            for (int k = k0; k < k1; k++) {
+                const uint32_t st = i % NK;
+                const bool there = nlate < 2 || weights();   // with LAG 2: then its scores' buffer is free, too
+                const bool ok = wait_for(full_k + st, (i / NK) & 1, &dead, a.err) && q_here;
+                __syncwarp();
+                tc_after();
+                if (one && ok) {
+                    const uint64_t kd = kdesc + st * (C::SLOT / 16), qd = qdesc + qb * (N * HD / 16);
+#pragma unroll
+                    for (int kk = 0; kk < HD / 32; kk++)
+                        mma_e4m3(so + (i & 1) * N, kd + kk * 16, qd + kk * 16, idesc, kk > 0);
+#pragma unroll
+                    for (int x = 0; x < C::PG; x++)
+                        if (x == (int)(n % C::PG)) mma_commit(&s_full[x][sets[x] & 1]);
+                    mma_commit(empty_k + st);
+                    if (k + 1 == k1) mma_commit(q_empty + qb);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int x = 0; x < C::PG; x++) sets[x] += x == (int)(n % C::PG);
+                if (nlate == C::LAG) {
+                    const uint32_t t = i - nlate;
+                    values(t, C::LAG == 2 ? there : weights());
+                }
+                const Late l = {min(TB, nblk - k * TB), (int)(n % C::PG) * C::HH, k == k0, k + 1 == k1};
+                if (nlate == 0) l0 = l;
+                else l1 = l;
+                nlate++;
+                i++;
+            }
+            qi++;
         }
+        flush();
     } else if (warp >= FIRST_Q && (C::PG == 1 || warp < FIRST_Q + Q_WARPS)) {   // ---------- queries
         // a wide tile's first ones by all the warps that have nothing to do yet
         const int qw = warp - FIRST_Q;
