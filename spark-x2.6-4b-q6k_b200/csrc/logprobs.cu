@@ -13,10 +13,15 @@
 // a thread in flight; each thread keeps its own (m, S, A) in base 2, pairs of values by one f32x2
 // instruction, and moves m when a vector of values passes it. The best k (k <= 32) are a list over a
 // warp's lanes, as 64-bit keys (order of the value, then of the index). A vector is looked at again only
-// if its largest value reaches the best k-th value that any warp of the CTA has seen, which starts
-// at the k-th largest of a warp's lane maxima; lists join by half cleaners (5 exchanges). A row alone is
-// cut over many CTAs (rows x splits fill the SMs); the last one to arrive, by a ticket that it resets,
-// joins the parts.
+// if its largest value reaches the best k-th value that the CTA has seen, which starts at the k-th
+// largest of its lane maxima (one row of 131072, 20 alternatives: 8.7 us, and 13.2 when it starts at the
+// best warp's k-th, which 20 of 32 lanes pass); lists join by half cleaners (5 exchanges). A row alone
+// is cut over many CTAs (rows x splits fill the SMs); the last one to arrive, by a ticket that it
+// resets, joins the parts.
+//
+// Measured: 1024 x 131072 bf16, 5 alternatives, 63 us (4.3 TB/s, 0.66 of a copy's rate); 61 x 50021
+// f16, 1 alternative, 8.6 us; 1 x 131072 f32, 20 alternatives, 8.7 us, of which 1 us is the load, 3 the
+// launch and the ticket, and the rest the lists: compare and exchange, one behind the other.
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -119,7 +124,12 @@ __device__ __forceinline__ Key clean(Key k, int lane) {   // a bitonic sequence,
     for (int o = 16; o > 0; o >>= 1) k = exchange(k, o, !(lane & o));
     return k;
 }
-__device__ __forceinline__ Key sort32(Key k, int lane) {   // descending
+__device__ __forceinline__ float exchange(float k, int o, bool large) {
+    const float p = __shfl_xor_sync(0xffffffffu, k, o);
+    return large ? fmaxf(k, p) : fminf(k, p);
+}
+template <typename K>
+__device__ __forceinline__ K sort32(K k, int lane) {   // descending
 #pragma unroll
     for (int n = 2; n <= 32; n <<= 1)
 #pragma unroll
@@ -187,6 +197,7 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
     __shared__ Key wk[LP_WARPS][32];
     __shared__ uint32_t bar_s;                 // order of the best k-th value seen
     __shared__ int last_in;
+    __shared__ float tops[32];
     __shared__ __align__(16) uint32_t look_s[LP_WARPS][UN * 4];   // one lane's values, for the whole warp to look at
     pdl_trigger();
     pdl_wait();
@@ -280,18 +291,17 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
             a2 = pack2(t2.x, t2.y);
         }
         if (!a.top) return;
-        if (!barred) {   // a first bar: the k-th largest of the warp's lane maxima, the best warp's
+        if (!barred) {
+            // a first bar: the k-th largest of a warp's lane maxima, the best warp's, or the k-th largest of 32
+            // of the CTA's, the same number of each warp's largest, if that is more
             barred = true;
-            float k = mx;
-#pragma unroll
-            for (int n = 2; n <= 32; n <<= 1)
-#pragma unroll
-                for (int o = n >> 1; o > 0; o >>= 1) {
-                    const float p = __shfl_xor_sync(0xffffffffu, k, o);
-                    k = !(lane & o) == !(lane & n) ? fmaxf(k, p) : fminf(k, p);
-                }
+            constexpr int EACH = 32 / LP_WARPS;
+            float k = sort32(mx, lane);
             if (lane == kth) atomicMax(&bar_s, order_of(k));
+            if (lane < EACH) tops[warp * EACH + lane] = k;
             __syncthreads();
+            k = sort32(tops[lane], lane);
+            tv = __shfl_sync(0xffffffffu, k, kth);
         }
         const float seen = value_of((Key) * (volatile uint32_t *)&bar_s << 32);
         tv = fmaxf(tv, seen);
@@ -418,14 +428,16 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float *pc = p + (size_t)min(c0 + i * LP_WARPS, a.splits - 1) * LP_PART;
-                q[i] = Stat{__ldcg(pc), __ldcg(pc + 1), __ldcg(pc + 2)};
-                k[i] = __ldcg(reinterpret_cast<const Key *>(pc + 4) + 31 - lane);
+                const bool in = c0 + i * LP_WARPS < a.splits;
+                q[i] = in ? Stat{__ldcg(pc), __ldcg(pc + 1), __ldcg(pc + 2)} : Stat{-INFINITY, 0.f, 0.f};
+                k[i] = in ? __ldcg(reinterpret_cast<const Key *>(pc + 4) + (i & 1 ? 31 - lane : lane)) : 0;
             }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (c0 + i * LP_WARPS >= a.splits) break;
-                if (lane == 0) st = join(st, q[i]);
-                if (a.top) list = merge(list, k[i], lane);
+            if (lane == 0) st = join(st, join(join(q[0], q[1]), join(q[2], q[3])));
+            if (a.top) {
+                k[0] = merge(k[0], k[1], lane);
+                k[2] = merge(k[2], k[3], lane);
+                list = merge(list, __shfl_sync(0xffffffffu, merge(k[0], __shfl_sync(0xffffffffu, k[2], 31 - lane), lane),
+                                               31 - lane), lane);
             }
         }
         cta();
@@ -449,8 +461,8 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
 
 // The CTAs of a row and their threads. An SM holds 768 threads: 6 CTAs of 128, so that about as many
 // rows (or parts of rows) as the SMs hold run side by side and share the memory until the end; few
-// rows go over up to 64 CTAs of 512 threads each, whose 16 warps join the parts' lists faster
-// (131072 f32 values, 20 alternatives: see the file's head). A CTA has at least one tile of values.
+// rows go over up to 64 CTAs of 512 threads each, whose 16 warps join the parts' lists faster. A CTA
+// has at least one vector a thread.
 int plan(const LpArgs &a, int size, int *chunk, int *threads) {
     const int slots = 6 * sm_count();
     *threads = (long long)a.rows * LP_SPLITS <= slots ? 512 : 128;
