@@ -20,7 +20,7 @@
 // resets, joins the parts.
 //
 // Measured: 1024 x 131072 bf16, 5 alternatives, 63 us (4.3 TB/s, 0.66 of a copy's rate); 61 x 50021
-// f16, 1 alternative, 8.6 us; 1 x 131072 f32, 20 alternatives, 8.7 us, of which 1 us is the load, 3 the
+// f16, 1 alternative, 8.6 us; 1 x 131072 f32, 20 alternatives, 8.5 us, of which 1 us is the load, 3 the
 // launch and the ticket, and the rest the lists: compare and exchange, one behind the other.
 #include <cuda_bf16.h>
 
@@ -459,16 +459,20 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
     }
 }
 
-// The CTAs of a row and their threads. An SM holds 768 threads: 6 CTAs of 128, so that about as many
-// rows (or parts of rows) as the SMs hold run side by side and share the memory until the end; few
-// rows go over up to 64 CTAs of 512 threads each, whose 16 warps join the parts' lists faster. A CTA
-// has at least one vector a thread.
+// The CTAs of a row and their threads. Few rows, whose tiles of 4 vectors a thread (32 KB) are no more
+// than the SMs: CTAs of 512 threads, one an SM, one tile each; their 16 warps look at a tile's best and
+// join the parts' lists faster (12 x 131072 bf16, 8 alternatives: 8.0 us, and 11.3 with 128 threads;
+// 64 x 10000: 5.0 and 9.1), and smaller tiles would only make more parts (12 x 10000: 4.9, and 9.1 as 3
+// parts of a vector a thread). Else an SM holds 6 CTAs of 128 threads, so that about as many rows (or parts of
+// rows) as the SMs hold run side by side and share the memory until the end (24 x 131072: 9.8 us, and
+// 13.2 with 512), and so for rows that 128 threads read at once (12 x 1000: 5.5 us, and 6.8 with 512).
 int plan(const LpArgs &a, int size, int *chunk, int *threads) {
-    const int slots = 6 * sm_count();
-    *threads = (long long)a.rows * LP_SPLITS <= slots ? 512 : 128;
-    const int tile = *threads * (16 / size);
-    long long s = *threads == 512 ? LP_SPLITS : slots / a.rows;
-    const long long most = ((long long)a.vocab + tile - 1) / tile;
+    const int slots = 6 * sm_count(), n = 16 / size;
+    const long long tiles = ((long long)a.vocab + 4 * 512 * n - 1) / (4 * 512 * n);
+    *threads = a.vocab > 128 * n && a.rows * tiles <= sm_count() ? 512 : 128;
+    const int tile = *threads * n;
+    long long s = *threads == 512 ? tiles : slots / a.rows;
+    const long long most = ((long long)a.vocab + tile - 1) / tile;   // a vector a thread at least
     if (s > most) s = most;
     if (s > LP_SPLITS) s = LP_SPLITS;
     if (s < 1) s = 1;
