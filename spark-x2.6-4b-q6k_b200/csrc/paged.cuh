@@ -57,12 +57,44 @@ __device__ __forceinline__ void unit_dims(int u, int pdim, int &d0, int &d1) {
     }
 }
 
+// Two f32 side by side, each operation rounded as its scalar form.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // Cosine and sine of the f32 product position * frequency (model.rs:431-439's angle). The whole turns
-// are taken out in f64, where a turn count up to 2^24 still leaves 29 bits of the fraction, and the
-// rest goes to sincospi: one path for every position, where sincosf branches at large angles.
+// are taken out with 1 / 2 pi as the sum of two f32 and the product's own rounding error added, so a turn
+// count up to 2^24 still leaves 24 bits of the fraction, and the rest goes to sincospi: one path for every
+// position, where sincosf branches at large angles.
 __device__ __forceinline__ void angle(int pos, float freq, float &c, float &s) {
-    const double turns = (double)__fmul_rn((float)pos, freq) * 0.15915494309189533577;
-    sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+    constexpr double INV = 0.15915494309189533577;
+    constexpr float HI = (float)INV, LO = (float)(INV - (double)HI);
+    const float p = __fmul_rn((float)pos, freq), t = __fmul_rn(p, HI);
+    const float rest = __fmaf_rn(p, LO, __fmaf_rn(p, HI, -t));
+    sincospif(2.0f * ((t - rintf(t)) + rest), &s, &c);
 }
 
 // 8 values of a row as they lie in memory: two pieces of 4 (dims d0 .. and d1 ..)
@@ -118,11 +150,13 @@ struct Raw {
 
 // The rotation of a unit's 4 pairs, each product rounded (model.rs:431-439).
 __device__ __forceinline__ void rotate_unit(float (&a)[4], float (&b)[4], const float (&c)[4], const float (&s)[4]) {
+    const f32x2 minus = pack2(-1.0f, -1.0f);
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float p = a[i], q = b[i];
-        a[i] = __fsub_rn(__fmul_rn(p, c[i]), __fmul_rn(q, s[i]));
-        b[i] = __fadd_rn(__fmul_rn(q, c[i]), __fmul_rn(p, s[i]));
+    for (int i = 0; i < 4; i += 2) {
+        const f32x2 p = pack2(a[i], a[i + 1]), q = pack2(b[i], b[i + 1]), cc = pack2(c[i], c[i + 1]), ss = pack2(s[i], s[i + 1]);
+        const float2 x = unpack2(fma2(mul2(q, ss), minus, mul2(p, cc))), y = unpack2(add2(mul2(q, cc), mul2(p, ss)));
+        a[i] = x.x, a[i + 1] = x.y;
+        b[i] = y.x, b[i + 1] = y.y;
     }
 }
 

@@ -45,8 +45,8 @@ namespace {
 
 constexpr int AP_WARPS = 4, AP_THREADS = AP_WARPS * 32, AP_ROWS = BLOCK / AP_WARPS;
 constexpr int AP_WIDTH = 256;              // values of a row that a warp takes at once
-constexpr int AP_CTAS = 6;                 // CTAs of an SM
-constexpr int AP_BLOCKS = 8;               // the most blocks of a CTA
+template <typename T>
+constexpr int AP_CTAS = sizeof(T) == 4 ? 5 : 6;   // CTAs of an SM: two items' rows stay in registers
 
 struct AppendArgs {
     Pool pool;
@@ -56,7 +56,7 @@ struct AppendArgs {
     int kvec, vvec;                        // alignment of the rows' pieces: 0 none, 1 four values, 2 eight too
     const float *freq;
     int pdim;
-    int passes, blocks;                    // head groups and blocks of a CTA
+    int passes;                            // head groups of a CTA
     int *err;
 };
 
@@ -82,14 +82,14 @@ __device__ __forceinline__ float2 e4m3x2_f32(uint32_t w) {
 __device__ __forceinline__ int spread(int piece) { return piece ^ ((piece >> 3) & 7); }
 
 // A block that the call appends to: its page and place in it, its first position, the call's rows
-// lo .. hi - 1 of it; row r of the block is row `row` + r of the call. hi 0: no block.
+// lo .. hi - 1 of it; row r of the block is row `row` + r of the call.
 struct Block {
     int page, bp, pos, lo, hi, row;
 };
 
 template <typename T, int HD, bool KEYS>
-__device__ __forceinline__ void append_blocks(const AppendArgs &a, const Block *blocks, int nb, uint8_t *tile, float2 *turn,
-                                              float (*wmax)[AP_WARPS]) {
+__device__ __forceinline__ void append_block(const AppendArgs &a, const Block b, uint8_t *tile, float *turn_c,
+                                             float *turn_s, float (*wmax)[AP_WARPS]) {
     constexpr int LPR = HD / 8, GH = AP_WIDTH / HD, PER = AP_WIDTH / AP_THREADS;   // lanes of a head; heads; pieces of a thread
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPR, u = lane % LPR;
     const int pdim = KEYS ? a.pdim : 0, half = pdim / 2;
@@ -101,37 +101,34 @@ __device__ __forceinline__ void append_blocks(const AppendArgs &a, const Block *
     const long long ld = KEYS ? a.ldk : a.ldv;
     const int vec = KEYS ? a.kvec : a.vvec;
     const int g0 = blockIdx.y * a.passes, groups = min(a.passes, (a.pool.kv_heads + GH - 1) / GH - g0);
-    // item: a head group of a block; its rows come while the one before is worked on
+    const int lo = b.lo, hi = b.hi, page = b.page, bp = b.bp;
+    // a head group's rows come while the one before is worked on
     Raw<T> next[AP_ROWS];
-    auto fetch = [&](int it) {
-        const Block &b = blocks[it / groups];
-        const int head = (g0 + it % groups) * GH + sub;
+    auto fetch = [&](int g) {
+        const int head = g * GH + sub, from = head < a.pool.kv_heads ? lo : BLOCK;
+        const T *at = rows + (long long)(b.row + 2 * warp) * ld + (long long)head * HD;
 #pragma unroll
         for (int i = 0; i < AP_ROWS; i++) {
             // warp w: rows 2w, 2w + 1, 2w + 8, 2w + 9, which are bytes 4w .. 4w + 3 of a value dim
-            const int r = 2 * warp + (i & 1) + 8 * (i >> 1);
-            if (head < a.pool.kv_heads && r >= b.lo && r < b.hi)
-                next[i].load(rows + (size_t)(b.row + r) * ld + (size_t)head * HD, d0, d1, vec);
+            const int dr = (i & 1) + 8 * (i >> 1), r = 2 * warp + dr;
+            if (r >= from && r < hi) next[i].load(at + dr * ld, d0, d1, vec);
             else next[i].none();
         }
     };
-    fetch(0);
-    for (int it = 0; it < nb * groups; it++) {
-        const Block b = blocks[it / groups];
-        const int g = g0 + it % groups, lo = b.lo, hi = b.hi, page = b.page, bp = b.bp;
-        if constexpr (KEYS)
-            if (half && it % groups == 0) {   // the rows' angles, for all heads
-                for (int i = threadIdx.x; i < BLOCK * half; i += AP_THREADS) {
-                    const int r = i / half;
-                    if (r >= lo && r < hi) angle(b.pos + r, __ldg(a.freq + i - r * half), turn[i].x, turn[i].y);
-                }
-                __syncthreads();
-            }
+    fetch(g0);
+    if constexpr (KEYS)
+        if (half) {   // the rows' angles, for all heads
+            for (int r = warp; r < BLOCK; r += AP_WARPS)
+                if (r >= lo && r < hi)
+                    for (int i = lane; i < half; i += 32)
+                        angle(b.pos + r, __ldg(a.freq + i), turn_c[r * half + i], turn_s[r * half + i]);
+            __syncthreads();
+        }
+    for (int g = g0; g < g0 + groups; g++) {
         float x[AP_ROWS][8];
 #pragma unroll
         for (int i = 0; i < AP_ROWS; i++) next[i].f32(x[i]);
-        if (it + 1 < nb * groups) fetch(it + 1);
-        if (hi == 0) continue;   // the same for the CTA
+        if (g + 1 < g0 + groups) fetch(g + 1);
         const int head = g * GH + sub;
         const bool real = head < a.pool.kv_heads;
         const size_t bi = block_index(a.pool, page, min(head, a.pool.kv_heads - 1), bp);
@@ -153,9 +150,9 @@ __device__ __forceinline__ void append_blocks(const AppendArgs &a, const Block *
             for (int i = 0; i < AP_ROWS; i++) {
                 const int r = 2 * warp + (i & 1) + 8 * (i >> 1);
                 if (r < lo || r >= hi) continue;
-                const float4 *t = reinterpret_cast<const float4 *>(turn + r * half + d0);
-                const float4 t0 = t[0], t1 = t[1];
-                const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y, t0.w, t1.y, t1.w};
+                const float4 c4 = *reinterpret_cast<const float4 *>(turn_c + r * half + d0);
+                const float4 s4 = *reinterpret_cast<const float4 *>(turn_s + r * half + d0);
+                const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
                 float p[4], q[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) p[e] = x[i][e], q[e] = x[i][4 + e];
@@ -211,13 +208,19 @@ __device__ __forceinline__ void append_blocks(const AppendArgs &a, const Block *
         }
         // the new rows (all of the tile when nothing earlier is in the block); none where the scale is no number
         const float inv = __fdiv_rn(1.0f, d);
-        const bool fine = d < INFINITY;
         uint32_t q[AP_ROWS][4];   // e4m3 pairs
 #pragma unroll
         for (int i = 0; i < AP_ROWS; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                q[i][e] = fine ? e4m3x2(__fmul_rn(x[i][2 * e], inv), __fmul_rn(x[i][2 * e + 1], inv)) : 0u;
+            for (int e = 0; e < 4; e++) {
+                const float2 y = unpack2(mul2(pack2(x[i][2 * e], x[i][2 * e + 1]), pack2(inv, inv)));
+                q[i][e] = e4m3x2(y.x, y.y);
+            }
+        if (!(d < INFINITY))
+#pragma unroll
+            for (int i = 0; i < AP_ROWS; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) q[i][e] = 0;
         if (KEYS) {
 #pragma unroll
             for (int i = 0; i < AP_ROWS; i++) {
@@ -256,59 +259,50 @@ __device__ __forceinline__ void append_blocks(const AppendArgs &a, const Block *
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(AP_THREADS, AP_CTAS) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(AP_THREADS, AP_CTAS<T>) append_kernel(const AppendArgs a) {
     __shared__ __align__(16) uint8_t tile[BLOCK * AP_WIDTH];
-    __shared__ __align__(16) float2 turn[BLOCK * HD / 2];
+    __shared__ __align__(16) float turn_c[BLOCK * HD / 2], turn_s[BLOCK * HD / 2];
     __shared__ float wmax[AP_WIDTH / HD][AP_WARPS];
-    __shared__ int4 who[AP_BLOCKS];      // sequence, its first row, its rows, its cached tokens
-    __shared__ Block blocks[AP_BLOCKS];
+    __shared__ int4 who;      // sequence, its first row, its rows, its cached tokens
     pdl_trigger();
-    if (threadIdx.x < AP_BLOCKS) who[threadIdx.x].x = -1;
+    if (threadIdx.x == 0) who.x = -1;
     __syncthreads();
     pdl_wait();
-    const int u0 = blockIdx.x * a.blocks;
+    const int unit = blockIdx.x;
     // Units of sequence s: row0[s] / 16 + 2 s up to the next one's; n rows touch at most
     // n / 16 + 2 blocks, so each sequence's blocks fit.
     for (int s = threadIdx.x; s < a.b.nseq; s += AP_THREADS) {
         const int r0 = __ldg(a.b.row0 + s), r1 = __ldg(a.b.row0 + s + 1), len = __ldg(a.b.kv_len + s);
-        const int b0 = r0 / BLOCK + 2 * s, b1 = r1 / BLOCK + 2 * s + 2;
-        if (r1 > r0)
-            for (int u = max(b0, u0); u < min(b1, u0 + a.blocks); u++) who[u - u0] = make_int4(s, r0, r1 - r0, len);
+        if (r1 > r0 && unit >= r0 / BLOCK + 2 * s && unit < r1 / BLOCK + 2 * s + 2) who = make_int4(s, r0, r1 - r0, len);
     }
     __syncthreads();
-    if (threadIdx.x < a.blocks) {
-        const int4 w = who[threadIdx.x];
-        const int first = w.w - w.z, blk = first / BLOCK + (u0 + (int)threadIdx.x - w.y / BLOCK - 2 * w.x);
-        const int per = a.pool.page_tokens / BLOCK;
-        Block b{0, 0, 0, 0, 0, 0};
-        if (w.x >= 0 && (first < 0 || blk * BLOCK < w.w)) {
-            int page = -1;
-            if (first >= 0 && blk >= 0 && w.y >= 0 && w.y + w.z <= a.b.rows && blk / per < a.b.max_pages)
-                page = __ldg(a.b.table + (size_t)w.x * a.b.max_pages + blk / per);
-            if (page >= 0 && page < a.pool.pages)
-                b = Block{page, blk % per, blk * BLOCK, max(first - blk * BLOCK, 0), min(w.w - blk * BLOCK, BLOCK),
-                          w.y + blk * BLOCK - first};
-            else if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
-        }
-        blocks[threadIdx.x] = b;
+    const int4 w = who;
+    const int first = w.w - w.z, blk = first / BLOCK + (unit - w.y / BLOCK - 2 * w.x);
+    if (w.x < 0 || (first >= 0 && blk * BLOCK >= w.w)) return;   // no block
+    const int per = a.pool.page_tokens / BLOCK;
+    int page = -1;
+    if (first >= 0 && blk >= 0 && w.y >= 0 && w.y + w.z <= a.b.rows && blk / per < a.b.max_pages)
+        page = __ldg(a.b.table + (size_t)w.x * a.b.max_pages + blk / per);
+    if (page < 0 || page >= a.pool.pages) {
+        if (a.err && threadIdx.x == 0) atomicExch(a.err, DEV_BAD_INDEX);
+        return;
     }
-    __syncthreads();
-    if (blockIdx.z == 0) append_blocks<T, HD, true>(a, blocks, a.blocks, tile, turn, wmax);
-    else append_blocks<T, HD, false>(a, blocks, a.blocks, tile, turn, wmax);
+    const Block b{page, blk % per, blk * BLOCK, max(first - blk * BLOCK, 0), min(w.w - blk * BLOCK, BLOCK), w.y + blk * BLOCK - first};
+    if (blockIdx.z == 0) append_block<T, HD, true>(a, b, tile, turn_c, turn_s, wmax);
+    else append_block<T, HD, false>(a, b, tile, turn_c, turn_s, wmax);
 }
 
 template <typename T, int HD>
 cudaError_t launch(AppendArgs a, cudaStream_t s) {
     const int groups = (a.pool.kv_heads + AP_WIDTH / HD - 1) / (AP_WIDTH / HD);
-    // A CTA takes all head groups of a block, and then up to AP_BLOCKS blocks, as long as every SM
-    // still gets its CTAs: the groups share a block's angles, the blocks hide each other's loads.
-    const int slots = AP_CTAS * sm_count(), units = a.b.rows / BLOCK;   // whole blocks: about what there is to do
-    long long most = 2ll * groups * units / slots;
+    // A CTA walks several head groups of its block, as long as every SM still gets its CTAs: they share the
+    // block's angles and hide each other's loads (16384 bf16 rows of 4 groups: 28 us with all 4, 30.6 with 2,
+    // 38.5 with 1; 4096 rows: 10.0 with 2, 10.4 with 1, 12.8 with 4; one row: 3.8 with 1, 5.3 with 2).
+    const int slots = AP_CTAS<T> * sm_count(), units = a.b.rows / BLOCK;   // whole blocks: about what there is to do
+    const long long most = 2ll * groups * units / slots;
     a.passes = most < 1 ? 1 : most < groups ? (int)most : groups;
     a.passes = (groups + (groups + a.passes - 1) / a.passes - 1) / ((groups + a.passes - 1) / a.passes);
-    most /= groups;
-    a.blocks = most < 1 ? 1 : most < AP_BLOCKS ? (int)most : AP_BLOCKS;
-    const dim3 grid((a.b.rows / BLOCK + 2 * a.b.nseq + a.blocks - 1) / a.blocks, (groups + a.passes - 1) / a.passes, 2);
+    const dim3 grid(units + 2 * a.b.nseq, (groups + a.passes - 1) / a.passes, 2);
     return launch_pdl(append_kernel<T, HD>, grid, dim3(AP_THREADS), 0, s, a);
 }
 template <typename T>
@@ -338,7 +332,7 @@ extern "C" int spk_paged_append(const spk_kv_pool *pool, const spk_kv_batch *bat
     if ((uintptr_t)k % size || (uintptr_t)v % size) return set_error("%s: unaligned rows", who);
     if (pool->kv_heads > 65535) return set_error("%s: %d KV heads", who, pool->kv_heads);
     const AppendArgs a{pool_of(pool), batch_of(batch), k, v, ldk, ldv, rows_aligned(k, ldk, size), rows_aligned(v, ldv, size),
-                       freq, freq ? pdim : 0, 1, 1, device_error_ptr()};
+                       freq, freq ? pdim : 0, 1, device_error_ptr()};
     const cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = type == T_F32   ? launch<float>(a, s)
                           : type == T_F16 ? launch<__half>(a, s)
