@@ -81,10 +81,11 @@ __device__ __forceinline__ float2 e4m3x2_f32(uint32_t w) {
 // 16-byte piece of the staging tile, spread so that a warp's 4-byte writes (pieces 8 apart) meet few banks
 __device__ __forceinline__ int spread(int piece) { return piece ^ ((piece >> 3) & 7); }
 
-// A block that the call appends to: its page and place in it, its first position, the call's rows
-// lo .. hi - 1 of it; row r of the block is row `row` + r of the call.
+// A block that the call appends to: its place in the pool for KV head 0, its first position, the
+// call's rows lo .. hi - 1 of it; row r of the block is row `row` + r of the call.
 struct Block {
-    int page, bp, pos, lo, hi, row;
+    size_t at;
+    int pos, lo, hi, row;
 };
 
 template <typename T, int HD, bool KEYS>
@@ -101,7 +102,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const Block b,
     const long long ld = KEYS ? a.ldk : a.ldv;
     const int vec = KEYS ? a.kvec : a.vvec;
     const int g0 = blockIdx.y * a.passes, groups = min(a.passes, (a.pool.kv_heads + GH - 1) / GH - g0);
-    const int lo = b.lo, hi = b.hi, page = b.page, bp = b.bp;
+    const int lo = b.lo, hi = b.hi, per = a.pool.page_tokens / BLOCK;
     // a head group's rows come while the one before is worked on
     Raw<T> next[AP_ROWS];
     auto fetch = [&](int g) {
@@ -131,7 +132,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const Block b,
         if (g + 1 < g0 + groups) fetch(g + 1);
         const int head = g * GH + sub;
         const bool real = head < a.pool.kv_heads;
-        const size_t bi = block_index(a.pool, page, min(head, a.pool.kv_heads - 1), bp);
+        const size_t bi = b.at + (size_t)min(head, a.pool.kv_heads - 1) * per;
         // earlier rows and their scale, on their way while the new rows come in
         uint4 old[PER];
         float d_old = 0.f;
@@ -141,7 +142,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const Block b,
             for (int i = 0; i < PER; i++) {
                 const int pc = i * AP_THREADS + threadIdx.x, hd = g * GH + pc / HD;
                 if (hd < a.pool.kv_heads)
-                    old[i] = reinterpret_cast<const uint4 *>(pool + block_index(a.pool, page, hd, bp) * (BLOCK * HD))[pc % HD];
+                    old[i] = reinterpret_cast<const uint4 *>(pool + (b.at + (size_t)hd * per) * (BLOCK * HD))[pc % HD];
             }
         }
         float mx = 0.f;
@@ -179,7 +180,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const Block b,
                 float m2 = max_nan(max_nan(wmax[hs][0], wmax[hs][1]), max_nan(wmax[hs][2], wmax[hs][3]));
                 const int hd = g * GH + hs;
                 if (hd >= a.pool.kv_heads) continue;
-                const float o2 = scales[block_index(a.pool, page, hd, bp)];
+                const float o2 = scales[b.at + (size_t)hd * per];
                 m2 = max_nan(max_nan(__fdiv_rn(m2, E4M3_MAX), SCALE_MIN), o2);
                 const float ratio = m2 > o2 ? __fdiv_rn(o2, m2) : 1.0f;
                 // keys: piece = (8-token group, 16-dim chunk, token): one token; values: one dim's 16 tokens
@@ -251,7 +252,7 @@ __device__ __forceinline__ void append_block(const AppendArgs &a, const Block b,
         for (int i = 0; i < PER; i++) {
             const int pc = i * AP_THREADS + threadIdx.x, hd = g * GH + pc / HD;
             if (hd < a.pool.kv_heads)
-                reinterpret_cast<uint4 *>(pool + block_index(a.pool, page, hd, bp) * (BLOCK * HD))[pc % HD] =
+                reinterpret_cast<uint4 *>(pool + (b.at + (size_t)hd * per) * (BLOCK * HD))[pc % HD] =
                     reinterpret_cast<const uint4 *>(tile)[spread(pc)];
         }
         if (u == 0 && warp == 0 && real) scales[bi] = d;
@@ -287,7 +288,8 @@ __global__ void __launch_bounds__(AP_THREADS, AP_CTAS<T>) append_kernel(const Ap
         if (a.err && threadIdx.x == 0) atomicExch(a.err, DEV_BAD_INDEX);
         return;
     }
-    const Block b{page, blk % per, blk * BLOCK, max(first - blk * BLOCK, 0), min(w.w - blk * BLOCK, BLOCK), w.y + blk * BLOCK - first};
+    const Block b{block_index(a.pool, page, 0, blk % per), blk * BLOCK, max(first - blk * BLOCK, 0),
+                  min(w.w - blk * BLOCK, BLOCK), w.y + blk * BLOCK - first};
     if (blockIdx.z == 0) append_block<T, HD, true>(a, b, tile, turn_c, turn_s, wmax);
     else append_block<T, HD, false>(a, b, tile, turn_c, turn_s, wmax);
 }
