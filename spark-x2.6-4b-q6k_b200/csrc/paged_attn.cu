@@ -252,6 +252,14 @@ __device__ __forceinline__ bool bar_or(int id, int n, bool x) {
     return r != 0;
 }
 
+// Not inlined: an SM fetches a call's instructions anew (about 100 KB), and a dozen copies of this one were 5 to
+// 10 KB of them (64 sequences 41.5 -> 40.2 us, 24 x 8 drafted tokens 31.2 -> 30.4).
+__device__ __noinline__ float2 turn_of(int pos, float freq) {
+    float2 t;
+    angle(pos, freq, t.x, t.y);
+    return t;
+}
+
 // ------------------------------------------------------------------ the line of work
 // Lengths are in blocks and fit 32 bits (the entry point refuses a batch that could not).
 struct Seq {
@@ -692,7 +700,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             auto turn = [&](int tok) {   // the heads of a token share its angles
                 if (lane < a.pdim / 8 && tok != turned) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) angle(pos0 + tok, fr[e], cs[e], sn[e]);
+                    for (int e = 0; e < 4; e++) {
+                        const float2 t = turn_of(pos0 + tok, fr[e]);
+                        cs[e] = t.x, sn[e] = t.y;
+                    }
                     turned = tok;
                 }
             };
@@ -1156,19 +1167,26 @@ int launch_one(const AttnParams &a, cudaStream_t s, const char *who) {
     return e == cudaSuccess ? 0 : cuda_fail(who, e);
 }
 
-// The columns follow the rows that a sequence has per KV head on average: the narrowest tile that
-// holds them, since a tile's cost grows with its columns and a second tile reads the cache again.
+// The columns follow the rows that a sequence has per KV head on average. A tile's cost grows with its
+// columns and a second tile reads the cache again, from L2; where the one outweighs the other was measured
+// (us; 64 sequences of up to 3000 keys, 8 of 6000, 1 of 16000; heads of 256):
+//   f32   8 rows: 6 a tile 41.3 21.8 26.1, 24 a tile 42.5 24.2 29.0;  16 rows: 51.0 23.6 30.7, 46.5 27.4 33.6
+//   f16   8 rows: 5 a tile 38.9 20.8 25.3, 10 a tile 32.7 23.7 29.3;  24 rows: 10 a tile 50.5 27.5 33.7, 32 a
+//         tile 43.8 29.0 40.6;  32 rows: 54.1 34.7 37.7, 42.7 31.6 45.5
+//   bf16 128 rows: 32 a tile of three terms 51.6 46.6 51.3, 64 of two 62.8 53.9 58.6;  256 rows: 66.9 53.3 71.4,
+//         67.7 52.3 70.6;  1024 rows, 8 and 1 sequences: 157.7 209.9, 137.9 149.5
 template <typename T, int HD>
 int launch(const AttnParams &a, cudaStream_t s, const char *who) {
     const long long per = ((long long)a.b.rows * a.group + a.b.nseq - 1) / a.b.nseq;
     if constexpr (sizeof(T) == 4) {
-        if (per <= 6) return launch_one<T, Cfg<HD, 32, 5, 6, 1, 2>>(a, s, who);
+        if (per <= 12) return launch_one<T, Cfg<HD, 32, 5, 6, 1, 2>>(a, s, who);
         return launch_one<T, Cfg<HD, 128, 5, 24, 3, 1>>(a, s, who);
     } else {
         if (per <= 5) return launch_one<T, Cfg<HD, 16, 3, 5, 1, 2>>(a, s, who);
-        if (per <= 10) return launch_one<T, Cfg<HD, 32, 3, 10, 1, 2>>(a, s, who);
-        if constexpr (__is_same(T, __half)) return launch_one<T, Cfg<HD, 96, 3, 32, 4, 1>>(a, s, who);
-        else return launch_one<T, Cfg<HD, 128, 2, 64, 4, 1>>(a, s, who);
+        if (per <= 24) return launch_one<T, Cfg<HD, 32, 3, 10, 1, 2>>(a, s, who);
+        if constexpr (__is_same(T, __nv_bfloat16))
+            if (per > 192) return launch_one<T, Cfg<HD, 128, 2, 64, 4, 1>>(a, s, who);
+        return launch_one<T, Cfg<HD, 96, 3, 32, 4, 1>>(a, s, who);
     }
 }
 
