@@ -324,6 +324,33 @@ def test_attention_window(cuda, window, typ, rows):
     check_attention(c, typ, window=window, freq=freqs(cuda, 128))
 
 
+# On average 9, 21, 30, 170 and 290 rows of a sequence per KV head: a tile of every width, whole and cut.
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,group,page", [(64, 2, 16), (128, 4, 32), (256, 1, 128)])
+@pytest.mark.parametrize("mean", [9, 21, 30, 170, 290])
+@pytest.mark.parametrize("window", [0, 131])
+def test_attention_tiles_of_every_width(cuda, window, mean, hd, group, page, typ):
+    n = max(1, mean // group)
+    c = Case(cuda, [2 * n - 1, 1], [260, 1000], kv=2, hd=hd, heads=2 * group, page=page, seed=mean + hd)
+    check_attention(c, typ, window=window, freq=freqs(cuda, hd // 2), gate=c.randn(c.heads, typ))
+
+
+@pytest.mark.parametrize("rows", [[1], [12], [60], [300]])
+def test_attention_poison_under_every_width(cuda, rows):
+    """A poisoned block is NaN for the rows that see it and nothing to the rows before it."""
+    import torch
+
+    c = Case(cuda, rows, [40], kv=1, hd=64, heads=2, page=16, seed=2)
+    q = c.randn(c.heads * 64, "bf16")
+    clean = c.batch.attention(q).clone()
+    last = (c.len[0] - 1) // 16                       # the block of the last token
+    c.cache.v_scale[c.table[0][last], 0, 0] = float("nan")
+    got = c.batch.attention(q)
+    assert check_errors() == 0
+    sees = torch.arange(c.len[0] - rows[0], c.len[0], device=cuda) >= 16 * last
+    assert torch.isnan(got[sees]).all() and torch.equal(got[~sees], clean[~sees])
+
+
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
 def test_attention_with_scales_far_apart(cuda, typ):
     """Block scales over 13 orders of magnitude, some of the smallest allowed: no weight is lost under
