@@ -10,13 +10,15 @@
 // so that a block which is read holds nothing that was not appended. A NaN or infinity makes the
 // block's scale NaN or infinite (its rows read as NaN) and never a stored byte.
 //
-// What bounds it: bytes (each value read once, one byte written) for prompts, the chain of
-// dependent loads (sequence -> page -> row) for steps. A CTA of 4 warps takes one block, keys or
-// values, and 256 values of a row at a time (256 / head_dim heads side by side): a warp 4 of the 16
-// rows, a lane 8 values of each, so that a head's amax is a max in registers, a shuffle tree and one
-// exchange between the warps. The bytes meet in shared memory (4 KB, 16-byte pieces spread over the
-// banks) and leave as 16-byte stores. Where there are many blocks a CTA walks several head groups,
-// which share the rows' angles: a cosine and sine cost as much as ten values' rounding and storing.
+// What bounds it: the issue slots for prompts (19 warp instructions per 32 values: conversions, angles,
+// the rotation, addresses), the chain of dependent loads (sequence -> page -> row) for steps. A CTA of 4
+// warps takes one block, keys or values, and 256 values of a row at a time (256 / head_dim heads
+// side by side): a warp 4 of the 16 rows, a lane 8 values of each, so that a head's amax is a max in registers, a
+// shuffle tree and one exchange between the warps. The bytes meet in shared memory (4 KB, 16-byte
+// pieces spread over the banks) and leave as 16-byte stores. Where there are many blocks a CTA walks
+// several head groups, which share the rows' angles: a cosine and sine cost as much as ten values'
+// rounding and storing. Measured: 16384 bf16 rows of 4 heads of 256, keys and values, 27 us (101 MB, 3.7 TB/s, 0.57
+// of a copy's rate); 13 f32 prompts of up to 1501 rows 12.8 us (44 MB); one row 3.7 us.
 #include "paged.cuh"
 
 namespace spk {
