@@ -227,9 +227,9 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
     const int kth = max(a.top, 1) - 1;
     float tv = a.top ? -INFINITY : NAN;        // what a value has to reach; nothing reaches a NaN
     bool barred = false;
-    // UN vectors of this thread, the first at value i0, the others STEP values apart; edge: some of
-    // their values lie outside of the range (they are -inf) and are not tokens
-    auto eat = [&](const uint32_t (&w)[UN][4], int i0, int used, bool edge) {
+    // UN vectors of this thread, the first at value i0, the others STEP values apart; edge: those
+    // before c0 and from `stop` on are not this call's (they are -inf) and are not offered
+    auto eat = [&](const uint32_t (&w)[UN][4], int i0, int used, bool edge, int stop) {
         constexpr int STEP = LP_THREADS * N;
         uint32_t q = V::max_(V::max_(w[0][0], w[0][1]), V::max_(w[0][2], w[0][3]));
 #pragma unroll
@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
             const float2 f = V::two(q);
             mx = fmaxf(f.x, f.y);
         }
+        mx = fmaxf(mx, -INFINITY);   // nothing but NaN ranks as -inf
         if (mx > st.m) {
             const float2 s = unpack2(s2), t = unpack2(a2);
             st.s = s.x + s.y;
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
             for (int h = 0; h < UN * N; h += 32) {   // 16 or 32 values
                 const int v = h + lane, i = base + (v / N) * STEP + v % N;
                 Key k = 0;
-                if (v < UN * N && (!edge || (i >= c0 && i < c1))) {
+                if (v < UN * N && (!edge || (i >= c0 && i < stop))) {
                     const float f = fmaxf(V::one(reinterpret_cast<const T *>(look_s[warp]) + v), -INFINITY);
                     if (f >= tv) k = key_of(f, i);
                 }
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
             uint32_t n[UN][4];
             const bool more = b + STRIDE < full;
             if (more) fetch(n, b + STRIDE);
-            eat(w, (b + (int)threadIdx.x) * N - mis, UN, false);
+            eat(w, (b + (int)threadIdx.x) * N - mis, UN, false, 0);
             if (more)
 #pragma unroll
                 for (int u = 0; u < UN; u++)
@@ -379,7 +380,8 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
                         }
                 }
             }
-            eat(w, (b + (int)threadIdx.x) * N - mis, (end - b + LP_THREADS - 1) / LP_THREADS, true);
+            eat(w, (b + (int)threadIdx.x) * N - mis, (end - b + LP_THREADS - 1) / LP_THREADS, true,
+                min(c1, end * N - mis));
         }
     }
     const float2 s = unpack2(s2), t = unpack2(a2);

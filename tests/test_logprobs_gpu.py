@@ -130,6 +130,29 @@ def test_rows_without_a_distribution(cuda, typ):
         assert logp.isnan().tolist() == [False, True, False, True, True, False, True, False]
 
 
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [900, 9000, 70000])
+def test_alternatives_of_rows_with_many_nan(cuda, typ, vocab):
+    """A NaN ranks as -inf, however many lie side by side; the order of the rest stays."""
+    x, t = rand(cuda, 4, vocab, typ, seed=vocab)
+    x[0, :vocab // 2] = float("nan")
+    x[1, ::2] = float("nan")
+    x[2, 40:] = float("nan")
+    x[3] = float("nan")
+    check(x, t, 20, cuda)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shift", [0, 1, 3, 5])
+@pytest.mark.parametrize("vocab,left", [(900, 0), (900, 3), (9000, 7), (70000, 2)])
+def test_alternatives_of_rows_with_few_tokens_left(cuda, vocab, left, shift, typ):
+    """Fewer tokens that can come than alternatives asked for, in rows of any alignment: the masked ones
+    follow in their order, each once."""
+    x, t = rand(cuda, 5, vocab, typ, seed=vocab + left, shift=shift, pad=3)
+    x[:, :vocab - left] = float("-inf")
+    check(x, t, 20, cuda)
+
+
 def test_targets(cuda):
     import torch
 
