@@ -19,8 +19,8 @@
 // is cut over many CTAs (rows x splits fill the SMs); the last one to arrive, by a ticket that it
 // resets, joins the parts.
 //
-// Measured: 1024 x 131072 bf16, 5 alternatives, 63 us (4.3 TB/s, 0.66 of a copy's rate); 61 x 50021
-// f16, 1 alternative, 8.6 us; 1 x 131072 f32, 20 alternatives, 8.5 us, of which 1 us is the load, 3 the
+// Measured: 1024 x 131072 bf16, 5 alternatives, 64 us (4.2 TB/s, 0.65 of a copy's rate; with 3 tokens left in each row 127); 61 x 50021
+// f16, 1 alternative, 8.7 us; 1 x 131072 f32, 20 alternatives, 8.7 us, of which 1 us is the load, 3 the
 // launch and the ticket, and the rest the lists: compare and exchange, one behind the other.
 #include <cuda_bf16.h>
 
@@ -306,9 +306,13 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
         }
         const float seen = value_of((Key) * (volatile uint32_t *)&bar_s << 32);
         tv = fmaxf(tv, seen);
-        unsigned left = __ballot_sync(0xffffffffu, mx >= tv);
-        if (!left) return;
-        while (left) {   // the lanes with a value that may count: the warp looks at one lane's values together
+        if (!__any_sync(0xffffffffu, mx >= tv)) return;
+        // the lanes with a value that may count: the warp looks at one lane's values together. The best that a lane may
+        // have is its largest at its first place: equal values behind a full list are passed over
+        const Key best = key_of(mx, max(i0, c0));
+        Key last = __shfl_sync(0xffffffffu, list, kth);
+        unsigned left = __ballot_sync(0xffffffffu, mx >= tv && best > last);
+        while (left) {
             const int src = __ffs(left) - 1;
             left &= left - 1;
             if (lane == src)
@@ -328,8 +332,9 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
                 offer(list, k, kth, lane);
             }
             __syncwarp();
+            last = __shfl_sync(0xffffffffu, list, kth);
+            left &= __ballot_sync(0xffffffffu, best > last);
         }
-        const Key last = __shfl_sync(0xffffffffu, list, kth);
         if (last) {
             tv = fmaxf(tv, value_of(last));
             if (lane == 0 && value_of(last) > seen) atomicMax(&bar_s, (uint32_t)(last >> 32));
