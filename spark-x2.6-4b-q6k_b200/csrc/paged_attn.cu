@@ -24,8 +24,8 @@
 // prompt chunks the softmax's instructions, 64 bf16 rows against each 128 keys. Measured, heads of 256, 4 a KV
 // head: one f32 row over 131072 keys 63 us (269 MB, 4.3 TB/s; a tile comes every 2850 clocks, what
 // the memory gives an SM, and 20 us are start, queries and joining); 64 bf16 rows of as many sequences of up to
-// 9000 keys 40 us (86 MB; a tile takes the MMA warp 2600 clocks, a change of group 14000); 2048 bf16 rows behind
-// 6144 cached ones 445 us (240 GFLOP, 0.54 PFLOP/s; of a tile's 3500 clocks the split of the weights
+// 9000 keys 41 us (86 MB; a tile takes the MMA warp 2600 clocks, a change of group 14000); 2048 bf16 rows behind
+// 6144 cached ones 450 us (240 GFLOP, 0.53 PFLOP/s; of a tile's 3500 clocks the split of the weights
 // into terms takes 1350, the scores' way out of the tensor memory and their scaling 900).
 //
 // Work split: all (sequence, KV head, row tile) groups stand in one line, each as long as the
