@@ -65,6 +65,11 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ unsigned long long pack2(float a, float b) {
     unsigned long long r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -250,8 +255,8 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
             a2 = pack2(st.a, 0.f);
         }
         if (st.m > V::LOW_M && st.m < HUGE_M) {
-            const float nm = -st.m * LOG2E;
-            const unsigned long long nm2 = pack2(nm, nm), l2 = pack2(LOG2E, LOG2E);
+            // x - m first: it is exact near the maximum, where a rounded m log2 e would shift every exponent
+            const unsigned long long nm2 = pack2(-st.m, -st.m), l2 = pack2(LOG2E, LOG2E);
 #pragma unroll
             for (int u = 0; u < UN; u++) {
                 if (u >= used) break;   // the same for the CTA
@@ -261,7 +266,7 @@ __global__ void __launch_bounds__(LP_THREADS, 768 / LP_THREADS) logprobs_kernel(
                     if constexpr (sizeof(T) == 4)
                         f = make_float2(__uint_as_float(V::floor_(w[u][e])), __uint_as_float(V::floor_(w[u][e + 1])));
                     else f = V::two(V::floor_(w[u][e >> 1]));
-                    const unsigned long long t = fma2(pack2(f.x, f.y), l2, nm2);
+                    const unsigned long long t = mul2(add2(pack2(f.x, f.y), nm2), l2);
                     const float2 tt = unpack2(t);
                     const unsigned long long p = pack2(ex2f_(tt.x), ex2f_(tt.y));
                     s2 = add2(s2, p);

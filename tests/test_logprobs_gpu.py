@@ -153,6 +153,28 @@ def test_alternatives_of_rows_with_few_tokens_left(cuda, vocab, left, shift, typ
     check(x, t, 20, cuda)
 
 
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("offset", [1e2, -1e3, 1e4, -1e4, 6e4, -6e4, 1e6, -1e9, 1e30, -1e30])
+def test_logits_far_from_zero(cuda, offset, typ):
+    """A constant added to a row changes nothing but the values' own rounding, and a row masked whole by any
+    finite value is the uniform distribution: the bounds above hold as they are, since x - m is exact near the
+    maximum."""
+    import torch
+
+    if not np.isfinite(float(torch.tensor(offset).to(ttype(typ)))):
+        pytest.skip("past the type's range")
+    for rows, vocab in ((1, 30000), (5, 4097), (900, 700)):
+        x, t = rand(cuda, rows, vocab, "f32", seed=rows)
+        x = (x.double() + offset).to(ttype(typ))
+        x[0] = offset
+        if rows > 1:
+            x[1] = offset
+            x[1, vocab // 2:] = 3.0         # masked by the offset (or the other way round)
+        x = x.contiguous()
+        assert x.isfinite().all()
+        check(x, t, 6, cuda)
+
+
 def test_targets(cuda):
     import torch
 
