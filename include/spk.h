@@ -484,7 +484,9 @@ int spk_paged_append(const spk_kv_pool *pool, const spk_kv_batch *batch, const v
 /* Causal grouped-query attention of the rows over their sequences' pages (append them first):
  *   out[t][h] = sigmoid(gate[t][h]) * softmax_j(scale * rope(q[t][h]) . K_j) V_j
  * over j in [0, pos_t] (window 0) or (pos_t - window, pos_t]; q head h reads KV head
- * h / (heads / kv_heads), any group. Sums and softmax in f32. A row that sees nothing gets 0.
+ * h / (heads / kv_heads), any group. The softmax and all sums are in f32; queries and weights meet the
+ * cached bytes as sums of e4m3 terms: queries to the bits of their type, weights to its bits near a row's
+ * largest one and to at least 2^-28 (bf16), 2^-31 (f16), 2^-37 (f32) of that. A row that sees nothing gets 0.
  * workspace: spk_paged_attn_workspace_bytes(head_dim) device bytes for the device current at the
  * call, zeroed once and left ready; calls that share one must not overlap on the GPU. No sync. */
 typedef struct {

@@ -13,20 +13,27 @@
 // e4m3 straight from the bulk copies; the query rows are the N columns of the B operand, and what
 // 8 bits lack is made up in columns: a number x is the sum of T e4m3 terms, x = t0 + t1 / 32 +
 // t2 / 1024 .., each term the rounding of what the ones before left (4 bits and a sign a term), and
-// each term has a column of its own, so that it keeps its own scale and nothing underflows:
-//   S^T[128 keys][term, row]  = K . q^T     scores: sum of a row's T columns
-//   O^T[hd][term, row]       += V^T . P^T   weights split the same way, one byte a column
-// Products of e4m3 pairs are exact and are added in f32, so T terms carry about 4.6 T bits: two
-// hold bf16 (8 bits), three f16 (11), five f32.
+// each term has a column of its own, so that it keeps its own scale:
+//   S^T[128 keys][term, row]  = K . q^T     scores: sum of a row's TQ columns
+//   O^T[hd][term, row]       += V^T . P^T   weights split the same way, TP bytes a row
+// Products of e4m3 pairs are exact and are added in f32. A number near the largest keeps about
+// 4.6 bits a term: two terms hold a bf16 query (8 bits), three an f16 one, five an f32 one.
+//
+// Weights need range, too: a row's keys may share what one key leaves them, 2^-17 of it each in a cache of 131072.
+// What the last term cannot hold is lost, and it is lost from O alone. Its smallest byte is 2^-9 under the terms'
+// steps (32 each, LAST before the last), and a row's largest weight stands at 2^6 to 2^8, so n keys
+// lose at most n times these shares of the row's sum:
+//   bf16 three terms 2^-10 / (32 x 128) / 2^6 = 2^-28;  f16 four 2^-32 (2^-31, the weights are taken by f16);  f32 five 2^-37
+// which at 131072 keys is a quarter of half a unit of bf16 and of f16. (Two terms, 2^-21, lose whole contexts:
+// behind a first token of value 0 with nine tenths of the weight, a third of 32768 others' sum was gone.)
 //
 // What bounds it: for few rows the cached bytes, read once per KV head (an MMA of 16 columns costs
 // what its A bytes cost to read from shared memory, and the softmax runs on keys x rows alone); for
-// prompt chunks the softmax's instructions, 64 bf16 rows against each 128 keys. Measured, heads of 256, 4 a KV
+// prompt chunks the softmax's instructions, 48 or 64 bf16 rows against each 128 keys. Measured, heads of 256, 4 a KV
 // head: one f32 row over 131072 keys 63 us (269 MB, 4.3 TB/s; a tile comes every 2850 clocks, what
 // the memory gives an SM, and 20 us are start, queries and joining); 64 bf16 rows of as many sequences of up to
 // 9000 keys 41 us (86 MB; a tile takes the MMA warp 2600 clocks, a change of group 14000); 2048 bf16 rows behind
-// 6144 cached ones 450 us (240 GFLOP, 0.53 PFLOP/s; of a tile's 3500 clocks the split of the weights
-// into terms takes 1350, the scores' way out of the tensor memory and their scaling 900).
+// 6144 cached ones 570 us (240 GFLOP, 0.42 PFLOP/s).
 //
 // Work split: all (sequence, KV head, row tile) groups stand in one line, each as long as the
 // tokens it reads plus COST for its fixed cost; the line is cut into equal ranges, one per CTA,
@@ -44,9 +51,10 @@ namespace paged {
 namespace {
 
 constexpr float M_NONE = -1e30f;      // reference of a part that has seen nothing
-// Weights are 2^(s' - m): a new reference sits W_TOP below the largest score, so weights start at 8, and
-// it moves only when a score passes m + 8, so they end at 256 (e4m3 holds 448).
-constexpr float W_TOP = 3.0f, W_MAX = 8.0f;
+// Weights are 2^(s' - m): a new reference sits W_TOP below the largest score, so weights start at 64, and
+// it moves only when a score passes m + 8, so they end at 256 (e4m3 holds 448). More room above would cost
+// the small ones (the terms' bytes end at 2^-9), less would move the reference more often.
+constexpr float W_TOP = 6.0f, W_MAX = 8.0f;
 constexpr float STEP = 32.0f;         // a term's scale over the one before: half an ulp of 256 is 8
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int TILE = 128, TB = TILE / BLOCK;   // keys of a tile, its blocks
@@ -68,30 +76,35 @@ struct AttnParams {
     int *err;
 };
 
-// N columns, T terms, R rows a tile (T R <= N). SG warpgroups share a tile's rows (wide tiles: more
+// R rows a tile, queries of TQ terms, weights of TP. SG warpgroups share a tile's rows (wide tiles: more
 // warps hide the softmax's latencies); PG sets of them take the groups in turn (narrow tiles: one
 // set's last products and outputs run beside the next one's first scores).
-template <int HD_, int N_, int T_, int R_, int SG_, int PG_>
+template <int HD_, int R_, int TQ_, int TP_, int SG_, int PG_>
 struct Cfg {
-    static constexpr int HD = HD_, N = N_, T = T_, R = R_, SG = SG_, PG = PG_;
+    static constexpr int HD = HD_, R = R_, TQ = TQ_, TP = TP_, SG = SG_, PG = PG_;
+    static constexpr int CS = (TQ * R + 15) / 16 * 16, CO = (TP * R + 15) / 16 * 16;   // columns of scores, of outputs
+    // a step of 64 loses nothing of the largest weights (what the terms before leave is at most 8, times the
+    // step), one of 128 a bit of those past 128, which bf16 does not have
+    static constexpr float LAST = TP == 3 ? 128.0f : 64.0f;
     static constexpr int RG = R / SG;                         // rows of a warpgroup, side by side
     static constexpr int CH = SG == 1 ? R : 8;                // rows handled together
     static constexpr int NC = RG / CH;
     static constexpr int LD = 8;                              // columns of a tensor-memory access
-    static constexpr int LC = SG == 1 ? (T * R + 7) / 8 * 8 : CH * T;   // columns of a chunk: all, or CH a term
+    // columns of a chunk: all, or CH a term
+    static constexpr int LCS = SG == 1 ? (TQ * R + 7) / 8 * 8 : CH * TQ, LCO = SG == 1 ? (TP * R + 7) / 8 * 8 : CH * TP;
     static constexpr int KB = BLOCK * HD;                     // bytes of a block's keys (or values)
     static constexpr int SLOT = TB * KB;                      // a tile's keys (or values)
     // slots of keys and of values: a tile's keys are done with its scores, its values much later
-    static constexpr int NK = N >= 96 ? (HD == 256 ? 2 : 4) : HD == 256 ? 3 : HD == 128 ? 6 : 8;
-    static constexpr int NV = N >= 96 ? (HD == 256 ? 1 : 2) : NK;
+    static constexpr int NK = SG > 1 ? (HD == 256 ? 2 : 4) : HD == 256 ? 3 : HD == 128 ? 6 : 8;
+    static constexpr int NV = SG > 1 ? (HD == 256 ? 1 : 2) : NK;
     static constexpr int SCR = NK <= 4 ? 8 : 16;              // tiles whose scales are kept: the copies are up to NK + 3 ahead
     // P: 16 keys of every column, then the next 16, 64 bytes further than they need so that the byte
     // stores of a warp's two runs of 16 keys meet different banks.
-    static constexpr int PK = N * 16 + 64, PB = TILE / 16 * PK, NP = 2;
+    static constexpr int PK = CO * 16 + 64, PB = TILE / 16 * PK, NP = 2;
     static constexpr int HH = HD == 256 ? 2 : 1;              // 128-dim halves of the output
-    static constexpr int TC = (2 + HH * PG) * N, TCOLS = TC <= 64 ? 64 : TC <= 128 ? 128 : TC <= 256 ? 256 : 512;
+    static constexpr int TC = 2 * CS + HH * PG * CO, TCOLS = TC <= 64 ? 64 : TC <= 128 ? 128 : TC <= 256 ? 256 : 512;
     static constexpr int MW = 160 * (SG == 1 ? 1 : 4);        // weights that a merge of parts holds at once
-    static constexpr size_t V_OFF = (size_t)NK * SLOT, Q_OFF = V_OFF + (size_t)NV * SLOT, P_OFF = Q_OFF + (size_t)2 * N * HD;
+    static constexpr size_t V_OFF = (size_t)NK * SLOT, Q_OFF = V_OFF + (size_t)NV * SLOT, P_OFF = Q_OFF + (size_t)2 * CS * HD;
     static constexpr size_t SMEM = P_OFF + (size_t)NP * PB;
     // a group's fixed cost in blocks: what evened out the CTAs' times over 64 sequences of 1 to 9000 tokens
     // (narrow: 8 40.4 us, 16 40.6, 32 42.0, 64 46.7) and 24 of 8 rows each (wide: 8 46 us, 16 37, 32 31, 64 33)
@@ -99,7 +112,7 @@ struct Cfg {
     static constexpr int LAG = PG == 1 ? 2 : 1;               // tiles that the values are behind the scores
     static constexpr int WARPS = FIRST_Q + Q_WARPS + 4 * SG * PG, THREADS = WARPS * 32;
     static constexpr int PART = (R * (HD + 2) + 3) / 4 * 4;   // floats of a partial: O, then m, then l; read 16 bytes at a time
-    static_assert(T * R <= N && TC <= 512 && R % SG == 0 && RG % CH == 0, "");
+    static_assert(TC <= 512 && R % SG == 0 && RG % CH == 0, "");
     // access x of chunk ch of warpgroup sg: its column
     static __device__ __forceinline__ int col(int sg, int ch, int x) { return SG == 1 ? 8 * x : x * R + sg * RG + ch * CH; }
     static constexpr int TS = SG == 1 ? R : CH;               // a chunk's terms lie this far apart
@@ -164,27 +177,32 @@ __device__ __forceinline__ float2 e4m3x2_f32(uint32_t w) {
     return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
 }
 
-// Two weights as T e4m3 terms, a pair of bytes each. Two terms go by f16 (11 bits, they hold 9).
-template <int T>
-__device__ __forceinline__ void split(float a, float b, uint32_t (&w)[T]) {
-    if constexpr (T == 2) {
-        const __half2 h = __floats2half2_rn(a, b);
-        uint16_t x, y;
-        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(x) : "r"(*reinterpret_cast<const uint32_t *>(&h)));
-        uint32_t f;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f) : "h"(x));
-        const __half2 r = __hmul2(__hsub2(h, *reinterpret_cast<const __half2 *>(&f)), __float2half2_rn(STEP));
-        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(y) : "r"(*reinterpret_cast<const uint32_t *>(&r)));
-        w[0] = x;
-        w[1] = y;
+// Two weights as TP e4m3 terms, a pair of bytes each. Up to four terms go by f16, whose 11 bits and 2^-24
+// they hold.
+template <typename C>
+__device__ __forceinline__ void split(float a, float b, uint32_t (&w)[C::TP]) {
+    constexpr int T = C::TP;
+    if constexpr (T <= 4) {
+        __half2 h = __floats2half2_rn(a, b);
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            uint16_t x;
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(x) : "r"(*reinterpret_cast<const uint32_t *>(&h)));
+            w[t] = x;
+            if (t + 1 < T) {
+                uint32_t f;
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f) : "h"(x));
+                h = __hmul2(__hsub2(h, *reinterpret_cast<const __half2 *>(&f)), __float2half2_rn(t + 2 < T ? STEP : C::LAST));
+            }
+        }
     } else {
 #pragma unroll
         for (int t = 0; t < T; t++) {
             w[t] = e4m3x2(a, b);
             if (t + 1 < T) {
                 const float2 v = e4m3x2_f32(w[t]);
-                a = (a - v.x) * STEP;
-                b = (b - v.y) * STEP;
+                a = (a - v.x) * (t + 2 < T ? STEP : C::LAST);
+                b = (b - v.y) * (t + 2 < T ? STEP : C::LAST);
             }
         }
     }
@@ -361,7 +379,7 @@ __device__ __noinline__ bool walk_next(const AttnParams &a, const uint32_t *pre,
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a) {
-    constexpr int HD = C::HD, N = C::N, TT = C::T, R = C::R, NK = C::NK, NV = C::NV, QB = 2, NP = C::NP, SCR = C::SCR;
+    constexpr int HD = C::HD, CS = C::CS, CO = C::CO, TQ = C::TQ, TP = C::TP, R = C::R, NK = C::NK, NV = C::NV, QB = 2, NP = C::NP, SCR = C::SCR;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ uint64_t full_k[NK], empty_k[NK], full_v[NV], empty_v[NV], sc_full[SCR], p_full[2], pv_done[2], q_full[QB], q_empty[QB];
     // a set waits on barriers that only its own tiles move, or on ones that its tile's scores imply: a wait by
@@ -573,8 +591,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
         // The whole warp walks and waits and one elected thread issues, so the walk's state and the descriptors
         // are the same in all its lanes (2048-row chunk 448 us; all of it in a branch of lane 0: 465).
         const bool one = elect_one();
-        const uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
-        const uint32_t so = __shfl_sync(0xffffffffu, tmem, 0), oo = so + 2 * N;
+        const uint32_t desc0 = (1u << 4) | ((128u >> 4) << 24);
+        const uint32_t sdesc = desc0 | ((uint32_t)(CS >> 3) << 17), odesc = desc0 | ((uint32_t)(CO >> 3) << 17);
+        const uint32_t so = __shfl_sync(0xffffffffu, tmem, 0), oo = so + 2 * CS;
         // descriptors move by their address field alone
         const uint64_t kdesc = smem_desc(smem_u32(smem), 128, 8 * HD);
         const uint64_t qdesc = smem_desc(smem_u32(qs), 128, 8 * HD);
@@ -612,8 +631,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     if (2 * kk < l.nb)
 #pragma unroll
                         for (int h = 0; h < C::HH; h++)
-                            mma_e4m3(oo + (l.po + h) * N, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * (2 * C::PK / 16),
-                                     idesc, !l.first || kk > 0);
+                            mma_e4m3(oo + (l.po + h) * CO, vd + (2 * kk * C::KB + h * 2048) / 16, pd + kk * (2 * C::PK / 16),
+                                     odesc, !l.first || kk > 0);
                 mma_commit(pv_done + (t & 1));
                 if (l.last) mma_commit(o_full + l.po / C::HH);
                 mma_commit(empty_v + st);
@@ -652,10 +671,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 __syncwarp();
                 tc_after();
                 if (one && ok) {
-                    const uint64_t kd = kdesc + st * (C::SLOT / 16), qd = qdesc + qb * (N * HD / 16);
+                    const uint64_t kd = kdesc + st * (C::SLOT / 16), qd = qdesc + qb * (CS * HD / 16);
 #pragma unroll
                     for (int kk = 0; kk < HD / 32; kk++)
-                        mma_e4m3(so + (i & 1) * N, kd + kk * 16, qd + kk * 16, idesc, kk > 0);
+                        mma_e4m3(so + (i & 1) * CS, kd + kk * 16, qd + kk * 16, sdesc, kk > 0);
 #pragma unroll
                     for (int x = 0; x < C::PG; x++)
                         if (x == (int)(n % C::PG)) mma_commit(&s_full[x][sets[x] & 1]);
@@ -745,7 +764,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             const bool sane = ex >= 8 && ex <= 246;
             const float dn = sane ? __uint_as_float((uint32_t)(260 - ex) << 23) : 1.0f;
             const float up = sane ? __uint_as_float((uint32_t)(ex - 6) << 23) : 1.0f;
-            uint8_t *dst = qs + (size_t)qb * N * HD;
+            uint8_t *dst = qs + (size_t)qb * CS * HD;
             if (qi >= QB) wait_for(q_empty + qb, ((qi / QB) - 1) & 1, &dead, a.err);
 #pragma unroll 1
             for (int r0 = 0; r0 < RW; r0 += RB) {
@@ -767,14 +786,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                         y[e] = fmaf(y[e], dn, y[e] - y[e]);
                     }
 #pragma unroll
-                    for (int t = 0; t < TT; t++) {
+                    for (int t = 0; t < TQ; t++) {
                         const int n = t * R + row;
                         uint8_t *col = dst + (n >> 3) * (8 * HD) + (n & 7) * 16;
                         const uint32_t x0 = e4m3x2(x[0], x[1]), x1 = e4m3x2(x[2], x[3]);
                         const uint32_t y0 = e4m3x2(y[0], y[1]), y1 = e4m3x2(y[2], y[3]);
                         *reinterpret_cast<uint32_t *>(col + (d0 >> 4) * 128 + (d0 & 15)) = x0 | (x1 << 16);
                         *reinterpret_cast<uint32_t *>(col + (d1 >> 4) * 128 + (d1 & 15)) = y0 | (y1 << 16);
-                        if (t + 1 < TT) {   // what is left, on the next term's scale
+                        if (t + 1 < TQ) {   // what is left, on the next term's scale
                             const float2 p0 = e4m3x2_f32(x0), p1 = e4m3x2_f32(x1), p2 = e4m3x2_f32(y0), p3 = e4m3x2_f32(y1);
                             x[0] = (x[0] - p0.x) * STEP, x[1] = (x[1] - p0.y) * STEP;
                             x[2] = (x[2] - p1.x) * STEP, x[3] = (x[3] - p1.y) * STEP;
@@ -797,7 +816,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
         const uint32_t lane_at = (uint32_t)(32 * q4) << 16;
         // byte of this key in a column of P: values lie in the order of paged.cuh
         const int kbyte = (key >> 4) * C::PK + place(key & 15);
-        constexpr int RG = C::RG, CH = C::CH, LC = C::LC, LD = C::LD, TS = C::TS;
+        constexpr int RG = C::RG, CH = C::CH, LCS = C::LCS, LCO = C::LCO, LD = C::LD, TS = C::TS;
         float *mr = mref[wg];
         uint32_t i = 0, qi = 0, mine_i = 0, own = 0;   // tiles and groups with tiles so far; those of this set
         for (uint32_t n = 0; group(n, g); n++) {
@@ -807,7 +826,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 qi += k1 > k0;
                 continue;
             }
-            const uint32_t otm = tmem + lane_at + (2 + pg * C::HH) * N;   // the group's sums
+            const uint32_t otm = tmem + lane_at + 2 * CS + pg * C::HH * CO;   // the group's sums
             const int p_lo = g.p_lo, p_hi = g.p_hi, see0 = g.see0, window = a.window;
             const int row = sg * RG + key, c = g.c0 + row;   // the row that this thread keeps the books of
             const bool mine = key < RG && c <= g.c1;
@@ -838,18 +857,18 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 float t[RG];         // s' - m
 #pragma unroll
                 for (int ch = 0; ch < C::NC; ch++) {
-                    float v[LC];
+                    float v[LCS];
 #pragma unroll
-                    for (int x = 0; x < LC / LD; x++)
-                        tm_ld<LD>(tmem + lane_at + (i & 1) * N + C::col(sg, ch, x), v + LD * x);
+                    for (int x = 0; x < LCS / LD; x++)
+                        tm_ld<LD>(tmem + lane_at + (i & 1) * CS + C::col(sg, ch, x), v + LD * x);
                     tm_wait(v);
                     if constexpr (RG % 2 == 0) {
                         const f32x2 fa2 = pack2(fa, fa), fb2 = pack2(fb, fb), step2 = pack2(1.0f / STEP, 1.0f / STEP);
 #pragma unroll
                         for (int r = 0; r < CH; r += 2) {
-                            f32x2 u = pack2(v[(TT - 1) * TS + r], v[(TT - 1) * TS + r + 1]);
+                            f32x2 u = pack2(v[(TQ - 1) * TS + r], v[(TQ - 1) * TS + r + 1]);
 #pragma unroll
-                            for (int x = TT - 2; x >= 0; x--) u = fma2(u, step2, pack2(v[x * TS + r], v[x * TS + r + 1]));
+                            for (int x = TQ - 2; x >= 0; x--) u = fma2(u, step2, pack2(v[x * TS + r], v[x * TS + r + 1]));
                             const float2 s = unpack2(fma2(u, fa2, fb2));
                             t[ch * CH + r] = s.x;
                             t[ch * CH + r + 1] = s.y;
@@ -857,9 +876,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     } else {
 #pragma unroll
                         for (int r = 0; r < CH; r++) {
-                            float u = v[(TT - 1) * TS + r];
+                            float u = v[(TQ - 1) * TS + r];
 #pragma unroll
-                            for (int x = TT - 2; x >= 0; x--) u = fmaf(u, 1.0f / STEP, v[x * TS + r]);
+                            for (int x = TQ - 2; x >= 0; x--) u = fmaf(u, 1.0f / STEP, v[x * TS + r]);
                             t[ch * CH + r] = fmaf(u, fa, fb);
                         }
                     }
@@ -934,20 +953,20 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                             if (!(over >> ch & 1u)) continue;
 #pragma unroll 1
                             for (int h = 0; h < C::HH; h++) {
-                                float v[LC];
+                                float v[LCO];
 #pragma unroll
-                                for (int x = 0; x < LC / LD; x++)
-                                    tm_ld<LD>(otm + h * N + C::col(sg, ch, x), v + LD * x);
+                                for (int x = 0; x < LCO / LD; x++)
+                                    tm_ld<LD>(otm + h * CO + C::col(sg, ch, x), v + LD * x);
                                 tm_wait(v);
 #pragma unroll
                                 for (int r = 0; r < TS; r++) {
                                     const float f = ex2(-fs[wg][ch * CH + r]);
 #pragma unroll
-                                    for (int x = r; x < LC; x += TS) v[x] *= f;
+                                    for (int x = r; x < LCO; x += TS) v[x] *= f;
                                 }
 #pragma unroll
-                                for (int x = 0; x < LC / LD; x++)
-                                    tm_st<LD>(otm + h * N + C::col(sg, ch, x), v + LD * x);
+                                for (int x = 0; x < LCO / LD; x++)
+                                    tm_st<LD>(otm + h * CO + C::col(sg, ch, x), v + LD * x);
                             }
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -972,10 +991,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                                 if (!edge || t[r + e] != -INFINITY) l[r + e] = fmaf(x[e], isv, l[r + e]);
                             }
                     }
-                    uint32_t b[TT];
-                    split<TT>(x[0], x[1], b);
+                    uint32_t b[TP];
+                    split<C>(x[0], x[1], b);
 #pragma unroll
-                    for (int tt = 0; tt < TT; tt++) {
+                    for (int tt = 0; tt < TP; tt++) {
                         const int n = tt * R + sg * RG + r;
                         pb[n * 16] = (uint8_t)b[tt];
                         if (r + 1 < RG) pb[(n + 1) * 16] = (uint8_t)(b[tt] >> 8);
@@ -1048,16 +1067,16 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
 #pragma unroll 1
             for (int x0 = 0; x0 < C::HH * C::NC; x0++) {
                 const int h = x0 / C::NC, ch = x0 - h * C::NC, d = 128 * h + key;
-                float v[LC];
+                float v[LCO];
 #pragma unroll
-                for (int x = 0; x < LC / LD; x++)
-                    tm_ld<LD>(otm + h * N + C::col(sg, ch, x), v + LD * x);
+                for (int x = 0; x < LCO / LD; x++)
+                    tm_ld<LD>(otm + h * CO + C::col(sg, ch, x), v + LD * x);
                 tm_wait(v);
 #pragma unroll
                 for (int r = 0; r < CH; r++) {
-                    float o = v[(TT - 1) * TS + r];
+                    float o = v[(TP - 1) * TS + r];
 #pragma unroll
-                    for (int x = TT - 2; x >= 0; x--) o = fmaf(o, 1.0f / STEP, v[x * TS + r]);
+                    for (int x = TP - 2; x >= 0; x--) o = fmaf(o, 1.0f / (x == TP - 2 ? C::LAST : STEP), v[x * TS + r]);
                     const int rr = ch * CH + r, ro = sg * RG + rr;
                     const float f = fs[wg][rr];
                     if (d >= HD || ro >= rows) continue;
@@ -1176,22 +1195,23 @@ int launch_one(const AttnParams &a, cudaStream_t s, const char *who) {
 // columns and a second tile reads the cache again, from L2; where the one outweighs the other was measured
 // (us; 64 sequences of up to 3000 keys, 8 of 6000, 1 of 16000; heads of 256):
 //   f32   8 rows: 6 a tile 41.3 21.8 26.1, 24 a tile 42.5 24.2 29.0;  16 rows: 51.0 23.6 30.7, 46.5 27.4 33.6
-//   f16   8 rows: 5 a tile 38.9 20.8 25.3, 10 a tile 32.7 23.7 29.3;  24 rows: 10 a tile 50.5 27.5 33.7, 32 a
+//   bf16  8 rows: 5 a tile 38.9 20.8 25.3, 10 a tile 32.7 23.7 29.3;  24 rows: 10 a tile 50.5 27.5 33.7, 32 a
 //         tile 43.8 29.0 40.6;  32 rows: 54.1 34.7 37.7, 42.7 31.6 45.5
-//   bf16 128 rows: 32 a tile of three terms 51.6 46.6 51.3, 64 of two 62.8 53.9 58.6;  256 rows: 66.9 53.3 71.4,
-//         67.7 52.3 70.6;  1024 rows, 8 and 1 sequences: 157.7 209.9, 137.9 149.5
+// bf16 queries of 193 rows and more are of two terms, which is what bf16 itself holds: the scores' columns that this
+// saves are the output's (heads of 256: 2 x 96 + 2 x 144 of 512, 48 rows a tile, and 40 at the most with three).
 template <typename T, int HD>
 int launch(const AttnParams &a, cudaStream_t s, const char *who) {
     const long long per = ((long long)a.b.rows * a.group + a.b.nseq - 1) / a.b.nseq;
     if constexpr (sizeof(T) == 4) {
-        if (per <= 12) return launch_one<T, Cfg<HD, 32, 5, 6, 1, 2>>(a, s, who);
-        return launch_one<T, Cfg<HD, 128, 5, 24, 3, 1>>(a, s, who);
+        if (per <= 12) return launch_one<T, Cfg<HD, 6, 5, 5, 1, 2>>(a, s, who);
+        return launch_one<T, Cfg<HD, 24, 5, 5, 3, 1>>(a, s, who);
     } else {
-        if (per <= 5) return launch_one<T, Cfg<HD, 16, 3, 5, 1, 2>>(a, s, who);
-        if (per <= 24) return launch_one<T, Cfg<HD, 32, 3, 10, 1, 2>>(a, s, who);
-        if constexpr (__is_same(T, __nv_bfloat16))
-            if (per > 192) return launch_one<T, Cfg<HD, 128, 2, 64, 4, 1>>(a, s, who);
-        return launch_one<T, Cfg<HD, 96, 3, 32, 4, 1>>(a, s, who);
+        constexpr bool B = __is_same(T, __nv_bfloat16);
+        if (per <= 5) return launch_one<T, Cfg<HD, 5, 3, B ? 3 : 4, 1, 2>>(a, s, who);
+        if (per <= 24) return launch_one<T, Cfg<HD, B ? 10 : 8, 3, B ? 3 : 4, 1, 2>>(a, s, who);
+        if constexpr (B)
+            if (per > 192) return launch_one<T, Cfg<HD, HD == 256 ? 48 : 64, 2, 3, HD == 256 ? 3 : 4, 1>>(a, s, who);
+        return launch_one<T, Cfg<HD, 32, 3, B ? 3 : 4, 4, 1>>(a, s, who);
     }
 }
 

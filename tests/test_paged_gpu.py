@@ -376,6 +376,58 @@ def test_attention_takes_queries_of_any_size(cuda, typ, size):
     check_attention(c, typ, q=q, tol=max(TOL[typ], 3e3 * 2.0 ** -19 if size > 1 else 0))
 
 
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 12, 40, 300])
+@pytest.mark.parametrize("n,mass", [(8000, 0.9), (32768, 0.9), (131072, 0.9), (131072, 0.99)])
+def test_attention_small_weights_count(cuda, n, mass, rows, typ):
+    """A first token with nearly all of the weight and a value of 0, as models park attention: the output is
+    what the other keys' weights, down to 2^-24 of the first one's, make of their values. 152 sequences over
+    the same pages, so that a CTA has the whole context of a group under one reference.
+
+    Bound. The values have a mean of half their spread, so the output is about (1 - mass) / 2 of the spread. All weights lie
+    above half of the last term's smallest byte (2^-28 of the first token's for bf16, 2^-31 f16, 2^-37 f32), so their
+    errors are roundings, as likely up as down, and add as sqrt(n): TOL, as elsewhere."""
+    import torch
+
+    from spk import paged
+
+    hd, page, nseq = 64, 128, 152
+    g = torch.Generator(device=cuda)
+    g.manual_seed(n + rows)
+    pages = -(-n // page)
+    cache = paged.PagedCache(pages, page, 1, hd, device=cuda)
+    k = torch.randn(pages, 1, page, hd, generator=g, device=cuda) * 50
+    v = torch.randn(pages, 1, page, hd, generator=g, device=cuda) * 80 + 40
+    k[..., 0] = 0
+    k[0, 0, :16], v[0, 0, 0] = 0, 0
+    k[0, 0, 0, 0] = 400
+    cache.k_pool.copy_(pack_k(k.clamp(-440, 440).to(torch.float16)).to(torch.float8_e4m3fn))
+    cache.v_pool.copy_(pack_v(v.clamp(-440, 440).to(torch.float16)).to(torch.float8_e4m3fn))
+    cache.k_scale.fill_(0.01)
+    cache.v_scale.fill_(0.01)
+    # the others' weights average e^(1/8): scores of spread 1/2
+    first = np.log(mass / (1 - mass) * n) + 0.125
+    cache.k_scale[0, 0, 0] = first * hd ** 0.5 / 4 / float(cache.k_pool[0, 0, 0, 0, 0, 0].float())
+    i32 = lambda x: torch.as_tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    row0, kv_len = i32(np.arange(nseq + 1) * rows), i32([n] * nseq)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda).repeat(nseq, 1)
+    q = torch.randn(nseq * rows, hd, generator=g, device=cuda).to(ttype(typ))
+    q[:, 0] = 4
+    b = paged.PagedBatch(cache, row0, kv_len, table, rows=nseq * rows, heads=1)
+    got = b.attention(q)
+    assert check_errors() == 0
+    kk = (unpack_k(cache.k_pool)[:, 0] * cache.k_scale[:, 0].double().repeat_interleave(16, -1)[..., None]).reshape(-1, hd)[:n]
+    vv = (unpack_v(cache.v_pool)[:, 0] * 0.01).reshape(-1, hd)[:n]
+    hide = torch.arange(n, device=cuda)[None] > torch.arange(n - rows, n, device=cuda)[:, None]
+    for s in (0, 77, nseq - 1):
+        at = slice(s * rows, (s + 1) * rows)
+        w = torch.softmax((q[at].double() @ kk.T / hd ** 0.5).masked_fill(hide, float("-inf")), -1)
+        assert abs(w[:, 0].mean().item() - mass) < 0.05
+        want = w @ vv
+        err = ((got[at].double() - want).norm() / want.norm()).item()
+        assert err < TOL[typ], err
+
+
 def test_attention_ignores_what_no_row_sees(cuda):
     """NaN bytes and scales in pages that are not the sequence's and behind its last block, NaN bytes behind
     its last token in that block, and a poisoned block that only other rows see."""
