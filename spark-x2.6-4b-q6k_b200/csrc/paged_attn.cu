@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     __shared__ Seg segs[SQ];                            // the CTA's groups, as warp 0 finds them; k0 < 0: no more
     __shared__ float4 scales[SCR][TB];                  // dk, log2 dv, 1 / dv of a tile's blocks
     __shared__ uint32_t pre[MAX_SEQ + 1], wsum[C::WARPS];
-    __shared__ float q_up[4];                           // score factor of a query tile: the softmax may be two behind
+    __shared__ __align__(16) float q_up[4][(R + 3) / 4 * 4];   // score factors of a tile's rows: the softmax may be two behind
     __shared__ int dead;                                // a wait ran out: what follows no longer waits
     constexpr int G = C::SG * C::PG;
     __shared__ float red[G][4][C::RG];                  // per row: the warps' maxima, then their sums
@@ -399,7 +399,6 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
     __shared__ int pos_s[C::PG][R];                     // per row: position, -1 past the tile's last row
     __shared__ size_t out_s[C::PG][R];                  // per row: where its output lies
     __shared__ float merge_s[C::PG][2 * C::MW];         // a row's weights of the parts, and their sums before
-    __shared__ float amax_s[C::WARPS - FIRST_Q];
     __shared__ int last_in[C::PG];
     __shared__ uint32_t tmem_s;
     __shared__ Walk walk_s;                             // the walk behind the CTA's first group
@@ -741,71 +740,59 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     else raw[r].none();
                 }
             };
-            // the tile's largest finite value: the rotation grows a pair by at most sqrt(2)
-            float mx = 0.f;
+            uint8_t *dst = qs + (size_t)qb * CS * HD;
 #pragma unroll 1
             for (int r0 = 0; r0 < RW; r0 += RB) {
                 load(r0);
-                if (r0 == 0) turn((c0 + w0) / a.group);   // while the rows are on their way
-#pragma unroll
-                for (int r = 0; r < RB; r++) {
-                    float x[8];
-                    raw[r].f32(x);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+                if (r0 == 0) {
+                    turn((c0 + w0) / a.group);   // while the rows are on their way
+                    if (qi >= QB) wait_for(q_empty + qb, ((qi / QB) - 1) & 1, &dead, a.err);
                 }
-            }
-            mx = warp_max(mx);
-            if (lane == 0) amax_s[qw] = mx;
-            bar_sync(5, helpers * 32);
-            for (int e = 0; e < helpers; e++) mx = fmaxf(mx, amax_s[e]);
-            // times 2^(6 - e), so that it lies in [64, 128); a tile of zeros stays
-            const int ex = (int)(__float_as_uint(mx) >> 23);
-            const bool sane = ex >= 8 && ex <= 246;
-            const float dn = sane ? __uint_as_float((uint32_t)(260 - ex) << 23) : 1.0f;
-            const float up = sane ? __uint_as_float((uint32_t)(ex - 6) << 23) : 1.0f;
-            uint8_t *dst = qs + (size_t)qb * CS * HD;
-            if (qi >= QB) wait_for(q_empty + qb, ((qi / QB) - 1) & 1, &dead, a.err);
-#pragma unroll 1
-            for (int r0 = 0; r0 < RW; r0 += RB) {
-                if (RW > RB) load(r0);
 #pragma unroll
                 for (int r = 0; r < RB; r++) {
                     const int row = w0 + r0 + r;
                     if (r0 + r >= RW || row >= R) continue;
-                    float v[8], x[4], y[4];
+                    float v[8], x[4], y[4], mx = 0.f;
                     raw[r].f32(v);
+                    // times 2^(6 - e), e the exponent of the row's largest finite value, which then lies in [64, 128) (a
+                    // row of nothing but values under 2^-120 lower); the rotation grows a pair by at most sqrt(2). A row's
+                    // own scale: no other row decides how exactly it is held.
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = v[e], y[e] = v[4 + e];
+                    for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
+                    mx = warp_max(mx);
+                    const uint32_t ex = min(max(__float_as_uint(mx) >> 23, 7u), 254u);
+                    const float dn = __uint_as_float((260u - ex) << 23);
+                    if (lane == 0) q_up[qi & 3][row] = __uint_as_float((ex - 6u) << 23) * a.scale;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {   // an infinity becomes a NaN, which e4m3 has
+                        x[e] = fmaf(v[e], dn, v[e] - v[e]);
+                        y[e] = fmaf(v[4 + e], dn, v[4 + e] - v[4 + e]);
+                    }
                     turn((c0 + row) / a.group);
                     if (lane < a.pdim / 8) rotate_unit(x, y, cs, sn);
-                    if (lane >= HD / 8) continue;
+                    if (lane < HD / 8) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[e] = fmaf(x[e], dn, x[e] - x[e]);   // an infinity becomes a NaN, which e4m3 has
-                        y[e] = fmaf(y[e], dn, y[e] - y[e]);
-                    }
-#pragma unroll
-                    for (int t = 0; t < TQ; t++) {
-                        const int n = t * R + row;
-                        uint8_t *col = dst + (n >> 3) * (8 * HD) + (n & 7) * 16;
-                        const uint32_t x0 = e4m3x2(x[0], x[1]), x1 = e4m3x2(x[2], x[3]);
-                        const uint32_t y0 = e4m3x2(y[0], y[1]), y1 = e4m3x2(y[2], y[3]);
-                        *reinterpret_cast<uint32_t *>(col + (d0 >> 4) * 128 + (d0 & 15)) = x0 | (x1 << 16);
-                        *reinterpret_cast<uint32_t *>(col + (d1 >> 4) * 128 + (d1 & 15)) = y0 | (y1 << 16);
-                        if (t + 1 < TQ) {   // what is left, on the next term's scale
-                            const float2 p0 = e4m3x2_f32(x0), p1 = e4m3x2_f32(x1), p2 = e4m3x2_f32(y0), p3 = e4m3x2_f32(y1);
-                            x[0] = (x[0] - p0.x) * STEP, x[1] = (x[1] - p0.y) * STEP;
-                            x[2] = (x[2] - p1.x) * STEP, x[3] = (x[3] - p1.y) * STEP;
-                            y[0] = (y[0] - p2.x) * STEP, y[1] = (y[1] - p2.y) * STEP;
-                            y[2] = (y[2] - p3.x) * STEP, y[3] = (y[3] - p3.y) * STEP;
+                        for (int t = 0; t < TQ; t++) {
+                            const int n = t * R + row;
+                            uint8_t *col = dst + (n >> 3) * (8 * HD) + (n & 7) * 16;
+                            const uint32_t x0 = e4m3x2(x[0], x[1]), x1 = e4m3x2(x[2], x[3]);
+                            const uint32_t y0 = e4m3x2(y[0], y[1]), y1 = e4m3x2(y[2], y[3]);
+                            *reinterpret_cast<uint32_t *>(col + (d0 >> 4) * 128 + (d0 & 15)) = x0 | (x1 << 16);
+                            *reinterpret_cast<uint32_t *>(col + (d1 >> 4) * 128 + (d1 & 15)) = y0 | (y1 << 16);
+                            if (t + 1 < TQ) {   // what is left, on the next term's scale
+                                const float2 p0 = e4m3x2_f32(x0), p1 = e4m3x2_f32(x1), p2 = e4m3x2_f32(y0), p3 = e4m3x2_f32(y1);
+                                x[0] = (x[0] - p0.x) * STEP, x[1] = (x[1] - p0.y) * STEP;
+                                x[2] = (x[2] - p1.x) * STEP, x[3] = (x[3] - p1.y) * STEP;
+                                y[0] = (y[0] - p2.x) * STEP, y[1] = (y[1] - p2.y) * STEP;
+                                y[2] = (y[2] - p3.x) * STEP, y[3] = (y[3] - p3.y) * STEP;
+                            }
                         }
                     }
                 }
             }
-            if (qw == 0 && lane == 0) q_up[qi & 3] = up * a.scale;
             fence_proxy_async();
-            bar_sync(5, helpers * 32);   // all rows are there, and amax_s is free again
+            __syncwarp();
+            if (helpers > Q_WARPS) bar_sync(5, helpers * 32);   // the helpers' rows are there, too
             if (keeps && lane == 0) mbar_arrive(q_full + qb);
             qi++;
         }
@@ -852,7 +839,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 const float4 sc = scales[i % SCR][key >> 4];
                 const float fb = sc.y, isv = sc.z;
                 const int j0 = start + k * TILE, j = j0 + key;
-                const float fa = sc.x * q_up[qi & 3];
+                const float *fq = q_up[qi & 3] + sg * RG;
                 const bool edge = j0 + TILE - 1 > p_lo || (window > 0 && j0 <= p_hi - window);
                 float t[RG];         // s' - m
 #pragma unroll
@@ -863,13 +850,14 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                         tm_ld<LD>(tmem + lane_at + (i & 1) * CS + C::col(sg, ch, x), v + LD * x);
                     tm_wait(v);
                     if constexpr (RG % 2 == 0) {
-                        const f32x2 fa2 = pack2(fa, fa), fb2 = pack2(fb, fb), step2 = pack2(1.0f / STEP, 1.0f / STEP);
+                        const f32x2 fa2 = pack2(sc.x, sc.x), fb2 = pack2(fb, fb), step2 = pack2(1.0f / STEP, 1.0f / STEP);
 #pragma unroll
                         for (int r = 0; r < CH; r += 2) {
                             f32x2 u = pack2(v[(TQ - 1) * TS + r], v[(TQ - 1) * TS + r + 1]);
 #pragma unroll
                             for (int x = TQ - 2; x >= 0; x--) u = fma2(u, step2, pack2(v[x * TS + r], v[x * TS + r + 1]));
-                            const float2 s = unpack2(fma2(u, fa2, fb2));
+                            const float2 f = *reinterpret_cast<const float2 *>(fq + ch * CH + r);
+                            const float2 s = unpack2(fma2(u, mul2(fa2, pack2(f.x, f.y)), fb2));
                             t[ch * CH + r] = s.x;
                             t[ch * CH + r + 1] = s.y;
                         }
@@ -879,7 +867,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                             float u = v[(TQ - 1) * TS + r];
 #pragma unroll
                             for (int x = TQ - 2; x >= 0; x--) u = fmaf(u, 1.0f / STEP, v[x * TS + r]);
-                            t[ch * CH + r] = fmaf(u, fa, fb);
+                            t[ch * CH + r] = fmaf(u, sc.x * fq[ch * CH + r], fb);
                         }
                     }
                 }

@@ -376,6 +376,39 @@ def test_attention_takes_queries_of_any_size(cuda, typ, size):
     check_attention(c, typ, q=q, tol=max(TOL[typ], 3e3 * 2.0 ** -19 if size > 1 else 0))
 
 
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("mean", [2, 9, 30, 290])
+@pytest.mark.parametrize("size", [3e4, 1e8, 2.0 ** 123])
+def test_attention_rows_of_mixed_size(cuda, size, mean, typ):
+    """A row is held as exactly beside rows of any other size as alone: TOL for the ordinary rows, each on its
+    own, whose bits do not change when the others (a later token, another head) are ordinary, too; a row so large
+    that one key has all of its weight gets that key's value."""
+    import torch
+
+    if typ == "f16" and size > 65504:
+        pytest.skip("past the type's range")
+    n = max(1, mean // 2)
+    c = Case(cuda, [n, n], [70, 300], kv=1, hd=128, heads=2, page=32, seed=mean)
+    q = c.randn(256, typ)
+    plain = c.batch.attention(q, freq=freqs(cuda, 64)).clone()
+    large = torch.zeros(2 * n, 2, dtype=torch.bool, device=cuda)
+    large[n - 1, 1] = large[2 * n - 1, 0] = large[n // 2, 0] = True
+    big = q.reshape(-1, 2, 128).clone()
+    big[large] = (big[large].double() * (size if typ != "f16" else 4000)).to(big.dtype)
+    assert big.isfinite().all()
+    got = c.batch.attention(big.reshape(q.shape), freq=freqs(cuda, 64))
+    assert check_errors() == 0
+    assert torch.equal(got.reshape(-1, 2, 128)[~large], plain.reshape(-1, 2, 128)[~large])
+    want = want_attention(c, q, freq=freqs(cuda, 64)).reshape(-1, 2, 128)[~large]
+    err = (got.reshape(-1, 2, 128)[~large].double() - want).norm(dim=-1) / want.norm(dim=-1)
+    assert (err < TOL[typ]).all(), err.max()
+    sure = want_attention(c, big.reshape(q.shape), freq=freqs(cuda, 64)).reshape(-1, 2, 128)[large]
+    gap = want_attention(c, big.reshape(q.shape), freq=freqs(cuda, 64), scale=128 ** -0.5 * 0.97).reshape(-1, 2, 128)[large]
+    one = (sure == gap).all(-1)      # one key has all of it, and would with scores 3 % nearer to each other
+    err = (got.reshape(-1, 2, 128)[large].double() - sure).norm(dim=-1) / sure.norm(dim=-1)
+    assert one.any() and (err[one] < TOL[typ]).all(), err
+
+
 @pytest.mark.parametrize("typ", ["f16", "bf16"])
 @pytest.mark.parametrize("rows", [1, 12, 40, 300])
 @pytest.mark.parametrize("n,mass", [(8000, 0.9), (32768, 0.9), (131072, 0.9), (131072, 0.99)])
