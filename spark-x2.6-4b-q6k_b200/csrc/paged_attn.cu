@@ -86,6 +86,9 @@ struct Cfg {
     // a step of 64 loses nothing of the largest weights (what the terms before leave is at most 8, times the
     // step), one of 128 a bit of those past 128, which bf16 does not have
     static constexpr float LAST = TP == 3 ? 128.0f : 64.0f;
+    // The tensor cores cut their f32 sums towards 0: n keys of values of one sign end up to n x 3.3e-10 short (131072:
+    // 4.3e-5 of the sum), which f32 outputs would show. Theirs leave the tensor memory every 64 tiles (2.7e-6).
+    static constexpr int RUN = TP >= 5 ? 64 : 0;
     static constexpr int RG = R / SG;                         // rows of a warpgroup, side by side
     static constexpr int CH = SG == 1 ? R : 8;                // rows handled together
     static constexpr int NC = RG / CH;
@@ -605,7 +608,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
         // narrow tile waits for memory, and its values leave their slot sooner. The oldest late tile is i - nlate.
         struct Late {
             int nb, po;           // its blocks, where its sums lie
-            bool first, last;     // of its group
+            bool first, last;     // of its sums; of its group
         };
         Late l0 = {0, 0, false, false}, l1 = l0;   // the oldest, the one behind it
         int nlate = 0;
@@ -687,7 +690,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                     const uint32_t t = i - nlate;
                     values(t, C::LAG == 2 ? there : weights());
                 }
-                const Late l = {min(TB, nblk - k * TB), (int)(n % C::PG) * C::HH, k == k0, k + 1 == k1};
+                const bool fresh = C::RUN ? (k - k0) % (C::RUN ? C::RUN : 1) == 0 : k == k0;
+                const Late l = {min(TB, nblk - k * TB), (int)(n % C::PG) * C::HH, fresh, k + 1 == k1};
                 if (nlate == 0) l0 = l;
                 else l1 = l;
                 nlate++;
@@ -828,6 +832,22 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
             float l[RG];
 #pragma unroll
             for (int r = 0; r < RG; r++) l[r] = 0.f;
+            float run[C::RUN ? C::HH * RG : 1];   // the outputs of the runs of tiles that are over
+            bool runs = false;
+            // chunk x of this thread's output dims: the terms' sums together
+            auto sums = [&](int x, float (&o)[CH]) {
+                const int h = x / C::NC, ch = x - h * C::NC;
+                float v[LCO];
+#pragma unroll
+                for (int y = 0; y < LCO / LD; y++) tm_ld<LD>(otm + h * CO + C::col(sg, ch, y), v + LD * y);
+                tm_wait(v);
+#pragma unroll
+                for (int r = 0; r < CH; r++) {
+                    o[r] = v[(TP - 1) * TS + r];
+#pragma unroll
+                    for (int y = TP - 2; y >= 0; y--) o[r] = fmaf(o[r], 1.0f / (y == TP - 2 ? C::LAST : STEP), v[y * TS + r]);
+                }
+            };
             bar_sync(bid, 128);
             for (int k = k0; k < k1; k++, i++) {
                 const int nb = min(TB, nblk - k * TB);
@@ -951,6 +971,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                                     const float f = ex2(-fs[wg][ch * CH + r]);
 #pragma unroll
                                     for (int x = r; x < LCO; x += TS) v[x] *= f;
+                                    if (C::RUN && runs && r < CH) run[h * RG + ch * CH + r] *= f;
                                 }
 #pragma unroll
                                 for (int x = 0; x < LCO / LD; x++)
@@ -960,6 +981,20 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
                 }
+                if constexpr (C::RUN > 0)
+                    if (k > k0 && (k - k0) % C::RUN == 0) {   // the next products start new sums
+                        wait_for(pv_done + ((i - 1) & 1), ((i - 1) >> 1) & 1, &dead, a.err);
+                        __syncwarp();
+                        tc_after();
+#pragma unroll 1
+                        for (int x = 0; x < C::HH * C::NC; x++) {
+                            float o[CH];
+                            sums(x, o);
+#pragma unroll
+                            for (int r = 0; r < CH; r++) run[x * CH + r] = (runs ? run[x * CH + r] : 0.f) + o[r];
+                        }
+                        runs = true;
+                    }
                 if (i >= NP) wait_for(pv_done + ((i - NP) & 1), ((i - NP) >> 1) & 1, &dead, a.err);   // P's buffer is free
                 uint8_t *pb = ps + (size_t)(i % NP) * C::PB + kbyte;
 #pragma unroll
@@ -1055,16 +1090,12 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
 #pragma unroll 1
             for (int x0 = 0; x0 < C::HH * C::NC; x0++) {
                 const int h = x0 / C::NC, ch = x0 - h * C::NC, d = 128 * h + key;
-                float v[LCO];
-#pragma unroll
-                for (int x = 0; x < LCO / LD; x++)
-                    tm_ld<LD>(otm + h * CO + C::col(sg, ch, x), v + LD * x);
-                tm_wait(v);
+                float os[CH];
+                sums(x0, os);
 #pragma unroll
                 for (int r = 0; r < CH; r++) {
-                    float o = v[(TP - 1) * TS + r];
-#pragma unroll
-                    for (int x = TP - 2; x >= 0; x--) o = fmaf(o, 1.0f / (x == TP - 2 ? C::LAST : STEP), v[x * TS + r]);
+                    float o = os[r];
+                    if (C::RUN && runs) o += run[x0 * CH + r];
                     const int rr = ch * CH + r, ro = sg * RG + rr;
                     const float f = fs[wg][rr];
                     if (d >= HD || ro >= rows) continue;

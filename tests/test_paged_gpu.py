@@ -409,7 +409,7 @@ def test_attention_rows_of_mixed_size(cuda, size, mean, typ):
     assert one.any() and (err[one] < TOL[typ]).all(), err
 
 
-@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows", [1, 12, 40, 300])
 @pytest.mark.parametrize("n,mass", [(8000, 0.9), (32768, 0.9), (131072, 0.9), (131072, 0.99)])
 def test_attention_small_weights_count(cuda, n, mass, rows, typ):
