@@ -290,7 +290,7 @@ __device__ __noinline__ float2 turn_of(int pos, float freq) {
 // Lengths are in blocks and fit 32 bits (the entry point refuses a batch that could not).
 struct Seq {
     int r0, n, len, tiles;            // rows of the call, cached tokens, row tiles
-    int c, slope;                     // group j is at most (c + slope (j + 1)) / 16 blocks long
+    int c, rate;                      // group j takes up to (c + rate (j + 1) / 2^15) / 16 blocks: R / group tokens more each
 };
 __device__ __forceinline__ Seq seq_of(const AttnParams &a, int s, int R) {
     Seq q;
@@ -303,19 +303,20 @@ __device__ __forceinline__ Seq seq_of(const AttnParams &a, int s, int R) {
         q.n = 0;
     }
     q.tiles = (int)(((long long)q.n * a.group + R - 1) / R);
-    const int step = (R + a.group - 1) / a.group, pos0 = max(0, q.len - q.n);
-    if (a.window > 0 && a.window < q.len) {
-        q.c = min(q.len, a.window + step + BLOCK);
-        q.slope = 0;
+    const bool windowed = a.window > 0 && a.window < q.len;
+    if (windowed || q.len < q.n) {    // every group alike: a window and a tile's rows, or the whole sequence
+        q.c = windowed ? min(q.len, a.window + (R + a.group - 1) / a.group + BLOCK) : max(0, q.len);
+        q.rate = 0;
     } else {
-        q.c = pos0;
-        q.slope = step;
+        q.c = q.len - q.n + 2;
+        q.rate = (R * 32768 + a.group - 1) / a.group;
     }
     return q;
 }
-// Length of group j and of groups 0 .. j - 1: the tokens' sum, a partial block each, the fixed costs.
+// Length of groups 0 .. j - 1: the tokens' sum (group i sees at most len - n + (i + 1) R / group + 1 of them), a
+// partial block each, the fixed costs. 64 bits hold it: the entry point's bound is 2^35 on j^2 R / group.
 __device__ __forceinline__ uint32_t before(const Seq &q, uint32_t j, int cost) {
-    const unsigned long long t = (unsigned long long)j * q.c + (unsigned long long)q.slope * j * (j + 1) / 2;
+    const unsigned long long t = (unsigned long long)j * q.c + ((unsigned long long)q.rate * j * (j + 1) >> 16);
     return (uint32_t)(t / BLOCK) + j * (cost + 2);
 }
 
@@ -1192,9 +1193,9 @@ constexpr int MAX_R = 64;
 
 template <typename T, typename C>
 int launch_one(const AttnParams &a, cudaStream_t s, const char *who) {
-    // the line of work, at its longest: every row tile as long as the page table
+    // the line of work, at its longest: every row tile as long as the page table and a tile's tokens (before())
     const long long tiles = (long long)a.b.rows * a.group / C::R + a.b.nseq;
-    const long long blocks = (long long)a.b.max_pages * a.pool.page_tokens / BLOCK + C::COST + 3;
+    const long long blocks = ((long long)a.b.max_pages * a.pool.page_tokens + C::R / a.group + 3 + (tiles >> 15)) / BLOCK + C::COST + 4;
     if ((double)tiles * blocks * a.pool.kv_heads > 2147483000.0)
         return set_error("%s: %d rows over up to %d pages of %d tokens are too much for one call", who, a.b.rows,
                          a.b.max_pages, a.pool.page_tokens);

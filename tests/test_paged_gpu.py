@@ -549,6 +549,26 @@ def test_attention_many_sequences(cuda, typ):
     check_attention(c, typ, window=0)
 
 
+def test_attention_line_of_work_of_many_heads_a_kv_head(cuda):
+    """Thousands of heads on one KV head: 375467 row tiles of 24 columns, 24 / 4096 tokens each. Their lengths add up to
+    less than 32 bits only if a tile is not taken to be a token longer than the one before it."""
+    import torch
+
+    heads, n, hd = 4096, 2200, 64
+    c = Case(cuda, [n], [0], kv=1, hd=hd, heads=heads, page=64, seed=14)
+    q = c.randn(heads * hd, "f32")
+    out = torch.full_like(q, float("nan"))
+    c.batch.attention(q, out)
+    assert check_errors() == 0 and out.isfinite().all()
+    pg = c.table[0]
+    k, v = ((u[pg, 0] * s[pg, 0].double().repeat_interleave(16, -1)[..., None]).reshape(-1, hd)[:n]
+            for u, s in ((unpack_k(c.cache.k_pool), c.cache.k_scale), (unpack_v(c.cache.v_pool), c.cache.v_scale)))
+    for i in (0, 1, 700, 1500, n - 1):
+        want = torch.softmax(q[i].reshape(heads, hd).double() @ k[:i + 1].T / 8, -1) @ v[:i + 1]
+        got = out[i].reshape(heads, hd).double()
+        assert ((got - want).norm() / want.norm()).item() < TOL["f32"], i
+
+
 def test_attention_rows_that_see_nothing_are_zero_and_bad_batches_reported(cuda):
     import spk
 

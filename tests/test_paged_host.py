@@ -79,6 +79,16 @@ def test_attention_refuses_a_batch_past_its_line_of_work():
 
 
 @needs_lib
+def test_attention_refuses_many_heads_past_the_line_of_work():
+    """480000 row tiles of less than a token over a table of 80000 tokens: 2.4e9 blocks."""
+    p = pool(pages=2000, page_tokens=64, kv_heads=1, head_dim=64)
+    b = batch(nseq=1, rows=90000, max_pages=1250)
+    a = paged._Attn(q=P, ldq=128 * 64, type=0, heads=128, out=P, ldout=128 * 64, workspace=P)
+    assert spk.lib().spk_paged_attn(C.addressof(p), C.addressof(b), C.addressof(a), None) == -1
+    assert "too much" in spk.last_error()
+
+
+@needs_lib
 def test_no_rows_is_a_call_that_does_nothing():
     p, b = pool(), batch(rows=0)
     a = paged._Attn(type=0, heads=4)
