@@ -511,7 +511,8 @@ int spk_paged_attn(const spk_kv_pool *pool, const spk_kv_batch *batch, const spk
  * NULL) of the distribution in nats, and the `top` (0 to 32) most likely tokens with their log
  * probabilities, ties to the lower index, [rows][top]. -inf is a token that cannot come. A row
  * with a NaN or +inf, or nothing but -inf, gives NaN. workspace: spk_logprobs_workspace_bytes
- * device bytes, zeroed once and left ready; calls that share one must not overlap. One launch. */
+ * device bytes (at most 250 KB), zeroed once and left ready, for calls of up to that many rows; calls that share
+ * one must not overlap. One launch. */
 size_t spk_logprobs_workspace_bytes(int rows, int vocab);
 int spk_logprobs(const void *logits, int type, int rows, int vocab, long long ld, const int *target, float *logp,
                  float *entropy, int top, int *top_ids, float *top_logp, void *workspace, void *stream);

@@ -45,7 +45,7 @@ struct LpArgs {
     float *logp, *entropy;
     int *ids;
     float *best;
-    unsigned int *tickets;                 // [rows], zero at rest
+    unsigned int *tickets;                 // [rows that are split], zero at rest
     float *part;                           // [rows][splits][LP_PART]
     int *err;
 };
@@ -502,7 +502,10 @@ cudaError_t launch(LpArgs &a, cudaStream_t s) {
                           : launch_pdl(logprobs_kernel<T, 128>, grid, dim3(128), 0, s, a);
 }
 
-size_t ticket_bytes(int rows) { return ((size_t)rows * 4 + 255) / 256 * 256; }
+// Rows that are split, and their parts: no more than the CTAs side by side (plan()). The tickets lie at the same
+// place for every number of rows, so that a workspace may serve calls of fewer rows, too.
+int most_parts() { return 6 * sm_count(); }
+size_t ticket_bytes() { return ((size_t)most_parts() * 4 + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace spk
@@ -512,7 +515,8 @@ extern "C" {
 size_t spk_logprobs_workspace_bytes(int rows, int vocab) {
     using namespace spk;
     if (rows < 1 || vocab < 1) return 0;
-    return ticket_bytes(rows) + (size_t)rows * LP_SPLITS * LP_PART * sizeof(float);
+    const long long parts = (long long)rows * LP_SPLITS;
+    return ticket_bytes() + (size_t)(parts < most_parts() ? parts : most_parts()) * LP_PART * sizeof(float);
 }
 int spk_logprobs(const void *logits, int type, int rows, int vocab, long long ld, const int *target, float *logp,
                  float *entropy, int top, int *top_ids, float *top_logp, void *workspace, void *stream) {
@@ -540,7 +544,7 @@ int spk_logprobs(const void *logits, int type, int rows, int vocab, long long ld
     a.ids = top_ids;
     a.best = top_logp;
     a.tickets = (unsigned int *)workspace;
-    a.part = (float *)((uint8_t *)workspace + ticket_bytes(rows));
+    a.part = (float *)((uint8_t *)workspace + ticket_bytes());
     a.err = device_error_ptr();
     const cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = type == 0 ? launch<float>(a, s) : type == 1 ? launch<__half>(a, s) : launch<__nv_bfloat16>(a, s);

@@ -192,6 +192,28 @@ def test_targets(cuda):
     assert spk.lib().spk_check_device_error() == -1 and spk.lib().spk_check_device_error() == 0
 
 
+def test_a_workspace_serves_calls_of_fewer_rows(cuda):
+    """One workspace of 128 rows, for 20, 128, 1 and 128 of them, each cut over several CTAs."""
+    import torch
+
+    import spk
+
+    x, t = rand(cuda, 128, 60000, "f32", seed=8)
+    x = x.contiguous()
+    L = spk.lib()
+    ws = torch.zeros(L.spk_logprobs_workspace_bytes(128, 60000), dtype=torch.uint8, device=cuda)
+    want = torch.log_softmax(x.double(), -1)
+    for rows in (20, 128, 1, 128):
+        logp = torch.full((rows,), 7.0, device=cuda)
+        ids, best = torch.full((rows, 2), -1, dtype=torch.int32, device=cuda), torch.zeros(rows, 2, device=cuda)
+        spk.check(L.spk_logprobs(x.data_ptr(), 0, rows, 60000, 60000, t.data_ptr(), logp.data_ptr(), None, 2, ids.data_ptr(),
+                                 best.data_ptr(), ws.data_ptr(), None))
+        torch.cuda.synchronize()
+        w = want[:rows].gather(1, t[:rows].long()[:, None])[:, 0]
+        assert ((logp.double() - w).abs() <= 2e-6 + 1e-6 * w.abs()).all(), rows
+        assert torch.equal(ids.long(), want[:rows].topk(2)[1]), rows
+
+
 def test_optional_outputs_and_streams(cuda):
     import torch
 

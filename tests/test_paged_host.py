@@ -117,6 +117,14 @@ def test_workspace_sizes():
     assert L.spk_logprobs_workspace_bytes(3, 100) < L.spk_logprobs_workspace_bytes(300, 100)
 
 
+@needs_lib
+def test_logprobs_workspace_is_no_larger_than_its_parts():
+    """Rows past the CTAs that run side by side are not split: a workspace does not grow with them."""
+    size = spk.lib().spk_logprobs_workspace_bytes
+    assert all(size(n, 131072) <= size(n + 1, 131072) for n in range(1, 2000))
+    assert size(65535, 131072) == size(1000, 10) < 300000
+
+
 def test_value_order_is_a_permutation_with_its_inverse():
     assert sorted(paged.ORDER) == list(range(paged.BLOCK))
     place = [4 * ((i & 7) >> 1) + (i & 1) + 2 * (i >> 3) for i in range(paged.BLOCK)]
