@@ -140,13 +140,21 @@ class PageTable:
 
     def reserve(self, seq, tokens: int) -> list:
         """The pages of sequence `seq` for `tokens` tokens, more of them when it needs more."""
-        have = self.held.setdefault(seq, [])
-        need = -(-tokens // self.page_tokens) - len(have)
+        need = -(-tokens // self.page_tokens) - len(self.held.get(seq, ()))
         if need > len(self.free):
             raise SpkError(f"sequence {seq} needs {need} more pages, {len(self.free)} are free")
+        have = self.held.setdefault(seq, [])
         for _ in range(need):
             have.append(self.free.pop())
         return have
+
+    def trim(self, seq, pages: int) -> None:
+        """Gives back the pages of `seq` past the first `pages`, the last one first."""
+        have = self.held.get(seq, [])
+        while len(have) > pages:
+            self.free.append(have.pop())
+        if not have:
+            self.held.pop(seq, None)
 
     def release(self, seq) -> None:
         self.free += self.held.pop(seq, [])[::-1]

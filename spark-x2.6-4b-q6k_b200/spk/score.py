@@ -15,13 +15,14 @@ from . import SpkError, check, lib
 from .paged import _rows, stream_of, type_of
 
 MAX_TOP = 32
+MAX_ROWS = 65535    # of a call
 
 
 class LogProbs:
     def __init__(self, rows: int, vocab: int, top: int = 0, device="cuda"):
         import torch
 
-        if not 0 <= rows <= 65535 or vocab < 1 or not 0 <= top <= min(MAX_TOP, vocab):
+        if not 0 <= rows <= MAX_ROWS or vocab < 1 or not 0 <= top <= min(MAX_TOP, vocab):
             raise SpkError(f"{rows} rows of {vocab} with {top} alternatives (0 to {MAX_TOP})")
         self.rows, self.vocab, self.top = rows, vocab, top
         self.logp = torch.empty(rows, device=device)

@@ -7,21 +7,22 @@ new tokens of any of them, in one call: every layer appends the rows' keys and v
 pages with the rotation on the way (spk_paged_append), attends over the pages (spk_paged_attn, the gate
 in its epilogue), and the head's logits end in each token's log probability, the entropy and the most
 likely alternatives (spk_logprobs). A sequence may be continued by later calls, and dropped with
-``release``.
+``release``. A call that raises leaves the sequences as they were, as long and on the same pages.
 
     python -m spk.serve [--layers N] [--sequences N] [--tokens N]    # synthetic weights
 """
 from __future__ import annotations
 
 import ctypes as C
+from contextlib import contextmanager
 from dataclasses import dataclass
 
 import numpy as np
 
 from . import SpkError, check, dev_bytes, lib
 from .model import MATS, ModelConfig, mat_shapes, upload_container
-from .paged import PagedBatch, PagedCache, PageTable, rope_freq
-from .score import LogProbs
+from .paged import MAX_SEQ, PagedBatch, PagedCache, PageTable, rope_freq
+from .score import MAX_ROWS, MAX_TOP, LogProbs
 
 GEMM_ROWS = 128     # rows of one spk_vq_lut_gemm call
 HEAD_ROWS = 8       # rows of one spk_q80_tile_head call
@@ -108,19 +109,53 @@ class PagedScorer:
         self.table.release(seq)
         self.len.pop(seq, None)
 
+    def _check(self, new: dict, rows_most=None, top: int = 0) -> list:
+        """The sequences of a call that have tokens; raises where the call cannot be done. Changes nothing."""
+        cfg, seqs = self.cfg, [s for s in new if len(new[s])]
+        if not 0 <= top <= min(MAX_TOP, cfg.vocab):
+            raise SpkError(f"{top} alternatives (0 to {min(MAX_TOP, cfg.vocab)})")
+        if len(seqs) > MAX_SEQ:
+            raise SpkError(f"{len(seqs)} sequences in a call (up to {MAX_SEQ})")
+        rows = sum(len(new[s]) for s in seqs)
+        if rows_most is not None and rows > rows_most:
+            raise SpkError(f"{rows} tokens in a call (up to {rows_most})")
+        for s in seqs:
+            if not all(0 <= t < cfg.vocab for t in new[s]):
+                raise SpkError(f"sequence {s}: a token id outside the vocabulary of {cfg.vocab}")
+        return seqs
+
+    @contextmanager
+    def _kept(self, seqs):
+        """The sequences' lengths and pages as they were, if what follows raises. Rows that it appended are written
+        over by the next call; a block that holds earlier tokens, too, may keep a larger scale from them."""
+        was = {s: (self.len.get(s), len(self.table.held.get(s, ()))) for s in seqs}
+        try:
+            yield
+        except BaseException:
+            for s in reversed(seqs):
+                n, pages = was[s]
+                self.table.trim(s, pages)
+                if n is None:
+                    self.len.pop(s, None)
+                else:
+                    self.len[s] = n
+            raise
+
     def forward(self, new: dict):
         """Rows of new tokens {sequence: [ids]} through the decoder: logits [rows][vocab] (f32), the
         sequences in the order given. Their keys and values stay in the cache."""
+        seqs = self._check(new)
+        with self._kept(seqs):
+            return self._forward(new, seqs)
+
+    def _forward(self, new: dict, seqs: list):
         import torch
 
         cfg, dev = self.cfg, self.device
-        seqs = [s for s in new if len(new[s])]
         rows = sum(len(new[s]) for s in seqs)
         if not rows:
             return torch.empty(0, cfg.vocab, device=dev)
         for s in seqs:
-            if not all(0 <= t < cfg.vocab for t in new[s]):
-                raise SpkError(f"sequence {s}: a token id outside the vocabulary of {cfg.vocab}")
             self.table.reserve(s, self.len.get(s, 0) + len(new[s]))
         for s in seqs:
             self.len[s] = self.len.get(s, 0) + len(new[s])
@@ -134,7 +169,7 @@ class PagedScorer:
         check(L.spk_q80_dequant(picked.data_ptr(), rows * cfg.hidden // 32, h.data_ptr(), st))
         new_ = lambda width: torch.empty(rows, width, device=dev)  # noqa: E731
         qkv, gate, att = new_(cfg.q_dim + 2 * cfg.kv_dim), new_(cfg.heads), new_(cfg.q_dim)
-        ga, up = new_(cfg.inter), new_(cfg.inter)
+        ga, up, logits = new_(cfg.inter), new_(cfg.inter), new_(cfg.vocab)
         batch = PagedBatch(self.caches[0], row0, kv_len, table, rows=rows, heads=cfg.heads)
         for (m, in_norm, post_norm), cache, full in zip(self.layers, self.caches, cfg.full):
             batch.use(cache)
@@ -147,7 +182,6 @@ class PagedScorer:
             m["gate"](h, ga, post_norm, cfg.eps)
             m["up"](h, up, post_norm, cfg.eps)
             m["down"](torch.nn.functional.gelu(ga).mul_(up), h, accumulate=True)     # erf form, model.rs:253-258
-        logits = torch.empty(rows, cfg.vocab, device=dev)
         for r in range(0, rows, HEAD_ROWS):
             n = min(HEAD_ROWS, rows - r)
             check(L.spk_q80_tile_head(self.head.data_ptr(), cfg.vocab, cfg.hidden, n, h[r].data_ptr(), h.stride(0),
@@ -159,12 +193,13 @@ class PagedScorer:
         """Scores new tokens {sequence: [ids]}: {sequence: Scored}. Synchronizes."""
         import torch
 
-        logits = self.forward(new)
-        seqs = [s for s in new if len(new[s])]
+        seqs = self._check(new, MAX_ROWS, top)
         target = torch.tensor([t for s in seqs for t in list(new[s][1:]) + [-1]], dtype=torch.int32, device=self.device)
         lp = LogProbs(len(target), self.cfg.vocab, top, device=self.device)
-        logp, ent, ids, best = [t.tolist() for t in lp(logits, target)] if len(target) else ([], [], [], [])
-        check(lib().spk_check_device_error(), "feed")
+        with self._kept(seqs):
+            logits = self._forward(new, seqs)
+            logp, ent, ids, best = [t.tolist() for t in lp(logits, target)] if len(target) else ([], [], [], [])
+            check(lib().spk_check_device_error(), "feed")
         out, r = {s: Scored([], [], []) for s in new}, 0
         for s in seqs:
             n = len(new[s])

@@ -146,6 +146,21 @@ def test_page_table_hands_out_and_takes_back():
     assert t.reserve("c", 49) == [0, 1, 3, 4]
 
 
+def test_page_table_after_a_refusal_and_a_trim():
+    t = paged.PageTable(4, 16)
+    t.reserve("a", 20)
+    was = list(t.free), {s: list(p) for s, p in t.held.items()}
+    with pytest.raises(spk.SpkError):
+        t.reserve("b", 33)
+    assert (t.free, t.held) == was       # not even an empty entry
+    t.reserve("a", 50)
+    t.trim("a", 2)
+    t.trim("nobody", 0)
+    assert t.held["a"] == [0, 1] and t.reserve("c", 16)
+    t.trim("c", 0)
+    assert "c" not in t.held
+
+
 @pytest.mark.parametrize("kw", [dict(head_dim=80), dict(page_tokens=24), dict(pages=0), dict(kv_heads=0)])
 def test_cache_refuses(kw):
     d = dict(pages=4, page_tokens=32, kv_heads=2, head_dim=64, device="cpu")

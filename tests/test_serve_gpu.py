@@ -88,6 +88,51 @@ def test_what_it_refuses(model):
     assert sc.feed({}) == {}
 
 
+def test_a_call_that_fails_leaves_the_sequences_as_they_were(model):
+    """Refused before anything is appended, or failed under way (no memory, a wait that ran out): the same tokens fed
+    afterwards are scored as by a scorer that never saw the failure. Scores are compared as they are: a block's scale
+    is that of its rows, and the tokens that come again are the same."""
+    from unittest import mock
+
+    import spk
+    from spk import serve
+
+    cfg, _, sc = model
+    rng = np.random.default_rng(4)
+    a, b = rng.integers(0, cfg.vocab, 50).tolist(), rng.integers(0, cfg.vocab, 20).tolist()
+    parts = [{"a": a[:20]}, {"a": a[20:], "b": b}]
+    fresh = [sc.feed(p, top=3) for p in parts]
+    for s in "ab":
+        sc.release(s)
+
+    def state():
+        return dict(sc.len), {s: list(p) for s, p in sc.table.held.items()}, list(sc.table.free)
+
+    def refuses(new, **kw):
+        was = state()
+        with pytest.raises((spk.SpkError, MemoryError)):
+            sc.feed(new, **kw)
+        assert state() == was
+
+    got = []
+    for p in parts:
+        refuses(p, top=33)
+        refuses(p, top=-1)
+        refuses({**p, "x": [cfg.vocab]})
+        refuses({**p, "x": [1] * 640})                           # pages for some of them
+        refuses({**p, **{i: [1] for i in range(1024)}})          # more sequences than a call takes
+        refuses({**p, "x": [1] * 65536})                         # more rows than log probabilities are of
+        for what in ("PagedBatch.attention", "LogProbs.__call__"):
+            with mock.patch.object(getattr(serve, what.split(".")[0]), what.split(".")[1], side_effect=MemoryError):
+                refuses(p, top=3)
+        with mock.patch.object(serve, "lib", lambda: mock.Mock(wraps=spk.lib(), spk_check_device_error=lambda: -1)):
+            refuses(p, top=3)
+        got.append(sc.feed(p, top=3))
+    assert got == fresh
+    for s in "ab":
+        sc.release(s)
+
+
 def test_it_runs_as_a_command(cuda, capsys):
     import sys
     from unittest import mock
