@@ -326,7 +326,7 @@ extern "C" int spk_paged_append(const spk_kv_pool *pool, const spk_kv_batch *bat
     if (check_pool(pool, who) || check_batch(batch, who)) return -1;
     if (type < T_F32 || type > T_BF16) return set_error("%s: type %d (0 f32, 1 f16, 2 bf16)", who, type);
     const long long width = (long long)pool->kv_heads * pool->head_dim;
-    if (pdim < 0 || pdim % 8 || pdim > pool->head_dim || (pdim > 0 && !freq))
+    if (pdim < 0 || pdim % 8 || pdim > pool->head_dim || (pdim > 0 && !freq) || (uintptr_t)freq % 4)
         return set_error("%s: pdim %d (a multiple of 8 up to head_dim, with its frequencies)", who, pdim);
     if (batch->rows == 0) return 0;
     if (!k || !v) return set_error("%s: null rows", who);

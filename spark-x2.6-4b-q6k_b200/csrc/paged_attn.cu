@@ -1262,7 +1262,7 @@ int spk_paged_attn(const spk_kv_pool *pool, const spk_kv_batch *batch, const spk
     if (p->type < T_F32 || p->type > T_BF16) return set_error("%s: type %d (0 f32, 1 f16, 2 bf16)", who, p->type);
     if (p->heads < 1 || p->heads % pool->kv_heads)
         return set_error("%s: %d heads over %d KV heads", who, p->heads, pool->kv_heads);
-    if (p->pdim < 0 || p->pdim % 8 || p->pdim > pool->head_dim || (p->pdim > 0 && !p->freq))
+    if (p->pdim < 0 || p->pdim % 8 || p->pdim > pool->head_dim || (p->pdim > 0 && !p->freq) || (uintptr_t)p->freq % 4)
         return set_error("%s: pdim %d (a multiple of 8 up to head_dim, with its frequencies)", who, p->pdim);
     if (p->window < 0) return set_error("%s: window %d", who, p->window);
     if (batch->rows == 0) return 0;

@@ -97,6 +97,19 @@ def _rows(t, rows: int, width: int, what: str, like=None):
     return ld
 
 
+def _angles(freq, t):
+    """(address, rotated dims) of the frequencies for the rows t: the kernels read f32 values side by side."""
+    if freq is None:
+        return None, 0
+    import torch
+
+    if freq.dtype != torch.float32 or not freq.is_contiguous():
+        raise SpkError(f"freq is f32, its values side by side; got {freq.dtype} with strides {freq.stride()}")
+    if freq.get_device() != t.get_device():
+        raise SpkError(f"freq lies on {freq.device}, the rows on {t.device}")
+    return ptr(freq), 2 * freq.numel()
+
+
 class PagedCache:
     """One layer's keys and values of every sequence. Needs no initial contents."""
 
@@ -208,8 +221,9 @@ class PagedBatch:
         keys are rotated over their first 2 * len(freq) dims when freq is given."""
         width = self.cache.kv_heads * self.cache.head_dim
         ldk, ldv = _rows(k, self.rows, width, "k"), _rows(v, self.rows, width, "v", k)
-        check(self._append(self._pool_p, self._batch_p, k.data_ptr(), ldk, v.data_ptr(), ldv, type_of(k), ptr(freq),
-                           0 if freq is None else 2 * freq.numel(), stream_of(k, stream)))
+        f, pdim = _angles(freq, k)
+        check(self._append(self._pool_p, self._batch_p, k.data_ptr(), ldk, v.data_ptr(), ldv, type_of(k), f, pdim,
+                           stream_of(k, stream)))
 
     def attention(self, q, out=None, window: int = 0, freq=None, gate=None, scale: float = 0.0, stream=None):
         """out [rows][heads * head_dim] (made when not given): attention of the rows, which have been
@@ -227,6 +241,6 @@ class PagedBatch:
         if gate is not None:
             a.ldgate = _rows(gate, self.rows, self.heads, "gate", q)
             a.gate = gate.data_ptr()
-        a.freq, a.pdim = (None, 0) if freq is None else (ptr(freq), 2 * freq.numel())
+        a.freq, a.pdim = _angles(freq, q)
         check(self._attn(self._pool_p, self._batch_p, self._attn_p, stream_of(q, stream)))
         return out

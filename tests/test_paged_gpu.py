@@ -592,6 +592,28 @@ def test_attention_rows_that_see_nothing_are_zero_and_bad_batches_reported(cuda)
         assert check_errors() == 0
 
 
+def test_frequencies_are_f32_side_by_side_on_the_rows_device(cuda):
+    """Anything else would be read past its end or as other numbers."""
+    import torch
+
+    import spk
+
+    c = Case(cuda, [2, 1], [5, 30], kv=2, hd=64, heads=4, page=16, seed=3)
+    q, k, v, good = c.randn(256, "f32"), c.randn(128, "f32"), c.randn(128, "f32"), freqs(cuda, 32)
+    before = c.cache.k_pool.view(torch.uint8).clone()
+    wide = torch.zeros(16, 2, device=cuda)
+    wide[:, 0] = good
+    for bad in (good.double(), good.half(), good.bfloat16(), good.int(), wide[:, 0], good.flip(0)[::2], good.cpu(), freqs(cuda, 64)[:31],
+                freqs(cuda, 128)):
+        for call in (lambda: c.batch.append(k, v, freq=bad), lambda: c.batch.attention(q, freq=bad)):
+            with pytest.raises(spk.SpkError):
+                call()
+    torch.cuda.synchronize()
+    assert torch.equal(before, c.cache.k_pool.view(torch.uint8))
+    check_append(c, k, v, wide[:, 0].contiguous())
+    check_attention(c, "f32", q=q, freq=good)
+
+
 def test_append_then_attention_is_attention_over_the_rounded_rows(cuda):
     """The two together, over pages as they come, against attention in 64 bits over what the cache holds."""
     c = Case(cuda, [60, 1, 9], [10, 200, 0], kv=4, hd=256, heads=16, page=32, seed=11)

@@ -69,6 +69,14 @@ def test_attention_refuses(kw):
 
 
 @needs_lib
+def test_unaligned_frequencies_are_refused():
+    p, b = pool(), batch()
+    a = paged._Attn(q=P, ldq=512, type=0, heads=4, out=P, ldout=512, workspace=P, freq=P + 2, pdim=64)
+    assert spk.lib().spk_paged_append(C.addressof(p), C.addressof(b), P, 256, P, 256, 0, P + 1, 64, None) == -1
+    assert spk.lib().spk_paged_attn(C.addressof(p), C.addressof(b), C.addressof(a), None) == -1
+
+
+@needs_lib
 def test_attention_refuses_a_batch_past_its_line_of_work():
     """Row tiles times blocks of the longest table has to fit 32 bits."""
     p = pool(pages=1 << 20, page_tokens=1024, kv_heads=64)
