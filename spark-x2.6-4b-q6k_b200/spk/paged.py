@@ -83,8 +83,9 @@ def rope_freq(theta: float, pdim: int, device="cuda"):
     return torch.from_numpy((np.float32(1) / np.power(np.float32(theta), i / np.float32(pdim))).astype(np.float32)).to(device)
 
 
-def _rows(t, rows: int, width: int, what: str, like=None):
-    """A row matrix [rows][width] whose last axis is dense: its row stride in elements."""
+def _rows(t, rows: int, width: int, what: str, like=None, on=None):
+    """A row matrix [rows][width] whose last axis is dense: its row stride in elements. `like`: rows of the same type
+    and device; `on`: the device that it has to lie on."""
     if t.shape != (rows, width):
         raise SpkError(f"{what} is [{rows}, {width}]; got {list(t.shape)}")
     ld, one = t.stride()
@@ -94,6 +95,8 @@ def _rows(t, rows: int, width: int, what: str, like=None):
         raise SpkError("libspk takes device buffers; got a host tensor")
     if like is not None and (t.dtype != like.dtype or t.get_device() != like.get_device()):
         raise SpkError(f"{what} is {t.dtype} on {t.device}, the other rows {like.dtype} on {like.device}")
+    if on is not None and t.device != on:
+        raise SpkError(f"{what} lies on {t.device}, the pool on {on}")
     return ld
 
 
@@ -220,7 +223,7 @@ class PagedBatch:
         """Rows k, v [rows][kv_heads * head_dim] (views of a wider matrix are fine) into the pages;
         keys are rotated over their first 2 * len(freq) dims when freq is given."""
         width = self.cache.kv_heads * self.cache.head_dim
-        ldk, ldv = _rows(k, self.rows, width, "k"), _rows(v, self.rows, width, "v", k)
+        ldk, ldv = _rows(k, self.rows, width, "k", on=self.cache.device), _rows(v, self.rows, width, "v", k)
         f, pdim = _angles(freq, k)
         check(self._append(self._pool_p, self._batch_p, k.data_ptr(), ldk, v.data_ptr(), ldv, type_of(k), f, pdim,
                            stream_of(k, stream)))
@@ -231,11 +234,12 @@ class PagedBatch:
         through a sigmoid, `window` 0 sees every earlier token, `scale` 0 is 1 / sqrt(head_dim)."""
         width = self.heads * self.cache.head_dim
         a = self._a
+        a.ldq = _rows(q, self.rows, width, "q", on=self.cache.device)
         if out is None:
             import torch
 
             out = torch.empty(self.rows, width, dtype=q.dtype, device=q.device)
-        a.ldq, a.ldout = _rows(q, self.rows, width, "q"), _rows(out, self.rows, width, "out", q)
+        a.ldout = _rows(out, self.rows, width, "out", q)
         a.q, a.out, a.type, a.window, a.scale = q.data_ptr(), out.data_ptr(), type_of(q), window, scale
         a.gate = None
         if gate is not None:

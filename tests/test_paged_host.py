@@ -193,3 +193,25 @@ def test_python_checks_of_rows():
         paged.type_of(torch.zeros(1, dtype=torch.float64))
     with pytest.raises(spk.SpkError):
         score.LogProbs(3, 10, top=11, device="cpu")
+
+
+def test_rows_of_another_device_than_the_pool_are_refused():
+    """The pool's, the batch's and the rows' addresses go to one device, whichever tensor is looked at first."""
+    from unittest import mock
+
+    import torch
+
+    def rows(device):
+        t = mock.Mock(shape=(3, 128), dtype=torch.float32, is_cuda=True, device=torch.device(device))
+        t.stride.return_value, t.get_device.return_value = (128, 1), t.device.index
+        return t
+
+    pool = torch.device("cuda:0")
+    assert paged._rows(rows("cuda:0"), 3, 128, "k", on=pool) == 128
+    with pytest.raises(spk.SpkError):
+        paged._rows(rows("cuda:1"), 3, 128, "k", on=pool)
+    b = mock.Mock(spec=paged.PagedBatch, cache=mock.Mock(kv_heads=2, head_dim=64, device=pool), rows=3, heads=2, _a=paged._Attn())
+    with pytest.raises(spk.SpkError, match="pool"):
+        paged.PagedBatch.append(b, rows("cuda:1"), rows("cuda:1"))
+    with pytest.raises(spk.SpkError, match="pool"):
+        paged.PagedBatch.attention(b, rows("cuda:1"), rows("cuda:1"))
