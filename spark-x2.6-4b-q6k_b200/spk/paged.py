@@ -11,7 +11,10 @@ their contents move. ``PageTable`` hands out pages.
     batch.append(k, v, freq=freq)                  # rows into the pages, keys rotated on the way
     batch.attention(q, out, freq=freq, gate=g)     # causal attention over them
 
-Calls go to torch's current stream unless a stream is given, and do not synchronize.
+Calls go to torch's current stream unless a stream is given, and do not synchronize. What an object
+here makes for itself may be used on any stream. Tensors that are handed in are ordered with a given
+stream by the caller, as between any two streams; they may be dropped after the call. Output that a
+call makes belongs to the call's stream.
 """
 from __future__ import annotations
 
@@ -74,6 +77,49 @@ def stream_of(t, stream) -> int:
     return stream.cuda_stream if stream is not None else _cuda[1](i)
 
 
+class Owned:
+    """Buffers that an object makes for itself, on the stream then current. A first call on another stream
+    waits for what that one had before it, since the buffers' memory may be in use there until then or their
+    zeroing on its way, and keeps them from being handed out again before the call is done with them. (A call that is
+    being captured does neither: a capture begins when the device is idle, and the graph's owner keeps what it reads.)"""
+
+    def __init__(self, *tensors):
+        import torch
+
+        self.tensors, self.seen, self.made = tensors, set(), None
+        dev = tensors[0].device
+        if dev.type == "cuda":
+            with torch.cuda.device(dev):
+                self.seen.add(torch.cuda.current_stream().cuda_stream)
+                if not torch.cuda.is_current_stream_capturing():
+                    self.made = torch.cuda.Event()
+                    self.made.record()
+
+    def use(self, raw: int, stream) -> None:
+        """Before a launch on the stream `raw`, `stream` as it was given to the call."""
+        if raw in self.seen:
+            return
+        import torch
+
+        s = stream if stream is not None else torch.cuda.current_stream(self.tensors[0].device)
+        with torch.cuda.stream(s):
+            if torch.cuda.is_current_stream_capturing():
+                return
+        if self.made is not None:
+            s.wait_event(self.made)
+        for t in self.tensors:
+            t.record_stream(s)
+        self.seen.add(raw)
+
+
+def lent(stream, *tensors) -> None:
+    """Tensors handed in to a call on a stream of its own: not handed out again before it is done with them."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
 def rope_freq(theta: float, pdim: int, device="cuda"):
     """1 / theta^(2i / pdim), the rotation's frequencies (model.rs:416-429), f32 on the device."""
     import numpy as np
@@ -130,6 +176,7 @@ class PagedCache:
         self.k_scale = torch.empty(pages, kv_heads, page_tokens // BLOCK, device=device)
         self.v_scale = torch.empty_like(self.k_scale)
         self.device = self.k_pool.device
+        self.owned = Owned(self.k_pool, self.v_pool, self.k_scale, self.v_scale)
         self._c = _Pool(self.k_pool.data_ptr(), self.v_pool.data_ptr(), self.k_scale.data_ptr(),
                         self.v_scale.data_ptr(), pages, page_tokens, kv_heads, head_dim)
 
@@ -207,6 +254,7 @@ class PagedBatch:
         with torch.cuda.device(cache.device):
             self.workspace = torch.zeros(L.spk_paged_attn_workspace_bytes(cache.head_dim), dtype=torch.uint8,
                                          device=cache.device)
+        self.owned = Owned(self.workspace)
         self._a = _Attn(heads=heads, workspace=self.workspace.data_ptr())
         self._pool_p, self._batch_p, self._attn_p = C.addressof(cache._c), C.addressof(self._b), C.addressof(self._a)
         self._append, self._attn = L.spk_paged_append, L.spk_paged_attn
@@ -225,8 +273,10 @@ class PagedBatch:
         width = self.cache.kv_heads * self.cache.head_dim
         ldk, ldv = _rows(k, self.rows, width, "k", on=self.cache.device), _rows(v, self.rows, width, "v", k)
         f, pdim = _angles(freq, k)
-        check(self._append(self._pool_p, self._batch_p, k.data_ptr(), ldk, v.data_ptr(), ldv, type_of(k), f, pdim,
-                           stream_of(k, stream)))
+        typ, raw = type_of(k), stream_of(k, stream)
+        self.cache.owned.use(raw, stream)
+        check(self._append(self._pool_p, self._batch_p, k.data_ptr(), ldk, v.data_ptr(), ldv, typ, f, pdim, raw))
+        lent(stream, k, v, freq, *self._keep)
 
     def attention(self, q, out=None, window: int = 0, freq=None, gate=None, scale: float = 0.0, stream=None):
         """out [rows][heads * head_dim] (made when not given): attention of the rows, which have been
@@ -238,7 +288,8 @@ class PagedBatch:
         if out is None:
             import torch
 
-            out = torch.empty(self.rows, width, dtype=q.dtype, device=q.device)
+            with torch.cuda.stream(stream):      # None: the current one
+                out = torch.empty(self.rows, width, dtype=q.dtype, device=q.device)
         a.ldout = _rows(out, self.rows, width, "out", q)
         a.q, a.out, a.type, a.window, a.scale = q.data_ptr(), out.data_ptr(), type_of(q), window, scale
         a.gate = None
@@ -246,5 +297,9 @@ class PagedBatch:
             a.ldgate = _rows(gate, self.rows, self.heads, "gate", q)
             a.gate = gate.data_ptr()
         a.freq, a.pdim = _angles(freq, q)
-        check(self._attn(self._pool_p, self._batch_p, self._attn_p, stream_of(q, stream)))
+        raw = stream_of(q, stream)
+        self.cache.owned.use(raw, stream)
+        self.owned.use(raw, stream)
+        check(self._attn(self._pool_p, self._batch_p, self._attn_p, raw))
+        lent(stream, q, out, gate, freq, *self._keep)
         return out

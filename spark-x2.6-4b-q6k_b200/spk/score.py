@@ -7,12 +7,12 @@
 
 logp[i] = log softmax(logits[i])[target[i]], entropy[i] in nats, ids / best [rows][top] the most
 likely tokens and their log probabilities, ties to the lower id. The buffers are the object's own
-and are written again by its next call.
+and are written again by its next call; calls may be on any stream, one after the other.
 """
 from __future__ import annotations
 
 from . import SpkError, check, lib
-from .paged import _rows, stream_of, type_of
+from .paged import Owned, _rows, lent, stream_of, type_of
 
 MAX_TOP = 32
 MAX_ROWS = 65535    # of a call
@@ -31,6 +31,7 @@ class LogProbs:
         self.best = torch.empty(rows, top, device=device)
         L = lib()
         self.workspace = torch.zeros(L.spk_logprobs_workspace_bytes(rows, vocab), dtype=torch.uint8, device=device)
+        self.owned = Owned(self.logp, self.entropy, self.ids, self.best, self.workspace)
         self._fn = L.spk_logprobs
         self._out = (self.logp.data_ptr(), self.entropy.data_ptr(), top, self.ids.data_ptr(), self.best.data_ptr(),
                      self.workspace.data_ptr())
@@ -45,6 +46,8 @@ class LogProbs:
             raise SpkError(f"target is int32 [{self.rows}]; got {target.dtype} {list(target.shape)}")
         if target.device != logits.device or self.logp.device != logits.device:
             raise SpkError("logits, target and the object's buffers lie on different devices")
-        check(self._fn(logits.data_ptr(), type_of(logits), self.rows, self.vocab, ld, target.data_ptr(), *self._out,
-                       stream_of(logits, stream)))
+        typ, raw = type_of(logits), stream_of(logits, stream)
+        self.owned.use(raw, stream)
+        check(self._fn(logits.data_ptr(), typ, self.rows, self.vocab, ld, target.data_ptr(), *self._out, raw))
+        lent(stream, logits, target)
         return self.logp, self.entropy, self.ids, self.best

@@ -230,3 +230,37 @@ def test_optional_outputs_and_streams(cuda):
     s.synchronize()
     w = torch.log_softmax(x.double(), -1)
     assert np.allclose(ent.cpu(), -(w.exp() * w).sum(-1).cpu(), atol=1e-5)
+
+
+def test_a_given_stream_is_ordered_with_the_objects_own_buffers(cuda):
+    """A first call on another stream than the object's, which is still busy with its zeroing; logits dropped after
+    the call; then a call that is captured."""
+    import torch
+
+    from spk import score
+
+    x, t = rand(cuda, 3, 60000, "f32", seed=2)
+    x = x.contiguous()
+    want = torch.log_softmax(x.double(), -1).gather(1, t.long()[:, None])[:, 0]
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    junk = torch.full((score.LogProbs(3, 60000, 2, device=cuda).workspace.numel(),), 255, dtype=torch.uint8, device=cuda)
+    del junk
+    torch.cuda._sleep(100_000_000)
+    lp = score.LogProbs(3, 60000, 2, device=cuda)
+    mine = x.clone()
+    s.wait_stream(torch.cuda.current_stream())      # the logits are the caller's to order
+    logp = lp(mine, t, stream=s)[0]
+    del mine
+    junk = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    assert ((logp.double() - want).abs() < 2e-5).all()
+    lp = score.LogProbs(3, 60000, 2, device=cuda)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        lp(x, t)
+    lp.logp.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert ((lp.logp.double() - want).abs() < 2e-5).all() and junk.sum() == 0

@@ -663,6 +663,60 @@ def test_on_a_stream_and_in_a_graph(cuda):
     assert check_errors() == 0
 
 
+def test_a_given_stream_is_ordered_with_the_objects_own_buffers(cuda):
+    """Calls on a stream of their own while the current one is busy: the output does not take memory that the
+    current stream still reads, the workspace's zeroing and the pool's earlier owner are waited for, and what is
+    dropped after the call is not handed out again before the call has read it."""
+    import torch
+
+    from spk import paged
+
+    kv, hd, n = 2, 128, 3000
+    g = torch.Generator(device=cuda)
+    g.manual_seed(6)
+    q, k, v = (torch.randn(n, w * hd, generator=g, device=cuda) for w in (8, 2, 2))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    row0, kv_len, table = i32([0, n]), i32([n]), torch.arange(47, dtype=torch.int32, device=cuda)[None].contiguous()
+    cache = paged.PagedCache(47, 64, kv, hd, device=cuda)
+    batch = paged.PagedBatch(cache, row0, kv_len, table, rows=n, heads=8)
+    batch.append(k, v)
+    want = batch.attention(q).clone()
+    pools = [t.view(torch.uint8).clone() for t in (cache.k_pool, cache.v_pool)]
+    busy = lambda: torch.cuda._sleep(100_000_000)   # noqa: E731  (some 50 ms)
+    s = torch.cuda.Stream()
+    for _ in range(3):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        # memory that the current stream reads late and that is free for its next owner
+        old = [torch.full((n, 8 * hd), 7.0, device=cuda), torch.full_like(pools[0], 9), torch.full_like(pools[1], 9),
+               torch.full_like(batch.workspace, 255)]
+        busy()
+        kept = [t.clone() for t in old]
+        del old
+        c2 = paged.PagedCache(47, 64, kv, hd, device=cuda)
+        b2 = paged.PagedBatch(c2, row0, kv_len, table, rows=n, heads=8)
+        b2.append(k, v, stream=s)
+        out = b2.attention(q, stream=s)
+        torch.cuda.synchronize()
+        assert all((t == x).all() for t, x in zip(kept, (7.0, 9, 9, 255)))
+        assert torch.equal(out, want)
+        assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(pools, (c2.k_pool, c2.v_pool)))
+    # dropped after the call, which comes late
+    args = [t.clone() for t in (q, k, v, row0, kv_len, table)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        busy()
+    b3 = paged.PagedBatch(cache, *args[3:], rows=n, heads=8)
+    b3.append(args[1], args[2], stream=s)
+    out = b3.attention(args[0], stream=s)
+    shapes = [(t.shape, t.dtype) for t in args] + [(b3.workspace.shape, torch.uint8)]
+    del args, b3
+    junk = [torch.full(sh, 99, dtype=dt, device=cuda) for sh, dt in shapes for _ in range(2)]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and check_errors() == 0
+    del junk
+
+
 def test_offsets_past_32_bits(cuda):
     """Pages whose bytes lie past 4 GiB of the pool."""
     import torch
