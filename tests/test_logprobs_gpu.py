@@ -175,6 +175,18 @@ def test_logits_far_from_zero(cuda, offset, typ):
         check(x, t, 6, cuda)
 
 
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+def test_rows_past_2_to_the_31(cuda, typ):
+    """Rows whose elements lie past 2^31 of their matrix, and past 2^32 of its bytes."""
+    import torch
+
+    ld, rows, vocab = 2 ** 30 + 17, 3, 9001
+    x = torch.empty(2 * ld + vocab, dtype=ttype(typ), device=cuda).as_strided((rows, vocab), (ld, 1))
+    y, t = rand(cuda, rows, vocab, typ, seed=9)
+    x.copy_(y)
+    check(x, t, 5, cuda)
+
+
 def test_targets(cuda):
     import torch
 

@@ -212,6 +212,21 @@ def test_append_token_by_token_keeps_every_row(cuda):
             assert ((seq[i] - x[i].double()).abs() <= lim * 1.01).all()
 
 
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+def test_append_every_step_of_a_block_follows_the_definition(cuda, typ):
+    """40 single tokens of growing size: after each one the block's new and earlier rows are one rounding of what the
+    definition makes of the bytes before it."""
+    import torch
+
+    c = Case(cuda, [1], [39], kv=2, hd=64, page=16, seed=21)
+    for i in range(40):
+        c.len = [i + 1]
+        c.kv_len.fill_(i + 1)
+        size = 0.1 * 1.15 ** i if i % 5 else 0.01
+        check_append(c, c.randn(128, typ, scale=size), c.randn(128, typ, scale=size), freqs(cuda, 32))
+    assert (c.cache.k_scale[c.table[0][:3]] > 0).all() and torch.isfinite(c.cache.values()[0][c.table[0][:3]]).all()
+
+
 def test_append_many_sequences_and_long_runs(cuda):
     """More blocks than a CTA takes at once, several head groups, 700 sequences of one row."""
     c = Case(cuda, [6000], [5], kv=6, hd=128, page=64, seed=2)
@@ -509,6 +524,33 @@ def test_attention_poisoned_block_reaches_only_the_rows_that_see_it(cuda, typ):
         c.cache.v_scale[c.table[0][4], 0] = 0.01
 
 
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_attention_beside_a_poisoned_block_is_what_it_is_without(cuda, which, typ):
+    """The rows before a poisoned block, those whose window has left it, and the other KV head's: the same values."""
+    import torch
+
+    c = Case(cuda, [120], [20], kv=2, hd=64, heads=4, page=16, seed=3)
+    q = c.randn(c.heads * c.hd, typ)
+    scale, at = getattr(c.cache, which), (c.table[0][4], 0)       # tokens 64 .. 79 of KV head 0 (heads 0, 1)
+    good = scale[at].clone()
+    for window in (0, 16):
+        want = want_attention(c, q, window=window).reshape(120, 4, 64)
+        for bad in (float("nan"), float("inf")):
+            scale[at] = bad
+            got = c.batch.attention(q, window=window).double().reshape(120, 4, 64)
+            scale[at] = good
+            assert check_errors() == 0
+            pos = torch.arange(20, 140, device=cuda)
+            sees = (pos >= 64) & ((pos - window < 79) if window else torch.ones_like(pos, dtype=torch.bool))
+            if bad != bad:
+                assert got[sees][:, :2].isnan().all()
+            assert (~sees).sum() > 40
+            for a, b in ((got[~sees], want[~sees]), (got[:, 2:], want[:, 2:])):
+                assert (((a - b).norm(dim=-1) / b.norm(dim=-1)) < 4 * TOL[typ]).all()
+                assert ((a - b).norm() / b.norm()).item() < TOL[typ]
+
+
 def test_attention_nan_query_stays_in_its_row(cuda):
     for typ, rows in (("f32", [1]), ("bf16", [50])):
         c = Case(cuda, rows, [70], kv=1, hd=128, heads=4, page=32, seed=2)
@@ -741,6 +783,44 @@ def test_offsets_past_32_bits(cuda):
         w = w.masked_fill(torch.ones(130, 130, device=cuda).triu(1).bool(), float("-inf"))
         want = torch.softmax(w, -1) @ vv[h]
         assert ((got[:, h] - want).norm() / want.norm()).item() < TOL["bf16"]
+
+
+def test_offsets_past_2_to_the_32(cuda):
+    """Pages whose bytes lie past 2^32 of the pool, rows whose elements lie past 2^31 of their matrix."""
+    import torch
+
+    from spk import paged
+
+    pages, page, kv, hd, n, ld = 17000, 128, 8, 256, 3, 2 ** 30 + 24
+    cache = paged.PagedCache(pages, page, kv, hd, device=cuda)
+    assert (pages - 2) * kv * page * hd > 2 ** 32 and 2 * ld > 2 ** 31
+    c = Case(cuda, [n], [127], kv=kv, hd=hd, heads=kv, page=page, seed=15)
+    c.cache, c.table = cache, [[pages - 1, pages - 2]]
+    c.tab = torch.tensor(c.table, dtype=torch.int32, device=cuda)
+    store = torch.empty(n * ld, dtype=torch.bfloat16, device=cuda)
+    row = lambda o, w: store[o:].as_strided((n, w), (ld, 1))  # noqa: E731
+    q, k, v, out = row(0, kv * hd), row(2048, kv * hd), row(4096, kv * hd), row(6144, kv * hd)
+    c.rows = [127]
+    c.len = [127]
+    first = paged.PagedBatch(cache, torch.tensor([0, 127], dtype=torch.int32, device=cuda),
+                             torch.tensor([127], dtype=torch.int32, device=cuda), c.tab, rows=127, heads=kv)
+    kk, vv = c.randn(kv * hd, "bf16"), c.randn(kv * hd, "bf16")
+    first.append(kk, vv)
+    for t in (q, k, v):
+        t.copy_(torch.randn(n, kv * hd, generator=c.g, device=cuda))
+    b = paged.PagedBatch(cache, c.row0, c.kv_len, c.tab, rows=n, heads=kv)
+    b.append(k, v)
+    b.attention(q, out)
+    assert check_errors() == 0
+    for name, rows in (("k", torch.cat([kk, k])), ("v", torch.cat([vv, v]))):
+        got = unpack_pages(cache, name, c.table[0])
+        got = torch.cat([got[p] for p in c.table[0]], 1)[:, :130].transpose(0, 1).reshape(130, -1)
+        assert ((got - rows.double()).norm() / rows.double().norm()).item() < 2 ** -4
+        kk, vv = (got, vv) if name == "k" else (kk, got)
+    w = torch.einsum("ihd,jhd->hij", q.double().reshape(n, kv, hd), kk.reshape(130, kv, hd)) / 16
+    w = w.masked_fill(torch.arange(130, device=cuda)[None] > torch.arange(127, 130, device=cuda)[:, None], float("-inf"))
+    want = torch.einsum("hij,jhd->ihd", torch.softmax(w, -1), vv.reshape(130, kv, hd)).reshape(n, -1)
+    assert ((out.double() - want).norm() / want.norm()).item() < TOL["bf16"]
 
 
 def unpack_pages(cache, name, pages):
