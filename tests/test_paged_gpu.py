@@ -656,6 +656,40 @@ def test_frequencies_are_f32_side_by_side_on_the_rows_device(cuda):
     check_attention(c, "f32", q=q, freq=good)
 
 
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,old", [([1], [40000]), ([9, 1, 30], [3000, 500, 9000]), ([400], [2000])])
+def test_attention_repeats_itself_bit_for_bit(cuda, rows, old, typ):
+    """Parts of a group are joined in the CTAs' order, whichever comes last."""
+    import torch
+
+    c = Case(cuda, rows, old, kv=2, hd=128, heads=8, page=64, seed=len(rows))
+    q = c.randn(c.heads * c.hd, typ)
+    first = c.batch.attention(q, freq=freqs(cuda, 64)).clone()
+    for _ in range(20):
+        assert torch.equal(c.batch.attention(q, freq=freqs(cuda, 64)), first)
+    assert check_errors() == 0
+
+
+def test_calls_without_rows(cuda):
+    import torch
+
+    from spk import paged, score
+
+    c = Case(cuda, [3, 2], [5, 30], kv=2, hd=64, heads=4, page=16, seed=3)
+    s = torch.cuda.Stream()
+    none = paged.PagedBatch(c.cache, torch.zeros(3, dtype=torch.int32, device=cuda), c.kv_len, c.tab, rows=0, heads=4)
+    before = c.cache.k_pool.view(torch.uint8).clone()
+    e = lambda w: torch.empty(0, w, device=cuda)  # noqa: E731
+    for stream in (None, s):
+        none.append(e(128), e(128), stream=stream)
+        assert none.attention(e(256), stream=stream).shape == (0, 256)
+        lp = score.LogProbs(0, 100, 3, device=cuda)
+        logp, ent, ids, best = lp(e(100), torch.empty(0, dtype=torch.int32, device=cuda), stream=stream)
+        assert logp.numel() == 0 and ids.shape == (0, 3)
+    torch.cuda.synchronize()
+    assert check_errors() == 0 and torch.equal(before, c.cache.k_pool.view(torch.uint8))
+
+
 def test_append_then_attention_is_attention_over_the_rounded_rows(cuda):
     """The two together, over pages as they come, against attention in 64 bits over what the cache holds."""
     c = Case(cuda, [60, 1, 9], [10, 200, 0], kv=4, hd=256, heads=16, page=32, seed=11)
