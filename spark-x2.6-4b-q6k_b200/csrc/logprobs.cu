@@ -8,8 +8,8 @@
 // row that holds a NaN or +inf, or only -inf, has no distribution: NaN for logp, H and the
 // alternatives' values (their indices stay those of the order, a NaN ranking as -inf).
 //
-// What bounds it: the row's bytes, then the exponentials (16 a clock and SM: 30 us of the 42 us that
-// 1024 x 131072 bf16 values take to read). A CTA streams a range of a row, 16 bytes a load, four loads
+// What bounds it: the row's bytes, then the exponentials (16 a clock and SM: 30 us beside the 42 us that
+// 1024 x 131072 bf16 values take to read; the unit is busy 56 % of the time, the issue slots 58 %). A CTA streams a range of a row, 16 bytes a load, four loads
 // a thread in flight; each thread keeps its own (m, S, A) in base 2, pairs of values by one f32x2
 // instruction, and moves m when a vector of values passes it. The best k (k <= 32) are a list over a
 // warp's lanes, as 64-bit keys (order of the value, then of the index). A vector is looked at again only
@@ -19,9 +19,10 @@
 // is cut over many CTAs (rows x splits fill the SMs); the last one to arrive, by a ticket that it
 // resets, joins the parts.
 //
-// Measured: 1024 x 131072 bf16, 5 alternatives, 64 us (4.2 TB/s, 0.65 of a copy's rate; with 3 tokens left in each row 127); 61 x 50021
-// f16, 1 alternative, 8.7 us; 1 x 131072 f32, 20 alternatives, 8.7 us, of which 1 us is the load, 3 the
-// launch and the ticket, and the rest the lists: compare and exchange, one behind the other.
+// Measured: 1024 x 131072 bf16, 5 alternatives, 67 us (4.0 TB/s, 0.62 of a copy's rate; with 3 tokens left in each row 127,
+// whole rows of the type's lowest value 175), f32 114 us; 61 x 50021 f16, 1 alternative, 8.9 us; 1 x 131072 f32, 20
+// alternatives, 8.5 us, of which 1 us is the load, 3 the launch and the ticket, and the rest the lists: compare and
+// exchange, one behind the other.
 #include <cuda_bf16.h>
 
 #include "common.cuh"

@@ -17,8 +17,9 @@
 // shuffle tree and one exchange between the warps. The bytes meet in shared memory (4 KB, 16-byte
 // pieces spread over the banks) and leave as 16-byte stores. Where there are many blocks a CTA walks
 // several head groups, which share the rows' angles: a cosine and sine cost as much as ten values'
-// rounding and storing. Measured: 16384 bf16 rows of 4 heads of 256, keys and values, 27 us (101 MB, 3.7 TB/s, 0.57
-// of a copy's rate); 13 f32 prompts of up to 1501 rows 12.8 us (44 MB); one row 3.7 us.
+// rounding and storing. Measured, launched one by one on rows that are not in L2: 16384 bf16 rows of 4 heads of 256,
+// keys and values, 29 us (101 MB, 3.5 TB/s, 0.54 of a copy's rate); 13 f32 prompts of up to 1501 rows 15.7 us (44 MB);
+// one row 5.9 us, which is a launch's distance from the next. In a graph, over the same rows again: 27, 12.7 and 3.7 us.
 #include "paged.cuh"
 
 namespace spk {
@@ -300,7 +301,7 @@ template <typename T, int HD>
 cudaError_t launch(AppendArgs a, cudaStream_t s) {
     const int groups = (a.pool.kv_heads + AP_WIDTH / HD - 1) / (AP_WIDTH / HD);
     // A CTA walks several head groups of its block, as long as every SM still gets its CTAs: they share the
-    // block's angles and hide each other's loads (16384 bf16 rows of 4 groups: 28 us with all 4, 30.6 with 2,
+    // block's angles and hide each other's loads (in a graph: 16384 bf16 rows of 4 groups: 28 us with all 4, 30.6 with 2,
     // 38.5 with 1; 4096 rows: 10.0 with 2, 10.4 with 1, 12.8 with 4; one row: 3.8 with 1, 5.3 with 2).
     const int slots = AP_CTAS<T> * sm_count(), units = a.b.rows / BLOCK;   // whole blocks: about what there is to do
     const long long most = 2ll * groups * units / slots;

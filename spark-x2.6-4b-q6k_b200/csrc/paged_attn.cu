@@ -30,10 +30,10 @@
 // What bounds it: for few rows the cached bytes, read once per KV head (an MMA of 16 columns costs
 // what its A bytes cost to read from shared memory, and the softmax runs on keys x rows alone); for
 // prompt chunks the softmax's instructions, 48 or 64 bf16 rows against each 128 keys. Measured, heads of 256, 4 a KV
-// head: one f32 row over 131072 keys 63 us (269 MB, 4.3 TB/s; a tile comes every 2850 clocks, what
-// the memory gives an SM, and 20 us are start, queries and joining); 64 bf16 rows of as many sequences of up to
-// 9000 keys 41 us (86 MB; a tile takes the MMA warp 2600 clocks, a change of group 14000); 2048 bf16 rows behind
-// 6144 cached ones 570 us (240 GFLOP, 0.42 PFLOP/s).
+// head: one f32 row over 131072 keys 63 us (269 MB, 4.3 TB/s; some 20 us are start, queries and joining);
+// 64 bf16 rows of as many sequences of up to 9000 keys 43 us (86 MB; a change of group costs as much as several
+// tiles); 2048 rows behind 6144 cached ones: bf16 570 us (240 GFLOP, 0.42 PFLOP/s; the tensor pipe is busy a quarter
+// of the time, the issue slots half of it), f16 750, f32 1030.
 //
 // Work split: all (sequence, KV head, row tile) groups stand in one line, each as long as the
 // tokens it reads plus COST for its fixed cost; the line is cut into equal ranges, one per CTA,
@@ -110,7 +110,7 @@ struct Cfg {
     static constexpr size_t V_OFF = (size_t)NK * SLOT, Q_OFF = V_OFF + (size_t)NV * SLOT, P_OFF = Q_OFF + (size_t)2 * CS * HD;
     static constexpr size_t SMEM = P_OFF + (size_t)NP * PB;
     // a group's fixed cost in blocks: what evened out the CTAs' times over 64 sequences of 1 to 9000 tokens
-    // (narrow: 8 40.4 us, 16 40.6, 32 42.0, 64 46.7) and 24 of 8 rows each (wide: 8 46 us, 16 37, 32 31, 64 33)
+    // (narrow: 8 40.3 us, 16 41.3, 32 41.5, 64 46.8) and 24 of 8 rows each (wide: 8 41 us, 16 36, 32 32, 64 37)
     static constexpr int COST = PG == 1 ? 32 : 16;
     static constexpr int LAG = PG == 1 ? 2 : 1;               // tiles that the values are behind the scores
     static constexpr int WARPS = FIRST_Q + Q_WARPS + 4 * SG * PG, THREADS = WARPS * 32;
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                 for (uint32_t y = 0; y < (1u << 20) && !mbar_try_wait(full_v + x % NV, (x / NV) & 1); y++) {}
     } else if (warp == 1) {   // ------------------------------------------------------ MMAs
         // The whole warp walks and waits and one elected thread issues, so the walk's state and the descriptors
-        // are the same in all its lanes (2048-row chunk 448 us; all of it in a branch of lane 0: 465).
+        // are the same in all its lanes (all of it in a branch of lane 0: 4 % more for a 2048-row chunk).
         const bool one = elect_one();
         const uint32_t desc0 = (1u << 4) | ((128u >> 4) << 24);
         const uint32_t sdesc = desc0 | ((uint32_t)(CS >> 3) << 17), odesc = desc0 | ((uint32_t)(CO >> 3) << 17);
@@ -1213,12 +1213,18 @@ int launch_one(const AttnParams &a, cudaStream_t s, const char *who) {
 
 // The columns follow the rows that a sequence has per KV head on average. A tile's cost grows with its
 // columns and a second tile reads the cache again, from L2; where the one outweighs the other was measured
-// (us; 64 sequences of up to 3000 keys, 8 of 6000, 1 of 16000; heads of 256):
-//   f32   8 rows: 6 a tile 41.3 21.8 26.1, 24 a tile 42.5 24.2 29.0;  16 rows: 51.0 23.6 30.7, 46.5 27.4 33.6
-//   bf16  8 rows: 5 a tile 38.9 20.8 25.3, 10 a tile 32.7 23.7 29.3;  24 rows: 10 a tile 50.5 27.5 33.7, 32 a
-//         tile 43.8 29.0 40.6;  32 rows: 54.1 34.7 37.7, 42.7 31.6 45.5
+// (us; 64 sequences of 1200 keys, 8 of 6000, 1 of 16000; heads of 256, and of 128 in brackets):
+//   f32   8 rows: 6 a tile 96 47 26 (78 38 24), 24 a tile 80 47 30 (66 35 25);  16: 138 62 31 (113 49 27), 84 50 35 (69 38 29)
+//   f16   4 rows: 5 a tile 32 32 22, 8 a tile 33 32 22;  8: 81 45 25 (69 36 22), 50 33 28 (42 26 23);
+//         24: 8 a tile 122 61 31 (103 48 26), 32 a tile 79 48 41 (69 38 35);  32: 157 74 35 (132 59 30), 81 50 46 (69 38 36)
+//   bf16  4 rows: 5 a tile 31 32 22, 10 a tile 36 32 24;  8: 79 45 25 (69 36 22), 55 34 30 (47 28 24);
+//         24: 10 a tile 135 63 34 (116 51 29), 32 a tile 76 47 40 (64 36 34);  32: 173 77 38 (151 63 33), 78 48 44 (64 36 35);
+//         192: 32 a tile 348 150 63 (320 121 52), 48 (64) a tile 307 129 63 (243 106 56);  256: 456 190 74 (421 154 62),
+//         453 174 72 (323 129 63);  1024, 8 and 1 sequences: 658 211 (561 178), 544 183 (426 145)
+// so one long sequence of up to 24 rows sets the narrow tiles' end and 192 rows the widest ones' start.
 // bf16 queries of 193 rows and more are of two terms, which is what bf16 itself holds: the scores' columns that this
-// saves are the output's (heads of 256: 2 x 96 + 2 x 144 of 512, 48 rows a tile, and 40 at the most with three).
+// saves are the output's (heads of 256: 2 x 96 + 2 x 144 of 512, 48 rows a tile, and 40 at the most with three). A
+// 2048-row chunk is off by 1.8e-3 of its output, and by 1.7e-3 from the rounding to bf16 alone.
 template <typename T, int HD>
 int launch(const AttnParams &a, cudaStream_t s, const char *who) {
     const long long per = ((long long)a.b.rows * a.group + a.b.nseq - 1) / a.b.nseq;

@@ -190,7 +190,8 @@ class PagedScorer:
         return logits
 
     def feed(self, new: dict, top: int = 0) -> dict:
-        """Scores new tokens {sequence: [ids]}: {sequence: Scored}. Synchronizes."""
+        """Scores new tokens {sequence: [ids]}: {sequence: Scored}. Synchronizes. The first token of a sequence's
+        later part is not scored: its distribution was the last row of the part before."""
         import torch
 
         seqs = self._check(new, MAX_ROWS, top)
