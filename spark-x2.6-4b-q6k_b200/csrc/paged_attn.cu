@@ -50,7 +50,7 @@ namespace spk {
 namespace paged {
 namespace {
 
-constexpr float M_NONE = -1e30f;      // reference of a part that has seen nothing
+constexpr float M_NONE = -INFINITY;   // reference of a part that has seen nothing
 // Weights are 2^(s' - m): a new reference sits W_TOP below the largest score, so weights start at 64, and
 // it moves only when a score passes m + 8, so they end at 256 (e4m3 holds 448). More room above would cost
 // the small ones (the terms' bytes end at 2^-9), less would move the reference more often.
@@ -1138,7 +1138,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) attn_kernel(const AttnParams a)
                             for (int p = lane; p < parts; p += 32) M = fmaxf(M, wt[r * parts + p]);
                             M = warp_max(M);
                             for (int p = lane; p < parts; p += 32) {
-                                const float f = ex2(wt[r * parts + p] - M);
+                                const float m = wt[r * parts + p], f = m == M_NONE ? 0.f : ex2(m - M);
                                 wt[r * parts + p] = f;
                                 L = fmaf(wl[r * parts + p], f, L);
                             }

@@ -656,6 +656,25 @@ def test_frequencies_are_f32_side_by_side_on_the_rows_device(cuda):
     check_attention(c, "f32", q=q, freq=good)
 
 
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [[1], [300]])
+def test_attention_of_scores_that_are_all_far_below_zero(cuda, rows, typ):
+    """Every key the same and every query its opposite, of any size: the mean of the values seen, in one part or in many."""
+    import torch
+
+    c = Case(cuda, rows, [20000], kv=1, hd=64, heads=1, page=64, seed=5)
+    c.cache.k_pool.copy_(c.cache.k_pool[0, 0, 0, :, :1].expand_as(c.cache.k_pool))
+    c.cache.k_scale.fill_(0.01)
+    c.cache.v_scale.fill_(0.01)
+    q = -unpack_k(c.cache.k_pool[:1])[0, 0, :1].expand(rows[0], 64)
+    v = (unpack_v(c.cache.v_pool)[:, 0] * 0.01)[c.table[0]].reshape(-1, 64)
+    mean = (v.cumsum(0) / torch.arange(1, len(v) + 1, device=cuda)[:, None])[20000:20000 + rows[0]]
+    for size in (1e-3, 1e25, 1e33):
+        got = c.batch.attention((q * size).to(ttype(typ))).double()
+        assert check_errors() == 0
+        assert ((got - mean).norm() / mean.norm()).item() < TOL[typ], size
+
+
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows,old", [([1], [40000]), ([9, 1, 30], [3000, 500, 9000]), ([400], [2000])])
 def test_attention_repeats_itself_bit_for_bit(cuda, rows, old, typ):
