@@ -505,6 +505,77 @@ typedef struct {
 size_t spk_paged_attn_workspace_bytes(int head_dim);
 int spk_paged_attn(const spk_kv_pool *pool, const spk_kv_batch *batch, const spk_paged_attn_args *args, void *stream);
 
+/* The same in 4 bits: a row of a KV head (head_dim values of one token) is head_dim / 2 bytes of codes and head_dim / 16 scale
+ * bytes, keys and values apart, 4.5 bits a value. Code c stands for 0, .5, 1, 1.5, 2, 3, 4, 6 (c & 7), negative with bit 3;
+ * scale byte b for the f16 number of the bits b << 7; a value is code x scale. Per (page, KV head):
+ *   k, v               [page_tokens][head_dim / 2]     byte i of a row: dims 2 i (low half) and 2 i + 1
+ *   k_scale, v_scale   [page_tokens][head_dim / 16]
+ * The pool needs no initial contents; a call writes the rows that it appends and nothing else. head_dim 64, 128 or 256;
+ * page_tokens a multiple of 16; buffers 16-byte aligned. */
+typedef struct {
+    void *k, *v;                /* device [pages][kv_heads][page_tokens * head_dim / 2] bytes */
+    void *k_scale, *v_scale;    /* device [pages][kv_heads][page_tokens * head_dim / 16] bytes */
+    int pages, page_tokens, kv_heads, head_dim;
+} spk_kv4_pool;
+
+/* A projection's rows: queries and keys normalised and rotated, queries out, keys and values into the pages, in one pass.
+ * Per head, with q_norm / k_norm ([head_dim] f32, 16-byte aligned; NULL: none): x / sqrt(mean x^2 + eps) * norm. Then, with
+ * freq, the rotation by f32(position * freq[i]), i < pdim / 2 (pdim a multiple of 16), of the pairs (i, i + pdim / 2), or
+ * (2 i, 2 i + 1) where `interleaved`. heads 0: no queries. q_out may be q itself (the same rows and stride).
+ * Rounding, per group of 16 values: the scale is the number of 4 significant bits nearest to amax / 6 (ties to even, 2^-14 to
+ * 10240), a code the nearest to value / scale (ties to the even code, at most 6 in magnitude); both are decided exactly
+ * for the f32 value at hand. A NaN or infinity makes its group's scale byte 255 (NaN). */
+typedef struct {
+    const void *q;              /* [rows][heads * head_dim] of type, rows ldq elements apart */
+    long long ldq;
+    void *q_out;                /* the same, ldq_out apart */
+    long long ldq_out;
+    const void *k, *v;          /* [rows][kv_heads * head_dim] */
+    long long ldk, ldv;
+    int type, heads;            /* 0 f32, 1 f16, 2 bf16 (all rows) */
+    const float *q_norm, *k_norm;
+    float eps;
+    const float *freq;          /* device [pdim / 2], or NULL: no rotation */
+    int pdim, interleaved;
+} spk_paged4_append_args;
+int spk_paged4_append(const spk_kv4_pool *pool, const spk_kv_batch *batch, const spk_paged4_append_args *args, void *stream);
+
+/* The batch's rows back from the pages: values in f32, f16 or bf16 (exact in each), or with SPK_PAGED4_PARTS the codes as e4m3
+ * bytes and the scales as f16 numbers, [rows][kv_heads * head_dim / 16]. k or v may be NULL. A row whose page
+ * is none is left as it was. */
+#define SPK_PAGED4_PARTS 3
+typedef struct {
+    int type;
+    void *k, *v;                /* [rows][kv_heads * head_dim], ldk / ldv elements apart */
+    long long ldk, ldv;
+    void *k_scale, *v_scale;    /* with SPK_PAGED4_PARTS */
+    long long ldk_scale, ldv_scale;
+} spk_paged4_read_args;
+int spk_paged4_read(const spk_kv4_pool *pool, const spk_kv_batch *batch, const spk_paged4_read_args *args, void *stream);
+
+/* Causal grouped-query attention of the rows over their sequences' 4-bit pages (append them first; queries come as
+ * spk_paged4_append leaves them):
+ *   out[t][h] = sigmoid(gate[t][h]) * softmax_j(scale * q[t][h] . K_j) V_j
+ * over j in [0, pos_t] (window 0) or (pos_t - window, pos_t]; q head h reads KV head h / (heads / kv_heads), any group. The
+ * softmax and all sums are in f32; queries and weights meet the cached values as f16 numbers on a power of two of their row,
+ * f32 rows' as two. A row that sees nothing gets 0; a row that sees a token of which a group is NaN gets NaN.
+ * workspace: spk_paged4_attn_workspace_bytes(head_dim) device bytes for the device current at the call, zeroed once and
+ * left ready; calls that share one must not overlap on the GPU. No sync. */
+typedef struct {
+    const void *q;              /* [rows][heads * head_dim] of type, rows ldq elements apart */
+    long long ldq;
+    int type, heads;            /* 0 f32, 1 f16, 2 bf16 (q, gate and out) */
+    int window;
+    float scale;                /* 0: 1 / sqrt(head_dim) */
+    const void *gate;           /* [rows][heads] pre-sigmoid, rows ldgate apart, or NULL */
+    long long ldgate;
+    void *out;                  /* [rows][heads * head_dim], rows ldout apart */
+    long long ldout;
+    void *workspace;
+} spk_paged4_attn_args;
+size_t spk_paged4_attn_workspace_bytes(int head_dim);
+int spk_paged4_attn(const spk_kv4_pool *pool, const spk_kv_batch *batch, const spk_paged4_attn_args *args, void *stream);
+
 /* What rows of logits say (scoring, n-best; the reference keeps the argmax alone, model.rs:594-604):
  * for each of `rows` rows of `vocab` values of `type` (0 f32, 1 f16, 2 bf16), ld apart: logp (may
  * be NULL) the log probability of target[row] (0 where the target is negative), entropy (may be

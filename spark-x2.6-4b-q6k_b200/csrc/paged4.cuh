@@ -1,0 +1,54 @@
+// paged4.cuh — what the paged 4-bit cache's kernels share (paged4_append.cu, paged4_attn.cu).
+//
+// A row of a KV head (head_dim values of one token) is kept as groups of 16 values: a code of 4 bits a value and a scale
+// byte a group, keys and values apart, 4.5 bits a value. Code c stands for 0, .5, 1, 1.5, 2, 3, 4, 6 (c & 7) with the
+// sign of bit 3 (e2m1); scale byte b for the f16 number of the bits b << 7, five of exponent and three of fraction. A value is
+// code x scale: at most six bits of fraction, so f16 holds it exactly (2^-15 to 61440), and so do bf16 and f32: what the
+// kernels multiply is what the cache stands for. Per (page, KV head):
+//   codes   [page_tokens][head_dim / 2]    byte i of a row: dims 2 i (low half) and 2 i + 1
+//   scales  [page_tokens][head_dim / 16]
+// A row's codes and scales depend on that row alone, so a call never touches what an earlier one wrote. A group that held a
+// NaN or an infinity has the scale byte 255 (f16 NaN) and reads as NaN.
+#pragma once
+#include "paged.cuh"
+
+namespace spk {
+namespace paged4 {
+
+using paged::BLOCK;
+using paged::Batch;
+using paged::MAX_SEQ;
+using paged::T_BF16;
+using paged::T_F16;
+using paged::T_F32;
+
+constexpr int GROUP = 16;                       // values that share a scale
+constexpr float SCALE_MIN = 0x1p-14f, SCALE_MAX = 10240.0f;   // 6 x 10240 is the largest six-bit number under f16's end
+constexpr uint32_t POISON = 0xf8;               // scale bytes from here on are no numbers
+
+struct Pool {
+    uint8_t *k, *v, *ks, *vs;
+    int pages, page_tokens, kv_heads, hd;
+};
+inline Pool pool_of(const spk_kv4_pool *p) {
+    return Pool{(uint8_t *)p->k, (uint8_t *)p->v, (uint8_t *)p->k_scale, (uint8_t *)p->v_scale, p->pages, p->page_tokens, p->kv_heads, p->head_dim};
+}
+int check_pool(const spk_kv4_pool *p, const char *who);
+
+// A token's row among the rows of a pool: (page, KV head, token of the page).
+__device__ __forceinline__ size_t row_index(const Pool &p, int page, int head, int tok) {
+    return ((size_t)page * p.kv_heads + head) * p.page_tokens + tok;
+}
+
+// The two values of a byte of codes, f16: the low half's in the low half.
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(w));
+}
+// Whether one of four scale bytes is no number: a five-bit exponent of ones carries out of its field.
+__device__ __forceinline__ uint32_t poisoned(uint32_t w) { return (((w >> 3) & 0x1f1f1f1fu) + 0x01010101u) & 0x20202020u; }
+
+}  // namespace paged4
+}  // namespace spk

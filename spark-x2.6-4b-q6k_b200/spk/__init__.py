@@ -125,6 +125,10 @@ _PROTOS = {
     "spk_paged_append": ([_vp, _vp, _vp, _ll, _vp, _ll, _i, _vp, _i, _vp], _i),
     "spk_paged_attn_workspace_bytes": ([_i], C.c_size_t),
     "spk_paged_attn": ([_vp, _vp, _vp, _vp], _i),
+    "spk_paged4_append": ([_vp, _vp, _vp, _vp], _i),
+    "spk_paged4_read": ([_vp, _vp, _vp, _vp], _i),
+    "spk_paged4_attn_workspace_bytes": ([_i], C.c_size_t),
+    "spk_paged4_attn": ([_vp, _vp, _vp, _vp], _i),
     "spk_logprobs_workspace_bytes": ([_i, _i], C.c_size_t),
     "spk_logprobs": ([_vp, _i, _i, _i, _ll, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp], _i),
 }

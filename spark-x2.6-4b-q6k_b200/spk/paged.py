@@ -231,12 +231,40 @@ class PageTable:
                             dtype=torch.int32, device=device)
 
 
+def _attend(batch, q, out, window, gate, scale, stream, *more):
+    """The batch's attention call: the rows' checks, the output, the stream; `more`: other tensors that it reads."""
+    width = batch.heads * batch.cache.head_dim
+    a = batch._a
+    a.ldq = _rows(q, batch.rows, width, "q", on=batch.cache.device)
+    if out is None:
+        import torch
+
+        with torch.cuda.stream(stream):      # None: the current one
+            out = torch.empty(batch.rows, width, dtype=q.dtype, device=q.device)
+    a.ldout = _rows(out, batch.rows, width, "out", q)
+    a.q, a.out, a.type, a.window, a.scale = q.data_ptr(), out.data_ptr(), type_of(q), window, scale
+    a.gate = None
+    if gate is not None:
+        a.ldgate = _rows(gate, batch.rows, batch.heads, "gate", q)
+        a.gate = gate.data_ptr()
+    raw = stream_of(q, stream)
+    batch.cache.owned.use(raw, stream)
+    batch.owned.use(raw, stream)
+    check(batch._attn(batch._pool_p, batch._batch_p, batch._attn_p, raw))
+    lent(stream, q, out, gate, *more, *batch._keep)
+    return out
+
+
 class PagedBatch:
     """The rows of a call over a pool. row0 int32 [nseq + 1], kv_len int32 [nseq] (the call's rows
     counted), table int32 [nseq][max_pages], on the pool's device; `rows` = row0[nseq]. Holds the
     attention's workspace: calls of one batch must not overlap on the GPU."""
 
+    _cache = PagedCache
+
     def __init__(self, cache: PagedCache, row0, kv_len, table, rows: int, heads: int):
+        if not isinstance(cache, self._cache):
+            raise SpkError(f"{type(self).__name__} takes a {self._cache.__name__}; got a {type(cache).__name__}")
         import torch
 
         nseq = kv_len.numel()
@@ -250,18 +278,26 @@ class PagedBatch:
         self.cache, self.rows, self.heads = cache, rows, heads
         self._keep = (row0, kv_len, table)
         self._b = _Batch(nseq, rows, row0.data_ptr(), kv_len.data_ptr(), table.data_ptr(), table.shape[1])
-        L = lib()
-        with torch.cuda.device(cache.device):
-            self.workspace = torch.zeros(L.spk_paged_attn_workspace_bytes(cache.head_dim), dtype=torch.uint8,
-                                         device=cache.device)
+        self._bind()
         self.owned = Owned(self.workspace)
-        self._a = _Attn(heads=heads, workspace=self.workspace.data_ptr())
         self._pool_p, self._batch_p, self._attn_p = C.addressof(cache._c), C.addressof(self._b), C.addressof(self._a)
+
+    def _bind(self) -> None:
+        """The workspace, the attention's arguments and the entry points."""
+        import torch
+
+        L = lib()
+        with torch.cuda.device(self.cache.device):
+            self.workspace = torch.zeros(L.spk_paged_attn_workspace_bytes(self.cache.head_dim), dtype=torch.uint8,
+                                         device=self.cache.device)
+        self._a = _Attn(heads=self.heads, workspace=self.workspace.data_ptr())
         self._append, self._attn = L.spk_paged_append, L.spk_paged_attn
 
     def use(self, cache: PagedCache) -> None:
         """Turns the batch to another layer's pool of the same geometry (the page table is the layers' own)."""
         c = self.cache
+        if not isinstance(cache, self._cache):
+            raise SpkError(f"{type(self).__name__} takes a {self._cache.__name__}; got a {type(cache).__name__}")
         if (cache.pages, cache.page_tokens, cache.kv_heads, cache.head_dim, cache.device) != (
                 c.pages, c.page_tokens, c.kv_heads, c.head_dim, c.device):
             raise SpkError("a pool of another geometry")
@@ -282,24 +318,5 @@ class PagedBatch:
         """out [rows][heads * head_dim] (made when not given): attention of the rows, which have been
         appended, over their sequences; q is rotated when freq is given, `gate` [rows][heads] goes
         through a sigmoid, `window` 0 sees every earlier token, `scale` 0 is 1 / sqrt(head_dim)."""
-        width = self.heads * self.cache.head_dim
-        a = self._a
-        a.ldq = _rows(q, self.rows, width, "q", on=self.cache.device)
-        if out is None:
-            import torch
-
-            with torch.cuda.stream(stream):      # None: the current one
-                out = torch.empty(self.rows, width, dtype=q.dtype, device=q.device)
-        a.ldout = _rows(out, self.rows, width, "out", q)
-        a.q, a.out, a.type, a.window, a.scale = q.data_ptr(), out.data_ptr(), type_of(q), window, scale
-        a.gate = None
-        if gate is not None:
-            a.ldgate = _rows(gate, self.rows, self.heads, "gate", q)
-            a.gate = gate.data_ptr()
-        a.freq, a.pdim = _angles(freq, q)
-        raw = stream_of(q, stream)
-        self.cache.owned.use(raw, stream)
-        self.owned.use(raw, stream)
-        check(self._attn(self._pool_p, self._batch_p, self._attn_p, raw))
-        lent(stream, q, out, gate, freq, *self._keep)
-        return out
+        self._a.freq, self._a.pdim = _angles(freq, q)
+        return _attend(self, q, out, window, gate, scale, stream, freq)

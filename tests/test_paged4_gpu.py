@@ -1,0 +1,638 @@
+"""spk_paged4_append, spk_paged4_read and spk_paged4_attn against a 64-bit restatement of their definitions.
+
+Bounds. Rows that are rounded as they are (values; keys without a norm or a rotation) have one right code and scale: equality.
+A rotated or normalised key is off by f32 rounding before its rounding to 4 bits: the norm's sum, square root and two products,
+cosine and sine to 2 ulp, two products and a sum, under 2^-20 of its pair's length; the stored code has to be right for some value within
+that, and the scale for some amax within it. Queries: the same, and their type's rounding (half a unit).
+
+Attention reads the cache exactly (a value is an f16 number). Its error, against the sum W = sum_j p_j |V_j| of what it adds: the weights'
+rounding (f16: 2^-12 each, the sum that divides by them rounded alike, so 2^-11 together; f32: two terms, 2^-22), the scores' f32 sums and their
+queries' rounding (f16 rows exact, bf16 rows exact above 2^-24 of the largest, f32 rows 2^-22 of the largest): 2^-20 S with S the largest sum_d |q_d k_d|
+scale of the row, the sums of the outputs, which the tensor cores cut towards 0: 2^-22 for each of at most 64 + n / 64 additions; and the output type's half unit. With the
+gate's exponential and the division 2^-20 more. Weights are f16 numbers, the largest between 2^12 and 2^15, so a small one is off by half of f16's
+last bit, 2^-25, which is 2^-37 of the largest: 2^-37 max p sum_j |V_j| besides."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TINY = {"f32": 2.0 ** -149, "f16": 2.0 ** -25, "bf16": 2.0 ** -133}
+HAVE = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+EDGES = [(0.25, False), (0.75, True), (1.25, False), (1.75, True), (2.5, False), (3.5, True), (5.0, False)]   # up at the tie
+
+
+def ttype(name):
+    import torch
+
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def freqs(dev, pdim, theta=1e4):
+    from spk import paged
+
+    return paged.rope_freq(theta, pdim, dev) if pdim else None
+
+
+def check_errors():
+    import spk
+
+    return spk.lib().spk_check_device_error()
+
+
+class Case:
+    """A 4-bit pool with random contents where sequences have tokens and poison everywhere else, a page table in random
+    order, and a batch over it."""
+
+    def __init__(self, dev, rows, old, kv=2, hd=128, page=32, heads=None, seed=0, pages=None, scales=(95, 120)):
+        import torch
+
+        from spk import paged4
+
+        self.dev, self.rows, self.len, self.kv, self.hd, self.page = dev, rows, [a + b for a, b in zip(rows, old)], kv, hd, page
+        g = self.g = torch.Generator(device=dev)
+        g.manual_seed(seed)
+        need = [max(0, -(-n // page)) for n in self.len]
+        total = sum(need) + 2
+        order = torch.randperm(total, generator=g, device=dev).int().cpu().tolist()
+        if pages:
+            order = [pages - 1 - p for p in order]      # the pool's far end
+        width = max(1, max(need))
+        self.table = [[order.pop() for _ in range(n)] + [-1] * (width - n) for n in need]
+        c = self.cache = paged4.Paged4Cache(pages or total, page, kv, hd, device=dev)
+        c.k_scale.fill_(255)
+        c.v_scale.fill_(255)
+        for s, n in enumerate(self.len):
+            for i, p in enumerate(self.table[s][:need[s]]):
+                m = min(page, n - i * page)
+                for pool, scale in ((c.k_pool, c.k_scale), (c.v_pool, c.v_scale)):
+                    pool[p].random_(0, 256, generator=g)
+                    scale[p, :, :m] = torch.randint(*scales, (kv, m, hd // 16), generator=g, device=dev).to(torch.uint8)
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+        self.row0 = i32(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32).tolist())
+        self.kv_len, self.tab = i32(self.len), i32(self.table)
+        self.heads = heads or kv
+        self.batch = paged4.Paged4Batch(c, self.row0, self.kv_len, self.tab, rows=sum(rows), heads=self.heads)
+
+    def randn(self, width, typ, scale=1.0):
+        import torch
+
+        return torch.randn(sum(self.rows), width, generator=self.g, device=self.dev).mul_(scale).to(ttype(typ))
+
+    def places(self):
+        """(page, token of the page) of every row."""
+        at = [(self.table[s][p // self.page], p % self.page) for s, (n, L) in enumerate(zip(self.rows, self.len)) for p in range(L - n, L)]
+        return [p for p, _ in at], [o for _, o in at]
+
+    def positions(self):
+        return [p for n, L in zip(self.rows, self.len) for p in range(L - n, L)]
+
+    def cached(self, s, name):
+        """[kv][len][hd] of sequence s, in 64 bits."""
+        import torch
+
+        c, n = self.cache, self.len[s]
+        take = torch.tensor(self.table[s][:-(-n // self.page)], dtype=torch.long, device=self.dev)
+        pool, b = (c.k_pool, c.k_scale) if name == "k" else (c.v_pool, c.v_scale)
+        return numbers(pool[take], b[take]).transpose(0, 1).reshape(self.kv, -1, self.hd)[:, :n]
+
+
+def numbers(pool, b):
+    import torch
+
+    have = torch.tensor(HAVE + [-x for x in HAVE], dtype=torch.float64, device=pool.device)
+    x = torch.stack([have[(pool & 15).long()], have[(pool >> 4).long()]], -1).flatten(-2)
+    return x * (b.to(torch.int16) << 7).view(torch.float16).double().repeat_interleave(16, -1)
+
+
+# ------------------------------------------------------------------------------------------ append
+
+def scale_byte(amax):
+    """The byte of the number of 4 significant bits nearest to amax / 6, ties to even, in 64 bits; 255 for an infinite one."""
+    import torch
+
+    m, e = torch.frexp((amax / 6).clamp(2.0 ** -14, 10240))
+    b = (torch.ldexp((m * 16).round(), e - 4).half().view(torch.int16) >> 7).to(torch.uint8)
+    return torch.where(amax.isfinite(), b, torch.full_like(b, 255))
+
+
+def codes(x, b, slack=None):
+    """The code magnitudes of x / d by comparison with the borders; with slack, the lowest and highest that some value within it has."""
+    import torch
+
+    d = (b.to(torch.int16) << 7).view(torch.float16).double().repeat_interleave(16, -1)
+    lo, hi = (x.abs(), x.abs()) if slack is None else ((x.abs() - slack).clamp(min=0), x.abs() + slack)
+    count = lambda a: sum(((a >= e * d) if up else (a > e * d)).to(torch.uint8) for e, up in EDGES)  # noqa: E731
+    return count(lo), count(hi)
+
+
+def head_rows(x, n, hd, w, eps, pos, freq, inter):
+    """(rows normalised and rotated, their pairs' lengths) in 64 bits."""
+    import torch
+
+    x = x.double().reshape(-1, n, hd)
+    if w is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * w.double()
+    size = x.abs()
+    if freq is None:
+        return x, size
+    h = freq.numel()
+    ang = (torch.tensor(pos, dtype=torch.float32, device=x.device)[:, None] * freq[None]).double()
+    c, s = ang.cos()[:, None], ang.sin()[:, None]
+    i, j = (slice(0, 2 * h, 2), slice(1, 2 * h, 2)) if inter else (slice(0, h), slice(h, 2 * h))
+    y, size = x.clone(), size.clone()
+    y[..., i], y[..., j] = x[..., i] * c - x[..., j] * s, x[..., j] * c + x[..., i] * s
+    size[..., i] = size[..., j] = torch.hypot(x[..., i], x[..., j])
+    return y, size
+
+
+def unpacked(pool):
+    import torch
+
+    return torch.stack([pool & 15, pool >> 4], -1).flatten(-2)
+
+
+def check_append(c, k, v, q=None, freq=None, inter=False, wq=None, wk=None, eps=1e-6, typ="f32", exact_k=False):
+    import torch
+
+    before = [t.clone() for t in (c.cache.k_pool, c.cache.v_pool, c.cache.k_scale, c.cache.v_scale)]
+    q_out = torch.full_like(q.contiguous(), 777.0) if q is not None else None
+    got = c.batch.append(k, v, freq=freq, interleaved=inter, q=q, q_out=q_out, q_norm=wq, k_norm=wk, eps=eps)
+    assert check_errors() == 0
+    pg, off = c.places()
+    pos = c.positions()
+    if q is not None:
+        assert got is q_out
+        y, size = head_rows(q, c.heads, c.hd, wq, eps, pos, freq, inter)
+        y, size = y.flatten(1), size.flatten(1)
+        assert ((got.double() - y).abs() <= HALF[typ] * y.abs() + TINY[typ] + 2.0 ** -20 * size).all()
+    for name, x in (("k", k), ("v", v)):
+        pool, scale = (c.cache.k_pool, c.cache.k_scale) if name == "k" else (c.cache.v_pool, c.cache.v_scale)
+        if name == "k":
+            y, size = head_rows(x, c.kv, c.hd, wk, eps, pos, freq, inter)
+        else:
+            y, size = x.double().reshape(-1, c.kv, c.hd), None
+        code, b = unpacked(pool[pg, :, off]), scale[pg, :, off]
+        amax = y.abs().unflatten(-1, (-1, 16)).amax(-1)
+        if name == "v" or exact_k or (wk is None and freq is None):
+            assert torch.equal(b, scale_byte(amax)), name
+            lo, hi = codes(y, b)
+        else:
+            slack = 2.0 ** -20 * size
+            s16 = slack.unflatten(-1, (-1, 16)).amax(-1)
+            assert ((b >= scale_byte(amax - s16)) & (b <= scale_byte(amax + s16))).all()
+            lo, hi = codes(y, b, slack)
+        real = amax.isfinite().repeat_interleave(16, -1)
+        assert ((code & 7 >= lo) & (code & 7 <= hi))[real].all() and (code[~real] == 0).all(), name
+        sure = (y != 0) & (lo > 0) & real
+        assert ((code >> 3).bool() == (y < 0))[sure].all()
+    # nothing else was touched
+    for was, now in zip(before, (c.cache.k_pool, c.cache.v_pool, c.cache.k_scale, c.cache.v_scale)):
+        if len(pg):
+            now = now.clone()
+            now[pg, :, off] = was[pg, :, off]
+        assert torch.equal(was, now)
+
+
+APPENDS = [
+    # rows, tokens before, kv, hd, page, heads, type, pdim, interleaved, norms
+    ([1], [4103], 4, 256, 64, 16, "f32", 64, False, False),
+    ([1], [0], 1, 64, 16, 1, "bf16", 0, False, False),
+    ([1, 0, 1, 1], [5, 9, 0, 47], 2, 128, 16, 4, "f16", 128, False, True),
+    ([33, 1, 0, 16, 7], [3, 0, 2, 16, 90], 4, 256, 32, 8, "f32", 256, True, False),
+    ([33, 1, 0, 16, 7], [3, 0, 2, 16, 90], 3, 64, 48, 15, "bf16", 32, False, True),
+    ([130, 65], [0, 1], 2, 256, 128, 10, "bf16", 64, False, True),
+    ([17, 40], [31, 0], 8, 64, 16, 8, "f16", 16, True, True),
+    ([50], [100000], 2, 128, 64, 6, "f32", 64, False, True),
+    ([3] * 70, list(range(70)), 1, 128, 16, 3, "f16", 32, True, False),
+]
+
+
+@pytest.mark.parametrize("rows,old,kv,hd,page,heads,typ,pdim,inter,norm", APPENDS)
+def test_append(cuda, rows, old, kv, hd, page, heads, typ, pdim, inter, norm):
+    import torch
+
+    c = Case(cuda, rows, old, kv, hd, page, heads, seed=5)
+    qkv = c.randn((heads + 2 * kv) * hd, typ)
+    q, k, v = qkv[:, :heads * hd], qkv[:, heads * hd:(heads + kv) * hd], qkv[:, (heads + kv) * hd:]
+    w = [torch.rand(hd, generator=c.g, device=cuda) + 0.5 for _ in "qk"] if norm else [None, None]
+    check_append(c, k, v, q, freqs(cuda, pdim), inter, w[0], w[1], typ=typ)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("off,pad", [(0, 1), (1, 0), (3, 5), (8, 8)])
+def test_append_takes_rows_of_any_stride_and_alignment(cuda, typ, off, pad):
+    c = Case(cuda, [5, 9], [0, 3], 2, 64, 16, 4, seed=6)
+    wide = c.randn(8 * 64 + off + pad, typ)[:, off:]
+    check_append(c, wide[:, 256:384], wide[:, 384:512], wide[:, :256], freqs(cuda, 32), typ=typ)
+
+
+def test_append_in_place_and_without_queries(cuda):
+    import torch
+
+    for kw in (dict(), dict(freq=freqs(cuda, 128)), dict(freq=freqs(cuda, 64), interleaved=True), dict(q_norm=torch.rand(128, device=cuda) + 0.5)):
+        c = Case(cuda, [9, 20], [4, 0], 2, 128, 16, 6, seed=7)
+        k, v, q = c.randn(256, "bf16"), c.randn(256, "bf16"), c.randn(768, "bf16")
+        apart = c.batch.append(k, v, q=q, **kw)
+        assert c.batch.append(k, v, q=q, q_out=q, **kw) is q and torch.equal(q, apart)
+        pools = [t.clone() for t in (c.cache.k_pool, c.cache.v_pool, c.cache.k_scale, c.cache.v_scale)]
+        kw.pop("q_norm", None)
+        assert c.batch.append(k, v, **kw) is None
+        assert all(torch.equal(a, b) for a, b in zip(pools, (c.cache.k_pool, c.cache.v_pool, c.cache.k_scale, c.cache.v_scale)))
+
+
+def test_values_on_and_beside_the_borders(cuda):
+    """f32 values at each border times each scale, a unit under and over it: the codes are those of exact arithmetic."""
+    import torch
+
+    mant = torch.arange(8, 16, dtype=torch.float64, device=cuda) / 8
+    rows = []
+    for e in (-14, -13, 0, 7, 13):
+        for m in mant.tolist():
+            d = m * 2.0 ** e
+            if d > 10240:
+                continue
+            for nudge in (-1, 0, 1):
+                x = torch.tensor([t * d for t, _ in EDGES] + [6 * d] + [t * d for t in HAVE], dtype=torch.float32, device=cuda)
+                x[:7] = torch.nextafter(x[:7], torch.full_like(x[:7], float("inf") if nudge > 0 else 0.0)) if nudge else x[:7]
+                rows.append(x * torch.where(torch.arange(16, device=cuda) % 3 == 1, -1.0, 1.0))
+    # amax on and beside the borders between two scales
+    for e in (-14, 3, 12):
+        for m in range(17, 32, 2):
+            for nudge in (-1, 0, 1):
+                a = torch.tensor(6 * m / 16 * 2.0 ** e, dtype=torch.float32, device=cuda)
+                a = torch.nextafter(a, torch.full_like(a, float("inf") if nudge > 0 else 0.0)) if nudge else a
+                rows.append(torch.cat([a[None], a * torch.linspace(-0.9, 0.9, 15, device=cuda)]))
+    # next to nothing, and more than there is
+    for a in (0.0, 1e-45, 1e-30, 2.0 ** -16, 6 * 2.0 ** -14, 61439.0, 61440.0, 63000.0, 65504.0, 1e30, 3.4e38):
+        rows.append(torch.linspace(-1, 1, 16, device=cuda) * a)
+    while len(rows) % 8:
+        rows.append(torch.zeros(16, device=cuda))
+    x = torch.cat(rows).reshape(-1, 128)
+    for typ in ("f32", "bf16", "f16"):
+        c = Case(cuda, [x.shape[0]], [0], 1, 128, 16, 1)
+        t = x.to(ttype(typ))
+        if typ == "f16":
+            t = t.clamp(-65504, 65504)
+        check_append(c, t.flip(0).contiguous(), t, typ=typ)
+
+
+def test_append_of_no_numbers_poisons_their_group_alone(cuda):
+    import torch
+
+    c = Case(cuda, [6], [2], 2, 64, 16, 2)
+    k, v = c.randn(128, "f32"), c.randn(128, "f32")
+    v[0, 3], v[1, 40], k[2, 70], k[3, 127] = float("nan"), float("inf"), float("-inf"), float("nan")
+    c.batch.append(k, v)
+    pg, off = c.places()
+    kb, vb = c.cache.k_scale[pg, :, off].reshape(6, 8), c.cache.v_scale[pg, :, off].reshape(6, 8)
+    assert (kb == 255).nonzero().tolist() == [[2, 4], [3, 7]]
+    assert (vb == 255).nonzero().tolist() == [[0, 0], [1, 2]]
+    rk, rv = c.batch.read(dtype=torch.float32)
+    assert rk.isnan().reshape(6, 8, 16).any(-1).nonzero().tolist() == [[2, 4], [3, 7]]
+    assert rv.isnan().reshape(6, 8, 16).all(-1).nonzero().tolist() == [[0, 0], [1, 2]]
+
+
+# -------------------------------------------------------------------------------------------- read
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,old,kv,hd,page", [([1], [0], 1, 64, 16), ([40], [4000], 4, 256, 64), ([33, 0, 5, 300], [0, 4, 100, 9], 3, 128, 48), ([7] * 90, [1] * 90, 2, 64, 16)])
+def test_read(cuda, typ, rows, old, kv, hd, page):
+    import torch
+
+    c = Case(cuda, rows, old, kv, hd, page, scales=(8, 227))
+    pg, off = c.places()
+    want = [numbers(p[pg, :, off], b[pg, :, off]).flatten(1) for p, b in ((c.cache.k_pool, c.cache.k_scale), (c.cache.v_pool, c.cache.v_scale))]
+    for got, w in zip(c.batch.read(dtype=ttype(typ)), want):
+        assert got.dtype == ttype(typ) and torch.equal(got.double(), w)
+    # rows that lie apart, at odd places; the columns between stay
+    wide = torch.full((sum(rows), 2 * kv * hd + 7), 5.0, dtype=ttype(typ), device=cuda)
+    k, v = wide[:, 1:1 + kv * hd], wide[:, 4 + kv * hd:4 + 2 * kv * hd]
+    c.batch.read(k, v)
+    assert torch.equal(k.double(), want[0]) and torch.equal(v.double(), want[1])
+    assert (wide[:, [0, 1 + kv * hd, 3 + kv * hd, -1]] == 5).all()
+    only = c.batch.read(v=v)[0]
+    assert only.dtype == v.dtype and torch.equal(only.double(), want[0])
+    ka, sa, va, sv = c.batch.parts()
+    assert torch.equal(ka.double() * sa.double().repeat_interleave(16, -1), want[0])
+    assert torch.equal(va.double() * sv.double().repeat_interleave(16, -1), want[1])
+    assert torch.equal(sv.view(torch.int16) >> 7, c.cache.v_scale[pg, :, off].flatten(1).to(torch.int16))
+    assert check_errors() == 0
+
+
+# --------------------------------------------------------------------------------------- attention
+
+def want_attention(c, q, window=0, gate=None, scale=0.0):
+    """(output, bound without the type's rounding) in 64 bits."""
+    import torch
+
+    scale = scale or c.hd ** -0.5
+    two = q.dtype == torch.float32
+    out, tol, at = [], [], 0
+    for s, (n, L) in enumerate(zip(c.rows, c.len)):
+        if n == 0:
+            continue
+        ks, vs = c.cached(s, "k"), c.cached(s, "v")
+        qq = q[at:at + n].double().reshape(n, c.kv, c.heads // c.kv, c.hd)
+        i, j = torch.arange(L - n, L, device=q.device)[:, None], torch.arange(L, device=q.device)
+        see = (j <= i) & (j > i - window) if window else j <= i
+        w = torch.einsum("nkgd,kjd->nkgj", qq, ks) * scale
+        size = torch.einsum("nkgd,kjd->nkgj", qq.abs(), ks.abs()) * abs(scale)
+        hide = ~see[:, None, None]
+        w = w.masked_fill(hide, float("-inf"))
+        p = torch.softmax(w, -1)
+        p = torch.where(hide, torch.zeros_like(p), p)       # a row that sees nothing: 0
+        o = torch.einsum("nkgj,kjd->nkgd", p, vs.nan_to_num())
+        W = torch.einsum("nkgj,kjd->nkgd", p, vs.nan_to_num().abs())
+        bad = (vs.isnan().any(-1) | ks.isnan().any(-1))     # [kv][j]
+        hit = (see[:, None] & bad[None]).any(-1)            # [n][kv]
+        o[hit] = float("nan")
+        S = size.masked_fill(hide, 0).nan_to_num().amax(-1, keepdim=True)
+        t = W * ((2.0 ** -21 if two else 2.0 ** -11) + 2.0 ** -20 * S + 2.0 ** -22 * (64 + L / 64) + 2.0 ** -20)
+        seen = torch.einsum("nj,kjd->nkd", see.double(), vs.nan_to_num().abs())
+        t = t + 2.0 ** -37 * p.amax(-1, keepdim=True) * seen[:, :, None]
+        out.append(o.reshape(n, c.heads, c.hd))
+        tol.append(t.reshape(n, c.heads, c.hd))
+        at += n
+    o, t = torch.cat(out), torch.cat(tol)
+    if gate is not None:
+        sg = torch.sigmoid(gate.double())[..., None]
+        o, t = o * sg, t * sg
+    return o.flatten(1), t.flatten(1)
+
+
+def check_attention(c, q, typ, window=0, gate=None, scale=0.0, out=None):
+    import torch
+
+    got = c.batch.attention(q, out, window=window, gate=gate, scale=scale)
+    assert check_errors() == 0
+    want, tol = want_attention(c, q, window, gate, scale)
+    if not want.isnan().any():
+        off = (got.double() - want).abs()
+        bound = tol + HALF[typ] * want.abs() + TINY[typ]
+        assert (off <= bound).all(), (off / bound).max()
+        return got
+    assert torch.equal(got.isnan(), want.isnan())
+    ok = ~want.isnan()
+    assert ((got.double() - want).abs()[ok] <= (tol + HALF[typ] * want.abs() + TINY[typ])[ok]).all()
+    return got
+
+
+ATTNS = [
+    # rows, tokens before, kv, hd, page, heads, window
+    ([1], [0], 1, 64, 16, 1, 0),
+    ([1], [4103], 4, 256, 64, 16, 512),
+    ([1, 1, 0, 1, 1], [0, 15, 7, 16, 2000], 2, 128, 32, 8, 0),
+    ([1] * 40, [37 * i for i in range(40)], 2, 256, 48, 8, 0),
+    ([3, 8, 1, 0, 5], [0, 100, 31, 8, 64], 2, 64, 16, 10, 0),
+    ([8, 8, 8], [500, 3, 129], 4, 128, 32, 32, 0),
+    ([70, 1, 33], [0, 300, 64], 2, 256, 64, 6, 0),
+    ([200], [0], 1, 128, 16, 5, 0),
+    ([150, 9], [77, 130], 2, 64, 32, 16, 40),
+    ([300], [1000], 1, 256, 128, 4, 17),
+    ([64, 40], [3, 0], 3, 128, 16, 3, 1),
+    ([5], [40], 1, 64, 16, 40, 0),
+]
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,old,kv,hd,page,heads,window", ATTNS)
+def test_attention(cuda, rows, old, kv, hd, page, heads, window, typ):
+    c = Case(cuda, rows, old, kv, hd, page, heads, seed=11)
+    q = c.randn(heads * hd, typ, 0.4)
+    check_attention(c, q, typ, window)
+    check_attention(c, c.randn(heads * hd, typ, 3.0), typ, window, gate=c.randn(heads, typ), scale=0.01)
+
+
+def test_long_context(cuda):
+    for typ, hd, kv, heads in (("f32", 256, 2, 8), ("bf16", 128, 1, 8), ("f16", 64, 2, 2)):
+        c = Case(cuda, [1], [70000], kv, hd, 128, heads, seed=2)
+        check_attention(c, c.randn(heads * hd, typ, 0.3), typ)
+        c = Case(cuda, [40], [20000], kv, hd, 128, heads, seed=3)
+        check_attention(c, c.randn(heads * hd, typ, 0.3), typ)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+def test_queries_of_any_size(cuda, typ):
+    """Rows of zeros, tiny and huge ones beside each other; scores past f32's range are none of an exact form's either."""
+    c = Case(cuda, [6, 40], [30, 5], 1, 128, 16, 2, seed=4)
+    q = c.randn(256, typ)
+    size = [0.0, 2.0 ** -14, 1.0, 100.0, 1e-3, 1e4]
+    for r in range(q.shape[0]):
+        q[r] *= size[r % 6]
+    check_attention(c, q, typ, scale=1e-4)
+    if typ != "f16":
+        q = c.randn(256, typ)
+        for r in range(q.shape[0]):
+            q[r] *= [1e30, 1e-30, 1e-37, 1.0][r % 4]
+        check_attention(c, q, typ, scale=1e-30)
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [[4, 2], [90, 41]])
+def test_poison_reaches_the_rows_that_see_it(cuda, rows, typ):
+    """NaN groups of keys and of values: rows before them, of other sequences and other KV heads stay."""
+    c = Case(cuda, rows, [60, 17], 2, 128, 16, 4, seed=8)
+    for s, p, h, grp, side in ((0, c.len[0] - 2, 0, 3, "v"), (0, c.len[0] - 1, 1, 7, "k"), (1, 5, 1, 0, "v"), (0, 61, 1, 2, "v")):
+        pool = c.cache.k_scale if side == "k" else c.cache.v_scale
+        pool[c.table[s][p // 16], h, p % 16, grp] = 255 if p != 5 else 248
+    q = c.randn(512, typ, 0.4)
+    for window in (0, 20):
+        got = check_attention(c, q, typ, window)
+        assert got.isnan().any() and not got.isnan().all()
+
+
+def test_scores_far_from_zero_and_one_key_that_takes_all(cuda):
+    import torch
+
+    for typ in ("f32", "f16", "bf16"):
+        c = Case(cuda, [2, 60], [300, 100], 1, 64, 16, 4, seed=9)
+        q = c.randn(256, typ)
+        for scale in (3.0, -3.0):
+            check_attention(c, q, typ, scale=scale)
+        # every key alike but one, whose value is small: the others' share counts
+        c.cache.k_pool.fill_(0x22)
+        c.cache.k_scale[c.cache.k_scale != 255] = 112
+        c.cache.k_pool[c.table[0][0], 0, 3] = 0x66
+        q = torch.full_like(q, 0.25)
+        check_attention(c, q, typ)
+
+
+def test_rows_that_see_nothing_and_rows_of_nobody(cuda):
+    """kv_len under the call's rows: the first ones sit before the sequence and see nothing. Rows behind the last sequence stay."""
+    import torch
+
+    from spk import paged4
+
+    for n in (3, 70):
+        c = Case(cuda, [n, n], [0, 20], 2, 64, 16, 4, seed=10)
+        c.kv_len[0] = n - 2
+        q = c.randn(256, "f32")
+        out = torch.full((2 * n + 5, 256), 9.0, device=cuda)
+        qq = torch.cat([q, torch.ones(5, 256, device=cuda)])
+        b = paged4.Paged4Batch(c.cache, c.row0, c.kv_len, c.tab, rows=2 * n + 5, heads=4)
+        b.attention(qq, out)
+        assert check_errors() == 0
+        assert (out[:2] == 0).all() and (out[2 * n:] == 9).all() and not (out[2:2 * n] == 0).all(1).any()
+        # appended rows and read ones of nobody
+        was = c.cache.v_pool.clone()
+        c.kv_len[0] = n
+        k = torch.randn(2 * n + 5, 128, device=cuda)
+        back = torch.full((2 * n + 5, 128), 9.0, device=cuda)
+        qo = torch.full((2 * n + 5, 256), 9.0, device=cuda)
+        b.append(k, k, q=qq, q_out=qo)
+        b.read(back, back.clone())
+        assert check_errors() == 0
+        assert (back[2 * n:] == 9).all() and (qo[2 * n:] == 9).all() and (qo[:2 * n] == qq[:2 * n]).all()
+        pg, off = c.places()
+        now = c.cache.v_pool.clone()
+        now[pg, :, off] = was[pg, :, off]
+        assert torch.equal(now, was)
+
+
+def test_offsets_past_32_bits(cuda):
+    """A pool whose codes pass 2^32 bytes, its far end in use."""
+    import torch
+
+    c = Case(cuda, [37], [200], 4, 256, 128, 16, pages=70000, seed=12)
+    assert c.cache.k_pool.numel() > 1 << 32
+    qkv = c.randn(24 * 256, "bf16")
+    q, k, v = qkv[:, :4096], qkv[:, 4096:5120], qkv[:, 5120:]
+    c.batch.append(k, v)
+    pg, off = c.places()
+    got = numbers(c.cache.v_pool[pg, :, off], c.cache.v_scale[pg, :, off]).flatten(1)
+    assert torch.equal(c.batch.read(dtype=torch.float32)[1].double(), got)
+    d = (c.cache.v_scale[pg, :, off].to(torch.int16) << 7).view(torch.float16).double().flatten(1).repeat_interleave(16, -1)
+    assert ((got - v.double()).abs() <= d).all()          # half the widest step, between codes 4 and 6
+    check_attention(c, q, "bf16")
+
+
+def test_bad_pages_are_reported_and_nothing_is_read_outside(cuda):
+    import torch
+
+    c = Case(cuda, [4, 5], [30, 40], 2, 64, 16, 4, seed=13)
+    was = [t.clone() for t in (c.cache.k_pool, c.cache.k_scale)]
+    for bad in (-1, c.cache.pages, 1 << 30):
+        c.tab[1, 0] = bad                                   # a page of the cached tokens, then of the new ones
+        c.batch.attention(c.randn(256, "f32"))
+        assert check_errors() != 0 and check_errors() == 0
+        c.tab[1] = bad
+        k = c.randn(128, "f32")
+        c.batch.append(k, k)
+        assert check_errors() != 0 and check_errors() == 0
+        c.batch.read()
+        assert check_errors() != 0 and check_errors() == 0
+    pg, off = c.places()
+    now = c.cache.k_pool.clone()
+    now[pg, :, off] = was[0][pg, :, off]
+    assert torch.equal(now, was[0])
+
+
+def test_a_run_of_them_in_a_graph_on_another_stream(cuda):
+    """Append, attend and read as one captured graph, replayed on new rows and lengths; and call by call on a given stream."""
+    import torch
+
+    c = Case(cuda, [1, 1, 5], [20, 47, 0], 2, 128, 16, 8, seed=14)
+    freq, w = freqs(cuda, 64), torch.rand(128, device=cuda) + 0.5
+    qkv = c.randn(12 * 128, "bf16")
+    q, k, v = qkv[:, :1024], qkv[:, 1024:1280], qkv[:, 1280:]
+    qo, out, rk, rv = torch.empty_like(q.contiguous()), torch.empty(7, 1024, dtype=q.dtype, device=cuda), *(torch.empty(7, 256, device=cuda) for _ in "kv")
+
+    def step(**kw):
+        c.batch.append(k, v, freq=freq, q=q, q_out=qo, q_norm=w, k_norm=w, **kw)
+        c.batch.attention(qo, out, window=30, **kw)
+        c.batch.read(rk, rv, **kw)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in range(3):
+        qkv.copy_(torch.randn(qkv.shape, generator=c.g, device=cuda))
+        for t in (qo, out, rk, rv):
+            t.zero_()
+        graph.replay()
+        got = [t.clone() for t in (qo, out, rk, rv)]
+        for t in (qo, out, rk, rv):
+            t.zero_()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        step(stream=s)
+        torch.cuda.current_stream().wait_stream(s)
+        assert all(torch.equal(a, b) for a, b in zip(got, (qo, out, rk, rv)))
+        want, tol = want_attention(c, qo, 30)
+        assert ((out.double() - want).abs() <= tol + HALF["bf16"] * want.abs()).all()
+    made = c.batch.append(k, v, q=q, stream=s), c.batch.attention(qo, stream=s), *c.batch.read(stream=s), *c.batch.parts(stream=s)
+    s.synchronize()
+    assert [t.shape[0] for t in made] == [7] * 8
+    assert check_errors() == 0
+
+
+def test_attention_repeats_itself(cuda):
+    import torch
+
+    c = Case(cuda, [1] * 9 + [50], [3000] * 9 + [900], 2, 256, 64, 8, seed=15)
+    q = c.randn(2048, "bf16")
+    first = c.batch.attention(q)
+    for _ in range(5):
+        assert torch.equal(first, c.batch.attention(q))
+
+
+def test_a_row_does_not_depend_on_the_other_rows(cuda):
+    """Sequences of a batch, attended together and one by one."""
+    import torch
+
+    from spk import paged4
+
+    c = Case(cuda, [1, 4, 2], [100, 900, 31], 2, 128, 32, 8, seed=16)
+    q = c.randn(1024, "f32", 0.4)
+    all_ = c.batch.attention(q)
+    at = 0
+    for s, n in enumerate(c.rows):
+        one = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+        b = paged4.Paged4Batch(c.cache, one, c.kv_len[s:s + 1].clone(), c.tab[s:s + 1].clone(), rows=n, heads=8)
+        got = b.attention(q[at:at + n])
+        assert (got - all_[at:at + n]).norm() <= 1e-6 * got.norm()
+        at += n
+
+
+def test_what_the_binding_refuses(cuda):
+    import torch
+
+    import spk
+    from spk import paged, paged4
+
+    c = Case(cuda, [3], [5], 2, 64, 16, 4)
+    k, v, q = c.randn(128, "f32"), c.randn(128, "f32"), c.randn(256, "f32")
+    b = c.batch
+    bad = [
+        lambda: b.append(k[:2], v), lambda: b.append(k, v.half()), lambda: b.append(k.t().contiguous().t(), v), lambda: b.append(k.cpu(), v),
+        lambda: b.append(k.double(), v.double()), lambda: b.append(k, v, q=q[:, :100]), lambda: b.append(k, v, q=q, q_out=q.half()),
+        lambda: b.append(k, v, q_out=q), lambda: b.append(k, v, q_norm=torch.ones(64, device=cuda)),
+        lambda: b.append(k, v, k_norm=torch.ones(63, device=cuda)), lambda: b.append(k, v, k_norm=torch.ones(64, device=cuda).half()),
+        lambda: b.append(k, v, k_norm=torch.ones(128, device=cuda)[::2]), lambda: b.append(k, v, k_norm=torch.ones(65, device=cuda)[1:]),
+        lambda: b.append(k, v, freq=torch.ones(4, device=cuda)), lambda: b.append(k, v, freq=torch.ones(40, device=cuda)),
+        lambda: b.append(k, v, freq=torch.ones(16, device=cuda).half()), lambda: b.append(k, v, k_norm=torch.ones(64, device=cuda), eps=-1.0),
+        lambda: b.append(k, v, k_norm=torch.ones(64, device=cuda), eps=float("nan")),
+        lambda: b.attention(q[:, :64]), lambda: b.attention(q, window=-1), lambda: b.attention(q, gate=q), lambda: b.attention(q, out=q.half()),
+        lambda: b.read(k[:, :64]), lambda: b.read(k, v.half()), lambda: b.parts([k, k, k, k]), lambda: b.read(dtype=torch.float64),
+        lambda: b.use(paged.PagedCache(4, 16, 2, 64, device=cuda)), lambda: b.use(paged4.Paged4Cache(4, 32, 2, 64, device=cuda)),
+        lambda: paged4.Paged4Batch(paged.PagedCache(4, 16, 2, 64, device=cuda), c.row0, c.kv_len, c.tab, rows=3, heads=4),
+        lambda: paged.PagedBatch(c.cache, c.row0, c.kv_len, c.tab, rows=3, heads=4),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(spk.SpkError):
+            f()
+            pytest.fail(f"call {i} was taken")
+    assert check_errors() == 0
+
+
+def test_calls_without_rows(cuda):
+    import torch
+
+    c = Case(cuda, [0, 0], [5, 0], 2, 64, 16, 4)
+    z = torch.empty(0, 128, device=cuda)
+    assert c.batch.append(z, z, q=torch.empty(0, 256, device=cuda)).shape == (0, 256)
+    assert c.batch.attention(torch.empty(0, 256, device=cuda)).shape == (0, 256)
+    assert c.batch.read()[0].shape == (0, 128) and c.batch.parts()[1].shape == (0, 8)
+    assert check_errors() == 0
