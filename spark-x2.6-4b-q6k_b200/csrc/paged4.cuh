@@ -50,5 +50,29 @@ __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&h)[4]) {
 // Whether one of four scale bytes is no number: a five-bit exponent of ones carries out of its field.
 __device__ __forceinline__ uint32_t poisoned(uint32_t w) { return (((w >> 3) & 0x1f1f1f1fu) + 0x01010101u) & 0x20202020u; }
 
+// The attention's arguments. A kernel takes the sequences whose rows per KV head (rows x group) are from `from` to `to`.
+struct AttnParams {
+    Pool pool;
+    Batch b;
+    const void *q, *gate;
+    void *out;
+    long long ldq, ldgate, ldout;
+    int heads, group, window;
+    float scale;                                        // softmax scale * log2(e)
+    long long from, to;
+    unsigned int *tickets;                              // [gridDim.x], zero at rest
+    float *part;                                        // [gridDim.x][2][part_floats]
+    int *err;
+    __device__ __forceinline__ bool takes(long long columns) const { return columns >= from && columns <= to; }
+};
+// Weights are f16 numbers 2^(s - m): a new reference m puts the row's largest at 2^12, and it moves when one passes 2^15. A
+// weight is then kept down to 2^-24, 2^-36 of the largest.
+constexpr float W_TOP = 12.0f, W_MAX = 15.0f;
+
+// Floats of one CTA's part of a group of R query rows: O, then m, then l.
+__host__ __device__ constexpr int part_floats(int R, int hd) { return R * (hd + 2); }
+constexpr int WIDE_R = 128;                             // query rows of a group of the kernel for many rows
+int attn_wide(const AttnParams &a, int type, cudaStream_t s, const char *who);   // paged4_attn_wide.cu
+
 }  // namespace paged4
 }  // namespace spk

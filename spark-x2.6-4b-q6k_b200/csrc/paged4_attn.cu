@@ -19,8 +19,11 @@
 // Work split: paged_line.cuh's line of groups of 8 query rows. A CTA's warps take a group's blocks of 16 tokens in turn, each
 // with a ring of its own that cp.async fills and a softmax of its own; they meet at the end of the group. Groups that
 // several CTAs share leave (O, m, l) in the workspace, and the last CTA to arrive adds the parts in CTA order.
+#include <limits.h>
+
 #include "paged4.cuh"
 #include "paged_line.cuh"
+#include "paged_tc.cuh"
 
 namespace spk {
 namespace paged4 {
@@ -29,43 +32,14 @@ namespace {
 using paged::Seg;
 using paged::Seq;
 using paged::Walk;
+using paged::ex2;
+using paged::from_f32;
+using paged::to_f32;
 
 constexpr int R = 8;                                    // query rows of a group
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float W_TOP = 12.0f, W_MAX = 15.0f;           // log2 of the largest weight: at a new reference, at most
 constexpr int COST = 8;                                 // a group's fixed cost in blocks
 
-struct AttnParams {
-    Pool pool;
-    Batch b;
-    const void *q, *gate;
-    void *out;
-    long long ldq, ldgate, ldout;
-    int heads, group, window;
-    float scale;                                        // softmax scale * log2(e)
-    unsigned int *tickets;                              // [gridDim.x], zero at rest
-    float *part;                                        // [gridDim.x][2][part_floats]
-    int *err;
-    __device__ __forceinline__ bool takes(long long) const { return true; }
-};
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T v) {
-    if constexpr (sizeof(T) == 4) return v;
-    else if constexpr (__is_same(T, __half)) return __half2float(v);
-    else return __bfloat162float(v);
-}
-template <typename T>
-__device__ __forceinline__ T from_f32(float v) {
-    if constexpr (sizeof(T) == 4) return v;
-    else if constexpr (__is_same(T, __half)) return __float2half_rn(v);
-    else return __float2bfloat16_rn(v);
-}
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -105,7 +79,6 @@ struct Cfg {
     static constexpr int TB = WARPS;                     // blocks of a tile of the line: one a warp
     static constexpr int WORDS = HD / 64;                // words of 8 dims in a lane's share of a token's values
 };
-__host__ __device__ constexpr int part_floats(int hd) { return R * (hd + 2); }
 
 template <typename C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnParams a) {
@@ -431,7 +404,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
         }
         __syncthreads();
         const bool whole = sg.f0 == sg.f1;
-        float *slot = a.part + ((size_t)blockIdx.x * 2 + (sg.k0 == 0 ? 1 : 0)) * part_floats(HD);
+        float *slot = a.part + ((size_t)blockIdx.x * 2 + (sg.k0 == 0 ? 1 : 0)) * part_floats(R, HD);
         const float *sums = reinterpret_cast<const float *>(smem + C::Q_BYTES);
         for (int x = tid; x < cols * (HD / 4); x += C::THREADS) {
             const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
@@ -471,9 +444,9 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
             }
             __syncthreads();
             if (last_s) {
-                const size_t step = (size_t)2 * part_floats(HD);
+                const size_t step = (size_t)2 * part_floats(R, HD);
                 const float *p0 = a.part + (size_t)sg.f0 * step;   // CTA f0: slot 1, the others: slot 0
-                auto part = [&](int p) { return p0 + p * step + (p == 0 ? part_floats(HD) : 0); };
+                auto part = [&](int p) { return p0 + p * step + (p == 0 ? part_floats(R, HD) : 0); };
                 for (int x = tid; x < cols * (HD / 4); x += C::THREADS) {
                     const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
                     float M = -INFINITY, L = 0.f;
@@ -507,6 +480,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
     }
 }
 
+constexpr long long NARROW = 64;                       // rows per KV head up to which a sequence is this kernel's
 constexpr size_t TICKETS = 4096;                        // bytes before the partials: one word per CTA
 constexpr int MAX_CTAS = 3;                             // of an SM
 
@@ -545,7 +519,8 @@ extern "C" {
 size_t spk_paged4_attn_workspace_bytes(int head_dim) {
     using namespace spk::paged4;
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
-    return TICKETS + (size_t)spk::sm_count() * MAX_CTAS * 2 * part_floats(head_dim) * sizeof(float);
+    const size_t narrow = (size_t)MAX_CTAS * part_floats(R, head_dim), wide = part_floats(WIDE_R, head_dim);
+    return TICKETS + (size_t)spk::sm_count() * 2 * (narrow > wide ? narrow : wide) * sizeof(float);
 }
 
 int spk_paged4_attn(const spk_kv4_pool *pool, const spk_kv_batch *batch, const spk_paged4_attn_args *p, void *stream) {
@@ -583,6 +558,15 @@ int spk_paged4_attn(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
     a.part = (float *)((uint8_t *)p->workspace + TICKETS);
     a.err = device_error_ptr();
     const cudaStream_t s = (cudaStream_t)stream;
+    if ((long long)batch->rows * a.group > NARROW) {
+        // some sequence may have many rows
+        a.from = NARROW + 1;
+        a.to = LLONG_MAX;
+        const int rc = attn_wide(a, p->type, s, who);
+        if (rc || batch->nseq == 1) return rc;
+    }
+    a.from = 0;
+    a.to = NARROW;
     return p->type == T_F32 ? launch<float>(a, s, who) : p->type == T_F16 ? launch<__half>(a, s, who) : launch<__nv_bfloat16>(a, s, who);
 }
 
