@@ -9,9 +9,11 @@
 // Both are decided exactly: for d the f32 quotient's neighbour is checked against 6 (d + half a step), which f32 holds; the quotient
 // x / d is corrected by its own residual, so that a tie is a tie, and moved off a border that it was only rounded to.
 //
-// What bounds append: the rows' bytes. A warp takes 256 values (256 / head_dim heads side by side), 8 consecutive ones a
-// lane, which is one 16-byte load of 16-bit rows and one word of codes; a group is two lanes, a head's norm a shuffle tree, the other half of a
-// rotated pair 8 shuffles. A CTA takes a tile of tokens, whose angles it computes once for all heads.
+// What bounds append: the rows' bytes, and beside them the shared-memory pipe (shuffles). A warp takes 256 values at a time (256 /
+// head_dim heads side by side), 8 consecutive ones a lane, which is one 16-byte load of 16-bit rows and one word of codes; a group is two lanes, a head's norm
+// a shuffle tree, the other half of a rotated pair 8 shuffles. A token's items (queries, keys, values) are one warp's where there are
+// many tokens, so that it looks its place up and computes its angles once, and several warps' where there are few; the norms' weights stay in
+// registers, the next items' rows are on their way. No warp waits for another.
 #include "paged4.cuh"
 
 namespace spk {
@@ -30,8 +32,11 @@ int check_pool(const spk_kv4_pool *p, const char *who) {
 
 namespace {
 
-constexpr int AP_WARPS = 8, AP_THREADS = AP_WARPS * 32;
-constexpr int MAX_TILE = 16;               // tokens of a tile
+constexpr int AP_WARPS = 4, AP_THREADS = AP_WARPS * 32;
+template <typename T>
+constexpr int AP_CTAS = sizeof(T) == 4 ? 4 : 5;                 // of an SM
+template <typename T>
+constexpr int AP_BATCH = 4;   // items whose loads go out together
 
 struct AppendArgs {
     Pool pool;
@@ -41,42 +46,48 @@ struct AppendArgs {
     long long ldq, ldqo, ldk, ldv;
     int vec;                               // 16-byte pieces: bit 0 q, 1 q_out, 2 k, 3 v
     const float *qw, *kw, *freq;
-    int heads, pdim, interleaved, tile;    // q heads (0: none), rotated dims, tokens of a tile
+    int heads, pdim, interleaved;          // q heads (0: none), rotated dims
     float eps;
     int *err;
 };
 
+// 8 values of a row as they lie in memory
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, bool vec, float (&x)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        if (vec) {
-            const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = p[i];
-        }
-    } else {
-        uint32_t w[4];
+struct Raw8 {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void load(const T *p, bool vec) {
         if (vec) {
             const uint4 a = *reinterpret_cast<const uint4 *>(p);
             w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+            if constexpr (sizeof(T) == 4) {
+                const uint4 b = *(reinterpret_cast<const uint4 *>(p) + 1);
+                w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                w[i] = reinterpret_cast<const uint16_t *>(p)[2 * i] | (uint32_t)reinterpret_cast<const uint16_t *>(p)[2 * i + 1] << 16;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (__is_same(T, __half)) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                x[2 * i] = f.x, x[2 * i + 1] = f.y;
-            } else {
-                x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            for (int i = 0; i < (int)(2 * sizeof(T)); i++) {
+                if constexpr (sizeof(T) == 4) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+                else w[i] = reinterpret_cast<const uint16_t *>(p)[2 * i] | (uint32_t)reinterpret_cast<const uint16_t *>(p)[2 * i + 1] << 16;
             }
         }
     }
-}
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int i = 0; i < (int)(2 * sizeof(T)); i++) w[i] = 0;
+    }
+    __device__ __forceinline__ void f32(paged::f32x2 (&x)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (sizeof(T) == 4) x[i] = paged::pack2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+            else if constexpr (__is_same(T, __half)) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                x[i] = paged::pack2(f.x, f.y);
+            } else {
+                x[i] = paged::pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+            }
+        }
+    }
+};
 template <typename T>
 __device__ __forceinline__ uint32_t two(float a, float b) {   // 16-bit types: a pair, a in the low half
     if constexpr (__is_same(T, __half)) {
@@ -88,7 +99,13 @@ __device__ __forceinline__ uint32_t two(float a, float b) {   // 16-bit types: a
     }
 }
 template <typename T>
-__device__ __forceinline__ void store8(T *p, bool vec, const float (&x)[8]) {
+__device__ __forceinline__ void store8(T *p, bool vec, const paged::f32x2 (&v)[4]) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = paged::unpack2(v[i]);
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
     if constexpr (sizeof(T) == 4) {
         if (vec) {
             reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -111,45 +128,58 @@ __device__ __forceinline__ void store8(T *p, bool vec, const float (&x)[8]) {
 
 // The scale of a group whose largest magnitude is amax: its byte, and d.
 __device__ __forceinline__ uint32_t scale_of(float amax, float &d) {
-    if (!(amax < INFINITY)) {
-        d = 0.f;
-        return 0xffu;
-    }
-    const float t = fminf(fmaxf(__fdiv_rn(amax, 6.0f), SCALE_MIN), SCALE_MAX);
-    uint32_t b = __float_as_uint(t) >> 20;                        // the 4 leading bits
-    const float mid = __uint_as_float((b << 20) | 0x80000u);      // and the middle to the next
-    const float six = 6.0f * mid;                                 // 8 bits: exact
+    const float t = fminf(fmaxf(amax * (1.0f / 6.0f), SCALE_MIN), SCALE_MAX);
+    uint32_t b = __float_as_uint(t) >> 20;                        // the 4 leading bits, or of the number a unit beside
+    const float six = 6.0f * __uint_as_float((b << 20) | 0x80000u);   // six times the middle to the next: 8 bits, exact
     if (t < SCALE_MAX && (amax > six || (amax == six && (b & 1)))) b++;
-    d = __uint_as_float(b << 20);
-    return b - (112u << 3);                                       // f16's exponent bias
+    const bool number = amax < INFINITY;
+    d = number ? __uint_as_float(b << 20) : 0.f;
+    return number ? b - (112u << 3) : 0xffu;                      // f16's exponent bias
 }
 
-// x / d with the code decided: the corrected quotient, off a border that it does not truly meet. `wide`: x may have more bits
-// than a border times d (f32 values, or ones computed here); 16-bit values are either on it or 2^-12 away.
-__device__ __forceinline__ float ratio(float x, float d, float inv, bool wide) {
-    float t = __fmul_rn(x, inv);
-    t = __fmaf_rn(__fmaf_rn(-t, d, x), inv, t);
-    if (wide) {
-        const float rest = __fmaf_rn(-t, d, x);                   // exact: the true quotient lies on its side of t
-        const uint32_t u = __float_as_uint(t);
-        if (rest != 0.f && !(u & 1)) t = __uint_as_float((rest > 0.f) == (t > 0.f) ? u + 1 : u - 1);   // borders are even
+// The codes of 8 values under d (0: none). A corrected quotient is the nearest f32 to x / d: a tie is a tie. `wide`: x may have more bits
+// than a border times d (f32 values, or ones computed here; 16-bit values are on a border or 2^-12 away), so a quotient that was rounded to
+// a border (all of them have 21 zeros at the end) is moved off it, to the side that its residual, which is exact, says.
+template <bool WIDE>
+__device__ __forceinline__ uint32_t codes8(const paged::f32x2 (&x)[4], float d) {
+    using namespace paged;
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d));
+    const f32x2 i2 = pack2(inv, inv), nd = pack2(-d, -d);
+    float t[8];
+    uint32_t low = ~0u;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        const f32x2 q = mul2(x[e / 2], i2);
+        const float2 r = unpack2(fma2(fma2(q, nd, x[e / 2]), i2, q));
+        t[e] = r.x, t[e + 1] = r.y;
+        if (WIDE) low = min(low, min(__float_as_uint(r.x) & 0x1fffffu, __float_as_uint(r.y) & 0x1fffffu));
     }
-    return t;
-}
-__device__ __forceinline__ uint32_t codes2(float a, float b) {    // a in the low half
+    if (WIDE && low == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float2 xe = unpack2(x[e / 2]);
+            const float rest = __fmaf_rn(-t[e], d, e & 1 ? xe.y : xe.x);
+            const uint32_t u = __float_as_uint(t[e]);
+            if (rest != 0.f && t[e] != 0.f && !(u & 0x1fffffu)) t[e] = __uint_as_float((rest > 0.f) == (t[e] > 0.f) ? u + 1 : u - 1);
+        }
+    }
     uint32_t r;
-    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tmov.b32 %0, {t, 0, 0, 0};\n\t}" : "=r"(r) : "f"(b), "f"(a));
-    return r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r)
+        : "f"(t[0]), "f"(t[1]), "f"(t[2]), "f"(t[3]), "f"(t[4]), "f"(t[5]), "f"(t[6]), "f"(t[7]));
+    return d > 0.f ? r : 0u;
 }
 
-// max of |a|, |b| that keeps a NaN
-__device__ __forceinline__ float max_abs(float a, float b) {
+// max of m, |a|, |b| that keeps a NaN
+__device__ __forceinline__ float max_abs(float m, float a, float b) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
     return r;
 }
 
-// Where the rows of a call lie. Row t: the sequence whose rows hold it, or -1.
+// Where the rows of a call lie: the sequences in shared memory.
 struct Rows {
     int row0[MAX_SEQ + 1], len[MAX_SEQ];
     __device__ __forceinline__ void load(const Batch &b, int tid, int threads) {
@@ -157,9 +187,10 @@ struct Rows {
             row0[s] = __ldg(b.row0 + s);
             if (s < b.nseq) len[s] = __ldg(b.kv_len + s);
         }
+        __syncthreads();
     }
-    // the row's place in the pool for KV head 0 and its position; false: it belongs to nobody, or the batch does not fit
-    __device__ __forceinline__ bool find(const Pool &p, const Batch &b, int t, size_t &at, int &pos, int *err) const {
+    // row t's place in the pool for KV head 0, and its position; -1: it belongs to nobody, or the batch does not fit
+    __device__ __forceinline__ long long find(const Pool &p, const Batch &b, int t, int &pos, int *err) const {
         int lo = 0, hi = b.nseq;          // the last sequence that starts at or before t
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -167,140 +198,185 @@ struct Rows {
             else hi = mid;
         }
         const int r0 = row0[lo], r1 = row0[lo + 1];
-        if (t < r0 || t >= r1) return false;
+        if (t >= b.rows || t < r0 || t >= r1) return -1;
         pos = len[lo] - (r1 - t);
         int page = -1;
         if (r0 >= 0 && r1 <= b.rows && len[lo] >= r1 - r0 && pos / p.page_tokens < b.max_pages)
             page = __ldg(b.table + (size_t)lo * b.max_pages + pos / p.page_tokens);
         if (page < 0 || page >= p.pages) {
             if (err) atomicExch(err, DEV_BAD_INDEX);
-            return false;
+            return -1;
         }
-        at = row_index(p, page, 0, pos % p.page_tokens);
-        return true;
+        return (long long)row_index(p, page, 0, pos % p.page_tokens);
     }
 };
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) {
-    constexpr int LPR = HD / 8, GH = 256 / HD;                     // lanes of a head, heads of a warp
+// The work of a call: a token's `per` items of 256 values belong to a team of `team` warps, which takes every `teams`-th token.
+struct Share {
+    int first, x0, team, teams;
+    __device__ __forceinline__ Share(int rows, int per) {
+        const long long warps = (long long)gridDim.x * (blockDim.x / 32), w = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+        team = (int)max(1ll, min((long long)per, warps / rows));
+        teams = (int)(warps / team);
+        first = w / team < teams ? (int)(w / team) : rows;
+        x0 = (int)(w % team);
+    }
+};
+// CTAs of a call
+int ctas_of(long long rows, int per, int warps, int most) {
+    return (int)max(1ll, min((long long)most, (rows * per + warps - 1) / warps));
+}
+
+__device__ __noinline__ float2 turn_of(int pos, float freq) {
+    float2 t;
+    paged::angle(pos, freq, t.x, t.y);
+    return t;
+}
+
+template <typename T, int HD, bool VEC>
+__global__ void __launch_bounds__(AP_THREADS, AP_CTAS<T>) append_kernel(const AppendArgs a) {
+    using namespace paged;
+    constexpr int LPR = HD / 8, GH = 256 / HD, BATCH = AP_BATCH<T>;   // lanes of a head, heads of a warp
     __shared__ Rows rows;
-    __shared__ size_t at_s[MAX_TILE];                              // a token's place, position (-1: none)
-    __shared__ int pos_s[MAX_TILE];
-    extern __shared__ __align__(16) float turn[];                  // [tile][pdim / 2] cosines, then sines
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane / LPR, u = lane % LPR;
-    const int all = a.heads + 2 * a.pool.kv_heads, per = (all + GH - 1) / GH, half = a.pdim / 2, tile = a.tile;
-    float *cs = turn, *sn = turn + tile * half;
+    const int lane = threadIdx.x & 31, sub = lane / LPR, u = lane % LPR;
+    const int kv = a.pool.kv_heads, pq = (a.heads + GH - 1) / GH, pk = (kv + GH - 1) / GH, per = pq + 2 * pk;   // a token's items: queries, keys, values
+    const int half = a.pdim / 2;
+    const bool swap = a.interleaved, turned = 8 * u < a.pdim;
+    // the lane that has the other halves of this one's pairs; the first of the 4 angles that this one works out
+    const bool low = 8 * u < half;
+    const int other = swap || !turned ? lane : low ? lane + half / 8 : lane - half / 8, angle0 = swap ? 4 * u : low ? 8 * u : 8 * u - half + 4;
     pdl_trigger();
     pdl_wait();
-    rows.load(a.b, tid, AP_THREADS);
-    __syncthreads();
-    const int tiles = (a.b.rows + tile - 1) / tile;
-    for (int tl = blockIdx.x; tl < tiles; tl += gridDim.x) {
-        const int t0 = tl * tile, nt = min(tile, a.b.rows - t0);
-        if (tid < nt) {
-            size_t at = 0;
-            int pos = 0;
-            pos_s[tid] = rows.find(a.pool, a.b, t0 + tid, at, pos, a.err) ? pos : -1;
-            at_s[tid] = at;
+    rows.load(a.b, threadIdx.x, AP_THREADS);
+    const Share sh(a.b.rows, per);
+
+    auto weights = [&](const float *w, f32x2 (&to)[4]) {
+        if (!w) return;
+        const float4 w0 = __ldg(reinterpret_cast<const float4 *>(w + 8 * u)), w1 = __ldg(reinterpret_cast<const float4 *>(w + 8 * u) + 1);
+        to[0] = pack2(w0.x, w0.y), to[1] = pack2(w0.z, w0.w), to[2] = pack2(w1.x, w1.y), to[3] = pack2(w1.z, w1.w);
+    };
+    f32x2 qw[4], kw[4];
+    weights(a.qw, qw);
+    weights(a.kw, kw);
+    auto norm = [&](f32x2 (&x)[4], const f32x2 (&w)[4]) {
+        f32x2 s2 = mul2(x[0], x[0]);
+#pragma unroll
+        for (int e = 1; e < 4; e++) s2 = fma2(x[e], x[e], s2);
+        const float2 ab = unpack2(s2);
+        float ss = ab.x + ab.y;
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float rs = rsqrtf(fmaf(ss, 1.0f / HD, a.eps));
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = mul2(mul2(x[e], pack2(rs, rs)), w[e]);
+    };
+    // the token's factors of a dim and of its pair's other dim; 1 and 0 where nothing is rotated
+    f32x2 cs[4], sn[4];
+    auto angles = [&](int pos) {
+        float c[4], s[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float2 t = turned ? turn_of(pos, __ldg(a.freq + angle0 + e)) : make_float2(1.f, 0.f);
+            c[e] = t.x, s[e] = t.y;
         }
-        __syncthreads();
-        for (int i = tid; i < nt * half; i += AP_THREADS) {
-            const int r = i / half, j = i - r * half;
-            paged::angle(pos_s[r], __ldg(a.freq + j), cs[i], sn[i]);
-        }
-        if (half) __syncthreads();
-        for (int it = warp; it < nt * per; it += AP_WARPS) {
-            const int r = it / per, head = (it - r * per) * GH + sub;
-            const bool live = head < all && pos_s[r] >= 0;
-            const int kind = head < a.heads ? 0 : head < a.heads + a.pool.kv_heads ? 1 : 2;   // q, k, v
-            const int h = kind == 0 ? head : kind == 1 ? head - a.heads : head - a.heads - a.pool.kv_heads;
-            const T *src = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
-                           (long long)(t0 + r) * (kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv) + (long long)h * HD + 8 * u;
-            float x[8];
-            if (live) load8<T>(src, a.vec >> (kind == 0 ? 0 : kind + 1) & 1, x);
-            else {
+        if (swap) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = 0.f;
-            }
-            const float *w = kind == 0 ? a.qw : kind == 1 ? a.kw : nullptr;
-            if (__any_sync(0xffffffffu, w != nullptr)) {
-                float ss = 0.f;
+            for (int e = 0; e < 4; e++) cs[e] = pack2(c[e], c[e]), sn[e] = pack2(-s[e], s[e]);
+        } else {   // low lanes worked out the first 4 of their 8 angles, the others the last 4
 #pragma unroll
-                for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-                for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                if (w) {
-                    const float rs = __frsqrt_rn(fmaf(ss, 1.0f / HD, a.eps));
-                    const float4 w0 = __ldg(reinterpret_cast<const float4 *>(w + 8 * u)), w1 = __ldg(reinterpret_cast<const float4 *>(w + 8 * u) + 1);
-                    const float ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = x[i] * rs * ww[i];
-                }
-            }
-            if (half) {
-                const bool turned = kind < 2 && 8 * u < a.pdim;
-                const float *c = cs + r * half, *s = sn + r * half;
-                if (a.interleaved) {
-                    if (turned) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float cc = c[4 * u + i], ss = s[4 * u + i], p = x[2 * i], q = x[2 * i + 1];
-                            x[2 * i] = p * cc - q * ss;
-                            x[2 * i + 1] = q * cc + p * ss;
-                        }
-                    }
-                } else {
-                    const bool low = 8 * u < half;
-                    const int other = lane + (low ? half / 8 : -(half / 8)), j = low ? 8 * u : 8 * u - half;
-                    float y[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], turned ? other : lane);
-                    if (turned) {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float cc = c[j + i], ss = s[j + i];
-                            x[i] = low ? x[i] * cc - y[i] * ss : x[i] * cc + y[i] * ss;
-                        }
-                    }
-                }
-            }
-            if (live && kind == 0)
-                store8<T>((T *)a.q_out + (long long)(t0 + r) * a.ldqo + (long long)h * HD + 8 * u, a.vec >> 1 & 1, x);
-            if (__any_sync(0xffffffffu, kind > 0)) {
-                float mx = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; i++) mx = max_abs(mx, x[i]);
-                mx = max_abs(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                float d;
-                const uint32_t b = scale_of(mx, d);
-                const float inv = d > 0.f ? __fdiv_rn(1.0f, d) : 0.f;
-                const bool wide = sizeof(T) == 4 || (kind == 1 && (a.kw || half));
-                uint32_t code = 0;
-#pragma unroll
-                for (int i = 0; i < 8; i += 2)
-                    code |= codes2(ratio(x[i], d, inv, wide), ratio(x[i + 1], d, inv, wide)) << (4 * i);
-                if (!(d > 0.f)) code = 0;
-                if (live && kind > 0) {
-                    const size_t at = at_s[r] + (size_t)h * a.pool.page_tokens;
-                    reinterpret_cast<uint32_t *>((kind == 1 ? a.pool.k : a.pool.v) + at * (HD / 2))[u] = code;
-                    if (!(u & 1)) ((kind == 1 ? a.pool.ks : a.pool.vs) + at * (HD / GROUP))[u >> 1] = (uint8_t)b;
-                }
+            for (int e = 0; e < 4; e += 2) {
+                const float oc0 = __shfl_sync(0xffffffffu, c[e], other), oc1 = __shfl_sync(0xffffffffu, c[e + 1], other);
+                const float os0 = __shfl_sync(0xffffffffu, s[e], other), os1 = __shfl_sync(0xffffffffu, s[e + 1], other);
+                cs[e / 2] = low ? pack2(c[e], c[e + 1]) : pack2(oc0, oc1);
+                cs[2 + e / 2] = low ? pack2(oc0, oc1) : pack2(c[e], c[e + 1]);
+                sn[e / 2] = low ? pack2(-s[e], -s[e + 1]) : pack2(os0, os1);
+                sn[2 + e / 2] = low ? pack2(-os0, -os1) : pack2(s[e], s[e + 1]);
             }
         }
-        __syncthreads();   // the tile's places and angles are free
+    };
+    auto rotate = [&](f32x2 (&x)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float2 v = unpack2(x[e]);
+            const f32x2 y = swap ? pack2(v.y, v.x) : pack2(__shfl_sync(0xffffffffu, v.x, other), __shfl_sync(0xffffffffu, v.y, other));
+            x[e] = fma2(y, sn[e], mul2(x[e], cs[e]));
+        }
+    };
+    // A warp has every team-th of a token's items, queries, keys and values counted on. `items` of a row, `before` them
+    // those of the others: heads of 256 values side by side, a batch's loads before its work.
+    auto first_of = [&](int before) {
+        const int x = (sh.x0 - before) % sh.team;
+        return x < 0 ? x + sh.team : x;
+    };
+    auto row = [&](const T *src, int before, int items, int heads, auto &&work) {
+        for (int x = first_of(before); x < items; x += BATCH * sh.team) {
+            Raw8<T> raw[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) {
+                const int xi = x + i * sh.team;
+                if (xi < items && (GH == 1 || xi * GH + sub < heads)) raw[i].load(src + xi * 256, VEC);
+                else raw[i].none();
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) {
+                const int xi = x + i * sh.team;
+                if (xi >= items) break;
+                f32x2 v[4];
+                raw[i].f32(v);
+                work(v, xi * GH + sub, GH == 1 || xi * GH + sub < heads);
+            }
+        }
+    };
+
+    long long places = -1;              // lane i: place and position of the team's i-th token from `count` & ~31 on
+    int poses = 0, count = 0;
+    for (int t = sh.first; t < a.b.rows; t += sh.teams, count++) {
+        if (!(count & 31)) {
+            const long long tt = (long long)t + (long long)lane * sh.teams;
+            places = tt < a.b.rows ? rows.find(a.pool, a.b, (int)tt, poses, a.err) : -1;
+        }
+        const long long at = __shfl_sync(0xffffffffu, places, count & 31);
+        const int pos = __shfl_sync(0xffffffffu, poses, count & 31);
+        if (at < 0) continue;
+        if (half) angles(pos);
+        T *qo = (T *)a.q_out + (long long)t * a.ldqo + 8 * u;
+        row((const T *)a.q + (long long)t * a.ldq + lane * 8, 0, pq, a.heads, [&](f32x2 (&v)[4], int h, bool live) {
+            if (a.qw) norm(v, qw);
+            if (half) rotate(v);
+            if (live) store8<T>(qo + h * HD, VEC, v);
+        });
+        auto keep = [&](uint8_t *codes, uint8_t *scales, const f32x2 (&v)[4], int h, bool live, bool wide) {
+            float mx = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float2 f = unpack2(v[e]);
+                mx = max_abs(mx, f.x, f.y);
+            }
+            mx = max_abs(mx, __shfl_xor_sync(0xffffffffu, mx, 1), 0.f);
+            float d;
+            const uint32_t b = scale_of(mx, d), code = wide ? codes8<true>(v, d) : codes8<false>(v, d);
+            if (live) {
+                const size_t to = (size_t)at + (size_t)h * a.pool.page_tokens;
+                reinterpret_cast<uint32_t *>(codes + to * (HD / 2))[u] = code;
+                if (!(u & 1)) (scales + to * (HD / GROUP))[u >> 1] = (uint8_t)b;
+            }
+        };
+        row((const T *)a.k + (long long)t * a.ldk + lane * 8, pq, pk, kv, [&](f32x2 (&v)[4], int h, bool live) {
+            if (a.kw) norm(v, kw);
+            if (half) rotate(v);
+            keep(a.pool.k, a.pool.ks, v, h, live, sizeof(T) == 4 || a.kw || half);
+        });
+        row((const T *)a.v + (long long)t * a.ldv + lane * 8, pq + pk, pk, kv,
+            [&](f32x2 (&v)[4], int h, bool live) { keep(a.pool.v, a.pool.vs, v, h, live, sizeof(T) == 4); });
     }
 }
 
 template <typename T>
 cudaError_t launch(const AppendArgs &a, cudaStream_t s) {
-    const int hd = a.pool.hd, per = (a.heads + 2 * a.pool.kv_heads + 256 / hd - 1) / (256 / hd);
-    AppendArgs p = a;
-    p.tile = min(MAX_TILE, max(1, 2 * AP_WARPS / per));
-    const int tiles = (a.b.rows + p.tile - 1) / p.tile;
-    const size_t smem = (size_t)p.tile * a.pdim * sizeof(float);
-    auto k = hd == 256 ? append_kernel<T, 256> : hd == 128 ? append_kernel<T, 128> : append_kernel<T, 64>;
-    return launch_pdl(k, dim3(min(tiles, 4 * sm_count())), dim3(AP_THREADS), smem, s, p);
+    const int hd = a.pool.hd, gh = 256 / hd, per = (a.heads + gh - 1) / gh + 2 * ((a.pool.kv_heads + gh - 1) / gh);
+    auto k = a.vec == 15 ? (hd == 256 ? append_kernel<T, 256, true> : hd == 128 ? append_kernel<T, 128, true> : append_kernel<T, 64, true>)
+                         : (hd == 256 ? append_kernel<T, 256, false> : hd == 128 ? append_kernel<T, 128, false> : append_kernel<T, 64, false>);
+    return launch_pdl(k, dim3(ctas_of(a.b.rows, per, AP_WARPS, AP_CTAS<T> * sm_count())), dim3(AP_THREADS), 0, s, a);
 }
 
 // ------------------------------------------------------------------ cached rows back
@@ -314,8 +390,16 @@ struct ReadArgs {
     int *err;
 };
 struct Codes {};                           // e4m3 codes and f16 scales, apart
+template <typename T>
+struct Out {
+    using type = T;
+};
+template <>
+struct Out<Codes> {
+    using type = uint8_t;
+};
 
-constexpr int RD_THREADS = 256;
+constexpr int RD_THREADS = 128, RD_CTAS = 12;
 
 // e4m3 bytes of four codes
 __device__ __forceinline__ uint32_t code_bytes(uint32_t four) {
@@ -324,57 +408,94 @@ __device__ __forceinline__ uint32_t code_bytes(uint32_t four) {
     return mag | sign;
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(RD_THREADS) read_kernel(const ReadArgs a) {
-    constexpr int WORDS = HD / 8;                                  // of 8 codes
+template <typename T, int HD, bool VEC>
+__global__ void __launch_bounds__(RD_THREADS, RD_CTAS) read_kernel(const ReadArgs a) {
+    constexpr int LPR = HD / 8, GH = 256 / HD, BATCH = 4;          // lanes of a head, heads of a warp, items whose loads go out together
+    constexpr bool APART = __is_same(T, Codes);
+    using O = typename Out<T>::type;
     __shared__ Rows rows;
+    const int lane = threadIdx.x & 31, sub = lane / LPR, u = lane % LPR;
+    const int kv = a.pool.kv_heads, parts = (kv + GH - 1) / GH, per = 2 * parts;   // a token's items: keys, values
+    const size_t step = (size_t)GH * a.pool.page_tokens, mine = (size_t)sub * a.pool.page_tokens;   // rows of the pool from item to item
     pdl_trigger();
     pdl_wait();
     rows.load(a.b, threadIdx.x, RD_THREADS);
-    __syncthreads();
-    const int side = blockIdx.y, hw = a.pool.kv_heads * WORDS;
-    const uint8_t *pool = side ? a.pool.v : a.pool.k, *scales = side ? a.pool.vs : a.pool.ks;
-    if (!a.out[side]) return;
-    for (long long i = (long long)blockIdx.x * RD_THREADS + threadIdx.x; i < (long long)a.b.rows * hw; i += (long long)gridDim.x * RD_THREADS) {
-        const int t = (int)(i / hw), x = (int)(i - (long long)t * hw), h = x / WORDS, u = x % WORDS;
-        size_t at;
-        int pos;
-        if (!rows.find(a.pool, a.b, t, at, pos, a.err)) continue;
-        at += (size_t)h * a.pool.page_tokens;
-        const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(pool + at * (HD / 2)) + u);
-        const uint32_t sb = (uint32_t)__ldg(scales + at * (HD / GROUP) + (u >> 1)) << 7;
-        const long long to = (long long)t * a.ld[side] + (long long)h * HD + 8 * u;
-        if constexpr (__is_same(T, Codes)) {
-            uint8_t *p = (uint8_t *)a.out[side] + to;
-            const uint32_t lo = code_bytes(w & 0xffffu), hi = code_bytes(w >> 16);
-            if (a.vec >> side & 1) *reinterpret_cast<uint2 *>(p) = make_uint2(lo, hi);
-            else {
+    const Share sh(a.b.rows, per);
+    long long places = -1;              // lane i: place of the team's i-th token from `count` & ~31 on
+    int count = 0;
+    for (int t = sh.first; t < a.b.rows; t += sh.teams, count++) {
+        if (!(count & 31)) {
+            const long long tt = (long long)t + (long long)lane * sh.teams;
+            int pos;
+            places = tt < a.b.rows ? rows.find(a.pool, a.b, (int)tt, pos, a.err) : -1;
+        }
+        const long long at = __shfl_sync(0xffffffffu, places, count & 31);
+        if (at < 0) continue;
+        const size_t row = (size_t)at + mine;
+        const uint8_t *kc = a.pool.k + row * (HD / 2) + 4 * u, *vc = a.pool.v + row * (HD / 2) + 4 * u;
+        const uint8_t *ks = a.pool.ks + row * (HD / GROUP) + (u >> 1), *vs = a.pool.vs + row * (HD / GROUP) + (u >> 1);
+        O *ko = (O *)a.out[0] + (long long)t * a.ld[0] + lane * 8, *vo = (O *)a.out[1] + (long long)t * a.ld[1] + lane * 8;
+        for (int x = sh.x0; x < per; x += BATCH * sh.team) {
+            uint32_t w[BATCH], sb[BATCH];
 #pragma unroll
-                for (int e = 0; e < 8; e++) p[e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+            for (int i = 0; i < BATCH; i++) {
+                const int xi = x + i * sh.team, side = xi >= parts, it = side ? xi - parts : xi;
+                w[i] = sb[i] = 0;
+                if (xi < per && (GH == 1 || it * GH + sub < kv) && a.out[side]) {
+                    w[i] = __ldg(reinterpret_cast<const uint32_t *>((side ? vc : kc) + it * step * (HD / 2)));
+                    sb[i] = __ldg((side ? vs : ks) + it * step * (HD / GROUP));
+                }
             }
-            if (!(u & 1)) ((uint16_t *)a.sc[side])[(long long)t * a.lds[side] + h * (HD / GROUP) + (u >> 1)] = (uint16_t)sb;
-        } else {
-            uint32_t c[4];
-            codes_f16(w, c);
-            const uint32_t ss = sb | sb << 16;
-            float v[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float2 f = __half22float2(__hmul2(*reinterpret_cast<const __half2 *>(&c[e]), *reinterpret_cast<const __half2 *>(&ss)));
-                v[2 * e] = f.x, v[2 * e + 1] = f.y;
+            for (int i = 0; i < BATCH; i++) {
+                const int xi = x + i * sh.team, side = xi >= parts, it = side ? xi - parts : xi;
+                if (xi >= per) break;
+                if ((GH > 1 && it * GH + sub >= kv) || !a.out[side]) continue;
+                O *to = (side ? vo : ko) + it * 256;
+                if constexpr (APART) {
+                    const uint32_t lo = code_bytes(w[i] & 0xffffu), hi = code_bytes(w[i] >> 16);
+                    if (VEC) *reinterpret_cast<uint2 *>(to) = make_uint2(lo, hi);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) to[e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+                    }
+                    if (!(u & 1)) ((uint16_t *)a.sc[side])[(long long)t * a.lds[side] + (it * GH + sub) * (HD / GROUP) + (u >> 1)] = (uint16_t)(sb[i] << 7);
+                } else {
+                    uint32_t c[4];
+                    codes_f16(w[i], c);
+                    const uint32_t ss = sb[i] * 0x00800080u;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const __half2 h = __hmul2(*reinterpret_cast<const __half2 *>(&c[e]), *reinterpret_cast<const __half2 *>(&ss));
+                        c[e] = *reinterpret_cast<const uint32_t *>(&h);
+                    }
+                    if constexpr (__is_same(T, __half)) {
+                        if (VEC) *reinterpret_cast<uint4 *>(to) = make_uint4(c[0], c[1], c[2], c[3]);
+                        else {
+#pragma unroll
+                            for (int e = 0; e < 8; e++) reinterpret_cast<uint16_t *>(to)[e] = (uint16_t)(c[e >> 1] >> (16 * (e & 1)));
+                        }
+                    } else {
+                        paged::f32x2 v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&c[e]));
+                            v[e] = paged::pack2(f.x, f.y);
+                        }
+                        store8<T>(to, VEC, v);
+                    }
+                }
             }
-            store8<T>((T *)a.out[side] + to, a.vec >> side & 1, v);
         }
     }
 }
 
 template <typename T>
 cudaError_t launch_read(const ReadArgs &a, cudaStream_t s) {
-    const int hd = a.pool.hd;
-    const long long items = (long long)a.b.rows * a.pool.kv_heads * (hd / 8);
-    auto k = hd == 256 ? read_kernel<T, 256> : hd == 128 ? read_kernel<T, 128> : read_kernel<T, 64>;
-    const long long ctas = (items + RD_THREADS - 1) / RD_THREADS;
-    return launch_pdl(k, dim3((unsigned)min(ctas, 8ll * sm_count()), 2), dim3(RD_THREADS), 0, s, a);
+    const int hd = a.pool.hd, per = 2 * ((a.pool.kv_heads + 256 / hd - 1) / (256 / hd));
+    auto k = a.vec == 3 ? (hd == 256 ? read_kernel<T, 256, true> : hd == 128 ? read_kernel<T, 128, true> : read_kernel<T, 64, true>)
+                        : (hd == 256 ? read_kernel<T, 256, false> : hd == 128 ? read_kernel<T, 128, false> : read_kernel<T, 64, false>);
+    return launch_pdl(k, dim3(ctas_of(a.b.rows, per, RD_THREADS / 32, RD_CTAS * sm_count())), dim3(RD_THREADS), 0, s, a);
 }
 
 }  // namespace
@@ -405,7 +526,7 @@ int spk_paged4_append(const spk_kv4_pool *pool, const spk_kv_batch *batch, const
     auto whole = [&](const void *at, long long ld) { return (uintptr_t)at % 16 == 0 && ld * size % 16 == 0 ? 1 : 0; };
     AppendArgs a{pool_of(pool), paged::batch_of(batch), p->q, p->k, p->v, p->q_out, p->ldq, p->ldq_out, p->ldk, p->ldv,
                  whole(p->q, p->ldq) | whole(p->q_out, p->ldq_out) << 1 | whole(p->k, p->ldk) << 2 | whole(p->v, p->ldv) << 3,
-                 p->q_norm, p->k_norm, p->freq, p->heads, p->freq ? p->pdim : 0, p->interleaved ? 1 : 0, 1, p->eps, device_error_ptr()};
+                 p->q_norm, p->k_norm, p->freq, p->heads, p->freq ? p->pdim : 0, p->interleaved ? 1 : 0, p->eps, device_error_ptr()};
     const cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = p->type == T_F32 ? launch<float>(a, s) : p->type == T_F16 ? launch<__half>(a, s) : launch<__nv_bfloat16>(a, s);
     return e == cudaSuccess ? 0 : cuda_fail(who, e);
@@ -425,7 +546,10 @@ int spk_paged4_read(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
     const int size = parts ? 1 : p->type == T_F32 ? 4 : 2;
     ReadArgs a{pool_of(pool), paged::batch_of(batch), {p->k, p->v}, {p->k_scale, p->v_scale}, {p->ldk, p->ldv}, {p->ldk_scale, p->ldv_scale}, 0, device_error_ptr()};
     for (int i = 0; i < 2; i++) {
-        if (!a.out[i]) continue;
+        if (!a.out[i]) {
+            a.vec |= 1 << i;
+            continue;
+        }
         if (parts && (!a.sc[i] || (uintptr_t)a.sc[i] % 2)) return set_error("%s: scales are null or unaligned", who);
         if (batch->rows > 1 && (a.ld[i] < width || (parts && a.lds[i] < swidth)))
             return set_error("%s: row strides %lld, %lld under %lld, %lld", who, a.ld[i], a.lds[i], width, swidth);

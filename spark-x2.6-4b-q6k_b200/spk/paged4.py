@@ -100,41 +100,50 @@ class Paged4Batch(PagedBatch):
         self._append, self._attn, self._read = L.spk_paged4_append, L.spk_paged4_attn, L.spk_paged4_read
         self._ap, self._rd = _Append4(), _Read4()
         self._ap_p, self._rd_p = C.addressof(self._ap), C.addressof(self._rd)
+        wide, self._f32 = self.cache.kv_heads * self.cache.head_dim, torch.float32
+        self._parts = [(w, t, side + name) for side in "kv" for w, t, name in ((wide, torch.float8_e4m3fn, ""), (wide // GROUP, torch.float16, "_scale"))]
 
     def append(self, k, v, freq=None, q=None, q_out=None, q_norm=None, k_norm=None, eps: float = 1e-6, interleaved: bool = False,
                stream=None):
         """Rows k, v [rows][kv_heads * head_dim] into the pages, and queries q [rows][heads * head_dim] to q_out (made when not
         given, returned; q itself for in place). q_norm, k_norm: f32 [head_dim], the weights of an RMS norm of each head.
         freq: the rotation of the first 2 * len(freq) dims, pairs half of that apart or, `interleaved`, side by side."""
-        import torch
-
         c, a = self.cache, self._ap
         width = c.kv_heads * c.head_dim
         a.ldk, a.ldv = _rows(k, self.rows, width, "k", on=c.device), _rows(v, self.rows, width, "v", k)
         a.k, a.v, a.type = k.data_ptr(), v.data_ptr(), type_of(k)
-        a.q = a.q_out = None
-        a.heads = 0
         if q is not None:
             wide = self.heads * c.head_dim
             a.ldq = _rows(q, self.rows, wide, "q", k)
             if q_out is None:
+                import torch
+
                 with torch.cuda.stream(stream):      # None: the current one
                     q_out = torch.empty(self.rows, wide, dtype=q.dtype, device=q.device)
             a.ldq_out = _rows(q_out, self.rows, wide, "q_out", k)
             a.q, a.q_out, a.heads = q.data_ptr(), q_out.data_ptr(), self.heads
         elif q_out is not None or q_norm is not None:
             raise SpkError("q_out and q_norm go with q")
-        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if w is not None and (w.dtype != torch.float32 or w.shape != (c.head_dim,) or not w.is_contiguous() or w.device != c.device):
-                raise SpkError(f"{name} is f32 [{c.head_dim}] on {c.device}; got {w.dtype} {list(w.shape)} on {w.device}")
-            setattr(a, name, None if w is None else w.data_ptr())
-        a.eps, a.interleaved = eps, int(interleaved)
+        else:
+            a.q, a.q_out, a.heads = None, None, 0
+        a.q_norm, a.k_norm = self._norm(q_norm, "q_norm"), self._norm(k_norm, "k_norm")
+        a.eps, a.interleaved = eps, interleaved
         a.freq, a.pdim = _angles(freq, k)
         raw = stream_of(k, stream)
         c.owned.use(raw, stream)
         check(self._append(self._pool_p, self._batch_p, self._ap_p, raw))
-        lent(stream, k, v, q, q_out, q_norm, k_norm, freq, *self._keep)
+        if stream is not None:
+            lent(stream, k, v, q, q_out, q_norm, k_norm, freq, *self._keep)
         return q_out
+
+    def _norm(self, w, name: str):
+        """The address of a norm's weights."""
+        if w is None:
+            return None
+        c = self.cache
+        if w.dtype != self._f32 or w.shape != (c.head_dim,) or not w.is_contiguous() or w.device != c.device:
+            raise SpkError(f"{name} is f32 [{c.head_dim}] on {c.device}; got {w.dtype} {list(w.shape)} on {w.device}")
+        return w.data_ptr()
 
     def attention(self, q, out=None, window: int = 0, gate=None, scale: float = 0.0, stream=None):
         """out [rows][heads * head_dim] (made when not given): attention of the rows, which have been appended, over their
@@ -145,10 +154,10 @@ class Paged4Batch(PagedBatch):
     def read(self, k=None, v=None, dtype=None, stream=None):
         """The rows' keys and values as the cache has them, (k, v) [rows][kv_heads * head_dim]: into k and v where given, else
         new rows of `dtype` (bf16 when not given)."""
-        import torch
-
         c = self.cache
         if k is None or v is None:
+            import torch
+
             given = v if k is None else k
             if given is not None:
                 dtype = given.dtype
@@ -165,21 +174,20 @@ class Paged4Batch(PagedBatch):
     def parts(self, out=None, stream=None):
         """The rows as the cache has them, apart: [k codes, k scales, v codes, v scales], codes e4m3
         [rows][kv_heads * head_dim], scales f16 [rows][kv_heads * head_dim / 16]. out: four such tensors."""
-        import torch
-
-        c = self.cache
-        width = c.kv_heads * c.head_dim
-        kinds = [(w, t) for _ in "kv" for w, t in ((width, torch.float8_e4m3fn), (width // GROUP, torch.float16))]
+        c, a = self.cache, self._rd
         if out is None:
+            import torch
+
             with torch.cuda.stream(stream):
-                out = [torch.empty(self.rows, w, dtype=t, device=c.device) for w, t in kinds]
-        a, names = self._rd, ("k", "k_scale", "v", "v_scale")
-        for t, (w, dtype), name in zip(out, kinds, names):
+                out = [torch.empty(self.rows, w, dtype=t, device=c.device) for w, t, _ in self._parts]
+        k, ks, v, vs = out
+        for t, (w, dtype, name) in zip(out, self._parts):
             if t.dtype != dtype:
                 raise SpkError(f"{name} is {dtype}; got {t.dtype}")
-            setattr(a, "ld" + name, _rows(t, self.rows, w, name, on=c.device))
-            setattr(a, name, t.data_ptr())
-        a.type = PARTS
+        (wide, *_), (few, *_) = self._parts[:2]
+        a.ldk, a.ldv = _rows(k, self.rows, wide, "k", on=c.device), _rows(v, self.rows, wide, "v", k)
+        a.ldk_scale, a.ldv_scale = _rows(ks, self.rows, few, "k_scale", on=c.device), _rows(vs, self.rows, few, "v_scale", ks)
+        a.k, a.v, a.k_scale, a.v_scale, a.type = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), PARTS
         self._read_rows(stream, *out)
         return out
 
@@ -187,4 +195,5 @@ class Paged4Batch(PagedBatch):
         raw = stream_of(out[0], stream)
         self.cache.owned.use(raw, stream)
         check(self._read(self._pool_p, self._batch_p, self._rd_p, raw))
-        lent(stream, *out, *self._keep)
+        if stream is not None:
+            lent(stream, *out, *self._keep)
