@@ -8,9 +8,10 @@
 // What bounds it: the cached bytes (288 a token and KV head of 256), so they go from the copies straight to the registers that multiply
 // them: cvt.f16x2.e2m1x2 and a product with the group's scale, both exact, give the operands of mma.sync m16n8k16. (The tensor memory path would
 // write them to shared memory as f16 and read them back, eight times the cached bytes each way, which the cache's own rate does not leave room for.)
-//   S[16][8 tokens] = Q K^T:  A = the tile's 8 query rows as f16 (rows 8..15: what f16 left of f32 rows), B = keys
-//   O^T[16 dims][8]  += V^T P^T:  A = values, two tokens' codes of a dim side by side, B = the weights, which are the S
-//                                 accumulators as they lie; f32 rows' weights are two f16 terms.
+//   S^T[16 tokens][8 rows] = K Q^T:    A = keys, B = the tile's 8 query rows as f16 (f32 rows are two terms)
+//   O^T[16 dims][8 rows]  += V^T P^T:  A = values, two tokens' codes of a dim side by side, B = the weights, which are the scores'
+//                                      accumulators turned round (f32 rows': two terms)
+// Four f32 rows or fewer have their second terms in the columns of the other four, which costs nothing.
 // The contraction's order is free, so a lane takes 16 (8) consecutive bytes of a token as its share of K.
 // Queries stand on a power of two of their row (2^14 to 2^15 at the largest), weights are 2^(s - m) with the row's largest at
 // 2^12 to 2^15: a reference m moves only when a score passes it by 15, and a weight is kept down to 2^-24, 2^-36 of the
@@ -38,12 +39,20 @@ using paged::to_f32;
 
 constexpr int R = 8;                                    // query rows of a group
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int COST = 8;                                 // a group's fixed cost in blocks
+constexpr int MAX_CTAS_ALL = 512;                       // CTAs of a call: the parts of a group
+constexpr int RUN = 16, MAX_JOIN = 32;                  // parts that are added together; at most
+constexpr int COST = 16;                                // a group's fixed cost in blocks
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// An 8 x 8 matrix of f16, a row's two in a lane, the other way round
+__device__ __forceinline__ uint32_t transpose(uint32_t a) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
 }
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -62,6 +71,11 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int n)
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
 }
 
+template <bool B>
+struct Flag {
+    static constexpr bool value = B;
+};
+
 template <typename T_, int HD_, int WARPS_, int STAGES_, int CTAS_>
 struct Cfg {
     using T = T_;
@@ -75,7 +89,9 @@ struct Cfg {
     static constexpr int Q_BYTES = STEPS * 32 * QREG * 4;
     static constexpr int RING = WARPS * STAGES * STAGE;
     static constexpr int MERGE = WARPS * R * HD * 4;     // the warps' sums at a group's end, where the rings were
-    static constexpr int SMEM = Q_BYTES + (RING > MERGE ? RING : MERGE);
+    // a merge of parts: their weights, and what the threads that share a value add up
+    static constexpr int JOIN = R * MAX_JOIN * 4 + THREADS * 16;
+    static constexpr int SMEM = Q_BYTES + (RING > MERGE ? (RING > JOIN ? RING : JOIN) : (MERGE > JOIN ? MERGE : JOIN));
     static constexpr int TB = WARPS;                     // blocks of a tile of the line: one a warp
     static constexpr int WORDS = HD / 64;                // words of 8 dims in a lane's share of a token's values
 };
@@ -83,7 +99,7 @@ struct Cfg {
 template <typename C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnParams a) {
     using T = typename C::T;
-    constexpr int HD = C::HD, ROW = C::ROW, SROW = C::SROW, WARPS = C::WARPS, WORDS = C::WORDS;
+    constexpr int HD = C::HD, ROW = C::ROW, SROW = C::SROW, STEPS = C::STEPS, WARPS = C::WARPS, WORDS = C::WORDS;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t pre[MAX_SEQ + 1], wsum[WARPS];
     __shared__ float up_s[R], m_s[WARPS][R], l_s[WARPS][R], gate_s[R];
@@ -143,6 +159,16 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
     __syncthreads();
 
     const int per = a.pool.page_tokens / BLOCK;
+    // Where the lane's 16-byte pieces of a block (piece lane + 32 x) lie in a stage: keys in order, pieces of odd tokens in each other's
+    // halves (heads of 256); values with tokens 2t of a phase in neighbouring rows, so that both are read without bank conflicts.
+    const int tok_l = lane / (ROW / 16), pc_l = lane % (ROW / 16), slot_l = (tok_l >> 1 & 3) | (tok_l & 1) << 2 | (tok_l & 8);
+    const uint32_t kd = tok_l * ROW + 16 * (HD == 256 ? pc_l ^ 4 * (tok_l & 1) : pc_l);
+    const uint32_t vd = C::V_OFF + slot_l * ROW + 16 * (HD == 256 ? pc_l ^ 2 * (slot_l & 3) : HD == 128 ? pc_l ^ (slot_l & 2) : pc_l);
+    const uint32_t vd_odd = C::V_OFF + (slot_l + 2) * ROW + 16 * (pc_l ^ 2 * ((slot_l + 2) & 3));   // heads of 256: 4 tokens on
+    auto kdst = [&](int x) { return kd + 512 * x; };
+    auto vdst = [&](int x) { return HD == 256 ? ((x & 1) ? vd_odd : vd) + 1024 * (x >> 1) : vd + 512 * x; };
+    const uint32_t sd = (lane < 16 ? C::KS_OFF : C::VS_OFF) + (lane & 15) * SROW;
+    const uint8_t *k_l = a.pool.k + 16 * lane, *v_l = a.pool.v + 16 * lane, *s_l = (lane < 16 ? a.pool.ks : a.pool.vs) + (lane & 15) * SROW;
     while (true) {
         const Seg sg = seg_s;
         if (sg.k0 < 0) break;
@@ -150,59 +176,77 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
         // blocks of this warp: first + WARPS i, i < count
         const int nblk = min(sg.nblk, sg.k1 * C::TB), first = sg.k0 * C::TB + warp, count = first < nblk ? (nblk - first + WARPS - 1) / WARPS : 0;
         const int *table = a.b.table + (size_t)sg.s * a.b.max_pages;
-        // lane i has the page of block 32 c + i of the warp's
-        auto pages = [&](int c) {
+        // the tile's queries, on their way while the blocks' places are looked up
+        constexpr int QROWS = R / WARPS > 0 ? R / WARPS : 1;
+        T qraw[QROWS][HD / 32];
+#pragma unroll
+        for (int y = 0; y < QROWS; y++) {
+            const int r = warp + y * WARPS, col = sg.c0 + r, tok = col / a.group, h = sg.kvh * a.group + col % a.group;
+            const T *src = (const T *)a.q + (long long)(sg.r0 + tok) * a.ldq + (long long)h * HD;
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) qraw[y][i] = r < cols ? src[lane + 32 * i] : from_f32<T>(0.f);
+        }
+        // lane i has the place in the pool of block 32 c + i of the warp's; -1: a page that is none
+        auto places = [&](int c) {
             const int i = 32 * c + lane;
-            int page = 0;
+            long long at = -1;
             if (i < count) {
-                page = __ldg(table + (sg.start / BLOCK + first + WARPS * i) / per);
-                if (page < 0 || page >= a.pool.pages) {
-                    if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
-                    page = -1;
-                }
+                const int blk = sg.start / BLOCK + first + WARPS * i, page = __ldg(table + blk / per);
+                if (page >= 0 && page < a.pool.pages) at = (long long)row_index(a.pool, page, sg.kvh, blk % per * BLOCK);
+                else if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
             }
-            return page;
+            return at;
         };
-        int pg = pages(0), pg_next = pages(1);
+        long long pl = places(0), pl_next = places(1);
+        uint32_t to_stage = 0;
         auto fetch = [&](int i) {
             if (i < count) {
-                const int page = __shfl_sync(0xffffffffu, pg, i & 31);
+                const long long at = __shfl_sync(0xffffffffu, pl, i & 31);
                 if ((i & 31) == 31) {
-                    pg = pg_next;
-                    pg_next = pages(i / 32 + 2);
+                    pl = pl_next;
+                    pl_next = places(i / 32 + 2);
                 }
-                const int blk = first + WARPS * i, tok0 = sg.start + blk * BLOCK, in = (sg.start / BLOCK + blk) % per * BLOCK;
-                const size_t at = row_index(a.pool, max(page, 0), sg.kvh, in);
-                const uint32_t st = ring_u + (i % C::STAGES) * C::STAGE;
-                // tokens that no row sees arrive as zeros
-                auto live = [&](int tok) { return page >= 0 && tok0 + tok >= sg.see0 && tok0 + tok <= sg.p_hi; };
-                constexpr int PIECES = ROW / 16;
+                const int tok0 = sg.start + (first + WARPS * i) * BLOCK;
+                const uint32_t st = ring_u + to_stage;
+                to_stage = to_stage == (C::STAGES - 1) * C::STAGE ? 0 : to_stage + C::STAGE;
+                const size_t row = at < 0 ? 0 : (size_t)at;
+                const uint8_t *kc = k_l + row * ROW, *vc = v_l + row * ROW, *sc = s_l + row * SROW;
+                const uint32_t sdst = st + sd;
+                if (at >= 0 && tok0 >= sg.see0 && tok0 + BLOCK - 1 <= sg.p_hi) {
 #pragma unroll
-                for (int x = lane; x < BLOCK * PIECES; x += 32) {
-                    const int tok = x / PIECES, pc = x % PIECES;
-                    const int kp = HD == 256 ? pc ^ 4 * (tok & 1) : pc;
-                    const int slot = (tok >> 1 & 3) | (tok & 1) << 2 | (tok & 8), vp = HD == 256 ? pc ^ 2 * (slot & 3) : HD == 128 ? pc ^ (slot & 2) : pc;
-                    const int n = live(tok) ? 16 : 0;
-                    copy_async<16>(st + tok * ROW + 16 * kp, a.pool.k + (at + tok) * ROW + 16 * pc, n);
-                    copy_async<16>(st + C::V_OFF + slot * ROW + 16 * vp, a.pool.v + (at + tok) * ROW + 16 * pc, n);
+                    for (int x = 0; x < ROW / 32; x++) {
+                        copy_async<16>(st + kdst(x), kc + 512 * x, 16);
+                        copy_async<16>(st + vdst(x), vc + 512 * x, 16);
+                    }
+                    copy_async<SROW>(sdst, sc, SROW);
+                } else {   // tokens that no row sees arrive as zeros
+                    auto live = [&](int tok) { return at >= 0 && tok0 + tok >= sg.see0 && tok0 + tok <= sg.p_hi; };
+#pragma unroll
+                    for (int x = 0; x < ROW / 32; x++) {
+                        const int n = live((lane + 32 * x) / (ROW / 16)) ? 16 : 0;
+                        copy_async<16>(st + kdst(x), kc + 512 * x, n);
+                        copy_async<16>(st + vdst(x), vc + 512 * x, n);
+                    }
+                    copy_async<SROW>(sdst, sc, live(lane & 15) ? SROW : 0);
                 }
-                const int tok = lane & 15;
-                copy_async<SROW>(st + (lane < 16 ? C::KS_OFF : C::VS_OFF) + tok * SROW, (lane < 16 ? a.pool.ks : a.pool.vs) + (at + tok) * SROW, live(tok) ? SROW : 0);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
         for (int i = 0; i < C::STAGES - 1; i++) fetch(i);
 
-        // the tile's queries, f16 on the row's own power of two, where the lanes' shares of A lie
-        for (int r = warp; r < R; r += WARPS) {
-            const int col = sg.c0 + r, tok = col / a.group, h = sg.kvh * a.group + col % a.group;
+        // f32 rows, four of them at most: the second terms take the columns of rows 4..7
+        const bool spare = C::TWO && cols <= 4;
+        // the tile's queries, f16 on the row's own power of two, where the lanes' shares of B lie
+#pragma unroll
+        for (int y = 0; y < QROWS; y++) {
+            const int r = warp + y * WARPS, col = sg.c0 + r, tok = col / a.group, h = sg.kvh * a.group + col % a.group;
+            if (r >= R) break;
             const bool real = r < cols;
             float x[HD / 32], mx = 0.f;
-            const T *src = (const T *)a.q + (long long)(sg.r0 + tok) * a.ldq + (long long)h * HD;
 #pragma unroll
             for (int i = 0; i < HD / 32; i++) {
-                x[i] = real ? to_f32<T>(src[lane + 32 * i]) : 0.f;
+                x[i] = to_f32<T>(qraw[y][i]);
                 mx = fmaxf(mx, fabsf(x[i]));
             }
 #pragma unroll
@@ -215,10 +259,14 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
                 const int d = lane + 32 * i;
                 const int part = HD == 256 ? d >> 7 : 0, tt = HD == 64 ? d >> 4 : d >> 5 & 3, w = HD == 64 ? d >> 3 & 1 : d >> 3 & 3;
                 const int step = (HD == 64 ? 2 * w : 8 * part + 2 * w) + (d >> 2 & 1), reg = d >> 1 & 1;
-                __half *q = reinterpret_cast<__half *>(qs) + (((step * 32 + 4 * r + tt) * C::QREG + (C::TWO ? 2 * reg : reg)) * 2 + (d & 1));
                 const __half hi = __float2half_rn(x[i] * f);
-                *q = hi;
-                if constexpr (C::TWO) q[2] = __float2half_rn(x[i] * f - __half2float(hi));
+                __half *q = reinterpret_cast<__half *>(qs) + ((step * 32 + 4 * r + tt) * C::QREG + reg) * 2 + (d & 1);
+                if (r < 4 || !spare) *q = hi;
+                if constexpr (C::TWO) {
+                    const __half lo = __float2half_rn(x[i] * f - __half2float(hi));
+                    if (!spare) q[4] = lo;
+                    else if (r < 4) q[16 * C::QREG * 2] = lo;      // the columns of rows 4..7
+                }
             }
             if (lane == 0) {
                 up_s[r] = a.scale * __int_as_float((127 - e) << 23);
@@ -228,117 +276,141 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
         }
         __syncthreads();
 
-        const float up = up_s[g];
-        const int pos = pos_s[g], low = a.window > 0 ? pos - a.window : -1;   // the row sees (low, pos]
-        float acc[HD / 16][4], m = -INFINITY, l = 0.f;
+        uint32_t qr[STEPS][2];
+#pragma unroll
+        for (int x = 0; x < STEPS; x++) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(qs + (x * 32 + lane) * C::QREG * 4);
+            qr[x][0] = v.x, qr[x][1] = v.y;
+        }
+        // the lane's rows: columns 2t and 2t + 1 of the scores and the outputs
+        const int row0 = spare ? 2 * (t & 1) : 2 * t;
+        const float up0 = up_s[row0], up1 = up_s[row0 + 1];
+        const int pos0 = pos_s[row0], pos1 = pos_s[row0 + 1], back = a.window > 0 ? a.window : INT_MAX;   // a row sees (pos - back, pos]
+        float acc[HD / 16][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
         for (int i = 0; i < HD / 16; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[i][e] = 0.f;
+        uint32_t at_stage = 0;
 
+        auto blocks = [&](auto spare_) {
+        constexpr bool SPARE = decltype(spare_)::value;
         for (int i = 0; i < count; i++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
             __syncwarp();
             fetch(i + C::STAGES - 1);
-            const uint8_t *st = ring + (i % C::STAGES) * C::STAGE;
+            const uint8_t *st = ring + at_stage;
+            at_stage = at_stage == (C::STAGES - 1) * C::STAGE ? 0 : at_stage + C::STAGE;
             const int tok0 = sg.start + (first + WARPS * i) * BLOCK;
-            // scores of tokens 0..7 (s[0], s[1]: tokens 2t, 2t + 1) and 8..15
-            float s[4];
+            // scores: tokens g and g + 8 (c[.][0], c[.][1] and c[.][2], c[.][3]) of the lane's two rows, even and odd steps apart
+            float c[2][4] = {};
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const int tok = 8 * n + g;
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int h = 0; h < (HD == 256 ? 2 : 1); h++) {
+                uint32_t w[2][4], sc[2][2];
 #pragma unroll
-                for (int h = 0; h < (HD == 256 ? 2 : 1); h++) {
-                    uint32_t w[4], sc[2];
+                for (int n = 0; n < 2; n++) {
+                    const int tok = 8 * n + g;
                     if constexpr (HD == 64) {
                         const uint2 v = *reinterpret_cast<const uint2 *>(st + tok * ROW + 8 * t);
-                        w[0] = v.x, w[1] = v.y, w[2] = w[3] = 0;
+                        w[n][0] = v.x, w[n][1] = v.y, w[n][2] = w[n][3] = 0;
                         const uint32_t b = st[C::KS_OFF + tok * SROW + t];
-                        sc[0] = sc[1] = b * 0x00800080u;
+                        sc[n][0] = sc[n][1] = b * 0x00800080u;
                     } else {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(st + tok * ROW + 16 * (HD == 256 ? (4 * h + t) ^ 4 * (tok & 1) : t));
-                        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                        const uint4 v = *reinterpret_cast<const uint4 *>(st + tok * ROW + 16 * (HD == 256 ? (4 * h + t) ^ 4 * (g & 1) : t));
+                        w[n][0] = v.x, w[n][1] = v.y, w[n][2] = v.z, w[n][3] = v.w;
                         const uint32_t b = *reinterpret_cast<const uint16_t *>(st + C::KS_OFF + tok * SROW + 8 * h + 2 * t);
-                        sc[0] = (b & 0xff) * 0x00800080u;
-                        sc[1] = (b >> 8) * 0x00800080u;
+                        sc[n][0] = (b & 0xff) * 0x00800080u;
+                        sc[n][1] = (b >> 8) * 0x00800080u;
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < (HD == 64 ? 2 : 4); x++) {
+                    uint32_t k[2][4];
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        codes_f16(w[n][x], k[n]);
+#pragma unroll
+                        for (int y = 0; y < 4; y++) k[n][y] = hmul2(k[n][y], sc[n][x >> 1]);
                     }
 #pragma unroll
-                    for (int x = 0; x < (HD == 64 ? 2 : 4); x++) {
-                        uint32_t k[4];
-                        codes_f16(w[x], k);
-#pragma unroll
-                        for (int y = 0; y < 2; y++) {
-                            const uint8_t *q = qs + ((8 * h + 2 * x + y) * 32 + lane) * C::QREG * 4;
-                            const uint32_t b0 = hmul2(k[2 * y], sc[x >> 1]), b1 = hmul2(k[2 * y + 1], sc[x >> 1]);
-                            if constexpr (C::TWO) {
-                                const uint4 v = *reinterpret_cast<const uint4 *>(q);
-                                mma(c, v.x, v.y, v.z, v.w, b0, b1);
-                            } else {
-                                const uint2 v = *reinterpret_cast<const uint2 *>(q);
-                                mma(c, v.x, 0u, v.y, 0u, b0, b1);
-                            }
+                    for (int y = 0; y < 2; y++) {
+                        const int step = 8 * h + 2 * x + y;
+                        mma(c[y], k[0][2 * y], k[1][2 * y], k[0][2 * y + 1], k[1][2 * y + 1], qr[step][0], qr[step][1]);
+                        if constexpr (C::TWO && !SPARE) {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(qs + (step * 32 + lane) * 16 + 8);
+                            mma(c[y], k[0][2 * y], k[1][2 * y], k[0][2 * y + 1], k[1][2 * y + 1], v.x, v.y);
                         }
                     }
                 }
-                s[2 * n] = (C::TWO ? c[0] + c[2] : c[0]) * up;
-                s[2 * n + 1] = (C::TWO ? c[1] + c[3] : c[1]) * up;
             }
-            // the lane's tokens of the values: 2t, 2t + 1, 2t + 8, 2t + 9
+            float s[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                s[x] = c[0][x] + c[1][x];
+                if constexpr (SPARE) s[x] += __shfl_xor_sync(0xffffffffu, s[x], 2);
+                s[x] *= x & 1 ? up1 : up0;
+            }
+            // what a row does not see; rows that are none have no place in the outputs
+            if (tok0 + BLOCK - 1 > sg.p_lo || tok0 <= sg.p_hi - back) {
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int p = tok0 + g + 8 * (x >> 1), pos = x & 1 ? pos1 : pos0;
+                    if (p > pos || p <= pos - back) s[x] = -INFINITY;
+                }
+            }
+            // the values' scales of the lane's tokens in their product: 2t, 2t + 1, 2t + 8, 2t + 9
             uint32_t vs[4];
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                const int tok = 2 * t + (x & 1) + 8 * (x >> 1);
-                const uint8_t *at = st + C::VS_OFF + tok * SROW;
+                const uint8_t *at = st + C::VS_OFF + (2 * t + (x & 1) + 8 * (x >> 1)) * SROW;
                 vs[x] = HD == 256 ? *reinterpret_cast<const uint16_t *>(at + 2 * g) : HD == 128 ? at[g] : at[g >> 1];
-                // what the row does not see
-                const int p = tok0 + tok;
-                if (p > pos || p <= low) s[x] = -INFINITY;
             }
             if (__any_sync(0xffffffffu, poisoned(vs[0] | vs[1] << 16) | poisoned(vs[2] | vs[3] << 16))) {
-                uint32_t bad = 0;
+                uint32_t bad = 0;         // a bit a token of the block
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
+                for (int x = 0; x < 4; x++)
                     if (poisoned(vs[x])) {
-                        bad |= 1u << x;
+                        bad |= 1u << (2 * t + (x & 1) + 8 * (x >> 1));
                         vs[x] = 0;
                     }
-                }
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+                bad = __reduce_or_sync(0xffffffffu, bad);
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
-                    const int p = tok0 + 2 * t + (x & 1) + 8 * (x >> 1);
-                    if ((bad >> x & 1) && p <= pos && p > low) s[x] = NAN;
+                    const int tok = g + 8 * (x >> 1), p = tok0 + tok, pos = x & 1 ? pos1 : pos0;
+                    if ((bad >> tok & 1) && p <= pos && p > pos - back) s[x] = NAN;
                 }
             }
             // a row's reference moves when one of its scores passes it by W_MAX
-            const float most = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-            if (__any_sync(0xffffffffu, most > m + W_MAX)) {
-                float x = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                const float was = m;
-                if (x > m + W_MAX) m = x - W_TOP;
-                const float f = was == -INFINITY ? 0.f : ex2(was - m);
-                l *= f;
-                const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+            const float t0 = fmaxf(s[0], s[2]), t1 = fmaxf(s[1], s[3]);
+            if (__any_sync(0xffffffffu, t0 > m0 + W_MAX || t1 > m1 + W_MAX)) {
+                float x0 = t0, x1 = t1;
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
+                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
+                }
+                const float was0 = m0, was1 = m1;
+                if (x0 > m0 + W_MAX) m0 = x0 - W_TOP;
+                if (x1 > m1 + W_MAX) m1 = x1 - W_TOP;
+                const float f0 = was0 == -INFINITY ? 0.f : ex2(was0 - m0), f1 = was1 == -INFINITY ? 0.f : ex2(was1 - m1);
+                l0 *= f0, l1 *= f1;
 #pragma unroll
                 for (int d = 0; d < HD / 16; d++) acc[d][0] *= f0, acc[d][1] *= f1, acc[d][2] *= f0, acc[d][3] *= f1;
             }
-            const float ref = m == -INFINITY ? 0.f : m;
-            float p[4];
-#pragma unroll
-            for (int x = 0; x < 4; x++) p[x] = ex2(s[x] - ref);
-            const uint32_t p0 = pack_f16(p[0], p[1]), p1 = pack_f16(p[2], p[3]);
-            uint32_t e0 = 0, e1 = 0;
+            const float ref0 = m0 == -INFINITY ? 0.f : m0, ref1 = m1 == -INFINITY ? 0.f : m1;
+            const float w0 = ex2(s[0] - ref0), w1 = ex2(s[1] - ref1), w2 = ex2(s[2] - ref0), w3 = ex2(s[3] - ref1);
+            uint32_t p0 = pack_f16(w0, w1), p1 = pack_f16(w2, w3), e0 = 0, e1 = 0;
             const float2 h0 = unpack_f16(p0), h1 = unpack_f16(p1);
             if constexpr (C::TWO) {
-                e0 = pack_f16(p[0] - h0.x, p[1] - h0.y);
-                e1 = pack_f16(p[2] - h1.x, p[3] - h1.y);
-                l += (p[0] + p[1]) + (p[2] + p[3]);
+                e0 = pack_f16(w0 - h0.x, w1 - h0.y);
+                e1 = pack_f16(w2 - h1.x, w3 - h1.y);
+                l0 += w0 + w2, l1 += w1 + w3;
+                if (SPARE && t >= 2) p0 = e0, p1 = e1;
             } else {
-                l += (h0.x + h0.y) + (h1.x + h1.y);
+                l0 += h0.x + h1.x, l1 += h0.y + h1.y;
             }
+            p0 = transpose(p0), p1 = transpose(p1);       // from token by row to row by token
+            if constexpr (C::TWO && !SPARE) e0 = transpose(e0), e1 = transpose(e1);
             // values: two tokens' codes of a dim in a byte, their scales in a pair
             uint32_t w[4][WORDS];
 #pragma unroll
@@ -375,27 +447,33 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
                 for (int x = 0; x < 4; x++) {
                     const uint32_t a0 = hmul2(ae[x], sa), a1 = hmul2(ao[x], sa), a2 = hmul2(be[x], sb), a3 = hmul2(bo[x], sb);
                     mma(acc[4 * y + x], a0, a1, a2, a3, p0, p1);
-                    if constexpr (C::TWO) mma(acc[4 * y + x], a0, a1, a2, a3, e0, e1);
+                    if constexpr (C::TWO && !SPARE) mma(acc[4 * y + x], a0, a1, a2, a3, e0, e1);
                 }
             }
         }
+        };
+        if (C::TWO && spare) blocks(Flag<true>());
+        else blocks(Flag<false>());
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        // the row's sum over its four lanes
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) {
-            m_s[warp][g] = m;
-            l_s[warp][g] = l;
+        // the rows' sums over their eight lanes
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+        }
+        if (g == 0 && (!spare || t < 2)) {
+            m_s[warp][row0] = m0, m_s[warp][row0 + 1] = m1;
+            l_s[warp][row0] = l0, l_s[warp][row0 + 1] = l1;
         }
         __syncthreads();                                  // the rings are done with, too
         // columns 2t, 2t + 1 of acc on the CTA's common reference, into the warps' share of the rings
         float *mine = reinterpret_cast<float *>(smem + C::Q_BYTES) + warp * R * HD;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const int r = 2 * t + e;
+            const int r = 2 * t + e, rm = spare ? r & 3 : r;
             float M = -INFINITY;
-            for (int w = 0; w < WARPS; w++) M = fmaxf(M, m_s[w][r]);
-            const float mw = m_s[warp][r], f = mw == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(mw - M);
+            for (int w = 0; w < WARPS; w++) M = fmaxf(M, m_s[w][rm]);
+            const float mw = m_s[warp][rm], f = mw == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(mw - M);
 #pragma unroll
             for (int d = 0; d < HD / 16; d += 2) {
                 float4 v = make_float4(acc[d][e] * f, acc[d][2 + e] * f, acc[d + 1][e] * f, acc[d + 1][2 + e] * f);
@@ -406,6 +484,16 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
         const bool whole = sg.f0 == sg.f1;
         float *slot = a.part + ((size_t)blockIdx.x * 2 + (sg.k0 == 0 ? 1 : 0)) * part_floats(R, HD);
         const float *sums = reinterpret_cast<const float *>(smem + C::Q_BYTES);
+        auto output = [&](int r, int d, float4 o, float L) {
+            const float f = L == 0.f ? 0.f : gate_s[r] / L;
+            if (L == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
+            const int col = sg.c0 + r;
+            T *dst = (T *)a.out + (long long)(sg.r0 + col / a.group) * a.ldout + (long long)(sg.kvh * a.group + col % a.group) * HD + d;
+            dst[0] = from_f32<T>(o.x * f);
+            dst[1] = from_f32<T>(o.y * f);
+            dst[2] = from_f32<T>(o.z * f);
+            dst[3] = from_f32<T>(o.w * f);
+        };
         for (int x = tid; x < cols * (HD / 4); x += C::THREADS) {
             const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
             float M = -INFINITY, L = 0.f;
@@ -415,16 +503,13 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
             for (int w = 0; w < WARPS; w++) {
                 const float4 v = *reinterpret_cast<const float4 *>(sums + (w * R + r) * HD + d);
                 o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+                if (spare) {
+                    const float4 y = *reinterpret_cast<const float4 *>(sums + (w * R + r + 4) * HD + d);
+                    o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+                }
             }
-            if (whole) {
-                const float f = L == 0.f ? 0.f : gate_s[r] / L;
-                const int col = sg.c0 + r;
-                T *dst = (T *)a.out + (long long)(sg.r0 + col / a.group) * a.ldout + (long long)(sg.kvh * a.group + col % a.group) * HD + d;
-                dst[0] = from_f32<T>(L == 0.f ? 0.f : o.x * f);
-                dst[1] = from_f32<T>(L == 0.f ? 0.f : o.y * f);
-                dst[2] = from_f32<T>(L == 0.f ? 0.f : o.z * f);
-                dst[3] = from_f32<T>(L == 0.f ? 0.f : o.w * f);
-            } else {
+            if (whole) output(r, d, o, L);
+            else {
                 *reinterpret_cast<float4 *>(slot + r * HD + d) = o;
                 if (d == 0) {
                     slot[R * HD + r] = M;
@@ -432,40 +517,82 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
                 }
             }
         }
-        if (!whole) {   // the last CTA of the group adds all parts in CTA order
-            const int parts = sg.f1 - sg.f0 + 1;
-            __syncthreads();
-            if (tid == 0) {
-                __threadfence();   // for all of them: their stores came before the barrier
-                const bool last = atomicAdd(a.tickets + sg.f0, 1u) == (unsigned)(parts - 1);
-                if (last) a.tickets[sg.f0] = 0u;
-                __threadfence();
-                last_s = last;
-            }
-            __syncthreads();
-            if (last_s) {
-                const size_t step = (size_t)2 * part_floats(R, HD);
-                const float *p0 = a.part + (size_t)sg.f0 * step;   // CTA f0: slot 1, the others: slot 0
-                auto part = [&](int p) { return p0 + p * step + (p == 0 ? part_floats(R, HD) : 0); };
-                for (int x = tid; x < cols * (HD / 4); x += C::THREADS) {
-                    const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
-                    float M = -INFINITY, L = 0.f;
-                    for (int p = 0; p < parts; p++) M = fmaxf(M, __ldcg(part(p) + R * HD + r));
+        if (!whole) {
+            // Parts are added in CTA order. Many of them (a long sequence of few rows) in two steps, so that no CTA reads more than a few: the last
+            // CTA of each RUN to arrive leaves its run's sum in the place of the run's first part, and the last one of those adds the runs.
+            const int parts = sg.f1 - sg.f0 + 1, mine = (int)blockIdx.x - sg.f0, runs = parts > 2 * RUN ? (parts + RUN - 1) / RUN : 1;
+            auto part = [&](int p) { return a.part + ((size_t)(sg.f0 + p) * 2 + (p == 0)) * part_floats(R, HD); };   // CTA f0: slot 1, the others: slot 0
+            auto last_of = [&](unsigned int *ticket, int n) {
+                __syncthreads();
+                if (tid == 0) {
+                    __threadfence();   // for all of them: their stores came before the barrier
+                    const bool last = atomicAdd(ticket, 1u) == (unsigned)(n - 1);
+                    if (last) *ticket = 0u;
+                    __threadfence();
+                    last_s = last;
+                }
+                __syncthreads();
+                return last_s != 0;
+            };
+            // the sum of n parts, `step` apart from part `at` on: to the outputs, or to the first one's place
+            auto join = [&](int at, int step, int n, bool done) {
+                float *wt = reinterpret_cast<float *>(smem + C::Q_BYTES), *red = wt + R * MAX_JOIN;
+                for (int r = warp; r < cols; r += WARPS) {   // the parts' weights: a warp per row
+                    const float m = lane < n ? __ldcg(part(at + step * lane) + R * HD + r) : -INFINITY, x = lane < n ? __ldcg(part(at + step * lane) + R * HD + R + r) : 0.f;
+                    float M = m;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                    const float f = m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(m - M);
+                    if (lane < n) wt[r * MAX_JOIN + lane] = f;
+                    const float L = warp_sum(m == -INFINITY ? x : x * f);
+                    if (lane == 0) m_s[0][r] = M, l_s[0][r] = L;
+                }
+                __syncthreads();
+                // an item: 4 values of a row; `ways` threads share its parts, 8 loads on their way
+                const int items = cols * (HD / 4), ways = max(1, min(C::THREADS / items, (n + 7) / 8));
+                for (int x0 = 0; x0 < items; x0 += C::THREADS) {   // one turn where several threads share an item
+                    const int x = ways > 1 ? tid % items : x0 + tid, way = ways > 1 ? tid / items : 0;
+                    const int r = x / (HD / 4), d = 4 * (x % (HD / 4)), a0 = n * way / ways, a1 = n * (way + 1) / ways;
                     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int p = 0; p < parts; p++) {
-                        const float mp = __ldcg(part(p) + R * HD + r), lp = __ldcg(part(p) + R * HD + R + r);
-                        const float f = mp == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(mp - M);
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(p) + r * HD + d));
-                        L = mp == -INFINITY ? L + lp : fmaf(lp, f, L);
-                        o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+                    const bool own = x < items && way < ways;
+                    if (own)
+                        for (int p = a0; p < a1; p += 8) {
+                            float4 v[8];
+#pragma unroll
+                            for (int y = 0; y < 8; y++)   // past the last part: the last one again, left out
+                                v[y] = __ldcg(reinterpret_cast<const float4 *>(part(at + step * min(p + y, a1 - 1)) + r * HD + d));
+#pragma unroll
+                            for (int y = 0; y < 8; y++) {
+                                const float f = wt[r * MAX_JOIN + min(p + y, a1 - 1)];
+                                if (p + y < a1) o.x = fmaf(v[y].x, f, o.x), o.y = fmaf(v[y].y, f, o.y), o.z = fmaf(v[y].z, f, o.z), o.w = fmaf(v[y].w, f, o.w);
+                            }
+                        }
+                    if (ways > 1) {
+                        if (own && way > 0) *reinterpret_cast<float4 *>(red + 4 * ((way - 1) * items + x)) = o;
+                        __syncthreads();
+                        if (own && way == 0)
+                            for (int w = 1; w < ways; w++) {
+                                const float4 y = *reinterpret_cast<const float4 *>(red + 4 * ((w - 1) * items + x));
+                                o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+                            }
                     }
-                    const float f = L == 0.f ? 0.f : gate_s[r] / L;
-                    const int col = sg.c0 + r;
-                    T *dst = (T *)a.out + (long long)(sg.r0 + col / a.group) * a.ldout + (long long)(sg.kvh * a.group + col % a.group) * HD + d;
-                    dst[0] = from_f32<T>(L == 0.f ? 0.f : o.x * f);
-                    dst[1] = from_f32<T>(L == 0.f ? 0.f : o.y * f);
-                    dst[2] = from_f32<T>(L == 0.f ? 0.f : o.z * f);
-                    dst[3] = from_f32<T>(L == 0.f ? 0.f : o.w * f);
+                    if (own && way == 0) {
+                        if (done) output(r, d, o, l_s[0][r]);
+                        else {   // the places that this run's parts had are read by this CTA alone
+                            float *to = part(at);
+                            __stcg(reinterpret_cast<float4 *>(to + r * HD + d), o);
+                            if (d == 0) __stcg(to + R * HD + r, m_s[0][r]), __stcg(to + R * HD + R + r, l_s[0][r]);
+                        }
+                    }
+                }
+            };
+            if (runs == 1) {
+                if (last_of(a.tickets + sg.f0, parts)) join(0, 1, parts, true);
+            } else {
+                const int run = mine / RUN, n = min(RUN, parts - run * RUN);
+                if (last_of(a.tickets + MAX_CTAS_ALL * (run == 0 ? 1 : 2) + sg.f0 + run * RUN, n)) {
+                    join(run * RUN, 1, n, false);
+                    if (last_of(a.tickets + sg.f0, runs)) join(0, RUN, runs, true);
                 }
             }
         }
@@ -481,7 +608,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
 }
 
 constexpr long long NARROW = 64;                       // rows per KV head up to which a sequence is this kernel's
-constexpr size_t TICKETS = 4096;                        // bytes before the partials: one word per CTA
+constexpr size_t TICKETS = 3 * MAX_CTAS_ALL * sizeof(unsigned int);   // before the partials: three words per CTA
 constexpr int MAX_CTAS = 3;                             // of an SM
 
 template <typename C>
@@ -540,7 +667,7 @@ int spk_paged4_attn(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
     const int size = p->type == T_F32 ? 4 : 2;
     if (((uintptr_t)p->q | (uintptr_t)p->out | (uintptr_t)p->gate) % size) return set_error("%s: unaligned rows", who);
     if ((uintptr_t)p->workspace % 16) return set_error("%s: the workspace is not 16-byte aligned", who);
-    if ((size_t)sm_count() * MAX_CTAS * sizeof(unsigned int) > TICKETS) return set_error("%s: a device of %d SMs", who, sm_count());
+    if (sm_count() * MAX_CTAS > MAX_CTAS_ALL) return set_error("%s: a device of %d SMs", who, sm_count());
     AttnParams a;
     a.pool = pool_of(pool);
     a.b = paged::batch_of(batch);
