@@ -40,8 +40,9 @@ using paged::to_f32;
 constexpr int R = 8;                                    // query rows of a group
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_CTAS_ALL = 512;                       // CTAs of a call: the parts of a group
-constexpr int RUN = 16, MAX_JOIN = 32;                  // parts that are added together; at most
-constexpr int COST = 16;                                // a group's fixed cost in blocks
+constexpr int RUN = 16, MAX_JOIN = 32;                  // parts that are added together; at most (a lane each)
+static_assert(2 * RUN <= MAX_JOIN && MAX_CTAS_ALL <= RUN * MAX_JOIN, "");
+constexpr int COST = 20;                                // a group's fixed cost in blocks
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -96,6 +97,95 @@ struct Cfg {
     static constexpr int WORDS = HD / 64;                // words of 8 dims in a lane's share of a token's values
 };
 
+// Sums and parts hold the four values of a lane of an output tile side by side, lane after lane: the first dim of those at `at`.
+template <int HD>
+__device__ __forceinline__ int dims_of(int at) { return (at >> 2 & 7) * (HD / 8) + (at >> 5) * 4; }
+
+// Four outputs of row r of a group's tile
+template <typename C>
+__device__ __forceinline__ void output(const AttnParams &a, const Seg &sg, int r, int at, float4 o, float L, float gate) {
+    using T = typename C::T;
+    const float f = L == 0.f ? 0.f : gate / L;
+    if (L == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int col = sg.c0 + r;
+    T *dst = (T *)a.out + (long long)(sg.r0 + col / a.group) * a.ldout + (long long)(sg.kvh * a.group + col % a.group) * C::HD + dims_of<C::HD>(at);
+    dst[0] = from_f32<T>(o.x * f);
+    dst[1] = from_f32<T>(o.y * f);
+    dst[2] = from_f32<T>(o.z * f);
+    dst[3] = from_f32<T>(o.w * f);
+}
+
+// Part p of a group, in CTA order: CTA f0's second slot, the others' first one
+template <typename C>
+__device__ __forceinline__ float *part_of(const AttnParams &a, const Seg &sg, int p) {
+    return a.part + ((size_t)(sg.f0 + p) * 2 + (p == 0)) * part_floats(R, C::HD);
+}
+
+// The sum of n parts of a group, `step` apart from part `at` on, by the CTA: to the outputs, or to the first one's place, which this CTA
+// alone reads. Not inlined: the loads on their way would cost the main loop its registers.
+template <typename C>
+__device__ __noinline__ void join(const AttnParams &a, const Seg &sg, float *wt, const float *gate_s, int at, int step, int n, bool done) {
+    constexpr int HD = C::HD, WARPS = C::WARPS;
+    __shared__ float M_s[R], L_s[R];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cols = sg.c1 - sg.c0 + 1;
+    auto part = [&](int p) { return part_of<C>(a, sg, p); };
+    float *red = wt + R * MAX_JOIN;
+                    // an item: 4 values of a row; `ways` threads share its parts, 8 loads on their way
+                    const int items = cols * (HD / 4), ways = max(1, min(C::THREADS / items, (n + 7) / 8));
+                    const int way = ways > 1 ? tid / items : 0, a0 = n * way / ways, a1 = n * (way + 1) / ways;
+                    float4 v[8];
+                    auto load = [&](int x, int p) {
+                        const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
+    #pragma unroll
+                        for (int y = 0; y < 8; y++)   // past the last part: the last one again, left out
+                            v[y] = __ldcg(reinterpret_cast<const float4 *>(part(at + step * min(p + y, a1 - 1)) + r * HD + d));
+                    };
+                    const int first = ways > 1 ? tid % items : tid;
+                    if (first < items && way < ways) load(first, a0);
+                    for (int r = warp; r < cols; r += WARPS) {   // the parts' weights: a warp per row
+                        const float m = lane < n ? __ldcg(part(at + step * lane) + R * HD + r) : -INFINITY, x = lane < n ? __ldcg(part(at + step * lane) + R * HD + R + r) : 0.f;
+                        float M = m;
+    #pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+                        const float f = m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(m - M);
+                        if (lane < n) wt[r * MAX_JOIN + lane] = f;
+                        const float L = warp_sum(m == -INFINITY ? x : x * f);
+                        if (lane == 0) M_s[r] = M, L_s[r] = L;
+                    }
+                    __syncthreads();
+                    for (int x0 = 0; x0 < items; x0 += C::THREADS) {   // one turn where several threads share an item
+                        const int x = ways > 1 ? first : x0 + tid, r = x / (HD / 4), d = 4 * (x % (HD / 4));
+                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                        const bool own = x < items && way < ways;
+                        if (own)
+                            for (int p = a0; p < a1; p += 8) {
+                                if (x0 > 0 || p > a0) load(x, p);
+    #pragma unroll
+                                for (int y = 0; y < 8; y++) {
+                                    const float f = wt[r * MAX_JOIN + min(p + y, a1 - 1)];
+                                    if (p + y < a1) o.x = fmaf(v[y].x, f, o.x), o.y = fmaf(v[y].y, f, o.y), o.z = fmaf(v[y].z, f, o.z), o.w = fmaf(v[y].w, f, o.w);
+                                }
+                            }
+                        if (ways > 1) {
+                            if (own && way > 0) *reinterpret_cast<float4 *>(red + 4 * ((way - 1) * items + x)) = o;
+                            __syncthreads();
+                            if (own && way == 0)
+                                for (int w = 1; w < ways; w++) {
+                                    const float4 y = *reinterpret_cast<const float4 *>(red + 4 * ((w - 1) * items + x));
+                                    o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+                                }
+                        }
+                        if (own && way == 0) {
+                            if (done) output<C>(a, sg, r, d, o, L_s[r], gate_s[r]);
+                            else {
+                                float *to = part(at);
+                                __stcg(reinterpret_cast<float4 *>(to + r * HD + d), o);
+                                if (d == 0) __stcg(to + R * HD + r, M_s[r]), __stcg(to + R * HD + R + r, L_s[r]);
+                            }
+                        }
+                    }
+}
+
 template <typename C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnParams a) {
     using T = typename C::T;
@@ -104,7 +194,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
     __shared__ uint32_t pre[MAX_SEQ + 1], wsum[WARPS];
     __shared__ float up_s[R], m_s[WARPS][R], l_s[WARPS][R], gate_s[R];
     __shared__ int pos_s[R];
-    __shared__ Seg seg_s;
+    __shared__ Seg seg_s[2];                                // this group and the next one: the slowest warp still reads the first
     __shared__ Walk walk_s;
     __shared__ int last_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -141,7 +231,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
     }
     if (tid == 0) {
         pre[a.b.nseq] = base;
-        seg_s.k0 = -1;
+        seg_s[0].k0 = -1;
     }
     __syncthreads();
     const uint32_t chunk = max((base + gridDim.x - 1) / gridDim.x, (uint32_t)C::TB), x0 = chunk * blockIdx.x;
@@ -153,7 +243,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
             w.x1 = min(base, x0 + chunk);
             paged::walk_at(a, pre, s, R, COST, w);
             Seg first;
-            if (paged::walk_next<C::TB>(a, pre, R, COST, w, first)) seg_s = first;
+            if (paged::walk_next<C::TB>(a, pre, R, COST, w, first)) seg_s[0] = first;
             walk_s = w;
         }
     __syncthreads();
@@ -169,15 +259,15 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
     auto vdst = [&](int x) { return HD == 256 ? ((x & 1) ? vd_odd : vd) + 1024 * (x >> 1) : vd + 512 * x; };
     const uint32_t sd = (lane < 16 ? C::KS_OFF : C::VS_OFF) + (lane & 15) * SROW;
     const uint8_t *k_l = a.pool.k + 16 * lane, *v_l = a.pool.v + 16 * lane, *s_l = (lane < 16 ? a.pool.ks : a.pool.vs) + (lane & 15) * SROW;
-    while (true) {
-        const Seg sg = seg_s;
+    for (int turn = 0;; turn ^= 1) {
+        const Seg sg = seg_s[turn];
         if (sg.k0 < 0) break;
         const int cols = sg.c1 - sg.c0 + 1;
         // blocks of this warp: first + WARPS i, i < count
         const int nblk = min(sg.nblk, sg.k1 * C::TB), first = sg.k0 * C::TB + warp, count = first < nblk ? (nblk - first + WARPS - 1) / WARPS : 0;
         const int *table = a.b.table + (size_t)sg.s * a.b.max_pages;
         // the tile's queries, on their way while the blocks' places are looked up
-        constexpr int QROWS = R / WARPS > 0 ? R / WARPS : 1;
+        constexpr int QROWS = (R + WARPS - 1) / WARPS;
         T qraw[QROWS][HD / 32];
 #pragma unroll
         for (int y = 0; y < QROWS; y++) {
@@ -477,23 +567,13 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
 #pragma unroll
             for (int d = 0; d < HD / 16; d += 2) {
                 float4 v = make_float4(acc[d][e] * f, acc[d][2 + e] * f, acc[d + 1][e] * f, acc[d + 1][2 + e] * f);
-                *reinterpret_cast<float4 *>(mine + r * HD + g * (HD / 8) + 2 * d) = v;
+                *reinterpret_cast<float4 *>(mine + r * HD + 16 * d + 4 * g) = v;   // as dims_of() says
             }
         }
         __syncthreads();
         const bool whole = sg.f0 == sg.f1;
         float *slot = a.part + ((size_t)blockIdx.x * 2 + (sg.k0 == 0 ? 1 : 0)) * part_floats(R, HD);
         const float *sums = reinterpret_cast<const float *>(smem + C::Q_BYTES);
-        auto output = [&](int r, int d, float4 o, float L) {
-            const float f = L == 0.f ? 0.f : gate_s[r] / L;
-            if (L == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
-            const int col = sg.c0 + r;
-            T *dst = (T *)a.out + (long long)(sg.r0 + col / a.group) * a.ldout + (long long)(sg.kvh * a.group + col % a.group) * HD + d;
-            dst[0] = from_f32<T>(o.x * f);
-            dst[1] = from_f32<T>(o.y * f);
-            dst[2] = from_f32<T>(o.z * f);
-            dst[3] = from_f32<T>(o.w * f);
-        };
         for (int x = tid; x < cols * (HD / 4); x += C::THREADS) {
             const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
             float M = -INFINITY, L = 0.f;
@@ -508,7 +588,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
                     o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
                 }
             }
-            if (whole) output(r, d, o, L);
+            if (whole) output<C>(a, seg_s[turn], r, d, o, L, gate_s[r]);
             else {
                 *reinterpret_cast<float4 *>(slot + r * HD + d) = o;
                 if (d == 0) {
@@ -521,78 +601,26 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
             // Parts are added in CTA order. Many of them (a long sequence of few rows) in two steps, so that no CTA reads more than a few: the last
             // CTA of each RUN to arrive leaves its run's sum in the place of the run's first part, and the last one of those adds the runs.
             const int parts = sg.f1 - sg.f0 + 1, mine = (int)blockIdx.x - sg.f0, runs = parts > 2 * RUN ? (parts + RUN - 1) / RUN : 1;
-            auto part = [&](int p) { return a.part + ((size_t)(sg.f0 + p) * 2 + (p == 0)) * part_floats(R, HD); };   // CTA f0: slot 1, the others: slot 0
+            float *wt = reinterpret_cast<float *>(smem + C::Q_BYTES);
             auto last_of = [&](unsigned int *ticket, int n) {
                 __syncthreads();
-                if (tid == 0) {
-                    __threadfence();   // for all of them: their stores came before the barrier
-                    const bool last = atomicAdd(ticket, 1u) == (unsigned)(n - 1);
+                if (tid == 0) {   // releases what all of them stored before the barrier, and acquires the others' stores
+                    unsigned int was;
+                    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(was) : "l"(ticket) : "memory");
+                    const bool last = was == (unsigned)(n - 1);
                     if (last) *ticket = 0u;
-                    __threadfence();
                     last_s = last;
                 }
                 __syncthreads();
                 return last_s != 0;
             };
-            // the sum of n parts, `step` apart from part `at` on: to the outputs, or to the first one's place
-            auto join = [&](int at, int step, int n, bool done) {
-                float *wt = reinterpret_cast<float *>(smem + C::Q_BYTES), *red = wt + R * MAX_JOIN;
-                for (int r = warp; r < cols; r += WARPS) {   // the parts' weights: a warp per row
-                    const float m = lane < n ? __ldcg(part(at + step * lane) + R * HD + r) : -INFINITY, x = lane < n ? __ldcg(part(at + step * lane) + R * HD + R + r) : 0.f;
-                    float M = m;
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-                    const float f = m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(m - M);
-                    if (lane < n) wt[r * MAX_JOIN + lane] = f;
-                    const float L = warp_sum(m == -INFINITY ? x : x * f);
-                    if (lane == 0) m_s[0][r] = M, l_s[0][r] = L;
-                }
-                __syncthreads();
-                // an item: 4 values of a row; `ways` threads share its parts, 8 loads on their way
-                const int items = cols * (HD / 4), ways = max(1, min(C::THREADS / items, (n + 7) / 8));
-                for (int x0 = 0; x0 < items; x0 += C::THREADS) {   // one turn where several threads share an item
-                    const int x = ways > 1 ? tid % items : x0 + tid, way = ways > 1 ? tid / items : 0;
-                    const int r = x / (HD / 4), d = 4 * (x % (HD / 4)), a0 = n * way / ways, a1 = n * (way + 1) / ways;
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                    const bool own = x < items && way < ways;
-                    if (own)
-                        for (int p = a0; p < a1; p += 8) {
-                            float4 v[8];
-#pragma unroll
-                            for (int y = 0; y < 8; y++)   // past the last part: the last one again, left out
-                                v[y] = __ldcg(reinterpret_cast<const float4 *>(part(at + step * min(p + y, a1 - 1)) + r * HD + d));
-#pragma unroll
-                            for (int y = 0; y < 8; y++) {
-                                const float f = wt[r * MAX_JOIN + min(p + y, a1 - 1)];
-                                if (p + y < a1) o.x = fmaf(v[y].x, f, o.x), o.y = fmaf(v[y].y, f, o.y), o.z = fmaf(v[y].z, f, o.z), o.w = fmaf(v[y].w, f, o.w);
-                            }
-                        }
-                    if (ways > 1) {
-                        if (own && way > 0) *reinterpret_cast<float4 *>(red + 4 * ((way - 1) * items + x)) = o;
-                        __syncthreads();
-                        if (own && way == 0)
-                            for (int w = 1; w < ways; w++) {
-                                const float4 y = *reinterpret_cast<const float4 *>(red + 4 * ((w - 1) * items + x));
-                                o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
-                            }
-                    }
-                    if (own && way == 0) {
-                        if (done) output(r, d, o, l_s[0][r]);
-                        else {   // the places that this run's parts had are read by this CTA alone
-                            float *to = part(at);
-                            __stcg(reinterpret_cast<float4 *>(to + r * HD + d), o);
-                            if (d == 0) __stcg(to + R * HD + r, m_s[0][r]), __stcg(to + R * HD + R + r, l_s[0][r]);
-                        }
-                    }
-                }
-            };
             if (runs == 1) {
-                if (last_of(a.tickets + sg.f0, parts)) join(0, 1, parts, true);
+                if (last_of(a.tickets + sg.f0, parts)) join<C>(a, seg_s[turn], wt, gate_s, 0, 1, parts, true);
             } else {
                 const int run = mine / RUN, n = min(RUN, parts - run * RUN);
                 if (last_of(a.tickets + MAX_CTAS_ALL * (run == 0 ? 1 : 2) + sg.f0 + run * RUN, n)) {
-                    join(run * RUN, 1, n, false);
-                    if (last_of(a.tickets + sg.f0, runs)) join(0, RUN, runs, true);
+                    join<C>(a, seg_s[turn], wt, gate_s, run * RUN, 1, n, false);
+                    if (last_of(a.tickets + sg.f0, runs)) join<C>(a, seg_s[turn], wt, gate_s, 0, RUN, runs, true);
                 }
             }
         }
@@ -601,7 +629,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
             Seg nx;
             if (!paged::walk_next<C::TB>(a, pre, R, COST, w, nx)) nx.k0 = -1;
             walk_s = w;
-            seg_s = nx;
+            seg_s[turn ^ 1] = nx;
         }
         __syncthreads();
     }
@@ -632,7 +660,7 @@ int launch_one(const AttnParams &a, cudaStream_t s, const char *who) {
 
 template <typename T>
 int launch(const AttnParams &a, cudaStream_t s, const char *who) {
-    return a.pool.hd == 256   ? launch_one<Cfg<T, 256, 4, 3, 3>>(a, s, who)
+    return a.pool.hd == 256   ? launch_one<Cfg<T, 256, 4, 4, 2>>(a, s, who)
            : a.pool.hd == 128 ? launch_one<Cfg<T, 128, 4, 4, 3>>(a, s, who)
                               : launch_one<Cfg<T, 64, 4, 4, 3>>(a, s, who);
 }
