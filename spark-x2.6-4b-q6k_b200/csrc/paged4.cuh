@@ -65,8 +65,8 @@ struct AttnParams {
     int *err;
     __device__ __forceinline__ bool takes(long long columns) const { return columns >= from && columns <= to; }
 };
-// Weights are f16 numbers 2^(s - m): a new reference m puts the row's largest at 2^12, and it moves when one passes 2^15. A
-// weight is then kept down to 2^-24, 2^-36 of the largest.
+// Weights are f16 numbers 2^(s - m): a new reference m puts the row's largest at 2^W_TOP (the kernel for many rows: less), and it moves when
+// one passes 2^W_MAX. A weight is kept down to 2^-24, 2^-36 of the largest.
 constexpr float W_TOP = 12.0f, W_MAX = 15.0f;
 
 // Floats of one CTA's part of a group of R query rows: O, then m, then l.

@@ -11,6 +11,8 @@
 //
 // Work split: paged_line.cuh's line of groups of 128 rows, one CTA per SM. Warps: 0-3 queries, softmax and outputs,
 // 4-11 codes to f16, 12 the MMAs. Each walks the CTA's groups by itself; they meet at mbarriers.
+#include <limits.h>
+
 #include "paged4.cuh"
 #include "paged_line.cuh"
 #include "paged_tc.cuh"
@@ -23,16 +25,21 @@ using namespace paged;
 
 constexpr int N = 64, TB = N / BLOCK;                   // tokens of a tile, its blocks
 constexpr int R = WIDE_R;
+constexpr int QCH = R * 128;                            // 64 dims of the queries' second terms
 constexpr int SM_WARPS = 4, DQ_WARPS = 8, MMA_WARP = SM_WARPS + DQ_WARPS, WARPS = MMA_WARP + 1, THREADS = WARPS * 32;
 constexpr int COST = 32;                                // a group's fixed cost in blocks
+constexpr int NONE = INT_MIN;                           // no page
 
 template <typename T_, int HD_>
 struct Cfg {
     using T = T_;
     static constexpr int HD = HD_;
     static constexpr bool TWO = sizeof(T) == 4;
+    // log2 of the largest weight at a new reference: the further under W_MAX, the fewer moves, each of which takes a warp's outputs
+    // through its registers; a weight is kept down to 2^-24 under it.
+    static constexpr float TOP = TWO ? 10.0f : 6.0f;
     static constexpr int TILE = N * HD * 2;             // bytes of a tile's keys (or values) in f16
-    static constexpr int CH = N * 128, QCH = R * 128;   // 64 dims of them, of the queries' second terms
+    static constexpr int CH = N * 128;                  // 64 dims of them
     static constexpr int V_OFF = 2 * TILE, Q_OFF = 4 * TILE;
     static constexpr size_t SMEM = Q_OFF + (TWO ? R * HD * 2 : 0) + 1024;
     static constexpr int PARTS = HD / 32;               // a thread's shares of a token
@@ -237,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 for (int k = 0; k < HD / 16; k++) {
                     const uint64_t b = desc(kb + i * C::TILE + (k / 4) * C::CH + (k % 4) * 32, 0);
                     mma_ts(d, tmem + C::QC + 8 * k, b, id_s, k > 0);
-                    if constexpr (TWO) mma_ss(d, desc(qb + (k / 4) * C::QCH + (k % 4) * 32, 0), b, id_s, true);
+                    if constexpr (TWO) mma_ss(d, desc(qb + (k / 4) * QCH + (k % 4) * 32, 0), b, id_s, true);
                 }
                 mma_commit(empty_k + i);
                 mma_commit(s_full + i);
@@ -283,16 +290,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
         for (; sg.k0 >= 0; next(sg)) {
             const int n = tiles_of(sg);
             const int *table = a.b.table + (size_t)sg.s * a.b.max_pages;
-            // the thread's row in the pool for tile j of the group: -1 where no row sees the token
+            // the page of the thread's token of tile j, as the table has it; NONE where no row sees the token
             auto page_of = [&](int j) {
                 const int blk = (sg.k0 + j) * TB + tok / BLOCK, at = sg.start + (sg.k0 + j) * N + tok;
-                if (j >= n || blk >= sg.nblk || at < sg.see0 || at > sg.p_hi) return -1;
-                const int page = __ldg(table + (sg.start / BLOCK + blk) / per);
-                if (page < 0 || page >= a.pool.pages) {
-                    if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
-                    return -1;
-                }
-                return page;
+                return j >= n || blk >= sg.nblk || at < sg.see0 || at > sg.p_hi ? NONE : __ldg(table + (sg.start / BLOCK + blk) / per);
             };
             auto row_of = [&](int page, int j) {
                 const int blk = sg.start / BLOCK + (sg.k0 + j) * TB + tok / BLOCK;
@@ -300,24 +301,25 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             };
             struct Raw {
                 uint4 c[U];
-                uint32_t s[U], check;
-            } raw;
-            auto load = [&](bool keys, int page, int j) {
+                uint32_t s[U], vs[U];            // vs, beside keys: their tokens' scales of values, looked at for poison
+            };
+            auto load = [&](Raw &raw, bool keys, int page, int j) {
 #pragma unroll
-                for (int u = 0; u < U; u++) raw.c[u] = make_uint4(0, 0, 0, 0), raw.s[u] = 0;
-                raw.check = 0;
-                if (page >= 0 && !idle) {
+                for (int u = 0; u < U; u++) raw.c[u] = make_uint4(0, 0, 0, 0), raw.s[u] = raw.vs[u] = 0;
+                const bool seen = page != NONE, there = page >= 0 && page < a.pool.pages;
+                if (seen && !there && a.err) atomicExch(a.err, DEV_BAD_INDEX);
+                if (there && !idle) {
                     const size_t at = row_of(page, j);
 #pragma unroll
                     for (int u = 0; u < U; u++) {
                         const int x = part + 4 * u;
                         raw.c[u] = __ldg(reinterpret_cast<const uint4 *>((keys ? a.pool.k : a.pool.v) + at * (HD / 2)) + x);
                         raw.s[u] = __ldg(reinterpret_cast<const uint16_t *>((keys ? a.pool.ks : a.pool.vs) + at * (HD / GROUP)) + x);
-                        if (keys) raw.check |= poisoned(__ldg(reinterpret_cast<const uint16_t *>(a.pool.vs + at * (HD / GROUP)) + x));
+                        if (keys) raw.vs[u] = __ldg(reinterpret_cast<const uint16_t *>(a.pool.vs + at * (HD / GROUP)) + x);
                     }
                 }
             };
-            auto convert = [&](uint8_t *to, bool keys) {
+            auto convert = [&](const Raw &raw, uint8_t *to, bool keys) {
                 if (idle) return;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
@@ -340,33 +342,45 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 }
             };
             if (n == 0) continue;
-            // items: K0, K1, V0, K2, V1, .. V(n-1). The next one's bytes come while one is converted, a tile's page two
-            // items before them.
-            int p0 = page_of(0), p1 = -1, p2 = page_of(1);   // of the last keys' tile, the one before, the one behind
-            load(true, p0, 0);
-            for (int it = 0; it < 2 * n; it++) {
-                const bool keys = it == 0 || ((it & 1) && it < 2 * n - 1);
+            // items: K0, K1, V0, K2, V1, .. V(n-1). Two are on their way while one is converted; a tile's page comes before them.
+            int p0 = NONE, p1 = NONE, p2 = page_of(0);               // pages of the last keys' tile, the one before, the one behind
+            auto load_item = [&](Raw &raw, int m) {
+                if (m >= 2 * n) return;
+                if (m == 0 || ((m & 1) && m < 2 * n - 1)) {      // keys of tile (m + 1) / 2
+                    p1 = p0;
+                    p0 = p2;
+                    load(raw, true, p0, (m + 1) / 2);
+                    p2 = page_of((m + 1) / 2 + 1);
+                } else if (m == 2 * n - 1) {
+                    load(raw, false, p0, n - 1);
+                } else {
+                    load(raw, false, p1, m / 2 - 1);
+                }
+            };
+            auto item = [&](Raw &raw, int m) {
+                const bool keys = m == 0 || ((m & 1) && m < 2 * n - 1);
                 const uint32_t c = keys ? kc : vc, i = c & 1;
                 if (c > 1) wait_for((keys ? empty_k : empty_v) + i, ((c >> 1) - 1) & 1, &dead, a.err);
-                if (keys && raw.check) atomicOr(&bad[c & 3][tok >> 5], 1u << (tok & 31));
-                convert(smem + (keys ? 0 : C::V_OFF) + i * C::TILE, keys);
+                if (keys) {
+                    uint32_t poison = 0;
+#pragma unroll
+                    for (int u = 0; u < U; u++) poison |= poisoned(raw.vs[u]);
+                    if (poison) atomicOr(&bad[c & 3][tok >> 5], 1u << (tok & 31));
+                }
+                convert(raw, smem + (keys ? 0 : C::V_OFF) + i * C::TILE, keys);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive((keys ? full_k : full_v) + i);
                 if (keys) kc++;
                 else vc++;
-                const int nx = it + 1;
-                if (nx == 2 * n) break;
-                if ((nx & 1) && nx < 2 * n - 1) {            // keys of tile (nx + 1) / 2
-                    p1 = p0;
-                    p0 = p2;
-                    load(true, p0, (nx + 1) / 2);
-                    p2 = page_of((nx + 1) / 2 + 1);
-                } else if (nx == 2 * n - 1) {
-                    load(false, p0, n - 1);
-                } else {
-                    load(false, p1, nx / 2 - 1);
-                }
+                load_item(raw, m + 2);
+            };
+            Raw ra, rb;
+            load_item(ra, 0);
+            load_item(rb, 1);
+            for (int m = 0; m < 2 * n; m += 2) {
+                item(ra, m);
+                item(rb, m + 1);
             }
         }
     } else {
@@ -421,7 +435,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                         lo[i] = pack_f16(p - b.x, q - b.y);
                     }
                     if constexpr (TWO)
-                        *reinterpret_cast<uint4 *>(smem + C::Q_OFF + (c >> 1) * C::QCH + r * 128 + ((((c & 1) * 4 + y) ^ (r & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        *reinterpret_cast<uint4 *>(smem + C::Q_OFF + (c >> 1) * QCH + r * 128 + ((((c & 1) * 4 + y) ^ (r & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 __syncwarp();
                 tm_st16(mine + C::QC + 16 * c, hi);
@@ -442,41 +456,44 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 wait_for(s_full + i, (tc >> 1) & 1, &dead, a.err);
                 __syncwarp();
                 tc_after();
-                float s[N];
-                tm_ld32(mine + C::SC + i * N, s);
-                tm_ld32(mine + C::SC + i * N + 32, s + 32);
-                tm_wait_ld(s, N);
                 const int t0 = sg.start + (sg.k0 + j) * N;
+                const bool edge = __any_sync(0xffffffffu, t0 + N - 1 > row.pos || t0 <= row.low);
+                const uint32_t b0 = *(volatile uint32_t *)&bad[tc & 3][0], b1 = *(volatile uint32_t *)&bad[tc & 3][1];   // tokens with poisoned values
+                // 32 of the row's scores under a reference. They are read twice, for the largest and for the weights: 64 of
+                // them do not fit the registers beside the rest.
+                auto scores = [&](int c, float ref, float (&s)[32]) {
+                    tm_ld32(mine + C::SC + i * N + 32 * c, s);
+                    tm_wait_ld(s, 32);
+                    const f32x2 up2 = pack2(row.up, row.up), ref2 = pack2(-ref, -ref);
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2) {
+                        const float2 v = unpack2(fma2(pack2(s[x], s[x + 1]), up2, ref2));
+                        s[x] = v.x, s[x + 1] = v.y;
+                    }
+                    if (edge || (b0 | b1)) {
+                        const uint32_t flags = c ? b1 : b0;
+#pragma unroll
+                        for (int x = 0; x < 32; x++) {
+                            const int p = t0 + 32 * c + x;
+                            if (p > row.pos || p <= row.low) s[x] = -INFINITY;
+                            else if (flags >> x & 1) s[x] = NAN;
+                        }
+                    }
+                };
                 const float ref = m == -INFINITY ? 0.f : m;
-                const f32x2 up2 = pack2(row.up, row.up), ref2 = pack2(-ref, -ref);
-#pragma unroll
-                for (int x = 0; x < N; x += 2) {
-                    const float2 v = unpack2(fma2(pack2(s[x], s[x + 1]), up2, ref2));
-                    s[x] = v.x, s[x + 1] = v.y;
-                }
-                if (__any_sync(0xffffffffu, t0 + N - 1 > row.pos || t0 <= row.low)) {
-#pragma unroll
-                    for (int x = 0; x < N; x++)
-                        if (t0 + x > row.pos || t0 + x <= row.low) s[x] = -INFINITY;
-                }
-                const uint32_t b0 = *(volatile uint32_t *)&bad[tc & 3][0], b1 = *(volatile uint32_t *)&bad[tc & 3][1];
-                if (b0 | b1) {   // tokens with poisoned values
-#pragma unroll
-                    for (int x = 0; x < N; x++)
-                        if (((x < 32 ? b0 : b1) >> (x & 31) & 1) && t0 + x <= row.pos && t0 + x > row.low) s[x] = NAN;
-                    bar_sync(1, SM_WARPS * 32);
-                    if (tid < 2) bad[tc & 3][tid] = 0;
-                    __syncwarp();
-                }
                 float mx = -INFINITY;
 #pragma unroll
-                for (int x = 0; x < N; x += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(mx) : "f"(s[x]), "f"(s[x + 1]));
+                for (int c = 0; c < N / 32; c++) {
+                    float s[32], m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    scores(c, ref, s);
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(m4[x / 2 & 3]) : "f"(s[x]), "f"(s[x + 1]));
+                    mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                }
                 const bool move = mx > W_MAX || (m == -INFINITY && mx > -INFINITY);
                 if (__any_sync(0xffffffffu, move)) {
-                    const float delta = move ? mx - W_TOP : 0.f, f = m == -INFINITY ? 0.f : ex2(-delta);
+                    const float delta = move ? mx - C::TOP : 0.f, f = m == -INFINITY ? 0.f : ex2(-delta);
                     if (move) m = ref + delta;
-#pragma unroll
-                    for (int x = 0; x < N; x++) s[x] -= delta;
                     l0 *= f, l1 *= f;
                     if (j > 0) {   // what the outputs have so far, behind the products before
                         wait_for(pv_done + (i ^ 1), ((tc - 1) >> 1) & 1, &dead, a.err);
@@ -494,26 +511,40 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                         }
                     }
                 }
+                const float now = m == -INFINITY ? 0.f : m;
+                uint32_t hi[N / 32][16], lo[N / 32][16];   // the weights lie where the scores were: f32's second terms wait for the last of those
 #pragma unroll
                 for (int c = 0; c < N / 32; c++) {
-                    uint32_t hi[16], lo[16];
+                    float s[32];
+                    scores(c, now, s);
 #pragma unroll
                     for (int x = 0; x < 16; x++) {
-                        const float p = ex2(s[32 * c + 2 * x]), q = ex2(s[32 * c + 2 * x + 1]);
-                        hi[x] = pack_f16(p, q);
+                        const float p = ex2(s[2 * x]), q = ex2(s[2 * x + 1]);
+                        hi[c][x] = pack_f16(p, q);
                         if constexpr (__is_same(T, __nv_bfloat16)) l0 += p, l1 += q;   // f16's rounding is beneath bf16's
                         else {
-                            const float2 b = unpack_f16(hi[x]);
+                            const float2 b = unpack_f16(hi[c][x]);
                             if constexpr (TWO) {
-                                lo[x] = pack_f16(p - b.x, q - b.y);
+                                lo[c][x] = pack_f16(p - b.x, q - b.y);
                                 l0 += p, l1 += q;
                             } else {
                                 l0 += b.x, l1 += b.y;
                             }
                         }
                     }
-                    tm_st16(mine + C::SC + i * N + 16 * c, hi);
-                    if constexpr (TWO) tm_st16(mine + C::SC + i * N + N / 2 + 16 * c, lo);
+                    if constexpr (!TWO) tm_st16(mine + C::SC + i * N + 16 * c, hi[c]);
+                }
+                if constexpr (TWO) {
+#pragma unroll
+                    for (int c = 0; c < N / 32; c++) {
+                        tm_st16(mine + C::SC + i * N + 16 * c, hi[c]);
+                        tm_st16(mine + C::SC + i * N + N / 2 + 16 * c, lo[c]);
+                    }
+                }
+                if (b0 | b1) {
+                    bar_sync(1, SM_WARPS * 32);
+                    if (tid < 2) bad[tc & 3][tid] = 0;
+                    __syncwarp();
                 }
                 tm_wait_st();
                 tc_before();

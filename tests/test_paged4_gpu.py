@@ -9,8 +9,9 @@ Attention reads the cache exactly (a value is an f16 number). Its error, against
 rounding (f16: 2^-12 each, the sum that divides by them rounded alike, so 2^-11 together; f32: two terms, 2^-22), the scores' f32 sums and their
 queries' rounding (f16 rows exact, bf16 rows exact above 2^-24 of the largest, f32 rows 2^-22 of the largest): 2^-20 S with S the largest sum_d |q_d k_d|
 scale of the row, the sums of the outputs, which the tensor cores cut towards 0: 2^-22 for each of at most 64 + n / 64 additions; and the output type's half unit. With the
-gate's exponential and the division 2^-20 more. Weights are f16 numbers, the largest between 2^12 and 2^15, so a small one is off by half of f16's
-last bit, 2^-25, which is 2^-37 of the largest: 2^-37 max p sum_j |V_j| besides."""
+gate's exponential and the division 2^-20 more. Weights are f16 numbers, the largest between 2^12 and 2^15 (many rows
+of a sequence: 2^10, and 2^6 for 16-bit rows), so a small one is off by half of f16's last bit, 2^-25, which is 2^-37 (2^-35, 2^-31) of the
+largest: that times max p sum_j |V_j| besides."""
 import numpy as np
 import pytest
 
@@ -349,7 +350,7 @@ def want_attention(c, q, window=0, gate=None, scale=0.0):
         S = size.masked_fill(hide, 0).nan_to_num().amax(-1, keepdim=True)
         t = W * ((2.0 ** -21 if two else 2.0 ** -11) + 2.0 ** -20 * S + 2.0 ** -22 * (64 + L / 64) + 2.0 ** -20)
         seen = torch.einsum("nj,kjd->nkd", see.double(), vs.nan_to_num().abs())
-        t = t + 2.0 ** -37 * p.amax(-1, keepdim=True) * seen[:, :, None]
+        t = t + (2.0 ** -35 if two else 2.0 ** -31) * p.amax(-1, keepdim=True) * seen[:, :, None]
         out.append(o.reshape(n, c.heads, c.hd))
         tol.append(t.reshape(n, c.heads, c.hd))
         at += n
