@@ -28,6 +28,7 @@ constexpr int R = WIDE_R;
 constexpr int QCH = R * 128;                            // 64 dims of the queries' second terms
 constexpr int SM_WARPS = 4, DQ_WARPS = 8, MMA_WARP = SM_WARPS + DQ_WARPS, WARPS = MMA_WARP + 1, THREADS = WARPS * 32;
 constexpr int COST = 32;                                // a group's fixed cost in blocks
+constexpr int RUN = 16, MAX_CTAS = 512;                 // parts that are added together (a join takes 32); CTAs of a call
 constexpr int NONE = INT_MIN;                           // no page
 
 template <typename T_, int HD_>
@@ -41,9 +42,10 @@ struct Cfg {
     static constexpr int TILE = N * HD * 2;             // bytes of a tile's keys (or values) in f16
     static constexpr int CH = N * 128;                  // 64 dims of them
     static constexpr int V_OFF = 2 * TILE, Q_OFF = 4 * TILE;
-    static constexpr size_t SMEM = Q_OFF + (TWO ? R * HD * 2 : 0) + 1024;
-    static constexpr int PARTS = HD / 32;               // a thread's shares of a token
-    static constexpr int UNITS = N * PARTS / (DQ_WARPS * 32);   // shares of a thread (0: half of the threads have one)
+    static constexpr int STG_OFF = Q_OFF + (TWO ? R * HD * 2 : 0);   // 4 KB a softmax warp: rows of 128 bytes between their owners and global memory
+    static constexpr size_t SMEM = STG_OFF + SM_WARPS * 4096 + 1024;
+    static constexpr int PIECES = HD / 32;              // 16-byte pieces of a token's codes
+    static constexpr int U = N * PIECES > DQ_WARPS * 32 ? N * PIECES / (DQ_WARPS * 32) : 1;   // pieces of a thread
     static constexpr int QC = HD, SC = HD + HD / 2;     // columns of tensor memory: outputs 0.., queries, scores
     static constexpr int TCOLS = SC + 2 * N <= 256 ? 256 : 512;
 };
@@ -133,6 +135,73 @@ struct Row {
     int pos, low;                                       // it sees the tokens (low, pos]
     long long out;                                      // where its output lies (-1: no row)
 };
+
+// The sum of n parts (32 at most) of the group that begins at CTA f0, `step` apart from part `at` on, by the softmax warps: to the outputs, or to the first
+// one's place, which this CTA alone reads. wt: 16 KB.
+template <typename C>
+__device__ __noinline__ void join(const AttnParams &a, int f0, int rows, float *wt, const float *sig_s, const long long *out_s, int at, int step, int n, bool done, int ovec) {
+    using T = typename C::T;
+    constexpr int HD = C::HD;
+    const int tid = threadIdx.x;
+    auto part = [&](int p) { return a.part + ((size_t)(f0 + p) * 2 + (p == 0)) * part_floats(R, HD); };   // CTA f0: its second slot, the others: the first
+    if (tid < rows) {   // the parts' weights, [n][R]
+        float M = -INFINITY, L = 0.f;
+#pragma unroll 4
+        for (int p = 0; p < n; p++) {
+            const float m = __ldcg(part(at + step * p) + R * HD + tid);
+            wt[p * R + tid] = m;
+            M = fmaxf(M, m);
+        }
+#pragma unroll 4
+        for (int p = 0; p < n; p++) {
+            const float m = wt[p * R + tid], l = __ldcg(part(at + step * p) + R * HD + R + tid), f = m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(m - M);
+            wt[p * R + tid] = f;
+            L += m == -INFINITY ? l : l * f;
+        }
+        if (done) {
+            const float fo = L == 0.f ? 0.f : sig_s[tid] / L;
+            for (int p = 0; p < n; p++) wt[p * R + tid] = L == 0.f ? 0.f : wt[p * R + tid] * fo;
+        } else {
+            float *to = part(at) + R * HD;
+            __stcg(to + tid, M);
+            __stcg(to + R + tid, L);
+        }
+    }
+    bar_sync(1, SM_WARPS * 32);
+    const int items = rows * (HD / 4);                   // of 4 values
+    for (int x0 = tid; x0 < items; x0 += 4 * SM_WARPS * 32) {
+        float4 o[4] = {};
+        for (int p = 0; p < n; p++) {
+            const float *src = part(at + step * p);
+            float4 v[4];
+#pragma unroll
+            for (int y = 0; y < 4; y++) v[y] = __ldcg(reinterpret_cast<const float4 *>(src) + min(x0 + y * SM_WARPS * 32, items - 1));
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const float f = wt[p * R + min(x0 + y * SM_WARPS * 32, items - 1) / (HD / 4)];
+                if (f == 0.f) continue;                  // nothing seen, or nothing to say
+                o[y].x = fmaf(v[y].x, f, o[y].x), o[y].y = fmaf(v[y].y, f, o[y].y), o[y].z = fmaf(v[y].z, f, o[y].z), o[y].w = fmaf(v[y].w, f, o[y].w);
+            }
+        }
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+            const int x = x0 + y * SM_WARPS * 32;
+            if (x >= items) break;
+            if (!done) __stcg(reinterpret_cast<float4 *>(part(at)) + x, o[y]);
+            else {
+                T *dst = (T *)a.out + out_s[x / (HD / 4)] + 4 * (x % (HD / 4));
+                T t[4] = {from_f32<T>(o[y].x), from_f32<T>(o[y].y), from_f32<T>(o[y].z), from_f32<T>(o[y].w)};
+                if (ovec) {
+                    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(t);
+                    else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(t);
+                } else {
+#pragma unroll
+                    for (int z = 0; z < 4; z++) dst[z] = t[z];
+                }
+            }
+        }
+    }
+}
 
 template <typename C>
 __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, const int qvec, const int ovec) {
@@ -282,90 +351,112 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             groups++;
         }
     } else if (warp >= SM_WARPS) {
-        // codes to f16. Thread: token `tok` of a tile, 32 dims `part` (and `part` + 4 at heads of 256)
-        const int dt = tid - SM_WARPS * 32, tok = dt % N, part = dt / N, per = a.pool.page_tokens / BLOCK;
-        constexpr int U = C::UNITS > 0 ? C::UNITS : 1;
-        const bool idle = part >= C::PARTS;
+        // codes to f16. A thread's piece is 32 dims of a token, the next thread's the next 32, so that a warp's loads lie side by side;
+        // at heads of 256 it has a second one, 32 tokens on.
+        constexpr int U = C::U, PIECES = C::PIECES;
+        const int dt = tid - SM_WARPS * 32, x = dt % PIECES, tok0 = dt / PIECES, per = a.pool.page_tokens / BLOCK;
+        const bool idle = tok0 >= N;
+        // Which of its four 16-byte results a thread stores first: eight neighbours then meet all banks
+        const int turn = HD == 256 ? x >> 1 : HD == 128 ? 2 * (x >> 1) : 0;
+        const int per_tile = TB / per, per_rest = TB % per;
         uint32_t kc = 0, vc = 0;
         for (; sg.k0 >= 0; next(sg)) {
             const int n = tiles_of(sg);
             const int *table = a.b.table + (size_t)sg.s * a.b.max_pages;
-            // the page of the thread's token of tile j, as the table has it; NONE where no row sees the token
-            auto page_of = [&](int j) {
-                const int blk = (sg.k0 + j) * TB + tok / BLOCK, at = sg.start + (sg.k0 + j) * N + tok;
-                return j >= n || blk >= sg.nblk || at < sg.see0 || at > sg.p_hi ? NONE : __ldg(table + (sg.start / BLOCK + blk) / per);
+            // A token's place: its page as the table has it (NONE where no row sees it) and its token of the page
+            struct Place {
+                int page[U], tok[U];
             };
-            auto row_of = [&](int page, int j) {
-                const int blk = sg.start / BLOCK + (sg.k0 + j) * TB + tok / BLOCK;
-                return row_index(a.pool, page, sg.kvh, blk % per * BLOCK + tok % BLOCK);
+            int at_j = 0, idx[U], rest[U];                       // the next tile to be looked up; its blocks' pages of the table, blocks of those
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int blk = sg.start / BLOCK + sg.k0 * TB + (tok0 + 32 * u) / BLOCK;
+                idx[u] = blk / per;
+                rest[u] = blk % per;
+            }
+            auto look_up = [&](Place &pl) {
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int at = sg.start + (sg.k0 + at_j) * N + tok0 + 32 * u;
+                    pl.page[u] = idle || at_j >= n || at < sg.see0 || at > sg.p_hi ? NONE : __ldg(table + idx[u]);
+                    pl.tok[u] = rest[u] * BLOCK + tok0 % BLOCK;
+                    idx[u] += per_tile;
+                    rest[u] += per_rest;
+                    if (rest[u] >= per) rest[u] -= per, idx[u]++;
+                }
+                at_j++;
             };
             struct Raw {
                 uint4 c[U];
                 uint32_t s[U], vs[U];            // vs, beside keys: their tokens' scales of values, looked at for poison
             };
-            auto load = [&](Raw &raw, bool keys, int page, int j) {
+            auto load = [&](Raw &raw, bool keys, const Place &pl) {
 #pragma unroll
-                for (int u = 0; u < U; u++) raw.c[u] = make_uint4(0, 0, 0, 0), raw.s[u] = raw.vs[u] = 0;
-                const bool seen = page != NONE, there = page >= 0 && page < a.pool.pages;
-                if (seen && !there && a.err) atomicExch(a.err, DEV_BAD_INDEX);
-                if (there && !idle) {
-                    const size_t at = row_of(page, j);
-#pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        const int x = part + 4 * u;
+                for (int u = 0; u < U; u++) {
+                    raw.c[u] = make_uint4(0, 0, 0, 0), raw.s[u] = raw.vs[u] = 0;
+                    const bool there = pl.page[u] >= 0 && pl.page[u] < a.pool.pages;
+                    if (there) {
+                        const size_t at = row_index(a.pool, pl.page[u], sg.kvh, pl.tok[u]);
                         raw.c[u] = __ldg(reinterpret_cast<const uint4 *>((keys ? a.pool.k : a.pool.v) + at * (HD / 2)) + x);
                         raw.s[u] = __ldg(reinterpret_cast<const uint16_t *>((keys ? a.pool.ks : a.pool.vs) + at * (HD / GROUP)) + x);
                         if (keys) raw.vs[u] = __ldg(reinterpret_cast<const uint16_t *>(a.pool.vs + at * (HD / GROUP)) + x);
-                    }
+                    } else if (pl.page[u] != NONE && a.err) atomicExch(a.err, DEV_BAD_INDEX);
                 }
             };
             auto convert = [&](const Raw &raw, uint8_t *to, bool keys) {
                 if (idle) return;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    const int x = part + 4 * u;
+                    const int tok = tok0 + 32 * u;
                     uint32_t s2 = raw.s[u];
                     if (!keys) {   // poisoned values become 0: their tokens' weights say NaN where they are seen
                         if ((s2 & 0xff) >= POISON) s2 &= 0xff00;
                         if ((s2 >> 8) >= POISON) s2 &= 0x00ff;
                     }
-                    const uint32_t sc[2] = {(s2 & 0xff) * 0x00800080u, (s2 >> 8) * 0x00800080u};
-                    const uint32_t wd[4] = {raw.c[u].x, raw.c[u].y, raw.c[u].z, raw.c[u].w};
+                    uint32_t wd[4] = {raw.c[u].x, raw.c[u].y, raw.c[u].z, raw.c[u].w}, sc[2] = {(s2 & 0xff) * 0x00800080u, (s2 >> 8) * 0x00800080u};
+                    if (HD == 256 && (turn & 1)) {
+                        const uint32_t w0 = wd[0];
+                        wd[0] = wd[1], wd[1] = wd[2], wd[2] = wd[3], wd[3] = w0;
+                    }
+                    if (HD >= 128 && (turn & 2)) {
+                        const uint32_t w0 = wd[0], w1 = wd[1], s0 = sc[0];
+                        wd[0] = wd[2], wd[1] = wd[3], wd[2] = w0, wd[3] = w1;
+                        sc[0] = sc[1], sc[1] = s0;
+                    }
                     uint8_t *row = to + (x >> 1) * C::CH + tok * 128;
 #pragma unroll
-                    for (int y = 0; y < 4; y++) {
+                    for (int y = 0; y < 4; y++) {   // result (y + turn) % 4; its scale is the piece's first or second
+                        const int z = (y + turn) & 3;
+                        const uint32_t scale = HD == 256 && (y & 1) ? ((turn & 1) ? sc[(y >> 1) ^ 1] : sc[y >> 1]) : sc[y >> 1];
                         uint32_t h[4];
                         codes_f16(wd[y], h);
-                        const uint4 v = make_uint4(hmul2(h[0], sc[y >> 1]), hmul2(h[1], sc[y >> 1]), hmul2(h[2], sc[y >> 1]), hmul2(h[3], sc[y >> 1]));
-                        *reinterpret_cast<uint4 *>(row + ((((x & 1) * 4 + y) ^ (tok & 7)) << 4)) = v;
+                        const uint4 v = make_uint4(hmul2(h[0], scale), hmul2(h[1], scale), hmul2(h[2], scale), hmul2(h[3], scale));
+                        *reinterpret_cast<uint4 *>(row + ((((x & 1) * 4 + z) ^ (tok & 7)) << 4)) = v;
                     }
                 }
             };
             if (n == 0) continue;
             // items: K0, K1, V0, K2, V1, .. V(n-1). Two are on their way while one is converted; a tile's page comes before them.
-            int p0 = NONE, p1 = NONE, p2 = page_of(0);               // pages of the last keys' tile, the one before, the one behind
+            Place p0, p1, p2;                                    // of the last keys' tile, the one before, the one behind
+            look_up(p2);
+            p0 = p2;
             auto load_item = [&](Raw &raw, int m) {
                 if (m >= 2 * n) return;
                 if (m == 0 || ((m & 1) && m < 2 * n - 1)) {      // keys of tile (m + 1) / 2
                     p1 = p0;
                     p0 = p2;
-                    load(raw, true, p0, (m + 1) / 2);
-                    p2 = page_of((m + 1) / 2 + 1);
-                } else if (m == 2 * n - 1) {
-                    load(raw, false, p0, n - 1);
-                } else {
-                    load(raw, false, p1, m / 2 - 1);
-                }
+                    load(raw, true, p0);
+                    look_up(p2);
+                } else load(raw, false, m == 2 * n - 1 ? p0 : p1);
             };
             auto item = [&](Raw &raw, int m) {
                 const bool keys = m == 0 || ((m & 1) && m < 2 * n - 1);
                 const uint32_t c = keys ? kc : vc, i = c & 1;
                 if (c > 1) wait_for((keys ? empty_k : empty_v) + i, ((c >> 1) - 1) & 1, &dead, a.err);
                 if (keys) {
-                    uint32_t poison = 0;
 #pragma unroll
-                    for (int u = 0; u < U; u++) poison |= poisoned(raw.vs[u]);
-                    if (poison) atomicOr(&bad[c & 3][tok >> 5], 1u << (tok & 31));
+                    for (int u = 0; u < U; u++)
+                        if (poisoned(raw.vs[u])) atomicOr(&bad[c & 3][(tok0 + 32 * u) >> 5], 1u << ((tok0 + 32 * u) & 31));
                 }
                 convert(raw, smem + (keys ? 0 : C::V_OFF) + i * C::TILE, keys);
                 fence_proxy_async();
@@ -389,56 +480,76 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
         __shared__ float sig_s[R];
         __shared__ long long out_s[R];
         uint32_t tc = 0, groups = 0;
+        uint8_t *stg = smem + C::STG_OFF + warp * 4096;               // 32 rows of 128 bytes, 16-byte pieces spread as their row says
+        const uint32_t own = lane * 128, cut = lane & 7;              // this thread's row of them
         // the row of a group that is this thread's, its queries to where the MMAs read them
         auto queries = [&](const Seg &g) {
             Row row{0.f, 1.f, -1, -1, -1};
             if (g.k0 < 0) return row;
-            const int col = g.c0 + r, tok = col / a.group, h = g.kvh * a.group + col % a.group;
-            const bool real = col <= g.c1;
-            const T *src = (const T *)a.q + (long long)(g.r0 + tok) * a.ldq + (long long)h * HD;
-            if (real) {
+            const int col = g.c0 + r, tok = col / a.group, h = g.kvh * a.group + col % a.group, rows = g.c1 - g.c0 + 1 - 32 * warp;   // of this warp
+            const long long src = (long long)(g.r0 + tok) * a.ldq + (long long)h * HD;
+            if (col <= g.c1) {
                 row.pos = g.pos0 + tok;
                 row.low = a.window > 0 ? row.pos - a.window : -1;
                 row.out = (long long)(g.r0 + tok) * a.ldout + (long long)h * HD;
                 if (a.gate) row.sig = 1.0f / (1.0f + __expf(-to_f32<T>(((const T *)a.gate)[(long long)(g.r0 + tok) * a.ldgate + h])));
             }
             if (tiles_of(g) == 0) return row;
+            // the rows' largest: HD / 8 lanes a row
+            constexpr int LPR = HD / 8, GH = 32 / LPR;
             float mx = 0.f;
-            if (real)
 #pragma unroll 4
-                for (int d = 0; d < HD; d += 8) {
+            for (int it = 0; it < LPR; it++) {
+                const int rr = it * GH + lane / LPR;
+                const long long at = __shfl_sync(0xffffffffu, src, rr);
+                float y = 0.f;
+                if (rr < rows) {
                     float x[8];
-                    row8<T>(src + d, qvec, x);
+                    row8<T>((const T *)a.q + at + 8 * (lane % LPR), qvec, x);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]));
+                    for (int i = 0; i < 8; i++) y = fmaxf(y, fabsf(x[i]));
                 }
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
+                y = __shfl_sync(0xffffffffu, y, (lane % GH) * LPR);
+                if (lane / GH == it) mx = y;
+            }
             const int e = mx > 0.f && mx < INFINITY ? min(14 - ilogbf(mx), 126) : 0;   // 2^e brings the largest into [2^14, 2^15)
             const float f = __int_as_float((e + 127) << 23);
             row.up = a.scale * __int_as_float((127 - e) << 23);
-#pragma unroll 2
-            for (int c = 0; c < HD / 32; c++) {
-                uint32_t hi[16];
-#pragma unroll
-                for (int y = 0; y < 4; y++) {
+            for (int c = 0; c < HD / 64; c++) {
+#pragma unroll 4
+                for (int it = 0; it < 8; it++) {
+                    const int rr = 4 * it + lane / 8, pc = lane % 8;
+                    const long long at = __shfl_sync(0xffffffffu, src, rr);
+                    const float fr = __shfl_sync(0xffffffffu, f, rr);
                     float x[8];
-                    if (real) row8<T>(src + 32 * c + 8 * y, qvec, x);
+                    if (rr < rows) row8<T>((const T *)a.q + at + 64 * c + 8 * pc, qvec, x);
                     else {
 #pragma unroll
                         for (int i = 0; i < 8; i++) x[i] = 0.f;
                     }
-                    uint32_t lo[4];
+                    uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float p = x[2 * i] * f, q = x[2 * i + 1] * f;
-                        hi[4 * y + i] = pack_f16(p, q);
-                        const float2 b = unpack_f16(hi[4 * y + i]);
+                        const float p = x[2 * i] * fr, q = x[2 * i + 1] * fr;
+                        hi[i] = pack_f16(p, q);
+                        const float2 b = unpack_f16(hi[i]);
                         lo[i] = pack_f16(p - b.x, q - b.y);
                     }
-                    if constexpr (TWO)
-                        *reinterpret_cast<uint4 *>(smem + C::Q_OFF + (c >> 1) * QCH + r * 128 + ((((c & 1) * 4 + y) ^ (r & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    const uint32_t to = rr * 128 + ((pc ^ (rr & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(stg + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (TWO) *reinterpret_cast<uint4 *>(smem + C::Q_OFF + c * QCH + warp * 4096 + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 __syncwarp();
-                tm_st16(mine + C::QC + 16 * c, hi);
+                uint32_t w[32];
+#pragma unroll
+                for (int y = 0; y < 8; y++) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(stg + own + ((y ^ cut) << 4));
+                    w[4 * y] = v.x, w[4 * y + 1] = v.y, w[4 * y + 2] = v.z, w[4 * y + 3] = v.w;
+                }
+                __syncwarp();
+                tm_st32(mine + C::QC + 32 * c, w);
             }
             tm_wait_st();
             tc_before();
@@ -459,37 +570,57 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 const int t0 = sg.start + (sg.k0 + j) * N;
                 const bool edge = __any_sync(0xffffffffu, t0 + N - 1 > row.pos || t0 <= row.low);
                 const uint32_t b0 = *(volatile uint32_t *)&bad[tc & 3][0], b1 = *(volatile uint32_t *)&bad[tc & 3][1];   // tokens with poisoned values
-                // 32 of the row's scores under a reference. They are read twice, for the largest and for the weights: 64 of
-                // them do not fit the registers beside the rest.
-                auto scores = [&](int c, float ref, float (&s)[32]) {
-                    tm_ld32(mine + C::SC + i * N + 32 * c, s);
-                    tm_wait_ld(s, 32);
+                // The weights under the reference as it stands, and the largest score. Where one is too large (and at a group's start) the
+                // reference moves, and they are taken again from the scores, which lie there until the weights are stored.
+                uint32_t hi[N / 32][16], lo[N / 32][16];
+                float d0, d1;
+                auto weigh = [&](float ref) {
+                    float most = -INFINITY;
+                    f32x2 sum = pack2(0.f, 0.f);
                     const f32x2 up2 = pack2(row.up, row.up), ref2 = pack2(-ref, -ref);
 #pragma unroll
-                    for (int x = 0; x < 32; x += 2) {
-                        const float2 v = unpack2(fma2(pack2(s[x], s[x + 1]), up2, ref2));
-                        s[x] = v.x, s[x + 1] = v.y;
-                    }
-                    if (edge || (b0 | b1)) {
-                        const uint32_t flags = c ? b1 : b0;
+                    for (int c = 0; c < N / 32; c++) {
+                        float s[32], m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        tm_ld32(mine + C::SC + i * N + 32 * c, s);
+                        tm_wait_ld(s, 32);
 #pragma unroll
-                        for (int x = 0; x < 32; x++) {
-                            const int p = t0 + 32 * c + x;
-                            if (p > row.pos || p <= row.low) s[x] = -INFINITY;
-                            else if (flags >> x & 1) s[x] = NAN;
+                        for (int x = 0; x < 32; x += 2) {
+                            const float2 v = unpack2(fma2(pack2(s[x], s[x + 1]), up2, ref2));
+                            s[x] = v.x, s[x + 1] = v.y;
                         }
+                        if (edge || (b0 | b1)) {
+                            const uint32_t flags = c ? b1 : b0;
+#pragma unroll
+                            for (int x = 0; x < 32; x++) {
+                                const int p = t0 + 32 * c + x;
+                                if (p > row.pos || p <= row.low) s[x] = -INFINITY;
+                                else if (flags >> x & 1) s[x] = NAN;
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < 32; x += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(m4[x / 2 & 3]) : "f"(s[x]), "f"(s[x + 1]));
+#pragma unroll
+                        for (int x = 0; x < 16; x++) {
+                            const float p = ex2(s[2 * x]), q = ex2(s[2 * x + 1]);
+                            hi[c][x] = pack_f16(p, q);
+                            if constexpr (__is_same(T, __nv_bfloat16)) sum = add2(sum, pack2(p, q));   // f16's rounding is beneath bf16's
+                            else {
+                                const float2 b = unpack_f16(hi[c][x]);
+                                if constexpr (TWO) {
+                                    lo[c][x] = pack_f16(p - b.x, q - b.y);
+                                    sum = add2(sum, pack2(p, q));
+                                } else {
+                                    sum = add2(sum, pack2(b.x, b.y));
+                                }
+                            }
+                        }
+                        most = fmaxf(most, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
                     }
+                    const float2 v = unpack2(sum);
+                    d0 = v.x, d1 = v.y;
+                    return most;
                 };
-                const float ref = m == -INFINITY ? 0.f : m;
-                float mx = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < N / 32; c++) {
-                    float s[32], m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    scores(c, ref, s);
-#pragma unroll
-                    for (int x = 0; x < 32; x += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(m4[x / 2 & 3]) : "f"(s[x]), "f"(s[x + 1]));
-                    mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-                }
+                const float ref = m == -INFINITY ? 0.f : m, mx = weigh(ref);
                 const bool move = mx > W_MAX || (m == -INFINITY && mx > -INFINITY);
                 if (__any_sync(0xffffffffu, move)) {
                     const float delta = move ? mx - C::TOP : 0.f, f = m == -INFINITY ? 0.f : ex2(-delta);
@@ -510,29 +641,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                             tm_st32(mine + 32 * c, u);
                         }
                     }
+                    weigh(m == -INFINITY ? 0.f : m);
                 }
-                const float now = m == -INFINITY ? 0.f : m;
-                uint32_t hi[N / 32][16], lo[N / 32][16];   // the weights lie where the scores were: f32's second terms wait for the last of those
+                l0 += d0, l1 += d1;
+                if constexpr (!TWO) {
 #pragma unroll
-                for (int c = 0; c < N / 32; c++) {
-                    float s[32];
-                    scores(c, now, s);
-#pragma unroll
-                    for (int x = 0; x < 16; x++) {
-                        const float p = ex2(s[2 * x]), q = ex2(s[2 * x + 1]);
-                        hi[c][x] = pack_f16(p, q);
-                        if constexpr (__is_same(T, __nv_bfloat16)) l0 += p, l1 += q;   // f16's rounding is beneath bf16's
-                        else {
-                            const float2 b = unpack_f16(hi[c][x]);
-                            if constexpr (TWO) {
-                                lo[c][x] = pack_f16(p - b.x, q - b.y);
-                                l0 += p, l1 += q;
-                            } else {
-                                l0 += b.x, l1 += b.y;
-                            }
-                        }
-                    }
-                    if constexpr (!TWO) tm_st16(mine + C::SC + i * N + 16 * c, hi[c]);
+                    for (int c = 0; c < N / 32; c++) tm_st16(mine + C::SC + i * N + 16 * c, hi[c]);
                 }
                 if constexpr (TWO) {
 #pragma unroll
@@ -565,6 +679,29 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 tc_after();
             }
             const float f = !whole ? 1.0f : l == 0.f ? 0.f : row.sig / l;
+            const int mrows = sg.c1 - sg.c0 + 1 - 32 * warp;          // rows of this warp
+            // 32 columns of outputs at a time; rows leave by 16-byte pieces, eight lanes a row
+            auto leave = [&](uint8_t *base, long long to, int size, int c, bool vec) {   // a row's 128 bytes, from byte `to` + 128 c of base on
+                __syncwarp();
+#pragma unroll
+                for (int it = 0; it < 8; it++) {
+                    const int rr = 4 * it + lane / 8, pc = lane % 8;
+                    const long long at = __shfl_sync(0xffffffffu, to, rr);
+                    const uint4 v = *reinterpret_cast<const uint4 *>(stg + rr * 128 + ((pc ^ (rr & 7)) << 4));
+                    if (rr >= mrows) continue;
+                    uint8_t *dst = base + at + 128 * c + 16 * pc;
+                    if (vec) *reinterpret_cast<uint4 *>(dst) = v;
+                    else if (size == 4) {
+                        reinterpret_cast<uint32_t *>(dst)[0] = v.x, reinterpret_cast<uint32_t *>(dst)[1] = v.y;
+                        reinterpret_cast<uint32_t *>(dst)[2] = v.z, reinterpret_cast<uint32_t *>(dst)[3] = v.w;
+                    } else {
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int y = 0; y < 8; y++) reinterpret_cast<uint16_t *>(dst)[y] = (uint16_t)(w[y >> 1] >> (16 * (y & 1)));
+                    }
+                }
+                __syncwarp();
+            };
 #pragma unroll 1
             for (int c = 0; c < HD / 32; c++) {
                 float o[32];
@@ -573,32 +710,22 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                     tm_ld32(mine + 32 * c, o);
                     tm_wait_ld(o, 32);
                 }
-                if (!real) continue;
 #pragma unroll
                 for (int x = 0; x < 32; x++) o[x] = n == 0 || l == 0.f ? 0.f : o[x] * f;
-                if (!whole) {
+                if (!whole || sizeof(T) == 4) {
 #pragma unroll
-                    for (int x = 0; x < 32; x += 4) *reinterpret_cast<float4 *>(slot + (size_t)r * HD + 32 * c + x) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
-                } else {
-                    T *dst = (T *)a.out + row.out + 32 * c;
-                    if constexpr (sizeof(T) == 4) {
-                        if (ovec) {
+                    for (int y = 0; y < 8; y++) *reinterpret_cast<float4 *>(stg + own + ((y ^ cut) << 4)) = make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
+                    if (!whole) leave((uint8_t *)slot, (long long)r * HD * 4, 4, c, true);
+                    else leave((uint8_t *)a.out, row.out * 4, 4, c, ovec);
+                } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                            for (int x = 0; x < 32; x += 4) *reinterpret_cast<float4 *>(dst + x) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
-                            continue;
-                        }
-                    } else if (ovec) {
+                    for (int y = 0; y < 4; y++) {
+                        T v[8];
 #pragma unroll
-                        for (int x = 0; x < 32; x += 8) {
-                            T v[8];
-#pragma unroll
-                            for (int y = 0; y < 8; y++) v[y] = from_f32<T>(o[x + y]);
-                            *reinterpret_cast<uint4 *>(dst + x) = *reinterpret_cast<const uint4 *>(v);
-                        }
-                        continue;
+                        for (int z = 0; z < 8; z++) v[z] = from_f32<T>(o[8 * y + z]);
+                        *reinterpret_cast<uint4 *>(stg + own + (((4 * (c & 1) + y) ^ cut) << 4)) = *reinterpret_cast<const uint4 *>(v);
                     }
-#pragma unroll
-                    for (int x = 0; x < 32; x++) dst[x] = from_f32<T>(o[x]);
+                    if (c & 1) leave((uint8_t *)a.out, row.out * 2, 2, c >> 1, ovec);
                 }
             }
             if (n > 0) {
@@ -607,45 +734,36 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 if (lane == 0) mbar_arrive(&o_free);
                 groups++;
             }
-            if (!whole) {   // the last CTA of the group adds all parts in CTA order
-                const int parts = sg.f1 - sg.f0 + 1, rows = sg.c1 - sg.c0 + 1;
+            if (!whole) {
+                // parts are added in CTA order; many of them in two steps (paged4_attn.cu)
+                const int parts = sg.f1 - sg.f0 + 1, mine_p = (int)blockIdx.x - sg.f0, runs = parts > 2 * RUN ? (parts + RUN - 1) / RUN : 1;
                 if (real) {
                     slot[R * HD + r] = l == 0.f ? -INFINITY : m;
                     slot[R * HD + R + r] = l;
                 }
                 sig_s[r] = row.sig;
                 out_s[r] = row.out;
-                bar_sync(1, SM_WARPS * 32);
-                if (tid == 0) {
-                    __threadfence();   // for all of them: their stores came before the barrier
-                    const bool last = atomicAdd(a.tickets + sg.f0, 1u) == (unsigned)(parts - 1);
-                    if (last) a.tickets[sg.f0] = 0u;
-                    __threadfence();
-                    last_s = last;
-                }
-                bar_sync(1, SM_WARPS * 32);
-                if (last_s) {
-                    const size_t step = (size_t)2 * part_floats(R, HD);
-                    const float *p0 = a.part + (size_t)sg.f0 * step;   // CTA f0: slot 1, the others: slot 0
-                    auto part = [&](int p) { return p0 + p * step + (p == 0 ? part_floats(R, HD) : 0); };
-                    for (int x = tid; x < rows * (HD / 4); x += SM_WARPS * 32) {
-                        const int rr = x / (HD / 4), d = 4 * (x % (HD / 4));
-                        float M = -INFINITY, L = 0.f;
-                        for (int p = 0; p < parts; p++) M = fmaxf(M, __ldcg(part(p) + R * HD + rr));
-                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                        for (int p = 0; p < parts; p++) {
-                            const float mp = __ldcg(part(p) + R * HD + rr), lp = __ldcg(part(p) + R * HD + R + rr);
-                            const float fp = mp == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(mp - M);
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(p) + rr * HD + d));
-                            L = mp == -INFINITY ? L + lp : fmaf(lp, fp, L);
-                            o.x = fmaf(v.x, fp, o.x), o.y = fmaf(v.y, fp, o.y), o.z = fmaf(v.z, fp, o.z), o.w = fmaf(v.w, fp, o.w);
-                        }
-                        const float fo = L == 0.f ? 0.f : sig_s[rr] / L;
-                        T *dst = (T *)a.out + out_s[rr] + d;
-                        dst[0] = from_f32<T>(L == 0.f ? 0.f : o.x * fo);
-                        dst[1] = from_f32<T>(L == 0.f ? 0.f : o.y * fo);
-                        dst[2] = from_f32<T>(L == 0.f ? 0.f : o.z * fo);
-                        dst[3] = from_f32<T>(L == 0.f ? 0.f : o.w * fo);
+                auto last_of = [&](unsigned int *ticket, int count) {
+                    bar_sync(1, SM_WARPS * 32);
+                    if (tid == 0) {
+                        unsigned int was;
+                        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(was) : "l"(ticket) : "memory");
+                        const bool last = was == (unsigned)(count - 1);
+                        if (last) *ticket = 0u;
+                        last_s = last;
+                    }
+                    bar_sync(1, SM_WARPS * 32);
+                    return last_s != 0;
+                };
+                float *wt = reinterpret_cast<float *>(smem + C::STG_OFF);
+                const int rows = sg.c1 - sg.c0 + 1;
+                if (runs == 1) {
+                    if (last_of(a.tickets + sg.f0, parts)) join<C>(a, sg.f0, rows, wt, sig_s, out_s, 0, 1, parts, true, ovec);
+                } else {
+                    const int run = mine_p / RUN, count = min(RUN, parts - run * RUN);
+                    if (last_of(a.tickets + MAX_CTAS * (run == 0 ? 1 : 2) + sg.f0 + run * RUN, count)) {
+                        join<C>(a, sg.f0, rows, wt, sig_s, out_s, run * RUN, 1, count, false, ovec);
+                        if (last_of(a.tickets + sg.f0, runs)) join<C>(a, sg.f0, rows, wt, sig_s, out_s, 0, RUN, runs, true, ovec);
                     }
                 }
                 bar_sync(1, SM_WARPS * 32);   // sig_s, out_s and last_s are free again
