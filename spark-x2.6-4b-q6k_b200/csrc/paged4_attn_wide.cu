@@ -45,7 +45,7 @@ struct Cfg {
     static constexpr int STG_OFF = Q_OFF + (TWO ? R * HD * 2 : 0);   // 4 KB a softmax warp: rows of 128 bytes between their owners and global memory
     static constexpr size_t SMEM = STG_OFF + SM_WARPS * 4096 + 1024;
     static constexpr int PIECES = HD / 32;              // 16-byte pieces of a token's codes
-    static constexpr int U = N * PIECES > DQ_WARPS * 32 ? N * PIECES / (DQ_WARPS * 32) : 1;   // pieces of a thread
+    static constexpr int U = N * PIECES / (DQ_WARPS * 16);   // pieces of a thread: four warps have the keys, four the values
     static constexpr int QC = HD, SC = HD + HD / 2;     // columns of tensor memory: outputs 0.., queries, scores
     static constexpr int TCOLS = SC + 2 * N <= 256 ? 256 : 512;
 };
@@ -221,8 +221,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(full_k + i, DQ_WARPS);
-            mbar_init(full_v + i, DQ_WARPS);
+            mbar_init(full_k + i, DQ_WARPS / 2);
+            mbar_init(full_v + i, DQ_WARPS / 2);
             mbar_init(empty_k + i, 1);
             mbar_init(empty_v + i, 1);
             mbar_init(s_full + i, 1);
@@ -292,8 +292,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
     Seg sg = seg_s;
     Walk w;
     if (sg.k0 >= 0) w = walk_s;
-    auto next = [&](Seg &g) {
+    auto next = [&]() {   // by value: a group whose address is known would be read from memory again behind every barrier
+        Seg g;
         if (!walk_next<TB>(a, pre, R, COST, w, g)) g.k0 = -1;
+        return g;
     };
     auto tiles_of = [&](const Seg &g) { return g.k0 < 0 ? 0 : max(0, min(g.k1, (g.nblk + TB - 1) / TB) - g.k0); };
 
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             __syncwarp();
             kc++;
         };
-        for (; sg.k0 >= 0; next(sg)) {
+        for (; sg.k0 >= 0; sg = next()) {
             const int n = tiles_of(sg);
             if (n == 0) continue;
             wait_for(&q_full, groups & 1, &dead, a.err);
@@ -351,127 +353,115 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             groups++;
         }
     } else if (warp >= SM_WARPS) {
-        // codes to f16. A thread's piece is 32 dims of a token, the next thread's the next 32, so that a warp's loads lie side by side;
-        // at heads of 256 it has a second one, 32 tokens on.
-        constexpr int U = C::U, PIECES = C::PIECES;
-        const int dt = tid - SM_WARPS * 32, x = dt % PIECES, tok0 = dt / PIECES, per = a.pool.page_tokens / BLOCK;
-        const bool idle = tok0 >= N;
-        // Which of its four 16-byte results a thread stores first: eight neighbours then meet all banks
-        const int turn = HD == 256 ? x >> 1 : HD == 128 ? 2 * (x >> 1) : 0;
-        const int per_tile = TB / per, per_rest = TB % per;
-        uint32_t kc = 0, vc = 0;
-        for (; sg.k0 >= 0; next(sg)) {
-            const int n = tiles_of(sg);
-            const int *table = a.b.table + (size_t)sg.s * a.b.max_pages;
-            // A token's place: its page as the table has it (NONE where no row sees it) and its token of the page
-            struct Place {
-                int page[U], tok[U];
-            };
-            int at_j = 0, idx[U], rest[U];                       // the next tile to be looked up; its blocks' pages of the table, blocks of those
+        // Codes to f16: keys by four warps, values by four. A thread's piece is 32 dims of a token, the next thread's the next 32, so that a
+        // warp's loads lie side by side; its others are STEP tokens on each. Two tiles' bytes are on their way while one is converted.
+        // One code for both: the kernel's loops have to fit the instruction cache together (with keys, values and every second tile by code
+        // of their own, 2048-row chunks took 1.5 times as long).
+        {
+            const bool KEYS = warp < SM_WARPS + DQ_WARPS / 2;
+            constexpr int U = C::U, PIECES = C::PIECES, STEP = DQ_WARPS * 16 / PIECES;
+            const int dt = tid - (SM_WARPS + (KEYS ? 0 : DQ_WARPS / 2)) * 32, x = dt % PIECES, tok0 = dt / PIECES, per = a.pool.page_tokens / BLOCK;
+            const uint8_t *pool = (KEYS ? a.pool.k : a.pool.v) + 16 * x, *scales = (KEYS ? a.pool.ks : a.pool.vs) + 2 * x, *vscales = a.pool.vs + 2 * x;
+            uint64_t *full = KEYS ? full_k : full_v, *empty = KEYS ? empty_k : empty_v;
+            // Which of its four 16-byte results a thread stores first: eight neighbours then meet all banks
+            const int turn = HD == 256 ? x >> 1 : HD == 128 ? 2 * (x >> 1) : 0;
+            uint32_t to[4];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int blk = sg.start / BLOCK + sg.k0 * TB + (tok0 + 32 * u) / BLOCK;
-                idx[u] = blk / per;
-                rest[u] = blk % per;
-            }
-            auto look_up = [&](Place &pl) {
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int at = sg.start + (sg.k0 + at_j) * N + tok0 + 32 * u;
-                    pl.page[u] = idle || at_j >= n || at < sg.see0 || at > sg.p_hi ? NONE : __ldg(table + idx[u]);
-                    pl.tok[u] = rest[u] * BLOCK + tok0 % BLOCK;
-                    idx[u] += per_tile;
-                    rest[u] += per_rest;
-                    if (rest[u] >= per) rest[u] -= per, idx[u]++;
-                }
-                at_j++;
-            };
-            struct Raw {
-                uint4 c[U];
-                uint32_t s[U], vs[U];            // vs, beside keys: their tokens' scales of values, looked at for poison
-            };
-            auto load = [&](Raw &raw, bool keys, const Place &pl) {
+            for (int y = 0; y < 4; y++) to[y] = (KEYS ? 0 : C::V_OFF) + (x >> 1) * C::CH + tok0 * 128 + ((((x & 1) * 4 + ((y + turn) & 3)) ^ (tok0 & 7)) << 4);
+            const int per_tile = TB / per, per_rest = TB % per;
+            uint32_t tc = 0;
+            for (; sg.k0 >= 0; sg = next()) {
+                const int n = tiles_of(sg);
+                if (n == 0) continue;
+                const int *table = a.b.table + (size_t)sg.s * a.b.max_pages;
+                // A token's place: its page as the table has it (NONE where no row sees it) and its token of the page
+                struct Place {
+                    int page[U], tok[U];
+                };
+                int at_j = 0, idx[U], rest[U];                   // the next tile to be looked up; its blocks' pages of the table, blocks of those
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    raw.c[u] = make_uint4(0, 0, 0, 0), raw.s[u] = raw.vs[u] = 0;
-                    const bool there = pl.page[u] >= 0 && pl.page[u] < a.pool.pages;
-                    if (there) {
-                        const size_t at = row_index(a.pool, pl.page[u], sg.kvh, pl.tok[u]);
-                        raw.c[u] = __ldg(reinterpret_cast<const uint4 *>((keys ? a.pool.k : a.pool.v) + at * (HD / 2)) + x);
-                        raw.s[u] = __ldg(reinterpret_cast<const uint16_t *>((keys ? a.pool.ks : a.pool.vs) + at * (HD / GROUP)) + x);
-                        if (keys) raw.vs[u] = __ldg(reinterpret_cast<const uint16_t *>(a.pool.vs + at * (HD / GROUP)) + x);
-                    } else if (pl.page[u] != NONE && a.err) atomicExch(a.err, DEV_BAD_INDEX);
+                    const int blk = sg.start / BLOCK + sg.k0 * TB + (tok0 + STEP * u) / BLOCK;
+                    idx[u] = blk / per;
+                    rest[u] = blk % per;
                 }
-            };
-            auto convert = [&](const Raw &raw, uint8_t *to, bool keys) {
-                if (idle) return;
+                auto look_up = [&](Place &pl) {
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int tok = tok0 + 32 * u;
-                    uint32_t s2 = raw.s[u];
-                    if (!keys) {   // poisoned values become 0: their tokens' weights say NaN where they are seen
-                        if ((s2 & 0xff) >= POISON) s2 &= 0xff00;
-                        if ((s2 >> 8) >= POISON) s2 &= 0x00ff;
+                    for (int u = 0; u < U; u++) {
+                        const int at = sg.start + (sg.k0 + at_j) * N + tok0 + STEP * u;
+                        pl.page[u] = at_j >= n || at < sg.see0 || at > sg.p_hi ? NONE : __ldg(table + idx[u]);
+                        pl.tok[u] = rest[u] * BLOCK + tok0 % BLOCK;
+                        idx[u] += per_tile;
+                        rest[u] += per_rest;
+                        if (rest[u] >= per) rest[u] -= per, idx[u]++;
                     }
-                    uint32_t wd[4] = {raw.c[u].x, raw.c[u].y, raw.c[u].z, raw.c[u].w}, sc[2] = {(s2 & 0xff) * 0x00800080u, (s2 >> 8) * 0x00800080u};
-                    if (HD == 256 && (turn & 1)) {
-                        const uint32_t w0 = wd[0];
-                        wd[0] = wd[1], wd[1] = wd[2], wd[2] = wd[3], wd[3] = w0;
-                    }
-                    if (HD >= 128 && (turn & 2)) {
-                        const uint32_t w0 = wd[0], w1 = wd[1], s0 = sc[0];
-                        wd[0] = wd[2], wd[1] = wd[3], wd[2] = w0, wd[3] = w1;
-                        sc[0] = sc[1], sc[1] = s0;
-                    }
-                    uint8_t *row = to + (x >> 1) * C::CH + tok * 128;
+                    at_j++;
+                };
+                struct Raw {
+                    uint4 c[U];
+                    uint32_t s[U], vs[U];        // vs, beside keys: their tokens' scales of values, looked at for poison
+                };
+                auto load = [&](Raw &raw, const Place &pl) {
 #pragma unroll
-                    for (int y = 0; y < 4; y++) {   // result (y + turn) % 4; its scale is the piece's first or second
-                        const int z = (y + turn) & 3;
-                        const uint32_t scale = HD == 256 && (y & 1) ? ((turn & 1) ? sc[(y >> 1) ^ 1] : sc[y >> 1]) : sc[y >> 1];
-                        uint32_t h[4];
-                        codes_f16(wd[y], h);
-                        const uint4 v = make_uint4(hmul2(h[0], scale), hmul2(h[1], scale), hmul2(h[2], scale), hmul2(h[3], scale));
-                        *reinterpret_cast<uint4 *>(row + ((((x & 1) * 4 + z) ^ (tok & 7)) << 4)) = v;
+                    for (int u = 0; u < U; u++) {
+                        raw.c[u] = make_uint4(0, 0, 0, 0), raw.s[u] = raw.vs[u] = 0;
+                        if ((unsigned)pl.page[u] < (unsigned)a.pool.pages) {
+                            // fewer than 2^32 rows of a pool fit the device
+                            const size_t at = ((uint32_t)pl.page[u] * a.pool.kv_heads + sg.kvh) * a.pool.page_tokens + pl.tok[u];
+                            raw.c[u] = __ldg(reinterpret_cast<const uint4 *>(pool + at * (HD / 2)));
+                            raw.s[u] = __ldg(reinterpret_cast<const uint16_t *>(scales + at * (HD / GROUP)));
+                            if (KEYS) raw.vs[u] = __ldg(reinterpret_cast<const uint16_t *>(vscales + at * (HD / GROUP)));
+                        } else if (pl.page[u] != NONE && a.err) atomicExch(a.err, DEV_BAD_INDEX);
                     }
+                };
+                Place pl;                                        // of the next tile to be loaded
+                Raw raw, behind;
+                look_up(pl);
+                load(raw, pl);
+                look_up(pl);
+                load(behind, pl);
+                look_up(pl);
+#pragma unroll 1
+                for (int j = 0; j < n; j++) {
+                    const uint32_t i = tc & 1;
+                    if (tc > 1) wait_for(empty + i, ((tc >> 1) - 1) & 1, &dead, a.err);
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const int tok = tok0 + STEP * u;
+                        uint32_t s2 = raw.s[u];
+                        if (KEYS) {
+                            if (poisoned(raw.vs[u])) atomicOr(&bad[tc & 3][tok >> 5], 1u << (tok & 31));
+                        } else if (poisoned(s2)) {   // poisoned values become 0: their tokens' weights say NaN where they are seen
+                            if ((s2 & 0xff) >= POISON) s2 &= 0xff00;
+                            if ((s2 >> 8) >= POISON) s2 &= 0x00ff;
+                        }
+                        uint32_t wd[4] = {raw.c[u].x, raw.c[u].y, raw.c[u].z, raw.c[u].w}, sc[2] = {(s2 & 0xff) * 0x00800080u, (s2 >> 8) * 0x00800080u};
+                        if (HD == 256 && (turn & 1)) {
+                            const uint32_t w0 = wd[0];
+                            wd[0] = wd[1], wd[1] = wd[2], wd[2] = wd[3], wd[3] = w0;
+                        }
+                        if (HD >= 128 && (turn & 2)) {
+                            const uint32_t w0 = wd[0], w1 = wd[1], s0 = sc[0];
+                            wd[0] = wd[2], wd[1] = wd[3], wd[2] = w0, wd[3] = w1;
+                            sc[0] = sc[1], sc[1] = s0;
+                        }
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {   // result (y + turn) % 4; its scale is the piece's first or second
+                            const uint32_t scale = HD == 256 && (y & 1) ? ((turn & 1) ? sc[(y >> 1) ^ 1] : sc[y >> 1]) : sc[y >> 1];
+                            uint32_t h[4];
+                            codes_f16(wd[y], h);
+                            const uint4 v = make_uint4(hmul2(h[0], scale), hmul2(h[1], scale), hmul2(h[2], scale), hmul2(h[3], scale));
+                            *reinterpret_cast<uint4 *>(smem + i * C::TILE + to[y] + u * STEP * 128) = v;
+                        }
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full + i);
+                    tc++;
+                    raw = behind;
+                    load(behind, pl);
+                    look_up(pl);
                 }
-            };
-            if (n == 0) continue;
-            // items: K0, K1, V0, K2, V1, .. V(n-1). Two are on their way while one is converted; a tile's page comes before them.
-            Place p0, p1, p2;                                    // of the last keys' tile, the one before, the one behind
-            look_up(p2);
-            p0 = p2;
-            auto load_item = [&](Raw &raw, int m) {
-                if (m >= 2 * n) return;
-                if (m == 0 || ((m & 1) && m < 2 * n - 1)) {      // keys of tile (m + 1) / 2
-                    p1 = p0;
-                    p0 = p2;
-                    load(raw, true, p0);
-                    look_up(p2);
-                } else load(raw, false, m == 2 * n - 1 ? p0 : p1);
-            };
-            auto item = [&](Raw &raw, int m) {
-                const bool keys = m == 0 || ((m & 1) && m < 2 * n - 1);
-                const uint32_t c = keys ? kc : vc, i = c & 1;
-                if (c > 1) wait_for((keys ? empty_k : empty_v) + i, ((c >> 1) - 1) & 1, &dead, a.err);
-                if (keys) {
-#pragma unroll
-                    for (int u = 0; u < U; u++)
-                        if (poisoned(raw.vs[u])) atomicOr(&bad[c & 3][(tok0 + 32 * u) >> 5], 1u << ((tok0 + 32 * u) & 31));
-                }
-                convert(raw, smem + (keys ? 0 : C::V_OFF) + i * C::TILE, keys);
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive((keys ? full_k : full_v) + i);
-                if (keys) kc++;
-                else vc++;
-                load_item(raw, m + 2);
-            };
-            Raw ra, rb;
-            load_item(ra, 0);
-            load_item(rb, 1);
-            for (int m = 0; m < 2 * n; m += 2) {
-                item(ra, m);
-                item(rb, m + 1);
             }
         }
     } else {
@@ -585,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                         tm_wait_ld(s, 32);
 #pragma unroll
                         for (int x = 0; x < 32; x += 2) {
-                            const float2 v = unpack2(fma2(pack2(s[x], s[x + 1]), up2, ref2));
+                            const float2 v = unpack2(add2(mul2(pack2(s[x], s[x + 1]), up2), ref2));   // two roundings: the largest score's difference is exact, however large
                             s[x] = v.x, s[x + 1] = v.y;
                         }
                         if (edge || (b0 | b1)) {
@@ -620,9 +610,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                     d0 = v.x, d1 = v.y;
                     return most;
                 };
-                const float ref = m == -INFINITY ? 0.f : m, mx = weigh(ref);
-                const bool move = mx > W_MAX || (m == -INFINITY && mx > -INFINITY);
-                if (__any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+                for (int again = 0;; again = 1) {
+                    const float ref = m == -INFINITY ? 0.f : m, mx = weigh(ref);
+                    const bool move = mx > W_MAX || (m == -INFINITY && mx > -INFINITY);
+                    if (again || !__any_sync(0xffffffffu, move)) break;
                     const float delta = move ? mx - C::TOP : 0.f, f = m == -INFINITY ? 0.f : ex2(-delta);
                     if (move) m = ref + delta;
                     l0 *= f, l1 *= f;
@@ -640,8 +632,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                             for (int x = 0; x < 32; x++) u[x] = __float_as_uint(o[x] * f);
                             tm_st32(mine + 32 * c, u);
                         }
+                        tm_wait_st();
                     }
-                    weigh(m == -INFINITY ? 0.f : m);
                 }
                 l0 += d0, l1 += d1;
                 if constexpr (!TWO) {
@@ -667,8 +659,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 tc++;
             }
             // the next group's queries, then this one's outputs
-            Seg nx = sg;
-            next(nx);
+            const Seg nx = next();
             const Row rn = queries(nx);
             const bool whole = sg.f0 == sg.f1, real = row.out >= 0;
             const float l = l0 + l1;
