@@ -44,8 +44,7 @@ struct Cfg {
     static constexpr int V_OFF = 2 * TILE, Q_OFF = 4 * TILE;
     static constexpr int STG_OFF = Q_OFF + (TWO ? R * HD * 2 : 0);   // 4 KB a softmax warp: rows of 128 bytes between their owners and global memory
     static constexpr size_t SMEM = STG_OFF + SM_WARPS * 4096 + 1024;
-    static constexpr int PIECES = HD / 32;              // 16-byte pieces of a token's codes
-    static constexpr int U = N * PIECES / (DQ_WARPS * 16);   // pieces of a thread: four warps have the keys, four the values
+    static constexpr int TOKENS = HD == 64 ? 1 : 2, HALVES = HD == 256 ? 2 : 1;   // a converting thread's tokens, 64-byte halves of their rows
     static constexpr int QC = HD, SC = HD + HD / 2;     // columns of tensor memory: outputs 0.., queries, scores
     static constexpr int TCOLS = SC + 2 * N <= 256 ? 256 : 512;
 };
@@ -353,115 +352,104 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             groups++;
         }
     } else if (warp >= SM_WARPS) {
-        // Codes to f16: keys by four warps, values by four. A thread's piece is 32 dims of a token, the next thread's the next 32, so that a
-        // warp's loads lie side by side; its others are STEP tokens on each. Two tiles' bytes are on their way while one is converted.
+        // Codes to f16: keys by four warps, values by four. Eight neighbouring threads have the same 32 dims of eight tokens, so that their
+        // stores meet all banks; a warp has 64 bytes of eight rows at a time (heads of 64: all 32 bytes of sixteen). The next tile's bytes are on
+        // their way while one is converted, the pages of the one behind it.
         // One code for both: the kernel's loops have to fit the instruction cache together (with keys, values and every second tile by code
         // of their own, 2048-row chunks took 1.5 times as long).
-        {
-            const bool KEYS = warp < SM_WARPS + DQ_WARPS / 2;
-            constexpr int U = C::U, PIECES = C::PIECES, STEP = DQ_WARPS * 16 / PIECES;
-            const int dt = tid - (SM_WARPS + (KEYS ? 0 : DQ_WARPS / 2)) * 32, x = dt % PIECES, tok0 = dt / PIECES, per = a.pool.page_tokens / BLOCK;
-            const uint8_t *pool = (KEYS ? a.pool.k : a.pool.v) + 16 * x, *scales = (KEYS ? a.pool.ks : a.pool.vs) + 2 * x, *vscales = a.pool.vs + 2 * x;
-            uint64_t *full = KEYS ? full_k : full_v, *empty = KEYS ? empty_k : empty_v;
-            // Which of its four 16-byte results a thread stores first: eight neighbours then meet all banks
-            const int turn = HD == 256 ? x >> 1 : HD == 128 ? 2 * (x >> 1) : 0;
-            uint32_t to[4];
+        constexpr int G = C::TOKENS, H = C::HALVES, STEP = HD == 64 ? 64 : 32;   // tokens of a thread, 64-byte halves of their rows; tokens apart
+        const bool keys = warp < SM_WARPS + DQ_WARPS / 2;
+        const int w4 = warp & 3, x = HD == 64 ? lane >> 3 & 1 : lane >> 3, tok0 = HD == 64 ? w4 * 16 + (lane >> 4) * 8 + (lane & 7) : w4 * 8 + (lane & 7);
+        const int per = a.pool.page_tokens / BLOCK, per_tile = TB / per, per_rest = TB % per;
+        const uint8_t *pool = (keys ? a.pool.k : a.pool.v) + 16 * x, *scales = (keys ? a.pool.ks : a.pool.vs) + 2 * x, *vscales = a.pool.vs + 2 * x;
+        uint64_t *full = keys ? full_k : full_v, *empty = keys ? empty_k : empty_v;
+        uint32_t to[4];
 #pragma unroll
-            for (int y = 0; y < 4; y++) to[y] = (KEYS ? 0 : C::V_OFF) + (x >> 1) * C::CH + tok0 * 128 + ((((x & 1) * 4 + ((y + turn) & 3)) ^ (tok0 & 7)) << 4);
-            const int per_tile = TB / per, per_rest = TB % per;
-            uint32_t tc = 0;
-            for (; sg.k0 >= 0; sg = next()) {
-                const int n = tiles_of(sg);
-                if (n == 0) continue;
-                const int *table = a.b.table + (size_t)sg.s * a.b.max_pages;
-                // A token's place: its page as the table has it (NONE where no row sees it) and its token of the page
-                struct Place {
-                    int page[U], tok[U];
-                };
-                int at_j = 0, idx[U], rest[U];                   // the next tile to be looked up; its blocks' pages of the table, blocks of those
+        for (int y = 0; y < 4; y++) to[y] = (keys ? 0 : C::V_OFF) + (x >> 1) * C::CH + tok0 * 128 + ((((x & 1) * 4 + y) ^ (tok0 & 7)) << 4);
+        uint32_t tc = 0;
+        for (; sg.k0 >= 0; sg = next()) {
+            const int n = tiles_of(sg);
+            if (n == 0) continue;
+            const int *table = a.b.table + (size_t)sg.s * a.b.max_pages;
+            int at_j = 0, idx[G], rest[G], page[G], row[G];      // the next tile to be looked up: its blocks' pages of the table, blocks of those; a token's
+                                                                 // page as the table has it (NONE where no row sees it), its token of the page
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int blk = sg.start / BLOCK + sg.k0 * TB + (tok0 + STEP * u) / BLOCK;
-                    idx[u] = blk / per;
-                    rest[u] = blk % per;
+            for (int u = 0; u < G; u++) {
+                const int blk = sg.start / BLOCK + sg.k0 * TB + (tok0 + STEP * u) / BLOCK;
+                idx[u] = blk / per;
+                rest[u] = blk % per;
+            }
+            auto look_up = [&]() {
+#pragma unroll
+                for (int u = 0; u < G; u++) {
+                    const int at = sg.start + (sg.k0 + at_j) * N + tok0 + STEP * u;
+                    page[u] = at_j >= n || at < sg.see0 || at > sg.p_hi ? NONE : __ldg(table + idx[u]);
+                    row[u] = rest[u] * BLOCK + tok0 % BLOCK;
+                    idx[u] += per_tile;
+                    rest[u] += per_rest;
+                    if (rest[u] >= per) rest[u] -= per, idx[u]++;
                 }
-                auto look_up = [&](Place &pl) {
+                at_j++;
+            };
+            uint4 c[G][H];
+            uint32_t sc[G][H], vs[G][H];                         // vs, beside keys: their tokens' scales of values, looked at for poison
+            auto load = [&]() {
 #pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        const int at = sg.start + (sg.k0 + at_j) * N + tok0 + STEP * u;
-                        pl.page[u] = at_j >= n || at < sg.see0 || at > sg.p_hi ? NONE : __ldg(table + idx[u]);
-                        pl.tok[u] = rest[u] * BLOCK + tok0 % BLOCK;
-                        idx[u] += per_tile;
-                        rest[u] += per_rest;
-                        if (rest[u] >= per) rest[u] -= per, idx[u]++;
-                    }
-                    at_j++;
-                };
-                struct Raw {
-                    uint4 c[U];
-                    uint32_t s[U], vs[U];        // vs, beside keys: their tokens' scales of values, looked at for poison
-                };
-                auto load = [&](Raw &raw, const Place &pl) {
+                for (int u = 0; u < G; u++) {
+                    const bool there = (unsigned)page[u] < (unsigned)a.pool.pages;
+                    if (!there && page[u] != NONE && a.err) atomicExch(a.err, DEV_BAD_INDEX);
+                    // fewer than 2^32 rows of a pool fit the device
+                    const size_t at = there ? ((uint32_t)page[u] * a.pool.kv_heads + sg.kvh) * a.pool.page_tokens + row[u] : 0;
 #pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        raw.c[u] = make_uint4(0, 0, 0, 0), raw.s[u] = raw.vs[u] = 0;
-                        if ((unsigned)pl.page[u] < (unsigned)a.pool.pages) {
-                            // fewer than 2^32 rows of a pool fit the device
-                            const size_t at = ((uint32_t)pl.page[u] * a.pool.kv_heads + sg.kvh) * a.pool.page_tokens + pl.tok[u];
-                            raw.c[u] = __ldg(reinterpret_cast<const uint4 *>(pool + at * (HD / 2)));
-                            raw.s[u] = __ldg(reinterpret_cast<const uint16_t *>(scales + at * (HD / GROUP)));
-                            if (KEYS) raw.vs[u] = __ldg(reinterpret_cast<const uint16_t *>(vscales + at * (HD / GROUP)));
-                        } else if (pl.page[u] != NONE && a.err) atomicExch(a.err, DEV_BAD_INDEX);
+                    for (int h = 0; h < H; h++) {
+                        sc[u][h] = vs[u][h] = 0;                 // whatever the codes are: they stand for 0
+                        if (there) {
+                            c[u][h] = __ldg(reinterpret_cast<const uint4 *>(pool + at * (HD / 2) + 64 * h));
+                            sc[u][h] = __ldg(reinterpret_cast<const uint16_t *>(scales + at * (HD / GROUP) + 8 * h));
+                            if (keys) vs[u][h] = __ldg(reinterpret_cast<const uint16_t *>(vscales + at * (HD / GROUP) + 8 * h));
+                        }
                     }
-                };
-                Place pl;                                        // of the next tile to be loaded
-                Raw raw, behind;
-                look_up(pl);
-                load(raw, pl);
-                look_up(pl);
-                load(behind, pl);
-                look_up(pl);
+                }
+            };
+#pragma unroll
+            for (int u = 0; u < G; u++)
+#pragma unroll
+                for (int h = 0; h < H; h++) c[u][h] = make_uint4(0, 0, 0, 0);
+            look_up();
+            load();
+            look_up();
 #pragma unroll 1
-                for (int j = 0; j < n; j++) {
-                    const uint32_t i = tc & 1;
-                    if (tc > 1) wait_for(empty + i, ((tc >> 1) - 1) & 1, &dead, a.err);
+            for (int j = 0; j < n; j++) {
+                const uint32_t i = tc & 1;
+                if (tc > 1) wait_for(empty + i, ((tc >> 1) - 1) & 1, &dead, a.err);
 #pragma unroll
-                    for (int u = 0; u < U; u++) {
+                for (int u = 0; u < G; u++)
+#pragma unroll
+                    for (int h = 0; h < H; h++) {
                         const int tok = tok0 + STEP * u;
-                        uint32_t s2 = raw.s[u];
-                        if (KEYS) {
-                            if (poisoned(raw.vs[u])) atomicOr(&bad[tc & 3][tok >> 5], 1u << (tok & 31));
-                        } else if (poisoned(s2)) {   // poisoned values become 0: their tokens' weights say NaN where they are seen
-                            if ((s2 & 0xff) >= POISON) s2 &= 0xff00;
-                            if ((s2 >> 8) >= POISON) s2 &= 0x00ff;
+                        uint32_t s2 = sc[u][h];
+                        if (poisoned(keys ? vs[u][h] : s2)) {
+                            if (keys) atomicOr(&bad[tc & 3][tok >> 5], 1u << (tok & 31));
+                            else {   // poisoned values become 0: their tokens' weights say NaN where they are seen
+                                if ((s2 & 0xff) >= POISON) s2 &= 0xff00;
+                                if ((s2 >> 8) >= POISON) s2 &= 0x00ff;
+                            }
                         }
-                        uint32_t wd[4] = {raw.c[u].x, raw.c[u].y, raw.c[u].z, raw.c[u].w}, sc[2] = {(s2 & 0xff) * 0x00800080u, (s2 >> 8) * 0x00800080u};
-                        if (HD == 256 && (turn & 1)) {
-                            const uint32_t w0 = wd[0];
-                            wd[0] = wd[1], wd[1] = wd[2], wd[2] = wd[3], wd[3] = w0;
-                        }
-                        if (HD >= 128 && (turn & 2)) {
-                            const uint32_t w0 = wd[0], w1 = wd[1], s0 = sc[0];
-                            wd[0] = wd[2], wd[1] = wd[3], wd[2] = w0, wd[3] = w1;
-                            sc[0] = sc[1], sc[1] = s0;
-                        }
+                        const uint32_t wd[4] = {c[u][h].x, c[u][h].y, c[u][h].z, c[u][h].w}, s4[2] = {(s2 & 0xff) * 0x00800080u, (s2 >> 8) * 0x00800080u};
 #pragma unroll
-                        for (int y = 0; y < 4; y++) {   // result (y + turn) % 4; its scale is the piece's first or second
-                            const uint32_t scale = HD == 256 && (y & 1) ? ((turn & 1) ? sc[(y >> 1) ^ 1] : sc[y >> 1]) : sc[y >> 1];
-                            uint32_t h[4];
-                            codes_f16(wd[y], h);
-                            const uint4 v = make_uint4(hmul2(h[0], scale), hmul2(h[1], scale), hmul2(h[2], scale), hmul2(h[3], scale));
-                            *reinterpret_cast<uint4 *>(smem + i * C::TILE + to[y] + u * STEP * 128) = v;
+                        for (int y = 0; y < 4; y++) {
+                            uint32_t f[4];
+                            codes_f16(wd[y], f);
+                            const uint4 v = make_uint4(hmul2(f[0], s4[y >> 1]), hmul2(f[1], s4[y >> 1]), hmul2(f[2], s4[y >> 1]), hmul2(f[3], s4[y >> 1]));
+                            *reinterpret_cast<uint4 *>(smem + i * C::TILE + to[y] + u * STEP * 128 + h * 2 * C::CH) = v;
                         }
                     }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full + i);
-                    tc++;
-                    raw = behind;
-                    load(behind, pl);
-                    look_up(pl);
-                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + i);
+                tc++;
+                load();
+                look_up();
             }
         }
     } else {
