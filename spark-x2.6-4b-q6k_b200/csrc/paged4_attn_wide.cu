@@ -383,7 +383,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
 #pragma unroll
                 for (int u = 0; u < G; u++) {
                     const int at = sg.start + (sg.k0 + at_j) * N + tok0 + STEP * u;
-                    page[u] = at_j >= n || at < sg.see0 || at > sg.p_hi ? NONE : __ldg(table + idx[u]);
+                    const bool seen = at_j < n && at >= sg.see0 && at <= sg.p_hi;
+                    page[u] = __ldg(table + (seen ? idx[u] : 0));
+                    if (!seen) page[u] = NONE;
                     row[u] = rest[u] * BLOCK + tok0 % BLOCK;
                     idx[u] += per_tile;
                     rest[u] += per_rest;
@@ -392,29 +394,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 at_j++;
             };
             uint4 c[G][H];
-            uint32_t sc[G][H], vs[G][H];                         // vs, beside keys: their tokens' scales of values, looked at for poison
+            uint32_t sc[G][H], vs[G][H];                         // vs: the tokens' scales of values, which are looked at for poison beside keys, too
+            bool there[G];
             auto load = [&]() {
 #pragma unroll
                 for (int u = 0; u < G; u++) {
-                    const bool there = (unsigned)page[u] < (unsigned)a.pool.pages;
-                    if (!there && page[u] != NONE && a.err) atomicExch(a.err, DEV_BAD_INDEX);
-                    // fewer than 2^32 rows of a pool fit the device
-                    const size_t at = there ? ((uint32_t)page[u] * a.pool.kv_heads + sg.kvh) * a.pool.page_tokens + row[u] : 0;
+                    there[u] = (unsigned)page[u] < (unsigned)a.pool.pages;
+                    if (!there[u] && page[u] != NONE && a.err) atomicExch(a.err, DEV_BAD_INDEX);
+                    // fewer than 2^32 rows of a pool fit the device; a token that none sees has row 0's bytes under scales of 0
+                    const size_t at = there[u] ? ((uint32_t)page[u] * a.pool.kv_heads + sg.kvh) * a.pool.page_tokens + row[u] : 0;
 #pragma unroll
                     for (int h = 0; h < H; h++) {
-                        sc[u][h] = vs[u][h] = 0;                 // whatever the codes are: they stand for 0
-                        if (there) {
-                            c[u][h] = __ldg(reinterpret_cast<const uint4 *>(pool + at * (HD / 2) + 64 * h));
-                            sc[u][h] = __ldg(reinterpret_cast<const uint16_t *>(scales + at * (HD / GROUP) + 8 * h));
-                            if (keys) vs[u][h] = __ldg(reinterpret_cast<const uint16_t *>(vscales + at * (HD / GROUP) + 8 * h));
-                        }
+                        c[u][h] = __ldg(reinterpret_cast<const uint4 *>(pool + at * (HD / 2) + 64 * h));
+                        sc[u][h] = __ldg(reinterpret_cast<const uint16_t *>(scales + at * (HD / GROUP) + 8 * h));
+                        vs[u][h] = __ldg(reinterpret_cast<const uint16_t *>(vscales + at * (HD / GROUP) + 8 * h));
                     }
                 }
             };
-#pragma unroll
-            for (int u = 0; u < G; u++)
-#pragma unroll
-                for (int h = 0; h < H; h++) c[u][h] = make_uint4(0, 0, 0, 0);
             look_up();
             load();
             look_up();
@@ -427,8 +423,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
 #pragma unroll
                     for (int h = 0; h < H; h++) {
                         const int tok = tok0 + STEP * u;
-                        uint32_t s2 = sc[u][h];
-                        if (poisoned(keys ? vs[u][h] : s2)) {
+                        uint32_t s2 = there[u] ? sc[u][h] : 0;
+                        if (there[u] && poisoned(vs[u][h])) {
                             if (keys) atomicOr(&bad[tc & 3][tok >> 5], 1u << (tok & 31));
                             else {   // poisoned values become 0: their tokens' weights say NaN where they are seen
                                 if ((s2 & 0xff) >= POISON) s2 &= 0xff00;
