@@ -635,7 +635,13 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
     }
 }
 
-constexpr long long NARROW = 64;                       // rows per KV head up to which a sequence is this kernel's
+// Rows per KV head up to which a sequence is this kernel's. Each 8 of them read the cache again (from L2); the kernel for many rows takes 128
+// at once, and as long for one. Where they meet (us, here / there; heads of 256, of 128 in brackets; bf16):
+//   64 sequences of 1200 keys   32 rows 103 164 (64 102)   64: 187 179 (113 105)   128: 356 199 (210 107)
+//   8 of 6000                   32 rows 59 106 (40 63)     64: 100 104 (66 68)     128: 183 160 (115 84)
+//   1 of 16000                  64 rows 47 89 (33 53)     256: 123 131 (80 76)
+// f32 the same within a tenth. With few (sequence, KV head) pairs the wide kernel's parts are many and small, so the border lies higher.
+constexpr long long FEW_PAIRS = 8, NARROW_FEW = 256, NARROW = 64;
 constexpr size_t TICKETS = 3 * MAX_CTAS_ALL * sizeof(unsigned int);   // before the partials: three words per CTA
 constexpr int MAX_CTAS = 3;                             // of an SM
 
@@ -713,15 +719,15 @@ int spk_paged4_attn(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
     a.part = (float *)((uint8_t *)p->workspace + TICKETS);
     a.err = device_error_ptr();
     const cudaStream_t s = (cudaStream_t)stream;
-    if ((long long)batch->rows * a.group > NARROW) {
-        // some sequence may have many rows
-        a.from = NARROW + 1;
+    const long long narrow = (long long)batch->nseq * pool->kv_heads <= FEW_PAIRS ? NARROW_FEW : NARROW;
+    if ((long long)batch->rows * a.group > narrow) {   // some sequence may have many rows
+        a.from = narrow + 1;
         a.to = LLONG_MAX;
         const int rc = attn_wide(a, p->type, s, who);
         if (rc || batch->nseq == 1) return rc;
     }
     a.from = 0;
-    a.to = NARROW;
+    a.to = narrow;
     return p->type == T_F32 ? launch<float>(a, s, who) : p->type == T_F16 ? launch<__half>(a, s, who) : launch<__nv_bfloat16>(a, s, who);
 }
 

@@ -11,8 +11,6 @@
 //
 // Work split: paged_line.cuh's line of groups of 128 rows, one CTA per SM. Warps: 0-3 queries, softmax and outputs,
 // 4-11 codes to f16, 12 the MMAs. Each walks the CTA's groups by itself; they meet at mbarriers.
-#include <limits.h>
-
 #include "paged4.cuh"
 #include "paged_line.cuh"
 #include "paged_tc.cuh"
@@ -27,9 +25,8 @@ constexpr int N = 64, TB = N / BLOCK;                   // tokens of a tile, its
 constexpr int R = WIDE_R;
 constexpr int QCH = R * 128;                            // 64 dims of the queries' second terms
 constexpr int SM_WARPS = 4, DQ_WARPS = 8, MMA_WARP = SM_WARPS + DQ_WARPS, WARPS = MMA_WARP + 1, THREADS = WARPS * 32;
-constexpr int COST = 32;                                // a group's fixed cost in blocks
+constexpr int COST = 64;                                // a group's fixed cost in blocks
 constexpr int RUN = 16, MAX_CTAS = 512;                 // parts that are added together (a join takes 32); CTAs of a call
-constexpr int NONE = INT_MIN;                           // no page
 
 template <typename T_, int HD_>
 struct Cfg {
@@ -167,20 +164,25 @@ __device__ __noinline__ void join(const AttnParams &a, int f0, int rows, float *
         }
     }
     bar_sync(1, SM_WARPS * 32);
-    const int items = rows * (HD / 4);                   // of 4 values
+    const int items = rows * (HD / 4);                   // of 4 values; four of four parts on their way
     for (int x0 = tid; x0 < items; x0 += 4 * SM_WARPS * 32) {
         float4 o[4] = {};
-        for (int p = 0; p < n; p++) {
-            const float *src = part(at + step * p);
-            float4 v[4];
+        for (int p = 0; p < n; p += 4) {
+            float4 v[4][4];
 #pragma unroll
-            for (int y = 0; y < 4; y++) v[y] = __ldcg(reinterpret_cast<const float4 *>(src) + min(x0 + y * SM_WARPS * 32, items - 1));
+            for (int q = 0; q < 4; q++) {
+                const float4 *src = reinterpret_cast<const float4 *>(part(at + step * min(p + q, n - 1)));
 #pragma unroll
-            for (int y = 0; y < 4; y++) {
-                const float f = wt[p * R + min(x0 + y * SM_WARPS * 32, items - 1) / (HD / 4)];
-                if (f == 0.f) continue;                  // nothing seen, or nothing to say
-                o[y].x = fmaf(v[y].x, f, o[y].x), o[y].y = fmaf(v[y].y, f, o[y].y), o[y].z = fmaf(v[y].z, f, o[y].z), o[y].w = fmaf(v[y].w, f, o[y].w);
+                for (int y = 0; y < 4; y++) v[q][y] = __ldcg(src + min(x0 + y * SM_WARPS * 32, items - 1));
             }
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const float f = p + q < n ? wt[(p + q) * R + min(x0 + y * SM_WARPS * 32, items - 1) / (HD / 4)] : 0.f;
+                    if (f == 0.f) continue;              // nothing seen, or nothing to say
+                    o[y].x = fmaf(v[q][y].x, f, o[y].x), o[y].y = fmaf(v[q][y].y, f, o[y].y), o[y].z = fmaf(v[q][y].z, f, o[y].z), o[y].w = fmaf(v[q][y].w, f, o[y].w);
+                }
         }
 #pragma unroll
         for (int y = 0; y < 4; y++) {
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             if (n == 0) continue;
             const int *table = a.b.table + (size_t)sg.s * a.b.max_pages;
             int at_j = 0, idx[G], rest[G], page[G], row[G];      // the next tile to be looked up: its blocks' pages of the table, blocks of those; a token's
-                                                                 // page as the table has it (NONE where no row sees it), its token of the page
+                                                                 // page as the table has it, its token of the page (-1 where no row sees it)
 #pragma unroll
             for (int u = 0; u < G; u++) {
                 const int blk = sg.start / BLOCK + sg.k0 * TB + (tok0 + STEP * u) / BLOCK;
@@ -385,8 +387,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                     const int at = sg.start + (sg.k0 + at_j) * N + tok0 + STEP * u;
                     const bool seen = at_j < n && at >= sg.see0 && at <= sg.p_hi;
                     page[u] = __ldg(table + (seen ? idx[u] : 0));
-                    if (!seen) page[u] = NONE;
-                    row[u] = rest[u] * BLOCK + tok0 % BLOCK;
+                    row[u] = seen ? rest[u] * BLOCK + tok0 % BLOCK : -1;
                     idx[u] += per_tile;
                     rest[u] += per_rest;
                     if (rest[u] >= per) rest[u] -= per, idx[u]++;
@@ -399,8 +400,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             auto load = [&]() {
 #pragma unroll
                 for (int u = 0; u < G; u++) {
-                    there[u] = (unsigned)page[u] < (unsigned)a.pool.pages;
-                    if (!there[u] && page[u] != NONE && a.err) atomicExch(a.err, DEV_BAD_INDEX);
+                    there[u] = row[u] >= 0 && (unsigned)page[u] < (unsigned)a.pool.pages;
+                    if (!there[u] && row[u] >= 0 && a.err) atomicExch(a.err, DEV_BAD_INDEX);
                     // fewer than 2^32 rows of a pool fit the device; a token that none sees has row 0's bytes under scales of 0
                     const size_t at = there[u] ? ((uint32_t)page[u] * a.pool.kv_heads + sg.kvh) * a.pool.page_tokens + row[u] : 0;
 #pragma unroll
@@ -559,7 +560,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                         tm_wait_ld(s, 32);
 #pragma unroll
                         for (int x = 0; x < 32; x += 2) {
-                            const float2 v = unpack2(add2(mul2(pack2(s[x], s[x + 1]), up2), ref2));   // two roundings: the largest score's difference is exact, however large
+                            const float2 v = unpack2(mul2(pack2(s[x], s[x + 1]), up2));
                             s[x] = v.x, s[x + 1] = v.y;
                         }
                         if (edge || (b0 | b1)) {
@@ -575,7 +576,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                         for (int x = 0; x < 32; x += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(m4[x / 2 & 3]) : "f"(s[x]), "f"(s[x + 1]));
 #pragma unroll
                         for (int x = 0; x < 16; x++) {
-                            const float p = ex2(s[2 * x]), q = ex2(s[2 * x + 1]);
+                            const float2 w = unpack2(add2(pack2(s[2 * x], s[2 * x + 1]), ref2));   // the largest score's difference is exact, however large
+                            const float p = ex2(w.x), q = ex2(w.y);
                             hi[c][x] = pack_f16(p, q);
                             if constexpr (__is_same(T, __nv_bfloat16)) sum = add2(sum, pack2(p, q));   // f16's rounding is beneath bf16's
                             else {
@@ -597,10 +599,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
 #pragma unroll 1
                 for (int again = 0;; again = 1) {
                     const float ref = m == -INFINITY ? 0.f : m, mx = weigh(ref);
-                    const bool move = mx > W_MAX || (m == -INFINITY && mx > -INFINITY);
+                    const bool move = mx - ref > W_MAX || (m == -INFINITY && mx > -INFINITY);
                     if (again || !__any_sync(0xffffffffu, move)) break;
-                    const float delta = move ? mx - C::TOP : 0.f, f = m == -INFINITY ? 0.f : ex2(-delta);
-                    if (move) m = ref + delta;
+                    const float was = m;
+                    if (move) m = mx - C::TOP;
+                    const float f = was == -INFINITY ? 0.f : ex2(was - m);
                     l0 *= f, l1 *= f;
                     if (j > 0) {   // what the outputs have so far, behind the products before
                         wait_for(pv_done + (i ^ 1), ((tc - 1) >> 1) & 1, &dead, a.err);

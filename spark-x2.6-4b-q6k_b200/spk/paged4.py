@@ -16,6 +16,7 @@ Streams, ownership and lifetimes are spk.paged's.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import SpkError, check, lib
 from .paged import BLOCK, Owned, PagedBatch, _angles, _attend, _rows, lent, stream_of, type_of
@@ -47,6 +48,18 @@ class _Attn4(C.Structure):
 
 
 PARTS = 3           # spk_paged4_read's type: codes and scales apart
+
+# The arguments' fields in one go: a step's calls take less time than setting them one by one.
+_APPEND, _READ = struct.Struct("@PqPqPPqqiiPPfPii"), struct.Struct("@iPPqqPPqq")
+
+
+def _stride(t, shape, like, what: str):
+    """_rows() of a row matrix that has to be like `like` (type and device), without its words where all is well."""
+    if t.shape == shape and t.dtype == like.dtype and t.get_device() == like.get_device() >= 0:
+        ld, one = t.stride()
+        if one == 1:
+            return ld
+    return _rows(t, *shape, what, like)
 
 
 class Paged4Cache:
@@ -98,37 +111,38 @@ class Paged4Batch(PagedBatch):
                                          device=self.cache.device)
         self._a = _Attn4(heads=self.heads, workspace=self.workspace.data_ptr())
         self._append, self._attn, self._read = L.spk_paged4_append, L.spk_paged4_attn, L.spk_paged4_read
-        self._ap, self._rd = _Append4(), _Read4()
+        self._ap, self._rd = (C.c_char * C.sizeof(_Append4))(), (C.c_char * C.sizeof(_Read4))()
         self._ap_p, self._rd_p = C.addressof(self._ap), C.addressof(self._rd)
         wide, self._f32 = self.cache.kv_heads * self.cache.head_dim, torch.float32
-        self._parts = [(w, t, side + name) for side in "kv" for w, t, name in ((wide, torch.float8_e4m3fn, ""), (wide // GROUP, torch.float16, "_scale"))]
+        self._parts = [(wide, torch.float8_e4m3fn), (wide // GROUP, torch.float16)] * 2
+        self._kv_shape, self._q_shape = (torch.Size((self.rows, w)) for w in (wide, self.heads * self.cache.head_dim))
+        self._sc_shape, self._e4m3, self._f16 = torch.Size((self.rows, wide // GROUP)), torch.float8_e4m3fn, torch.float16
+        self._index = self.cache.device.index
 
     def append(self, k, v, freq=None, q=None, q_out=None, q_norm=None, k_norm=None, eps: float = 1e-6, interleaved: bool = False,
                stream=None):
         """Rows k, v [rows][kv_heads * head_dim] into the pages, and queries q [rows][heads * head_dim] to q_out (made when not
         given, returned; q itself for in place). q_norm, k_norm: f32 [head_dim], the weights of an RMS norm of each head.
         freq: the rotation of the first 2 * len(freq) dims, pairs half of that apart or, `interleaved`, side by side."""
-        c, a = self.cache, self._ap
-        width = c.kv_heads * c.head_dim
-        a.ldk, a.ldv = _rows(k, self.rows, width, "k", on=c.device), _rows(v, self.rows, width, "v", k)
-        a.k, a.v, a.type = k.data_ptr(), v.data_ptr(), type_of(k)
+        c = self.cache
+        if k.get_device() != self._index:
+            _rows(k, *self._kv_shape, "k", on=c.device)
+        ldk, ldv = _stride(k, self._kv_shape, k, "k"), _stride(v, self._kv_shape, k, "v")
+        at_q = at_out = ldq = ldo = heads = 0
         if q is not None:
-            wide = self.heads * c.head_dim
-            a.ldq = _rows(q, self.rows, wide, "q", k)
+            ldq = _stride(q, self._q_shape, k, "q")
             if q_out is None:
                 import torch
 
                 with torch.cuda.stream(stream):      # None: the current one
-                    q_out = torch.empty(self.rows, wide, dtype=q.dtype, device=q.device)
-            a.ldq_out = _rows(q_out, self.rows, wide, "q_out", k)
-            a.q, a.q_out, a.heads = q.data_ptr(), q_out.data_ptr(), self.heads
+                    q_out = torch.empty(self._q_shape, dtype=q.dtype, device=q.device)
+            ldo = _stride(q_out, self._q_shape, k, "q_out")
+            at_q, at_out, heads = q.data_ptr(), q_out.data_ptr(), self.heads
         elif q_out is not None or q_norm is not None:
             raise SpkError("q_out and q_norm go with q")
-        else:
-            a.q, a.q_out, a.heads = None, None, 0
-        a.q_norm, a.k_norm = self._norm(q_norm, "q_norm"), self._norm(k_norm, "k_norm")
-        a.eps, a.interleaved = eps, interleaved
-        a.freq, a.pdim = _angles(freq, k)
+        at_f, pdim = _angles(freq, k)
+        _APPEND.pack_into(self._ap, 0, at_q, ldq, at_out, ldo, k.data_ptr(), v.data_ptr(), ldk, ldv, type_of(k), heads,
+                          self._norm(q_norm, "q_norm"), self._norm(k_norm, "k_norm"), eps, at_f or 0, pdim, interleaved)
         raw = stream_of(k, stream)
         c.owned.use(raw, stream)
         check(self._append(self._pool_p, self._batch_p, self._ap_p, raw))
@@ -139,7 +153,7 @@ class Paged4Batch(PagedBatch):
     def _norm(self, w, name: str):
         """The address of a norm's weights."""
         if w is None:
-            return None
+            return 0
         c = self.cache
         if w.dtype != self._f32 or w.shape != (c.head_dim,) or not w.is_contiguous() or w.device != c.device:
             raise SpkError(f"{name} is f32 [{c.head_dim}] on {c.device}; got {w.dtype} {list(w.shape)} on {w.device}")
@@ -165,29 +179,28 @@ class Paged4Batch(PagedBatch):
                 new = [torch.empty(self.rows, c.kv_heads * c.head_dim, dtype=dtype or torch.bfloat16, device=c.device) if t is None else t
                        for t in (k, v)]
             k, v = new
-        a, width = self._rd, c.kv_heads * c.head_dim
-        a.ldk, a.ldv = _rows(k, self.rows, width, "k", on=c.device), _rows(v, self.rows, width, "v", k)
-        a.k, a.v, a.type = k.data_ptr(), v.data_ptr(), type_of(k)
+        if k.get_device() != self._index:
+            _rows(k, *self._kv_shape, "k", on=c.device)
+        _READ.pack_into(self._rd, 0, type_of(k), k.data_ptr(), v.data_ptr(), _stride(k, self._kv_shape, k, "k"), _stride(v, self._kv_shape, k, "v"), 0, 0, 0, 0)
         self._read_rows(stream, k, v)
         return k, v
 
     def parts(self, out=None, stream=None):
         """The rows as the cache has them, apart: [k codes, k scales, v codes, v scales], codes e4m3
         [rows][kv_heads * head_dim], scales f16 [rows][kv_heads * head_dim / 16]. out: four such tensors."""
-        c, a = self.cache, self._rd
         if out is None:
             import torch
 
             with torch.cuda.stream(stream):
-                out = [torch.empty(self.rows, w, dtype=t, device=c.device) for w, t, _ in self._parts]
+                out = [torch.empty(self.rows, w, dtype=t, device=self.cache.device) for w, t in self._parts]
         k, ks, v, vs = out
-        for t, (w, dtype, name) in zip(out, self._parts):
-            if t.dtype != dtype:
-                raise SpkError(f"{name} is {dtype}; got {t.dtype}")
-        (wide, *_), (few, *_) = self._parts[:2]
-        a.ldk, a.ldv = _rows(k, self.rows, wide, "k", on=c.device), _rows(v, self.rows, wide, "v", k)
-        a.ldk_scale, a.ldv_scale = _rows(ks, self.rows, few, "k_scale", on=c.device), _rows(vs, self.rows, few, "v_scale", ks)
-        a.k, a.v, a.k_scale, a.v_scale, a.type = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), PARTS
+        if k.dtype != self._e4m3 or ks.dtype != self._f16:
+            raise SpkError(f"codes are {self._e4m3}, scales {self._f16}; got {k.dtype} and {ks.dtype}")
+        if k.get_device() != self._index or ks.get_device() != self._index:
+            _rows(k, *self._kv_shape, "k codes", on=self.cache.device)
+            _rows(ks, *self._sc_shape, "k scales", on=self.cache.device)
+        _READ.pack_into(self._rd, 0, PARTS, k.data_ptr(), v.data_ptr(), _stride(k, self._kv_shape, k, "k codes"), _stride(v, self._kv_shape, k, "v codes"),
+                        ks.data_ptr(), vs.data_ptr(), _stride(ks, self._sc_shape, ks, "k scales"), _stride(vs, self._sc_shape, ks, "v scales"))
         self._read_rows(stream, *out)
         return out
 

@@ -1,4 +1,4 @@
-"""Scoring a batch of sequences over the paged 8-bit cache: the decoder of spk.model for many
+"""Scoring a batch of sequences over a paged cache in 8 or 4 bits: the decoder of spk.model for many
 sequences at once, where DeviceModel runs one.
 
 ``PagedScorer`` holds the same weights (the VQ projections re-laid for the tensor-core GEMM, the tied
@@ -6,10 +6,12 @@ Q8_0 head in its tile layout) and, per layer, a ``PagedCache`` that all sequence
 new tokens of any of them, in one call: every layer appends the rows' keys and values to the sequences'
 pages with the rotation on the way (spk_paged_append), attends over the pages (spk_paged_attn, the gate
 in its epilogue), and the head's logits end in each token's log probability, the entropy and the most
-likely alternatives (spk_logprobs). A sequence may be continued by later calls, and dropped with
+likely alternatives (spk_logprobs). With ``kv_bits=4`` the cache is a ``Paged4Cache`` (4.5 bits a value for 8.06, so nearly
+twice the tokens in the same memory): one spk_paged4_append rotates queries and keys and rounds keys and values, and
+spk_paged4_attn attends. A sequence may be continued by later calls, and dropped with
 ``release``. A call that raises leaves the sequences as they were, as long and on the same pages.
 
-    python -m spk.serve [--layers N] [--sequences N] [--tokens N]    # synthetic weights
+    python -m spk.serve [--layers N] [--sequences N] [--tokens N] [--kv-bits 8|4]    # synthetic weights
 """
 from __future__ import annotations
 
@@ -22,6 +24,7 @@ import numpy as np
 from . import SpkError, check, dev_bytes, lib
 from .model import MATS, ModelConfig, mat_shapes, upload_container
 from .paged import MAX_SEQ, PagedBatch, PagedCache, PageTable, rope_freq
+from .paged4 import Paged4Batch, Paged4Cache
 from .score import MAX_ROWS, MAX_TOP, LogProbs
 
 GEMM_ROWS = 128     # rows of one spk_vq_lut_gemm call
@@ -72,9 +75,12 @@ class _Matrix:
 
 
 class PagedScorer:
-    def __init__(self, cfg: ModelConfig, weights: dict, pages: int, page_tokens: int = 64, device="cuda:0"):
+    def __init__(self, cfg: ModelConfig, weights: dict, pages: int, page_tokens: int = 64, device="cuda:0", kv_bits: int = 8):
         import torch
 
+        if kv_bits not in (8, 4):
+            raise SpkError(f"a cache of {kv_bits} bits (8 or 4)")
+        self.kv_bits = kv_bits
         self.cfg, self.device = cfg, torch.device(device)
         put = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(self.device)  # noqa: E731
         shapes = mat_shapes(cfg)
@@ -99,7 +105,8 @@ class PagedScorer:
         dims = lambda part: int(cfg.head_dim * part)  # noqa: E731
         self.freq = {1: rope_freq(cfg.rope_theta_full, dims(cfg.rope_partial_full), self.device),
                      0: rope_freq(cfg.rope_theta_slide, dims(cfg.rope_partial_slide), self.device)}
-        self.caches = [PagedCache(pages, page_tokens, cfg.kv_heads, cfg.head_dim, self.device) for _ in range(cfg.layers)]
+        cache = PagedCache if kv_bits == 8 else Paged4Cache
+        self.caches = [cache(pages, page_tokens, cfg.kv_heads, cfg.head_dim, self.device) for _ in range(cfg.layers)]
         self.table = PageTable(pages, page_tokens)
         self.len: dict = {}
         torch.cuda.synchronize(self.device)
@@ -170,14 +177,20 @@ class PagedScorer:
         new_ = lambda width: torch.empty(rows, width, device=dev)  # noqa: E731
         qkv, gate, att = new_(cfg.q_dim + 2 * cfg.kv_dim), new_(cfg.heads), new_(cfg.q_dim)
         ga, up, logits = new_(cfg.inter), new_(cfg.inter), new_(cfg.vocab)
-        batch = PagedBatch(self.caches[0], row0, kv_len, table, rows=rows, heads=cfg.heads)
+        batch = (PagedBatch if self.kv_bits == 8 else Paged4Batch)(self.caches[0], row0, kv_len, table, rows=rows, heads=cfg.heads)
         for (m, in_norm, post_norm), cache, full in zip(self.layers, self.caches, cfg.full):
             batch.use(cache)
             freq = self.freq[int(bool(full))]
             m["qkv"](h, qkv, in_norm, cfg.eps)
             m["attn_gate"](h, gate, in_norm, cfg.eps)
-            batch.append(qkv[:, cfg.q_dim:cfg.q_dim + cfg.kv_dim], qkv[:, cfg.q_dim + cfg.kv_dim:], freq=freq)
-            batch.attention(qkv[:, :cfg.q_dim], att, window=0 if full else cfg.window, freq=freq, gate=gate)
+            q, k, v = qkv[:, :cfg.q_dim], qkv[:, cfg.q_dim:cfg.q_dim + cfg.kv_dim], qkv[:, cfg.q_dim + cfg.kv_dim:]
+            window = 0 if full else cfg.window
+            if self.kv_bits == 8:
+                batch.append(k, v, freq=freq)
+                batch.attention(q, att, window=window, freq=freq, gate=gate)
+            else:
+                batch.append(k, v, freq=freq, q=q, q_out=q)
+                batch.attention(q, att, window=window, gate=gate)
             m["out"](att, h, accumulate=True)
             m["gate"](h, ga, post_norm, cfg.eps)
             m["up"](h, up, post_norm, cfg.eps)
@@ -222,11 +235,12 @@ def main() -> None:
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--sequences", type=int, default=12)
     ap.add_argument("--tokens", type=int, default=200, help="of the longest sequence")
+    ap.add_argument("--kv-bits", type=int, default=8, choices=(8, 4), help="of the cache")
     a = ap.parse_args()
     cfg = small_config(layers=a.layers)
     rng = np.random.default_rng(0)
     seqs = {i: rng.integers(0, cfg.vocab, max(2, a.tokens * (i + 1) // a.sequences)).tolist() for i in range(a.sequences)}
-    scorer = PagedScorer(cfg, synth_weights(cfg, seed=1, exact_q80=True), pages=sum(len(t) // 32 + 1 for t in seqs.values()), page_tokens=32)
+    scorer = PagedScorer(cfg, synth_weights(cfg, seed=1, exact_q80=True), pages=sum(len(t) // 32 + 1 for t in seqs.values()), page_tokens=32, kv_bits=a.kv_bits)
     scorer.feed(seqs)
     for s in seqs:
         scorer.release(s)

@@ -333,6 +333,9 @@ def want_attention(c, q, window=0, gate=None, scale=0.0):
         if n == 0:
             continue
         ks, vs = c.cached(s, "k"), c.cached(s, "v")
+        bad = ~(vs.isfinite().all(-1) & ks.isfinite().all(-1))     # [kv][j]: scale bytes from 248 on are no numbers
+        vs = torch.where(vs.isfinite(), vs, torch.zeros_like(vs))
+        ks = torch.where(ks.isfinite(), ks, torch.zeros_like(ks))
         qq = q[at:at + n].double().reshape(n, c.kv, c.heads // c.kv, c.hd)
         i, j = torch.arange(L - n, L, device=q.device)[:, None], torch.arange(L, device=q.device)
         see = (j <= i) & (j > i - window) if window else j <= i
@@ -342,14 +345,13 @@ def want_attention(c, q, window=0, gate=None, scale=0.0):
         w = w.masked_fill(hide, float("-inf"))
         p = torch.softmax(w, -1)
         p = torch.where(hide, torch.zeros_like(p), p)       # a row that sees nothing: 0
-        o = torch.einsum("nkgj,kjd->nkgd", p, vs.nan_to_num())
-        W = torch.einsum("nkgj,kjd->nkgd", p, vs.nan_to_num().abs())
-        bad = (vs.isnan().any(-1) | ks.isnan().any(-1))     # [kv][j]
+        o = torch.einsum("nkgj,kjd->nkgd", p, vs)
+        W = torch.einsum("nkgj,kjd->nkgd", p, vs.abs())
         hit = (see[:, None] & bad[None]).any(-1)            # [n][kv]
         o[hit] = float("nan")
-        S = size.masked_fill(hide, 0).nan_to_num().amax(-1, keepdim=True)
+        S = size.masked_fill(hide, 0).amax(-1, keepdim=True)
         t = W * ((2.0 ** -21 if two else 2.0 ** -11) + 2.0 ** -20 * S + 2.0 ** -22 * (64 + L / 64) + 2.0 ** -20)
-        seen = torch.einsum("nj,kjd->nkd", see.double(), vs.nan_to_num().abs())
+        seen = torch.einsum("nj,kjd->nkd", see.double(), vs.abs())
         t = t + (2.0 ** -35 if two else 2.0 ** -31) * p.amax(-1, keepdim=True) * seen[:, :, None]
         out.append(o.reshape(n, c.heads, c.hd))
         tol.append(t.reshape(n, c.heads, c.hd))
@@ -392,6 +394,14 @@ ATTNS = [
     ([300], [1000], 1, 256, 128, 4, 17),
     ([64, 40], [3, 0], 3, 128, 16, 3, 1),
     ([5], [40], 1, 64, 16, 40, 0),
+    # few rows and many in one call, both sides of where another kernel has them
+    ([70, 1, 33, 5, 90, 0, 22], [0, 300, 64, 7, 1000, 5, 2], 2, 256, 64, 6, 0),
+    ([70, 1, 33, 5, 90, 0, 22], [0, 300, 64, 7, 1000, 5, 2], 3, 128, 16, 9, 0),
+    ([65, 64, 63, 1, 200, 2], [31, 32, 33, 0, 15, 900], 2, 64, 48, 2, 0),
+    ([40, 130, 17, 3, 1, 66], [900, 5, 0, 64, 128, 300], 2, 128, 32, 8, 50),
+    ([129], [5000], 2, 256, 16, 6, 0),
+    ([33] * 20, [70 * i for i in range(20)], 1, 256, 32, 4, 0),
+    ([257, 300], [0, 1], 8, 64, 16, 8, 7),
 ]
 
 
@@ -408,14 +418,16 @@ def test_long_context(cuda):
     for typ, hd, kv, heads in (("f32", 256, 2, 8), ("bf16", 128, 1, 8), ("f16", 64, 2, 2)):
         c = Case(cuda, [1], [70000], kv, hd, 128, heads, seed=2)
         check_attention(c, c.randn(heads * hd, typ, 0.3), typ)
-        c = Case(cuda, [40], [20000], kv, hd, 128, heads, seed=3)
-        check_attention(c, c.randn(heads * hd, typ, 0.3), typ)
+        for rows in (40, 300):
+            c = Case(cuda, [rows], [20000], kv, hd, 128, heads, seed=3)
+            check_attention(c, c.randn(heads * hd, typ, 0.3), typ)
 
 
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
-def test_queries_of_any_size(cuda, typ):
+@pytest.mark.parametrize("rows", [[6, 40], [6, 150]])
+def test_queries_of_any_size(cuda, rows, typ):
     """Rows of zeros, tiny and huge ones beside each other; scores past f32's range are none of an exact form's either."""
-    c = Case(cuda, [6, 40], [30, 5], 1, 128, 16, 2, seed=4)
+    c = Case(cuda, rows, [30, 5], 1, 128, 16, 2, seed=4)
     q = c.randn(256, typ)
     size = [0.0, 2.0 ** -14, 1.0, 100.0, 1e-3, 1e4]
     for r in range(q.shape[0]):
@@ -429,7 +441,7 @@ def test_queries_of_any_size(cuda, typ):
 
 
 @pytest.mark.parametrize("typ", ["f32", "bf16"])
-@pytest.mark.parametrize("rows", [[4, 2], [90, 41]])
+@pytest.mark.parametrize("rows", [[4, 2], [90, 41], [200, 141]])
 def test_poison_reaches_the_rows_that_see_it(cuda, rows, typ):
     """NaN groups of keys and of values: rows before them, of other sequences and other KV heads stay."""
     c = Case(cuda, rows, [60, 17], 2, 128, 16, 4, seed=8)
@@ -446,7 +458,7 @@ def test_scores_far_from_zero_and_one_key_that_takes_all(cuda):
     import torch
 
     for typ in ("f32", "f16", "bf16"):
-        c = Case(cuda, [2, 60], [300, 100], 1, 64, 16, 4, seed=9)
+        c = Case(cuda, [2, 90], [300, 100], 1, 64, 16, 4, seed=9)
         q = c.randn(256, typ)
         for scale in (3.0, -3.0):
             check_attention(c, q, typ, scale=scale)
@@ -464,7 +476,7 @@ def test_rows_that_see_nothing_and_rows_of_nobody(cuda):
 
     from spk import paged4
 
-    for n in (3, 70):
+    for n in (3, 70, 150):
         c = Case(cuda, [n, n], [0, 20], 2, 64, 16, 4, seed=10)
         c.kv_len[0] = n - 2
         q = c.randn(256, "f32")
@@ -512,7 +524,11 @@ def test_bad_pages_are_reported_and_nothing_is_read_outside(cuda):
 
     c = Case(cuda, [4, 5], [30, 40], 2, 64, 16, 4, seed=13)
     was = [t.clone() for t in (c.cache.k_pool, c.cache.k_scale)]
-    for bad in (-1, c.cache.pages, 1 << 30):
+    many = Case(cuda, [150, 160], [30, 40], 2, 64, 16, 4, seed=13)
+    for bad in (-1, c.cache.pages, 1 << 30, -(1 << 31)):
+        many.tab[1, 0] = bad if bad != c.cache.pages else many.cache.pages
+        many.batch.attention(many.randn(256, "bf16"))
+        assert check_errors() != 0 and check_errors() == 0
         c.tab[1, 0] = bad                                   # a page of the cached tokens, then of the new ones
         c.batch.attention(c.randn(256, "f32"))
         assert check_errors() != 0 and check_errors() == 0
@@ -572,11 +588,12 @@ def test_a_run_of_them_in_a_graph_on_another_stream(cuda):
 def test_attention_repeats_itself(cuda):
     import torch
 
-    c = Case(cuda, [1] * 9 + [50], [3000] * 9 + [900], 2, 256, 64, 8, seed=15)
-    q = c.randn(2048, "bf16")
-    first = c.batch.attention(q)
-    for _ in range(5):
-        assert torch.equal(first, c.batch.attention(q))
+    for rows, old in (([1] * 9 + [50], [3000] * 9 + [900]), ([1], [60000]), ([300], [9000]), ([70] * 3, [3000] * 3)):
+        c = Case(cuda, rows, old, 2, 256, 64, 8, seed=15)
+        q = c.randn(2048, "bf16")
+        first = c.batch.attention(q)
+        for _ in range(5):
+            assert torch.equal(first, c.batch.attention(q))
 
 
 def test_a_row_does_not_depend_on_the_other_rows(cuda):
@@ -626,6 +643,23 @@ def test_what_the_binding_refuses(cuda):
             f()
             pytest.fail(f"call {i} was taken")
     assert check_errors() == 0
+
+
+def test_references_past_any_unit(cuda):
+    """Scores so large that a unit of them is more than the weights' range: the largest key takes all, as in f32."""
+    import torch
+
+    for rows in ([2], [300]):
+        for typ in ("f32", "bf16"):
+            c = Case(cuda, rows, [100], 1, 64, 16, 2, seed=17)
+            c.cache.k_pool.copy_(c.cache.k_pool & 0x77)     # positive keys, one of them the largest by far
+            c.cache.k_scale[c.cache.k_scale != 255] = 100
+            c.cache.k_scale[c.table[0][0], 0, 3] = 140
+            c.cache.k_pool[c.table[0][0], 0, 3] = 0x77
+            q = torch.full((rows[0], 128), 1e4, device=cuda).to(ttype(typ))
+            got = c.batch.attention(q, scale=1e20)
+            want = numbers(c.cache.v_pool[c.table[0][0], 0, 3], c.cache.v_scale[c.table[0][0], 0, 3])
+            assert (got.double() - want.repeat(2)).abs().max() <= HALF[typ] * want.abs().max(), (rows, typ)
 
 
 def test_calls_without_rows(cuda):
