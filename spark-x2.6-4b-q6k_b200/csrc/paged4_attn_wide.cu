@@ -98,33 +98,6 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-// 8 values of a row
-template <typename T>
-__device__ __forceinline__ void row8(const T *p, bool vec, float *x) {
-    if constexpr (sizeof(T) == 4) {
-        if (vec) {
-            const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-            return;
-        }
-    } else if (vec) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (__is_same(T, __half)) {
-                const float2 f = unpack_f16(w[i]);
-                x[2 * i] = f.x, x[2 * i + 1] = f.y;
-            } else {
-                x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = to_f32<T>(p[i]);
-}
-
 // What a softmax thread knows of its row
 struct Row {
     float up, sig;                                      // factor of its scores, sigmoid of its gate
@@ -202,6 +175,119 @@ __device__ __noinline__ void join(const AttnParams &a, int f0, int rows, float *
             }
         }
     }
+}
+
+// A warp's queries, `rows` of 32 (src: where this thread's lies), to where the MMAs read them. Returns the factor of the row's scores. Not inlined: the
+// loads on their way would cost the main loop its registers.
+template <typename C, bool VEC>
+__device__ __noinline__ float queries_in(const AttnParams &a, uint8_t *smem, uint8_t *stg, uint32_t mine, long long src, int rows, uint64_t *q_full) {
+    using T = typename C::T;
+    constexpr int HD = C::HD, LPR = HD / 8, GH = 32 / LPR, B = sizeof(T) == 4 ? 4 : 8;   // lanes of a row, rows of a load, loads on their way
+    constexpr bool TWO = C::TWO;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    struct Eight {                                                    // values of a row, as they lie or (unaligned rows) as they are
+        uint4 w[sizeof(T) == 4 || !VEC ? 2 : 1];
+        __device__ __forceinline__ void load(const T *p) {
+            if constexpr (VEC) {
+                w[0] = __ldg(reinterpret_cast<const uint4 *>(p));
+                if constexpr (sizeof(T) == 4) w[1] = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
+            } else {
+                float *x = reinterpret_cast<float *>(w);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = to_f32<T>(p[i]);
+            }
+        }
+        __device__ __forceinline__ void f32(float (&x)[8]) const {
+            const uint32_t v[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+            if constexpr (sizeof(T) == 4 || !VEC) {
+                const uint32_t u[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = __uint_as_float(v[i]), x[4 + i] = __uint_as_float(u[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if constexpr (__is_same(T, __half)) {
+                        const float2 f = unpack_f16(v[i]);
+                        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+                    } else {
+                        x[2 * i] = __uint_as_float(v[i] << 16), x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+                    }
+                }
+            }
+        }
+    };
+    float up = 0.f;
+    if (rows > 0) {   // rows past the last one have its values, which nobody reads
+        float mx = 0.f;
+#pragma unroll 1
+        for (int i0 = 0; i0 < LPR; i0 += B) {                         // the rows' largest
+            Eight raw[B];
+#pragma unroll
+            for (int i = 0; i < B; i++) {
+                const long long at = __shfl_sync(0xffffffffu, src, min((i0 + i) * GH + lane / LPR, rows - 1));
+                raw[i].load((const T *)a.q + at + 8 * (lane % LPR));
+            }
+#pragma unroll
+            for (int i = 0; i < B; i++) {
+                float x[8], y = 0.f;
+                raw[i].f32(x);
+#pragma unroll
+                for (int e = 0; e < 8; e++) y = fmaxf(y, fabsf(x[e]));
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
+                y = __shfl_sync(0xffffffffu, y, (lane % GH) * LPR);
+                if (lane / GH == i0 + i) mx = y;
+            }
+        }
+        const int e = mx > 0.f && mx < INFINITY ? min(14 - ilogbf(mx), 126) : 0;   // 2^e brings the largest into [2^14, 2^15)
+        const float f = __int_as_float((e + 127) << 23);
+        up = a.scale * __int_as_float((127 - e) << 23);
+#pragma unroll 1
+        for (int c = 0; c < HD / 64; c++) {                           // 64 dims
+#pragma unroll 1
+            for (int i0 = 0; i0 < 8; i0 += B) {
+                Eight raw[B];
+#pragma unroll
+                for (int i = 0; i < B; i++) {
+                    const long long at = __shfl_sync(0xffffffffu, src, min(4 * (i0 + i) + lane / 8, rows - 1));
+                    raw[i].load((const T *)a.q + at + 64 * c + 8 * (lane % 8));
+                }
+#pragma unroll
+                for (int i = 0; i < B; i++) {
+                    const int rr = 4 * (i0 + i) + lane / 8, pc = lane % 8;
+                    const float fr = __shfl_sync(0xffffffffu, f, min(rr, rows - 1));
+                    float x[8];
+                    raw[i].f32(x);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int z = 0; z < 4; z++) {
+                        const float p = x[2 * z] * fr, q = x[2 * z + 1] * fr;
+                        hi[z] = pack_f16(p, q);
+                        const float2 b = unpack_f16(hi[z]);
+                        lo[z] = pack_f16(p - b.x, q - b.y);
+                    }
+                    const uint32_t to = rr * 128 + ((pc ^ (rr & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(stg + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (TWO) *reinterpret_cast<uint4 *>(smem + C::Q_OFF + c * QCH + warp * 4096 + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+            }
+            __syncwarp();
+            uint32_t w[32];
+#pragma unroll
+            for (int y = 0; y < 8; y++) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(stg + lane * 128 + ((y ^ (lane & 7)) << 4));
+                w[4 * y] = v.x, w[4 * y + 1] = v.y, w[4 * y + 2] = v.z, w[4 * y + 3] = v.w;
+            }
+            __syncwarp();
+            tm_st32(mine + C::QC + 32 * c, w);
+        }
+        tm_wait_st();
+        tc_before();
+        if constexpr (TWO) fence_proxy_async();
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full);
+    return up;
 }
 
 template <typename C>
@@ -470,67 +556,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 if (a.gate) row.sig = 1.0f / (1.0f + __expf(-to_f32<T>(((const T *)a.gate)[(long long)(g.r0 + tok) * a.ldgate + h])));
             }
             if (tiles_of(g) == 0) return row;
-            // the rows' largest: HD / 8 lanes a row
-            constexpr int LPR = HD / 8, GH = 32 / LPR;
-            float mx = 0.f;
-#pragma unroll 4
-            for (int it = 0; it < LPR; it++) {
-                const int rr = it * GH + lane / LPR;
-                const long long at = __shfl_sync(0xffffffffu, src, rr);
-                float y = 0.f;
-                if (rr < rows) {
-                    float x[8];
-                    row8<T>((const T *)a.q + at + 8 * (lane % LPR), qvec, x);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) y = fmaxf(y, fabsf(x[i]));
-                }
-#pragma unroll
-                for (int o = LPR / 2; o > 0; o >>= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
-                y = __shfl_sync(0xffffffffu, y, (lane % GH) * LPR);
-                if (lane / GH == it) mx = y;
-            }
-            const int e = mx > 0.f && mx < INFINITY ? min(14 - ilogbf(mx), 126) : 0;   // 2^e brings the largest into [2^14, 2^15)
-            const float f = __int_as_float((e + 127) << 23);
-            row.up = a.scale * __int_as_float((127 - e) << 23);
-            for (int c = 0; c < HD / 64; c++) {
-#pragma unroll 4
-                for (int it = 0; it < 8; it++) {
-                    const int rr = 4 * it + lane / 8, pc = lane % 8;
-                    const long long at = __shfl_sync(0xffffffffu, src, rr);
-                    const float fr = __shfl_sync(0xffffffffu, f, rr);
-                    float x[8];
-                    if (rr < rows) row8<T>((const T *)a.q + at + 64 * c + 8 * pc, qvec, x);
-                    else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = 0.f;
-                    }
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float p = x[2 * i] * fr, q = x[2 * i + 1] * fr;
-                        hi[i] = pack_f16(p, q);
-                        const float2 b = unpack_f16(hi[i]);
-                        lo[i] = pack_f16(p - b.x, q - b.y);
-                    }
-                    const uint32_t to = rr * 128 + ((pc ^ (rr & 7)) << 4);
-                    *reinterpret_cast<uint4 *>(stg + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if constexpr (TWO) *reinterpret_cast<uint4 *>(smem + C::Q_OFF + c * QCH + warp * 4096 + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
-                __syncwarp();
-                uint32_t w[32];
-#pragma unroll
-                for (int y = 0; y < 8; y++) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(stg + own + ((y ^ cut) << 4));
-                    w[4 * y] = v.x, w[4 * y + 1] = v.y, w[4 * y + 2] = v.z, w[4 * y + 3] = v.w;
-                }
-                __syncwarp();
-                tm_st32(mine + C::QC + 32 * c, w);
-            }
-            tm_wait_st();
-            tc_before();
-            if constexpr (TWO) fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full);
+            row.up = qvec ? queries_in<C, true>(a, smem, stg, mine, src, rows, &q_full) : queries_in<C, false>(a, smem, stg, mine, src, rows, &q_full);
             return row;
         };
         Row row = queries(sg);
