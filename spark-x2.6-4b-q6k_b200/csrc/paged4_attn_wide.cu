@@ -100,9 +100,8 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 }
 // What a softmax thread knows of its row
 struct Row {
-    float up, sig;                                      // factor of its scores, sigmoid of its gate
+    float up;                                           // factor of its scores
     int pos, low;                                       // it sees the tokens (low, pos]
-    long long out;                                      // where its output lies (-1: no row)
 };
 
 // The sum of n parts (32 at most) of the group that begins at CTA f0, `step` apart from part `at` on, by the softmax warps: to the outputs, or to the first
@@ -538,37 +537,50 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
     } else {
         const int r = tid;
         const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);   // the warp's lanes of tensor memory
-        __shared__ float sig_s[R];
-        __shared__ long long out_s[R];
+        // What a tile does not need lies in shared memory, so that the loop's registers hold what it does: the groups, and per row the
+        // sigmoid of its gate and where its output lies (-1: no row), of this group and the next
+        __shared__ Seg soft_s[2];
+        __shared__ float sig_s[2][R];
+        __shared__ long long out_s[2][R];
         uint32_t tc = 0, groups = 0;
         uint8_t *stg = smem + C::STG_OFF + warp * 4096;               // 32 rows of 128 bytes, 16-byte pieces spread as their row says
         const uint32_t own = lane * 128, cut = lane & 7;              // this thread's row of them
         // the row of a group that is this thread's, its queries to where the MMAs read them
-        auto queries = [&](const Seg &g) {
-            Row row{0.f, 1.f, -1, -1, -1};
+        auto queries = [&](int side) {
+            const Seg &g = soft_s[side];
+            Row row{0.f, -1, -1};
             if (g.k0 < 0) return row;
             const int col = g.c0 + r, tok = col / a.group, h = g.kvh * a.group + col % a.group, rows = g.c1 - g.c0 + 1 - 32 * warp;   // of this warp
             const long long src = (long long)(g.r0 + tok) * a.ldq + (long long)h * HD;
+            float sig = 1.f;
+            long long out = -1;
             if (col <= g.c1) {
                 row.pos = g.pos0 + tok;
                 row.low = a.window > 0 ? row.pos - a.window : -1;
-                row.out = (long long)(g.r0 + tok) * a.ldout + (long long)h * HD;
-                if (a.gate) row.sig = 1.0f / (1.0f + __expf(-to_f32<T>(((const T *)a.gate)[(long long)(g.r0 + tok) * a.ldgate + h])));
+                out = (long long)(g.r0 + tok) * a.ldout + (long long)h * HD;
+                if (a.gate) sig = 1.0f / (1.0f + __expf(-to_f32<T>(((const T *)a.gate)[(long long)(g.r0 + tok) * a.ldgate + h])));
             }
+            sig_s[side][r] = sig;
+            out_s[side][r] = out;
             if (tiles_of(g) == 0) return row;
             row.up = qvec ? queries_in<C, true>(a, smem, stg, mine, src, rows, &q_full) : queries_in<C, false>(a, smem, stg, mine, src, rows, &q_full);
             return row;
         };
-        Row row = queries(sg);
-        while (sg.k0 >= 0) {
-            const int n = tiles_of(sg);
+        auto group_is = [&](int side, const Seg &g) {
+            if (tid == 0) soft_s[side] = g;
+            bar_sync(1, SM_WARPS * 32);
+        };
+        group_is(0, sg);
+        Row row = queries(0);
+        for (int cur = 0; soft_s[cur].k0 >= 0; cur ^= 1) {
+            const int n = tiles_of(soft_s[cur]), start = soft_s[cur].start + soft_s[cur].k0 * N;
             float m = -INFINITY, l0 = 0.f, l1 = 0.f;
             for (int j = 0; j < n; j++) {
                 const uint32_t i = tc & 1;
                 wait_for(s_full + i, (tc >> 1) & 1, &dead, a.err);
                 __syncwarp();
                 tc_after();
-                const int t0 = sg.start + (sg.k0 + j) * N;
+                const int t0 = start + j * N;
                 const bool edge = __any_sync(0xffffffffu, t0 + N - 1 > row.pos || t0 <= row.low);
                 const uint32_t b0 = *(volatile uint32_t *)&bad[tc & 3][0], b1 = *(volatile uint32_t *)&bad[tc & 3][1];   // tokens with poisoned values
                 // The weights under the reference as it stands, and the largest score. Where one is too large (and at a group's start) the
@@ -672,9 +684,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 tc++;
             }
             // the next group's queries, then this one's outputs
-            const Seg nx = next();
-            const Row rn = queries(nx);
-            const bool whole = sg.f0 == sg.f1, real = row.out >= 0;
+            group_is(cur ^ 1, next());
+            row = queries(cur ^ 1);
+            const Seg &sg = soft_s[cur];
+            const bool whole = sg.f0 == sg.f1;
+            const long long row_out = out_s[cur][r];
             const float l = l0 + l1;
             float *slot = a.part + ((size_t)blockIdx.x * 2 + (sg.k0 == 0 ? 1 : 0)) * part_floats(R, HD);
             if (n > 0) {
@@ -682,7 +696,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 __syncwarp();
                 tc_after();
             }
-            const float f = !whole ? 1.0f : l == 0.f ? 0.f : row.sig / l;
+            const float f = !whole ? 1.0f : l == 0.f ? 0.f : sig_s[cur][r] / l;
             const int mrows = sg.c1 - sg.c0 + 1 - 32 * warp;          // rows of this warp
             // 32 columns of outputs at a time; rows leave by 16-byte pieces, eight lanes a row
             auto leave = [&](uint8_t *base, long long to, int size, int c, bool vec) {   // a row's 128 bytes, from byte `to` + 128 c of base on
@@ -720,7 +734,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
 #pragma unroll
                     for (int y = 0; y < 8; y++) *reinterpret_cast<float4 *>(stg + own + ((y ^ cut) << 4)) = make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
                     if (!whole) leave((uint8_t *)slot, (long long)r * HD * 4, 4, c, true);
-                    else leave((uint8_t *)a.out, row.out * 4, 4, c, ovec);
+                    else leave((uint8_t *)a.out, row_out * 4, 4, c, ovec);
                 } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
@@ -729,7 +743,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                         for (int z = 0; z < 8; z++) v[z] = from_f32<T>(o[8 * y + z]);
                         *reinterpret_cast<uint4 *>(stg + own + (((4 * (c & 1) + y) ^ cut) << 4)) = *reinterpret_cast<const uint4 *>(v);
                     }
-                    if (c & 1) leave((uint8_t *)a.out, row.out * 2, 2, c >> 1, ovec);
+                    if (c & 1) leave((uint8_t *)a.out, row_out * 2, 2, c >> 1, ovec);
                 }
             }
             if (n > 0) {
@@ -741,12 +755,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             if (!whole) {
                 // parts are added in CTA order; many of them in two steps (paged4_attn.cu)
                 const int parts = sg.f1 - sg.f0 + 1, mine_p = (int)blockIdx.x - sg.f0, runs = parts > 2 * RUN ? (parts + RUN - 1) / RUN : 1;
-                if (real) {
+                if (row_out >= 0) {
                     slot[R * HD + r] = l == 0.f ? -INFINITY : m;
                     slot[R * HD + R + r] = l;
                 }
-                sig_s[r] = row.sig;
-                out_s[r] = row.out;
                 auto last_of = [&](unsigned int *ticket, int count) {
                     bar_sync(1, SM_WARPS * 32);
                     if (tid == 0) {
@@ -762,18 +774,17 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                 float *wt = reinterpret_cast<float *>(smem + C::STG_OFF);
                 const int rows = sg.c1 - sg.c0 + 1;
                 if (runs == 1) {
-                    if (last_of(a.tickets + sg.f0, parts)) join<C>(a, sg.f0, rows, wt, sig_s, out_s, 0, 1, parts, true, ovec);
+                    if (last_of(a.tickets + sg.f0, parts)) join<C>(a, sg.f0, rows, wt, sig_s[cur], out_s[cur], 0, 1, parts, true, ovec);
                 } else {
                     const int run = mine_p / RUN, count = min(RUN, parts - run * RUN);
                     if (last_of(a.tickets + MAX_CTAS * (run == 0 ? 1 : 2) + sg.f0 + run * RUN, count)) {
-                        join<C>(a, sg.f0, rows, wt, sig_s, out_s, run * RUN, 1, count, false, ovec);
-                        if (last_of(a.tickets + sg.f0, runs)) join<C>(a, sg.f0, rows, wt, sig_s, out_s, 0, RUN, runs, true, ovec);
+                        join<C>(a, sg.f0, rows, wt, sig_s[cur], out_s[cur], run * RUN, 1, count, false, ovec);
+                        if (last_of(a.tickets + sg.f0, runs)) join<C>(a, sg.f0, rows, wt, sig_s[cur], out_s[cur], 0, RUN, runs, true, ovec);
                     }
                 }
-                bar_sync(1, SM_WARPS * 32);   // sig_s, out_s and last_s are free again
+                bar_sync(1, SM_WARPS * 32);   // last_s is free again, and the staging
             }
-            sg = nx;
-            row = rn;
+            bar_sync(1, SM_WARPS * 32);       // the group is done with: its place is the one behind the next's
         }
     }
     tc_before();
