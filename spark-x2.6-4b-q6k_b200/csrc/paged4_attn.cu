@@ -647,11 +647,6 @@ constexpr int MAX_CTAS = 3;                             // of an SM
 
 template <typename C>
 int launch_one(const AttnParams &a, cudaStream_t s, const char *who) {
-    // the line of work, at its longest: every row tile as long as the page table and a tile's tokens (before())
-    const long long tiles = (long long)a.b.rows * a.group / R + a.b.nseq;
-    const long long blocks = ((long long)a.b.max_pages * a.pool.page_tokens + R / a.group + 3 + (tiles >> 15)) / BLOCK + COST + 4;
-    if ((double)tiles * blocks * a.pool.kv_heads > 2147483000.0)
-        return set_error("%s: %d rows over up to %d pages of %d tokens are too much for one call", who, a.b.rows, a.b.max_pages, a.pool.page_tokens);
     static bool set[64];
     int dev = 0;
     cudaGetDevice(&dev);
@@ -720,7 +715,16 @@ int spk_paged4_attn(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
     a.err = device_error_ptr();
     const cudaStream_t s = (cudaStream_t)stream;
     const long long narrow = (long long)batch->nseq * pool->kv_heads <= FEW_PAIRS ? NARROW_FEW : NARROW;
-    if ((long long)batch->rows * a.group > narrow) {   // some sequence may have many rows
+    // the lines of work, at their longest: every row tile as long as the page table and a tile's tokens (before()); here a sequence has
+    // `narrow` rows at most
+    const bool many = (long long)batch->rows * a.group > narrow;          // some sequence may have more
+    const double tokens = (double)batch->max_pages * pool->page_tokens, pairs = pool->kv_heads;
+    const double here = fmin((double)batch->rows * a.group / R, (double)batch->nseq * (narrow / R)) + batch->nseq;
+    const double there = (double)batch->rows * a.group / WIDE_R + batch->nseq;
+    auto line = [&](double tiles, int R_, int cost) { return tiles * ((tokens + R_ / a.group + 3 + tiles / 32768) / BLOCK + cost + 5) * pairs; };
+    if (line(here, R, COST) > 2147483000.0 || (many && line(there, WIDE_R, WIDE_COST) > 2147483000.0))
+        return set_error("%s: %d rows over up to %d pages of %d tokens are too much for one call", who, batch->rows, batch->max_pages, pool->page_tokens);
+    if (many) {
         a.from = narrow + 1;
         a.to = LLONG_MAX;
         const int rc = attn_wide(a, p->type, s, who);

@@ -25,7 +25,7 @@ constexpr int N = 64, TB = N / BLOCK;                   // tokens of a tile, its
 constexpr int R = WIDE_R;
 constexpr int QCH = R * 128;                            // 64 dims of the queries' second terms
 constexpr int SM_WARPS = 4, DQ_WARPS = 8, MMA_WARP = SM_WARPS + DQ_WARPS, WARPS = MMA_WARP + 1, THREADS = WARPS * 32;
-constexpr int COST = 64;                                // a group's fixed cost in blocks
+constexpr int COST = WIDE_COST;
 constexpr int RUN = 16, MAX_CTAS = 512;                 // parts that are added together (a join takes 32); CTAs of a call
 
 template <typename T_, int HD_>
@@ -797,11 +797,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
 
 template <typename C>
 int launch_one(const AttnParams &a, cudaStream_t s, const char *who) {
-    // the line of work, at its longest: every row tile as long as the page table and a tile's tokens (before())
-    const long long tiles = (long long)a.b.rows * a.group / R + a.b.nseq;
-    const long long blocks = ((long long)a.b.max_pages * a.pool.page_tokens + R / a.group + 3 + (tiles >> 15)) / BLOCK + COST + 4;
-    if ((double)tiles * blocks * a.pool.kv_heads > 2147483000.0)
-        return set_error("%s: %d rows over up to %d pages of %d tokens are too much for one call", who, a.b.rows, a.b.max_pages, a.pool.page_tokens);
     static bool set[64];
     int dev = 0;
     cudaGetDevice(&dev);

@@ -402,6 +402,8 @@ ATTNS = [
     ([129], [5000], 2, 256, 16, 6, 0),
     ([33] * 20, [70 * i for i in range(20)], 1, 256, 32, 4, 0),
     ([257, 300], [0, 1], 8, 64, 16, 8, 7),
+    ([3], [40], 1, 64, 16, 200, 0),
+    ([9, 2], [100, 3], 1, 128, 16, 129, 30),
 ]
 
 
@@ -660,6 +662,24 @@ def test_references_past_any_unit(cuda):
             got = c.batch.attention(q, scale=1e20)
             want = numbers(c.cache.v_pool[c.table[0][0], 0, 3], c.cache.v_scale[c.table[0][0], 0, 3])
             assert (got.double() - want.repeat(2)).abs().max() <= HALF[typ] * want.abs().max(), (rows, typ)
+
+
+def test_long_prompts_of_several_sequences_are_taken(cuda):
+    """Two prompts over a table of 131072 tokens each, 8 heads a KV head: within the line of work of the kernel that has them."""
+    import torch
+
+    from spk import paged4
+
+    c = paged4.Paged4Cache(1024 + 2, 256, 4, 64, device=cuda)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    table = torch.zeros(2, 512, dtype=torch.int32, device=cuda)
+    rows = 262144
+    b = paged4.Paged4Batch(c, i32([0, 20, 40]), i32([20, 20]), table, rows=rows, heads=32)
+    k = torch.randn(rows, 256, device=cuda, dtype=torch.bfloat16)
+    b.append(k, k)
+    q = torch.randn(rows, 2048, device=cuda, dtype=torch.bfloat16)
+    b.attention(q, torch.empty_like(q))          # the arguments allow 262144 rows, the batch says 40
+    assert check_errors() == 0
 
 
 def test_calls_without_rows(cuda):

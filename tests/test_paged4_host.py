@@ -105,6 +105,15 @@ def test_attention_refuses_a_batch_past_its_line_of_work():
 
 
 @needs_lib
+def test_attention_refuses_many_sequences_past_the_line_of_work():
+    """1024 sequences of few rows over tables of 2^22 tokens, 64 KV heads: 1024 x 2^18 blocks x 64."""
+    p = pool(pages=1 << 20, page_tokens=1024, kv_heads=64)
+    b = batch(nseq=1024, rows=1024, max_pages=1 << 12)
+    assert call("spk_paged4_attn", p, b, attn_args(type=1, heads=64, ldq=64 * 128, ldout=64 * 128)) == -1
+    assert "too much" in spk.last_error()
+
+
+@needs_lib
 def test_no_rows_is_a_call_that_does_nothing():
     b = batch(rows=0)
     assert call("spk_paged4_append", pool(), b, paged4._Append4()) == 0
