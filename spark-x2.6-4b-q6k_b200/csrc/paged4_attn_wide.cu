@@ -397,12 +397,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             tc_after();
             if (ok && elect_one()) {
                 const uint32_t d = tmem + C::SC + i * N;
+                // f32 queries' second terms first, while the sum that each step rounds is small: against 64 bits the 13 f32 prompts of
+                // 20 to 700 rows are off by 1.1e-6 so, and by 1.5e-6 with the terms in turn; the time is the same
+                if constexpr (TWO) {
 #pragma unroll
-                for (int k = 0; k < HD / 16; k++) {
-                    const uint64_t b = desc(kb + i * C::TILE + (k / 4) * C::CH + (k % 4) * 32, 0);
-                    mma_ts(d, tmem + C::QC + 8 * k, b, id_s, k > 0);
-                    if constexpr (TWO) mma_ss(d, desc(qb + (k / 4) * QCH + (k % 4) * 32, 0), b, id_s, true);
+                    for (int k = 0; k < HD / 16; k++)
+                        mma_ss(d, desc(qb + (k / 4) * QCH + (k % 4) * 32, 0), desc(kb + i * C::TILE + (k / 4) * C::CH + (k % 4) * 32, 0), id_s, k > 0);
                 }
+#pragma unroll
+                for (int k = 0; k < HD / 16; k++)
+                    mma_ts(d, tmem + C::QC + 8 * k, desc(kb + i * C::TILE + (k / 4) * C::CH + (k % 4) * 32, 0), id_s, TWO || k > 0);
                 mma_commit(empty_k + i);
                 mma_commit(s_full + i);
             }
