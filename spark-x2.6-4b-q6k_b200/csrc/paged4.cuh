@@ -71,7 +71,7 @@ constexpr float W_TOP = 12.0f, W_MAX = 15.0f;
 
 // Floats of one CTA's part of a group of R query rows: O, then m, then l.
 __host__ __device__ constexpr int part_floats(int R, int hd) { return R * (hd + 2); }
-constexpr int WIDE_R = 128, WIDE_COST = 64;             // the kernel for many rows: query rows of a group, its fixed cost in blocks
+constexpr int WIDE_R = 128, WIDE_COST = 40;             // the kernel for many rows: query rows of a group, its fixed cost in blocks
 int attn_wide(const AttnParams &a, int type, cudaStream_t s, const char *who);   // paged4_attn_wide.cu
 
 }  // namespace paged4

@@ -9,11 +9,12 @@
 // Both are decided exactly: for d the f32 quotient's neighbour is checked against 6 (d + half a step), which f32 holds; the quotient
 // x / d is corrected by its own residual, so that a tie is a tie, and moved off a border that it was only rounded to.
 //
-// What bounds append: the rows' bytes, and beside them the shared-memory pipe (shuffles). A warp takes 256 values at a time (256 /
+// What bounds append: at the rows' bytes' rate the issue slots are half used (48 M warp instructions for 16384 rows of 24 heads, 122 for 256 values) and
+// a warp's chain (load, norm's tree of shuffles, rotation, scale, codes) waits for itself more often than for memory. A warp takes 256 values at a time (256 /
 // head_dim heads side by side), 8 consecutive ones a lane, which is one 16-byte load of 16-bit rows and one word of codes; a group is two lanes, a head's norm
 // a shuffle tree, the other half of a rotated pair 8 shuffles. A token's items (queries, keys, values) are one warp's where there are
 // many tokens, so that it looks its place up and computes its angles once, and several warps' where there are few; the norms' weights stay in
-// registers, the next items' rows are on their way. No warp waits for another.
+// registers, four items' rows are loaded before the first one's work. No warp waits for another. One token takes as long as its launch.
 #include "paged4.cuh"
 
 namespace spk {
@@ -32,11 +33,16 @@ int check_pool(const spk_kv4_pool *p, const char *who) {
 
 namespace {
 
+// Warps of an SM against registers a thread, and items whose loads go out and whose chains run together. 16384 bf16 rows (16 + 4 + 4 heads of
+// 256, normalised, rotated over 64 dims) take 94 us, 3.8 TB/s of rows, queries and cache, 58 % of the measured copy rate. With the read of codes and
+// scales behind it: 122 us so, 128 with one CTA less, 123 with one more, 139 with two items together, 128 with twice the warps in a CTA; 13 f32
+// prompts of up to 1501 rows 49, 59 with three CTAs, 57 with five. Rows through a ring of cp.async copies, more of them on their way, took 129 to 145
+// and 67: what it adds per item, in f32 two passes over each sector, costs more than the wait that it hides.
 constexpr int AP_WARPS = 4, AP_THREADS = AP_WARPS * 32;
 template <typename T>
 constexpr int AP_CTAS = sizeof(T) == 4 ? 4 : 5;                 // of an SM
 template <typename T>
-constexpr int AP_BATCH = 4;   // items whose loads go out together
+constexpr int AP_BATCH = 4;   // items
 
 struct AppendArgs {
     Pool pool;
@@ -399,7 +405,13 @@ struct Out<Codes> {
     using type = uint8_t;
 };
 
-constexpr int RD_THREADS = 128, RD_CTAS = 12;
+// Read is bound by issue slots (70 % used; a lane's 8 values take some 35 instructions) and needs warps to hide the lookups of places. 40 MB of
+// bf16 rows from 11 MB of cache take 16.7 us with 12 CTAs of an SM and two items' loads together, 48 % of the measured copy rate; 17.4 with four
+// items, 17.6 with 16 CTAs, 20.0 with 8. Codes and scales apart take fewer instructions: append and read of 13 f32 prompts 47.4 us with 16
+// CTAs, 49.6 with 12.
+constexpr int RD_THREADS = 128;
+template <typename T>
+constexpr int RD_CTAS = __is_same(T, Codes) ? 16 : 12;       // of an SM
 
 // e4m3 bytes of four codes
 __device__ __forceinline__ uint32_t code_bytes(uint32_t four) {
@@ -409,8 +421,8 @@ __device__ __forceinline__ uint32_t code_bytes(uint32_t four) {
 }
 
 template <typename T, int HD, bool VEC>
-__global__ void __launch_bounds__(RD_THREADS, RD_CTAS) read_kernel(const ReadArgs a) {
-    constexpr int LPR = HD / 8, GH = 256 / HD, BATCH = 4;          // lanes of a head, heads of a warp, items whose loads go out together
+__global__ void __launch_bounds__(RD_THREADS, RD_CTAS<T>) read_kernel(const ReadArgs a) {
+    constexpr int LPR = HD / 8, GH = 256 / HD, BATCH = 2;          // lanes of a head, heads of a warp, items whose loads go out together
     constexpr bool APART = __is_same(T, Codes);
     using O = typename Out<T>::type;
     __shared__ Rows rows;
@@ -495,7 +507,7 @@ cudaError_t launch_read(const ReadArgs &a, cudaStream_t s) {
     const int hd = a.pool.hd, per = 2 * ((a.pool.kv_heads + 256 / hd - 1) / (256 / hd));
     auto k = a.vec == 3 ? (hd == 256 ? read_kernel<T, 256, true> : hd == 128 ? read_kernel<T, 128, true> : read_kernel<T, 64, true>)
                         : (hd == 256 ? read_kernel<T, 256, false> : hd == 128 ? read_kernel<T, 128, false> : read_kernel<T, 64, false>);
-    return launch_pdl(k, dim3(ctas_of(a.b.rows, per, RD_THREADS / 32, RD_CTAS * sm_count())), dim3(RD_THREADS), 0, s, a);
+    return launch_pdl(k, dim3(ctas_of(a.b.rows, per, RD_THREADS / 32, RD_CTAS<T> * sm_count())), dim3(RD_THREADS), 0, s, a);
 }
 
 }  // namespace
