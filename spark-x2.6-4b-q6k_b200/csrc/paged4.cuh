@@ -1,4 +1,4 @@
-// paged4.cuh — what the paged 4-bit cache's kernels share (paged4_append.cu, paged4_attn.cu).
+// paged4.cuh — what the paged 4-bit cache's kernels share (paged4_append.cu, paged4_attn.cu, paged4_attn_wide.cu).
 //
 // A row of a KV head (head_dim values of one token) is kept as groups of 16 values: a code of 4 bits a value and a scale
 // byte a group, keys and values apart, 4.5 bits a value. Code c stands for 0, .5, 1, 1.5, 2, 3, 4, 6 (c & 7) with the
@@ -66,12 +66,13 @@ struct AttnParams {
     __device__ __forceinline__ bool takes(long long columns) const { return columns >= from && columns <= to; }
 };
 // Weights are f16 numbers 2^(s - m): a new reference m puts the row's largest at 2^W_TOP (the kernel for many rows: less), and it moves when
-// one passes 2^W_MAX. A weight is kept down to 2^-24, 2^-36 of the largest.
+// one passes 2^W_MAX. A weight is kept down to 2^-24: 2^-36 of the largest (many rows: 2^-34 in f32, 2^-30 in the 16-bit types).
 constexpr float W_TOP = 12.0f, W_MAX = 15.0f;
 
 // Floats of one CTA's part of a group of R query rows: O, then m, then l.
 __host__ __device__ constexpr int part_floats(int R, int hd) { return R * (hd + 2); }
-constexpr int WIDE_R = 128, WIDE_COST = 40;             // the kernel for many rows: query rows of a group, its fixed cost in blocks
+// the kernel for many rows: query rows of a group, its fixed cost in blocks (13 f32 prompts 125 us; 129 with 24, 130 with 64, 139 with 128)
+constexpr int WIDE_R = 128, WIDE_COST = 40;
 int attn_wide(const AttnParams &a, int type, cudaStream_t s, const char *who);   // paged4_attn_wide.cu
 
 }  // namespace paged4

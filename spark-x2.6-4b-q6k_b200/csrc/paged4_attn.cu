@@ -16,10 +16,18 @@
 // Queries stand on a power of two of their row (2^14 to 2^15 at the largest), weights are 2^(s - m) with the row's largest at
 // 2^12 to 2^15: a reference m moves only when a score passes it by 15, and a weight is kept down to 2^-24, 2^-36 of the
 // largest (half of it in its last bit). l adds the weights as they were rounded.
+// The matrix instructions cut their sums towards 0: a warp's 2048 blocks of values of one sign in one accumulator end up 1.5e-4 short. So f32 and f16
+// rows have a block's products in an accumulator of their own, added in f32 (1.1e-6; 131072 keys of one f32 row 50.7 -> 51.7 us, 24 x 8 f16 rows
+// 28.9 -> 29.2); bf16's half unit is 26 times what is lost.
 //
 // Work split: paged_line.cuh's line of groups of 8 query rows. A CTA's warps take a group's blocks of 16 tokens in turn, each
 // with a ring of its own that cp.async fills and a softmax of its own; they meet at the end of the group. Groups that
 // several CTAs share leave (O, m, l) in the workspace, and the last CTA to arrive adds the parts in CTA order.
+//
+// Measured: one f32 row of 16 heads on 4 of 256 over 131072 keys 51.8 us (151 MB of cache, 2.9 TB/s: some 600 warp instructions a block, 45 % of the
+// issue slots used by 8 warps an SM, 240 registers each), of which the start and the joining of 74 parts in two steps are some 15; 64 bf16 rows of up
+// to 9000 keys 33.2 us (48 MB); 24 x 8 f16 rows of 32 heads on 4 of 128 29.0 us; one row under a window of 512 14.8 us, launch, plan, queries, tiles and
+// joining each behind the one before.
 #include <limits.h>
 
 #include "paged4.cuh"
@@ -42,7 +50,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_CTAS_ALL = 512;                       // CTAs of a call: the parts of a group
 constexpr int RUN = 16, MAX_JOIN = 32;                  // parts that are added together; at most (a lane each)
 static_assert(2 * RUN <= MAX_JOIN && MAX_CTAS_ALL <= RUN * MAX_JOIN, "");
-constexpr int COST = 20;                                // a group's fixed cost in blocks
+constexpr int COST = 20;                                // a group's fixed cost in blocks (64 bf16 rows 33.3 us; 37.5 with 10, 45.9 with 5, 35.4 with 40)
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -384,7 +392,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
         uint32_t at_stage = 0;
 
         auto blocks = [&](auto spare_) {
-        constexpr bool SPARE = decltype(spare_)::value;
+        constexpr bool SPARE = decltype(spare_)::value, APART = !__is_same(typename C::T, __nv_bfloat16);
         for (int i = 0; i < count; i++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
             __syncwarp();
@@ -536,8 +544,15 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
                     const uint32_t a0 = hmul2(ae[x], sa), a1 = hmul2(ao[x], sa), a2 = hmul2(be[x], sb), a3 = hmul2(bo[x], sb);
-                    mma(acc[4 * y + x], a0, a1, a2, a3, p0, p1);
-                    if constexpr (C::TWO && !SPARE) mma(acc[4 * y + x], a0, a1, a2, a3, e0, e1);
+                    if constexpr (APART) {   // sums of blocks in f32 additions: the matrix instructions cut theirs towards 0
+                        float d[4] = {};
+                        mma(d, a0, a1, a2, a3, p0, p1);
+                        if constexpr (C::TWO && !SPARE) mma(d, a0, a1, a2, a3, e0, e1);
+#pragma unroll
+                        for (int z = 0; z < 4; z++) acc[4 * y + x][z] += d[z];
+                    } else {
+                        mma(acc[4 * y + x], a0, a1, a2, a3, p0, p1);
+                    }
                 }
             }
         }

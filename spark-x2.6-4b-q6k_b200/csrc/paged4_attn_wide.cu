@@ -11,6 +11,14 @@
 //
 // Work split: paged_line.cuh's line of groups of 128 rows, one CTA per SM. Warps: 0-3 queries, softmax and outputs,
 // 4-11 codes to f16, 12 the MMAs. Each walks the CTA's groups by itself; they meet at mbarriers.
+//
+// What bounds it: 2048 bf16 rows of 16 heads of 256 behind 6144 cached tokens are 240 GFLOP in 308 us, 0.78 PFLOP/s, 47 % of the measured
+// bf16 rate. A tile takes 1.6 us where its products take 0.76: the tensor pipe is busy 37 % of the time and 45 % of the issue slots are used; the
+// softmax warps are the longest chain (scores out of the tensor memory, exponentials, weights back), the converting warps nearly as long. Eight softmax
+// warps, two to 32 rows, would halve that chain, but 16 or 17 warps have 112 registers a thread or fewer: their loop spilled, 585 us and more (setmaxnreg
+// cannot help where the whole kernel is compiled for the launch's share). Outputs out of line (433 us for 368 then) and code of their own for keys,
+// values and every second tile (1.5 times) were slower too: the loops have to stay in the instruction cache. 13 f32 prompts of
+// up to 701 rows, 10 GFLOP counted once (f32 rows multiply twice), take 125 us: short groups of which several end in every CTA.
 #include "paged4.cuh"
 #include "paged_line.cuh"
 #include "paged_tc.cuh"
@@ -36,6 +44,9 @@ struct Cfg {
     // log2 of the largest weight at a new reference: the further under W_MAX, the fewer moves, each of which takes a warp's outputs
     // through its registers; a weight is kept down to 2^-24 under it.
     static constexpr float TOP = TWO ? 10.0f : 6.0f;
+    // Tiles whose outputs one accumulator adds. The tensor cores cut their sums towards 0, 4e-8 of what is there at each of a tile's 4 steps
+    // (f32: 8): 131072 keys of values of one sign ended up 6.6e-4 short. After a span f32 additions take the outputs over, in the workspace.
+    static constexpr int SPAN = TWO ? 32 : 256;
     static constexpr int TILE = N * HD * 2;             // bytes of a tile's keys (or values) in f16
     static constexpr int CH = N * 128;                  // 64 dims of them
     static constexpr int V_OFF = 2 * TILE, Q_OFF = 4 * TILE;
@@ -174,6 +185,40 @@ __device__ __noinline__ void join(const AttnParams &a, int f0, int rows, float *
             }
         }
     }
+}
+
+// A row's outputs and what `sums` has of it under another reference, f its factor (0: nothing yet): to there, or back to the tensor memory. A lane has its row
+// in 16-byte pieces 512 bytes apart, so that a warp's lie side by side.
+template <typename C, bool BACK>
+__device__ __noinline__ void take_over(uint32_t mine, float4 *sums, float f) {
+#pragma unroll 1
+    for (int c = 0; c < C::HD / 32; c++) {
+        float o[32];
+        float4 v[8];
+#pragma unroll
+        for (int y = 0; y < 8; y++) v[y] = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(sums + (8 * c + y) * 32);
+        tm_ld32(mine + 32 * c, o);
+        tm_wait_ld(o, 32);
+#pragma unroll
+        for (int y = 0; y < 8; y++) {
+            v[y].x = fmaf(v[y].x, f, o[4 * y]), v[y].y = fmaf(v[y].y, f, o[4 * y + 1]);
+            v[y].z = fmaf(v[y].z, f, o[4 * y + 2]), v[y].w = fmaf(v[y].w, f, o[4 * y + 3]);
+        }
+        if constexpr (BACK) {
+            uint32_t u[32];
+#pragma unroll
+            for (int y = 0; y < 8; y++) {
+                u[4 * y] = __float_as_uint(v[y].x), u[4 * y + 1] = __float_as_uint(v[y].y);
+                u[4 * y + 2] = __float_as_uint(v[y].z), u[4 * y + 3] = __float_as_uint(v[y].w);
+            }
+            tm_st32(mine + 32 * c, u);
+        } else {
+#pragma unroll
+            for (int y = 0; y < 8; y++) __stcg(sums + (8 * c + y) * 32, v[y]);
+        }
+    }
+    if constexpr (BACK) tm_wait_st();
+    tc_before();
 }
 
 // A warp's queries, `rows` of 32 (src: where this thread's lies), to where the MMAs read them. Returns the factor of the row's scores. Not inlined: the
@@ -430,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
 #pragma unroll
                     for (int k = 0; k < N / 16; k++) {
                         const uint64_t b = desc(vb + i * C::TILE + k * 2048, C::CH);
-                        mma_ts(tmem, tmem + C::SC + i * N + 8 * k, b, id_o, j > 0 || k > 0);
+                        mma_ts(tmem, tmem + C::SC + i * N + 8 * k, b, id_o, j % C::SPAN > 0 || k > 0);
                         if constexpr (TWO) mma_ts(tmem, tmem + C::SC + i * N + N / 2 + 8 * k, b, id_o, true);
                     }
                     mma_commit(empty_v + i);
@@ -579,113 +624,129 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
         for (int cur = 0; soft_s[cur].k0 >= 0; cur ^= 1) {
             const int n = tiles_of(soft_s[cur]), start = soft_s[cur].start + soft_s[cur].k0 * N;
             float m = -INFINITY, l0 = 0.f, l1 = 0.f;
-            for (int j = 0; j < n; j++) {
-                const uint32_t i = tc & 1;
-                wait_for(s_full + i, (tc >> 1) & 1, &dead, a.err);
-                __syncwarp();
-                tc_after();
-                const int t0 = start + j * N;
-                const bool edge = __any_sync(0xffffffffu, t0 + N - 1 > row.pos || t0 <= row.low);
-                const uint32_t b0 = *(volatile uint32_t *)&bad[tc & 3][0], b1 = *(volatile uint32_t *)&bad[tc & 3][1];   // tokens with poisoned values
-                // The weights under the reference as it stands, and the largest score. Where one is too large (and at a group's start) the
-                // reference moves, and they are taken again from the scores, which lie there until the weights are stored.
-                uint32_t hi[N / 32][16], lo[N / 32][16];
-                float d0, d1;
-                auto weigh = [&](float ref) {
-                    float most = -INFINITY;
-                    f32x2 sum = pack2(0.f, 0.f);
-                    const f32x2 up2 = pack2(row.up, row.up), ref2 = pack2(-ref, -ref);
+            float stood = -INFINITY;                                   // the reference of what the workspace has
+            // The CTA's place for a group's part: none but this group uses it until the group has left (whole groups come before one
+            // that goes on in the next CTA).
+            float *slot = a.part + ((size_t)blockIdx.x * 2 + (soft_s[cur].k0 == 0 ? 1 : 0)) * part_floats(R, HD);
+            float4 *sums = reinterpret_cast<float4 *>(slot) + warp * (8 * HD) + lane;
+            auto since = [&]() { return stood == -INFINITY ? 0.f : ex2(stood - m); };
+            for (int j = 0; j < n;) {                                   // spans
+                const int first = j, stop = min(n, j + C::SPAN);
+                for (; j < stop; j++) {
+                    const uint32_t i = tc & 1;
+                    wait_for(s_full + i, (tc >> 1) & 1, &dead, a.err);
+                    __syncwarp();
+                    tc_after();
+                    const int t0 = start + j * N;
+                    const bool edge = __any_sync(0xffffffffu, t0 + N - 1 > row.pos || t0 <= row.low);
+                    const uint32_t b0 = *(volatile uint32_t *)&bad[tc & 3][0], b1 = *(volatile uint32_t *)&bad[tc & 3][1];   // tokens with poisoned values
+                    // The weights under the reference as it stands, and the largest score. Where one is too large (and at a group's start) the
+                    // reference moves, and they are taken again from the scores, which lie there until the weights are stored.
+                    uint32_t hi[N / 32][16], lo[N / 32][16];
+                    float d0, d1;
+                    auto weigh = [&](float ref) {
+                        float most = -INFINITY;
+                        f32x2 sum = pack2(0.f, 0.f);
+                        const f32x2 up2 = pack2(row.up, row.up), ref2 = pack2(-ref, -ref);
 #pragma unroll
-                    for (int c = 0; c < N / 32; c++) {
-                        float s[32], m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                        tm_ld32(mine + C::SC + i * N + 32 * c, s);
-                        tm_wait_ld(s, 32);
+                        for (int c = 0; c < N / 32; c++) {
+                            float s[32], m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                            tm_ld32(mine + C::SC + i * N + 32 * c, s);
+                            tm_wait_ld(s, 32);
 #pragma unroll
-                        for (int x = 0; x < 32; x += 2) {
-                            const float2 v = unpack2(mul2(pack2(s[x], s[x + 1]), up2));
-                            s[x] = v.x, s[x + 1] = v.y;
-                        }
-                        if (edge || (b0 | b1)) {
-                            const uint32_t flags = c ? b1 : b0;
-#pragma unroll
-                            for (int x = 0; x < 32; x++) {
-                                const int p = t0 + 32 * c + x;
-                                if (p > row.pos || p <= row.low) s[x] = -INFINITY;
-                                else if (flags >> x & 1) s[x] = NAN;
+                            for (int x = 0; x < 32; x += 2) {
+                                const float2 v = unpack2(mul2(pack2(s[x], s[x + 1]), up2));
+                                s[x] = v.x, s[x + 1] = v.y;
                             }
-                        }
+                            if (edge || (b0 | b1)) {
+                                const uint32_t flags = c ? b1 : b0;
 #pragma unroll
-                        for (int x = 0; x < 32; x += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(m4[x / 2 & 3]) : "f"(s[x]), "f"(s[x + 1]));
-#pragma unroll
-                        for (int x = 0; x < 16; x++) {
-                            const float2 w = unpack2(add2(pack2(s[2 * x], s[2 * x + 1]), ref2));   // the largest score's difference is exact, however large
-                            const float p = ex2(w.x), q = ex2(w.y);
-                            hi[c][x] = pack_f16(p, q);
-                            if constexpr (__is_same(T, __nv_bfloat16)) sum = add2(sum, pack2(p, q));   // f16's rounding is beneath bf16's
-                            else {
-                                const float2 b = unpack_f16(hi[c][x]);
-                                if constexpr (TWO) {
-                                    lo[c][x] = pack_f16(p - b.x, q - b.y);
-                                    sum = add2(sum, pack2(p, q));
-                                } else {
-                                    sum = add2(sum, pack2(b.x, b.y));
+                                for (int x = 0; x < 32; x++) {
+                                    const int p = t0 + 32 * c + x;
+                                    if (p > row.pos || p <= row.low) s[x] = -INFINITY;
+                                    else if (flags >> x & 1) s[x] = NAN;
                                 }
                             }
+#pragma unroll
+                            for (int x = 0; x < 32; x += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(m4[x / 2 & 3]) : "f"(s[x]), "f"(s[x + 1]));
+#pragma unroll
+                            for (int x = 0; x < 16; x++) {
+                                const float2 w = unpack2(add2(pack2(s[2 * x], s[2 * x + 1]), ref2));   // the largest score's difference is exact, however large
+                                const float p = ex2(w.x), q = ex2(w.y);
+                                hi[c][x] = pack_f16(p, q);
+                                if constexpr (__is_same(T, __nv_bfloat16)) sum = add2(sum, pack2(p, q));   // f16's rounding is beneath bf16's
+                                else {
+                                    const float2 b = unpack_f16(hi[c][x]);
+                                    if constexpr (TWO) {
+                                        lo[c][x] = pack_f16(p - b.x, q - b.y);
+                                        sum = add2(sum, pack2(p, q));
+                                    } else {
+                                        sum = add2(sum, pack2(b.x, b.y));
+                                    }
+                                }
+                            }
+                            most = fmaxf(most, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
                         }
-                        most = fmaxf(most, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-                    }
-                    const float2 v = unpack2(sum);
-                    d0 = v.x, d1 = v.y;
-                    return most;
-                };
+                        const float2 v = unpack2(sum);
+                        d0 = v.x, d1 = v.y;
+                        return most;
+                    };
 #pragma unroll 1
-                for (int again = 0;; again = 1) {
-                    const float ref = m == -INFINITY ? 0.f : m, mx = weigh(ref);
-                    const bool move = mx - ref > W_MAX || (m == -INFINITY && mx > -INFINITY);
-                    if (again || !__any_sync(0xffffffffu, move)) break;
-                    const float was = m;
-                    if (move) m = mx - C::TOP;
-                    const float f = was == -INFINITY ? 0.f : ex2(was - m);
-                    l0 *= f, l1 *= f;
-                    if (j > 0) {   // what the outputs have so far, behind the products before
-                        wait_for(pv_done + (i ^ 1), ((tc - 1) >> 1) & 1, &dead, a.err);
+                    for (int again = 0;; again = 1) {
+                        const float ref = m == -INFINITY ? 0.f : m, mx = weigh(ref);
+                        const bool move = mx - ref > W_MAX || (m == -INFINITY && mx > -INFINITY);
+                        if (again || !__any_sync(0xffffffffu, move)) break;
+                        const float was = m;
+                        if (move) m = mx - C::TOP;
+                        const float f = was == -INFINITY ? 0.f : ex2(was - m);
+                        l0 *= f, l1 *= f;
+                        if (j > first) {   // what the outputs have so far, behind the products before
+                            wait_for(pv_done + (i ^ 1), ((tc - 1) >> 1) & 1, &dead, a.err);
+                            __syncwarp();
+                            tc_after();
+#pragma unroll 1
+                            for (int c = 0; c < HD / 32; c++) {
+                                float o[32];
+                                tm_ld32(mine + 32 * c, o);
+                                tm_wait_ld(o, 32);
+                                uint32_t u[32];
+#pragma unroll
+                                for (int x = 0; x < 32; x++) u[x] = __float_as_uint(o[x] * f);
+                                tm_st32(mine + 32 * c, u);
+                            }
+                            tm_wait_st();
+                        }
+                    }
+                    l0 += d0, l1 += d1;
+                    if constexpr (!TWO) {
+#pragma unroll
+                        for (int c = 0; c < N / 32; c++) tm_st16(mine + C::SC + i * N + 16 * c, hi[c]);
+                    }
+                    if constexpr (TWO) {
+#pragma unroll
+                        for (int c = 0; c < N / 32; c++) {
+                            tm_st16(mine + C::SC + i * N + 16 * c, hi[c]);
+                            tm_st16(mine + C::SC + i * N + N / 2 + 16 * c, lo[c]);
+                        }
+                    }
+                    if (b0 | b1) {
+                        bar_sync(1, SM_WARPS * 32);
+                        if (tid < 2) bad[tc & 3][tid] = 0;
                         __syncwarp();
-                        tc_after();
-#pragma unroll 1
-                        for (int c = 0; c < HD / 32; c++) {
-                            float o[32];
-                            tm_ld32(mine + 32 * c, o);
-                            tm_wait_ld(o, 32);
-                            uint32_t u[32];
-#pragma unroll
-                            for (int x = 0; x < 32; x++) u[x] = __float_as_uint(o[x] * f);
-                            tm_st32(mine + 32 * c, u);
-                        }
-                        tm_wait_st();
                     }
-                }
-                l0 += d0, l1 += d1;
-                if constexpr (!TWO) {
-#pragma unroll
-                    for (int c = 0; c < N / 32; c++) tm_st16(mine + C::SC + i * N + 16 * c, hi[c]);
-                }
-                if constexpr (TWO) {
-#pragma unroll
-                    for (int c = 0; c < N / 32; c++) {
-                        tm_st16(mine + C::SC + i * N + 16 * c, hi[c]);
-                        tm_st16(mine + C::SC + i * N + N / 2 + 16 * c, lo[c]);
-                    }
-                }
-                if (b0 | b1) {
-                    bar_sync(1, SM_WARPS * 32);
-                    if (tid < 2) bad[tc & 3][tid] = 0;
+                    tm_wait_st();
+                    tc_before();
                     __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full + i);
+                    tc++;
                 }
-                tm_wait_st();
-                tc_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + i);
-                tc++;
+                if (j < n) {
+                    wait_for(pv_done + ((tc - 1) & 1), ((tc - 1) >> 1) & 1, &dead, a.err);
+                    __syncwarp();
+                    tc_after();
+                    take_over<C, false>(mine, sums, since());
+                    stood = m;
+                }
             }
             // the next group's queries, then this one's outputs
             group_is(cur ^ 1, next());
@@ -694,11 +755,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             const bool whole = sg.f0 == sg.f1;
             const long long row_out = out_s[cur][r];
             const float l = l0 + l1;
-            float *slot = a.part + ((size_t)blockIdx.x * 2 + (sg.k0 == 0 ? 1 : 0)) * part_floats(R, HD);
             if (n > 0) {
                 wait_for(&o_full, groups & 1, &dead, a.err);
                 __syncwarp();
                 tc_after();
+                if (n > C::SPAN) {
+                    take_over<C, true>(mine, sums, since());
+                    tc_after();
+                    bar_sync(1, SM_WARPS * 32);                        // the place is read; parts may lie there now
+                }
             }
             const float f = !whole ? 1.0f : l == 0.f ? 0.f : sig_s[cur][r] / l;
             const int mrows = sg.c1 - sg.c0 + 1 - 32 * warp;          // rows of this warp

@@ -425,6 +425,49 @@ def test_long_context(cuda):
             check_attention(c, c.randn(heads * hd, typ, 0.3), typ)
 
 
+@pytest.mark.parametrize("typ", ["f32", "f16"])
+@pytest.mark.parametrize("size", [0.05, 30.0])
+@pytest.mark.parametrize("rows, nseq", [(1, 320), (128, 160)])
+def test_values_of_one_sign_in_a_long_context(cuda, rows, nseq, size, typ):
+    """Matrix instructions that cut their sums towards 0 are short by up to a unit, 2^-23 of the sum, each. So many sequences over the same
+    pages that a block of threads has whole ones to itself. Few rows: blocks of 16 tokens by themselves (two instructions of f32) and
+    f32 additions of 1024 of them a warp, each off by 2^-24 of the sum either way: their errors' root of 1024, four times over, and 2^-22. Many rows: 2048 tokens
+    (f32; 16-bit types 16384) an accumulator, 256 (1024) instructions. Beside that as in want_attention: 2^-21 (2^-11) for the weights, 2^-20 for the
+    scores and as much for the division, what the smallest weights lose, half a unit of the type. Large queries: keys that grow along the
+    context, so that the largest score so far keeps growing, too."""
+    import torch
+
+    from spk import paged4
+
+    n, page, hd = 65536, 128, 64
+    c = paged4.Paged4Cache(n // page, page, 1, hd, device=cuda)
+    g = torch.Generator(device=cuda)
+    g.manual_seed(21)
+    for pool, scale, keep in ((c.k_pool, c.k_scale, 0xff), (c.v_pool, c.v_scale, 0x77)):
+        pool.random_(0, 256, generator=g)
+        pool.bitwise_and_(keep)
+        scale.copy_(torch.randint(95, 103, scale.shape, generator=g, device=cuda).to(torch.uint8))
+    if size > 1:
+        c.k_scale -= torch.linspace(30, 0, n // page, device=cuda).to(torch.uint8)[:, None, None, None]
+    row0 = torch.arange(nseq + 1, dtype=torch.int32, device=cuda) * rows
+    table = torch.arange(n // page, dtype=torch.int32, device=cuda)[None].expand(nseq, -1).contiguous()
+    b = paged4.Paged4Batch(c, row0, torch.full((nseq,), n, dtype=torch.int32, device=cuda), table, rows=nseq * rows, heads=1)
+    q = (torch.randn(nseq * rows, hd, generator=g, device=cuda) * size).to(ttype(typ))
+    got = b.attention(q).double()
+    assert check_errors() == 0
+    k, v = (numbers(p, s)[:, 0].reshape(-1, hd) for p, s in ((c.k_pool, c.k_scale), (c.v_pool, c.v_scale)))
+    cut = 4 * 1024 ** 0.5 * 2.0 ** -24 + 2.0 ** -22 if rows == 1 else (256 if typ == "f32" else 1024) * 2.0 ** -23
+    for s in (0, 1, nseq // 2, nseq - 1):
+        x = q[s * rows].double() * hd ** -0.5
+        kk, vv = k[:n - rows + 1], v[:n - rows + 1]
+        p = torch.softmax(kk @ x, 0)
+        want = p @ vv
+        bound = cut + (2.0 ** -21 if typ == "f32" else 2.0 ** -11) + 2.0 ** -20 * (kk.abs() @ x.abs()).max() + 2.0 ** -20 + HALF[typ]
+        lost = (2.0 ** -35 if typ == "f32" else 2.0 ** -31) * p.max() * vv.sum(0)
+        off = (got[s * rows] - want).abs()
+        assert (off <= bound * want + lost).all(), (s, (off / want).max(), bound)
+
+
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows", [[6, 40], [6, 150]])
 def test_queries_of_any_size(cuda, rows, typ):
