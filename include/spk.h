@@ -558,7 +558,8 @@ int spk_paged4_read(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
  *   out[t][h] = sigmoid(gate[t][h]) * softmax_j(scale * q[t][h] . K_j) V_j
  * over j in [0, pos_t] (window 0) or (pos_t - window, pos_t]; q head h reads KV head h / (heads / kv_heads), any group. The
  * softmax and all sums are in f32; queries and weights meet the cached values as f16 numbers on a power of two of their row,
- * f32 rows' as two. A row that sees nothing gets 0; a row that sees a token of which a group is NaN gets NaN.
+ * f32 rows' as two, weights kept down to 2^-36 of the row's largest (a sequence of many rows: 2^-34 in f32, 2^-30 in the
+ * 16-bit types). A row that sees nothing gets 0; a row that sees a token of which a group is NaN gets NaN.
  * workspace: spk_paged4_attn_workspace_bytes(head_dim) device bytes for the device current at the call, zeroed once and
  * left ready; calls that share one must not overlap on the GPU. No sync. */
 typedef struct {
