@@ -651,11 +651,14 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
 }
 
 // Rows per KV head up to which a sequence is this kernel's. Each 8 of them read the cache again (from L2); the kernel for many rows takes 128
-// at once, and as long for one. Where they meet (us, here / there; heads of 256, of 128 in brackets; bf16):
-//   64 sequences of 1200 keys   32 rows 103 164 (64 102)   64: 187 179 (113 105)   128: 356 199 (210 107)
-//   8 of 6000                   32 rows 59 106 (40 63)     64: 100 104 (66 68)     128: 183 160 (115 84)
-//   1 of 16000                  64 rows 47 89 (33 53)     256: 123 131 (80 76)
-// f32 the same within a tenth. With few (sequence, KV head) pairs the wide kernel's parts are many and small, so the border lies higher.
+// at once, and as long for one. All sequences alike (us, here / there; heads of 256, of 128 in brackets; bf16, f32 within a third):
+//   64 sequences of 1200 keys   32 rows 109 112 (68 87)   64: 192 121 (116 90)   128: 361 137 (213 87)
+//   8 of 6000                   32 rows 59 70 (40 57)     64: 100 80 (66 60)     128: 182 92 (115 62)
+//   1 of 16000                  128 rows 71 110 (47 64)   256: 123 114 (79 69)   512: 226 105 (143 68)
+// By these the border would be 32 to 48 rows. It is 64, the rows of 8 tokens of 8 heads on one: of a batch with rows on both sides both kernels run, one
+// behind the other, and with the border at 40 ragged batches of up to 64 rows took twice as long (24 sequences of 1 to 8 tokens, 32 heads on 4 of 128,
+// up to 5000 keys: 66 us for 29; 64 such sequences 70 for 45). With few (sequence, KV head) pairs the wide kernel's parts are many and small, so
+// the border lies higher.
 constexpr long long FEW_PAIRS = 8, NARROW_FEW = 256, NARROW = 64;
 constexpr size_t TICKETS = 3 * MAX_CTAS_ALL * sizeof(unsigned int);   // before the partials: three words per CTA
 constexpr int MAX_CTAS = 3;                             // of an SM
