@@ -743,10 +743,13 @@ int spk_paged4_attn(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
     if (line(here, R, COST) > 2147483000.0 || (many && line(there, WIDE_R, WIDE_COST) > 2147483000.0))
         return set_error("%s: %d rows over up to %d pages of %d tokens are too much for one call", who, batch->rows, batch->max_pages, pool->page_tokens);
     if (many) {
-        a.from = narrow + 1;
+        // Which sequences a kernel has is decided where row0 is read; the arguments only say how many rows there may be. One sequence that may have many
+        // rows is the other kernel's, however few it has.
+        const bool one = batch->nseq == 1;
+        a.from = one ? 0 : narrow + 1;
         a.to = LLONG_MAX;
         const int rc = attn_wide(a, p->type, s, who);
-        if (rc || batch->nseq == 1) return rc;
+        if (rc || one) return rc;
     }
     a.from = 0;
     a.to = narrow;

@@ -734,3 +734,55 @@ def test_calls_without_rows(cuda):
     assert c.batch.attention(torch.empty(0, 256, device=cuda)).shape == (0, 256)
     assert c.batch.read()[0].shape == (0, 128) and c.batch.parts()[1].shape == (0, 8)
     assert check_errors() == 0
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("most", [70, 150, 300])
+def test_one_sequence_of_fewer_rows_than_the_call_allows(cuda, most, hd, typ):
+    """Arguments for `most` rows of 4 heads on a KV head, row0 that says 3: those rows, and none behind them."""
+    import torch
+
+    from spk import paged4
+
+    for kv in (1, 3, 10):                 # few pairs of sequence and KV head, and more
+        c = Case(cuda, [3], [50], kv, hd, 16, 4 * kv, seed=22)
+        q = c.randn(4 * kv * hd, typ, 0.4)
+        qq = torch.cat([q, torch.ones(most - 3, q.shape[1], dtype=q.dtype, device=cuda)])
+        out = torch.full_like(qq, 9.0)
+        paged4.Paged4Batch(c.cache, c.row0, c.kv_len, c.tab, rows=most, heads=4 * kv).attention(qq, out)
+        assert check_errors() == 0
+        want, tol = want_attention(c, q)
+        assert ((out[:3].double() - want).abs() <= tol + HALF[typ] * want.abs() + TINY[typ]).all()
+        assert (out[3:] == 9).all()
+
+
+def test_a_captured_chunk_replayed_with_a_shorter_one(cuda):
+    """A prompt's chunks by one graph of 150 rows: the last one has fewer, which the device's arrays say."""
+    import torch
+
+    for hd, typ in ((256, "bf16"), (64, "f32")):
+        c = Case(cuda, [150], [300], 2, hd, 32, 8, seed=23)
+        q, k, v = c.randn(8 * hd, typ, 0.4), c.randn(2 * hd, typ), c.randn(2 * hd, typ)
+        qo, out = torch.zeros_like(q), torch.zeros_like(q)
+
+        def step():
+            c.batch.append(k, v, q=q, q_out=qo)
+            c.batch.attention(qo, out)
+
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        for n in (150, 40, 7, 1, 0, 65):
+            c.rows, c.len = [n], [300 + n]
+            c.row0.copy_(torch.tensor([0, n]))
+            c.kv_len.copy_(torch.tensor([300 + n]))
+            out.fill_(9.0)
+            graph.replay()
+            assert check_errors() == 0
+            assert (out[n:] == 9).all()
+            if n:
+                want, tol = want_attention(c, qo[:n])
+                assert ((out[:n].double() - want).abs() <= tol + HALF[typ] * want.abs() + TINY[typ]).all(), n
