@@ -402,25 +402,27 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
             const int tok0 = sg.start + (first + WARPS * i) * BLOCK;
             // scores: tokens g and g + 8 (c[.][0], c[.][1] and c[.][2], c[.][3]) of the lane's two rows, even and odd steps apart
             float c[2][4] = {};
+            uint32_t kbad = 0;            // poisoned scales of keys: of token g in the lower half, of g + 8 in the upper one
 #pragma unroll
             for (int h = 0; h < (HD == 256 ? 2 : 1); h++) {
-                uint32_t w[2][4], sc[2][2];
+                uint32_t w[2][4], sc[2][2], sb[2];
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
                     const int tok = 8 * n + g;
                     if constexpr (HD == 64) {
                         const uint2 v = *reinterpret_cast<const uint2 *>(st + tok * ROW + 8 * t);
                         w[n][0] = v.x, w[n][1] = v.y, w[n][2] = w[n][3] = 0;
-                        const uint32_t b = st[C::KS_OFF + tok * SROW + t];
-                        sc[n][0] = sc[n][1] = b * 0x00800080u;
+                        sb[n] = st[C::KS_OFF + tok * SROW + t];
+                        sc[n][0] = sc[n][1] = sb[n] * 0x00800080u;
                     } else {
                         const uint4 v = *reinterpret_cast<const uint4 *>(st + tok * ROW + 16 * (HD == 256 ? (4 * h + t) ^ 4 * (g & 1) : t));
                         w[n][0] = v.x, w[n][1] = v.y, w[n][2] = v.z, w[n][3] = v.w;
-                        const uint32_t b = *reinterpret_cast<const uint16_t *>(st + C::KS_OFF + tok * SROW + 8 * h + 2 * t);
-                        sc[n][0] = (b & 0xff) * 0x00800080u;
-                        sc[n][1] = (b >> 8) * 0x00800080u;
+                        sb[n] = *reinterpret_cast<const uint16_t *>(st + C::KS_OFF + tok * SROW + 8 * h + 2 * t);
+                        sc[n][0] = (sb[n] & 0xff) * 0x00800080u;
+                        sc[n][1] = (sb[n] >> 8) * 0x00800080u;
                     }
                 }
+                kbad |= poisoned(sb[0] | sb[1] << 16);
 #pragma unroll
                 for (int x = 0; x < (HD == 64 ? 2 : 4); x++) {
                     uint32_t k[2][4];
@@ -463,8 +465,9 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
                 const uint8_t *at = st + C::VS_OFF + (2 * t + (x & 1) + 8 * (x >> 1)) * SROW;
                 vs[x] = HD == 256 ? *reinterpret_cast<const uint16_t *>(at + 2 * g) : HD == 128 ? at[g] : at[g >> 1];
             }
-            if (__any_sync(0xffffffffu, poisoned(vs[0] | vs[1] << 16) | poisoned(vs[2] | vs[3] << 16))) {
-                uint32_t bad = 0;         // a bit a token of the block
+            // A key's group is looked at like a value's: byte 248 is an infinity, whose score may be -inf and its weight 0.
+            if (__any_sync(0xffffffffu, poisoned(vs[0] | vs[1] << 16) | poisoned(vs[2] | vs[3] << 16) | kbad)) {
+                uint32_t bad = (kbad & 0xffff ? 1u << g : 0u) | (kbad >> 16 ? 1u << (g + 8) : 0u);         // a bit a token of the block
 #pragma unroll
                 for (int x = 0; x < 4; x++)
                     if (poisoned(vs[x])) {

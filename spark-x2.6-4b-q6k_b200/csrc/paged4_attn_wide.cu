@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full_k[2], empty_k[2], full_v[2], empty_v[2], s_full[2], p_full[2], pv_done[2], q_full, o_full, o_free;
     __shared__ uint32_t pre[MAX_SEQ + 1], wsum[WARPS];
-    __shared__ uint32_t bad[4][2];                      // tokens of a tile with poisoned values
+    __shared__ uint32_t bad[4][2];                      // tokens of a tile with poisoned keys or values
     __shared__ Walk walk_s;
     __shared__ Seg seg_s;
     __shared__ int dead, last_s;
@@ -559,7 +559,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                     for (int h = 0; h < H; h++) {
                         const int tok = tok0 + STEP * u;
                         uint32_t s2 = there[u] ? sc[u][h] : 0;
-                        if (there[u] && poisoned(vs[u][h])) {
+                        // a key's own scales, too: byte 248 is an infinity, whose score may be -inf and its weight 0
+                        if (there[u] && poisoned(vs[u][h] | sc[u][h] << 16)) {
                             if (keys) atomicOr(&bad[tc & 3][tok >> 5], 1u << (tok & 31));
                             else {   // poisoned values become 0: their tokens' weights say NaN where they are seen
                                 if ((s2 & 0xff) >= POISON) s2 &= 0xff00;
@@ -639,7 +640,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                     tc_after();
                     const int t0 = start + j * N;
                     const bool edge = __any_sync(0xffffffffu, t0 + N - 1 > row.pos || t0 <= row.low);
-                    const uint32_t b0 = *(volatile uint32_t *)&bad[tc & 3][0], b1 = *(volatile uint32_t *)&bad[tc & 3][1];   // tokens with poisoned values
+                    const uint32_t b0 = *(volatile uint32_t *)&bad[tc & 3][0], b1 = *(volatile uint32_t *)&bad[tc & 3][1];   // tokens with poisoned keys or values
                     // The weights under the reference as it stands, and the largest score. Where one is too large (and at a group's start) the
                     // reference moves, and they are taken again from the scores, which lie there until the weights are stored.
                     uint32_t hi[N / 32][16], lo[N / 32][16];

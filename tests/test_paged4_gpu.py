@@ -786,3 +786,23 @@ def test_a_captured_chunk_replayed_with_a_shorter_one(cuda):
             if n:
                 want, tol = want_attention(c, qo[:n])
                 assert ((out[:n].double() - want).abs() <= tol + HALF[typ] * want.abs() + TINY[typ]).all(), n
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [[3, 2], [150, 70]])
+def test_keys_under_scales_that_are_no_numbers(cuda, rows, hd, typ):
+    """Scale bytes from 248 (f16's infinity) to 255 of keys all of whose products with the queries are negative: NaN where they are seen."""
+    import torch
+
+    c = Case(cuda, rows, [60, 37], 2, hd, 16, 8, seed=24)
+    c.cache.k_pool.bitwise_and_(0x77).bitwise_or_(0x11)           # no zeros, none negative
+    groups = hd // 16
+    for i, byte in enumerate((248, 249, 255)):
+        p = 61 - 19 * i
+        c.cache.k_scale[c.table[0][p // 16], 0, p % 16, (5 * i + 1) % groups] = byte
+    c.cache.k_scale[c.table[1][2], 1, 4, groups - 1] = 248        # token 36 of the second sequence
+    q = c.randn(8 * hd, typ, 0.2).abs().clamp(min=0.01).neg()
+    for window in (0, 9):
+        got = check_attention(c, q, typ, window)
+        assert got.isnan().any() and not got.isnan().all()
