@@ -342,7 +342,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full_k[2], empty_k[2], full_v[2], empty_v[2], s_full[2], p_full[2], pv_done[2], q_full, o_full, o_free;
     __shared__ uint32_t pre[MAX_SEQ + 1], wsum[WARPS];
-    __shared__ uint32_t bad[4][2];                      // tokens of a tile with poisoned keys or values
+    // Tokens of a tile with poisoned keys or values, and how many softmax warps have read that there are some: the last one clears them. No barrier may depend
+    // on the flags: after a wait that ran out the warps may read different ones, and each still has to meet the others at every barrier.
+    __shared__ uint32_t bad[4][2], bad_read[4];
     __shared__ Walk walk_s;
     __shared__ Seg seg_s;
     __shared__ int dead, last_s;
@@ -367,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
         seg_s.k0 = -1;
         fence_mbar_init();
     }
-    if (tid < 8) bad[tid >> 1][tid & 1] = 0;
+    if (tid < 8) bad[tid >> 1][tid & 1] = bad_read[tid >> 1] = 0;
     if (warp == MMA_WARP) {   // this warp owns the tensor memory
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"((uint32_t)C::TCOLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -731,9 +733,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
                         }
                     }
                     if (b0 | b1) {
-                        bar_sync(1, SM_WARPS * 32);
-                        if (tid < 2) bad[tc & 3][tid] = 0;
                         __syncwarp();
+                        if (lane == 0 && atomicAdd(&bad_read[tc & 3], 1) == SM_WARPS - 1) bad[tc & 3][0] = bad[tc & 3][1] = bad_read[tc & 3] = 0;
                     }
                     tm_wait_st();
                     tc_before();

@@ -806,3 +806,15 @@ def test_keys_under_scales_that_are_no_numbers(cuda, rows, hd, typ):
     for window in (0, 9):
         got = check_attention(c, q, typ, window)
         assert got.isnan().any() and not got.isnan().all()
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+def test_poison_in_one_tile_after_another(cuda, typ):
+    """Poisoned values in tile after tile of a sequence of many rows, clean tiles behind them: a window's rows are NaN while
+    they see one, and numbers again after it."""
+    c = Case(cuda, [400, 90], [500, 0], 2, 128, 32, 8, seed=25)
+    for p in (*range(470, 640, 17), 700, 760):
+        c.cache.v_scale[c.table[0][p // 32], p % 2, p % 32, p % 8] = 255 if p % 3 else 248
+    for window in (30, 150):
+        got = check_attention(c, c.randn(1024, typ, 0.4), typ, window)
+        assert got.isnan().any() and not got.isnan().all()
