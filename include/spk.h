@@ -519,8 +519,8 @@ typedef struct {
 } spk_kv4_pool;
 
 /* A projection's rows: queries and keys normalised and rotated, queries out, keys and values into the pages, in one pass.
- * Per head, with q_norm / k_norm ([head_dim] f32, 16-byte aligned; NULL: none): x / sqrt(mean x^2 + eps) * norm. Then, with
- * freq, the rotation by f32(position * freq[i]), i < pdim / 2 (pdim a multiple of 16), of the pairs (i, i + pdim / 2), or
+ * Per head, with q_norm / k_norm ([head_dim] f32, 16-byte aligned; NULL: none): x / sqrt(mean x^2 + eps) * norm, whatever the head's
+ * size (squares that leave f32's range are taken on a power of two). Then, with freq, the rotation by f32(position * freq[i]), i < pdim / 2 (pdim a multiple of 16), of the pairs (i, i + pdim / 2), or
  * (2 i, 2 i + 1) where `interleaved`. heads 0: no queries. q_out may be q itself (the same rows and stride).
  * Rounding, per group of 16 values: the scale is the number of 4 significant bits nearest to amax / 6 (ties to even, 2^-14 to
  * 10240), a code the nearest to value / scale (ties to the even code, at most 6 in magnitude); both are decided exactly

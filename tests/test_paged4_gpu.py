@@ -818,3 +818,46 @@ def test_poison_in_one_tile_after_another(cuda, typ):
     for window in (30, 150):
         got = check_attention(c, c.randn(1024, typ, 0.4), typ, window)
         assert got.isnan().any() and not got.isnan().all()
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_norms_of_rows_of_any_size(cuda, hd, typ):
+    """Heads whose squares, or their sum, are out of f32's range: the norm is that of the formula."""
+    import torch
+
+    size = {"f32": [1e38, 1.0, 1e30, 1e19, 1e-19, 1e-25, 1e-38, 3e-41], "bf16": [1e38, 1.0, 1e30, 1e19, 1e-19, 1e-25, 1e-36, 1e-30],
+            "f16": [1e4, 1.0, 100.0, 1e-3]}[typ]
+    c = Case(cuda, [len(size) * 3, 5], [4, 0], 2, hd, 16, 4, seed=26)
+    q, k, v = c.randn(4 * hd, typ), c.randn(2 * hd, typ), c.randn(2 * hd, typ)
+    q.clamp_(-3, 3)
+    k.clamp_(-3, 3)
+    for i in range(q.shape[0]):
+        q[i] *= size[i % len(size)]
+        k[i] *= size[(i + 1) % len(size)]
+    q[2, :hd] *= size[0]                             # heads of one row apart, too
+    q[2].clamp_(-torch.finfo(q.dtype).max, torch.finfo(q.dtype).max)
+    w = [torch.rand(hd, generator=c.g, device=cuda) + 0.5 for _ in "qk"]
+    for eps in np.float32([1e-6, 0.0, 1e-35, 1e-45, 1e30]).tolist():          # eps is an f32 argument: 1e-45 is 1.4e-45
+        for freq in (freqs(cuda, 32), None):
+            if eps < 1:
+                check_append(c, k, v, q, freq, False, w[0], w[1], eps=eps, typ=typ)
+                continue
+            # Rows that are nothing beside eps leave under 2^-126, where a rounding is off by up to 2^-150 whatever the value: x r; times w <= 1.5, 2.5 of
+            # them; two products and a sum of the rotation, 2.5 (|cos| + |sin|) + 2 <= 6 of them, beside check_append's bound.
+            check_append(c, k, v, None, freq, False, None, w[1], eps=eps, typ=typ)
+            got = c.batch.append(k, v, freq=freq, q=q, q_norm=w[0], k_norm=w[1], eps=eps)
+            y, size = (t.flatten(1) for t in head_rows(q, 4, hd, w[0], eps, c.positions(), freq, False))
+            assert ((got.double() - y).abs() <= HALF[typ] * y.abs() + TINY[typ] + 2.0 ** -20 * size + 6 * 2.0 ** -150).all()
+
+
+def test_norms_of_rows_with_an_infinity(cuda):
+    """x / sqrt(mean x^2 + eps): 0 beside an infinity, NaN in its place; a NaN makes its head NaN."""
+    import torch
+
+    c = Case(cuda, [3], [0], 1, 64, 16, 2)
+    q, w = torch.ones(3, 128, device=cuda), torch.ones(64, device=cuda)
+    q[0, 5], q[1, 70] = float("inf"), float("nan")
+    got = c.batch.append(q[:, :64].contiguous(), q[:, :64].contiguous(), q=q, q_norm=w)
+    assert got[0, 5].isnan() and (got[0, :5] == 0).all() and (got[0, 6:64] == 0).all() and got[1, 64:].isnan().all()
+    assert not got[0, 64:].isnan().any() and not got[1, :64].isnan().any() and not got[2].isnan().any()
