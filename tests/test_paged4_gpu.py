@@ -840,11 +840,8 @@ def test_norms_of_rows_of_any_size(cuda, hd, typ):
     w = [torch.rand(hd, generator=c.g, device=cuda) + 0.5 for _ in "qk"]
     for eps in np.float32([1e-6, 0.0, 1e-35, 1e-45, 1e30]).tolist():          # eps is an f32 argument: 1e-45 is 1.4e-45
         for freq in (freqs(cuda, 32), None):
-            if eps < 1:
-                check_append(c, k, v, q, freq, False, w[0], w[1], eps=eps, typ=typ)
-                continue
             # Rows that are nothing beside eps leave under 2^-126, where a rounding is off by up to 2^-150 whatever the value: x r; times w <= 1.5, 2.5 of
-            # them; two products and a sum of the rotation, 2.5 (|cos| + |sin|) + 2 <= 6 of them, beside check_append's bound.
+            # them; two products and a sum of the rotation, 2.5 (|cos| + |sin|) + 2 <= 6 of them (not rotated, halved and added: 4.5), beside check_append's bound.
             check_append(c, k, v, None, freq, False, None, w[1], eps=eps, typ=typ)
             got = c.batch.append(k, v, freq=freq, q=q, q_norm=w[0], k_norm=w[1], eps=eps)
             y, size = (t.flatten(1) for t in head_rows(q, 4, hd, w[0], eps, c.positions(), freq, False))
@@ -861,3 +858,24 @@ def test_norms_of_rows_with_an_infinity(cuda):
     got = c.batch.append(q[:, :64].contiguous(), q[:, :64].contiguous(), q=q, q_norm=w)
     assert got[0, 5].isnan() and (got[0, :5] == 0).all() and (got[0, 6:64] == 0).all() and got[1, 64:].isnan().all()
     assert not got[0, 64:].isnan().any() and not got[1, :64].isnan().any() and not got[2].isnan().any()
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("hd,pdim", [(64, 16), (128, 32), (256, 64), (256, 240)])
+def test_dims_that_are_not_rotated_leave_as_they_came(cuda, hd, pdim, inter, typ):
+    """Infinities and zeros of either sign beside each other behind the rotated dims: the queries' bits."""
+    import torch
+
+    c = Case(cuda, [7, 30], [900, 2], 2, hd, 16, 4, seed=27)
+    q, k, v = c.randn(4 * hd, typ), c.randn(2 * hd, typ), c.randn(2 * hd, typ)
+    x = q.view(-1, 4, hd)
+    for d, to in ((pdim, float("inf")), (pdim + 3, -0.0), (pdim + 6, float("-inf")), (hd - 1, 0.0), (hd - 4, float("inf"))):
+        x[:, :, d] = to
+    x[3:9, 1, pdim:] = -0.0
+    got = c.batch.append(k, v, freq=freqs(cuda, pdim), q=q, interleaved=inter)
+    bits = torch.int32 if typ == "f32" else torch.int16
+    assert torch.equal(got.view(-1, 4, hd)[:, :, pdim:].contiguous().view(bits), x[:, :, pdim:].contiguous().view(bits))
+    y, size = head_rows(q, 4, hd, None, 0.0, c.positions(), freqs(cuda, pdim), inter)
+    off = (got.view(-1, 4, hd).double() - y)[:, :, :pdim].abs()
+    assert (off <= HALF[typ] * y[:, :, :pdim].abs() + TINY[typ] + 2.0 ** -20 * size[:, :, :pdim]).all()
