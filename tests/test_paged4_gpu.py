@@ -879,3 +879,53 @@ def test_dims_that_are_not_rotated_leave_as_they_came(cuda, hd, pdim, inter, typ
     y, size = head_rows(q, 4, hd, None, 0.0, c.positions(), freqs(cuda, pdim), inter)
     off = (got.view(-1, 4, hd).double() - y)[:, :, :pdim].abs()
     assert (off <= HALF[typ] * y[:, :, :pdim].abs() + TINY[typ] + 2.0 ** -20 * size[:, :, :pdim]).all()
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,old,kv,hd,heads,window", [([1, 3], [700, 90], 2, 256, 8, 0), ([1, 8, 2], [1000, 5, 300], 2, 128, 16, 40),
+                                                         ([2], [300], 1, 64, 4, 0), ([150, 80], [90, 300], 2, 256, 8, 0), ([300], [100], 1, 64, 2, 60),
+                                                         ([90, 70], [0, 33], 3, 128, 6, 0)])
+def test_attention_over_every_scale_that_append_writes(cuda, rows, old, kv, hd, heads, window, typ):
+    """Scale bytes 8 to 226, 2^-14 to 10240, at random in every row; all of the smallest, all of the largest."""
+    c = Case(cuda, rows, old, kv, hd, 16, heads, seed=28, scales=(8, 227))
+    check_attention(c, c.randn(heads * hd, typ, 2e-5), typ, window)
+    check_attention(c, c.randn(heads * hd, typ, 1.0), typ, window, scale=2.0 ** -18)
+    for scales in ((8, 9), (226, 227)):
+        c = Case(cuda, rows, old, kv, hd, 16, heads, seed=29, scales=scales)
+        check_attention(c, c.randn(heads * hd, typ, 1.0), typ, window, scale=16.0 if scales[0] == 8 else 2.0 ** -18)
+
+
+@pytest.mark.parametrize("size", [0.05, 30.0])
+@pytest.mark.parametrize("rows, nseq", [(1, 320), (128, 160)])
+def test_bf16_values_of_one_sign_in_a_long_context(cuda, rows, nseq, size):
+    """test_values_of_one_sign_in_a_long_context in bf16, whose few rows keep one accumulator: 65536 tokens are at most 1024 blocks of 16 of
+    a warp, an instruction each, short by up to a unit, 2^-23 of the sum; many rows: 16384 tokens, 1024 instructions."""
+    import torch
+
+    from spk import paged4
+
+    n, page, hd = 65536, 128, 64
+    c = paged4.Paged4Cache(n // page, page, 1, hd, device=cuda)
+    g = torch.Generator(device=cuda)
+    g.manual_seed(31)
+    for pool, scale, keep in ((c.k_pool, c.k_scale, 0xff), (c.v_pool, c.v_scale, 0x77)):
+        pool.random_(0, 256, generator=g)
+        pool.bitwise_and_(keep)
+        scale.copy_(torch.randint(95, 103, scale.shape, generator=g, device=cuda).to(torch.uint8))
+    if size > 1:
+        c.k_scale -= torch.linspace(30, 0, n // page, device=cuda).to(torch.uint8)[:, None, None, None]
+    row0 = torch.arange(nseq + 1, dtype=torch.int32, device=cuda) * rows
+    table = torch.arange(n // page, dtype=torch.int32, device=cuda)[None].expand(nseq, -1).contiguous()
+    b = paged4.Paged4Batch(c, row0, torch.full((nseq,), n, dtype=torch.int32, device=cuda), table, rows=nseq * rows, heads=1)
+    q = (torch.randn(nseq * rows, hd, generator=g, device=cuda) * size).bfloat16()
+    got = b.attention(q).double()
+    assert check_errors() == 0
+    k, v = (numbers(p, s)[:, 0].reshape(-1, hd) for p, s in ((c.k_pool, c.k_scale), (c.v_pool, c.v_scale)))
+    for s in (0, 1, nseq // 2, nseq - 1):
+        x = q[s * rows].double() * hd ** -0.5
+        kk, vv = k[:n - rows + 1], v[:n - rows + 1]
+        p = torch.softmax(kk @ x, 0)
+        want = p @ vv
+        bound = 1024 * 2.0 ** -23 + 2.0 ** -11 + 2.0 ** -20 * (kk.abs() @ x.abs()).max() + 2.0 ** -20 + HALF["bf16"]
+        off = (got[s * rows] - want).abs()
+        assert (off <= bound * want + 2.0 ** -31 * p.max() * vv.sum(0)).all(), (s, (off / want).max(), bound)
