@@ -654,15 +654,20 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
 }
 
 // Rows per KV head up to which a sequence is this kernel's. Each 8 of them read the cache again (from L2); the kernel for many rows takes 128
-// at once, and as long for one. All sequences alike (us, here / there; heads of 256, of 128 in brackets; bf16, f32 within a third):
-//   64 sequences of 1200 keys   32 rows 109 112 (68 87)   64: 192 121 (116 90)   128: 361 137 (213 87)
-//   8 of 6000                   32 rows 59 70 (40 57)     64: 100 80 (66 60)     128: 182 92 (115 62)
-//   1 of 16000                  128 rows 71 110 (47 64)   256: 123 114 (79 69)   512: 226 105 (143 68)
-// By these the border would be 32 to 48 rows. It is 64, the rows of 8 tokens of 8 heads on one: of a batch with rows on both sides both kernels run, one
-// behind the other, and with the border at 40 ragged batches of up to 64 rows took twice as long (24 sequences of 1 to 8 tokens, 32 heads on 4 of 128,
-// up to 5000 keys: 66 us for 29; 64 such sequences 70 for 45). With few (sequence, KV head) pairs the wide kernel's parts are many and small, so
-// the border lies higher.
-constexpr long long FEW_PAIRS = 8, NARROW_FEW = 256, NARROW = 64;
+// at once, and as long for one. All sequences alike (us, here / there; bf16, heads of 256 and in brackets of 128; f32 crosses over 8 rows later):
+//   64 sequences of 1200 keys   24 rows 88 117 (56 90)    40: 130 117 (80 89)     48: 150 119 (92 91)     64: 192 121 (117 90)
+//   24 of 5000                  24 rows 103 134 (68 117)  40: 157 130 (99 111)    48: 182 132 (115 112)   64: 235 135 (146 112)
+// Where a batch has rows on both sides, both kernels run, one behind the other, and neither fills the GPU: 24 sequences of 8 to 64 rows, 37 on average,
+// heads of 128: 63 us here, 82 there, 85 with the border at 40. So what counts is where most of the work is, which the mean over the sequences says:
+//   - under mean_many rows, few sequences have more, and one kernel for up to 128 rows is better than two: 60 sequences of 4 rows and 4 of 96, 1200
+//     keys: 48 us, 91 with the border at 64 (heads of 128: 33 and 62); 4 of 128 among them 55 and 101; 48 sequences of 20000 keys, four of 128 rows: 307 and 247.
+//   - from mean_many on, all but the smallest go to the other kernel: 40 to 64 rows, 52 on average, 5000 keys: 121 us, 166 with the border at 64; the
+//     smallest stay: 63 sequences of 4 rows and one of 1024: 93, 108 all there. 16 sequences of 500 keys, 48 rows on average, lose (34 to 56).
+// Over some 430 batches of 1 to 192 rows, 500 to 20000 keys, heads of 64, 128 and 256 this takes 1.05 times as long as the best border for each
+// batch; 64 for all of them 1.13, 32 1.20. With few (sequence, KV head) pairs the other kernel's parts are many and small, and the border lies higher:
+//   1 sequence of 16000 keys    128 rows 71 110 (47 64)   256: 123 114 (79 69)    512: 226 105 (143 68)
+constexpr long long FEW_PAIRS = 8, NARROW_FEW = 256, NARROW_MOST = 128, NARROW_LEAST = 32;
+constexpr long long mean_many(int hd) { return hd == 256 ? 44 : 60; }   // rows per KV head of a sequence
 constexpr size_t TICKETS = 3 * MAX_CTAS_ALL * sizeof(unsigned int);   // before the partials: three words per CTA
 constexpr int MAX_CTAS = 3;                             // of an SM
 
@@ -735,7 +740,8 @@ int spk_paged4_attn(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
     a.part = (float *)((uint8_t *)p->workspace + TICKETS);
     a.err = device_error_ptr();
     const cudaStream_t s = (cudaStream_t)stream;
-    const long long narrow = (long long)batch->nseq * pool->kv_heads <= FEW_PAIRS ? NARROW_FEW : NARROW;
+    const bool few = (long long)batch->nseq * pool->kv_heads <= FEW_PAIRS;
+    const long long narrow = few ? NARROW_FEW : (long long)batch->rows * a.group / batch->nseq < mean_many(pool->head_dim) ? NARROW_MOST : NARROW_LEAST;
     // the lines of work, at their longest: every row tile as long as the page table and a tile's tokens (before()); here a sequence has
     // `narrow` rows at most
     const bool many = (long long)batch->rows * a.group > narrow;          // some sequence may have more

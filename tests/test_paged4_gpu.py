@@ -929,3 +929,12 @@ def test_bf16_values_of_one_sign_in_a_long_context(cuda, rows, nseq, size):
         bound = 1024 * 2.0 ** -23 + 2.0 ** -11 + 2.0 ** -20 * (kk.abs() @ x.abs()).max() + 2.0 ** -20 + HALF["bf16"]
         off = (got[s * rows] - want).abs()
         assert (off <= bound * want + 2.0 ** -31 * p.max() * vv.sum(0)).all(), (s, (off / want).max(), bound)
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,group", [([1] * 12 + [30], 4), ([1] * 12 + [33, 32], 4), ([2] * 9 + [16] * 5, 8), ([11] * 9, 4), ([15] * 9, 4), ([8] * 6 + [9] * 6 + [1], 4), ([7, 9] * 5 + [0, 40], 8)])
+def test_sequences_on_both_sides_of_the_border(cuda, rows, group, hd, typ):
+    """Few large sequences among small ones, all alike, mixed: rows per KV head on average and at most, about where the kernels change."""
+    c = Case(cuda, rows, [(37 * i) % 200 for i in range(len(rows))], 1, hd, 16, group, seed=32)
+    check_attention(c, c.randn(group * hd, typ, 0.4), typ)
