@@ -507,7 +507,8 @@ int spk_paged_attn(const spk_kv_pool *pool, const spk_kv_batch *batch, const spk
 
 /* The same in 4 bits: a row of a KV head (head_dim values of one token) is head_dim / 2 bytes of codes and head_dim / 16 scale
  * bytes, keys and values apart, 4.5 bits a value. Code c stands for 0, .5, 1, 1.5, 2, 3, 4, 6 (c & 7), negative with bit 3;
- * scale byte b for the f16 number of the bits b << 7; a value is code x scale. Per (page, KV head):
+ * scale byte b, up to 226 (10240), for the f16 number of the bits b << 7, and above that for none; a value is code x scale. Per
+ * (page, KV head):
  *   k, v               [page_tokens][head_dim / 2]     byte i of a row: dims 2 i (low half) and 2 i + 1
  *   k_scale, v_scale   [page_tokens][head_dim / 16]
  * The pool needs no initial contents; a call writes the rows that it appends and nothing else. head_dim 64, 128 or 256;
@@ -559,7 +560,8 @@ int spk_paged4_read(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
  * over j in [0, pos_t] (window 0) or (pos_t - window, pos_t]; q head h reads KV head h / (heads / kv_heads), any group. The
  * softmax and all sums are in f32; queries and weights meet the cached values as f16 numbers on a power of two of their row,
  * f32 rows' as two, weights kept down to 2^-36 of the row's largest (a sequence of many rows: 2^-34 in f32, 2^-30 in the
- * 16-bit types). A row that sees nothing gets 0; a row that sees a token of which a group is NaN gets NaN.
+ * 16-bit types). A row that sees nothing gets 0; a row that sees a token of which a group is no number
+ * gets NaN.
  * workspace: spk_paged4_attn_workspace_bytes(head_dim) device bytes for the device current at the call, zeroed once and
  * left ready; calls that share one must not overlap on the GPU. No sync. */
 typedef struct {

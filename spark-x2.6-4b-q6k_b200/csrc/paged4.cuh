@@ -8,7 +8,8 @@
 //   codes   [page_tokens][head_dim / 2]    byte i of a row: dims 2 i (low half) and 2 i + 1
 //   scales  [page_tokens][head_dim / 16]
 // A row's codes and scales depend on that row alone, so a call never touches what an earlier one wrote. A group that held a
-// NaN or an infinity has the scale byte 255 (f16 NaN) and reads as NaN.
+// NaN or an infinity has the scale byte 255 (f16 NaN) and reads as NaN. The largest scale is 10240; for the attention every byte above it says that the group
+// is no number, whoever wrote it: a code of 6 under the next one is past f16's end, and an infinity among the values would reach the rows that do not see it.
 #pragma once
 #include "paged.cuh"
 
@@ -24,7 +25,7 @@ using paged::T_F32;
 
 constexpr int GROUP = 16;                       // values that share a scale
 constexpr float SCALE_MIN = 0x1p-14f, SCALE_MAX = 10240.0f;   // 6 x 10240 is the largest six-bit number under f16's end
-constexpr uint32_t POISON = 0xf8;               // scale bytes from here on are no numbers
+constexpr uint32_t POISON = 0xe3;               // scale bytes from here on, above SCALE_MAX, are no numbers
 
 struct Pool {
     uint8_t *k, *v, *ks, *vs;
@@ -47,8 +48,8 @@ __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&h)[4]) {
         : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
         : "r"(w));
 }
-// Whether one of four scale bytes is no number: a five-bit exponent of ones carries out of its field.
-__device__ __forceinline__ uint32_t poisoned(uint32_t w) { return (((w >> 3) & 0x1f1f1f1fu) + 0x01010101u) & 0x20202020u; }
+// Whether one of four scale bytes is no number: the upper bit, and a carry into it from the others.
+__device__ __forceinline__ uint32_t poisoned(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u * (0x100u - POISON)) & w & 0x80808080u; }
 
 // The attention's arguments. A kernel takes the sequences whose rows per KV head (rows x group) are from `from` to `to`.
 struct AttnParams {

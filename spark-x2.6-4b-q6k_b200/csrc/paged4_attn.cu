@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
                 const uint8_t *at = st + C::VS_OFF + (2 * t + (x & 1) + 8 * (x >> 1)) * SROW;
                 vs[x] = HD == 256 ? *reinterpret_cast<const uint16_t *>(at + 2 * g) : HD == 128 ? at[g] : at[g >> 1];
             }
-            // A key's group is looked at like a value's: byte 248 is an infinity, whose score may be -inf and its weight 0.
+            // A key's group is looked at like a value's: under byte 248, an infinity, a score may be -inf and its weight 0.
             if (__any_sync(0xffffffffu, poisoned(vs[0] | vs[1] << 16) | poisoned(vs[2] | vs[3] << 16) | kbad)) {
                 uint32_t bad = (kbad & 0xffff ? 1u << g : 0u) | (kbad >> 16 ? 1u << (g + 8) : 0u);         // a bit a token of the block
 #pragma unroll

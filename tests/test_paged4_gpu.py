@@ -938,3 +938,83 @@ def test_sequences_on_both_sides_of_the_border(cuda, rows, group, hd, typ):
     """Few large sequences among small ones, all alike, mixed: rows per KV head on average and at most, about where the kernels change."""
     c = Case(cuda, rows, [(37 * i) % 200 for i in range(len(rows))], 1, hd, 16, group, seed=32)
     check_attention(c, c.randn(group * hd, typ, 0.4), typ)
+
+
+@pytest.mark.parametrize("typ,hd,rows,calls", [("bf16", 64, [1, 1, 2], 60), ("f32", 128, [1], 60), ("f16", 256, [1, 3], 40), ("bf16", 64, [40, 33], 12), ("f32", 256, [70], 8)])
+def test_step_after_step_without_a_pause(cuda, typ, hd, rows, calls):
+    """Append and attend, call after call, launched one behind the other and as one graph: each call reads the lines that the one
+    before it read, too, with the rows behind them written since."""
+    import torch
+
+    from spk import paged4
+
+    n = len(rows)
+    c = Case(cuda, [calls * r for r in rows], [5] * n, 2, hd, 16, 8, seed=33)
+    q, k, v = c.randn(8 * hd, typ, 0.4), c.randn(2 * hd, typ), c.randn(2 * hd, typ)
+    first = np.concatenate([[0], np.cumsum(c.rows)])[:-1]
+    own = [sum(([first[s] + i * r + x for x in range(r)] for s, r in enumerate(rows)), []) for i in range(calls)]   # the call's rows among all
+    i32 = lambda t: torch.tensor(t, dtype=torch.int32, device=cuda)  # noqa: E731
+    row0 = i32(np.concatenate([[0], np.cumsum(rows)]).tolist())
+    lens = [i32([5 + (i + 1) * r for r in rows]) for i in range(calls)]
+    batches = [paged4.Paged4Batch(c.cache, row0, L, c.tab, rows=sum(rows), heads=8) for L in lens]
+    qs, ks, vs = ([t[torch.tensor(o, device=cuda)].contiguous() for o in own] for t in (q, k, v))
+    outs = [torch.zeros_like(t) for t in qs]
+
+    def run():
+        for b, x, y, z, o in zip(batches, qs, ks, vs, outs):
+            b.append(y, z)
+            b.attention(x, o)
+
+    def poison():
+        for s, L in enumerate(c.len):
+            for p in range(5, L):
+                for t in (c.cache.k_scale, c.cache.v_scale):
+                    t[c.table[s][p // 16], :, p % 16] = 255
+
+    for form in ("calls", "graph", "graph"):
+        poison()
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        if form == "calls":
+            run()
+            graph = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            got = torch.cat(outs)
+            with torch.cuda.graph(graph):
+                run()
+        else:
+            graph.replay()
+            got = torch.cat(outs)
+        assert check_errors() == 0
+        want, tol = want_attention(c, q)
+        at = torch.tensor(sum(own, []), device=cuda)
+        assert ((got.double() - want[at]).abs() <= tol[at] + HALF[typ] * want[at].abs() + TINY[typ]).all(), form
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [[3, 2], [150, 70]])
+def test_scales_above_all_that_append_writes(cuda, rows, hd, typ):
+    """Bytes 227 to 247, scales over 10240 under which a value may pass f16's end: NaN where they are seen, and nowhere else."""
+    import torch
+
+    c = Case(cuda, rows, [60, 37], 2, hd, 16, 8, seed=35)
+    c.cache.k_pool.bitwise_or_(0x77)                # 6 or -6: past f16's end under each of these scales
+    c.cache.v_pool.bitwise_or_(0x77)
+    q = c.randn(8 * hd, typ, 0.2)
+    clean = [t.clone() for t in (c.cache.k_scale, c.cache.v_scale)]
+    for i, byte in enumerate((227, 240, 247)):
+        p = 61 - 19 * i
+        (c.cache.k_scale if i == 1 else c.cache.v_scale)[c.table[0][p // 16], 0, p % 16, (5 * i + 1) % (hd // 16)] = byte
+    now = [t.clone() for t in (c.cache.k_scale, c.cache.v_scale)]
+    for window in (0, 9):
+        got = c.batch.attention(q, window=window)
+        assert check_errors() == 0
+        for t, was, to in zip((c.cache.k_scale, c.cache.v_scale), clean, now):
+            t.copy_(torch.where(to != was, torch.full_like(to, 255), to))
+        want = check_attention(c, q, typ, window)
+        assert got.isnan().any() and not got.isnan().all()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~got.isnan()], want[~want.isnan()])
+        for t, to in zip((c.cache.k_scale, c.cache.v_scale), now):
+            t.copy_(to)
