@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
 }
 
 // Rows per KV head up to which a sequence is this kernel's. Each 8 of them read the cache again (from L2); the kernel for many rows takes 128
-// at once, and as long for one. All sequences alike (us, here / there; bf16, heads of 256 and in brackets of 128; f32 crosses over 8 rows later):
+// at once, and as long for one. All sequences alike (us, here / there; bf16, heads of 256 and in brackets of 128; f32 crosses over 8 to 16 rows later, so its borders lie higher):
 //   64 sequences of 1200 keys   24 rows 88 117 (56 90)    40: 130 117 (80 89)     48: 150 119 (92 91)     64: 192 121 (117 90)
 //   24 of 5000                  24 rows 103 134 (68 117)  40: 157 130 (99 111)    48: 182 132 (115 112)   64: 235 135 (146 112)
 // Where a batch has rows on both sides, both kernels run, one behind the other, and neither fills the GPU: 24 sequences of 8 to 64 rows, 37 on average,
@@ -666,8 +666,9 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
 // Over some 430 batches of 1 to 192 rows, 500 to 20000 keys, heads of 64, 128 and 256 this takes 1.05 times as long as the best border for each
 // batch; 64 for all of them 1.13, 32 1.20. With few (sequence, KV head) pairs the other kernel's parts are many and small, and the border lies higher:
 //   1 sequence of 16000 keys    128 rows 71 110 (47 64)   256: 123 114 (79 69)    512: 226 105 (143 68)
-constexpr long long FEW_PAIRS = 8, NARROW_FEW = 256, NARROW_MOST = 128, NARROW_LEAST = 32;
-constexpr long long mean_many(int hd) { return hd == 256 ? 44 : 60; }   // rows per KV head of a sequence
+constexpr long long FEW_PAIRS = 8, NARROW_FEW = 256, NARROW_MOST = 128;
+constexpr long long narrow_least(bool f32) { return f32 ? 48 : 32; }
+constexpr long long mean_many(int hd, bool f32) { return hd == 256 ? (f32 ? 48 : 44) : 60; }   // rows per KV head of a sequence
 constexpr size_t TICKETS = 3 * MAX_CTAS_ALL * sizeof(unsigned int);   // before the partials: three words per CTA
 constexpr int MAX_CTAS = 3;                             // of an SM
 
@@ -741,7 +742,8 @@ int spk_paged4_attn(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
     a.err = device_error_ptr();
     const cudaStream_t s = (cudaStream_t)stream;
     const bool few = (long long)batch->nseq * pool->kv_heads <= FEW_PAIRS;
-    const long long narrow = few ? NARROW_FEW : (long long)batch->rows * a.group / batch->nseq < mean_many(pool->head_dim) ? NARROW_MOST : NARROW_LEAST;
+    const bool f32 = p->type == T_F32;
+    const long long narrow = few ? NARROW_FEW : (long long)batch->rows * a.group / batch->nseq < mean_many(pool->head_dim, f32) ? NARROW_MOST : narrow_least(f32);
     // the lines of work, at their longest: every row tile as long as the page table and a tile's tokens (before()); here a sequence has
     // `narrow` rows at most
     const bool many = (long long)batch->rows * a.group > narrow;          // some sequence may have more
