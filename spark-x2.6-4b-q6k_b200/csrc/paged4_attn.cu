@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) attn_kernel(const AttnPar
             }
             if (lane == 0) {
                 up_s[r] = a.scale * __int_as_float((127 - e) << 23);
-                pos_s[r] = real ? sg.pos0 + tok : -1;
+                pos_s[r] = real ? max(sg.pos0 + tok, -1) : -1;   // all before the first token alike
                 gate_s[r] = real && a.gate ? 1.0f / (1.0f + __expf(-to_f32<T>(((const T *)a.gate)[(long long)(sg.r0 + tok) * a.ldgate + h]))) : 1.0f;
             }
         }

@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kernel(const AttnParams a, co
             float sig = 1.f;
             long long out = -1;
             if (col <= g.c1) {
-                row.pos = g.pos0 + tok;
+                row.pos = max(g.pos0 + tok, -1);                      // all before the first token alike
                 row.low = a.window > 0 ? row.pos - a.window : -1;
                 out = (long long)(g.r0 + tok) * a.ldout + (long long)h * HD;
                 if (a.gate) sig = 1.0f / (1.0f + __expf(-to_f32<T>(((const T *)a.gate)[(long long)(g.r0 + tok) * a.ldgate + h])));

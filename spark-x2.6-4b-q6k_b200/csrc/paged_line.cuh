@@ -21,7 +21,7 @@ __device__ __forceinline__ Seq seq_of(const P &a, int s, int R) {
     Seq q;
     q.r0 = __ldg(a.b.row0 + s);
     q.n = __ldg(a.b.row0 + s + 1) - q.r0;
-    q.len = __ldg(a.b.kv_len + s);
+    q.len = max(__ldg(a.b.kv_len + s), 0);   // under 0 there is nothing to see either; positions do not leave 32 bits
     const long long room = (long long)a.b.max_pages * a.pool.page_tokens;
     if (q.n != 0 && (q.n < 0 || q.r0 < 0 || q.r0 > a.b.rows - q.n || q.len > room)) {   // not a batch: nothing is read
         if (a.err) atomicExch(a.err, DEV_BAD_INDEX);
@@ -84,7 +84,7 @@ __device__ __noinline__ bool walk_next(const P &a, const uint32_t *pre, int R, i
     while (w.base < w.x1) {
         const int G = a.group, c0 = w.j * R, c1 = min(c0 + R, w.q.n * G) - 1, pos0 = w.q.len - w.q.n;
         const int p_lo = pos0 + c0 / G, p_hi = pos0 + c1 / G;
-        const int see0 = a.window > 0 ? max(0, p_lo + 1 - a.window) : 0, b0 = see0 / BLOCK;
+        const int see0 = a.window > 0 && p_lo >= a.window ? p_lo + 1 - a.window : 0, b0 = see0 / BLOCK;
         const int nblk = p_hi < 0 ? 0 : p_hi / BLOCK + 1 - b0;
         const int nt = max(1, (nblk + TB - 1) / TB);   // one empty tile where nothing is seen
         const uint32_t t0 = w.base + cost;         // tile k stands at t0 + TB k, inside the group's length

@@ -1018,3 +1018,36 @@ def test_scales_above_all_that_append_writes(cuda, rows, hd, typ):
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~got.isnan()], want[~want.isnan()])
         for t, to in zip((c.cache.k_scale, c.cache.v_scale), now):
             t.copy_(to)
+
+
+@pytest.mark.parametrize("rows", [[3, 2], [70, 9]])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_lengths_that_are_none(cuda, rows, bits):
+    """kv_len under 0, down to the smallest there is: its rows see nothing, the others are as they were. A window as large as there is one."""
+    import torch
+
+    from spk import paged, paged4
+
+    c = Case(cuda, rows, [60, 37], 2, 64, 16, 8, seed=34)
+    q = c.randn(512, "f32")
+    if bits == 8:
+        cache = paged.PagedCache(c.cache.pages, 16, 2, 64, device=cuda)
+        for t in (cache.k_pool, cache.v_pool, cache.k_scale, cache.v_scale):
+            t.fill_(1.0)
+        batch = paged.PagedBatch(cache, c.row0, c.kv_len, c.tab, rows=sum(rows), heads=8)
+    else:
+        batch = c.batch
+    first = batch.attention(q)
+    assert torch.equal(batch.attention(q, window=(1 << 31) - 1), first)
+    for bad in (-1, -5, -(1 << 31), -(1 << 31) + 1, 0):
+        c.kv_len[0] = bad
+        for window in (0, 9, (1 << 31) - 1):
+            out = torch.full_like(q, 9.0)
+            batch.attention(q, out, window=window)
+            assert check_errors() == 0
+            assert (out[:rows[0]] == 0).all()
+            if window != 9:
+                assert (out[rows[0]:] - first[rows[0]:]).norm() <= 1e-6 * first[rows[0]:].norm()
+    c.kv_len[0] = rows[0] - 1                 # the first row alone lies before the sequence
+    big, none = batch.attention(q, window=(1 << 31) - 1), batch.attention(q)
+    assert torch.equal(big, none) and (big[0] == 0).all() and not (big[1:] == 0).all(1).any()
