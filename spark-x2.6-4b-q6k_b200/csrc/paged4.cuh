@@ -48,6 +48,16 @@ __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&h)[4]) {
         : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
         : "r"(w));
 }
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {   // a in the low half
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 // Whether one of four scale bytes is no number: the upper bit, and a carry into it from the others.
 __device__ __forceinline__ uint32_t poisoned(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u * (0x100u - POISON)) & w & 0x80808080u; }
 

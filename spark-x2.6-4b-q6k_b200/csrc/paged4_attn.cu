@@ -63,16 +63,6 @@ __device__ __forceinline__ uint32_t transpose(uint32_t a) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
     return r;
 }
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {   // a in the low half
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 // n bytes of a copy of N (4, 8 or 16); the rest becomes 0
 template <int N>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int n) {
@@ -138,60 +128,60 @@ __device__ __noinline__ void join(const AttnParams &a, const Seg &sg, float *wt,
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cols = sg.c1 - sg.c0 + 1;
     auto part = [&](int p) { return part_of<C>(a, sg, p); };
     float *red = wt + R * MAX_JOIN;
-                    // an item: 4 values of a row; `ways` threads share its parts, 8 loads on their way
-                    const int items = cols * (HD / 4), ways = max(1, min(C::THREADS / items, (n + 7) / 8));
-                    const int way = ways > 1 ? tid / items : 0, a0 = n * way / ways, a1 = n * (way + 1) / ways;
-                    float4 v[8];
-                    auto load = [&](int x, int p) {
-                        const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
-    #pragma unroll
-                        for (int y = 0; y < 8; y++)   // past the last part: the last one again, left out
-                            v[y] = __ldcg(reinterpret_cast<const float4 *>(part(at + step * min(p + y, a1 - 1)) + r * HD + d));
-                    };
-                    const int first = ways > 1 ? tid % items : tid;
-                    if (first < items && way < ways) load(first, a0);
-                    for (int r = warp; r < cols; r += WARPS) {   // the parts' weights: a warp per row
-                        const float m = lane < n ? __ldcg(part(at + step * lane) + R * HD + r) : -INFINITY, x = lane < n ? __ldcg(part(at + step * lane) + R * HD + R + r) : 0.f;
-                        float M = m;
-    #pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-                        const float f = m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(m - M);
-                        if (lane < n) wt[r * MAX_JOIN + lane] = f;
-                        const float L = warp_sum(m == -INFINITY ? x : x * f);
-                        if (lane == 0) M_s[r] = M, L_s[r] = L;
-                    }
-                    __syncthreads();
-                    for (int x0 = 0; x0 < items; x0 += C::THREADS) {   // one turn where several threads share an item
-                        const int x = ways > 1 ? first : x0 + tid, r = x / (HD / 4), d = 4 * (x % (HD / 4));
-                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                        const bool own = x < items && way < ways;
-                        if (own)
-                            for (int p = a0; p < a1; p += 8) {
-                                if (x0 > 0 || p > a0) load(x, p);
-    #pragma unroll
-                                for (int y = 0; y < 8; y++) {
-                                    const float f = wt[r * MAX_JOIN + min(p + y, a1 - 1)];
-                                    if (p + y < a1) o.x = fmaf(v[y].x, f, o.x), o.y = fmaf(v[y].y, f, o.y), o.z = fmaf(v[y].z, f, o.z), o.w = fmaf(v[y].w, f, o.w);
-                                }
-                            }
-                        if (ways > 1) {
-                            if (own && way > 0) *reinterpret_cast<float4 *>(red + 4 * ((way - 1) * items + x)) = o;
-                            __syncthreads();
-                            if (own && way == 0)
-                                for (int w = 1; w < ways; w++) {
-                                    const float4 y = *reinterpret_cast<const float4 *>(red + 4 * ((w - 1) * items + x));
-                                    o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
-                                }
-                        }
-                        if (own && way == 0) {
-                            if (done) output<C>(a, sg, r, d, o, L_s[r], gate_s[r]);
-                            else {
-                                float *to = part(at);
-                                __stcg(reinterpret_cast<float4 *>(to + r * HD + d), o);
-                                if (d == 0) __stcg(to + R * HD + r, M_s[r]), __stcg(to + R * HD + R + r, L_s[r]);
-                            }
-                        }
-                    }
+    // an item: 4 values of a row; `ways` threads share its parts, 8 loads on their way
+    const int items = cols * (HD / 4), ways = max(1, min(C::THREADS / items, (n + 7) / 8));
+    const int way = ways > 1 ? tid / items : 0, a0 = n * way / ways, a1 = n * (way + 1) / ways;
+    float4 v[8];
+    auto load = [&](int x, int p) {
+        const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
+#pragma unroll
+        for (int y = 0; y < 8; y++)   // past the last part: the last one again, left out
+            v[y] = __ldcg(reinterpret_cast<const float4 *>(part(at + step * min(p + y, a1 - 1)) + r * HD + d));
+    };
+    const int first = ways > 1 ? tid % items : tid;
+    if (first < items && way < ways) load(first, a0);
+    for (int r = warp; r < cols; r += WARPS) {   // the parts' weights: a warp per row
+        const float m = lane < n ? __ldcg(part(at + step * lane) + R * HD + r) : -INFINITY, x = lane < n ? __ldcg(part(at + step * lane) + R * HD + R + r) : 0.f;
+        float M = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float f = m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : ex2(m - M);
+        if (lane < n) wt[r * MAX_JOIN + lane] = f;
+        const float L = warp_sum(m == -INFINITY ? x : x * f);
+        if (lane == 0) M_s[r] = M, L_s[r] = L;
+    }
+    __syncthreads();
+    for (int x0 = 0; x0 < items; x0 += C::THREADS) {   // one turn where several threads share an item
+        const int x = ways > 1 ? first : x0 + tid, r = x / (HD / 4), d = 4 * (x % (HD / 4));
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        const bool own = x < items && way < ways;
+        if (own)
+            for (int p = a0; p < a1; p += 8) {
+                if (x0 > 0 || p > a0) load(x, p);
+#pragma unroll
+                for (int y = 0; y < 8; y++) {
+                    const float f = wt[r * MAX_JOIN + min(p + y, a1 - 1)];
+                    if (p + y < a1) o.x = fmaf(v[y].x, f, o.x), o.y = fmaf(v[y].y, f, o.y), o.z = fmaf(v[y].z, f, o.z), o.w = fmaf(v[y].w, f, o.w);
+                }
+            }
+        if (ways > 1) {
+            if (own && way > 0) *reinterpret_cast<float4 *>(red + 4 * ((way - 1) * items + x)) = o;
+            __syncthreads();
+            if (own && way == 0)
+                for (int w = 1; w < ways; w++) {
+                    const float4 y = *reinterpret_cast<const float4 *>(red + 4 * ((w - 1) * items + x));
+                    o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+                }
+        }
+        if (own && way == 0) {
+            if (done) output<C>(a, sg, r, d, o, L_s[r], gate_s[r]);
+            else {
+                float *to = part(at);
+                __stcg(reinterpret_cast<float4 *>(to + r * HD + d), o);
+                if (d == 0) __stcg(to + R * HD + r, M_s[r]), __stcg(to + R * HD + R + r, L_s[r]);
+            }
+        }
+    }
 }
 
 template <typename C>

@@ -15,8 +15,8 @@
 // What bounds it: 2048 bf16 rows of 16 heads of 256 behind 6144 cached tokens are 240 GFLOP in 308 us, 0.78 PFLOP/s, 47 % of the measured
 // bf16 rate. A tile takes 1.6 us where its products take 0.76: the tensor pipe is busy 37 % of the time and 45 % of the issue slots are used; the
 // softmax warps are the longest chain (scores out of the tensor memory, exponentials, weights back), the converting warps nearly as long. Eight softmax
-// warps, two to 32 rows, would halve that chain, but 16 or 17 warps have 112 registers a thread or fewer: their loop spilled, 585 us and more (setmaxnreg
-// cannot help where the whole kernel is compiled for the launch's share). Outputs out of line (433 us for 368 then) and code of their own for keys,
+// warps, two to 32 rows, would halve that chain, but 16 or 17 warps have 112 registers a thread or fewer: their loop spilled, 585 us and more (shares of
+// their own by setmaxnreg, more for the softmax warps and fewer for the others, have not been tried). Outputs out of line (433 us for 368 then) and code of their own for keys,
 // values and every second tile (1.5 times) were slower too: the loops have to stay in the instruction cache. 13 f32 prompts of
 // up to 701 rows, 10 GFLOP counted once (f32 rows multiply twice), take 125 us: short groups of which several end in every CTA.
 #include "paged4.cuh"
@@ -99,16 +99,6 @@ __device__ __forceinline__ void tm_wait_ld(float *v, int n) {   // the loads hav
     for (int i = 0; i < n; i++) asm volatile("" : "+f"(v[i]));
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {   // a in the low half
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 // What a softmax thread knows of its row
 struct Row {
     float up;                                           // factor of its scores
