@@ -521,8 +521,9 @@ typedef struct {
 
 /* A projection's rows: queries and keys normalised and rotated, queries out, keys and values into the pages, in one pass.
  * Per head, with q_norm / k_norm ([head_dim] f32, 16-byte aligned; NULL: none): x / sqrt(mean x^2 + eps) * norm, whatever the head's
- * size (squares that leave f32's range are taken on a power of two). Then, with freq, the rotation by f32(position * freq[i]), i < pdim / 2 (pdim a multiple of 16), of the pairs (i, i + pdim / 2), or
- * (2 i, 2 i + 1) where `interleaved`. heads 0: no queries. q_out may be q itself (the same rows and stride).
+ * size (squares that leave f32's range are taken on a power of two). Then, with freq, the rotation by f32(position * freq[i]),
+ * i < pdim / 2 (pdim a multiple of 16), of the pairs (i, i + pdim / 2), or (2 i, 2 i + 1) where `interleaved`; the dims behind
+ * them stay as they are. heads 0: no queries. q_out may be q itself (the same rows and stride).
  * Rounding, per group of 16 values: the scale is the number of 4 significant bits nearest to amax / 6 (ties to even, 2^-14 to
  * 10240), a code the nearest to value / scale (ties to the even code, at most 6 in magnitude); both are decided exactly
  * for the f32 value at hand. A NaN or infinity makes its group's scale byte 255 (NaN). */
@@ -560,8 +561,8 @@ int spk_paged4_read(const spk_kv4_pool *pool, const spk_kv_batch *batch, const s
  * over j in [0, pos_t] (window 0) or (pos_t - window, pos_t]; q head h reads KV head h / (heads / kv_heads), any group. The
  * softmax and all sums are in f32; queries and weights meet the cached values as f16 numbers on a power of two of their row,
  * f32 rows' as two, weights kept down to 2^-36 of the row's largest (a sequence of many rows: 2^-34 in f32, 2^-30 in the
- * 16-bit types). A row that sees nothing gets 0; a row that sees a token of which a group is no number
- * gets NaN.
+ * 16-bit types). A row that sees nothing gets 0 (also where kv_len is under the call's rows); a row that sees a token of which a
+ * group is no number gets NaN.
  * workspace: spk_paged4_attn_workspace_bytes(head_dim) device bytes for the device current at the call, zeroed once and
  * left ready; calls that share one must not overlap on the GPU. No sync. */
 typedef struct {

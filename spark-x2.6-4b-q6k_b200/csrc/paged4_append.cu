@@ -9,7 +9,7 @@
 // Both are decided exactly: for d the f32 quotient's neighbour is checked against 6 (d + half a step), which f32 holds; the quotient
 // x / d is corrected by its own residual, so that a tie is a tie, and moved off a border that it was only rounded to.
 //
-// What bounds append: at the rows' bytes' rate the issue slots are half used (48 M warp instructions for 16384 rows of 24 heads, 122 for 256 values) and
+// What bounds append: at the rows' bytes' rate the issue slots are half used (50 M warp instructions for 16384 rows of 24 heads, 128 for 256 values) and
 // a warp's chain (load, norm's tree of shuffles, rotation, scale, codes) waits for itself more often than for memory. A warp takes 256 values at a time (256 /
 // head_dim heads side by side), 8 consecutive ones a lane, which is one 16-byte load of 16-bit rows and one word of codes; a group is two lanes, a head's norm
 // a shuffle tree, the other half of a rotated pair 8 shuffles. A token's items (queries, keys, values) are one warp's where there are
@@ -36,9 +36,9 @@ int check_pool(const spk_kv4_pool *p, const char *who) {
 namespace {
 
 // Warps of an SM against registers a thread, and items whose loads go out and whose chains run together. 16384 bf16 rows (16 + 4 + 4 heads of
-// 256, normalised, rotated over 64 dims) take 94 us, 3.8 TB/s of rows, queries and cache, 58 % of the measured copy rate. With the read of codes and
-// scales behind it: 122 us so, 128 with one CTA less, 123 with one more, 139 with two items together, 128 with twice the warps in a CTA; 13 f32
-// prompts of up to 1501 rows 49, 59 with three CTAs, 57 with five. Rows through a ring of cp.async copies, more of them on their way, took 129 to 145
+// 256, normalised, rotated over 64 dims) take 95 us, 3.7 TB/s of rows, queries and cache, 57 % of the measured copy rate. With the read of codes and
+// scales behind it, 123 us now, these were chosen at 122: 128 with one CTA less, 123 with one more, 139 with two items together, 128 with twice the
+// warps in a CTA; 13 f32 prompts of up to 1501 rows, 47 now, at 49: 59 with three CTAs, 57 with five. Rows through a ring of cp.async copies, more of them on their way, took 129 to 145
 // and 67: what it adds per item, in f32 two passes over each sector, costs more than the wait that it hides.
 constexpr int AP_WARPS = 4, AP_THREADS = AP_WARPS * 32;
 template <typename T>
@@ -190,7 +190,7 @@ __device__ __forceinline__ float max_abs(float m, float a, float b) {
 // A head's mean square and eps between these: no square that counts in it was lost, none was infinite. Where it is not (values beyond 2^60, or all under
 // 2^-45 with as small an eps) the head is squared again on a power of two: up to 2^58 from 2^128, up from 2^-149 to 2^-49.
 // The test between a sum and its root costs 3 % of a prompt's append (16384 bf16 rows with their reading back 122 us without it, 126 so; 129 with such heads done
-// again behind a batch of items, 139 with one test for a batch).
+// again behind a batch of items, 139 with one test for a batch); 123 since each kind of pairs has its own code.
 constexpr float NORM_LOW = 0x1p-90f, NORM_HIGH = 0x1p120f, NORM_UP = 0x1p100f, NORM_DOWN = 0x1p-70f;
 
 // Where the rows of a call lie: the sequences in shared memory.

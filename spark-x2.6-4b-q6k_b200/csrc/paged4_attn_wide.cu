@@ -12,7 +12,7 @@
 // Work split: paged_line.cuh's line of groups of 128 rows, one CTA per SM. Warps: 0-3 queries, softmax and outputs,
 // 4-11 codes to f16, 12 the MMAs. Each walks the CTA's groups by itself; they meet at mbarriers.
 //
-// What bounds it: 2048 bf16 rows of 16 heads of 256 behind 6144 cached tokens are 240 GFLOP in 308 us, 0.78 PFLOP/s, 47 % of the measured
+// What bounds it: 2048 bf16 rows of 16 heads of 256 behind 6144 cached tokens are 240 GFLOP in 309 us, 0.78 PFLOP/s, 47 % of the measured
 // bf16 rate. A tile takes 1.6 us where its products take 0.76: the tensor pipe is busy 37 % of the time and 45 % of the issue slots are used; the
 // softmax warps are the longest chain (scores out of the tensor memory, exponentials, weights back), the converting warps nearly as long. Eight softmax
 // warps, two to 32 rows, would halve that chain, but 16 or 17 warps have 112 registers a thread or fewer: their loop spilled, 585 us and more (shares of

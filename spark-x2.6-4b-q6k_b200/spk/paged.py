@@ -14,7 +14,7 @@ their contents move. ``PageTable`` hands out pages.
 Calls go to torch's current stream unless a stream is given, and do not synchronize. What an object
 here makes for itself may be used on any stream. Tensors that are handed in are ordered with a given
 stream by the caller, as between any two streams; they may be dropped after the call. Output that a
-call makes belongs to the call's stream.
+call makes belongs to the call's stream. A batch is one host thread's at a time: its calls' arguments lie in it.
 """
 from __future__ import annotations
 

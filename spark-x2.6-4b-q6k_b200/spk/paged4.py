@@ -98,7 +98,8 @@ class Paged4Cache:
 
 
 class Paged4Batch(PagedBatch):
-    """The rows of a call over a 4-bit pool: PagedBatch's arguments, checks and limits."""
+    """The rows of a call over a 4-bit pool: PagedBatch's arguments, checks and limits. `rows` may be more than row0[nseq] (a padded buffer,
+    a captured graph): the rows behind it are left as they are."""
 
     _cache = Paged4Cache
 
