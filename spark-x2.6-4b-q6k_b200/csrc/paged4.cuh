@@ -78,6 +78,9 @@ struct AttnParams {
 };
 // Weights are f16 numbers 2^(s - m): a new reference m puts the row's largest at 2^W_TOP (the kernel for many rows: less), and it moves when
 // one passes 2^W_MAX. A weight is kept down to 2^-24: 2^-36 of the largest (many rows: 2^-34 in f32, 2^-30 in the 16-bit types).
+// f32 rows' weights are two f16 numbers, 22 bits. 16-bit rows' are one: off by half a step, 2^-11 of each weight, either way and so averaged over the keys, and what
+// is divided by is the sum of the weights as they were rounded (bf16 many rows: before, which bf16's own half step of 2^-8 hides). Against 64 bits that is 1e-5 beside the
+// 2e-4 of f16's output (24 x 8 rows), nothing beside bf16's; a second term would multiply the values twice.
 constexpr float W_TOP = 12.0f, W_MAX = 15.0f;
 
 // Floats of one CTA's part of a group of R query rows: O, then m, then l.

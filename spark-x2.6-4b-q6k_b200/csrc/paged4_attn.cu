@@ -26,7 +26,7 @@
 //
 // Measured: one f32 row of 16 heads on 4 of 256 over 131072 keys 51.8 us (151 MB of cache, 2.9 TB/s: some 600 warp instructions a block, 45 % of the
 // issue slots used by 8 warps an SM, 240 registers each), of which the start and the joining of 74 parts in two steps are some 15; 64 bf16 rows of up
-// to 9000 keys 33.2 us (48 MB); 24 x 8 f16 rows of 32 heads on 4 of 128 29.0 us; one row under a window of 512 14.8 us, launch, plan, queries, tiles and
+// to 9000 keys 33.1 us (48 MB); 24 x 8 f16 rows of 32 heads on 4 of 128 29.1 us; one row under a window of 512 14.6 us, launch, plan, queries, tiles and
 // joining each behind the one before.
 #include <limits.h>
 
